@@ -98,6 +98,14 @@ SIGNATURES = {
     "hb_latent_block": (_I, [_LW, _P, _P, _P, _P, _I, _I, _I, _P, _P, _Z, _P]),
     "hb_latent_shared_up": (_I, [_LW, _P, _I, _I, _P, _Z, _P]),
     "hb_latent_out": (_I, [_LW, _P, _I, _I, _P, _P, _Z, _P]),
+    "hb_mxfp4_quantize": (_I, [_P, _I, _L, _I, _P, _P, _P]),
+    "hb_mxfp4_dequantize": (_I, [_P, _P, _L, _I, _I, _P, _P]),
+    "hb_silu_mul_quant_mxfp4": (_I, [_P, _I, _L, _I, _I, _P, _P, _P]),
+    "hb_mxfp4_tiled_bytes": (_Z, [_L, _I]),
+    "hb_mxfp4_repack": (_I, [_P, _P, _I, _L, _I, _I, _P, _P]),
+    "hb_mxfp4_unpack": (_I, [_P, _I, _L, _I, _I, _P, _P, _P]),
+    "hb_mxfp4_linear_workspace_bytes": (_Z, [_L, _L, _I, _I]),
+    "hb_mxfp4_linear": (_I, [_P, _P, _I, _L, _P, _L, _I, _P, _I, _P, _Z, _P]),
 }
 
 
@@ -166,6 +174,15 @@ def workspace_status(ws: torch.Tensor | None) -> int:
 
 def workspace_reset(ws: torch.Tensor | None) -> None:
     check(lib().hb_workspace_reset(ptr(ws), 0 if ws is None else ws.numel(), stream()), "workspace_reset")
+
+
+def need_one_gpu(*tensors: torch.Tensor) -> None:
+    """`need_gpu`, and every tensor on the current device: a launch goes to that device's current stream."""
+    here = torch._C._cuda_getDevice() if any(t is not None and t.is_cuda for t in tensors) else -1
+    for t in tensors:
+        if t is not None and t.get_device() != here:
+            need_gpu(t)
+            raise ValueError(f"hibana_amd kernels run on the current device, cuda:{here}: got a tensor on {t.device}")
 
 
 def need_gpu(*tensors: torch.Tensor) -> None:

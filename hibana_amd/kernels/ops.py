@@ -5,7 +5,7 @@ from __future__ import annotations
 import torch
 
 from hibana_amd import _lib
-from hibana_amd.kernels import w3
+from hibana_amd.kernels import mxfp4, w3
 
 
 def w3_decode(lin, m: int, rows: int | None = None) -> bool:
@@ -37,6 +37,35 @@ def nvfp4_linear(x: torch.Tensor, lin, prequantized=None, relu2: bool = False) -
         code = lib.hb_nvfp4_gemm_ws(xc.data_ptr(), m, lin.tiled.data_ptr(), lin.scale2, n, k, int(relu2), y.data_ptr(), _lib.ptr(ws), need, _lib.stream())
         if code:
             _lib.check(code, "nvfp4_linear")
+    return y
+
+
+def mxfp4_linear(x, lin, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """x [M, K] -> [M, N] on a `Mxfp4Linear`: both operands in the microscaled four-bit format, FP32 sums rounded once. x is BF16,
+    FP16 or FP32, rounded to the format on the way (`mxfp4.quantize`'s codes), and the result of its type; or a `mxfp4.Mxfp4` that
+    holds it already, and the result of `dtype`. Once `lin.tile()` has run the call can be captured."""
+    ready = isinstance(x, mxfp4.Mxfp4)
+    kind = mxfp4.CODES if ready else mxfp4.TYPES.get(x.dtype)
+    out_type = dtype if ready else x.dtype
+    if kind is None or out_type not in mxfp4.TYPES or len(x.shape) != 2 or x.shape[1] != lin.in_features:
+        raise ValueError("mxfp4_linear: x must be BF16, FP16 or FP32 [M, in_features], or hold such rows")
+    if lin.tiled is None:
+        lin.tile()
+    _lib.need_one_gpu(*(x if ready else (x,)), lin.tiled)
+    m, n, k = x.shape[0], lin.out_features, lin.in_features
+    y = torch.empty((m, n), dtype=out_type, device=x.device)
+    if m:
+        lib = _lib.lib()
+        if ready:
+            xc, xs = mxfp4.flat(x, "mxfp4_linear")  # held until the launch is enqueued
+        else:
+            xc, xs = mxfp4.rows16(x), None
+        need = lib.hb_mxfp4_linear_workspace_bytes(m, n, k, kind)
+        ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+        code = lib.hb_mxfp4_linear(xc.data_ptr(), _lib.ptr(xs), kind, m, lin.tiled.data_ptr(), n, k, y.data_ptr(), mxfp4.TYPES[out_type], _lib.ptr(ws), need,
+                                   _lib.stream())
+        if code:
+            _lib.check(code, "mxfp4_linear")
     return y
 
 
@@ -92,6 +121,28 @@ def silu_mul_quant_groups(gate_up: torch.Tensor, pairs: int = 0, torch_chain: bo
         if code:
             _lib.check(code, "silu_mul_quant_groups")
     return q, scales
+
+
+def silu_mul_quant_mxfp4(gate_up: torch.Tensor, pairs: int = 0) -> mxfp4.Mxfp4:
+    """silu(gate) * up of [..., 2 I] (BF16, FP16 or FP32) rounded to the microscaled four-bit format in the same launch: the codes
+    that the exact product has; columns gate | up, or (`pairs`, a multiple of eight) both alternating in blocks of that many. I a
+    multiple of 32. A group with an infinite or undefined product stands for NaN."""
+    kind = mxfp4.TYPES.get(gate_up.dtype)
+    if kind is None or gate_up.ndim == 0 or gate_up.shape[-1] % 64:
+        raise ValueError("silu_mul_quant_mxfp4: BF16, FP16 or FP32 [..., 2 I] with I a multiple of 32")
+    half = gate_up.shape[-1] // 2
+    if pairs and (pairs < 0 or pairs % 8 or half % pairs):
+        raise ValueError("silu_mul_quant_mxfp4: pairs must be a multiple of eight dividing I")
+    _lib.need_one_gpu(gate_up)
+    lead = gate_up.shape[:-1]
+    codes = torch.empty((*lead, half // 2), dtype=torch.uint8, device=gate_up.device)
+    scales = torch.empty((*lead, half // mxfp4.GROUP), dtype=torch.uint8, device=gate_up.device)
+    if gate_up.numel():
+        gu = mxfp4.rows16(gate_up)
+        code = _lib.lib().hb_silu_mul_quant_mxfp4(gu.data_ptr(), kind, gate_up.numel() // (2 * half), half, pairs, codes.data_ptr(), scales.data_ptr(), _lib.stream())
+        if code:
+            _lib.check(code, "silu_mul_quant_mxfp4")
+    return mxfp4.Mxfp4(codes, scales)
 
 
 def route_topk(logits: torch.Tensor, k: int, slots: torch.Tensor | None = None, steps: int = 1, repeat: bool = False):

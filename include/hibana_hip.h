@@ -566,6 +566,35 @@ int hb_latent_shared_up(const hb_latent_weights* w, const void* x, int m, int to
 int hb_latent_out(const hb_latent_weights* w, const void* routed, int m, int topk, void* out, void* workspace,
                   size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------ microscaled four-bit (MXFP4)
+ *
+ * Values in groups of 32 along K: one power-of-two scale, an E8M0 byte b for 2^(b - 127) (255: NaN), and 32 E2M1 codes, two a byte,
+ * element 2 i in the low nibble. Row-major: codes [rows, k / 2], scales [rows, k / 32]; k a multiple of 32. The rounding of a group:
+ * b = max(floor(log2 of its largest magnitude) + 125, 0), codes the nearest E2M1 of x / 2^(b - 127), ties to the even code, beyond 6
+ * to 6; a group with an infinity or a NaN has b = 255 and codes 0. No counterpart in the reference. */
+enum { HB_BF16 = 0, HB_F16 = 1, HB_F32 = 2, HB_MXFP4 = 3 };  /* types of the arrays below */
+
+/* x [rows, k] (HB_BF16 / HB_F16 / HB_F32) -> codes, scales. x and codes on 16 bytes. */
+int hb_mxfp4_quantize(const void* x, int type, int64_t rows, int k, void* codes, void* scales, void* stream);
+/* The values back, [rows, k] of `type`: exact in FP32 and BF16, rounded (or infinite) where FP16 does not hold one. */
+int hb_mxfp4_dequantize(const void* codes, const void* scales, int64_t rows, int k, int type, void* out, void* stream);
+/* silu(gate) * up of gate_up [rows, 2 half] rounded to the format in one pass; the columns are gate | up or, `pairs` > 0 (a multiple
+ * of eight dividing half), blocks of `pairs` gate columns and their `pairs` up columns. The codes are the exact product's (one beyond
+ * FP32's range counts as an infinity). */
+int hb_silu_mul_quant_mxfp4(const void* gate_up, int type, int64_t rows, int half, int pairs, void* codes, void* scales, void* stream);
+
+/* The weights' tile layout: its bytes for a matrix [n, k] (any n; 0: a size the kernels do not take), row-major codes and scales of
+ * `matrices` stacked matrices into it, and back. `gated`: fc1 of gated experts, rows [up; gate], n a multiple of 64. */
+size_t hb_mxfp4_tiled_bytes(int64_t n, int k);
+int hb_mxfp4_repack(const void* codes, const void* scales, int matrices, int64_t n, int k, int gated, void* tiled, void* stream);
+int hb_mxfp4_unpack(const void* tiled, int matrices, int64_t n, int k, int gated, void* codes, void* scales, void* stream);
+
+/* y [m, n] = x w^T, FP32 sums rounded once: x [m, k] of y's type, rounded to the format on the way, or (HB_MXFP4) its codes with
+ * `x_scales`; w a matrix in the tile layout. `workspace`: plain scratch of hb_mxfp4_linear_workspace_bytes (NULL where that is 0). */
+size_t hb_mxfp4_linear_workspace_bytes(int64_t m, int64_t n, int k, int x_type);
+int hb_mxfp4_linear(const void* x, const void* x_scales, int x_type, int64_t m, const void* tiled, int64_t n, int k, void* y, int y_type,
+                    void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

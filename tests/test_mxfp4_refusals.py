@@ -1,0 +1,69 @@
+"""What the microscaled four-bit operators refuse, on the CPU: nothing is launched."""
+import ctypes as C
+
+import pytest
+import torch
+
+from hibana_amd import _lib
+from hibana_amd.kernels import mxfp4, ops
+from hibana_amd.weights.mxfp4 import Mxfp4Linear
+
+
+def test_the_library_refuses_before_a_launch():
+    lib = _lib.lib()
+    assert lib.hb_mxfp4_quantize(None, 0, 1, 32, 256, 256, None) == _lib.HB_ENULL
+    for kind, rows, k, x, codes in [(3, 1, 32, 256, 256), (-1, 1, 32, 256, 256), (0, 0, 32, 256, 256), (0, 1, 48, 256, 256), (0, 1, 0, 256, 256), (0, 1, 32, 258, 256),
+                                    (0, 1, 32, 256, 264), (0, 1 << 41, 32, 256, 256), (0, -1, 32, 256, 256)]:
+        assert lib.hb_mxfp4_quantize(x, kind, rows, k, codes, 256, None) == _lib.HB_EINVAL
+        assert lib.hb_mxfp4_dequantize(codes, 256, rows, k, kind, x, None) == _lib.HB_EINVAL
+    assert lib.hb_mxfp4_dequantize(256, None, 1, 32, 0, 256, None) == _lib.HB_ENULL
+    assert lib.hb_silu_mul_quant_mxfp4(256, 0, 1, 64, 0, None, 256, None) == _lib.HB_ENULL
+    for half, pairs in [(48, 0), (64, 12), (64, -8), (96, 64), (0, 0)]:
+        assert lib.hb_silu_mul_quant_mxfp4(256, 0, 1, half, pairs, 256, 256, None) == _lib.HB_EINVAL
+    assert lib.hb_mxfp4_tiled_bytes(16, 128) == 1024 + 256 and lib.hb_mxfp4_tiled_bytes(17, 544) == 2 * 5 * 1024 + 2 * 2 * 256
+    assert lib.hb_mxfp4_tiled_bytes(0, 128) == 0 and lib.hb_mxfp4_tiled_bytes(16, 48) == 0 and lib.hb_mxfp4_tiled_bytes(1 << 31, 32) == 0
+    assert lib.hb_mxfp4_repack(256, 256, 1, 96, 128, 1, 256, None) == _lib.HB_EINVAL  # gated rows go in units of 64
+    assert lib.hb_mxfp4_repack(256, 256, 65536, 64, 128, 0, 256, None) == _lib.HB_EINVAL
+    assert lib.hb_mxfp4_unpack(None, 1, 64, 128, 0, 256, 256, None) == _lib.HB_ENULL
+    need = lib.hb_mxfp4_linear_workspace_bytes(4, 64, 128, 0)
+    call = lambda **c: lib.hb_mxfp4_linear(*{**dict(x=256, xs=None, kind=0, m=4, w=256, n=64, k=128, y=256, to=0, ws=256, size=max(need, 1 << 20), stream=None), **c}.values())  # noqa: E731
+    assert call(x=None) == call(w=None) == call(y=None) == call(kind=3) == _lib.HB_ENULL
+    for c in [dict(m=0), dict(m=(1 << 19) + 1), dict(n=0), dict(k=33), dict(kind=1), dict(kind=4), dict(to=3), dict(x=264), dict(w=257), dict(y=257)]:
+        assert call(**c) == _lib.HB_EINVAL, c
+
+
+def test_python_refusals():
+    bf = torch.zeros(2, 64, dtype=torch.bfloat16)
+    for bad in (torch.zeros(2, 64, dtype=torch.int32), torch.zeros(2, 64, dtype=torch.float64), torch.zeros(2, 48), torch.zeros(())):
+        with pytest.raises(ValueError):
+            mxfp4.quantize(bad)
+    with pytest.raises(RuntimeError):
+        mxfp4.quantize(bf)  # no CPU path
+    held = mxfp4.Mxfp4(torch.zeros(2, 32, dtype=torch.uint8), torch.zeros(2, 2, dtype=torch.uint8))
+    with pytest.raises(RuntimeError):
+        mxfp4.dequantize(held)
+    with pytest.raises(ValueError):
+        mxfp4.dequantize(held, torch.float64)
+    for codes, scales in [(held.codes, held.scales[:, :1]), (held.codes.int(), held.scales), (held.codes[:, :8], held.scales[:, :1]), (held.codes, held.scales.int())]:
+        with pytest.raises(ValueError):
+            mxfp4.dequantize(mxfp4.Mxfp4(codes, scales))
+        with pytest.raises(ValueError):
+            Mxfp4Linear(codes, scales)
+    with pytest.raises(ValueError):
+        Mxfp4Linear(torch.zeros(2, 3, 32, dtype=torch.uint8), torch.zeros(2, 3, 2, dtype=torch.uint8))
+    with pytest.raises(RuntimeError):
+        Mxfp4Linear(*held).tile()
+    for bad, pairs in [(torch.zeros(2, 96), 0), (torch.zeros(2, 128, dtype=torch.float64), 0), (torch.zeros(2, 128), 12), (torch.zeros(2, 192), 64), (torch.zeros(2, 128), -8)]:
+        with pytest.raises(ValueError):
+            ops.silu_mul_quant_mxfp4(bad, pairs)
+    with pytest.raises(RuntimeError):
+        ops.silu_mul_quant_mxfp4(torch.zeros(2, 128))
+    lin = Mxfp4Linear(*held)
+    lin.tiled = torch.zeros(1280, dtype=torch.uint8)  # (not read: every call below is refused)
+    for bad in (torch.zeros(2, 32), torch.zeros(64), torch.zeros(2, 64, dtype=torch.float64), torch.zeros(1, 2, 64)):
+        with pytest.raises(ValueError):
+            ops.mxfp4_linear(bad, lin)
+    with pytest.raises(ValueError):
+        ops.mxfp4_linear(held, lin, torch.float64)
+    with pytest.raises(RuntimeError):
+        ops.mxfp4_linear(bf, lin)
