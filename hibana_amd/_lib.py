@@ -30,6 +30,11 @@ class HbLatentWeights(C.Structure):
                 ("experts_total", C.c_int), ("latent", C.c_int), ("hidden", C.c_int), ("shared_inter", C.c_int)]
 
 
+class HbMxfp4Experts(C.Structure):
+    _fields_ = [("fc1", C.c_void_p), ("fc2", C.c_void_p), ("experts", C.c_int), ("base", C.c_int), ("hidden", C.c_int), ("inter", C.c_int),
+                ("hidden_out", C.c_int), ("gated", C.c_int)]
+
+
 _P, _I, _L, _Z, _F = C.c_void_p, C.c_int, C.c_int64, C.c_size_t, C.c_float
 _LW = C.POINTER(HbLatentWeights)
 _EX = C.POINTER(HbW3Experts)
@@ -105,6 +110,8 @@ SIGNATURES = {
     "hb_mxfp4_repack": (_I, [_P, _P, _I, _L, _I, _I, _P, _P]),
     "hb_mxfp4_unpack": (_I, [_P, _I, _L, _I, _I, _P, _P, _P]),
     "hb_mxfp4_linear_workspace_bytes": (_Z, [_L, _L, _I, _I]),
+    "hb_mxfp4_moe_workspace_bytes": (_Z, [C.POINTER(HbMxfp4Experts), _I, _I]),
+    "hb_mxfp4_moe": (_I, [C.POINTER(HbMxfp4Experts), _P, _P, _P, _I, _I, _I, _P, _P, _Z, _P]),
     "hb_mxfp4_linear": (_I, [_P, _P, _I, _L, _P, _L, _I, _P, _I, _P, _Z, _P]),
 }
 

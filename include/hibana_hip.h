@@ -595,6 +595,20 @@ size_t hb_mxfp4_linear_workspace_bytes(int64_t m, int64_t n, int k, int x_type);
 int hb_mxfp4_linear(const void* x, const void* x_scales, int x_type, int64_t m, const void* tiled, int64_t n, int k, void* y, int y_type,
                     void* workspace, size_t workspace_bytes, void* stream);
 
+/* Routed experts, weights and activations both in the format: fc1 and fc2 are stacks of `experts` tile layouts, fc1 [2 inter or inter,
+ * hidden] (gated: rows [up; gate], laid out with `gated`; else ReLU^2), fc2 [hidden_out, inter]; hidden and inter multiples of 32,
+ * hidden_out of eight. x [m, hidden] BF16 is rounded to the format, h between the two products as well (from its FP32 value). An id
+ * outside base .. base + experts - 1 adds nothing. mode HB_MOE_SUM: out BF16 [m, hidden_out]; HB_MOE_PAIRS_F32 / _BF16: the
+ * pairs' outputs [m * topk, hidden_out] (those of skipped pairs unspecified). `workspace`: plain scratch, nothing in it need be zero. */
+typedef struct {
+  const void* fc1;
+  const void* fc2;
+  int experts, base, hidden, inter, hidden_out, gated;
+} hb_mxfp4_experts;
+size_t hb_mxfp4_moe_workspace_bytes(const hb_mxfp4_experts* experts, int m, int topk);
+int hb_mxfp4_moe(const hb_mxfp4_experts* experts, const void* x, const int32_t* ids, const float* weights, int m, int topk, int mode, void* out,
+                 void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

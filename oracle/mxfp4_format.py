@@ -46,25 +46,56 @@ def silu_mul(gate_up: torch.Tensor, pairs: int = 0) -> torch.Tensor:
     return gate / (1.0 + torch.exp(-gate)) * up
 
 
+def between(lo: torch.Tensor, hi: torch.Tensor):
+    """The smallest and the largest magnitude that the rounding of values with magnitudes lo .. hi [..., K] can give (a group's scale is
+    that of its largest: of lo's or of hi's, or equal for both)."""
+    def under(v, scale_of):
+        _, e = torch.frexp(scale_of.reshape(*v.shape[:-1], -1, GROUP).amax(-1))
+        unit = torch.ldexp(torch.ones(e.shape, dtype=torch.float64), (e - 3).clamp(min=-127)).repeat_interleave(GROUP, -1)
+        a = v / unit
+        code = (a > 0.25).long() + (a >= 0.75) + (a > 1.25) + (a >= 1.75) + (a > 2.5) + (a >= 3.5) + (a > 5.0)
+        return LEVELS[code] * unit
+    every = torch.stack([under(v, s) for v in (lo, hi) for s in (lo, hi)])
+    return every.amin(0), every.amax(0)
+
+
 def moe_pairs(x, ids, fc1, fc2, base: int = 0):
-    """FP64 [M, k, H_out]: each pair's expert output, zero where the id is not one of base .. base + E - 1. fc1 / fc2: (codes, scales)
-    stacked; gated (fc1 of 2 I rows, [up; gate]) or ReLU^2."""
+    """FP64 [M, k, H_out] twice: each pair's expert output (zero where the id is not one of base .. base + E - 1), and how far one
+    computed with FP32 sums may be from it. fc1 / fc2: (codes, scales) stacked; gated (fc1 of 2 I rows, [up; gate]) or ReLU^2.
+
+    An FP32 sum of K products is off by at most K 2^-24 sum |x w|; silu moves by at most 1.1 times its argument's change, and is
+    off by 2^-20 of its value at most where it is computed. That moves h, and where it moves a value of h over a border between two codes, the
+    product's operand."""
     m, k = ids.shape
     experts, inter = fc2[0].shape[0], 2 * fc2[0].shape[2]
     xq = through(x)
-    out = torch.zeros(m, k, fc2[0].shape[1], dtype=torch.float64)
+    out, off = (torch.zeros(m, k, fc2[0].shape[1], dtype=torch.float64) for _ in range(2))
     for e in sorted(set(ids.flatten().tolist())):
         if not base <= e < base + experts:
             continue
         row, slot = torch.nonzero(ids == e, as_tuple=True)
-        y = xq[row] @ dequantize(fc1[0][e - base], fc1[1][e - base]).T
-        h = y[:, inter:] / (1.0 + torch.exp(-y[:, inter:])) * y[:, :inter] if fc1[0].shape[1] == 2 * inter else y.clamp(min=0) ** 2
-        out[row, slot] = through(h) @ dequantize(fc2[0][e - base], fc2[1][e - base]).T
-    return out
+        w1, w2 = dequantize(fc1[0][e - base], fc1[1][e - base]), dequantize(fc2[0][e - base], fc2[1][e - base])
+        y = xq[row] @ w1.T
+        dy = w1.shape[1] * 2.0 ** -24 * (xq[row].abs() @ w1.abs().T)
+        if w1.shape[0] == 2 * inter:
+            up, gate, dup, dgate = y[:, :inter], y[:, inter:], dy[:, :inter], dy[:, inter:]
+            silu = gate / (1.0 + torch.exp(-gate))
+            h = silu * up
+            dh = 1.1 * dgate * (up.abs() + dup) + silu.abs() * dup + 2.0 ** -20 * h.abs()
+        else:
+            h = y.clamp(min=0) ** 2
+            dh = 2 * y.clamp(min=0) * dy + dy ** 2 + 2.0 ** -24 * h
+        hq = through(h)
+        least, most = between((h.abs() - dh).clamp(min=0), h.abs() + dh)
+        spread = torch.maximum(hq.abs() - least, most - hq.abs())
+        spread = spread + torch.where(dh >= h.abs(), most, torch.zeros_like(most))  # (a value that may be of the other sign)
+        out[row, slot] = hq @ w2.T
+        off[row, slot] = spread @ w2.abs().T + inter * 2.0 ** -24 * ((hq.abs() + spread) @ w2.abs().T)
+    return out, off
 
 
-def moe(x, ids, weights, fc1, fc2, base: int = 0) -> torch.Tensor:
-    """FP64 [M, H_out]: the weighted sum of a row's pairs."""
-    pairs = moe_pairs(x, ids, fc1, fc2, base)
-    named = (ids >= base) & (ids < base + fc2[0].shape[0])
-    return torch.where(named[..., None], pairs * weights.double()[..., None], torch.zeros_like(pairs)).sum(1)
+def moe(x, ids, weights, fc1, fc2, base: int = 0):
+    """FP64 [M, H_out] twice: the weighted sum of a row's pairs, and how far an FP32 one may be from it ahead of its last rounding."""
+    y, off = moe_pairs(x, ids, fc1, fc2, base)
+    w = torch.where((ids >= base) & (ids < base + fc2[0].shape[0]), weights.double(), torch.zeros(ids.shape, dtype=torch.float64))[..., None]
+    return (y * w).sum(1), (off * w.abs()).sum(1) + (ids.shape[1] + 1) * 2.0 ** -24 * (y * w).abs().sum(1)

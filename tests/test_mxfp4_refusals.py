@@ -67,3 +67,38 @@ def test_python_refusals():
         ops.mxfp4_linear(held, lin, torch.float64)
     with pytest.raises(RuntimeError):
         ops.mxfp4_linear(bf, lin)
+
+
+def test_routed_experts_refusals():
+    from hibana_amd.kernels import mxfp4_moe
+    lib = _lib.lib()
+    ok = dict(fc1=256, fc2=256, experts=8, base=0, hidden=256, inter=128, hidden_out=256, gated=1)
+    ex = _lib.HbMxfp4Experts(*ok.values())
+    need = lib.hb_mxfp4_moe_workspace_bytes(C.byref(ex), 4, 2)
+    assert need >= 8 * 256 * 4 and lib.hb_mxfp4_moe_workspace_bytes(None, 4, 2) == 0 and lib.hb_mxfp4_moe_workspace_bytes(C.byref(ex), 0, 2) == 0
+    call = lambda **c: lib.hb_mxfp4_moe(*{**dict(ex=C.byref(ex), x=256, ids=256, w=256, m=4, k=2, mode=0, out=256, ws=256, size=need, stream=None), **c}.values())  # noqa: E731
+    for c in [dict(ex=None), dict(x=None), dict(ids=None), dict(w=None), dict(out=None), dict(ws=None)]:
+        assert call(**c) == _lib.HB_ENULL, c
+    for c in [dict(m=0), dict(k=0), dict(mode=3), dict(mode=-1), dict(m=1 << 30), dict(x=264), dict(ids=258), dict(w=257), dict(out=260), dict(ws=264)]:
+        assert call(**c) == _lib.HB_EINVAL, c
+    assert call(size=need - 1) == _lib.HB_EWORKSPACE
+    for c in [dict(hidden=48), dict(inter=80), dict(hidden_out=260), dict(experts=0), dict(base=-1), dict(fc1=264), dict(hidden=0)]:
+        bad = _lib.HbMxfp4Experts(*{**ok, **c}.values())
+        assert lib.hb_mxfp4_moe_workspace_bytes(C.byref(bad), 4, 2) == 0 and call(ex=C.byref(bad)) == _lib.HB_EINVAL, c
+    assert call(ex=C.byref(_lib.HbMxfp4Experts(*{**ok, "fc2": None}.values()))) == _lib.HB_ENULL
+    u8 = lambda *s: torch.zeros(s, dtype=torch.uint8)  # noqa: E731
+    good = (u8(4, 64, 48), u8(4, 64, 3), u8(4, 96, 16), u8(4, 96, 1))
+    held = mxfp4_moe.Mxfp4Experts(*good)
+    assert held.gated and held.experts == 4
+    for i, t in [(0, u8(4, 64, 40)), (0, u8(4, 80, 48)), (1, u8(4, 64, 5)), (2, u8(3, 96, 16)), (2, u8(4, 96, 32))]:
+        with pytest.raises(ValueError):
+            mxfp4_moe.Mxfp4Experts(*(t if j == i else g for j, g in enumerate(good)))
+    with pytest.raises(ValueError):
+        mxfp4_moe.Mxfp4Experts(*good, base=-1)
+    x, ids, w = torch.zeros(2, 96, dtype=torch.bfloat16), torch.zeros(2, 3, dtype=torch.int32), torch.zeros(2, 3)
+    held.tiled1 = held.tiled2 = u8(1)  # (not read: every call below is refused)
+    for bad in [(x.float(), ids, w), (x[:, :64], ids, w), (x, ids[:1], w), (x, ids, w[:, :2]), (x[0], ids, w)]:
+        with pytest.raises(ValueError):
+            mxfp4_moe.mxfp4_moe(held, *bad)
+    with pytest.raises(RuntimeError):
+        mxfp4_moe.mxfp4_moe(held, x, ids, w)  # no CPU path
