@@ -1,6 +1,7 @@
 // The microscaled four-bit format: rounding to it (alone, and behind a gated activation), the values back, the weights' tile
 // layout, and the linear.
 #include <algorithm>
+#include <type_traits>
 
 #include "mxfp4.hpp"
 #include "stream_common.hpp"
@@ -133,9 +134,9 @@ __global__ __launch_bounds__(256) void mx_silu_quantize_kernel(const T* __restri
 
 // ------------------------------------------------------------------------------------------------ the weights' layout
 // The matrix row that row `r` of tile `t` holds. `gated_inter` (a gated pair [up; gate] of that many rows each): up and gate
-// tiles alternate, so that four consecutive tiles are the two factors of 32 consecutive columns of their product.
+// tiles alternate, so that two consecutive tiles are the two factors of 32 consecutive columns of their product.
 __device__ __forceinline__ int64_t mx_source_row(int t, int r, int gated_inter) {
-  return gated_inter ? (int64_t)(t & 1) * gated_inter + (t >> 1) * 16 + r : (int64_t)t * 16 + r;
+  return gated_inter ? (int64_t)(t & 1) * gated_inter + (t >> 1) * MX_ROWS + r : (int64_t)t * MX_ROWS + r;
 }
 
 // Row-major codes and scales of `matrices` matrices -> their tile layouts (UNPACK: the way back). A thread a (tile, lane): 16
@@ -152,8 +153,8 @@ __global__ __launch_bounds__(256) void mx_repack_kernel(uint8_t* __restrict__ co
   const int lane = (int)(i & 63);
   const int64_t tc = i >> 6;
   const int t = (int)(tc / (at.quads * 4)), c = (int)(tc - (int64_t)t * at.quads * 4);  // chunks past the last only have scales
-  const int64_t row = mx_source_row(t, lane & 15, gated_inter);
-  const int group = 4 * c + (lane >> 4);
+  const int64_t row = mx_source_row(t, lane & 31, gated_inter);
+  const int group = 2 * c + (lane >> 5);
   const bool in = row < n && group < k / 32;
   uint8_t* scale_at = tiled + at.codes() + ((int64_t)t * at.quads + (c >> 2)) * 256 + lane * 4 + (c & 3);
   i32x4_t* code_at = reinterpret_cast<i32x4_t*>(tiled + (((int64_t)t * at.chunks + c) * 64 + lane) * 16);
@@ -177,71 +178,7 @@ struct MxLinear {
   int k, waves;
 };
 
-// A row's group as the product's operand: rounded on the way (T: a value type), or read (uint8_t: row-major codes).
-template <typename T>
-__device__ __forceinline__ i32x4_t mx_acts(const void* x, const uint8_t*, int64_t row, int k, int group, uint32_t& byte) {
-  return mx_round_group<T>(static_cast<const T*>(x) + row * k + 32 * (int64_t)group, byte);
-}
-template <>
-__device__ __forceinline__ i32x4_t mx_acts<uint8_t>(const void* x, const uint8_t* scales, int64_t row, int k, int group, uint32_t& byte) {
-  byte = scales[row * (k / 32) + group];
-  return *reinterpret_cast<const i32x4_t*>(static_cast<const uint8_t*>(x) + row * (k / 2) + 16 * (int64_t)group);
-}
-
-// Up to sixteen rows: a workgroup NT tiles of weight rows, its wavefronts the chunks of K, their sums added through LDS in
-// wavefront order.
-template <typename T, typename Y, int NT>
-__global__ __launch_bounds__(1024) void mx_few_rows_kernel(MxLinear p) {
-  extern __shared__ f32x4_t part[];  // [waves][NT][64]
-  const MxLayout at(p.n, p.k);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
-  const int t0 = blockIdx.x * NT, groups = p.k / 32;
-  const int64_t row0 = (int64_t)blockIdx.y * 16;
-  const int c0 = (int)((int64_t)at.chunks * wave / p.waves), c1 = (int)((int64_t)at.chunks * (wave + 1) / p.waves);
-  const bool real = row0 + r < p.m;
-  f32x4_t acc[NT];
-#pragma unroll
-  for (int t = 0; t < NT; t++) acc[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  for (int c = c0; c < c1; c++) {
-    i32x4_t w[NT], a = {0, 0, 0, 0};
-    uint32_t sw[NT], sa = 0;
-#pragma unroll
-    for (int t = 0; t < NT; t++) {
-      const int tile = min(t0 + t, at.tiles - 1);  // past the last: its product is not stored
-      w[t] = *reinterpret_cast<const i32x4_t*>(p.w + (((int64_t)tile * at.chunks + c) * 64 + lane) * 16);
-      sw[t] = *reinterpret_cast<const uint32_t*>(p.w + at.codes() + ((int64_t)tile * at.quads + (c >> 2)) * 256 + lane * 4) >> (8 * (c & 3));
-    }
-    if (real && 4 * c + g < groups) a = mx_acts<T>(p.x, p.x_scales, row0 + r, p.k, 4 * c + g, sa);
-#pragma unroll
-    for (int t = 0; t < NT; t++) acc[t] = mx_mfma(w[t], sw[t], a, sa, acc[t]);
-  }
-#pragma unroll
-  for (int t = 0; t < NT; t++) part[(wave * NT + t) * 64 + lane] = acc[t];
-  __syncthreads();
-  for (int i = threadIdx.x; i < NT * 64; i += blockDim.x) {
-    f32x4_t sum = part[i];
-    for (int w = 1; w < p.waves; w++) sum += part[w * NT * 64 + i];
-    const int l = i & 63, t = t0 + (i >> 6);
-    const int64_t row = row0 + (l & 15), n = (int64_t)t * 16 + 4 * (l >> 4);
-    if (row < p.m)
-#pragma unroll
-      for (int j = 0; j < 4; j++)
-        if (n + j < p.n) static_cast<Y*>(p.y)[row * p.n + n + j] = mx_out<Y>(sum[j]);
-  }
-}
-
-// More than sixteen rows: both operands in the tile layout. A workgroup's WM x WN wavefronts hold WM MT x WN NT output tiles of 16 x 16;
-// two chunks of K of its rows of both operands are a stage, asked for while the stage before is multiplied, written to LDS (a tile as
-// it lies: a wavefront reads and writes 1024 consecutive bytes, no bank twice) when that is done, one barrier a stage. k past the matrix
-// has scale 0 on both sides: 2^-254 of anything is nothing in FP32, so what the codes hold there does not matter.
-struct MxTiles {
-  const uint8_t* a;
-  const uint8_t* w;
-  void* y;
-  int64_t m, n;
-  int k, rows_of_tiles;  // workgroups along m
-};
-
+// Four neighbouring results of a row, `left` of them inside the matrix.
 template <typename Y>
 __device__ __forceinline__ void mx_store4(Y* out, const f32x4_t& v, int64_t left, bool whole) {
   if (whole) {
@@ -254,137 +191,66 @@ __device__ __forceinline__ void mx_store4(Y* out, const f32x4_t& v, int64_t left
   }
 }
 
-template <int WM, int WN, int MT, int NT>
-struct MxTileCore {
-  static constexpr int WAVES = WM * WN, TA = WM * MT, TB = WN * NT, STAGE = 2 * (TA + TB), HELD = STAGE / WAVES;
-  static constexpr int LDS_BYTES = 2 * STAGE * 1024;
-  static_assert(STAGE % WAVES == 0, "whole tiles a wavefront");
-};
-
-template <typename Y, int WM, int WN, int MT, int NT>
-__global__ __launch_bounds__(64 * WM * WN) void mx_tile_kernel(MxTiles p) {
-  using Core = MxTileCore<WM, WN, MT, NT>;
-  constexpr int WAVES = Core::WAVES, TA = Core::TA, TB = Core::TB, HELD = Core::HELD, STAGE = Core::STAGE;
-  extern __shared__ i32x4_t lds[];  // [2][2 chunks][TA + TB][64]
-  const MxLayout la(p.m, p.k), lw(p.n, p.k);
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
-  // consecutive workgroups go to the eight dies in turn: each die walks a run of tiles, rows fastest, so that its L2 keeps a run of weights
-  const int total = gridDim.x, per = (total + 7) / 8, id = (int)(blockIdx.x % 8) * per + (int)(blockIdx.x / 8);
-  const int whole_runs = total % 8 ? total % 8 : 8;  // dies with `per` workgroups; the others have one less
-  const int at = (int)(blockIdx.x % 8) < whole_runs ? id : id - ((int)(blockIdx.x % 8) - whole_runs);
-  const int tm = at % p.rows_of_tiles, tn = at / p.rows_of_tiles;
-  const int a0 = tm * TA, b0 = tn * TB, stages = (la.chunks + 1) / 2;
-
-  const uint8_t* src[HELD];  // this wavefront's tiles of a stage, at chunk 0
-#pragma unroll
-  for (int j = 0; j < HELD; j++) {
-    const int t = (wave + j * WAVES) % (TA + TB);
-    const bool act = t < TA;
-    const int tile = act ? min(a0 + t, la.tiles - 1) : min(b0 + t - TA, lw.tiles - 1);
-    src[j] = (act ? p.a : p.w) + (int64_t)tile * la.chunks * 1024;
-  }
-  i32x4_t held[HELD];
-  auto ask = [&](int s) {
-#pragma unroll
-    for (int j = 0; j < HELD; j++) {
-      const int c = min(2 * s + (wave + j * WAVES) / (TA + TB), la.chunks - 1);
-      held[j] = *reinterpret_cast<const i32x4_t*>(src[j] + c * 1024 + lane * 16);
+// Few rows: a workgroup NT tiles of weight rows, its wavefronts the chunks of K. The first weights are asked for, then the workgroup puts
+// the activations into LDS, rounded on the way: each workgroup all of them, which costs less than a launch.
+template <typename T, typename Y, int NT, int RUN>
+__global__ __launch_bounds__(512) void mx_few_rows_kernel(MxLinear p) {
+  extern __shared__ f32x4_t part[];  // the activations, then [waves][NT * 4][64]
+  const MxLayout at(p.n, p.k);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), t0 = blockIdx.x * NT, rows = (int)p.m, groups = p.k / MX_GROUP;
+  MxStream<NT, RUN> s(p.w, at, t0, wave, p.waves);
+  const MxActs acts(part, rows, p.k);
+  for (int i = threadIdx.x; i < rows * groups; i += blockDim.x) {
+    const int r = i / groups, group = i - r * groups;
+    if constexpr (std::is_same_v<T, uint8_t>) {
+      acts.put(r, group, static_cast<const uint8_t*>(p.x) + (int64_t)r * (p.k / 2), p.x_scales + (int64_t)r * groups);
+    } else {
+      acts.put(r, group, static_cast<const T*>(p.x) + (int64_t)r * p.k + MX_GROUP * group);
     }
-  };
-  auto put = [&](int buf) {
-#pragma unroll
-    for (int j = 0; j < HELD; j++) lds[(buf * STAGE + wave + j * WAVES) * 64 + lane] = held[j];
-  };
-  uint32_t sa[MT], sb[NT];
-  auto scales = [&](int q) {
-#pragma unroll
-    for (int t = 0; t < MT; t++)
-      sa[t] = *reinterpret_cast<const uint32_t*>(p.a + la.codes() + ((int64_t)min(a0 + wm * MT + t, la.tiles - 1) * la.quads + q) * 256 + lane * 4);
-#pragma unroll
-    for (int t = 0; t < NT; t++)
-      sb[t] = *reinterpret_cast<const uint32_t*>(p.w + lw.codes() + ((int64_t)min(b0 + wn * NT + t, lw.tiles - 1) * lw.quads + q) * 256 + lane * 4);
-  };
-  f32x4_t acc[MT][NT];
-#pragma unroll
-  for (int i = 0; i < MT; i++)
-#pragma unroll
-    for (int j = 0; j < NT; j++) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-
-  ask(0);
-  scales(0);
-  put(0);
+  }
   __syncthreads();
-#define MX_CHUNK(BUF, C, OP)                                                                                                              \
-  {                                                                                                                                       \
-    const i32x4_t* at_a = lds + ((BUF) * STAGE + (C) * (TA + TB) + wm * MT) * 64 + lane;                                                   \
-    const i32x4_t* at_b = lds + ((BUF) * STAGE + (C) * (TA + TB) + TA + wn * NT) * 64 + lane;                                              \
-    i32x4_t fa[MT];                                                                                                                       \
-    _Pragma("unroll") for (int i = 0; i < MT; i++) fa[i] = at_a[i * 64];                                                                   \
-    _Pragma("unroll") for (int j = 0; j < NT; j++) {                                                                                       \
-      const i32x4_t fb = at_b[j * 64];                                                                                                    \
-      const i32x8_t wb = __builtin_shufflevector(fb, fb, 0, 1, 2, 3, -1, -1, -1, -1);                                                      \
-      _Pragma("unroll") for (int i = 0; i < MT; i++) {                                                                                     \
-        const i32x8_t wa = __builtin_shufflevector(fa[i], fa[i], 0, 1, 2, 3, -1, -1, -1, -1);                                              \
-        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wb, wa, acc[i][j], 4, 4, OP, (int)sb[j], OP, (int)sa[i]);             \
-      }                                                                                                                                   \
-    }                                                                                                                                     \
-  }
-  for (int s = 0; s < stages; s += 2) {
-    if (s + 1 < stages) ask(s + 1);
-    MX_CHUNK(0, 0, 0)
-    MX_CHUNK(0, 1, 1)
-    if (s + 1 < stages) {
-      put(1);
-      __syncthreads();
-      if (s + 2 < stages) ask(s + 2);
-      MX_CHUNK(1, 0, 2)
-      MX_CHUNK(1, 1, 3)
-      if (s + 2 < stages) {
-        scales((s + 2) / 2);
-        put(0);
-        __syncthreads();
-      }
-    }
-  }
-#undef MX_CHUNK
-  const int r = lane & 15, g = lane >> 4;
-  const bool aligned4 = p.n % 4 == 0;
-#pragma unroll
-  for (int i = 0; i < MT; i++) {
-    const int64_t row = (int64_t)(a0 + wm * MT + i) * 16 + r;
-    if (row >= p.m) continue;
-#pragma unroll
-    for (int j = 0; j < NT; j++) {
-      const int64_t n = (int64_t)(b0 + wn * NT + j) * 16 + 4 * g;
-      if (n < p.n) mx_store4<Y>(static_cast<Y*>(p.y) + row * p.n + n, acc[i][j], p.n - n, aligned4);
-    }
+  s.run(acts);
+  mx_hand_over<NT>(part, s.acc);
+  for (int i = threadIdx.x; i < NT * 256; i += blockDim.x) {
+    const f32x4_t sum = mx_joined<NT>(part, p.waves, i);
+    const int l = i & 63, q = (i >> 6) & 3, t = t0 + (i >> 8);
+    const int64_t row = l & 31, n = (int64_t)t * MX_ROWS + 8 * q + 4 * (l >> 5);
+    if (row < p.m && n < p.n) mx_store4<Y>(static_cast<Y*>(p.y) + row * p.n + n, sum, p.n - n, p.n % 4 == 0);
   }
 }
 
-// Many rows: 256 x 256 outputs a workgroup, 128 x 128 a wavefront (256 accumulator registers, one wavefront a SIMD), so that a matrix
-// instruction's operands come from LDS at 48 of the 128 bytes a cycle it gives ... Four buffers of one chunk of K; a chunk's 32 tiles come by
-// LDS-direct loads, asked for three steps ahead and waited for one step before they are read, so that a step can fetch the next
-// one's first fragments ahead of the barrier between them. A separate array a buffer: the compiler then knows that reading one
-// does not wait for the loads into another.
-struct MxBig {
-  static constexpr int TA = 16, TB = 16;
+// More rows: both operands in the tile layout. A workgroup's WM x WN wavefronts hold MT x NT output tiles of 32 x 32 each; 128 k of the
+// workgroup's rows of both operands are a step. LDS holds RING = 4 steps: a step's tiles come by LDS-direct loads (a tile as it lies: a
+// wavefront reads and writes 1024 consecutive bytes, no bank twice), asked for three steps ahead and waited for one step before they are
+// read, so that a step can fetch the next one's first fragments ahead of the barrier between them. A separate array a step: the
+// compiler then knows that reading one does not wait for the loads into another. k past the matrix has scale 0 on both sides: 2^-254 of
+// anything is nothing in FP32, so what is read in the place of its codes does not matter.
+//
+// Many rows take 2 x 2 wavefronts of 4 x 4 tiles: 256 accumulator registers, one wavefront a SIMD, and a matrix instruction's operands
+// come from LDS at half of the 128 bytes a cycle that it gives, what is asked for at a quarter.
+struct MxTiles {
+  const uint8_t* a;
+  const uint8_t* w;
+  void* y;
+  int64_t m, n;
+  int k, rows_of_tiles;  // workgroups along m
 };
 typedef __attribute__((address_space(3))) uint8_t* mx_lds_t;
 
 // mx_mfma with the sum staying in its accumulator registers (left to itself the compiler moves 256 of them about) and the scales in byte
 // OP of their words. The two wait states in front cover an operand that a vector instruction has just written, and hide behind the matrix
-// instruction before (16 cycles); mx_sums_done stands before the sums are read.
+// instruction before (32 cycles); mx_sums_done stands before the sums are read.
 template <int OP>
-__device__ __forceinline__ void mx_mfma_in_place(f32x4_t& acc, i32x4_t a, i32x4_t b, uint32_t sa, uint32_t sb) {
+__device__ __forceinline__ void mx_mfma_in_place(f32x16_t& acc, i32x4_t a, i32x4_t b, uint32_t sa, uint32_t sb) {
 #define MX_MFMA(SELECT) \
-  asm volatile("s_nop 1\n\tv_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 " SELECT " cbsz:4 blgp:4" : "+a"(acc) : "v"(a), "v"(b), "v"(sa), "v"(sb))
+  asm volatile("s_nop 1\n\tv_mfma_scale_f32_32x32x64_f8f6f4 %0, %1, %2, %0, %3, %4 " SELECT " cbsz:4 blgp:4" : "+a"(acc) : "v"(a), "v"(b), "v"(sa), "v"(sb))
   if constexpr (OP == 0) MX_MFMA("op_sel_hi:[0,0,0]");
   if constexpr (OP == 1) MX_MFMA("op_sel:[1,1,0] op_sel_hi:[0,0,0]");
   if constexpr (OP == 2) MX_MFMA("op_sel_hi:[1,1,0]");
   if constexpr (OP == 3) MX_MFMA("op_sel:[1,1,0] op_sel_hi:[1,1,0]");
 #undef MX_MFMA
 }
-__device__ __forceinline__ void mx_sums_done() { asm volatile("s_nop 15\n\ts_nop 7" ::: "memory"); }
+__device__ __forceinline__ void mx_sums_done() { asm volatile("s_nop 15\n\ts_nop 15" ::: "memory"); }
 
 // A buffer descriptor in scalar registers: what is read past `bytes` is zero.
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t mx_rows(const uint8_t* base, int bytes) {
@@ -393,168 +259,224 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t mx_rows(const uint8_t* base, i
   return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(hi << 32 | lo), 0, __builtin_amdgcn_readfirstlane(bytes), 0x00020000);
 }
 
-template <typename Y>
-__global__ __launch_bounds__(256, 1) void mx_big_kernel(MxTiles p) {
-  constexpr int T = MxBig::TA + MxBig::TB, ASKS = T / 4;
-  __shared__ i32x4_t buf0[T * 64], buf1[T * 64], buf2[T * 64], buf3[T * 64];
-  const MxLayout la(p.m, p.k), lw(p.n, p.k);
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave >> 1, wn = wave & 1;
-  const int total = gridDim.x, per = (total + 7) / 8, die = blockIdx.x % 8;
-  const int whole_runs = total % 8 ? total % 8 : 8;
-  const int at = die * per - (die > whole_runs ? die - whole_runs : 0) + (int)(blockIdx.x / 8);
-  const int tm = at % p.rows_of_tiles, tn = at / p.rows_of_tiles;
-  const int a0 = tm * MxBig::TA, b0 = tn * MxBig::TB, chunks = la.chunks;
-
-  // this wavefront's eight tiles of a chunk: of A for the first two wavefronts, of B for the others (past the last: the last again)
-  const bool act = wave < 2;
-  const int tiles = act ? la.tiles : lw.tiles, first = min((act ? a0 : b0) + (wave & 1) * 8, tiles - 1), left = min(8, tiles - first), row_bytes = chunks * 1024;
-  const __amdgpu_buffer_rsrc_t rows = mx_rows((act ? p.a : p.w) + (int64_t)first * row_bytes, left * row_bytes);
-#define MX_ASK(BUF, C)                                                                                                                    \
-  {                                                                                                                                       \
-    const int in_row = min((C), chunks - 1) * 1024;                                                                                       \
-    _Pragma("unroll") for (int j = 0; j < ASKS; j++)                                                                                      \
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rows, (mx_lds_t)(BUF + (wave * ASKS + j) * 64), 16, lane * 16, min(j, left - 1) * row_bytes + in_row, 0, 0); \
+// f(0), f(1) .. f(N - 1), each with its number as a constant.
+template <int N, int I = 0, class F>
+__device__ __forceinline__ void mx_unrolled(F&& f) {
+  if constexpr (I < N) {
+    f(std::integral_constant<int, I>());
+    mx_unrolled<N, I + 1>(f);
   }
+}
 
-  uint32_t sa[8], sb[8], na[8], nb[8];
-  auto scales = [&](int q) {
+// 32 rows x NT tiles of a wavefront's sums, stored. A lane holds four columns of one row, 8 or 16 bytes: stored as they are, an instruction
+// would touch 32 rows' lines. They go through the wavefront's own part of LDS and leave as whole rows of NT x 32 columns, 16 bytes a
+// lane; a row's 16-byte pieces are XORed with its number so that neither way meets a bank twice. (Where rows do not start on 16 bytes: as
+// they are.)
+template <typename Y, int NT>
+__device__ __forceinline__ void mx_store_rows(const MxTiles& p, i32x4_t* place, int64_t row0, int64_t n0, const f32x16_t (&sums)[NT]) {
+  constexpr int PIECES = NT * MX_ROWS * (int)sizeof(Y) / 16, ROWS = 64 / PIECES > 0 ? 64 / PIECES : 1;
+  const int lane = threadIdx.x & 63, r = lane & 31, g = lane >> 5;
+  Y* y = static_cast<Y*>(p.y);
+  if (p.n * (int)sizeof(Y) % 16 || reinterpret_cast<uintptr_t>(p.y) % 16) {
+    const int64_t row = row0 + r;
 #pragma unroll
-    for (int t = 0; t < 8; t++) {
-      na[t] = *reinterpret_cast<const uint32_t*>(p.a + la.codes() + ((int64_t)min(a0 + wm * 8 + t, la.tiles - 1) * la.quads + q) * 256 + lane * 4);
-      nb[t] = *reinterpret_cast<const uint32_t*>(p.w + lw.codes() + ((int64_t)min(b0 + wn * 8 + t, lw.tiles - 1) * lw.quads + q) * 256 + lane * 4);
+    for (int j = 0; j < NT; j++)
+#pragma unroll
+      for (int q = 0; q < 4; q++) {
+        const int64_t n = n0 + MX_ROWS * j + 8 * q + 4 * g;
+        if (row < p.m && n < p.n) mx_store4<Y>(y + row * p.n + n, mx_quarter(sums[j], q), p.n - n, false);
+      }
+    return;
+  }
+  uint8_t* bytes = reinterpret_cast<uint8_t*>(place);
+#pragma unroll
+  for (int j = 0; j < NT; j++)
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+      const int at = (MX_ROWS * j + 8 * q + 4 * g) * (int)sizeof(Y), piece = (at / 16) ^ (r & (PIECES - 1));
+      mx_store4<Y>(reinterpret_cast<Y*>(bytes + (r * PIECES + piece) * 16 + at % 16), mx_quarter(sums[j], q), 4, true);
     }
-  };
-  f32x4_t acc[8][8];
 #pragma unroll
-  for (int i = 0; i < 8; i++)
-#pragma unroll
-    for (int j = 0; j < 8; j++) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  for (int first = 0; first < MX_ROWS; first += ROWS) {
+    const int row = first + lane / PIECES, piece = lane % PIECES;
+    const int64_t n = n0 + piece * (16 / (int)sizeof(Y));
+    const i32x4_t v = place[row * PIECES + (piece ^ (row & (PIECES - 1)))];
+    if (row0 + row < p.m && n < p.n) *reinterpret_cast<i32x4_t*>(y + (row0 + row) * p.n + n) = v;
+  }
+}
 
-  scales(0);
-  MX_ASK(buf0, 0)
-  MX_ASK(buf1, 1)
-  MX_ASK(buf2, 2)
-  asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
-  __builtin_amdgcn_s_barrier();
-  i32x4_t fa[2][8], fb[4];
-#pragma unroll
-  for (int i = 0; i < 8; i++) fa[0][i] = buf0[(wm * 8 + i) * 64 + lane];
-  fb[0] = buf0[(16 + wn * 8) * 64 + lane];
-  fb[1] = buf0[(16 + wn * 8 + 1) * 64 + lane];
-#define MX_STEP(CUR, NEXT, ASKED, C, OP)                                                                                                   \
+template <typename Y, int WM, int WN, int MT, int NT>
+__global__ __launch_bounds__(64 * WM * WN, 1) void mx_ring_kernel(MxTiles p) {
+  constexpr int WAVES = WM * WN, TA = WM * MT, TB = WN * NT, T = TA + TB;
+  constexpr int ASKS_A = (2 * TA + WAVES - 1) / WAVES, ASKS_B = (2 * TB + WAVES - 1) / WAVES, ASKS = ASKS_A + ASKS_B;  // tiles a wavefront asks for a step
+  __shared__ i32x4_t buf0[2 * T * 64], buf1[2 * T * 64], buf2[2 * T * 64], buf3[2 * T * 64];  // [2 chunks][A tiles, B tiles][64]
+  const MxLayout la(p.m, p.k), lw(p.n, p.k);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
+  // consecutive workgroups go to the eight dies in turn: each die walks a run of tiles, rows fastest, so that its L2 keeps a run of weights
+  const int total = gridDim.x, per = (total + 7) / 8, die = blockIdx.x % 8, whole = total % 8 ? total % 8 : 8;  // the first `whole` dies have `per` workgroups, the others one less
+  const int at = die * per - (die > whole ? die - whole : 0) + (int)(blockIdx.x / 8);
+  const int a0 = at % p.rows_of_tiles * TA, b0 = at / p.rows_of_tiles * TB, chunks = la.chunks, row_bytes = chunks * 1024;
+
+  const int first_a = min(a0, la.tiles - 1), first_b = min(b0, lw.tiles - 1), left_a = min(TA, la.tiles - first_a), left_b = min(TB, lw.tiles - first_b);
+  const __amdgpu_buffer_rsrc_t rows_a = mx_rows(p.a + (int64_t)first_a * row_bytes, left_a * row_bytes);
+  const __amdgpu_buffer_rsrc_t rows_b = mx_rows(p.w + (int64_t)first_b * row_bytes, left_b * row_bytes);
+  // piece `wave + j * WAVES` of a step's 2 TA (2 TB): tile (that % TA) of chunk (that / TA); past the last piece, tile or chunk: the last again
+#define MX_ASK_OF(ROWS, TILES, LEFT, FIRST, BUF, S, J)                                                                                    \
   {                                                                                                                                       \
-    MX_ASK(ASKED, (C) + 3)                                                                                                               \
-    __builtin_amdgcn_sched_barrier(0);                                                                                                    \
-    _Pragma("unroll") for (int j = 0; j < 8; j++) {                                                                                       \
-      fb[(j + 2) & 3] = j < 6 ? CUR[(16 + wn * 8 + j + 2) * 64 + lane] : NEXT[(16 + wn * 8 + j - 6) * 64 + lane];                          \
-      fa[1 - ((OP) & 1)][j] = NEXT[(wm * 8 + j) * 64 + lane];                                                                             \
-      _Pragma("unroll") for (int i = 0; i < 8; i++) mx_mfma_in_place<OP>(acc[i][j], fb[j & 3], fa[(OP) & 1][i], sb[j], sa[i]);               \
-      __builtin_amdgcn_sched_barrier(0);                                                                                                  \
-    }                                                                                                                                     \
-    asm volatile("s_waitcnt vmcnt(8)" ::: "memory");                                                                                      \
-    __builtin_amdgcn_s_barrier();                                                                                                         \
-    __builtin_amdgcn_sched_barrier(0);                                                                                                    \
+    const int piece = min(wave + (J) * WAVES, 2 * TILES - 1), chunk = piece / TILES, tile = piece - chunk * TILES;                          \
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(ROWS, (mx_lds_t)(BUF + (chunk * T + FIRST + tile) * 64), 16, lane * 16,                       \
+                                             min(tile, LEFT - 1) * row_bytes + min(2 * (S) + chunk, chunks - 1) * 1024, 0, 0);            \
   }
-  for (int q = 0; q < la.quads; q++) {
+#define MX_ASK(BUF, S, J)                                         \
+  if constexpr ((J) < ASKS_B) {                                   \
+    MX_ASK_OF(rows_b, TB, left_b, TA, BUF, S, J)                  \
+  } else {                                                        \
+    MX_ASK_OF(rows_a, TA, left_a, 0, BUF, S, (J) - ASKS_B)        \
+  }
+
+  // the scales of this wavefront's tiles, a quad at a time
+  constexpr int SCALES = MT + NT;
+  const int scale_bytes = la.quads * 256, first_sa = min(a0 + wm * MT, la.tiles - 1), first_sb = min(b0 + wn * NT, lw.tiles - 1);
+  const int left_sa = min(MT, la.tiles - first_sa), left_sb = min(NT, lw.tiles - first_sb);
+  const __amdgpu_buffer_rsrc_t scales_a = mx_rows(p.a + la.codes() + (int64_t)first_sa * scale_bytes, left_sa * scale_bytes);
+  const __amdgpu_buffer_rsrc_t scales_b = mx_rows(p.w + lw.codes() + (int64_t)first_sb * scale_bytes, left_sb * scale_bytes);
+  uint32_t now[SCALES], next[SCALES];  // A's, then B's
+  auto scale = [&](int t, int q) {
+    next[t] = t < MT ? __builtin_amdgcn_raw_buffer_load_b32(scales_a, lane * 4, min(t, left_sa - 1) * scale_bytes + q * 256, 0)
+                     : __builtin_amdgcn_raw_buffer_load_b32(scales_b, lane * 4, min(t - MT, left_sb - 1) * scale_bytes + q * 256, 0);
+  };
+  f32x16_t acc[MT][NT];
 #pragma unroll
-    for (int t = 0; t < 8; t++) sa[t] = na[t], sb[t] = nb[t];
-    scales(min(q + 1, la.quads - 1));
-    MX_STEP(buf0, buf1, buf3, 4 * q, 0)
-    MX_STEP(buf1, buf2, buf0, 4 * q + 1, 1)
-    MX_STEP(buf2, buf3, buf1, 4 * q + 2, 2)
-    MX_STEP(buf3, buf0, buf2, 4 * q + 3, 3)
+  for (int i = 0; i < MT; i++)
+#pragma unroll
+    for (int j = 0; j < NT; j++)
+#pragma unroll
+      for (int e = 0; e < 16; e++) acc[i][j][e] = 0.f;
+
+#pragma unroll
+  for (int t = 0; t < SCALES; t++) scale(t, 0);
+  mx_unrolled<ASKS>([&](auto j) { MX_ASK(buf0, 0, j.value) });
+  mx_unrolled<ASKS>([&](auto j) { MX_ASK(buf1, 1, j.value) });
+  mx_unrolled<ASKS>([&](auto j) { MX_ASK(buf2, 2, j.value) });
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(ASKS) : "memory");
+  __builtin_amdgcn_s_barrier();
+  // a step: for each of its two chunks and each tile of B, the products with all tiles of A. Fragments come ahead of their use: B's two
+  // groups of products, A's a chunk.
+  constexpr int GROUPS = 2 * NT, AHEAD = GROUPS < 3 ? 1 : 2;
+  i32x4_t fa[2][MT], fb[4];
+  auto a_at = [&](const i32x4_t* buf, int chunk, int i) { return buf[(chunk * T + wm * MT + i) * 64 + lane]; };
+  auto b_at = [&](const i32x4_t* buf, int group) { return buf[(group / NT * T + TA + wn * NT + group % NT) * 64 + lane]; };
+#pragma unroll
+  for (int i = 0; i < MT; i++) fa[0][i] = a_at(buf0, 0, i);
+#pragma unroll
+  for (int j = 0; j < AHEAD; j++) fb[j] = b_at(buf0, j);
+  // What the step asks of memory (its tiles three steps on, and at a quad's first step the next quad's scales) goes out between the groups of products:
+  // in front of them all, it and the barrier would leave the matrix cores idle for a fifth of the step.
+#define MX_STEP(CUR, NEXT, ASKED, S, ODD)                                                                                                  \
+  mx_unrolled<GROUPS>([&](auto group) {                                                                                                   \
+    constexpr int v = group.value, u = v / NT, j = v % NT, ring = (ODD) * GROUPS + v;                                                      \
+    fb[(ring + AHEAD) & 3] = v + AHEAD < GROUPS ? b_at(CUR, v + AHEAD) : b_at(NEXT, v + AHEAD - GROUPS);                                   \
+    _Pragma("unroll") for (int i = j * MT / NT; i < (j + 1) * MT / NT; i++) fa[1 - u][i] = u == 0 ? a_at(CUR, 1, i) : a_at(NEXT, 0, i);     \
+    mx_unrolled<MT>([&](auto tile) {                                                                                                      \
+      constexpr int i = tile.value, at = v * MT + i;  /* the step's product */                                                            \
+      mx_mfma_in_place<2 * (ODD) + u>(acc[i][j], fb[ring & 3], fa[u][i], now[MT + j], now[i]);                                             \
+      constexpr int before = at * ASKS / (GROUPS * MT), after = (at + 1) * ASKS / (GROUPS * MT);                                           \
+      mx_unrolled<after - before>([&](auto k) { MX_ASK(ASKED, (S) + 3, before + k.value) });                                              \
+      if constexpr (!(ODD)) {                                                                                                             \
+        constexpr int from = at * SCALES / (GROUPS * MT), to = (at + 1) * SCALES / (GROUPS * MT);                                          \
+        mx_unrolled<to - from>([&](auto k) { scale(from + k.value, min((S) / 2 + 1, la.quads - 1)); });                                    \
+      }                                                                                                                                   \
+      __builtin_amdgcn_sched_barrier(0);                                                                                                  \
+    });                                                                                                                                   \
+  });                                                                                                                                     \
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"((ODD) ? ASKS : ASKS + SCALES) : "memory"); /* all but this step's have landed */                \
+  __builtin_amdgcn_s_barrier();                                                                                                           \
+  __builtin_amdgcn_sched_barrier(0);
+#define MX_QUAD                                                               \
+  _Pragma("unroll") for (int t = 0; t < SCALES; t++) now[t] = next[t];
+  for (int q = 0; q < la.quads; q += 2) {
+    MX_QUAD
+    MX_STEP(buf0, buf1, buf3, 2 * q, 0)
+    MX_STEP(buf1, buf2, buf0, 2 * q + 1, 1)
+    MX_QUAD
+    MX_STEP(buf2, buf3, buf1, 2 * q + 2, 0)
+    MX_STEP(buf3, buf0, buf2, 2 * q + 3, 1)
   }
+#undef MX_QUAD
 #undef MX_STEP
 #undef MX_ASK
+#undef MX_ASK_OF
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // what was asked for past the end arrives before the workgroup leaves its LDS
   mx_sums_done();
 #pragma unroll
-  for (int i = 0; i < 8; i++)
+  for (int i = 0; i < MT; i++)
 #pragma unroll
-    for (int j = 0; j < 8; j++) asm volatile("" : "+a"(acc[i][j]));
-  const int r = lane & 15, g = lane >> 4;
-  const bool aligned4 = p.n % 4 == 0;
+    for (int j = 0; j < NT; j++) asm volatile("" : "+a"(acc[i][j]));
+  __builtin_amdgcn_s_barrier();  // every wavefront has left the ring: each takes one of its buffers
+  i32x4_t* place = wave == 0 ? buf0 : wave == 1 ? buf1 : wave == 2 ? buf2 : buf3;
 #pragma unroll
-  for (int i = 0; i < 8; i++) {
-    const int64_t row = (int64_t)(a0 + wm * 8 + i) * 16 + r;
-    if (row >= p.m) continue;
-#pragma unroll
-    for (int j = 0; j < 8; j++) {
-      const int64_t n = (int64_t)(b0 + wn * 8 + j) * 16 + 4 * g;
-      if (n < p.n) mx_store4<Y>(static_cast<Y*>(p.y) + row * p.n + n, acc[i][j], p.n - n, aligned4);
-    }
-  }
+  for (int i = 0; i < MT; i++) mx_store_rows<Y, NT>(p, place, (int64_t)(a0 + wm * MT + i) * MX_ROWS, (int64_t)(b0 + wn * NT) * MX_ROWS, acc[i]);
 }
 
-// x [rows, k] rounded into the tile layout (rows past the last are left as they are: their results are not stored).
+// x [rows, k] rounded into the tile layout, a wavefront a tile: it reads 32 rows of 128 (FP32: 256) bytes, a lane its group,
+// whose codes are the 16 bytes that it owns. Rows past the last are left as they are (their results are not stored).
 template <typename T>
 __global__ __launch_bounds__(256) void mx_quantize_tiles_kernel(const T* __restrict__ x, int64_t rows, int k, uint8_t* __restrict__ tiled) {
   const MxLayout at(rows, k);
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int per_row = at.quads * 64;  // lanes of eight values, K in whole quads
-  const int64_t row = i / per_row;
-  if (row >= rows) return;  // whole groups leave together
-  const int e = (int)(i - row * per_row), group = e >> 2, c = group >> 2, lane = (group & 3) * 16 + (int)(row & 15);
-  const int64_t t = row >> 4;
-  uint32_t byte = 0, code = 0;
-  if (group < k / 32) {
-    Mx8<T> v;
-    v.load(x + row * k + 8 * e);
-    byte = mx_scale_byte(quad_max(v.amax()));
-    code = byte == 255u ? 0u : v.codes(mx_scale_value(byte));
-  }
-  if (c < at.chunks) *reinterpret_cast<uint32_t*>(tiled + ((t * at.chunks + c) * 64 + lane) * 16 + 4 * (e & 3)) = code;
-  if ((e & 3) == 0) tiled[at.codes() + (t * at.quads + (c >> 2)) * 256 + lane * 4 + (c & 3)] = (uint8_t)byte;
+  const int lane = threadIdx.x & 63, all = at.quads * 4;  // K's chunks in whole quads: those past the last only have scales
+  const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), t = i / all;
+  const int c = (int)(i - t * all), group = 2 * c + (lane >> 5);
+  const int64_t row = t * MX_ROWS + (lane & 31);
+  if (row >= rows) return;
+  uint32_t byte = 0;
+  i32x4_t code = {0, 0, 0, 0};
+  if (group < k / MX_GROUP) code = mx_round_group<T>(x + row * k + MX_GROUP * (int64_t)group, byte);
+  if (c < at.chunks) *reinterpret_cast<i32x4_t*>(tiled + ((t * at.chunks + c) * 64 + lane) * 16) = code;
+  tiled[at.codes() + (t * at.quads + (c >> 2)) * 256 + lane * 4 + (c & 3)] = (uint8_t)byte;
 }
 
-constexpr int MX_FEW_ROWS = 16;
+// Rows whose activations fit a workgroup's LDS twice a compute unit.
+static bool few_rows(int64_t m, int k) { return m <= MX_ROWS && MxActs::bytes(m, k) <= 64 * 1024; }
 
 template <typename Y, int WM, int WN, int MT, int NT>
-static int launch_tiles(MxTiles p, hipStream_t stream) {
-  using Core = MxTileCore<WM, WN, MT, NT>;
-  static const hipError_t raised = hipFuncSetAttribute(reinterpret_cast<const void*>(&mx_tile_kernel<Y, WM, WN, MT, NT>), hipFuncAttributeMaxDynamicSharedMemorySize, Core::LDS_BYTES);
-  if (raised != hipSuccess) return HB_ELAUNCH;
+static int launch_ring(MxTiles p, hipStream_t stream) {
   const MxLayout la(p.m, p.k), lw(p.n, p.k);
-  p.rows_of_tiles = (la.tiles + Core::TA - 1) / Core::TA;
-  const int64_t groups = (int64_t)p.rows_of_tiles * ((lw.tiles + Core::TB - 1) / Core::TB);
-  HB_LAUNCH((mx_tile_kernel<Y, WM, WN, MT, NT>), dim3((unsigned)groups), dim3(64 * WM * WN), Core::LDS_BYTES, stream, p);
+  p.rows_of_tiles = (la.tiles + WM * MT - 1) / (WM * MT);
+  const int64_t groups = (int64_t)p.rows_of_tiles * ((lw.tiles + WN * NT - 1) / (WN * NT));
+  HB_LAUNCH((mx_ring_kernel<Y, WM, WN, MT, NT>), dim3((unsigned)groups), dim3(64 * WM * WN), 0, stream, p);
   return HB_OK;
-}
-
-template <typename Y>
-static int launch_big(MxTiles p, hipStream_t stream) {
-  const MxLayout la(p.m, p.k), lw(p.n, p.k);
-  p.rows_of_tiles = (la.tiles + MxBig::TA - 1) / MxBig::TA;
-  HB_LAUNCH((mx_big_kernel<Y>), dim3((unsigned)(p.rows_of_tiles * ((lw.tiles + MxBig::TB - 1) / MxBig::TB))), dim3(256), 0, stream, p);
-  return HB_OK;
-}
-
-template <typename T, typename Y>
-static int launch_many(const MxLinear& p, uint8_t* tiles, hipStream_t stream) {
-  const MxLayout at(p.m, p.k);
-  if constexpr (std::is_same_v<T, uint8_t>) {
-    if (int e = hb_mxfp4_repack(p.x, p.x_scales, 1, p.m, p.k, 0, tiles, stream)) return e;
-  } else {
-    HB_LAUNCH((mx_quantize_tiles_kernel<T>), dim3((unsigned)((p.m * at.quads * 64 + 255) / 256)), dim3(256), 0, stream, static_cast<const T*>(p.x), p.m, p.k, tiles);
-  }
-  const MxTiles q{tiles, p.w, p.y, p.m, p.n, p.k, 0};
-  if (p.m <= 32) return launch_tiles<Y, 1, 4, 2, 2>(q, stream);
-  if (p.m <= 64) return launch_tiles<Y, 1, 4, 4, 2>(q, stream);
-  if (p.m <= 96) return launch_tiles<Y, 1, 4, 6, 2>(q, stream);
-  if (p.m <= 128) return launch_tiles<Y, 1, 4, 8, 2>(q, stream);
-  return launch_big<Y>(q, stream);
 }
 
 template <typename T, typename Y>
 static int launch_linear(const MxLinear& p0, uint8_t* tiles, hipStream_t stream) {
-  if (p0.m > MX_FEW_ROWS) return launch_many<T, Y>(p0, tiles, stream);
   MxLinear p = p0;
   const MxLayout at(p.n, p.k);
-  constexpr int NT = 4;
-  p.waves = std::min(at.chunks, 8);
-  const unsigned passes = (unsigned)((p.m + 15) / 16);
-  HB_LAUNCH((mx_few_rows_kernel<T, Y, NT>), dim3((unsigned)((at.tiles + NT - 1) / NT), passes), dim3(64 * p.waves), (size_t)p.waves * NT * 64 * 16, stream, p);
-  return HB_OK;
+  if (few_rows(p.m, p.k)) {
+    p.waves = std::min(at.chunks, 8);
+    const size_t acts = MxActs::bytes(p.m, p.k);
+    if (at.tiles < 512) {
+      if (at.chunks >= 32) {
+        HB_LAUNCH((mx_few_rows_kernel<T, Y, 1, 4>), dim3((unsigned)at.tiles), dim3(64 * p.waves), std::max(acts, (size_t)p.waves * 4096), stream, p);
+      } else {
+        HB_LAUNCH((mx_few_rows_kernel<T, Y, 1, 1>), dim3((unsigned)at.tiles), dim3(64 * p.waves), std::max(acts, (size_t)p.waves * 4096), stream, p);
+      }
+    } else {
+      HB_LAUNCH((mx_few_rows_kernel<T, Y, 2, 4>), dim3((unsigned)((at.tiles + 1) / 2)), dim3(64 * p.waves), std::max(acts, (size_t)p.waves * 8192), stream, p);
+    }
+    return HB_OK;
+  }
+  if constexpr (std::is_same_v<T, uint8_t>) {
+    if (int e = hb_mxfp4_repack(p.x, p.x_scales, 1, p.m, p.k, 0, tiles, stream)) return e;
+  } else {
+    const MxLayout rows(p.m, p.k);
+    HB_LAUNCH((mx_quantize_tiles_kernel<T>), dim3((unsigned)((int64_t)rows.tiles * rows.quads)), dim3(256), 0, stream, static_cast<const T*>(p.x), p.m, p.k, tiles);
+  }
+  const MxTiles q{tiles, p.w, p.y, p.m, p.n, p.k, 0};
+  if (p.m <= 32) return launch_ring<Y, 1, 4, 1, 1>(q, stream);
+  if (p.m <= 64) return launch_ring<Y, 1, 4, 2, 1>(q, stream);
+  if (p.m <= 96) return launch_ring<Y, 1, 4, 3, 1>(q, stream);
+  if (p.m <= 128) return launch_ring<Y, 1, 4, 4, 1>(q, stream);
+  return launch_ring<Y, 2, 2, 4, 4>(q, stream);
 }
 
 template <typename F>
@@ -614,7 +536,7 @@ extern "C" int hb_silu_mul_quant_mxfp4(const void* gate_up, int type, int64_t ro
 }
 
 // Sizes that the layout's indices and a launch's grid hold.
-static bool layout_holds(int64_t n, int k) { return n > 0 && k > 0 && k <= 1 << 25 && k % MX_GROUP == 0 && n <= (int64_t)1 << 30 && (n + 15) / 16 * ((k + 511) / 512) <= (int64_t)1 << 28; }
+static bool layout_holds(int64_t n, int k) { return n > 0 && k > 0 && k <= 1 << 23 && k % MX_GROUP == 0 && n <= (int64_t)1 << 30 && (n + 31) / 32 * ((k + 511) / 512) <= (int64_t)1 << 27; }
 
 extern "C" size_t hb_mxfp4_tiled_bytes(int64_t n, int k) { return layout_holds(n, k) ? (size_t)MxLayout(n, k).bytes() : 0; }
 
@@ -623,7 +545,7 @@ static int repack(bool unpack, void* codes, void* scales, int matrices, int64_t 
   if (!layout_holds(n, k) || matrices <= 0 || matrices > 65535 || (gated && n % 64)) return HB_EINVAL;
   if (!aligned(codes, 16) || !aligned(tiled, 16)) return HB_EINVAL;
   const MxLayout at(n, k);
-  const dim3 grid((unsigned)(((int64_t)at.tiles * at.quads * 256 + 255) / 256), (unsigned)matrices);
+  const dim3 grid((unsigned)(((int64_t)at.tiles * at.quads * 4 * 64 + 255) / 256), (unsigned)matrices);
   const int inter = gated ? (int)(n / 2) : 0;
   if (unpack) {
     HB_LAUNCH((mx_repack_kernel<true>), grid, dim3(256), 0, as_stream(stream), static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales), n, k, inter,
@@ -643,7 +565,7 @@ extern "C" int hb_mxfp4_unpack(const void* tiled, int matrices, int64_t n, int k
 
 extern "C" size_t hb_mxfp4_linear_workspace_bytes(int64_t m, int64_t n, int k, int x_type) {
   (void)x_type;
-  return m > MX_FEW_ROWS && layout_holds(n, k) && layout_holds(m, k) ? (size_t)MxLayout(m, k).bytes() : 0;
+  return m > 0 && layout_holds(n, k) && !few_rows(m, k) && layout_holds(m, k) ? (size_t)MxLayout(m, k).bytes() : 0;
 }
 
 extern "C" int hb_mxfp4_linear(const void* x, const void* x_scales, int x_type, int64_t m, const void* tiled, int64_t n, int k, void* y, int y_type,

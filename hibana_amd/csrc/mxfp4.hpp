@@ -15,22 +15,24 @@ namespace hb {
 
 typedef __attribute__((ext_vector_type(8))) int i32x8_t;
 typedef __attribute__((ext_vector_type(4))) int i32x4_t;
+typedef __attribute__((ext_vector_type(16))) float f32x16_t;
 typedef __attribute__((ext_vector_type(2))) _Float16 f16x2_t;
 typedef __attribute__((ext_vector_type(2))) unsigned short u16x2_t;
 typedef __attribute__((ext_vector_type(2))) float f32x2_t;
 
 constexpr int MX_GROUP = 32;
-constexpr int MX_ROWS = 16, MX_K = 128;  // a tile: what one matrix instruction takes of either operand
+constexpr int MX_ROWS = 32, MX_K = 64;  // a tile: what one matrix instruction takes of either operand
 
 // ------------------------------------------------------------------------------------------------ tile layout
-// A matrix [n, k] as the products read it: tiles of 16 rows x 128 k, [ceil(n / 16)][ceil(k / 128)], 1024 bytes of codes each, lane
-// l = 16 g + r of a wavefront owning the 16 bytes of row r, k = 32 g .. 32 g + 31: its operand of one
-// v_mfma_scale_f32_16x16x128_f8f6f4, so a tile is one 128-bit load a lane, 1024 consecutive bytes a wavefront. Behind the codes the
-// scales: four tiles' along K together, 256 bytes, lane l owning the four bytes of its row and its group in each of them.
-// Rows and k past the matrix hold code 0 and scale 0.
+// A matrix [n, k] as the products read it: tiles of 32 rows x 64 k, [ceil(n / 32)][ceil(k / 64)], 1024 bytes of codes each, lane
+// l = 32 g + r of a wavefront owning the 16 bytes of row r, k = 32 g .. 32 g + 31: its operand of one
+// v_mfma_scale_f32_32x32x64_f8f6f4, so a tile is one 128-bit load a lane, 1024 consecutive bytes a wavefront. Behind the codes the
+// scales: four tiles along K together (a quad), 256 bytes, lane l owning the four bytes of its row and its group in each of them; K in
+// whole pairs of quads. Rows and k past the matrix hold scale 0 (and code 0).
+// (32 x 32 x 64 and not 16 x 16 x 128: one wavefront a SIMD gets 9.2 PFLOP/s out of the former, 3.1 of the latter, four 9.5 and 4.6.)
 struct MxLayout {
-  int tiles, chunks, quads;  // 16-row tiles, 128-k chunks, groups of four chunks
-  __host__ __device__ MxLayout(int64_t n, int64_t k) : tiles((int)((n + MX_ROWS - 1) / MX_ROWS)), chunks((int)((k + MX_K - 1) / MX_K)), quads((chunks + 3) / 4) {}
+  int tiles, chunks, quads;  // 32-row tiles, 64-k chunks, groups of four chunks
+  __host__ __device__ MxLayout(int64_t n, int64_t k) : tiles((int)((n + MX_ROWS - 1) / MX_ROWS)), chunks((int)((k + MX_K - 1) / MX_K)), quads((chunks + 7) / 8 * 2) {}
   __host__ __device__ int64_t codes() const { return (int64_t)tiles * chunks * 1024; }
   __host__ __device__ int64_t bytes() const { return codes() + (int64_t)tiles * quads * 256; }
 };
@@ -124,7 +126,7 @@ __device__ __forceinline__ uint32_t quad_max(uint32_t x) {
   return o > x ? o : x;
 }
 
-// One lane's whole group of 32: the 16 bytes of codes, and the scale byte.
+// A lane's whole group of 32 values: the 16 bytes of codes and the scale byte (of a group that is not finite any codes: its scale is NaN).
 template <typename T>
 __device__ __forceinline__ i32x4_t mx_round_group(const T* p, uint32_t& byte) {
   Mx8<T> x[4];
@@ -132,24 +134,129 @@ __device__ __forceinline__ i32x4_t mx_round_group(const T* p, uint32_t& byte) {
   for (int j = 0; j < 4; j++) x[j].load(p + 8 * j);
   uint32_t m = x[0].amax();
 #pragma unroll
-  for (int j = 1; j < 4; j++) {
-    const uint32_t o = x[j].amax();
-    m = o > m ? o : m;
-  }
+  for (int j = 1; j < 4; j++) m = max(m, x[j].amax());
   byte = mx_scale_byte(m);
   const float s = mx_scale_value(byte);
-  const uint32_t finite = byte == 255u ? 0u : ~0u;
   i32x4_t c;
 #pragma unroll
-  for (int j = 0; j < 4; j++) c[j] = (int)(x[j].codes(s) & finite);
+  for (int j = 0; j < 4; j++) c[j] = (int)x[j].codes(s);
   return c;
 }
 
-// acc += (16 rows of a) x (16 rows of b)^T over 128 k, codes and scale bytes (in the low byte) in the lanes that own them. In the result
-// lane 16 g + r holds rows 4 g .. 4 g + 3 of a for row r of b.
-__device__ __forceinline__ f32x4_t mx_mfma(i32x4_t a, uint32_t sa, i32x4_t b, uint32_t sb, f32x4_t acc) {
+// The activations of a product of few rows, in LDS: codes [group][rows][16 bytes], scales [group][rows] behind them, so that the lanes of a
+// fragment read consecutive addresses.
+struct MxActs {
+  i32x4_t* codes;
+  uint8_t* scales;
+  int rows, groups;
+  __device__ __forceinline__ MxActs(void* lds, int rows, int k) : codes(static_cast<i32x4_t*>(lds)), scales(static_cast<uint8_t*>(lds) + (size_t)rows * (k / 2)), rows(rows), groups(k / MX_GROUP) {}
+  static __host__ __device__ size_t bytes(int64_t rows, int k) { return ((size_t)rows * (k / 2 + k / MX_GROUP) + 15) / 16 * 16; }
+  // Group `group` of row r: values rounded ...
+  template <typename T>
+  __device__ __forceinline__ void put(int r, int group, const T* values) const {
+    uint32_t byte;
+    codes[group * rows + r] = mx_round_group<T>(values, byte);
+    scales[group * rows + r] = (uint8_t)byte;
+  }
+  // ... or codes as they are.
+  __device__ __forceinline__ void put(int r, int group, const uint8_t* row_codes, const uint8_t* row_scales) const {
+    codes[group * rows + r] = *reinterpret_cast<const i32x4_t*>(row_codes + 16 * group);
+    scales[group * rows + r] = row_scales[group];
+  }
+};
+
+// acc += (32 rows of a) x (32 rows of b)^T over 64 k, codes and scale bytes (byte OP_A / OP_B of the words) in the lanes that own them. In the
+// result lane 32 g + r holds, in registers 4 q .. 4 q + 3, rows 8 q + 4 g .. + 3 of a for row r of b.
+template <int OP_A, int OP_B>
+__device__ __forceinline__ f32x16_t mx_mfma(i32x4_t a, uint32_t sa, i32x4_t b, uint32_t sb, f32x16_t acc) {
   const i32x8_t wa = __builtin_shufflevector(a, a, 0, 1, 2, 3, -1, -1, -1, -1), wb = __builtin_shufflevector(b, b, 0, 1, 2, 3, -1, -1, -1, -1);
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wa, wb, acc, 4, 4, 0, (int)sa, 0, (int)sb);  // 4: E2M1
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wa, wb, acc, 4, 4, OP_A, (int)sa, OP_B, (int)sb);  // 4: E2M1
+}
+__device__ __forceinline__ f32x4_t mx_quarter(const f32x16_t& v, int q) { return f32x4_t{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]}; }
+
+// A wavefront's sums over chunks c0 .. c1 - 1 (c0 a multiple of RUN: 1, 2 or 4) of NT tiles of weight rows from tile t0 (past the last: the
+// last again, not to be stored) and up to 32 activation rows: RUN chunks of weights are asked for ahead of the RUN that are multiplied.
+template <int NT, int RUN>
+struct MxStream {
+  const uint8_t *codes[NT], *scales[NT];
+  i32x4_t b[RUN][NT];
+  uint32_t sb[NT];
+  int c0, c1;
+  f32x16_t acc[NT];
+  __device__ __forceinline__ MxStream(const uint8_t* __restrict__ w, const MxLayout& at, int t0, int wave, int waves) {
+    const int lane = threadIdx.x & 63, runs = (at.chunks + RUN - 1) / RUN;
+    c0 = RUN * (runs * wave / waves);
+    c1 = min(at.chunks, RUN * (runs * (wave + 1) / waves));
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+      const int tile = min(t0 + t, at.tiles - 1);
+      codes[t] = w + (int64_t)tile * at.chunks * 1024 + lane * 16;
+      scales[t] = w + at.codes() + (int64_t)tile * at.quads * 256 + lane * 4;
+    }
+    ask(min(c0, at.chunks - 1));
+  }
+  __device__ __forceinline__ void ask(int c) {
+#pragma unroll
+    for (int t = 0; t < NT; t++) sb[t] = *reinterpret_cast<const uint32_t*>(scales[t] + (c >> 2) * 256);
+#pragma unroll
+    for (int u = 0; u < RUN; u++)
+#pragma unroll
+      for (int t = 0; t < NT; t++) b[u][t] = *reinterpret_cast<const i32x4_t*>(codes[t] + min(c + u, max(c1 - 1, 0)) * 1024);  // (past the end: asked for again, not multiplied)
+  }
+  template <int U>
+  __device__ __forceinline__ void step(const i32x4_t (&w)[RUN][NT], const uint32_t (&sw)[NT], const i32x4_t& a, uint32_t sa) {
+#pragma unroll
+    for (int t = 0; t < NT; t++) acc[t] = mx_mfma<U, 0>(w[U][t], sw[t], a, sa, acc[t]);
+  }
+  __device__ __forceinline__ void run(const MxActs& acts) {
+#pragma unroll
+    for (int t = 0; t < NT; t++)
+#pragma unroll
+      for (int i = 0; i < 16; i++) acc[t][i] = 0.f;
+    const int half = (threadIdx.x & 63) >> 5, r = min((int)(threadIdx.x & 31), acts.rows - 1);  // (rows past the last: that one again, not to be stored)
+    for (int c = c0; c < c1; c += RUN) {
+      i32x4_t now[RUN][NT], a[RUN];
+      uint32_t sw[NT], sa[RUN];
+#pragma unroll
+      for (int t = 0; t < NT; t++) sw[t] = RUN == 4 ? sb[t] : sb[t] >> (8 * (c & 3));
+#pragma unroll
+      for (int u = 0; u < RUN; u++) {
+        // (k past the matrix: the last group again; the weights' codes there are 0)
+        const int at = min(2 * (c + u) + half, acts.groups - 1) * acts.rows + r;
+        a[u] = acts.codes[at];
+        sa[u] = acts.scales[at];
+#pragma unroll
+        for (int t = 0; t < NT; t++) now[u][t] = b[u][t];
+      }
+      if (c + RUN < c1) ask(c + RUN);
+      step<0>(now, sw, a[0], sa[0]);
+      if constexpr (RUN > 1)
+        if (c + 1 < c1) step<1>(now, sw, a[1], sa[1]);
+      if constexpr (RUN > 2) {
+        if (c + 2 < c1) step<2>(now, sw, a[2], sa[2]);
+        if (c + 3 < c1) step<3>(now, sw, a[3], sa[3]);
+      }
+    }
+  }
+};
+
+// The wavefronts' sums of a workgroup added in wavefront order, through LDS: part [waves][NT * 4][64]. Entry i of NT * 256 is quarter
+// (i / 64) % 4 of tile i / 256, lane i % 64.
+template <int NT>
+__device__ __forceinline__ void mx_hand_over(f32x4_t* part, const f32x16_t (&acc)[NT]) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  __syncthreads();  // the activations' place
+#pragma unroll
+  for (int t = 0; t < NT; t++)
+#pragma unroll
+    for (int q = 0; q < 4; q++) part[((wave * NT + t) * 4 + q) * 64 + lane] = mx_quarter(acc[t], q);
+  __syncthreads();
+}
+template <int NT>
+__device__ __forceinline__ f32x4_t mx_joined(const f32x4_t* part, int waves, int i) {
+  f32x4_t sum = part[i];
+  for (int w = 1; w < waves; w++) sum += part[w * NT * 256 + i];
+  return sum;
 }
 
 // An FP32 sum in the result's type: one rounding.

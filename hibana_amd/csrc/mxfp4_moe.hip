@@ -22,104 +22,81 @@ struct MxMoe {
   void* y;                 // fc2: [pairs, n]
 };
 
-// One slot's (up to sixteen rows of an expert) product with NT tiles of weight rows; K split among the workgroup's wavefronts, their
-// sums added through LDS in wavefront order: sums[i] of the first NT * 64 threads, tile i / 64, lane i % 64.
-template <int NT>
-__device__ __forceinline__ f32x4_t mx_slot_sums(const MxMoe& p, const uint8_t* w, int t0, const uint8_t* codes, const uint8_t* scales, bool real, f32x4_t* part) {
-  const MxLayout at(p.n, p.k);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
-  const int c0 = at.chunks * wave / p.waves, c1 = at.chunks * (wave + 1) / p.waves;
-  f32x4_t acc[NT];
-#pragma unroll
-  for (int t = 0; t < NT; t++) acc[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  for (int c = c0; c < c1; c++) {
-    i32x4_t b[NT], a = {0, 0, 0, 0};
-    uint32_t sb[NT], sa = 0;
-#pragma unroll
-    for (int t = 0; t < NT; t++) {
-      const int tile = min(t0 + t, at.tiles - 1);  // past the last: not stored
-      b[t] = *reinterpret_cast<const i32x4_t*>(w + (((int64_t)tile * at.chunks + c) * 64 + lane) * 16);
-      sb[t] = *reinterpret_cast<const uint32_t*>(w + at.codes() + ((int64_t)tile * at.quads + (c >> 2)) * 256 + lane * 4) >> (8 * (c & 3));
-    }
-    if (real && 4 * c + g < p.k / 32) {
-      sa = scales[4 * c + g];
-      a = *reinterpret_cast<const i32x4_t*>(codes + 16 * (4 * c + g));
-    }
-#pragma unroll
-    for (int t = 0; t < NT; t++) acc[t] = mx_mfma(b[t], sb[t], a, sa, acc[t]);
+constexpr int MX_SLOT_ROWS = MX_ROWS;
+
+// A slot's (up to 32 rows of an expert) product with NT tiles of weight rows, K split among the workgroup's wavefronts: their sums in LDS.
+// row_of: the row of the activations that is the slot's row r.
+template <int NT, int RUN, class Row>
+__device__ __forceinline__ void mx_slot_product(const MxMoe& p, const uint8_t* w, int t0, int rows, Row&& row_of, f32x4_t* part) {
+  MxStream<NT, RUN> s(w, MxLayout(p.n, p.k), t0, __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), p.waves);
+  const MxActs acts(part, rows, p.k);
+  for (int i = threadIdx.x; i < rows * acts.groups; i += blockDim.x) {
+    const int r = i / acts.groups, group = i - r * acts.groups;
+    const int64_t row = row_of(r);
+    acts.put(r, group, p.aq + row * (p.k / 2), p.as + row * acts.groups);
   }
-#pragma unroll
-  for (int t = 0; t < NT; t++) part[(wave * NT + t) * 64 + lane] = acc[t];
   __syncthreads();
-  f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
-  if (threadIdx.x < NT * 64) {
-    sum = part[threadIdx.x];
-    for (int v = 1; v < p.waves; v++) sum += part[v * NT * 64 + threadIdx.x];
-  }
-  return sum;
+  s.run(acts);
+  mx_hand_over<NT>(part, s.acc);
 }
 
-// fc1: a workgroup 32 columns of h (gated: two pairs of an up and a gate tile) of a slot; h leaves rounded to the format.
+// fc1: a workgroup 32 columns of h of a slot (gated: the up tile and its gate tile); h leaves rounded to the format. Four lanes share a
+// row's group: wavefront q holds its columns 8 q + 4 g .. + 3 (g: the lane's half) ... joined through LDS.
 template <bool GATED>
-__global__ __launch_bounds__(1024) void mx_fc1_kernel(MxMoe p) {
-  constexpr int NT = GATED ? 4 : 2;
+__global__ __launch_bounds__(512) void mx_fc1_kernel(MxMoe p) {
+  constexpr int NT = GATED ? 2 : 1;
   extern __shared__ f32x4_t part[];
   const int32_t* entry = p.plan + PLAN_HEADER + 4 * (int)blockIdx.y;
   const int rows = entry[2], p0 = entry[1];
   if (rows == 0) return;
-  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-  const int64_t row = r < rows ? p.order[p0 + r] / p.topk : 0;
-  const f32x4_t sum = mx_slot_sums<NT>(p, p.w + entry[0] * p.expert_bytes, blockIdx.x * NT, p.aq + row * (p.k / 2), p.as + row * (p.k / 32), r < rows, part);
-  __syncthreads();
-  if (threadIdx.x < NT * 64) part[threadIdx.x] = sum;
-  __syncthreads();
-  if (threadIdx.x >= 64) return;
-  // a lane: row r, columns 4 g .. 4 g + 3 and 16 + 4 g .. of the 32
-  float h[8];
-#pragma unroll
-  for (int t = 0; t < 2; t++) {
-    const f32x4_t up = part[(GATED ? 2 * t : t) * 64 + lane], gate = GATED ? part[(2 * t + 1) * 64 + lane] : up;
+  const int lane = threadIdx.x & 63, r = lane & 31, g = lane >> 5;
+  mx_slot_product<NT, 4>(p, p.w + entry[0] * p.expert_bytes, blockIdx.x * NT, rows, [&](int i) { return (int64_t)(p.order[p0 + i] / p.topk); }, part);
+  const int q = threadIdx.x >> 6;  // the launch has at least four wavefronts
+  float h[4];
+  uint32_t top = 0;
+  if (q < 4) {
+    const f32x4_t up = mx_joined<NT>(part, p.waves, threadIdx.x), gate = GATED ? mx_joined<NT>(part, p.waves, 256 * (NT - 1) + threadIdx.x) : up;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
       const float u = fmaxf(up[j], 0.f);
-      h[4 * t + j] = GATED ? gate[j] / (1.0f + expf(-gate[j])) * up[j] : (up[j] != up[j] ? up[j] : u * u);
+      h[j] = GATED ? gate[j] / (1.0f + expf(-gate[j])) * up[j] : (up[j] != up[j] ? up[j] : u * u);
+      top = max(top, __float_as_uint(h[j]) & 0x7fffffffu);
     }
   }
-  uint32_t top = 0;
+  __syncthreads();  // the sums are read: their place takes the quarters' largest magnitudes
+  uint32_t* tops = reinterpret_cast<uint32_t*>(part);
+  if (q < 4) tops[q * 64 + lane] = top;
+  __syncthreads();
+  if (q >= 4 || r >= rows) return;
 #pragma unroll
-  for (int j = 0; j < 8; j++) top = max(top, __float_as_uint(h[j]) & 0x7fffffffu);
-  top = max(top, (uint32_t)__shfl_xor((int)top, 16));
-  top = max(top, (uint32_t)__shfl_xor((int)top, 32));
+  for (int v = 0; v < 4; v++) top = max(top, max(tops[v * 64 + r], tops[v * 64 + 32 + r]));
   const uint32_t byte = mx_scale_byte(top);
   const float s = mx_scale_value(byte);
-  if (r >= rows) return;
   const int64_t inter = GATED ? p.n / 2 : p.n, pos = p0 + r;
-#pragma unroll
-  for (int t = 0; t < 2; t++) {
-    uint32_t c = 0;
-    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, h[4 * t], h[4 * t + 1], s, 0);
-    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, h[4 * t + 2], h[4 * t + 3], s, 1);
-    *reinterpret_cast<uint16_t*>(p.hq + pos * (inter / 2) + 16 * blockIdx.x + 8 * t + 2 * g) = byte == 255u ? 0 : (uint16_t)c;
-  }
-  if (g == 0) p.hs[pos * (inter / 32) + blockIdx.x] = (uint8_t)byte;
+  uint32_t c = 0;
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, h[0], h[1], s, 0);
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, h[2], h[3], s, 1);
+  *reinterpret_cast<uint16_t*>(p.hq + pos * (inter / 2) + 16 * blockIdx.x + 4 * q + 2 * g) = byte == 255u ? 0 : (uint16_t)c;
+  if (q == 0 && g == 0) p.hs[pos * (inter / 32) + blockIdx.x] = (uint8_t)byte;
 }
 
-// fc2: a workgroup 64 output columns of a slot, written by pair.
-template <typename Y>
-__global__ __launch_bounds__(1024) void mx_fc2_kernel(MxMoe p) {
-  constexpr int NT = 4;
+// fc2: a workgroup NT tiles of output columns of a slot, written by pair.
+template <typename Y, int NT>
+__global__ __launch_bounds__(512) void mx_fc2_kernel(MxMoe p) {
   extern __shared__ f32x4_t part[];
   const int32_t* entry = p.plan + PLAN_HEADER + 4 * (int)blockIdx.y;
   const int rows = entry[2], p0 = entry[1];
   if (rows == 0) return;
-  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-  const int64_t pos = p0 + min(r, rows - 1);
-  const f32x4_t sum = mx_slot_sums<NT>(p, p.w + entry[0] * p.expert_bytes, blockIdx.x * NT, p.aq + pos * (p.k / 2), p.as + pos * (p.k / 32), r < rows, part);
-  const int n = (blockIdx.x * NT + (threadIdx.x >> 6)) * 16 + 4 * g;
-  if (threadIdx.x >= NT * 64 || r >= rows || n >= p.n) return;  // n and p.n are multiples of four
-  Y* out = static_cast<Y*>(p.y) + (int64_t)p.order[p0 + r] * p.n + n;
-#pragma unroll
-  for (int j = 0; j < 4; j++) out[j] = (Y)sum[j];
+  const int r = threadIdx.x & 31;
+  mx_slot_product<NT, 2>(p, p.w + entry[0] * p.expert_bytes, blockIdx.x * NT, rows, [&](int i) { return (int64_t)p0 + i; }, part);
+  const int64_t pair = r < rows ? p.order[p0 + r] : 0;
+  for (int i = threadIdx.x; i < NT * 256; i += blockDim.x) {
+    const f32x4_t sum = mx_joined<NT>(part, p.waves, i);
+    const int n = (blockIdx.x * NT + (i >> 8)) * MX_ROWS + 8 * ((i >> 6) & 3) + 4 * ((i & 63) >> 5);
+    if (r >= rows || n >= p.n) continue;  // n and p.n are multiples of four
+    typedef __attribute__((ext_vector_type(4))) Y y4_t;
+    *reinterpret_cast<y4_t*>(static_cast<Y*>(p.y) + pair * p.n + n) = y4_t{(Y)sum[0], (Y)sum[1], (Y)sum[2], (Y)sum[3]};
+  }
 }
 
 namespace {
@@ -180,27 +157,29 @@ extern "C" int hb_mxfp4_moe(const hb_mxfp4_experts* experts, const void* x, cons
   const bool sum = mode == HB_MOE_SUM;
   const MxWorkspace ws = carve(experts, workspace, m, topk, sum);
   if (workspace_bytes < ws.bytes) return HB_EWORKSPACE;
-  const int64_t pairs = (int64_t)m * topk, slots = moe_max_slots(pairs, experts->experts, 0);
+  const int64_t pairs = (int64_t)m * topk, slots = moe_max_slots(pairs, experts->experts, 0, MX_SLOT_ROWS);
   if (slots > 65535) return HB_EINVAL;
   hipStream_t s = as_stream(stream);
-  if (int e = moe_launch_plan(ids, pairs, experts->base, experts->experts, 0, ws.plan, s)) return e;
+  if (int e = moe_launch_plan(ids, pairs, experts->base, experts->experts, 0, ws.plan, s, MX_SLOT_ROWS)) return e;
   if (int e = hb_mxfp4_quantize(x, HB_BF16, m, experts->hidden, ws.xq, ws.xs, stream)) return e;
   const MxLayout l1(fc1_rows(experts), experts->hidden), l2(experts->hidden_out, experts->inter);
   MxMoe p1{static_cast<const uint8_t*>(experts->fc1), l1.bytes(), ws.xq, ws.xs, ws.plan.plan, ws.plan.order, fc1_rows(experts), experts->hidden, topk,
-           std::min(l1.chunks, 8), ws.hq, ws.hs, nullptr};
+           8, ws.hq, ws.hs, nullptr};
   MxMoe p2{static_cast<const uint8_t*>(experts->fc2), l2.bytes(), ws.hq, ws.hs, ws.plan.plan, ws.plan.order, experts->hidden_out, experts->inter, topk,
-           std::max(4, std::min(l2.chunks, 8)), nullptr, nullptr, sum ? ws.y : out};
-  const dim3 grid1((unsigned)(experts->inter / 32), (unsigned)slots), grid2((unsigned)((l2.tiles + 3) / 4), (unsigned)slots);
-  p1.waves = std::max(4, p1.waves);
+           4, nullptr, nullptr, sum ? ws.y : out};
+  const int most = (int)std::min<int64_t>(MX_SLOT_ROWS, pairs);
+  const size_t acts1 = MxActs::bytes(most, experts->hidden), acts2 = MxActs::bytes(most, experts->inter);
+  if (acts1 > 64 * 1024 || acts2 > 64 * 1024) return HB_EINVAL;
+  const dim3 grid1((unsigned)(experts->inter / 32), (unsigned)slots), grid2((unsigned)((l2.tiles + 1) / 2), (unsigned)slots);
   if (experts->gated) {
-    HB_LAUNCH((mx_fc1_kernel<true>), grid1, dim3(64 * p1.waves), (size_t)p1.waves * 4 * 1024, s, p1);
+    HB_LAUNCH((mx_fc1_kernel<true>), grid1, dim3(64 * p1.waves), std::max(acts1, (size_t)p1.waves * 2 * 4096), s, p1);
   } else {
-    HB_LAUNCH((mx_fc1_kernel<false>), grid1, dim3(64 * p1.waves), (size_t)p1.waves * 2 * 1024, s, p1);
+    HB_LAUNCH((mx_fc1_kernel<false>), grid1, dim3(64 * p1.waves), std::max(acts1, (size_t)p1.waves * 4096), s, p1);
   }
   if (mode == HB_MOE_PAIRS_BF16) {
-    HB_LAUNCH((mx_fc2_kernel<__bf16>), grid2, dim3(64 * p2.waves), (size_t)p2.waves * 4 * 1024, s, p2);
+    HB_LAUNCH((mx_fc2_kernel<__bf16, 2>), grid2, dim3(64 * p2.waves), std::max(acts2, (size_t)p2.waves * 2 * 4096), s, p2);
   } else {
-    HB_LAUNCH((mx_fc2_kernel<float>), grid2, dim3(64 * p2.waves), (size_t)p2.waves * 4 * 1024, s, p2);
+    HB_LAUNCH((mx_fc2_kernel<float, 2>), grid2, dim3(64 * p2.waves), std::max(acts2, (size_t)p2.waves * 2 * 4096), s, p2);
   }
   if (sum) {
     CombineParams c{};

@@ -20,7 +20,7 @@ def test_the_library_refuses_before_a_launch():
     assert lib.hb_silu_mul_quant_mxfp4(256, 0, 1, 64, 0, None, 256, None) == _lib.HB_ENULL
     for half, pairs in [(48, 0), (64, 12), (64, -8), (96, 64), (0, 0)]:
         assert lib.hb_silu_mul_quant_mxfp4(256, 0, 1, half, pairs, 256, 256, None) == _lib.HB_EINVAL
-    assert lib.hb_mxfp4_tiled_bytes(16, 128) == 1024 + 256 and lib.hb_mxfp4_tiled_bytes(17, 544) == 2 * 5 * 1024 + 2 * 2 * 256
+    assert lib.hb_mxfp4_tiled_bytes(32, 64) == 1024 + 512 and lib.hb_mxfp4_tiled_bytes(33, 544) == 2 * 9 * 1024 + 2 * 4 * 256
     assert lib.hb_mxfp4_tiled_bytes(0, 128) == 0 and lib.hb_mxfp4_tiled_bytes(16, 48) == 0 and lib.hb_mxfp4_tiled_bytes(1 << 31, 32) == 0
     assert lib.hb_mxfp4_repack(256, 256, 1, 96, 128, 1, 256, None) == _lib.HB_EINVAL  # gated rows go in units of 64
     assert lib.hb_mxfp4_repack(256, 256, 65536, 64, 128, 0, 256, None) == _lib.HB_EINVAL
