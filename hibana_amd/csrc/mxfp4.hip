@@ -1,7 +1,6 @@
 // The microscaled four-bit format: rounding to it (alone, and behind a gated activation), the values back, the weights' tile
 // layout, and the linear.
 #include <algorithm>
-#include <type_traits>
 
 #include "mxfp4.hpp"
 #include "stream_common.hpp"
@@ -257,15 +256,6 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t mx_rows(const uint8_t* base, i
   const uint64_t at = reinterpret_cast<uint64_t>(base);
   const uint64_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)at), hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(at >> 32));
   return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(hi << 32 | lo), 0, __builtin_amdgcn_readfirstlane(bytes), 0x00020000);
-}
-
-// f(0), f(1) .. f(N - 1), each with its number as a constant.
-template <int N, int I = 0, class F>
-__device__ __forceinline__ void mx_unrolled(F&& f) {
-  if constexpr (I < N) {
-    f(std::integral_constant<int, I>());
-    mx_unrolled<N, I + 1>(f);
-  }
 }
 
 // 32 rows x NT tiles of a wavefront's sums, stored. A lane holds four columns of one row, 8 or 16 bytes: stored as they are, an instruction

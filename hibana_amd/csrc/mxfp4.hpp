@@ -9,6 +9,8 @@
 // its scales down to 2^-127 were checked over every BF16 and FP16 value).
 #pragma once
 
+#include <type_traits>
+
 #include "common.hpp"
 
 namespace hb {
@@ -36,6 +38,15 @@ struct MxLayout {
   __host__ __device__ int64_t codes() const { return (int64_t)tiles * chunks * 1024; }
   __host__ __device__ int64_t bytes() const { return codes() + (int64_t)tiles * quads * 256; }
 };
+
+// f(0), f(1) .. f(N - 1), each with its number as a constant.
+template <int N, int I = 0, class F>
+__device__ __forceinline__ void mx_unrolled(F&& f) {
+  if constexpr (I < N) {
+    f(std::integral_constant<int, I>());
+    mx_unrolled<N, I + 1>(f);
+  }
+}
 
 // ------------------------------------------------------------------------------------------------ rounding
 __device__ __forceinline__ uint32_t mx_scale_byte(uint32_t amax_bits) {  // the FP32 bits of the group's largest magnitude
