@@ -251,13 +251,6 @@ __device__ __forceinline__ void mx_mfma_in_place(f32x16_t& acc, i32x4_t a, i32x4
 }
 __device__ __forceinline__ void mx_sums_done() { asm volatile("s_nop 15\n\ts_nop 15" ::: "memory"); }
 
-// A buffer descriptor in scalar registers: what is read past `bytes` is zero.
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t mx_rows(const uint8_t* base, int bytes) {
-  const uint64_t at = reinterpret_cast<uint64_t>(base);
-  const uint64_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)at), hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(at >> 32));
-  return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(hi << 32 | lo), 0, __builtin_amdgcn_readfirstlane(bytes), 0x00020000);
-}
-
 // 32 rows x NT tiles of a wavefront's sums, stored. A lane holds four columns of one row, 8 or 16 bytes: stored as they are, an instruction
 // would touch 32 rows' lines. They go through the wavefront's own part of LDS and leave as whole rows of NT x 32 columns, 16 bytes a
 // lane; a row's 16-byte pieces are XORed with its number so that neither way meets a bank twice. (Where rows do not start on 16 bytes: as

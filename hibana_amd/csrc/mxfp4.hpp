@@ -39,6 +39,13 @@ struct MxLayout {
   __host__ __device__ int64_t bytes() const { return codes() + (int64_t)tiles * quads * 256; }
 };
 
+// A buffer descriptor in scalar registers: what is read past `bytes` is zero.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t mx_rows(const uint8_t* base, uint32_t bytes) {
+  const uint64_t at = reinterpret_cast<uint64_t>(base);
+  const uint64_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)at), hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(at >> 32));
+  return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(hi << 32 | lo), 0, __builtin_amdgcn_readfirstlane((int)bytes), 0x00020000);
+}
+
 // f(0), f(1) .. f(N - 1), each with its number as a constant.
 template <int N, int I = 0, class F>
 __device__ __forceinline__ void mx_unrolled(F&& f) {

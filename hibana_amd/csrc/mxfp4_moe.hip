@@ -5,6 +5,7 @@
 #include <algorithm>
 
 #include "mxfp4.hpp"
+#include "plan.hpp"
 #include "stream_common.hpp"
 
 namespace hb {
@@ -12,6 +13,11 @@ namespace hb {
 constexpr int MX_SCAN_PAIRS = 512;  // up to this many pairs a workgroup finds its slot from the ids themselves
 constexpr int MX_MOE_WAVES = 4;     // wavefronts a workgroup: small ones, so that several on a compute unit cover each other's starts and ends
 constexpr int MX_MOE_TILES = 2;     // weight tiles a workgroup (wavefronts that share K) or a wavefront (that have their own)
+
+// Rows' scales lie as the instruction takes them: a word a (quad of chunks, half), so a lane's scales of four chunks are one load.
+constexpr int MX_STEP = 8;
+__host__ __device__ constexpr int64_t mx_scale_row(int k) { return (k + 255) / 256 * 8; }
+__device__ __forceinline__ int mx_scale_at(int group) { return (group >> 3) * 8 + (group & 1) * 4 + ((group >> 1) & 3); }
 
 struct MxMoe {
   const uint8_t* w;        // the experts' stacked tile layouts
@@ -24,6 +30,7 @@ struct MxMoe {
   const int32_t* plan;     // many
   const int32_t* order;
   int base, experts, n, k, topk, pairs, inter;
+  int span;                // many: units (of two tiles) a workgroup, or a wavefront
   uint8_t* hq;             // fc1: h by pair (few) or in sorted order (many)
   uint8_t* hs;
   void* y;                 // fc2: [pairs, n], or the rows' sums
@@ -80,20 +87,28 @@ __device__ __forceinline__ void mx_emit_h(const MxMoe& p, const f32x4_t& up, con
   c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, h[2], h[3], s, 1);
   if (real && column < p.inter / 32) {
     *reinterpret_cast<uint16_t*>(p.hq + pos * (p.inter / 2) + 16 * column + 4 * q + 2 * g) = byte == 255u ? 0 : (uint16_t)c;
-    if (q == 0 && g == 0) p.hs[pos * (p.inter / 32) + column] = (uint8_t)byte;
+    if (q == 0 && g == 0) {
+      if (p.plan) {
+        uint8_t* at = p.hs + pos * mx_scale_row(p.inter);
+        at[mx_scale_at(column)] = (uint8_t)byte;
+        if (column == p.inter / 32 - 1 && !(column & 1)) at[mx_scale_at(column + 1)] = 0;
+      } else {
+        p.hs[pos * (p.inter / 32) + column] = (uint8_t)byte;
+      }
+    }
   }
 }
 
 // The two tiles of a workgroup as h: gated, an up and a gate tile are 32 columns; else each tile is 32. `part`: [waves][2 * 4][64], read by
 // all behind a barrier that has passed.
 template <bool GATED>
-__device__ __forceinline__ void mx_finish_h(const MxMoe& p, f32x4_t* part, uint32_t* tops, bool real, int64_t pos) {
+__device__ __forceinline__ void mx_finish_h(const MxMoe& p, f32x4_t* part, uint32_t* tops, int unit, bool real, int64_t pos) {
   const f32x4_t first = mx_joined<2>(part, MX_MOE_WAVES, threadIdx.x), second = mx_joined<2>(part, MX_MOE_WAVES, 256 + threadIdx.x);
   if (GATED) {
-    mx_emit_h<true>(p, first, second, blockIdx.x, real, pos, tops);
+    mx_emit_h<true>(p, first, second, unit, real, pos, tops);
   } else {
-    mx_emit_h<false>(p, first, first, 2 * blockIdx.x, real, pos, tops);
-    mx_emit_h<false>(p, second, second, 2 * blockIdx.x + 1, real, pos, tops + 256);
+    mx_emit_h<false>(p, first, first, 2 * unit, real, pos, tops);
+    mx_emit_h<false>(p, second, second, 2 * unit + 1, real, pos, tops + 256);
   }
 }
 
@@ -123,7 +138,7 @@ __global__ __launch_bounds__(64 * MX_MOE_WAVES, RUN == 4 ? 3 : 4) void mx_fc1_fe
   s.run(acts);
   mx_hand_over<MX_MOE_TILES>(part, s.acc);
   const int r = threadIdx.x & 31;
-  mx_finish_h<GATED>(p, part, tops, r < rows, r < rows ? list[r] : 0);
+  mx_finish_h<GATED>(p, part, tops, blockIdx.x, r < rows, r < rows ? list[r] : 0);
 }
 
 // fc2 of the same slots, its results by pair.
@@ -163,6 +178,8 @@ __global__ __launch_bounds__(64 * MX_MOE_WAVES, RUN == 4 ? 3 : 4) void mx_fc2_fe
 // results added in wavefront order. Reads a row's experts whether or not other rows name them too.
 constexpr int MX_ROW_WAVES = 8;
 constexpr int MX_SINGLE_ROWS = 1;
+constexpr int MX_MANY_GROUPS = 1536;
+constexpr int MX_PLAN_PAIRS = 1024;  // from here the plan's launches share the pairs
 __global__ __launch_bounds__(64 * MX_ROW_WAVES, 2) void mx_fc2_row_kernel(MxMoe p) {
   __shared__ f32x4_t part[MX_ROW_WAVES * 4 * 8];
   const MxLayout at(p.n, p.k);
@@ -217,129 +234,213 @@ __global__ __launch_bounds__(64 * MX_ROW_WAVES, 2) void mx_fc2_row_kernel(MxMoe 
 }
 
 // ------------------------------------------------------------------------------------------------ many pairs
-// A slot of the plan (up to 32 MT rows of an expert) and its wavefronts' operands from memory: the activations' codes of a chunk are 32 bytes a
-// row, read where they lie. RUN chunks are asked for, then multiplied: the other wavefronts of the compute unit cover the wait.
-template <int MT>
-struct MxRows {
-  const uint8_t *codes[MT], *scales[MT];
-  int groups;
-  template <class Row>
-  __device__ __forceinline__ MxRows(const MxMoe& p, int rows, Row&& row_of) : groups(p.k / MX_GROUP) {
-#pragma unroll
-    for (int i = 0; i < MT; i++) {
-      const int64_t row = row_of(min(32 * i + (int)(threadIdx.x & 31), rows - 1));  // (past the last: that one again, not to be stored)
-      codes[i] = p.aq + row * (p.k / 2);
-      scales[i] = p.as + row * groups;
-    }
-  }
+// A wavefront's walk over steps of eight chunks of two weight tiles, for a slot of the plan (up to 32 MT rows of an expert). A step's weights, 16 KB
+// a wavefront, are asked for as soon as the step before has taken its own out of the registers, so they are on their way while sums
+// are joined, rounded and stored; a slot's activations (32 bytes of a row's chunk, read where they lie) stay in registers where one
+// step covers the wavefront's K.
+// x [rows, k] rounded for the products of many pairs, eight values a lane: codes by rows, scales as above (a last odd group's partner at 0).
+struct MxRound {
+  const __bf16* x;
+  int64_t lanes;
+  int k;
+  uint8_t *codes, *scales;
 };
-template <int MT, int RUN>
-__device__ __forceinline__ void mx_gathered(const uint8_t* __restrict__ w, const MxLayout& at, int t0, int c0, int c1, const MxRows<MT>& rows, int tiles_of_rows,
-                                            f32x16_t (&acc)[MT][MX_MOE_TILES]) {
-  constexpr int NT = MX_MOE_TILES;
-  const int lane = threadIdx.x & 63, half = lane >> 5;
-  const uint8_t *codes[NT], *scales[NT];
-#pragma unroll
-  for (int t = 0; t < NT; t++) {
-    const int tile = min(t0 + t, at.tiles - 1);
-    codes[t] = w + (int64_t)tile * at.chunks * 1024 + lane * 16;
-    scales[t] = w + at.codes() + (int64_t)tile * at.quads * 256 + lane * 4;
+__device__ __forceinline__ void mx_round_lane(const MxRound& job, int64_t i) {
+  if (i >= job.lanes) return;  // whole groups leave together
+  Mx8<__bf16> v;
+  v.load(job.x + 8 * i);
+  const uint32_t byte = mx_scale_byte(quad_max(v.amax()));
+  reinterpret_cast<uint32_t*>(job.codes)[i] = byte == 255u ? 0u : v.codes(mx_scale_value(byte));
+  if ((i & 3) == 0) {
+    const int groups = job.k / MX_GROUP;
+    const int64_t row = (i >> 2) / groups;
+    const int group = (int)((i >> 2) - row * groups);
+    uint8_t* at = job.scales + row * mx_scale_row(job.k);
+    at[mx_scale_at(group)] = (uint8_t)byte;
+    if (group == groups - 1 && (groups & 1)) at[mx_scale_at(groups)] = 0;
   }
-#pragma unroll
-  for (int i = 0; i < MT; i++)
-#pragma unroll
-    for (int t = 0; t < NT; t++)
-#pragma unroll
-      for (int e = 0; e < 16; e++) acc[i][t][e] = 0.f;
-  for (int c = c0; c < c1; c += RUN) {
-    i32x4_t b[RUN][NT], a[RUN][MT];
-    uint32_t sb[NT], sa[RUN][MT];
-#pragma unroll
-    for (int t = 0; t < NT; t++) sb[t] = *reinterpret_cast<const uint32_t*>(scales[t] + (c >> 2) * 256);
-#pragma unroll
-    for (int u = 0; u < RUN; u++) {
-      const int in = min(c + u, c1 - 1), group = min(2 * in + half, rows.groups - 1);
-#pragma unroll
-      for (int t = 0; t < NT; t++) b[u][t] = *reinterpret_cast<const i32x4_t*>(codes[t] + in * 1024);
-#pragma unroll
-      for (int i = 0; i < MT; i++) {
-        a[u][i] = *reinterpret_cast<const i32x4_t*>(rows.codes[i] + 16 * group);
-        sa[u][i] = rows.scales[i][group];
-      }
-    }
-#pragma unroll
-    for (int t = 0; t < NT; t++) sb[t] >>= 8 * (c & 3);
-    mx_unrolled<RUN>([&](auto u) {
-      if (c + u.value < c1) {
-#pragma unroll
-        for (int i = 0; i < MT; i++)
-          if (i < tiles_of_rows) {
-#pragma unroll
-            for (int t = 0; t < NT; t++) acc[i][t] = mx_mfma<u.value, 0>(b[u.value][t], sb[t], a[u.value][i], sa[u.value][i], acc[i][t]);
-          }
-      }
-    });
+}
+__global__ __launch_bounds__(256) void mx_quantize_rows_kernel(MxRound job) { mx_round_lane(job, (int64_t)blockIdx.x * 256 + threadIdx.x); }
+// The plan of a call of fewer pairs than its own launches share among workgroups, by the first workgroup, and the rounding beside it.
+__global__ __launch_bounds__(PLAN_THREADS) void mx_plan_round_kernel(const int32_t* ids, int pairs, int e_lo, int e_n, int32_t* __restrict__ plan, int32_t* __restrict__ order,
+                                                                     int slot_rows, int slot_cap, MxRound job) {
+  extern __shared__ int plan_lds[];
+  if (blockIdx.x == 0) {
+    plan_work<false>(ids, pairs, e_lo, e_n, 0, plan, order, slot_rows, slot_cap, nullptr, 1, 0, 0, plan_lds);
+  } else {
+    mx_round_lane(job, (int64_t)(blockIdx.x - 1) * PLAN_THREADS + threadIdx.x);
   }
 }
 
-// fc1: two weight tiles a workgroup, K split among its wavefronts.
+template <int MT>
+struct MxWalk {
+  static constexpr int NT = MX_MOE_TILES;
+  __amdgpu_buffer_rsrc_t w, ac, as;
+  uint32_t code_at[MT], scale_at[MT];  // the lane's rows of activations, from the slot's first
+  const MxLayout& at;
+  int c0, c1;  // chunks of this wavefront's share of K: c0 a multiple of four
+  i32x4_t b[MX_STEP][NT], a[MX_STEP][MT];
+  uint32_t sb[MX_STEP / 4][NT], sa[MX_STEP / 4][MT];
+  f32x16_t acc[MT][NT];
+  // rows_of_x: how many rows the activations have (their descriptors end behind them)
+  template <class Row>
+  __device__ __forceinline__ MxWalk(const MxMoe& p, const MxLayout& at, const uint8_t* matrix, int rows, uint32_t rows_of_x, int share, int shares, Row&& row_of)
+      : w(mx_rows(matrix, (uint32_t)at.bytes())), ac(mx_rows(p.aq, rows_of_x * (uint32_t)(p.k / 2))), as(mx_rows(p.as, rows_of_x * (uint32_t)mx_scale_row(p.k))), at(at) {
+    const int quads = (at.chunks + 3) / 4, half = (threadIdx.x & 63) >> 5;
+    c0 = 4 * (quads * share / shares);
+    c1 = min(at.chunks, 4 * (quads * (share + 1) / shares));
+#pragma unroll
+    for (int i = 0; i < MT; i++) {
+      const uint32_t row = row_of(min(32 * i + (int)(threadIdx.x & 31), rows - 1));  // (past the last: that one again, not to be stored)
+      code_at[i] = row * (uint32_t)(p.k / 2) + 16 * half;
+      scale_at[i] = row * (uint32_t)mx_scale_row(p.k) + 4 * half;
+    }
+  }
+  __device__ __forceinline__ int steps() const { return max(1, (c1 - c0 + MX_STEP - 1) / MX_STEP); }
+  // (chunks past the share's end are asked for where they are in the matrix, and not multiplied)
+  __device__ __forceinline__ void ask_weights(int t0, int c) {
+    const uint32_t lane = threadIdx.x & 63;
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+      const int tile = min(t0 + t, at.tiles - 1), of = tile * at.chunks * 1024, s = (int)at.codes() + (tile * at.quads + (c >> 2)) * 256;
+#pragma unroll
+      for (int u = 0; u < MX_STEP; u++) b[u][t] = __builtin_bit_cast(i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(w, lane * 16, of + min(c + u, at.chunks - 1) * 1024, 2));
+#pragma unroll
+      for (int u = 0; u < MX_STEP / 4; u++) sb[u][t] = __builtin_amdgcn_raw_buffer_load_b32(w, lane * 4, s + u * 256, 0);
+    }
+  }
+  __device__ __forceinline__ void ask_acts(int c) {
+#pragma unroll
+    for (int i = 0; i < MT; i++) {
+#pragma unroll
+      for (int u = 0; u < MX_STEP; u++) a[u][i] = __builtin_bit_cast(i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(ac, code_at[i], min(c + u, at.chunks - 1) * 32, 0));
+#pragma unroll
+      for (int u = 0; u < MX_STEP / 4; u++) sa[u][i] = __builtin_amdgcn_raw_buffer_load_b32(as, scale_at[i], ((c >> 2) + u) * 8, 0);
+    }
+  }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < MT; i++)
+#pragma unroll
+      for (int t = 0; t < NT; t++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) acc[i][t][e] = 0.f;
+  }
+  __device__ __forceinline__ void multiply(int c) {
+    mx_unrolled<MX_STEP>([&](auto u) {
+      if (c + u.value < c1) {
+#pragma unroll
+        for (int i = 0; i < MT; i++)
+#pragma unroll
+          for (int t = 0; t < NT; t++)
+            acc[i][t] = mx_mfma<u.value % 4, u.value % 4>(b[u.value][t], sb[u.value / 4][t], a[u.value][i], sa[u.value / 4][i], acc[i][t]);
+      }
+    });
+    __builtin_amdgcn_sched_barrier(0);  // the registers of b are free: what follows asks into them
+  }
+};
+
+// The plan's slot of this workgroup and its span of units (two tiles each): p.span of them, from p.span blockIdx.x.
+// fc1: K split among the wavefronts.
 template <bool GATED, int MT>
-__global__ __launch_bounds__(64 * MX_MOE_WAVES, MT == 1 ? 4 : 3) void mx_fc1_many_kernel(MxMoe p) {
+__global__ __launch_bounds__(64 * MX_MOE_WAVES, MT == 1 ? 3 : 2) void mx_fc1_many_kernel(MxMoe p) {
   __shared__ f32x4_t part[MX_MOE_WAVES * MX_MOE_TILES * 256];
   __shared__ uint32_t tops[GATED ? 256 : 512];
   const int32_t* entry = p.plan + PLAN_HEADER + 4 * (int)blockIdx.y;
   const int rows = entry[2], p0 = entry[1];
   if (rows == 0) return;
-  constexpr int RUN = 2;
   const MxLayout at(p.n, p.k);
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), runs = (at.chunks + RUN - 1) / RUN;
-  const MxRows<MT> from(p, rows, [&](int r) { return (int64_t)(p.order[p0 + r] / p.topk); });
-  f32x16_t acc[MT][MX_MOE_TILES];
-  mx_gathered<MT, RUN>(p.w + entry[0] * p.expert_bytes, at, blockIdx.x * MX_MOE_TILES, RUN * (runs * wave / MX_MOE_WAVES),
-                       min(at.chunks, RUN * (runs * (wave + 1) / MX_MOE_WAVES)), from, (rows + 31) / 32, acc);
+  const int units = (at.tiles + MX_MOE_TILES - 1) / MX_MOE_TILES, first = blockIdx.x * p.span, last = min(first + p.span, units);
+  MxWalk<MT> walk(p, at, p.w + entry[0] * p.expert_bytes, rows, (uint32_t)(p.pairs / p.topk), __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), MX_MOE_WAVES, [&](int r) { return (uint32_t)(p.order[p0 + r] / p.topk); });
+  const int steps = walk.steps();
+  walk.ask_weights(first * MX_MOE_TILES, walk.c0);
+  walk.ask_acts(walk.c0);
+  for (int unit = first; unit < last; unit++) {
+    walk.clear();
+    for (int s = 0; s < steps; s++) {
+      const int c = walk.c0 + s * MX_STEP;
+      walk.multiply(c);
+      if (s + 1 < steps) {
+        walk.ask_weights(unit * MX_MOE_TILES, c + MX_STEP);
+        walk.ask_acts(c + MX_STEP);
+      } else if (unit + 1 < last) {
+        walk.ask_weights((unit + 1) * MX_MOE_TILES, walk.c0);
+        if (steps > 1) walk.ask_acts(walk.c0);
+      }
+    }
 #pragma unroll
-  for (int i = 0; i < MT; i++) {
-    if (32 * i >= rows) break;
-    mx_hand_over<MX_MOE_TILES>(part, acc[i]);
-    const int r = 32 * i + (threadIdx.x & 31);
-    mx_finish_h<GATED>(p, part, tops, r < rows, p0 + r);
+    for (int i = 0; i < MT; i++) {
+      if (32 * i >= rows) break;
+      mx_hand_over<MX_MOE_TILES>(part, walk.acc[i]);
+      const int r = 32 * i + (threadIdx.x & 31);
+      mx_finish_h<GATED>(p, part, tops, unit, r < rows, p0 + r);
+    }
   }
 }
 
-// fc2: each wavefront two tiles of its own, all of K; a row's 64 results leave together (as mx_store_rows does it, the rows found through `order`).
-template <typename Y, int MT>
-__global__ __launch_bounds__(64 * MX_MOE_WAVES, MT == 1 ? 4 : 3) void mx_fc2_many_kernel(MxMoe p) {
+// fc2. SHARED: K split among the wavefronts as in fc1; else (short K) each wavefront has units of its own.
+template <typename Y, int MT, bool SHARED>
+__global__ __launch_bounds__(64 * MX_MOE_WAVES, MT == 1 ? 3 : 2) void mx_fc2_many_kernel(MxMoe p) {
   constexpr int NT = MX_MOE_TILES, PIECES = NT * MX_ROWS * (int)sizeof(Y) / 16, ROWS = 64 / PIECES;
-  __shared__ i32x4_t places[MX_MOE_WAVES][MX_ROWS * PIECES];
+  __shared__ f32x4_t part[SHARED ? MX_MOE_WAVES * NT * 256 : MX_MOE_WAVES * MX_ROWS * PIECES];
   const int32_t* entry = p.plan + PLAN_HEADER + 4 * (int)blockIdx.y;
   const int rows = entry[2], p0 = entry[1];
   if (rows == 0) return;
   const MxLayout at(p.n, p.k);
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), t0 = (blockIdx.x * MX_MOE_WAVES + wave) * NT;
-  if (t0 >= at.tiles) return;
-  const MxRows<MT> from(p, rows, [&](int r) { return (int64_t)p0 + r; });
-  f32x16_t acc[MT][NT];
-  mx_gathered<MT, 2>(p.w + entry[0] * p.expert_bytes, at, t0, 0, at.chunks, from, (rows + 31) / 32, acc);
-  i32x4_t* place = places[wave];
-  uint8_t* bytes = reinterpret_cast<uint8_t*>(place);
-  const int r = lane & 31, g = lane >> 5;
-#pragma unroll
-  for (int i = 0; i < MT; i++) {
-    if (32 * i >= rows) break;
-#pragma unroll
-    for (int j = 0; j < NT; j++)
-#pragma unroll
-      for (int q = 0; q < 4; q++) {
-        const int in = (MX_ROWS * j + 8 * q + 4 * g) * (int)sizeof(Y), piece = (in / 16) ^ (r & (PIECES - 1));
-        const f32x4_t v = mx_quarter(acc[i][j], q);
-        typedef __attribute__((ext_vector_type(4))) Y y4_t;
-        *reinterpret_cast<y4_t*>(bytes + (r * PIECES + piece) * 16 + in % 16) = y4_t{(Y)v[0], (Y)v[1], (Y)v[2], (Y)v[3]};
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 31, g = lane >> 5;
+  const int units = (at.tiles + NT - 1) / NT, by = SHARED ? 1 : MX_MOE_WAVES;
+  const int first = blockIdx.x * p.span * by + (SHARED ? 0 : wave), last = min((int)(blockIdx.x + 1) * p.span * by, units);
+  if (first >= last) return;
+  MxWalk<MT> walk(p, at, p.w + entry[0] * p.expert_bytes, rows, (uint32_t)p.pairs, SHARED ? wave : 0, SHARED ? MX_MOE_WAVES : 1, [&](int i) { return (uint32_t)(p0 + i); });
+  const int steps = walk.steps();
+  walk.ask_weights(first * NT, walk.c0);
+  walk.ask_acts(walk.c0);
+  typedef __attribute__((ext_vector_type(4))) Y y4_t;
+  for (int unit = first; unit < last; unit += by) {
+    walk.clear();
+    for (int s = 0; s < steps; s++) {
+      const int c = walk.c0 + s * MX_STEP;
+      walk.multiply(c);
+      if (s + 1 < steps) {
+        walk.ask_weights(unit * NT, c + MX_STEP);
+        walk.ask_acts(c + MX_STEP);
+      } else if (unit + by < last) {
+        walk.ask_weights((unit + by) * NT, walk.c0);
+        if (steps > 1) walk.ask_acts(walk.c0);
       }
+    }
 #pragma unroll
-    for (int first = 0; first < MX_ROWS; first += ROWS) {
-      const int row = first + lane / PIECES, piece = lane % PIECES, n = t0 * MX_ROWS + piece * (16 / (int)sizeof(Y));
-      const i32x4_t v = place[row * PIECES + (piece ^ (row & (PIECES - 1)))];
-      if (32 * i + row < rows && n < p.n) *reinterpret_cast<i32x4_t*>(static_cast<Y*>(p.y) + (int64_t)p.order[p0 + 32 * i + row] * p.n + n) = v;
+    for (int i = 0; i < MT; i++) {
+      if (32 * i >= rows) break;
+      if constexpr (SHARED) {
+        mx_hand_over<NT>(part, walk.acc[i]);
+        if (32 * i + r < rows) {
+          const int64_t pair = p.order[p0 + 32 * i + r];
+#pragma unroll
+          for (int t = 0; t < NT; t++) {
+            const f32x4_t v = mx_joined<NT>(part, MX_MOE_WAVES, 256 * t + threadIdx.x);
+            const int n = (unit * NT + t) * MX_ROWS + 8 * (threadIdx.x >> 6) + 4 * g;
+            if (n < p.n) *reinterpret_cast<y4_t*>(static_cast<Y*>(p.y) + pair * p.n + n) = y4_t{(Y)v[0], (Y)v[1], (Y)v[2], (Y)v[3]};
+          }
+        }
+      } else {  // a row's 64 results leave together, through the wavefront's own part of LDS (as mx_store_rows does it)
+        i32x4_t* place = reinterpret_cast<i32x4_t*>(part) + wave * MX_ROWS * PIECES;
+        uint8_t* bytes = reinterpret_cast<uint8_t*>(place);
+#pragma unroll
+        for (int j = 0; j < NT; j++)
+#pragma unroll
+          for (int q = 0; q < 4; q++) {
+            const int in = (MX_ROWS * j + 8 * q + 4 * g) * (int)sizeof(Y), piece = (in / 16) ^ (r & (PIECES - 1));
+            const f32x4_t v = mx_quarter(walk.acc[i][j], q);
+            *reinterpret_cast<y4_t*>(bytes + (r * PIECES + piece) * 16 + in % 16) = y4_t{(Y)v[0], (Y)v[1], (Y)v[2], (Y)v[3]};
+          }
+#pragma unroll
+        for (int from = 0; from < MX_ROWS; from += ROWS) {
+          const int row = from + lane / PIECES, piece = lane % PIECES, n = unit * NT * MX_ROWS + piece * (16 / (int)sizeof(Y));
+          const i32x4_t v = place[row * PIECES + (piece ^ (row & (PIECES - 1)))];
+          if (32 * i + row < rows && n < p.n) *reinterpret_cast<i32x4_t*>(static_cast<Y*>(p.y) + (int64_t)p.order[p0 + 32 * i + row] * p.n + n) = v;
+        }
+      }
     }
   }
 }
@@ -352,7 +453,7 @@ struct MxWorkspace {
   size_t bytes;
 };
 
-bool few_pairs(int64_t pairs, int hidden, int inter) { return pairs <= MX_SCAN_PAIRS && MxActs::bytes(std::min<int64_t>(pairs, MX_ROWS), std::max(hidden, inter)) <= 48 * 1024; }
+bool few_pairs(int64_t pairs, int hidden, int inter) { return pairs <= 64 && MxActs::bytes(std::min<int64_t>(pairs, MX_ROWS), std::max(hidden, inter)) <= 48 * 1024; }
 
 MxWorkspace carve(const hb_mxfp4_experts* ex, void* base, int64_t m, int topk, bool sum) {
   const int64_t pairs = m * topk;
@@ -368,10 +469,10 @@ MxWorkspace carve(const hb_mxfp4_experts* ex, void* base, int64_t m, int topk, b
     w.plan.plan_wide = reinterpret_cast<int32_t*>(take((size_t)64 * ex->experts * sizeof(int32_t)));
     w.plan.order = reinterpret_cast<int32_t*>(take((size_t)pairs * sizeof(int32_t)));
     w.xq = take((size_t)m * (ex->hidden / 2));
-    w.xs = take((size_t)m * (ex->hidden / 32));
+    w.xs = take((size_t)m * mx_scale_row(ex->hidden));
   }
   w.hq = take((size_t)pairs * (ex->inter / 2));
-  w.hs = take((size_t)pairs * (ex->inter / 32));
+  w.hs = take((size_t)pairs * mx_scale_row(ex->inter));
   w.y = sum ? take((size_t)pairs * ex->hidden_out * sizeof(float)) : nullptr;
   w.bytes = off;
   return w;
@@ -407,6 +508,7 @@ extern "C" int hb_mxfp4_moe(const hb_mxfp4_experts* experts, const void* x, cons
   const MxWorkspace ws = carve(experts, workspace, m, topk, sum);
   if (workspace_bytes < ws.bytes) return HB_EWORKSPACE;
   const int64_t pairs = (int64_t)m * topk;
+  if (pairs * (experts->inter / 2) >= (int64_t)1 << 32 || (int64_t)m * (experts->hidden / 2) >= (int64_t)1 << 32) return HB_EINVAL;  // the descriptors' reach
   hipStream_t s = as_stream(stream);
   const MxLayout l1(fc1_rows(experts), experts->hidden), l2(experts->hidden_out, experts->inter);
   MxMoe p1{}, p2{};
@@ -463,23 +565,48 @@ extern "C" int hb_mxfp4_moe(const hb_mxfp4_experts* experts, const void* x, cons
     const int slot_rows = tall ? 2 * MX_ROWS : MX_ROWS;
     const int64_t slots = moe_max_slots(pairs, experts->experts, 0, slot_rows);
     if (slots > 65535) return HB_EINVAL;
-    if (int e = moe_launch_plan(ids, pairs, experts->base, experts->experts, 0, ws.plan, s, slot_rows)) return e;
-    if (int e = hb_mxfp4_quantize(x, HB_BF16, m, experts->hidden, ws.xq, ws.xs, stream)) return e;
+    const MxRound job{static_cast<const __bf16*>(x), (int64_t)m * (experts->hidden / 8), experts->hidden, ws.xq, ws.xs};
+    const size_t plan_lds = ((size_t)(PLAN_WAVES + 1) * experts->experts + 3 * (PLAN_WAVES + 1)) * sizeof(int);
+    if (plan_lds > 64 * 1024 || experts->experts > PLAN_THREADS) return HB_EINVAL;
+    if (pairs < MX_PLAN_PAIRS) {
+      HB_LAUNCH(mx_plan_round_kernel, dim3(1 + (unsigned)((job.lanes + PLAN_THREADS - 1) / PLAN_THREADS)), dim3(PLAN_THREADS), plan_lds, s, ids, (int)pairs, experts->base,
+                experts->experts, ws.plan.plan, ws.plan.order, slot_rows, (int)slots, job);
+    } else {
+      if (int e = moe_launch_plan(ids, pairs, experts->base, experts->experts, 0, ws.plan, s, slot_rows)) return e;
+      HB_LAUNCH(mx_quantize_rows_kernel, dim3((unsigned)((job.lanes + 255) / 256)), dim3(256), 0, s, job);
+    }
     p1.plan = p2.plan = ws.plan.plan;
     p1.order = p2.order = ws.plan.order;
     p1.aq = ws.xq;
     p1.as = ws.xs;
-    auto launch = [&](auto kernel, unsigned groups, const MxMoe& p) { HB_LAUNCH(kernel, dim3(groups, (unsigned)slots), dim3(64 * MX_MOE_WAVES), 0, s, p); };
-    const unsigned own2 = (unsigned)((l2.tiles + MX_MOE_TILES * MX_MOE_WAVES - 1) / (MX_MOE_TILES * MX_MOE_WAVES));
+    // about six workgroups a compute unit where there are so many: each then has several units, whose weights it asks for ahead
+    const int64_t busy = std::min<int64_t>(slots, pairs / slot_rows + std::min<int64_t>(pairs, experts->experts) / 2 + 1);
+    auto span_of = [&](int64_t units, int64_t by) {
+      const int64_t spans = std::max<int64_t>(1, std::min<int64_t>((units + by - 1) / by, (MX_MANY_GROUPS + busy - 1) / busy));
+      return (int)(((units + by - 1) / by + spans - 1) / spans);
+    };
+    auto launch = [&](auto kernel, unsigned units, unsigned by, MxMoe& p) {
+      p.span = span_of(units, by);
+      HB_LAUNCH(kernel, dim3((units + by * p.span - 1) / (by * p.span), (unsigned)slots), dim3(64 * MX_MOE_WAVES), 0, s, p);
+    };
     if (experts->gated) {
-      launch(tall ? mx_fc1_many_kernel<true, 2> : mx_fc1_many_kernel<true, 1>, groups1, p1);
+      launch(tall ? mx_fc1_many_kernel<true, 2> : mx_fc1_many_kernel<true, 1>, groups1, 1, p1);
     } else {
-      launch(tall ? mx_fc1_many_kernel<false, 2> : mx_fc1_many_kernel<false, 1>, groups1, p1);
+      launch(tall ? mx_fc1_many_kernel<false, 2> : mx_fc1_many_kernel<false, 1>, groups1, 1, p1);
     }
+    const bool own = l2.chunks <= 2 * MX_STEP;
+    auto fc2 = [&](auto* type) {
+      using Y = std::remove_pointer_t<decltype(type)>;
+      if (own) {
+        launch(tall ? mx_fc2_many_kernel<Y, 2, false> : mx_fc2_many_kernel<Y, 1, false>, groups2, MX_MOE_WAVES, p2);
+      } else {
+        launch(tall ? mx_fc2_many_kernel<Y, 2, true> : mx_fc2_many_kernel<Y, 1, true>, groups2, 1, p2);
+      }
+    };
     if (narrow) {
-      launch(tall ? mx_fc2_many_kernel<__bf16, 2> : mx_fc2_many_kernel<__bf16, 1>, own2, p2);
+      fc2((__bf16*)nullptr);
     } else {
-      launch(tall ? mx_fc2_many_kernel<float, 2> : mx_fc2_many_kernel<float, 1>, own2, p2);
+      fc2((float*)nullptr);
     }
   }
   if (sum) {
