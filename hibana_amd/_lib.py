@@ -185,10 +185,10 @@ def workspace_reset(ws: torch.Tensor | None) -> None:
 
 def need_one_gpu(*tensors: torch.Tensor) -> None:
     """`need_gpu`, and every tensor on the current device: a launch goes to that device's current stream."""
-    here = torch._C._cuda_getDevice() if any(t is not None and t.is_cuda for t in tensors) else -1
+    here = torch._C._cuda_getDevice() if tensors[0].is_cuda else -2
     for t in tensors:
-        if t is not None and t.get_device() != here:
-            need_gpu(t)
+        if t.get_device() != here:
+            need_gpu(*tensors)
             raise ValueError(f"hibana_amd kernels run on the current device, cuda:{here}: got a tensor on {t.device}")
 
 

@@ -10,7 +10,7 @@
 
 namespace hb {
 
-constexpr int MX_SCAN_PAIRS = 512;  // up to this many pairs a workgroup finds its slot from the ids themselves
+constexpr int MX_SCAN_PAIRS = 64;   // up to this many pairs every wavefront finds its workgroup's slot from the ids themselves
 constexpr int MX_MOE_WAVES = 4;     // wavefronts a workgroup: small ones, so that several on a compute unit cover each other's starts and ends
 constexpr int MX_MOE_TILES = 2;     // weight tiles a workgroup (wavefronts that share K) or a wavefront (that have their own)
 
@@ -36,38 +36,25 @@ struct MxMoe {
   void* y;                 // fc2: [pairs, n], or the rows' sums
 };
 
-// The slot of a call of few pairs that begins at pair `first`, found by every workgroup for itself: an expert's pairs in ascending order,
-// cut into slots of 32; `list` (LDS) receives the slot's pairs. 0 rows: another workgroup's. All of the workgroup's threads call it, past the
-// barrier behind which `masks` (LDS) is written.
-__device__ __forceinline__ void mx_scan(const MxMoe& p, int id, uint64_t* masks) {
-  for (int i = threadIdx.x; i < MX_SCAN_PAIRS; i += 64 * MX_MOE_WAVES) {
-    const uint64_t same = __ballot(i < p.pairs && p.ids[i < p.pairs ? i : 0] == id);
-    if ((threadIdx.x & 63) == 0) masks[i >> 6] = same;
-  }
-}
-__device__ __forceinline__ int mx_slot_of(const uint64_t* masks, int first, int* list) {
-  int before = 0, total = 0, mine[MX_SCAN_PAIRS / (64 * MX_MOE_WAVES)];
-#pragma unroll
-  for (int v = 0; v < MX_SCAN_PAIRS / 64; v++) {
-    const uint64_t m = masks[v];
-    if (v == first >> 6) before = total + __popcll(m & ((1ull << (first & 63)) - 1ull));
-#pragma unroll
-    for (int j = 0; j < MX_SCAN_PAIRS / (64 * MX_MOE_WAVES); j++)
-      if (v == j * MX_MOE_WAVES + (int)(threadIdx.x >> 6)) mine[j] = (m >> (threadIdx.x & 63)) & 1 ? total + __popcll(m & ((1ull << (threadIdx.x & 63)) - 1ull)) : -1;
-    total += __popcll(m);
-  }
+// The slot of a call of few pairs that begins at pair `first`, found by every wavefront for itself: an expert's pairs in ascending order, cut
+// into slots of 32; lane r of `list` holds the slot's pair r. 0 rows: another workgroup's.
+__device__ __forceinline__ int mx_slot_of(const MxMoe& p, int id, int first, int& list) {
+  const int lane = threadIdx.x & 63;
+  const uint64_t same = __ballot(lane < p.pairs && p.ids[min(lane, p.pairs - 1)] == id);
+  const int rank = __popcll(same & ((1ull << lane) - 1ull)), before = __popcll(same & ((1ull << first) - 1ull));
   if (before % MX_ROWS) return 0;
-#pragma unroll
-  for (int j = 0; j < MX_SCAN_PAIRS / (64 * MX_MOE_WAVES); j++)
-    if (mine[j] >= before && mine[j] < before + MX_ROWS) list[mine[j] - before] = j * 64 * MX_MOE_WAVES + threadIdx.x;
-  return min(MX_ROWS, total - before);
+  // a pair of the slot hands its number to the lane of its place; the others theirs to places that nobody reads
+  const bool mine = ((same >> lane) & 1) && rank >= before && rank < before + MX_ROWS;
+  list = __builtin_amdgcn_ds_permute(4 * (mine ? rank - before : 32 + (lane & 31)), lane);
+  return min(MX_ROWS, (int)__popcll(same) - before);
 }
 
 // h of 32 x 32 values (row r of the slot, columns from 32 `column`) from the joined sums of up (and gate), rounded to the format: 256 threads, thread
-// i = 64 q + lane holds row lane % 32, columns 8 q + 4 (lane / 32) .. + 3. `tops`: 256 words of LDS that nobody else uses up to the next barrier.
+// i = 64 q + lane (of every 256) holds row lane % 32, columns 8 q + 4 (lane / 32) .. + 3. `tops`: a word of LDS a thread that nobody else uses up to
+// the next barrier.
 template <bool GATED>
 __device__ __forceinline__ void mx_emit_h(const MxMoe& p, const f32x4_t& up, const f32x4_t& gate, int column, bool real, int64_t pos, uint32_t* tops) {
-  const int lane = threadIdx.x & 63, r = lane & 31, g = lane >> 5, q = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, r = lane & 31, g = lane >> 5, q = (threadIdx.x >> 6) & 3;
   float h[4];
   uint32_t top = 0;
 #pragma unroll
@@ -78,8 +65,9 @@ __device__ __forceinline__ void mx_emit_h(const MxMoe& p, const f32x4_t& up, con
   }
   tops[threadIdx.x] = top;
   __syncthreads();
+  const uint32_t* of = tops + (threadIdx.x & ~255);
 #pragma unroll
-  for (int v = 0; v < 4; v++) top = max(top, max(tops[v * 64 + r], tops[v * 64 + 32 + r]));
+  for (int v = 0; v < 4; v++) top = max(top, max(of[v * 64 + r], of[v * 64 + 32 + r]));
   const uint32_t byte = mx_scale_byte(top);
   const float s = mx_scale_value(byte);
   uint32_t c = 0;
@@ -115,69 +103,63 @@ __device__ __forceinline__ void mx_finish_h(const MxMoe& p, f32x4_t* part, uint3
 // ------------------------------------------------------------------------------------------------ few pairs
 // fc1: a workgroup two weight tiles of the slot that begins at pair blockIdx.y (none: it leaves). The slot's expert is known from one
 // id, so the weights are on their way while the slot's rows are looked for and their activations rounded into LDS.
-template <bool GATED, int RUN>
-__global__ __launch_bounds__(64 * MX_MOE_WAVES, RUN == 4 ? 3 : 4) void mx_fc1_few_kernel(MxMoe p) {
-  extern __shared__ f32x4_t part[];
-  __shared__ uint64_t masks[MX_SCAN_PAIRS / 64];
-  __shared__ int list[MX_ROWS];
-  __shared__ uint32_t tops[GATED ? 256 : 512];
+constexpr int MX_FEW_WAVES = 8;
+template <int RUN, class Values>
+__device__ __forceinline__ int mx_few_product(const MxMoe& p, f32x4_t* part, int& list, Values&& values) {
   const int first = blockIdx.y, id = p.ids[first], e = id - p.base;
-  if (e < 0 || e >= p.experts) return;
-  MxStream<MX_MOE_TILES, RUN> s(p.w + e * p.expert_bytes, MxLayout(p.n, p.k), blockIdx.x * MX_MOE_TILES, __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), MX_MOE_WAVES);
-  mx_scan(p, id, masks);
-  __syncthreads();
-  const int rows = mx_slot_of(masks, first, list);
-  if (rows == 0) return;
-  __syncthreads();
+  if (e < 0 || e >= p.experts) return 0;
+  MxStream<MX_MOE_TILES, RUN> s(p.w + e * p.expert_bytes, MxLayout(p.n, p.k), blockIdx.x * MX_MOE_TILES, __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), MX_FEW_WAVES);
+  const int rows = mx_slot_of(p, id, first, list);
+  if (rows == 0) return 0;
   const MxActs acts(part, rows, p.k);
-  for (int i = threadIdx.x; i < rows * acts.groups; i += 64 * MX_MOE_WAVES) {
-    const int r = i / acts.groups, group = i - r * acts.groups;
-    acts.put(r, group, static_cast<const __bf16*>(p.x) + (int64_t)(list[r] / p.topk) * p.k + MX_GROUP * group);
+  for (int i = threadIdx.x; i < (rows * acts.groups + 63) / 64 * 64; i += 64 * MX_FEW_WAVES) {  // whole wavefronts: `list` lies across the lanes
+    const int r = i / acts.groups, group = i - r * acts.groups, pair = __shfl(list, min(r, rows - 1));
+    if (r < rows) values(acts, r, group, pair);
   }
   __syncthreads();
   s.run(acts);
   mx_hand_over<MX_MOE_TILES>(part, s.acc);
-  const int r = threadIdx.x & 31;
-  mx_finish_h<GATED>(p, part, tops, blockIdx.x, r < rows, r < rows ? list[r] : 0);
+  return rows;
+}
+
+template <bool GATED, int RUN>
+__global__ __launch_bounds__(64 * MX_FEW_WAVES, RUN == 4 ? 2 : 4) void mx_fc1_few_kernel(MxMoe p) {
+  extern __shared__ f32x4_t part[];
+  int list;
+  const int rows = mx_few_product<RUN>(p, part, list, [&](const MxActs& acts, int r, int group, int pair) {
+    acts.put(r, group, static_cast<const __bf16*>(p.x) + (int64_t)(pair / p.topk) * p.k + MX_GROUP * group);
+  });
+  if (rows == 0) return;
+  const int r = threadIdx.x & 31, upper = threadIdx.x >> 8;  // the threads' upper half: the second tile where each is 32 columns
+  const f32x4_t up = mx_joined<MX_MOE_TILES>(part, MX_FEW_WAVES, GATED ? threadIdx.x & 255 : threadIdx.x);
+  const f32x4_t gate = GATED ? mx_joined<MX_MOE_TILES>(part, MX_FEW_WAVES, 256 + (threadIdx.x & 255)) : up;
+  const int pair = __shfl(list, r);
+  __syncthreads();  // the sums are read: their place takes the quarters' largest magnitudes
+  mx_emit_h<GATED>(p, up, gate, GATED ? blockIdx.x : 2 * blockIdx.x + upper, r < rows && (!GATED || !upper), pair, reinterpret_cast<uint32_t*>(part));
 }
 
 // fc2 of the same slots, its results by pair.
 template <typename Y, int RUN>
-__global__ __launch_bounds__(64 * MX_MOE_WAVES, RUN == 4 ? 3 : 4) void mx_fc2_few_kernel(MxMoe p) {
+__global__ __launch_bounds__(64 * MX_FEW_WAVES, RUN == 4 ? 2 : 4) void mx_fc2_few_kernel(MxMoe p) {
   extern __shared__ f32x4_t part[];
-  __shared__ uint64_t masks[MX_SCAN_PAIRS / 64];
-  __shared__ int list[MX_ROWS];
-  const int first = blockIdx.y, id = p.ids[first], e = id - p.base;
-  if (e < 0 || e >= p.experts) return;
-  MxStream<MX_MOE_TILES, RUN> s(p.w + e * p.expert_bytes, MxLayout(p.n, p.k), blockIdx.x * MX_MOE_TILES, __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), MX_MOE_WAVES);
-  mx_scan(p, id, masks);
-  __syncthreads();
-  const int rows = mx_slot_of(masks, first, list);
-  if (rows == 0) return;
-  __syncthreads();
-  const MxActs acts(part, rows, p.k);
-  for (int i = threadIdx.x; i < rows * acts.groups; i += 64 * MX_MOE_WAVES) {
-    const int r = i / acts.groups, group = i - r * acts.groups;
-    acts.put(r, group, p.aq + (int64_t)list[r] * (p.k / 2), p.as + (int64_t)list[r] * acts.groups);
-  }
-  __syncthreads();
-  s.run(acts);
-  mx_hand_over<MX_MOE_TILES>(part, s.acc);
-  const int r = threadIdx.x & 31;
+  int list;
+  const int rows = mx_few_product<RUN>(p, part, list, [&](const MxActs& acts, int r, int group, int pair) {
+    acts.put(r, group, p.aq + (int64_t)pair * (p.k / 2), p.as + (int64_t)pair * acts.groups);
+  });
+  const int r = threadIdx.x & 31, pair = __shfl(list, r);
   if (r >= rows) return;
-#pragma unroll
-  for (int t = 0; t < MX_MOE_TILES; t++) {
-    const f32x4_t sum = mx_joined<MX_MOE_TILES>(part, MX_MOE_WAVES, 256 * t + threadIdx.x);
-    const int n = (blockIdx.x * MX_MOE_TILES + t) * MX_ROWS + 8 * (threadIdx.x >> 6) + 4 * ((threadIdx.x & 63) >> 5);
-    typedef __attribute__((ext_vector_type(4))) Y y4_t;
-    if (n < p.n) *reinterpret_cast<y4_t*>(static_cast<Y*>(p.y) + (int64_t)list[r] * p.n + n) = y4_t{(Y)sum[0], (Y)sum[1], (Y)sum[2], (Y)sum[3]};
-  }
+  const f32x4_t sum = mx_joined<MX_MOE_TILES>(part, MX_FEW_WAVES, threadIdx.x);
+  const int n = (blockIdx.x * MX_MOE_TILES + (threadIdx.x >> 8)) * MX_ROWS + 8 * ((threadIdx.x >> 6) & 3) + 4 * ((threadIdx.x & 63) >> 5);
+  typedef __attribute__((ext_vector_type(4))) Y y4_t;
+  if (n < p.n) *reinterpret_cast<y4_t*>(static_cast<Y*>(p.y) + (int64_t)pair * p.n + n) = y4_t{(Y)sum[0], (Y)sum[1], (Y)sum[2], (Y)sum[3]};
 }
 
 // fc2 and the weighted sum of one row (blockIdx.y): a workgroup one tile of columns, its wavefronts the row's pairs in turn, their weighted
 // results added in wavefront order. Reads a row's experts whether or not other rows name them too.
 constexpr int MX_ROW_WAVES = 8;
-constexpr int MX_SINGLE_ROWS = 1;
+// ... where a wavefront's share is short: up to this many chunks of a row's pairs. One row of 10 of 512 experts (2048, 512), 80 chunks, fc2 so and as slots
+// with a combine: 16.4 and 19.0 us the call, four rows 25.7 and 32.6; of 22 (1024, 2688), 924 chunks, one row 39.5 and 30.4.
+constexpr int MX_ROW_CHUNKS = 128;
 constexpr int MX_MANY_GROUPS = 1536;
 constexpr int MX_PLAN_PAIRS = 1024;  // from here the plan's launches share the pairs
 __global__ __launch_bounds__(64 * MX_ROW_WAVES, 2) void mx_fc2_row_kernel(MxMoe p) {
@@ -453,7 +435,7 @@ struct MxWorkspace {
   size_t bytes;
 };
 
-bool few_pairs(int64_t pairs, int hidden, int inter) { return pairs <= 64 && MxActs::bytes(std::min<int64_t>(pairs, MX_ROWS), std::max(hidden, inter)) <= 48 * 1024; }
+bool few_pairs(int64_t pairs, int hidden, int inter) { return pairs <= MX_SCAN_PAIRS && MxActs::bytes(std::min<int64_t>(pairs, MX_ROWS), std::max(hidden, inter)) <= 64 * 1024; }
 
 MxWorkspace carve(const hb_mxfp4_experts* ex, void* base, int64_t m, int topk, bool sum) {
   const int64_t pairs = m * topk;
@@ -537,18 +519,18 @@ extern "C" int hb_mxfp4_moe(const hb_mxfp4_experts* experts, const void* x, cons
   const unsigned groups1 = (unsigned)((l1.tiles + MX_MOE_TILES - 1) / MX_MOE_TILES), groups2 = (unsigned)((l2.tiles + MX_MOE_TILES - 1) / MX_MOE_TILES);
   if (few_pairs(pairs, experts->hidden, experts->inter)) {
     const int most = (int)std::min<int64_t>(MX_ROWS, pairs);
-    const size_t room = (size_t)MX_MOE_WAVES * MX_MOE_TILES * 4096;
+    const size_t room = (size_t)MX_FEW_WAVES * MX_MOE_TILES * 4096;
     p1.x = x;
     const size_t lds1 = std::max(room, MxActs::bytes(most, p1.k)), lds2 = std::max(room, MxActs::bytes(most, p2.k));
-    const dim3 grid1(groups1, (unsigned)pairs), grid2(groups2, (unsigned)pairs), block(64 * MX_MOE_WAVES);
-    const bool long1 = l1.chunks >= 4 * MX_MOE_WAVES, long2 = l2.chunks >= 4 * MX_MOE_WAVES;
+    const dim3 grid1(groups1, (unsigned)pairs), grid2(groups2, (unsigned)pairs), block(64 * MX_FEW_WAVES);
+    const bool long1 = l1.chunks >= 4 * MX_FEW_WAVES, long2 = l2.chunks >= 4 * MX_FEW_WAVES;
     auto launch = [&](auto kernel, dim3 grid, size_t lds, const MxMoe& p) { HB_LAUNCH(kernel, grid, block, lds, s, p); };
     if (experts->gated) {
       launch(long1 ? mx_fc1_few_kernel<true, 4> : mx_fc1_few_kernel<true, 2>, grid1, lds1, p1);
     } else {
       launch(long1 ? mx_fc1_few_kernel<false, 4> : mx_fc1_few_kernel<false, 2>, grid1, lds1, p1);
     }
-    if (sum && m <= MX_SINGLE_ROWS) {
+    if (sum && topk * l2.chunks <= MX_ROW_CHUNKS) {
       p2.y = out;
       HB_LAUNCH(mx_fc2_row_kernel, dim3((unsigned)l2.tiles, (unsigned)m), dim3(64 * MX_ROW_WAVES), 0, s, p2);
       return launch_status();

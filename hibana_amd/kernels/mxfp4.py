@@ -8,8 +8,6 @@ stands for NaN as a whole (scale byte 255, codes 0): the format has no other way
 """
 from __future__ import annotations
 
-from typing import NamedTuple
-
 import torch
 
 from hibana_amd import _lib
@@ -19,32 +17,79 @@ TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}  # HB_BF16, HB_F
 CODES = 3  # HB_MXFP4
 
 
-class Mxfp4(NamedTuple):
-    """Values [..., K] held in the format."""
-    codes: torch.Tensor   # uint8 [..., K / 2], element 2 i in the low nibble of byte i
-    scales: torch.Tensor  # uint8 [..., K / 32], byte b for 2^(b - 127), 255 for NaN
+class Mxfp4:
+    """Values [..., K] held in the format: `codes` uint8 [..., K / 2], element 2 i in the low nibble of byte i, and `scales` uint8
+    [..., K / 32], byte b for 2^(b - 127), 255 for NaN. Unpacks into the two. What a kernel here has rounded lies in one allocation, codes first,
+    and becomes the two tensors when they are asked for: a small call pays for one."""
+    __slots__ = ("_codes", "_scales", "_block", "shape")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
+        self._codes, self._scales, self._block = codes, scales, None
+        self.shape = (*codes.shape[:-1], codes.shape[-1] * 2) if codes.ndim else ()
+
+    @classmethod
+    def of_block(cls, block: torch.Tensor, shape: tuple[int, ...]) -> "Mxfp4":
+        """Codes and scales one behind the other in `block`."""
+        self = cls.__new__(cls)
+        self._codes = self._scales = None
+        self._block, self.shape = block, shape
+        return self
+
+    def _split(self) -> None:
+        *lead, k = self.shape
+        size = self._block.numel() * 16 // 17  # 16 bytes of codes to one of scales
+        self._codes = self._block[:size].view(*lead, k // 2)
+        self._scales = self._block[size:].view(*lead, k // GROUP)
 
     @property
-    def shape(self) -> tuple[int, ...]:
-        return (*self.codes.shape[:-1], self.codes.shape[-1] * 2)
+    def codes(self) -> torch.Tensor:
+        if self._codes is None:
+            self._split()
+        return self._codes
+
+    @property
+    def scales(self) -> torch.Tensor:
+        if self._scales is None:
+            self._split()
+        return self._scales
 
     @property
     def device(self) -> torch.device:
-        return self.codes.device
+        return (self._codes if self._block is None else self._block).device
+
+    def __iter__(self):
+        return iter((self.codes, self.scales))
+
+    def __reduce__(self):
+        return Mxfp4, (self.codes, self.scales)
 
 
 def check(q: Mxfp4, what: str) -> None:
-    if q.codes.dtype != torch.uint8 or q.scales.dtype not in (torch.uint8, torch.float8_e8m0fnu) or q.codes.ndim == 0 or q.codes.shape[-1] % 16 or \
-            q.scales.shape != (*q.codes.shape[:-1], q.codes.shape[-1] // 16):
+    codes, scales = q
+    if codes.dtype != torch.uint8 or scales.dtype not in (torch.uint8, torch.float8_e8m0fnu) or codes.ndim == 0 or codes.shape[-1] % 16 or \
+            scales.shape != (*codes.shape[:-1], codes.shape[-1] // 16):
         raise ValueError(f"{what}: codes uint8 [..., K / 2] and scales uint8 [..., K / 32], K a multiple of {GROUP}")
 
 
-def flat(q: Mxfp4, what: str) -> Mxfp4:
-    """The same values as whole rows, contiguous and on the boundaries the kernels read at (a copy only where they are not)."""
+def flat(q: Mxfp4, what: str) -> tuple[torch.Tensor, torch.Tensor]:
+    """Codes and scales as whole rows, contiguous and on the boundaries the kernels read at (a copy only where they are not)."""
     check(q, what)
     k = q.codes.shape[-1]
     codes, scales = q.codes.reshape(-1, k).contiguous(), q.scales.view(torch.uint8).reshape(-1, k // 16).contiguous()
-    return Mxfp4(codes if codes.data_ptr() % 16 == 0 else codes.clone(), scales)
+    return codes if codes.data_ptr() % 16 == 0 else codes.clone(), scales
+
+
+def places(q: Mxfp4, what: str):
+    """(address of the codes, address of the scales, what to hold until the launch that reads them is enqueued), on the current device."""
+    block = q._block
+    if block is not None:
+        _lib.need_one_gpu(block)
+        at = block.data_ptr()
+        return at, at + block.numel() * 16 // 17, block
+    check(q, what)
+    _lib.need_one_gpu(q.codes, q.scales)
+    held = flat(q, what)
+    return held[0].data_ptr(), held[1].data_ptr(), held
 
 
 def rows16(x: torch.Tensor) -> torch.Tensor:
@@ -56,18 +101,19 @@ def rows16(x: torch.Tensor) -> torch.Tensor:
 def quantize(x: torch.Tensor) -> Mxfp4:
     """x [..., K] (BF16, FP16 or FP32; K a multiple of 32) rounded to the format."""
     kind = TYPES.get(x.dtype)
-    if kind is None or x.ndim == 0 or x.shape[-1] % GROUP:
+    shape = tuple(x.shape)
+    if kind is None or not shape or shape[-1] % GROUP:
         raise ValueError(f"mxfp4.quantize: BF16, FP16 or FP32 [..., K], K a multiple of {GROUP}")
     _lib.need_one_gpu(x)
-    shape, k = x.shape, x.shape[-1]
-    codes = torch.empty((*shape[:-1], k // 2), dtype=torch.uint8, device=x.device)
-    scales = torch.empty((*shape[:-1], k // GROUP), dtype=torch.uint8, device=x.device)
-    if x.numel():
+    n = x.numel()
+    block = x.new_empty(n // GROUP * 17, dtype=torch.uint8)
+    if n:
         xc = rows16(x)  # held until the launch is enqueued
-        code = _lib.lib().hb_mxfp4_quantize(xc.data_ptr(), kind, x.numel() // k, k, codes.data_ptr(), scales.data_ptr(), _lib.stream())
+        at = block.data_ptr()
+        code = _lib.lib().hb_mxfp4_quantize(xc.data_ptr(), kind, n // shape[-1], shape[-1], at, at + n // 2, _lib.stream())
         if code:
             _lib.check(code, "mxfp4.quantize")
-    return Mxfp4(codes, scales)
+    return Mxfp4.of_block(block, shape)
 
 
 def dequantize(q: Mxfp4, dtype: torch.dtype = torch.float32) -> torch.Tensor:
@@ -75,12 +121,12 @@ def dequantize(q: Mxfp4, dtype: torch.dtype = torch.float32) -> torch.Tensor:
     kind = TYPES.get(dtype)
     if kind is None:
         raise ValueError("mxfp4.dequantize: to BF16, FP16 or FP32")
-    check(q, "mxfp4.dequantize")
-    _lib.need_one_gpu(q.codes, q.scales)
-    out = torch.empty(q.shape, dtype=dtype, device=q.codes.device)
-    if out.numel():
-        f = flat(q, "mxfp4.dequantize")
-        code = _lib.lib().hb_mxfp4_dequantize(f.codes.data_ptr(), f.scales.data_ptr(), f.codes.shape[0], q.shape[-1], kind, out.data_ptr(), _lib.stream())
+    codes, scales, held = places(q, "mxfp4.dequantize")
+    out = torch.empty(q.shape, dtype=dtype, device=q.device)
+    n = out.numel()
+    if n:
+        k = q.shape[-1]
+        code = _lib.lib().hb_mxfp4_dequantize(codes, scales, n // k, k, kind, out.data_ptr(), _lib.stream())
         if code:
             _lib.check(code, "mxfp4.dequantize")
     return out
@@ -98,12 +144,12 @@ def tile(q: Mxfp4, gated: bool = False) -> torch.Tensor:
     if size == 0:
         raise ValueError(f"mxfp4.tile: a matrix [{n}, {k}] is past what the kernels index")
     tiled = torch.empty((*q.codes.shape[:-2], size), dtype=torch.uint8, device=q.codes.device)
-    f = flat(q, "mxfp4.tile")
+    codes, scales = flat(q, "mxfp4.tile")
     lo = 0
     stacked = tiled.view(-1, size)
     while lo < stacked.shape[0]:  # a launch's grid holds 65535 matrices
         count = min(65535, stacked.shape[0] - lo)
-        _lib.check(_lib.lib().hb_mxfp4_repack(f.codes[lo * n:].data_ptr(), f.scales[lo * n:].data_ptr(), count, n, k, int(gated), stacked[lo:].data_ptr(),
+        _lib.check(_lib.lib().hb_mxfp4_repack(codes[lo * n:].data_ptr(), scales[lo * n:].data_ptr(), count, n, k, int(gated), stacked[lo:].data_ptr(),
                                               _lib.stream()), "mxfp4.tile")
         lo += count
     return tiled

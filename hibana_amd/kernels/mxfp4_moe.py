@@ -83,13 +83,15 @@ def _struct(experts: Mxfp4Experts) -> _lib.HbMxfp4Experts:
     """The experts as the library takes them: built once, and again when a tensor or a number of `experts` was replaced."""
     if experts.tiled1 is None or experts.tiled2 is None:
         tile(experts)
-    key = (experts.tiled1.data_ptr(), experts.tiled2.data_ptr(), experts.base, experts.shape1, experts.shape2)
     have = experts.__dict__.get("_packed")
-    if have is None or have[0] != key:
+    if have is None or have.of[0] is not experts.tiled1 or have.of[1] is not experts.tiled2 or have.of[2:] != (experts.base, experts.shape1, experts.shape2):
         (e, _, h), (_, h2, i) = experts.shape1, experts.shape2
-        have = key, _lib.HbMxfp4Experts(*key[:2], e, experts.base, h, i, h2, int(experts.gated))
+        have = _lib.HbMxfp4Experts(experts.tiled1.data_ptr(), experts.tiled2.data_ptr(), e, experts.base, h, i, h2, int(experts.gated))
+        have.of = (experts.tiled1, experts.tiled2, experts.base, experts.shape1, experts.shape2)
+        have.at = C.byref(have)
+        have.bytes_of = {}  # the workspace a call of (rows, k) takes
         experts._packed = have
-    return have[1]
+    return have
 
 
 def mxfp4_moe(experts: Mxfp4Experts, x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, pairs: bool = False, pairs_bf16: bool = False) -> torch.Tensor:
@@ -100,21 +102,25 @@ def mxfp4_moe(experts: Mxfp4Experts, x: torch.Tensor, ids: torch.Tensor, weights
         raise ValueError("mxfp4_moe: x must be BF16 [M, hidden]")
     if ids.ndim != 2 or ids.shape[0] != x.shape[0] or weights.shape != ids.shape:
         raise ValueError("mxfp4_moe: ids and weights must be [M, k]")
-    if experts.tiled1 is None or experts.tiled2 is None:
-        tile(experts)
+    st = _struct(experts)
     _lib.need_one_gpu(x, ids, weights, experts.tiled1, experts.tiled2)
     m, k = ids.shape
     mode = (2 if pairs_bf16 else 1) if pairs else 0
-    h_out = experts.shape2[1]
-    out = torch.empty((m * k, h_out) if pairs else (m, h_out), dtype=torch.float32 if mode == 1 else torch.bfloat16, device=x.device)
+    out = x.new_empty((m * k if pairs else m, experts.shape2[1]), dtype=torch.float32 if mode == 1 else torch.bfloat16)
     if m == 0 or k == 0:
         return out if pairs else out.zero_()
-    st = _struct(experts)
     lib = _lib.lib()
-    need = lib.hb_mxfp4_moe_workspace_bytes(C.byref(st), m, k)
-    ws = torch.empty(max(need, 16), dtype=torch.uint8, device=x.device)  # (of the capture's own pool in a captured call)
-    ids32, wt, xc = ids.to(torch.int32).contiguous(), weights.float().contiguous(), mxfp4.rows16(x)  # held until the launches are enqueued
-    code = lib.hb_mxfp4_moe(C.byref(st), xc.data_ptr(), ids32.data_ptr(), wt.data_ptr(), m, k, mode, out.data_ptr(), ws.data_ptr(), need, _lib.stream())
+    need = st.bytes_of.get((m, k))
+    if need is None:
+        if len(st.bytes_of) >= 4096:
+            st.bytes_of.clear()
+        need = st.bytes_of[m, k] = lib.hb_mxfp4_moe_workspace_bytes(st.at, m, k)
+    ws = experts.tiled1.new_empty(max(need, 16))  # (of the capture's own pool in a captured call)
+    # converted operands keep a name until the launches are enqueued
+    ids32 = ids if ids.dtype == torch.int32 and ids.is_contiguous() else ids.to(torch.int32).contiguous()
+    wt = weights if weights.dtype == torch.float32 and weights.is_contiguous() else weights.float().contiguous()
+    xc = mxfp4.rows16(x)
+    code = lib.hb_mxfp4_moe(st.at, xc.data_ptr(), ids32.data_ptr(), wt.data_ptr(), m, k, mode, out.data_ptr(), ws.data_ptr(), need, _lib.stream())
     if code:
         _lib.check(code, "mxfp4_moe")
     return out

@@ -47,23 +47,25 @@ def mxfp4_linear(x, lin, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     ready = isinstance(x, mxfp4.Mxfp4)
     kind = mxfp4.CODES if ready else mxfp4.TYPES.get(x.dtype)
     out_type = dtype if ready else x.dtype
-    if kind is None or out_type not in mxfp4.TYPES or len(x.shape) != 2 or x.shape[1] != lin.in_features:
+    to = mxfp4.TYPES.get(out_type)
+    if kind is None or to is None or len(x.shape) != 2 or x.shape[1] != lin.in_features:
         raise ValueError("mxfp4_linear: x must be BF16, FP16 or FP32 [M, in_features], or hold such rows")
     if lin.tiled is None:
         lin.tile()
-    _lib.need_one_gpu(*(x if ready else (x,)), lin.tiled)
+    if ready:
+        at, scales, held = mxfp4.places(x, "mxfp4_linear")
+        _lib.need_one_gpu(lin.tiled)
+    else:
+        _lib.need_one_gpu(x, lin.tiled)
+        held = mxfp4.rows16(x)  # held until the launch is enqueued
+        at, scales = held.data_ptr(), None
     m, n, k = x.shape[0], lin.out_features, lin.in_features
-    y = torch.empty((m, n), dtype=out_type, device=x.device)
+    y = lin.tiled.new_empty((m, n), dtype=out_type)
     if m:
         lib = _lib.lib()
-        if ready:
-            xc, xs = mxfp4.flat(x, "mxfp4_linear")  # held until the launch is enqueued
-        else:
-            xc, xs = mxfp4.rows16(x), None
         need = lib.hb_mxfp4_linear_workspace_bytes(m, n, k, kind)
-        ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
-        code = lib.hb_mxfp4_linear(xc.data_ptr(), _lib.ptr(xs), kind, m, lin.tiled.data_ptr(), n, k, y.data_ptr(), mxfp4.TYPES[out_type], _lib.ptr(ws), need,
-                                   _lib.stream())
+        ws = lin.tiled.new_empty(need) if need else None  # (of the capture's own pool in a captured call)
+        code = lib.hb_mxfp4_linear(at, scales, kind, m, lin.tiled.data_ptr(), n, k, y.data_ptr(), to, _lib.ptr(ws), need, _lib.stream())
         if code:
             _lib.check(code, "mxfp4_linear")
     return y
@@ -134,15 +136,15 @@ def silu_mul_quant_mxfp4(gate_up: torch.Tensor, pairs: int = 0) -> mxfp4.Mxfp4:
     if pairs and (pairs < 0 or pairs % 8 or half % pairs):
         raise ValueError("silu_mul_quant_mxfp4: pairs must be a multiple of eight dividing I")
     _lib.need_one_gpu(gate_up)
-    lead = gate_up.shape[:-1]
-    codes = torch.empty((*lead, half // 2), dtype=torch.uint8, device=gate_up.device)
-    scales = torch.empty((*lead, half // mxfp4.GROUP), dtype=torch.uint8, device=gate_up.device)
-    if gate_up.numel():
-        gu = mxfp4.rows16(gate_up)
-        code = _lib.lib().hb_silu_mul_quant_mxfp4(gu.data_ptr(), kind, gate_up.numel() // (2 * half), half, pairs, codes.data_ptr(), scales.data_ptr(), _lib.stream())
+    n = gate_up.numel() // 2
+    block = gate_up.new_empty(n // mxfp4.GROUP * 17, dtype=torch.uint8)
+    if n:
+        gu = mxfp4.rows16(gate_up)  # held until the launch is enqueued
+        at = block.data_ptr()
+        code = _lib.lib().hb_silu_mul_quant_mxfp4(gu.data_ptr(), kind, n // half, half, pairs, at, at + n // 2, _lib.stream())
         if code:
             _lib.check(code, "silu_mul_quant_mxfp4")
-    return mxfp4.Mxfp4(codes, scales)
+    return mxfp4.Mxfp4.of_block(block, (*gate_up.shape[:-1], half))
 
 
 def route_topk(logits: torch.Tensor, k: int, slots: torch.Tensor | None = None, steps: int = 1, repeat: bool = False):

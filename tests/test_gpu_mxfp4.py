@@ -95,6 +95,10 @@ def test_leading_axes_strides_offsets_and_nothing():
     _same(mxfp4.quantize(odd), om.quantize(x))
     part = mxfp4.Mxfp4(q.codes.flatten(0, 2)[::3, 16:64], q.scales.flatten(0, 2)[::3, 1:4])
     assert torch.equal(mxfp4.dequantize(part).cpu().double(), om.dequantize(part.codes.cpu(), part.scales.cpu()))
+    import copy
+    import pickle
+    for other in (copy.deepcopy(q), pickle.loads(pickle.dumps(q)), mxfp4.Mxfp4(*q)):
+        assert other.shape == q.shape and torch.equal(mxfp4.dequantize(other), mxfp4.dequantize(q))
     for shape in ((0, 64), (5, 0), (0,)):
         e = mxfp4.quantize(torch.empty(shape, device="cuda"))
         assert mxfp4.dequantize(e).shape == shape
