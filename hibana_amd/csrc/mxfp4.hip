@@ -195,16 +195,56 @@ __device__ __forceinline__ void mx_store4(Y* out, const f32x4_t& v, int64_t left
 template <typename T, typename Y, int NT, int RUN>
 __global__ __launch_bounds__(512) void mx_few_rows_kernel(MxLinear p) {
   extern __shared__ f32x4_t part[];  // the activations, then [waves][NT * 4][64]
+  constexpr int AT_ONCE = std::is_same_v<T, float> ? 4 : 8;
+  MxStream<NT, RUN> s;
   const MxLayout at(p.n, p.k);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), t0 = blockIdx.x * NT, rows = (int)p.m, groups = p.k / MX_GROUP;
-  MxStream<NT, RUN> s(p.w, at, t0, wave, p.waves);
   const MxActs acts(part, rows, p.k);
-  for (int i = threadIdx.x; i < rows * groups; i += blockDim.x) {
-    const int r = i / groups, group = i - r * groups;
-    if constexpr (std::is_same_v<T, uint8_t>) {
-      acts.put(r, group, static_cast<const uint8_t*>(p.x) + (int64_t)r * (p.k / 2), p.x_scales + (int64_t)r * groups);
-    } else {
-      acts.put(r, group, static_cast<const T*>(p.x) + (int64_t)r * p.k + MX_GROUP * group);
+  // Loads return in order: the first activations are asked for ahead of the weights, or they would stand behind all of them while nothing else is on its way.
+  if constexpr (std::is_same_v<T, uint8_t>) {
+    const int all = rows * groups;
+    auto source = [&](int i, i32x4_t& code, uint32_t& scale) {
+      code = *reinterpret_cast<const i32x4_t*>(static_cast<const uint8_t*>(p.x) + 16 * (int64_t)i);
+      scale = p.x_scales[i];
+    };
+    auto put = [&](int i, const i32x4_t& code, uint32_t scale) {
+      const int r = i / groups, at = (i - r * groups) * rows + r;
+      acts.codes[at] = code;
+      acts.scales[at] = (uint8_t)scale;
+    };
+    i32x4_t code[AT_ONCE];
+    uint32_t scale[AT_ONCE];
+#pragma unroll
+    for (int j = 0; j < AT_ONCE; j++) source(min((int)(threadIdx.x + j * blockDim.x), all - 1), code[j], scale[j]);
+    __builtin_amdgcn_sched_barrier(0);
+    s.begin(p.w, at, t0, wave, p.waves);
+#pragma unroll
+    for (int j = 0; j < AT_ONCE; j++)
+      if (threadIdx.x + j * blockDim.x < all) put(threadIdx.x + j * blockDim.x, code[j], scale[j]);
+    for (int i = threadIdx.x + AT_ONCE * blockDim.x; i < all; i += blockDim.x) {
+      source(i, code[0], scale[0]);
+      put(i, code[0], scale[0]);
+    }
+  } else {
+    const int all = rows * groups * 4;  // eight values from 8 i of the contiguous rows a lane
+    const uint32_t inverse = 0xffffffffu / (uint32_t)groups + 1u;  // i / groups = the upper half of i inverse: i below 32 groups, groups below 2^13
+    auto source = [&](Mx8<T>& v, int i) { v.load(static_cast<const T*>(p.x) + 8 * (int64_t)min(i, all - 1)); };
+    auto put = [&](int i, const Mx8<T>& v) {
+      const int r = groups == 1 ? i >> 2 : (int)__umulhi((uint32_t)i >> 2, inverse);
+      if (i < all) acts.put(r, (i >> 2) - r * groups, i & 3, v);
+    };
+    Mx8<T> v[AT_ONCE];
+#pragma unroll
+    for (int j = 0; j < AT_ONCE; j++) source(v[j], threadIdx.x + j * blockDim.x);
+    __builtin_amdgcn_sched_barrier(0);
+    s.begin(p.w, at, t0, wave, p.waves);
+#pragma unroll
+    for (int j = 0; j < AT_ONCE; j++) put(threadIdx.x + j * blockDim.x, v[j]);
+    for (int i0 = threadIdx.x + AT_ONCE * blockDim.x; i0 < all; i0 += AT_ONCE * blockDim.x) {
+#pragma unroll
+      for (int j = 0; j < AT_ONCE; j++) source(v[j], i0 + j * blockDim.x);
+#pragma unroll
+      for (int j = 0; j < AT_ONCE; j++) put(i0 + j * blockDim.x, v[j]);
     }
   }
   __syncthreads();
@@ -230,7 +270,7 @@ __global__ __launch_bounds__(512) void mx_few_rows_kernel(MxLinear p) {
 struct MxTiles {
   const uint8_t* a;
   const uint8_t* w;
-  void* y;
+  void* y;               // K shared by gridDim.y workgroups: their FP32 sums [shares, m, n]
   int64_t m, n;
   int k, rows_of_tiles;  // workgroups along m
 };
@@ -299,6 +339,8 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void mx_ring_kernel(MxTiles p) {
   const int total = gridDim.x, per = (total + 7) / 8, die = blockIdx.x % 8, whole = total % 8 ? total % 8 : 8;  // the first `whole` dies have `per` workgroups, the others one less
   const int at = die * per - (die > whole ? die - whole : 0) + (int)(blockIdx.x / 8);
   const int a0 = at % p.rows_of_tiles * TA, b0 = at / p.rows_of_tiles * TB, chunks = la.chunks, row_bytes = chunks * 1024;
+  const int pairs = la.quads / 2, q0 = 2 * (int)((int64_t)pairs * blockIdx.y / gridDim.y), q1 = 2 * (int)((int64_t)pairs * (blockIdx.y + 1) / gridDim.y);
+  p.y = static_cast<Y*>(p.y) + (int64_t)blockIdx.y * p.m * p.n;
 
   const int first_a = min(a0, la.tiles - 1), first_b = min(b0, lw.tiles - 1), left_a = min(TA, la.tiles - first_a), left_b = min(TB, lw.tiles - first_b);
   const __amdgpu_buffer_rsrc_t rows_a = mx_rows(p.a + (int64_t)first_a * row_bytes, left_a * row_bytes);
@@ -337,10 +379,10 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void mx_ring_kernel(MxTiles p) {
       for (int e = 0; e < 16; e++) acc[i][j][e] = 0.f;
 
 #pragma unroll
-  for (int t = 0; t < SCALES; t++) scale(t, 0);
-  mx_unrolled<ASKS>([&](auto j) { MX_ASK(buf0, 0, j.value) });
-  mx_unrolled<ASKS>([&](auto j) { MX_ASK(buf1, 1, j.value) });
-  mx_unrolled<ASKS>([&](auto j) { MX_ASK(buf2, 2, j.value) });
+  for (int t = 0; t < SCALES; t++) scale(t, q0);
+  mx_unrolled<ASKS>([&](auto j) { MX_ASK(buf0, 2 * q0, j.value) });
+  mx_unrolled<ASKS>([&](auto j) { MX_ASK(buf1, 2 * q0 + 1, j.value) });
+  mx_unrolled<ASKS>([&](auto j) { MX_ASK(buf2, 2 * q0 + 2, j.value) });
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(ASKS) : "memory");
   __builtin_amdgcn_s_barrier();
   // a step: for each of its two chunks and each tile of B, the products with all tiles of A. Fragments come ahead of their use: B's two
@@ -377,7 +419,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void mx_ring_kernel(MxTiles p) {
   __builtin_amdgcn_sched_barrier(0);
 #define MX_QUAD                                                               \
   _Pragma("unroll") for (int t = 0; t < SCALES; t++) now[t] = next[t];
-  for (int q = 0; q < la.quads; q += 2) {
+  for (int q = q0; q < q1; q += 2) {
     MX_QUAD
     MX_STEP(buf0, buf1, buf3, 2 * q, 0)
     MX_STEP(buf1, buf2, buf0, 2 * q + 1, 1)
@@ -413,53 +455,137 @@ __global__ __launch_bounds__(256) void mx_quantize_tiles_kernel(const T* __restr
   if (row >= rows) return;
   uint32_t byte = 0;
   i32x4_t code = {0, 0, 0, 0};
-  if (group < k / MX_GROUP) code = mx_round_group<T>(x + row * k + MX_GROUP * (int64_t)group, byte);
+  if (group < k / MX_GROUP) {
+    MxGroup<T> v;
+    v.load(x + row * k + MX_GROUP * (int64_t)group);
+    code = v.codes(byte);
+  }
   if (c < at.chunks) *reinterpret_cast<i32x4_t*>(tiled + ((t * at.chunks + c) * 64 + lane) * 16) = code;
   tiled[at.codes() + (t * at.quads + (c >> 2)) * 256 + lane * 4 + (c & 3)] = (uint8_t)byte;
 }
 
-// Rows whose activations fit a workgroup's LDS twice a compute unit.
-static bool few_rows(int64_t m, int k) { return m <= MX_ROWS && MxActs::bytes(m, k) <= 64 * 1024; }
+// The shares' sums added in their order and rounded, four columns a thread (`whole`) or one.
+template <typename Y>
+__global__ __launch_bounds__(256) void mx_join_kernel(const float* __restrict__ sums, int64_t count, int shares, int whole, Y* __restrict__ y) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (whole) {
+    if (4 * i >= count) return;
+    f32x4_t sum = reinterpret_cast<const f32x4_t*>(sums)[i];
+    for (int s = 1; s < shares; s++) sum += *reinterpret_cast<const f32x4_t*>(sums + s * count + 4 * i);
+    mx_store4<Y>(y + 4 * i, sum, 4, true);
+  } else {
+    if (i >= count) return;
+    float sum = sums[i];
+    for (int s = 1; s < shares; s++) sum += sums[s * count + i];
+    y[i] = mx_out<Y>(sum);
+  }
+}
+
+// How a call is made.
+struct MxPlan {
+  enum { FEW_ROUNDING, FEW, RING } way;
+  int mt, shares;    // RING: row tiles a wavefront (4 wide: 4 of the 2 x 2 form; 2 wide: its half), workgroups that share K
+  bool square;       // RING: the 2 x 2 forms
+  size_t tiles, bytes;  // workspace: of the activations, of all
+};
+// Few rows (their activations fit LDS): a wavefront's chunks of K and few weight rows a workgroup keep a small matrix's call short, and the rounding rides
+// in it while all of a workgroup's rows are not more than MX_ROUND_VALUES values; past that it is a launch of its own. Where the matrix alone
+// fills the device several times over, the ring takes over from there. us, 25600 x 5120: 8 rows 17.8 rounding inside, 17.4 ring; 16 rows 20.7 and
+// 17.3; 5120 x 5120: 8 rows 8.6 inside, 14.4 ring; 16 rows 10.6 inside, 7.4 and 2 for a launch of its own, 14.3 ring.
+constexpr int64_t MX_ROUND_VALUES = 48 * 1024;
+constexpr int MX_RING_TILES = 768;
+static MxPlan plan_of(int64_t m, int64_t n, int k, int x_type) {
+  const MxLayout rows(m, k), w(n, k);
+  MxPlan p{};
+  const size_t acts = MxActs::bytes(m, k);
+  const bool small = m * k <= MX_ROUND_VALUES;
+  if (m <= MX_ROWS && acts <= (w.tiles <= 256 ? 144 : 64) * 1024 && (small || w.tiles < MX_RING_TILES)) {
+    const bool rounds = x_type != HB_MXFP4 && !small;
+    p.way = rounds ? MxPlan::FEW : MxPlan::FEW_ROUNDING;
+    p.tiles = p.bytes = rounds ? (size_t)m * (k / 2 + k / MX_GROUP) : 0;
+    return p;
+  }
+  p.way = MxPlan::RING;
+  p.square = m > 128;
+  auto groups = [&](int mt) {
+    const int64_t high = p.square ? 2 * mt : mt, wide = p.square ? 2 * mt : 4;
+    return (rows.tiles + high - 1) / high * ((w.tiles + wide - 1) / wide);
+  };
+  p.mt = p.square ? (groups(4) >= 160 ? 4 : 2) : rows.tiles;
+  // K is shared where the tiles leave half the device idle, by up to eight workgroups of at least eight steps
+  p.shares = (int)std::max<int64_t>(1, std::min<int64_t>({256 / groups(p.mt), rows.quads / 4, 8}));
+  p.tiles = (size_t)(rows.bytes() + 255) / 256 * 256;
+  p.bytes = p.tiles + (p.shares > 1 ? (size_t)p.shares * m * n * sizeof(float) : 0);
+  return p;
+}
 
 template <typename Y, int WM, int WN, int MT, int NT>
-static int launch_ring(MxTiles p, hipStream_t stream) {
+static int launch_ring(MxTiles p, const MxPlan& plan, float* sums, hipStream_t stream) {
   const MxLayout la(p.m, p.k), lw(p.n, p.k);
   p.rows_of_tiles = (la.tiles + WM * MT - 1) / (WM * MT);
-  const int64_t groups = (int64_t)p.rows_of_tiles * ((lw.tiles + WN * NT - 1) / (WN * NT));
-  HB_LAUNCH((mx_ring_kernel<Y, WM, WN, MT, NT>), dim3((unsigned)groups), dim3(64 * WM * WN), 0, stream, p);
+  const dim3 grid((unsigned)(p.rows_of_tiles * ((lw.tiles + WN * NT - 1) / (WN * NT))), (unsigned)plan.shares);
+  if (plan.shares == 1) {
+    HB_LAUNCH((mx_ring_kernel<Y, WM, WN, MT, NT>), grid, dim3(64 * WM * WN), 0, stream, p);
+    return HB_OK;
+  }
+  Y* y = static_cast<Y*>(p.y);
+  p.y = sums;
+  HB_LAUNCH((mx_ring_kernel<float, WM, WN, MT, NT>), grid, dim3(64 * WM * WN), 0, stream, p);
+  const int64_t count = p.m * p.n;
+  const int whole = count % 4 == 0 && aligned(y, 4 * sizeof(Y)), each = whole ? 1024 : 256;
+  HB_LAUNCH((mx_join_kernel<Y>), dim3((unsigned)((count + each - 1) / each)), dim3(256), 0, stream, sums, count, plan.shares, whole, y);
+  return HB_OK;
+}
+
+template <typename T, typename Y, int NT, int RUN>
+static int launch_few(const MxLinear& p, const MxLayout& at, hipStream_t stream) {
+  const size_t lds = std::max(MxActs::bytes(p.m, p.k), (size_t)p.waves * NT * 4096);
+  if (lds > 64 * 1024) {
+    static const hipError_t raised = hipFuncSetAttribute(reinterpret_cast<const void*>(&mx_few_rows_kernel<T, Y, NT, RUN>), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+    if (raised != hipSuccess) return HB_ELAUNCH;
+  }
+  HB_LAUNCH((mx_few_rows_kernel<T, Y, NT, RUN>), dim3((unsigned)((at.tiles + NT - 1) / NT)), dim3(64 * p.waves), lds, stream, p);
   return HB_OK;
 }
 
 template <typename T, typename Y>
-static int launch_linear(const MxLinear& p0, uint8_t* tiles, hipStream_t stream) {
-  MxLinear p = p0;
-  const MxLayout at(p.n, p.k);
-  if (few_rows(p.m, p.k)) {
-    p.waves = std::min(at.chunks, 8);
-    const size_t acts = MxActs::bytes(p.m, p.k);
-    if (at.tiles < 512) {
-      if (at.chunks >= 32) {
-        HB_LAUNCH((mx_few_rows_kernel<T, Y, 1, 4>), dim3((unsigned)at.tiles), dim3(64 * p.waves), std::max(acts, (size_t)p.waves * 4096), stream, p);
-      } else {
-        HB_LAUNCH((mx_few_rows_kernel<T, Y, 1, 1>), dim3((unsigned)at.tiles), dim3(64 * p.waves), std::max(acts, (size_t)p.waves * 4096), stream, p);
-      }
-    } else {
-      HB_LAUNCH((mx_few_rows_kernel<T, Y, 2, 4>), dim3((unsigned)((at.tiles + 1) / 2)), dim3(64 * p.waves), std::max(acts, (size_t)p.waves * 8192), stream, p);
+static int launch_linear(MxLinear p, uint8_t* workspace, hipStream_t stream) {
+  constexpr bool held = std::is_same_v<T, uint8_t>;
+  const MxPlan plan = plan_of(p.m, p.n, p.k, held ? HB_MXFP4 : HB_F32);
+  if (plan.way == MxPlan::FEW) {
+    const int64_t lanes = p.m * (p.k / 8);
+    if constexpr (!held) {
+      uint8_t* scales = workspace + p.m * (p.k / 2);
+      HB_LAUNCH((mx_quantize_kernel<T>), dim3((unsigned)((lanes + 255) / 256)), dim3(256), 0, stream, static_cast<const T*>(p.x), lanes, workspace, scales);
+      p.x = workspace;
+      p.x_scales = scales;
     }
-    return HB_OK;
   }
-  if constexpr (std::is_same_v<T, uint8_t>) {
-    if (int e = hb_mxfp4_repack(p.x, p.x_scales, 1, p.m, p.k, 0, tiles, stream)) return e;
+  if (plan.way != MxPlan::RING) {
+    const MxLayout at(p.n, p.k);
+    p.waves = std::min(at.chunks, 8);
+    auto few = [&](auto* type) {
+      using X = std::remove_pointer_t<decltype(type)>;
+      if (at.tiles >= 512) return launch_few<X, Y, 2, 4>(p, at, stream);
+      return at.chunks >= 32 ? launch_few<X, Y, 1, 4>(p, at, stream) : launch_few<X, Y, 1, 1>(p, at, stream);
+    };
+    return plan.way == MxPlan::FEW ? few((uint8_t*)nullptr) : few((T*)nullptr);
+  }
+  if constexpr (held) {
+    if (int e = hb_mxfp4_repack(p.x, p.x_scales, 1, p.m, p.k, 0, workspace, stream)) return e;
   } else {
     const MxLayout rows(p.m, p.k);
-    HB_LAUNCH((mx_quantize_tiles_kernel<T>), dim3((unsigned)((int64_t)rows.tiles * rows.quads)), dim3(256), 0, stream, static_cast<const T*>(p.x), p.m, p.k, tiles);
+    HB_LAUNCH((mx_quantize_tiles_kernel<T>), dim3((unsigned)((int64_t)rows.tiles * rows.quads)), dim3(256), 0, stream, static_cast<const T*>(p.x), p.m, p.k, workspace);
   }
-  const MxTiles q{tiles, p.w, p.y, p.m, p.n, p.k, 0};
-  if (p.m <= 32) return launch_ring<Y, 1, 4, 1, 1>(q, stream);
-  if (p.m <= 64) return launch_ring<Y, 1, 4, 2, 1>(q, stream);
-  if (p.m <= 96) return launch_ring<Y, 1, 4, 3, 1>(q, stream);
-  if (p.m <= 128) return launch_ring<Y, 1, 4, 4, 1>(q, stream);
-  return launch_ring<Y, 2, 2, 4, 4>(q, stream);
+  const MxTiles q{workspace, p.w, p.y, p.m, p.n, p.k, 0};
+  float* sums = reinterpret_cast<float*>(workspace + plan.tiles);
+  if (plan.square) return plan.mt == 4 ? launch_ring<Y, 2, 2, 4, 4>(q, plan, sums, stream) : launch_ring<Y, 2, 2, 2, 2>(q, plan, sums, stream);
+  switch (plan.mt) {
+    case 1: return launch_ring<Y, 1, 4, 1, 1>(q, plan, sums, stream);
+    case 2: return launch_ring<Y, 1, 4, 2, 1>(q, plan, sums, stream);
+    case 3: return launch_ring<Y, 1, 4, 3, 1>(q, plan, sums, stream);
+  }
+  return launch_ring<Y, 1, 4, 4, 1>(q, plan, sums, stream);
 }
 
 template <typename F>
@@ -518,6 +644,7 @@ extern "C" int hb_silu_mul_quant_mxfp4(const void* gate_up, int type, int64_t ro
   });
 }
 
+constexpr int64_t MX_MOST_ROWS = (int64_t)1 << 24;
 // Sizes that the layout's indices and a launch's grid hold.
 static bool layout_holds(int64_t n, int k) { return n > 0 && k > 0 && k <= 1 << 23 && k % MX_GROUP == 0 && n <= (int64_t)1 << 30 && (n + 31) / 32 * ((k + 511) / 512) <= (int64_t)1 << 27; }
 
@@ -547,14 +674,13 @@ extern "C" int hb_mxfp4_unpack(const void* tiled, int matrices, int64_t n, int k
 }
 
 extern "C" size_t hb_mxfp4_linear_workspace_bytes(int64_t m, int64_t n, int k, int x_type) {
-  (void)x_type;
-  return m > 0 && layout_holds(n, k) && !few_rows(m, k) && layout_holds(m, k) ? (size_t)MxLayout(m, k).bytes() : 0;
+  return m > 0 && m <= MX_MOST_ROWS && layout_holds(n, k) && layout_holds(m, k) ? plan_of(m, n, k, x_type).bytes : 0;
 }
 
 extern "C" int hb_mxfp4_linear(const void* x, const void* x_scales, int x_type, int64_t m, const void* tiled, int64_t n, int k, void* y, int y_type,
                                void* workspace, size_t workspace_bytes, void* stream) {
   if (!x || !tiled || !y || (x_type == HB_MXFP4 && !x_scales)) return HB_ENULL;
-  if (m <= 0 || m > (int64_t)1 << 19 || !layout_holds(n, k) || y_type < HB_BF16 || y_type > HB_F32 || x_type < HB_BF16 || x_type > HB_MXFP4) return HB_EINVAL;
+  if (m <= 0 || m > MX_MOST_ROWS || !layout_holds(n, k) || y_type < HB_BF16 || y_type > HB_F32 || x_type < HB_BF16 || x_type > HB_MXFP4) return HB_EINVAL;
   if (x_type != HB_MXFP4 && x_type != y_type) return HB_EINVAL;
   if (!aligned(x, 16) || !aligned(tiled, 16) || !aligned(y, type_bytes(y_type))) return HB_EINVAL;
   const size_t need = hb_mxfp4_linear_workspace_bytes(m, n, k, x_type);

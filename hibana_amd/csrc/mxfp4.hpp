@@ -39,6 +39,7 @@ struct MxLayout {
   __host__ __device__ int64_t bytes() const { return codes() + (int64_t)tiles * quads * 256; }
 };
 
+constexpr int MX_NO_REUSE = 2;  // the cache policy of loads whose bytes nobody reads again
 // A buffer descriptor in scalar registers: what is read past `bytes` is zero.
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t mx_rows(const uint8_t* base, uint32_t bytes) {
   const uint64_t at = reinterpret_cast<uint64_t>(base);
@@ -144,22 +145,27 @@ __device__ __forceinline__ uint32_t quad_max(uint32_t x) {
   return o > x ? o : x;
 }
 
-// A lane's whole group of 32 values: the 16 bytes of codes and the scale byte (of a group that is not finite any codes: its scale is NaN).
+// A lane's whole group of 32 values: loaded, then the 16 bytes of codes and the scale byte (of a group that is not finite any codes: its scale
+// is NaN).
 template <typename T>
-__device__ __forceinline__ i32x4_t mx_round_group(const T* p, uint32_t& byte) {
+struct MxGroup {
   Mx8<T> x[4];
+  __device__ __forceinline__ void load(const T* p) {
 #pragma unroll
-  for (int j = 0; j < 4; j++) x[j].load(p + 8 * j);
-  uint32_t m = x[0].amax();
+    for (int j = 0; j < 4; j++) x[j].load(p + 8 * j);
+  }
+  __device__ __forceinline__ i32x4_t codes(uint32_t& byte) const {
+    uint32_t m = x[0].amax();
 #pragma unroll
-  for (int j = 1; j < 4; j++) m = max(m, x[j].amax());
-  byte = mx_scale_byte(m);
-  const float s = mx_scale_value(byte);
-  i32x4_t c;
+    for (int j = 1; j < 4; j++) m = max(m, x[j].amax());
+    byte = mx_scale_byte(m);
+    const float s = mx_scale_value(byte);
+    i32x4_t c;
 #pragma unroll
-  for (int j = 0; j < 4; j++) c[j] = (int)x[j].codes(s);
-  return c;
-}
+    for (int j = 0; j < 4; j++) c[j] = (int)x[j].codes(s);
+    return c;
+  }
+};
 
 // The activations of a product of few rows, in LDS: codes [group][rows][16 bytes], scales [group][rows] behind them, so that the lanes of a
 // fragment read consecutive addresses.
@@ -169,12 +175,13 @@ struct MxActs {
   int rows, groups;
   __device__ __forceinline__ MxActs(void* lds, int rows, int k) : codes(static_cast<i32x4_t*>(lds)), scales(static_cast<uint8_t*>(lds) + (size_t)rows * (k / 2)), rows(rows), groups(k / MX_GROUP) {}
   static __host__ __device__ size_t bytes(int64_t rows, int k) { return ((size_t)rows * (k / 2 + k / MX_GROUP) + 15) / 16 * 16; }
-  // Group `group` of row r: values rounded ...
+  // Eight values, quarter `part` of group `group` of row r, rounded with the three lanes beside that hold the others (a lane a group would
+  // read 64 bytes of its own at a time, twice as many lines an instruction as there are bytes for) ...
   template <typename T>
-  __device__ __forceinline__ void put(int r, int group, const T* values) const {
-    uint32_t byte;
-    codes[group * rows + r] = mx_round_group<T>(values, byte);
-    scales[group * rows + r] = (uint8_t)byte;
+  __device__ __forceinline__ void put(int r, int group, int part, const Mx8<T>& v) const {
+    const uint32_t byte = mx_scale_byte(quad_max(v.amax()));
+    reinterpret_cast<uint32_t*>(codes)[(group * rows + r) * 4 + part] = v.codes(mx_scale_value(byte));
+    if (part == 0) scales[group * rows + r] = (uint8_t)byte;
   }
   // ... or codes as they are.
   __device__ __forceinline__ void put(int r, int group, const uint8_t* row_codes, const uint8_t* row_scales) const {
@@ -196,30 +203,38 @@ __device__ __forceinline__ f32x4_t mx_quarter(const f32x16_t& v, int q) { return
 // last again, not to be stored) and up to 32 activation rows: RUN chunks of weights are asked for ahead of the RUN that are multiplied.
 template <int NT, int RUN>
 struct MxStream {
-  const uint8_t *codes[NT], *scales[NT];
+  __amdgpu_buffer_rsrc_t codes, scales;  // of the NT tiles
+  int code_at[NT], scale_at[NT];
   i32x4_t b[RUN][NT];
   uint32_t sb[NT];
   int c0, c1;
   f32x16_t acc[NT];
-  __device__ __forceinline__ MxStream(const uint8_t* __restrict__ w, const MxLayout& at, int t0, int wave, int waves) {
-    const int lane = threadIdx.x & 63, runs = (at.chunks + RUN - 1) / RUN;
+  // The first run is on its way from here.
+  __device__ __forceinline__ void begin(const uint8_t* matrix, const MxLayout& at, int t0, int wave, int waves) {
+    const int tiles = min(NT, at.tiles - t0);
+    codes = mx_rows(matrix + (int64_t)t0 * at.chunks * 1024, (uint32_t)tiles * at.chunks * 1024);
+    scales = mx_rows(matrix + at.codes() + (int64_t)t0 * at.quads * 256, (uint32_t)tiles * at.quads * 256);
+    const int runs = (at.chunks + RUN - 1) / RUN;
     c0 = RUN * (runs * wave / waves);
     c1 = min(at.chunks, RUN * (runs * (wave + 1) / waves));
 #pragma unroll
     for (int t = 0; t < NT; t++) {
-      const int tile = min(t0 + t, at.tiles - 1);
-      codes[t] = w + (int64_t)tile * at.chunks * 1024 + lane * 16;
-      scales[t] = w + at.codes() + (int64_t)tile * at.quads * 256 + lane * 4;
+      const int tile = min(t, at.tiles - 1 - t0);
+      code_at[t] = tile * at.chunks * 1024;
+      scale_at[t] = tile * at.quads * 256;
     }
     ask(min(c0, at.chunks - 1));
   }
+  // (no reuse: every weight byte is read once; chunks past the end are asked for again and not multiplied)
   __device__ __forceinline__ void ask(int c) {
+    const uint32_t lane = threadIdx.x & 63;
 #pragma unroll
-    for (int t = 0; t < NT; t++) sb[t] = *reinterpret_cast<const uint32_t*>(scales[t] + (c >> 2) * 256);
+    for (int t = 0; t < NT; t++) sb[t] = __builtin_amdgcn_raw_buffer_load_b32(scales, lane * 4, scale_at[t] + (c >> 2) * 256, 0);
 #pragma unroll
     for (int u = 0; u < RUN; u++)
 #pragma unroll
-      for (int t = 0; t < NT; t++) b[u][t] = *reinterpret_cast<const i32x4_t*>(codes[t] + min(c + u, max(c1 - 1, 0)) * 1024);  // (past the end: asked for again, not multiplied)
+      for (int t = 0; t < NT; t++)
+        b[u][t] = __builtin_bit_cast(i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(codes, lane * 16, code_at[t] + min(c + u, max(c1 - 1, 0)) * 1024, MX_NO_REUSE));
   }
   template <int U>
   __device__ __forceinline__ void step(const i32x4_t (&w)[RUN][NT], const uint32_t (&sw)[NT], const i32x4_t& a, uint32_t sa) {

@@ -104,17 +104,20 @@ __device__ __forceinline__ void mx_finish_h(const MxMoe& p, f32x4_t* part, uint3
 // fc1: a workgroup two weight tiles of the slot that begins at pair blockIdx.y (none: it leaves). The slot's expert is known from one
 // id, so the weights are on their way while the slot's rows are looked for and their activations rounded into LDS.
 constexpr int MX_FEW_WAVES = 8;
-template <int RUN, class Values>
+// PARTS lanes a group: values(acts, row of the slot, group, part, pair) puts it there.
+template <int RUN, int PARTS, class Values>
 __device__ __forceinline__ int mx_few_product(const MxMoe& p, f32x4_t* part, int& list, Values&& values) {
   const int first = blockIdx.y, id = p.ids[first], e = id - p.base;
   if (e < 0 || e >= p.experts) return 0;
-  MxStream<MX_MOE_TILES, RUN> s(p.w + e * p.expert_bytes, MxLayout(p.n, p.k), blockIdx.x * MX_MOE_TILES, __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), MX_FEW_WAVES);
+  MxStream<MX_MOE_TILES, RUN> s;
+  s.begin(p.w + e * p.expert_bytes, MxLayout(p.n, p.k), blockIdx.x * MX_MOE_TILES, __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), MX_FEW_WAVES);
   const int rows = mx_slot_of(p, id, first, list);
   if (rows == 0) return 0;
   const MxActs acts(part, rows, p.k);
-  for (int i = threadIdx.x; i < (rows * acts.groups + 63) / 64 * 64; i += 64 * MX_FEW_WAVES) {  // whole wavefronts: `list` lies across the lanes
-    const int r = i / acts.groups, group = i - r * acts.groups, pair = __shfl(list, min(r, rows - 1));
-    if (r < rows) values(acts, r, group, pair);
+  const int all = rows * acts.groups * PARTS;
+  for (int i = threadIdx.x; i < (all + 63) / 64 * 64; i += 64 * MX_FEW_WAVES) {  // whole wavefronts: `list` lies across the lanes
+    const int r = i / PARTS / acts.groups, group = i / PARTS - r * acts.groups, pair = __shfl(list, min(r, rows - 1));
+    if (i < all) values(acts, r, group, i % PARTS, pair);
   }
   __syncthreads();
   s.run(acts);
@@ -126,8 +129,10 @@ template <bool GATED, int RUN>
 __global__ __launch_bounds__(64 * MX_FEW_WAVES, RUN == 4 ? 2 : 4) void mx_fc1_few_kernel(MxMoe p) {
   extern __shared__ f32x4_t part[];
   int list;
-  const int rows = mx_few_product<RUN>(p, part, list, [&](const MxActs& acts, int r, int group, int pair) {
-    acts.put(r, group, static_cast<const __bf16*>(p.x) + (int64_t)(pair / p.topk) * p.k + MX_GROUP * group);
+  const int rows = mx_few_product<RUN, 4>(p, part, list, [&](const MxActs& acts, int r, int group, int quarter, int pair) {
+    Mx8<__bf16> v;
+    v.load(static_cast<const __bf16*>(p.x) + (int64_t)(pair / p.topk) * p.k + MX_GROUP * group + 8 * quarter);
+    acts.put(r, group, quarter, v);
   });
   if (rows == 0) return;
   const int r = threadIdx.x & 31, upper = threadIdx.x >> 8;  // the threads' upper half: the second tile where each is 32 columns
@@ -143,7 +148,7 @@ template <typename Y, int RUN>
 __global__ __launch_bounds__(64 * MX_FEW_WAVES, RUN == 4 ? 2 : 4) void mx_fc2_few_kernel(MxMoe p) {
   extern __shared__ f32x4_t part[];
   int list;
-  const int rows = mx_few_product<RUN>(p, part, list, [&](const MxActs& acts, int r, int group, int pair) {
+  const int rows = mx_few_product<RUN, 1>(p, part, list, [&](const MxActs& acts, int r, int group, int, int pair) {
     acts.put(r, group, p.aq + (int64_t)pair * (p.k / 2), p.as + (int64_t)pair * acts.groups);
   });
   const int r = threadIdx.x & 31, pair = __shfl(list, r);
@@ -286,7 +291,7 @@ struct MxWalk {
     for (int t = 0; t < NT; t++) {
       const int tile = min(t0 + t, at.tiles - 1), of = tile * at.chunks * 1024, s = (int)at.codes() + (tile * at.quads + (c >> 2)) * 256;
 #pragma unroll
-      for (int u = 0; u < MX_STEP; u++) b[u][t] = __builtin_bit_cast(i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(w, lane * 16, of + min(c + u, at.chunks - 1) * 1024, 2));
+      for (int u = 0; u < MX_STEP; u++) b[u][t] = __builtin_bit_cast(i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(w, lane * 16, of + min(c + u, at.chunks - 1) * 1024, MX_NO_REUSE));
 #pragma unroll
       for (int u = 0; u < MX_STEP / 4; u++) sb[u][t] = __builtin_amdgcn_raw_buffer_load_b32(w, lane * 4, s + u * 256, 0);
     }
@@ -467,6 +472,7 @@ int check(const hb_mxfp4_experts* ex) {
   if (ex->experts <= 0 || ex->base < 0 || ex->hidden <= 0 || ex->inter <= 0 || ex->hidden_out <= 0 || ex->hidden % 32 || ex->inter % 32 || ex->hidden_out % 8 ||
       ex->hidden > 1 << 20 || ex->inter > 1 << 20 || ex->hidden_out > 1 << 20 || ex->experts > 1 << 20 || ex->base > 1 << 28)
     return HB_EINVAL;
+  if (MxLayout(fc1_rows(ex), ex->hidden).bytes() >= (int64_t)1 << 31 || MxLayout(ex->hidden_out, ex->inter).bytes() >= (int64_t)1 << 31) return HB_EINVAL;  // offsets in one matrix
   return aligned(ex->fc1, 16) && aligned(ex->fc2, 16) ? HB_OK : HB_EINVAL;
 }
 }  // namespace

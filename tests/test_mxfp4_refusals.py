@@ -28,7 +28,7 @@ def test_the_library_refuses_before_a_launch():
     need = lib.hb_mxfp4_linear_workspace_bytes(4, 64, 128, 0)
     call = lambda **c: lib.hb_mxfp4_linear(*{**dict(x=256, xs=None, kind=0, m=4, w=256, n=64, k=128, y=256, to=0, ws=256, size=max(need, 1 << 20), stream=None), **c}.values())  # noqa: E731
     assert call(x=None) == call(w=None) == call(y=None) == call(kind=3) == _lib.HB_ENULL
-    for c in [dict(m=0), dict(m=(1 << 19) + 1), dict(n=0), dict(k=33), dict(kind=1), dict(kind=4), dict(to=3), dict(x=264), dict(w=257), dict(y=257)]:
+    for c in [dict(m=0), dict(m=(1 << 24) + 1), dict(n=0), dict(k=33), dict(kind=1), dict(kind=4), dict(to=3), dict(x=264), dict(w=257), dict(y=257)]:
         assert call(**c) == _lib.HB_EINVAL, c
 
 
