@@ -39,7 +39,7 @@ struct MxLayout {
   __host__ __device__ int64_t bytes() const { return codes() + (int64_t)tiles * quads * 256; }
 };
 
-constexpr int MX_NO_REUSE = 2;  // the cache policy of loads whose bytes nobody reads again
+constexpr int MX_NO_REUSE = 2;  // the cache policy of loads whose bytes are not read again soon
 // A buffer descriptor in scalar registers: what is read past `bytes` is zero.
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t mx_rows(const uint8_t* base, uint32_t bytes) {
   const uint64_t at = reinterpret_cast<uint64_t>(base);
@@ -225,7 +225,7 @@ struct MxStream {
     }
     ask(min(c0, at.chunks - 1));
   }
-  // (no reuse: every weight byte is read once; chunks past the end are asked for again and not multiplied)
+  // (chunks past the end are asked for again and not multiplied)
   __device__ __forceinline__ void ask(int c) {
     const uint32_t lane = threadIdx.x & 63;
 #pragma unroll
@@ -234,7 +234,7 @@ struct MxStream {
     for (int u = 0; u < RUN; u++)
 #pragma unroll
       for (int t = 0; t < NT; t++)
-        b[u][t] = __builtin_bit_cast(i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(codes, lane * 16, code_at[t] + min(c + u, max(c1 - 1, 0)) * 1024, MX_NO_REUSE));
+        b[u][t] = __builtin_bit_cast(i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(codes, lane * 16, code_at[t] + min(c + u, max(c1 - 1, 0)) * 1024, 0));
   }
   template <int U>
   __device__ __forceinline__ void step(const i32x4_t (&w)[RUN][NT], const uint32_t (&sw)[NT], const i32x4_t& a, uint32_t sa) {
