@@ -273,6 +273,7 @@ struct MxTiles {
   void* y;               // K shared by gridDim.y workgroups: their FP32 sums [shares, m, n]
   int64_t m, n;
   int k, rows_of_tiles;  // workgroups along m
+  int first, last;       // the tiles of weight rows that this launch covers
 };
 typedef __attribute__((address_space(3))) uint8_t* mx_lds_t;
 
@@ -338,7 +339,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void mx_ring_kernel(MxTiles p) {
   // consecutive workgroups go to the eight dies in turn: each die walks a run of tiles, rows fastest, so that its L2 keeps a run of weights
   const int total = gridDim.x, per = (total + 7) / 8, die = blockIdx.x % 8, whole = total % 8 ? total % 8 : 8;  // the first `whole` dies have `per` workgroups, the others one less
   const int at = die * per - (die > whole ? die - whole : 0) + (int)(blockIdx.x / 8);
-  const int a0 = at % p.rows_of_tiles * TA, b0 = at / p.rows_of_tiles * TB, chunks = la.chunks, row_bytes = chunks * 1024;
+  const int a0 = at % p.rows_of_tiles * TA, b0 = p.first + at / p.rows_of_tiles * TB, chunks = la.chunks, row_bytes = chunks * 1024;
   const int pairs = la.quads / 2, q0 = 2 * (int)((int64_t)pairs * blockIdx.y / gridDim.y), q1 = 2 * (int)((int64_t)pairs * (blockIdx.y + 1) / gridDim.y);
   p.y = static_cast<Y*>(p.y) + (int64_t)blockIdx.y * p.m * p.n;
 
@@ -494,6 +495,7 @@ struct MxPlan {
 // 17.3; 5120 x 5120: 8 rows 8.6 inside, 14.4 ring; 16 rows 10.6 inside, 7.4 and 2 for a launch of its own, 14.3 ring.
 constexpr int64_t MX_ROUND_VALUES = 48 * 1024;
 constexpr int MX_RING_TILES = 768;
+constexpr int MX_DEVICE = 256;  // compute units
 static MxPlan plan_of(int64_t m, int64_t n, int k, int x_type) {
   const MxLayout rows(m, k), w(n, k);
   MxPlan p{};
@@ -522,8 +524,9 @@ static MxPlan plan_of(int64_t m, int64_t n, int k, int x_type) {
 template <typename Y, int WM, int WN, int MT, int NT>
 static int launch_ring(MxTiles p, const MxPlan& plan, float* sums, hipStream_t stream) {
   const MxLayout la(p.m, p.k), lw(p.n, p.k);
+  if (!p.last) p.last = lw.tiles;
   p.rows_of_tiles = (la.tiles + WM * MT - 1) / (WM * MT);
-  const dim3 grid((unsigned)(p.rows_of_tiles * ((lw.tiles + WN * NT - 1) / (WN * NT))), (unsigned)plan.shares);
+  const dim3 grid((unsigned)(p.rows_of_tiles * ((p.last - p.first + WN * NT - 1) / (WN * NT))), (unsigned)plan.shares);
   if (plan.shares == 1) {
     HB_LAUNCH((mx_ring_kernel<Y, WM, WN, MT, NT>), grid, dim3(64 * WM * WN), 0, stream, p);
     return HB_OK;
@@ -577,8 +580,22 @@ static int launch_linear(MxLinear p, uint8_t* workspace, hipStream_t stream) {
     const MxLayout rows(p.m, p.k);
     HB_LAUNCH((mx_quantize_tiles_kernel<T>), dim3((unsigned)((int64_t)rows.tiles * rows.quads)), dim3(256), 0, stream, static_cast<const T*>(p.x), p.m, p.k, workspace);
   }
-  const MxTiles q{workspace, p.w, p.y, p.m, p.n, p.k, 0};
+  MxTiles q{workspace, p.w, p.y, p.m, p.n, p.k, 0, 0, 0};
   float* sums = reinterpret_cast<float*>(workspace + plan.tiles);
+  if (plan.square && plan.mt == 4) {
+    // The last columns of workgroups, those past whole rounds of the device, as four workgroups of 128 x 128 each in a launch behind: a
+    // round of a few large ones costs as much as a full one. 2048 rows of 25600 x 5120 (3.125 rounds): 162 us as one launch, 152 so.
+    const MxLayout rows(p.m, p.k), w(p.n, p.k);
+    const int high = (rows.tiles + 7) / 8, wide = (w.tiles + 7) / 8, whole = high * wide / MX_DEVICE * MX_DEVICE / high;
+    const int rest = (high * wide - whole * high) * 4;
+    if (whole && rest && rest <= 2 * MX_DEVICE) {
+      q.last = whole * 8;
+      if (int e = launch_ring<Y, 2, 2, 4, 4>(q, plan, sums, stream)) return e;
+      q.first = whole * 8;
+      q.last = w.tiles;
+      return launch_ring<Y, 2, 2, 2, 2>(q, plan, sums, stream);
+    }
+  }
   if (plan.square) return plan.mt == 4 ? launch_ring<Y, 2, 2, 4, 4>(q, plan, sums, stream) : launch_ring<Y, 2, 2, 2, 2>(q, plan, sums, stream);
   switch (plan.mt) {
     case 1: return launch_ring<Y, 1, 4, 1, 1>(q, plan, sums, stream);

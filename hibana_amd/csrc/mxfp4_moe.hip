@@ -49,13 +49,12 @@ __device__ __forceinline__ int mx_slot_of(const MxMoe& p, int id, int first, int
   return min(MX_ROWS, (int)__popcll(same) - before);
 }
 
-// h of 32 x 32 values (row r of the slot, columns from 32 `column`) from the joined sums of up (and gate), rounded to the format: 256 threads, thread
-// i = 64 q + lane (of every 256) holds row lane % 32, columns 8 q + 4 (lane / 32) .. + 3. `tops`: a word of LDS a thread that nobody else uses up to
-// the next barrier.
+// h of 32 x 32 values (row r of the slot, 32 columns) from the joined sums of up (and gate), rounded to the format: of every 256 threads, thread
+// i = 64 q + lane holds row lane % 32, columns 8 q + 4 (lane / 32) .. + 3. In two halves with a barrier between: a thread's largest magnitude goes to
+// its word of `tops` (LDS), then the group's gives the scale.
 template <bool GATED>
-__device__ __forceinline__ void mx_emit_h(const MxMoe& p, const f32x4_t& up, const f32x4_t& gate, int column, bool real, int64_t pos, uint32_t* tops) {
-  const int lane = threadIdx.x & 63, r = lane & 31, g = lane >> 5, q = (threadIdx.x >> 6) & 3;
-  float h[4];
+__device__ __forceinline__ f32x4_t mx_h(const f32x4_t& up, const f32x4_t& gate, uint32_t* tops) {
+  f32x4_t h;
   uint32_t top = 0;
 #pragma unroll
   for (int j = 0; j < 4; j++) {
@@ -64,8 +63,12 @@ __device__ __forceinline__ void mx_emit_h(const MxMoe& p, const f32x4_t& up, con
     top = max(top, __float_as_uint(h[j]) & 0x7fffffffu);
   }
   tops[threadIdx.x] = top;
-  __syncthreads();
+  return h;
+}
+__device__ __forceinline__ void mx_emit_h(const MxMoe& p, const f32x4_t& h, int column, bool real, int64_t pos, const uint32_t* tops) {
+  const int lane = threadIdx.x & 63, r = lane & 31, g = lane >> 5, q = (threadIdx.x >> 6) & 3;
   const uint32_t* of = tops + (threadIdx.x & ~255);
+  uint32_t top = 0;
 #pragma unroll
   for (int v = 0; v < 4; v++) top = max(top, max(of[v * 64 + r], of[v * 64 + 32 + r]));
   const uint32_t byte = mx_scale_byte(top);
@@ -73,30 +76,15 @@ __device__ __forceinline__ void mx_emit_h(const MxMoe& p, const f32x4_t& up, con
   uint32_t c = 0;
   c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, h[0], h[1], s, 0);
   c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, h[2], h[3], s, 1);
-  if (real && column < p.inter / 32) {
-    *reinterpret_cast<uint16_t*>(p.hq + pos * (p.inter / 2) + 16 * column + 4 * q + 2 * g) = byte == 255u ? 0 : (uint16_t)c;
-    if (q == 0 && g == 0) {
-      if (p.plan) {
-        uint8_t* at = p.hs + pos * mx_scale_row(p.inter);
-        at[mx_scale_at(column)] = (uint8_t)byte;
-        if (column == p.inter / 32 - 1 && !(column & 1)) at[mx_scale_at(column + 1)] = 0;
-      } else {
-        p.hs[pos * (p.inter / 32) + column] = (uint8_t)byte;
-      }
-    }
-  }
-}
-
-// The two tiles of a workgroup as h: gated, an up and a gate tile are 32 columns; else each tile is 32. `part`: [waves][2 * 4][64], read by
-// all behind a barrier that has passed.
-template <bool GATED>
-__device__ __forceinline__ void mx_finish_h(const MxMoe& p, f32x4_t* part, uint32_t* tops, int unit, bool real, int64_t pos) {
-  const f32x4_t first = mx_joined<2>(part, MX_MOE_WAVES, threadIdx.x), second = mx_joined<2>(part, MX_MOE_WAVES, 256 + threadIdx.x);
-  if (GATED) {
-    mx_emit_h<true>(p, first, second, unit, real, pos, tops);
+  if (!real || column >= p.inter / 32) return;
+  *reinterpret_cast<uint16_t*>(p.hq + pos * (p.inter / 2) + 16 * column + 4 * q + 2 * g) = byte == 255u ? 0 : (uint16_t)c;
+  if (q || g) return;
+  if (p.plan) {
+    uint8_t* at = p.hs + pos * mx_scale_row(p.inter);
+    at[mx_scale_at(column)] = (uint8_t)byte;
+    if (column == p.inter / 32 - 1 && !(column & 1)) at[mx_scale_at(column + 1)] = 0;
   } else {
-    mx_emit_h<false>(p, first, first, 2 * unit, real, pos, tops);
-    mx_emit_h<false>(p, second, second, 2 * unit + 1, real, pos, tops + 256);
+    p.hs[pos * (p.inter / 32) + column] = (uint8_t)byte;
   }
 }
 
@@ -140,7 +128,10 @@ __global__ __launch_bounds__(64 * MX_FEW_WAVES, RUN == 4 ? 2 : 4) void mx_fc1_fe
   const f32x4_t gate = GATED ? mx_joined<MX_MOE_TILES>(part, MX_FEW_WAVES, 256 + (threadIdx.x & 255)) : up;
   const int pair = __shfl(list, r);
   __syncthreads();  // the sums are read: their place takes the quarters' largest magnitudes
-  mx_emit_h<GATED>(p, up, gate, GATED ? blockIdx.x : 2 * blockIdx.x + upper, r < rows && (!GATED || !upper), pair, reinterpret_cast<uint32_t*>(part));
+  uint32_t* tops = reinterpret_cast<uint32_t*>(part);
+  const f32x4_t h = mx_h<GATED>(up, gate, tops);
+  __syncthreads();
+  mx_emit_h(p, h, GATED ? blockIdx.x : 2 * blockIdx.x + upper, r < rows && (!GATED || !upper), pair, tops);
 }
 
 // fc2 of the same slots, its results by pair.
@@ -284,23 +275,25 @@ struct MxWalk {
     }
   }
   __device__ __forceinline__ int steps() const { return max(1, (c1 - c0 + MX_STEP - 1) / MX_STEP); }
-  // (chunks past the share's end are asked for where they are in the matrix, and not multiplied)
+  // (chunks past the share's end: the last again, which costs no trip to memory, and not multiplied)
   __device__ __forceinline__ void ask_weights(int t0, int c) {
     const uint32_t lane = threadIdx.x & 63;
+    const int last = max(c1 - 1, 0);
 #pragma unroll
     for (int t = 0; t < NT; t++) {
       const int tile = min(t0 + t, at.tiles - 1), of = tile * at.chunks * 1024, s = (int)at.codes() + (tile * at.quads + (c >> 2)) * 256;
 #pragma unroll
-      for (int u = 0; u < MX_STEP; u++) b[u][t] = __builtin_bit_cast(i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(w, lane * 16, of + min(c + u, at.chunks - 1) * 1024, MX_NO_REUSE));
+      for (int u = 0; u < MX_STEP; u++) b[u][t] = __builtin_bit_cast(i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(w, lane * 16, of + min(c + u, last) * 1024, MX_NO_REUSE));
 #pragma unroll
       for (int u = 0; u < MX_STEP / 4; u++) sb[u][t] = __builtin_amdgcn_raw_buffer_load_b32(w, lane * 4, s + u * 256, 0);
     }
   }
   __device__ __forceinline__ void ask_acts(int c) {
+    const int last = max(c1 - 1, 0);
 #pragma unroll
     for (int i = 0; i < MT; i++) {
 #pragma unroll
-      for (int u = 0; u < MX_STEP; u++) a[u][i] = __builtin_bit_cast(i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(ac, code_at[i], min(c + u, at.chunks - 1) * 32, 0));
+      for (int u = 0; u < MX_STEP; u++) a[u][i] = __builtin_bit_cast(i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(ac, code_at[i], min(c + u, last) * 32, 0));
 #pragma unroll
       for (int u = 0; u < MX_STEP / 4; u++) sa[u][i] = __builtin_amdgcn_raw_buffer_load_b32(as, scale_at[i], ((c >> 2) + u) * 8, 0);
     }
@@ -328,30 +321,33 @@ struct MxWalk {
 };
 
 // The plan's slot of this workgroup and its span of units (two tiles each): p.span of them, from p.span blockIdx.x.
-// fc1: K split among the wavefronts.
-template <bool GATED, int MT>
+// fc1: KS wavefronts share a unit's K, as many as leave each about a step of it; the workgroup's 4 / KS groups of them have units of their own, whose
+// sums become h together.
+template <bool GATED, int MT, int KS>
 __global__ __launch_bounds__(64 * MX_MOE_WAVES, MT == 1 ? 3 : 2) void mx_fc1_many_kernel(MxMoe p) {
+  constexpr int SUBS = MX_MOE_WAVES / KS, PER = GATED ? 1 : 2;  // groups of wavefronts; 32 columns of h a unit
   __shared__ f32x4_t part[MX_MOE_WAVES * MX_MOE_TILES * 256];
-  __shared__ uint32_t tops[GATED ? 256 : 512];
+  __shared__ uint32_t tops[SUBS * PER * 256];
   const int32_t* entry = p.plan + PLAN_HEADER + 4 * (int)blockIdx.y;
   const int rows = entry[2], p0 = entry[1];
   if (rows == 0) return;
   const MxLayout at(p.n, p.k);
-  const int units = (at.tiles + MX_MOE_TILES - 1) / MX_MOE_TILES, first = blockIdx.x * p.span, last = min(first + p.span, units);
-  MxWalk<MT> walk(p, at, p.w + entry[0] * p.expert_bytes, rows, (uint32_t)(p.pairs / p.topk), __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), MX_MOE_WAVES, [&](int r) { return (uint32_t)(p.order[p0 + r] / p.topk); });
+  const int units = (at.tiles + MX_MOE_TILES - 1) / MX_MOE_TILES, first = blockIdx.x * p.span * SUBS, last = min(first + p.span * SUBS, units);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), sub = wave / KS;
+  MxWalk<MT> walk(p, at, p.w + entry[0] * p.expert_bytes, rows, (uint32_t)(p.pairs / p.topk), wave % KS, KS, [&](int r) { return (uint32_t)(p.order[p0 + r] / p.topk); });
   const int steps = walk.steps();
-  walk.ask_weights(first * MX_MOE_TILES, walk.c0);
+  walk.ask_weights((first + sub) * MX_MOE_TILES, walk.c0);
   walk.ask_acts(walk.c0);
-  for (int unit = first; unit < last; unit++) {
+  for (int unit = first; unit < last; unit += SUBS) {
     walk.clear();
     for (int s = 0; s < steps; s++) {
       const int c = walk.c0 + s * MX_STEP;
       walk.multiply(c);
       if (s + 1 < steps) {
-        walk.ask_weights(unit * MX_MOE_TILES, c + MX_STEP);
+        walk.ask_weights((unit + sub) * MX_MOE_TILES, c + MX_STEP);
         walk.ask_acts(c + MX_STEP);
-      } else if (unit + 1 < last) {
-        walk.ask_weights((unit + 1) * MX_MOE_TILES, walk.c0);
+      } else if (unit + SUBS < last) {
+        walk.ask_weights((unit + SUBS + sub) * MX_MOE_TILES, walk.c0);
         if (steps > 1) walk.ask_acts(walk.c0);
       }
     }
@@ -359,8 +355,17 @@ __global__ __launch_bounds__(64 * MX_MOE_WAVES, MT == 1 ? 3 : 2) void mx_fc1_man
     for (int i = 0; i < MT; i++) {
       if (32 * i >= rows) break;
       mx_hand_over<MX_MOE_TILES>(part, walk.acc[i]);
+      f32x4_t h[SUBS * PER];
+#pragma unroll
+      for (int e = 0; e < SUBS * PER; e++) {
+        const f32x4_t* of = part + e / PER * KS * MX_MOE_TILES * 256;
+        const f32x4_t up = mx_joined<MX_MOE_TILES>(of, KS, 256 * (e % PER) + threadIdx.x);
+        h[e] = mx_h<GATED>(up, GATED ? mx_joined<MX_MOE_TILES>(of, KS, 256 + threadIdx.x) : up, tops + 256 * e);
+      }
+      __syncthreads();
       const int r = 32 * i + (threadIdx.x & 31);
-      mx_finish_h<GATED>(p, part, tops, unit, r < rows, p0 + r);
+#pragma unroll
+      for (int e = 0; e < SUBS * PER; e++) mx_emit_h(p, h[e], PER * (unit + e / PER) + e % PER, r < rows, p0 + r, tops + 256 * e);
     }
   }
 }
@@ -577,10 +582,20 @@ extern "C" int hb_mxfp4_moe(const hb_mxfp4_experts* experts, const void* x, cons
       p.span = span_of(units, by);
       HB_LAUNCH(kernel, dim3((units + by * p.span - 1) / (by * p.span), (unsigned)slots), dim3(64 * MX_MOE_WAVES), 0, s, p);
     };
+    auto fc1 = [&](auto gated) {
+      constexpr bool G = decltype(gated)::value;
+      if (l1.chunks <= MX_STEP) {
+        launch(tall ? mx_fc1_many_kernel<G, 2, 1> : mx_fc1_many_kernel<G, 1, 1>, groups1, 4, p1);
+      } else if (l1.chunks <= 2 * MX_STEP) {
+        launch(tall ? mx_fc1_many_kernel<G, 2, 2> : mx_fc1_many_kernel<G, 1, 2>, groups1, 2, p1);
+      } else {
+        launch(tall ? mx_fc1_many_kernel<G, 2, 4> : mx_fc1_many_kernel<G, 1, 4>, groups1, 1, p1);
+      }
+    };
     if (experts->gated) {
-      launch(tall ? mx_fc1_many_kernel<true, 2> : mx_fc1_many_kernel<true, 1>, groups1, 1, p1);
+      fc1(std::true_type());
     } else {
-      launch(tall ? mx_fc1_many_kernel<false, 2> : mx_fc1_many_kernel<false, 1>, groups1, 1, p1);
+      fc1(std::false_type());
     }
     const bool own = l2.chunks <= 2 * MX_STEP;
     auto fc2 = [&](auto* type) {
