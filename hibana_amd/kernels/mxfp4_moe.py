@@ -67,6 +67,10 @@ class Mxfp4Experts:
         """Stacked BF16, FP16 or FP32 matrices, rounded to the format."""
         return cls(*mxfp4.quantize(fc1), *mxfp4.quantize(fc2), base=base)
 
+    def __call__(self, x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor) -> torch.Tensor:
+        """`mxfp4_moe`, as a block that takes any experts calls it (`NemotronMoe`, its routed scaling factor in fc2 or the weights)."""
+        return mxfp4_moe(self, x, ids, weights)
+
 
 def tile(experts: Mxfp4Experts, release: bool = False) -> Mxfp4Experts:
     """Build the kernels' layout of both stacks (once); `release` drops the tensors by rows."""

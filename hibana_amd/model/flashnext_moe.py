@@ -9,6 +9,9 @@
                                                                than w3.MAX_ROWS rows, or HIBANA_W3_DECODE off - run on them)
     out     = bf16(bf16(routed) + sigmoid(x . shared_gate_vec) * shared)
 
+Routed experts in the microscaled four-bit format (`Mxfp4Experts`, their activations four bits wide too) take the 3-bit ones' place
+where they are given: `mxfp4_moe`, the shared expert on its two linears (`Mlp`: `Mxfp4Linear` or `Nvfp4Linear`), the combine over both.
+
 The block is assembled from tensors already on the device (a loader's job ends there). The routed experts are a
 `W3Experts`; the shared expert is either a one-expert `W3Experts` or the pair of linears the reference holds
 (`shared_gate_up` with rows [gate; up], `shared_down`), whose 3-bit copies are re-stored once, at construction, in the
@@ -21,7 +24,10 @@ from __future__ import annotations
 
 import torch
 
-from hibana_amd.kernels import ops, w3, w3_moe
+from hibana_amd.kernels import mxfp4_moe, ops, w3, w3_moe
+from hibana_amd.model.mlp import Mlp
+from hibana_amd.weights.modelopt import Nvfp4Linear
+from hibana_amd.weights.mxfp4 import Mxfp4Linear
 
 
 def shared_from_linears(gate_up: w3.W3Weight, down: w3.W3Weight) -> w3_moe.W3Experts:
@@ -45,10 +51,10 @@ class MoeLayer:
     MIN_GUARANTEE = 2  # hibana/model/flashnext/moe.py:146-149
     MIN_CAP = 16
 
-    def __init__(self, router: torch.Tensor, shared_gate: torch.Tensor, experts: w3_moe.W3Experts, topk: int, shared: w3_moe.W3Experts | None = None,
+    def __init__(self, router: torch.Tensor, shared_gate: torch.Tensor, experts: w3_moe.W3Experts | mxfp4_moe.Mxfp4Experts, topk: int, shared: w3_moe.W3Experts | None = None,
                  shared_gate_up=None, shared_down=None, keep: int = 0, budget: int = 0, per_request: int = 0):
-        """router BF16 [E, H]; shared_gate [1, H] or [H] (the shared expert's sigmoid gate); `experts` this rank's 3-bit
-        experts (a range base .. base + experts - 1 of the E); the shared expert as `shared`, or as the two linears
+        """router BF16 [E, H]; shared_gate [1, H] or [H] (the shared expert's sigmoid gate); `experts` this rank's 3-bit (or
+        microscaled four-bit) experts (a range base .. base + experts - 1 of the E); the shared expert as `shared`, or as the two linears
         `shared_gate_up` / `shared_down` with 3-bit copies attached (`.w3`). `keep` (below topk; topk or more, or 0, is
         the served route): each token's own top experts in decode and verify forwards; with `budget`, the cap on the
         distinct experts such a forward reads, `per_request` its share a request
@@ -63,6 +69,11 @@ class MoeLayer:
         self.per_request = per_request
         self.shared_gate = shared_gate.float().reshape(1, -1).contiguous()
         self.shared_gate_vec = self.shared_gate.reshape(-1)
+        self.w3 = self.mxfp4 = self.shared = self.shared_mlp = None
+        self.shared_gate_up, self.shared_down = shared_gate_up, shared_down
+        if isinstance(experts, mxfp4_moe.Mxfp4Experts):
+            self._take_mxfp4(experts, shared)
+            return
         self.w3 = w3_moe.tile(experts)
         if experts.base + experts.experts > self.experts:
             raise ValueError(f"3-bit experts {experts.base}..{experts.base + experts.experts - 1}: the model has {self.experts}")
@@ -73,15 +84,29 @@ class MoeLayer:
             else:
                 shared = shared_from_linears(shared_gate_up.w3, shared_down.w3)
         self.shared = None if shared is None else w3_moe.tile(shared)
-        self.shared_gate_up, self.shared_down = shared_gate_up, shared_down
+
+    def _take_mxfp4(self, experts: mxfp4_moe.Mxfp4Experts, shared) -> None:
+        if experts.base + experts.experts > self.experts:
+            raise ValueError(f"experts {experts.base}..{experts.base + experts.experts - 1}: the model has {self.experts}")
+        if experts.shape1[2] != self.hidden or experts.shape2[1] != self.hidden:
+            raise ValueError(f"MoeLayer: the experts' inputs and outputs are rows of {experts.shape1[2]} and {experts.shape2[1]}, the router's of {self.hidden}")
+        linears = (self.shared_gate_up, self.shared_down)
+        if shared is not None or any(lin is not None for lin in linears) and not all(isinstance(lin, (Mxfp4Linear, Nvfp4Linear)) for lin in linears):
+            raise ValueError("MoeLayer: the shared expert beside microscaled four-bit experts is two linears, Mxfp4Linear or Nvfp4Linear")
+        if linears[0] is not None:
+            if linears[0].in_features != self.hidden:
+                raise ValueError(f"MoeLayer: a shared expert on rows of {linears[0].in_features}, the router's of {self.hidden}")
+            self.shared_mlp = Mlp(*linears)
+        self.mxfp4 = mxfp4_moe.tile(experts)
 
     @property
     def expert_bytes(self) -> int:
-        return self.w3.bytes
+        return (self.w3 if self.mxfp4 is None else self.mxfp4).bytes
 
     @property
     def bytes(self) -> int:
-        return self.expert_bytes + self.router.numel() * 2 + (self.shared.bytes if self.shared is not None else 0)
+        shared = self.shared.bytes if self.shared is not None else self.shared_gate_up.bytes + self.shared_down.bytes if self.shared_mlp is not None else 0
+        return self.expert_bytes + self.router.numel() * 2 + shared
 
     @staticmethod
     def _padding(ctx):
@@ -119,6 +144,8 @@ class MoeLayer:
 
     def routed(self, x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor) -> torch.Tensor:
         """The routed experts' weighted sum (this rank's part) for x [M, H] -> BF16 [M, H]."""
+        if self.mxfp4 is not None:
+            return mxfp4_moe.mxfp4_moe(self.mxfp4, x, ids, weights)
         return w3_moe.w3_moe(self.w3, x, ids, weights, experts_total=self.experts)
 
     def shared_on_linears(self, m: int) -> bool:
@@ -133,6 +160,12 @@ class MoeLayer:
 
     def __call__(self, x: torch.Tensor, ctx=None) -> torch.Tensor:
         x = x.contiguous()
+        if self.mxfp4 is not None:
+            ids, weights = self.route(x, ctx)
+            if self.shared_mlp is None:
+                return self.routed(x, ids, weights)
+            pairs = mxfp4_moe.mxfp4_moe(self.mxfp4, x, ids, weights, pairs=True, pairs_bf16=x.shape[0] >= w3_moe.WIDE_ROWS)
+            return ops.moe_combine_pairs(pairs, ids, weights, self.shared_mlp(x), x, self.shared_gate_vec, self.mxfp4.base, self.mxfp4.experts)
         if self.shared_on_linears(x.shape[0]):
             # the reference's own chain: the experts' unsummed pair outputs (BF16 from WIDE_ROWS rows), the shared expert
             # on its linears (silu(gate) * up in between), the combine over both
