@@ -1,6 +1,7 @@
 // The microscaled four-bit format: rounding to it (alone, and behind a gated activation), the values back, the weights' tile
 // layout, and the linear.
 #include <algorithm>
+#include <atomic>
 
 #include "mxfp4.hpp"
 #include "stream_common.hpp"
@@ -301,7 +302,7 @@ __device__ __forceinline__ void mx_store_rows(const MxTiles& p, i32x4_t* place, 
   constexpr int PIECES = NT * MX_ROWS * (int)sizeof(Y) / 16, ROWS = 64 / PIECES > 0 ? 64 / PIECES : 1;
   const int lane = threadIdx.x & 63, r = lane & 31, g = lane >> 5;
   Y* y = static_cast<Y*>(p.y);
-  if (p.n * (int)sizeof(Y) % 16 || reinterpret_cast<uintptr_t>(p.y) % 16) {
+  if (p.n * (int)sizeof(Y) % 16) {
     const int64_t row = row0 + r;
 #pragma unroll
     for (int j = 0; j < NT; j++)
@@ -535,7 +536,7 @@ static int launch_ring(MxTiles p, const MxPlan& plan, float* sums, hipStream_t s
   p.y = sums;
   HB_LAUNCH((mx_ring_kernel<float, WM, WN, MT, NT>), grid, dim3(64 * WM * WN), 0, stream, p);
   const int64_t count = p.m * p.n;
-  const int whole = count % 4 == 0 && aligned(y, 4 * sizeof(Y)), each = whole ? 1024 : 256;
+  const int whole = count % 4 == 0, each = whole ? 1024 : 256;
   HB_LAUNCH((mx_join_kernel<Y>), dim3((unsigned)((count + each - 1) / each)), dim3(256), 0, stream, sums, count, plan.shares, whole, y);
   return HB_OK;
 }
@@ -544,8 +545,15 @@ template <typename T, typename Y, int NT, int RUN>
 static int launch_few(const MxLinear& p, const MxLayout& at, hipStream_t stream) {
   const size_t lds = std::max(MxActs::bytes(p.m, p.k), (size_t)p.waves * NT * 4096);
   if (lds > 64 * 1024) {
-    static const hipError_t raised = hipFuncSetAttribute(reinterpret_cast<const void*>(&mx_few_rows_kernel<T, Y, NT, RUN>), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
-    if (raised != hipSuccess) return HB_ELAUNCH;
+    // set for a device once: the attribute is the loaded kernel's, and each device has its own
+    static std::atomic<uint64_t> raised{0};
+    int device = 0;
+    if (hipGetDevice(&device) != hipSuccess) return HB_ELAUNCH;
+    const uint64_t bit = device < 64 ? 1ull << device : 0;
+    if (!(raised.load(std::memory_order_acquire) & bit)) {
+      if (hipFuncSetAttribute(reinterpret_cast<const void*>(&mx_few_rows_kernel<T, Y, NT, RUN>), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024) != hipSuccess) return HB_ELAUNCH;
+      raised.fetch_or(bit, std::memory_order_release);
+    }
   }
   HB_LAUNCH((mx_few_rows_kernel<T, Y, NT, RUN>), dim3((unsigned)((at.tiles + NT - 1) / NT)), dim3(64 * p.waves), lds, stream, p);
   return HB_OK;
@@ -614,7 +622,12 @@ static int by_type(int type, F&& f) {
   }
   return HB_EINVAL;
 }
-static size_t type_bytes(int type) { return type == HB_F32 ? 4 : 2; }
+// launch(first row, rows): a launch holds 2^32 threads, so 2^31 lanes of eight values at a time.
+template <typename F>
+static void by_rows(int64_t rows, int lanes, F&& launch) {
+  const int64_t most = std::max<int64_t>(1, ((int64_t)1 << 31) / lanes);
+  for (int64_t lo = 0; lo < rows; lo += most) launch(lo, std::min(most, rows - lo));
+}
 
 }  // namespace hb
 
@@ -626,9 +639,11 @@ extern "C" int hb_mxfp4_quantize(const void* x, int type, int64_t rows, int k, v
   if (!aligned(x, 16) || !aligned(codes, 16)) return HB_EINVAL;
   return by_type(type, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    const int64_t lanes = rows * (k / 8);
-    HB_LAUNCH((mx_quantize_kernel<T>), dim3((unsigned)((lanes + 255) / 256)), dim3(256), 0, as_stream(stream), static_cast<const T*>(x), lanes,
-              static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales));
+    by_rows(rows, k / 8, [&](int64_t lo, int64_t count) {
+      const int64_t lanes = count * (k / 8);
+      HB_LAUNCH((mx_quantize_kernel<T>), dim3((unsigned)((lanes + 255) / 256)), dim3(256), 0, as_stream(stream), static_cast<const T*>(x) + lo * k, lanes,
+                static_cast<uint8_t*>(codes) + lo * (k / 2), static_cast<uint8_t*>(scales) + lo * (k / MX_GROUP));
+    });
     return launch_status();
   });
 }
@@ -639,9 +654,11 @@ extern "C" int hb_mxfp4_dequantize(const void* codes, const void* scales, int64_
   if (!aligned(codes, 16) || !aligned(out, 16)) return HB_EINVAL;
   return by_type(type, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    const int64_t lanes = rows * (k / 8);
-    HB_LAUNCH((mx_dequantize_kernel<T>), dim3((unsigned)((lanes + 255) / 256)), dim3(256), 0, as_stream(stream), static_cast<const uint8_t*>(codes),
-              static_cast<const uint8_t*>(scales), lanes, static_cast<T*>(out));
+    by_rows(rows, k / 8, [&](int64_t lo, int64_t count) {
+      const int64_t lanes = count * (k / 8);
+      HB_LAUNCH((mx_dequantize_kernel<T>), dim3((unsigned)((lanes + 255) / 256)), dim3(256), 0, as_stream(stream), static_cast<const uint8_t*>(codes) + lo * (k / 2),
+                static_cast<const uint8_t*>(scales) + lo * (k / MX_GROUP), lanes, static_cast<T*>(out) + lo * k);
+    });
     return launch_status();
   });
 }
@@ -654,16 +671,18 @@ extern "C" int hb_silu_mul_quant_mxfp4(const void* gate_up, int type, int64_t ro
   if (!aligned(gate_up, 16) || !aligned(codes, 16)) return HB_EINVAL;
   return by_type(type, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    const int64_t lanes = rows * (half / 8);
-    HB_LAUNCH((mx_silu_quantize_kernel<T>), dim3((unsigned)((lanes + 255) / 256)), dim3(256), 0, as_stream(stream), static_cast<const T*>(gate_up), rows, half,
-              pairs, static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales));
+    by_rows(rows, half / 8, [&](int64_t lo, int64_t count) {
+      HB_LAUNCH((mx_silu_quantize_kernel<T>), dim3((unsigned)((count * (half / 8) + 255) / 256)), dim3(256), 0, as_stream(stream),
+                static_cast<const T*>(gate_up) + lo * 2 * half, count, half, pairs, static_cast<uint8_t*>(codes) + lo * (half / 2),
+                static_cast<uint8_t*>(scales) + lo * (half / MX_GROUP));
+    });
     return launch_status();
   });
 }
 
 constexpr int64_t MX_MOST_ROWS = (int64_t)1 << 24;
-// Sizes that the layout's indices and a launch's grid hold.
-static bool layout_holds(int64_t n, int k) { return n > 0 && k > 0 && k <= 1 << 23 && k % MX_GROUP == 0 && n <= (int64_t)1 << 30 && (n + 31) / 32 * ((k + 511) / 512) <= (int64_t)1 << 27; }
+// Sizes that the layout's indices and a launch's 2^32 threads hold (a matrix of 2^37 values).
+static bool layout_holds(int64_t n, int k) { return n > 0 && k > 0 && k <= 1 << 23 && k % MX_GROUP == 0 && n <= (int64_t)1 << 30 && (n + 31) / 32 * ((k + 511) / 512) < (int64_t)1 << 23; }
 
 extern "C" size_t hb_mxfp4_tiled_bytes(int64_t n, int k) { return layout_holds(n, k) ? (size_t)MxLayout(n, k).bytes() : 0; }
 
@@ -699,7 +718,7 @@ extern "C" int hb_mxfp4_linear(const void* x, const void* x_scales, int x_type, 
   if (!x || !tiled || !y || (x_type == HB_MXFP4 && !x_scales)) return HB_ENULL;
   if (m <= 0 || m > MX_MOST_ROWS || !layout_holds(n, k) || y_type < HB_BF16 || y_type > HB_F32 || x_type < HB_BF16 || x_type > HB_MXFP4) return HB_EINVAL;
   if (x_type != HB_MXFP4 && x_type != y_type) return HB_EINVAL;
-  if (!aligned(x, 16) || !aligned(tiled, 16) || !aligned(y, type_bytes(y_type))) return HB_EINVAL;
+  if (!aligned(x, 16) || !aligned(tiled, 16) || !aligned(y, 16)) return HB_EINVAL;
   const size_t need = hb_mxfp4_linear_workspace_bytes(m, n, k, x_type);
   if (need && !workspace) return HB_ENULL;
   if (!aligned(workspace, 16) || !layout_holds(m, k)) return HB_EINVAL;

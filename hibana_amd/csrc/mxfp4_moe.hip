@@ -116,7 +116,7 @@ __device__ __forceinline__ int mx_few_product(const MxMoe& p, f32x4_t* part, int
 template <bool GATED, int RUN>
 __global__ __launch_bounds__(64 * MX_FEW_WAVES, RUN == 4 ? 2 : 4) void mx_fc1_few_kernel(MxMoe p) {
   extern __shared__ f32x4_t part[];
-  int list;
+  int list = 0;
   const int rows = mx_few_product<RUN, 4>(p, part, list, [&](const MxActs& acts, int r, int group, int quarter, int pair) {
     Mx8<__bf16> v;
     v.load(static_cast<const __bf16*>(p.x) + (int64_t)(pair / p.topk) * p.k + MX_GROUP * group + 8 * quarter);
@@ -138,7 +138,7 @@ __global__ __launch_bounds__(64 * MX_FEW_WAVES, RUN == 4 ? 2 : 4) void mx_fc1_fe
 template <typename Y, int RUN>
 __global__ __launch_bounds__(64 * MX_FEW_WAVES, RUN == 4 ? 2 : 4) void mx_fc2_few_kernel(MxMoe p) {
   extern __shared__ f32x4_t part[];
-  int list;
+  int list = 0;
   const int rows = mx_few_product<RUN, 1>(p, part, list, [&](const MxActs& acts, int r, int group, int, int pair) {
     acts.put(r, group, p.aq + (int64_t)pair * (p.k / 2), p.as + (int64_t)pair * acts.groups);
   });
@@ -445,9 +445,17 @@ struct MxWorkspace {
   size_t bytes;
 };
 
+// Rows a pass of a call takes (more go in several, one behind the other): what keeps the slots of 64 rows and the experts' last ones within a grid,
+// and the activations within a buffer descriptor's reach.
+int most_rows(const hb_mxfp4_experts* ex, int topk) {
+  const int64_t pairs = std::min<int64_t>((int64_t)1 << 21, (((int64_t)1 << 32) - 1) / (ex->inter / 2)), rows = (((int64_t)1 << 32) - 1) / (ex->hidden / 2);
+  return (int)std::max<int64_t>(1, std::min(pairs / topk, rows));
+}
+
 bool few_pairs(int64_t pairs, int hidden, int inter) { return pairs <= MX_SCAN_PAIRS && MxActs::bytes(std::min<int64_t>(pairs, MX_ROWS), std::max(hidden, inter)) <= 64 * 1024; }
 
 MxWorkspace carve(const hb_mxfp4_experts* ex, void* base, int64_t m, int topk, bool sum) {
+  m = std::min<int64_t>(m, most_rows(ex, topk));
   const int64_t pairs = m * topk;
   MxWorkspace w{};
   size_t off = 0;
@@ -472,10 +480,14 @@ MxWorkspace carve(const hb_mxfp4_experts* ex, void* base, int64_t m, int topk, b
 
 int fc1_rows(const hb_mxfp4_experts* ex) { return ex->gated ? 2 * ex->inter : ex->inter; }
 
+size_t plan_lds_of(int experts) { return ((size_t)(PLAN_WAVES + 1) * experts + 3 * (PLAN_WAVES + 1)) * sizeof(int); }
+constexpr int MX_MOST_TOPK = 4096;
+constexpr int MX_MOST_EXPERTS = 960;  // the plan's counts of them lie in 64 KB of LDS
+
 int check(const hb_mxfp4_experts* ex) {
   if (!ex || !ex->fc1 || !ex->fc2) return HB_ENULL;
   if (ex->experts <= 0 || ex->base < 0 || ex->hidden <= 0 || ex->inter <= 0 || ex->hidden_out <= 0 || ex->hidden % 32 || ex->inter % 32 || ex->hidden_out % 8 ||
-      ex->hidden > 1 << 20 || ex->inter > 1 << 20 || ex->hidden_out > 1 << 20 || ex->experts > 1 << 20 || ex->base > 1 << 28)
+      ex->hidden > 1 << 20 || ex->inter > 1 << 20 || ex->hidden_out > 1 << 20 || ex->experts > MX_MOST_EXPERTS || ex->base > 1 << 28)
     return HB_EINVAL;
   if (MxLayout(fc1_rows(ex), ex->hidden).bytes() >= (int64_t)1 << 31 || MxLayout(ex->hidden_out, ex->inter).bytes() >= (int64_t)1 << 31) return HB_EINVAL;  // offsets in one matrix
   return aligned(ex->fc1, 16) && aligned(ex->fc2, 16) ? HB_OK : HB_EINVAL;
@@ -487,22 +499,16 @@ int check(const hb_mxfp4_experts* ex) {
 using namespace hb;
 
 extern "C" size_t hb_mxfp4_moe_workspace_bytes(const hb_mxfp4_experts* experts, int m, int topk) {
-  if (check(experts) != HB_OK || m <= 0 || topk <= 0 || (int64_t)m * topk > 0x3fffffff) return 0;
+  if (check(experts) != HB_OK || m <= 0 || topk <= 0 || topk > MX_MOST_TOPK || (int64_t)m * topk > 0x3fffffff) return 0;
   return carve(experts, nullptr, m, topk, true).bytes;
 }
 
-extern "C" int hb_mxfp4_moe(const hb_mxfp4_experts* experts, const void* x, const int32_t* ids, const float* weights, int m, int topk, int mode, void* out,
-                            void* workspace, size_t workspace_bytes, void* stream) {
-  if (int e = check(experts)) return e;
-  if (!x || !ids || !weights || !out || !workspace) return HB_ENULL;
-  if (m <= 0 || topk <= 0 || (int64_t)m * topk > 0x3fffffff || mode < HB_MOE_SUM || mode > HB_MOE_PAIRS_BF16) return HB_EINVAL;
-  if (!aligned(x, 16) || !aligned(ids, 4) || !aligned(weights, 4) || !aligned(out, 16) || !aligned(workspace, 16)) return HB_EINVAL;
+// One pass: m <= most_rows. `wide`: the pairs of a sum in BF16.
+static int moe_pass(const hb_mxfp4_experts* experts, const void* x, const int32_t* ids, const float* weights, int m, int topk, int mode, bool wide, void* out,
+                    void* workspace, hipStream_t s) {
   const bool sum = mode == HB_MOE_SUM;
   const MxWorkspace ws = carve(experts, workspace, m, topk, sum);
-  if (workspace_bytes < ws.bytes) return HB_EWORKSPACE;
   const int64_t pairs = (int64_t)m * topk;
-  if (pairs * (experts->inter / 2) >= (int64_t)1 << 32 || (int64_t)m * (experts->hidden / 2) >= (int64_t)1 << 32) return HB_EINVAL;  // the descriptors' reach
-  hipStream_t s = as_stream(stream);
   const MxLayout l1(fc1_rows(experts), experts->hidden), l2(experts->hidden_out, experts->inter);
   MxMoe p1{}, p2{};
   p1.w = static_cast<const uint8_t*>(experts->fc1);
@@ -553,14 +559,12 @@ extern "C" int hb_mxfp4_moe(const hb_mxfp4_experts* experts, const void* x, cons
     }
   } else {
     // a summed prefill-sized call keeps its pair outputs in BF16, half the traffic of its widest tensor, as the framework's other routed calls do
-    narrow = narrow || (sum && m >= MOE_WIDE_ROWS);
+    narrow = narrow || (sum && wide);
     const bool tall = pairs >= (int64_t)experts->experts * 24;
     const int slot_rows = tall ? 2 * MX_ROWS : MX_ROWS;
     const int64_t slots = moe_max_slots(pairs, experts->experts, 0, slot_rows);
-    if (slots > 65535) return HB_EINVAL;
     const MxRound job{static_cast<const __bf16*>(x), (int64_t)m * (experts->hidden / 8), experts->hidden, ws.xq, ws.xs};
-    const size_t plan_lds = ((size_t)(PLAN_WAVES + 1) * experts->experts + 3 * (PLAN_WAVES + 1)) * sizeof(int);
-    if (plan_lds > 64 * 1024 || experts->experts > PLAN_THREADS) return HB_EINVAL;
+    const size_t plan_lds = plan_lds_of(experts->experts);
     if (pairs < MX_PLAN_PAIRS) {
       HB_LAUNCH(mx_plan_round_kernel, dim3(1 + (unsigned)((job.lanes + PLAN_THREADS - 1) / PLAN_THREADS)), dim3(PLAN_THREADS), plan_lds, s, ids, (int)pairs, experts->base,
                 experts->experts, ws.plan.plan, ws.plan.order, slot_rows, (int)slots, job);
@@ -627,4 +631,21 @@ extern "C" int hb_mxfp4_moe(const hb_mxfp4_experts* experts, const void* x, cons
     moe_launch_combine(c, s);
   }
   return launch_status();
+}
+
+extern "C" int hb_mxfp4_moe(const hb_mxfp4_experts* experts, const void* x, const int32_t* ids, const float* weights, int m, int topk, int mode, void* out,
+                            void* workspace, size_t workspace_bytes, void* stream) {
+  if (int e = check(experts)) return e;
+  if (!x || !ids || !weights || !out || !workspace) return HB_ENULL;
+  if (m <= 0 || topk <= 0 || topk > MX_MOST_TOPK || (int64_t)m * topk > 0x3fffffff || mode < HB_MOE_SUM || mode > HB_MOE_PAIRS_BF16) return HB_EINVAL;
+  if (!aligned(x, 16) || !aligned(ids, 4) || !aligned(weights, 4) || !aligned(out, 16) || !aligned(workspace, 16)) return HB_EINVAL;
+  if (workspace_bytes < carve(experts, nullptr, m, topk, mode == HB_MOE_SUM).bytes) return HB_EWORKSPACE;
+  const int most = most_rows(experts, topk);
+  const int64_t row = (int64_t)experts->hidden_out * (mode == HB_MOE_SUM ? 2 : mode == HB_MOE_PAIRS_F32 ? 4 * topk : 2 * topk);  // bytes
+  for (int lo = 0; lo < m; lo += std::min(most, m - lo)) {
+    if (int e = moe_pass(experts, static_cast<const uint16_t*>(x) + (int64_t)lo * experts->hidden, ids + (int64_t)lo * topk, weights + (int64_t)lo * topk, std::min(most, m - lo),
+                         topk, mode, m >= MOE_WIDE_ROWS, static_cast<uint8_t*>(out) + lo * row, workspace, as_stream(stream)))
+      return e;
+  }
+  return HB_OK;
 }

@@ -155,6 +155,13 @@ def tile(q: Mxfp4, gated: bool = False) -> torch.Tensor:
     return tiled
 
 
+def check_tiled(tiled: torch.Tensor | None, shape: tuple[int, ...], what: str) -> None:
+    """That `tiled` has the layout's bytes for matrices of `shape` ([N, K] or [E, N, K])."""
+    size = _lib.lib().hb_mxfp4_tiled_bytes(*shape[-2:])
+    if tiled is None or size == 0 or tiled.dtype != torch.uint8 or tuple(tiled.shape) != (*shape[:-2], size) or not tiled.is_contiguous() or tiled.data_ptr() % 16:
+        raise ValueError(f"{what}: not the layout of {list(shape)}")
+
+
 def untile(tiled: torch.Tensor, n: int, k: int, gated: bool = False) -> Mxfp4:
     """The inverse of `tile`."""
     size = _lib.lib().hb_mxfp4_tiled_bytes(n, k)

@@ -4,7 +4,7 @@
     out = sum_k w_k down h_k                                                                              (FP32, rounded once)
 
 fc1 [E, 2 I, H] with rows [up; gate] (gated) or [E, I, H] (ReLU^2), fc2 [E, H_out, I]; H and I multiples of 32. Deterministic,
-graph-capturable, any number of rows. No counterpart in the reference.
+graph-capturable, any number of rows (past about two million pairs in passes). No counterpart in the reference.
 """
 from __future__ import annotations
 
@@ -15,6 +15,8 @@ import torch
 
 from hibana_amd import _lib
 from hibana_amd.kernels import mxfp4
+
+MAX_EXPERTS = 960  # of one object: a plan's counts of them lie in LDS
 
 
 @dataclass
@@ -37,6 +39,11 @@ class Mxfp4Experts:
         (e1, n1, h), (e2, h2, i) = self.shape1, self.shape2
         if e1 != e2 or n1 not in (i, 2 * i) or not e1 or h2 % 8 or self.base < 0:
             raise ValueError("Mxfp4Experts: fc1 [E, 2 I or I, H], fc2 [E, H_out, I], H_out a multiple of eight, base not negative")
+        if e1 > MAX_EXPERTS:
+            raise ValueError(f"Mxfp4Experts: {e1} experts, the kernels take {MAX_EXPERTS}")
+        for tiled, codes, shape in ((self.tiled1, self.fc1_codes, self.shape1), (self.tiled2, self.fc2_codes, self.shape2)):
+            if tiled is not None or codes is None:
+                mxfp4.check_tiled(tiled, shape, "Mxfp4Experts")
 
     def __getstate__(self):
         """A copy or a pickle takes the tensors, not the structure of their addresses that `_struct` keeps here."""

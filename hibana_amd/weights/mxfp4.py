@@ -28,6 +28,8 @@ class Mxfp4Linear:
             if self.codes.ndim != 2 or not self.codes.numel():
                 raise ValueError("Mxfp4Linear: codes uint8 [N, K / 2]")
             self.out_features, self.in_features = self.codes.shape[0], 2 * self.codes.shape[1]
+        if self.tiled is not None or self.codes is None:
+            mxfp4.check_tiled(self.tiled, (self.out_features, self.in_features), "Mxfp4Linear")
 
     @classmethod
     def from_dense(cls, weight: torch.Tensor, pairs: int = 0) -> "Mxfp4Linear":

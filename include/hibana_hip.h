@@ -584,22 +584,23 @@ int hb_mxfp4_dequantize(const void* codes, const void* scales, int64_t rows, int
 int hb_silu_mul_quant_mxfp4(const void* gate_up, int type, int64_t rows, int half, int pairs, void* codes, void* scales, void* stream);
 
 /* The weights' tile layout: its bytes for a matrix [n, k] (any n; 0: a size the kernels do not take), row-major codes and scales of
- * `matrices` stacked matrices into it, and back. `gated`: fc1 of gated experts, rows [up; gate], n a multiple of 64. */
+ * `matrices` (up to 65535) stacked matrices into it, and back. `gated`: fc1 of gated experts, rows [up; gate], n a multiple of 64. */
 size_t hb_mxfp4_tiled_bytes(int64_t n, int k);
 int hb_mxfp4_repack(const void* codes, const void* scales, int matrices, int64_t n, int k, int gated, void* tiled, void* stream);
 int hb_mxfp4_unpack(const void* tiled, int matrices, int64_t n, int k, int gated, void* codes, void* scales, void* stream);
 
 /* y [m, n] = x w^T, FP32 sums rounded once: x [m, k] of y's type, rounded to the format on the way, or (HB_MXFP4) its codes with
- * `x_scales`; w a matrix in the tile layout. `workspace`: plain scratch of hb_mxfp4_linear_workspace_bytes (NULL where that is 0). */
+ * `x_scales`; w a matrix in the tile layout; x, tiled, y and the workspace on 16 bytes, m up to 2^24. `workspace`: plain scratch of hb_mxfp4_linear_workspace_bytes (NULL where that is 0). */
 size_t hb_mxfp4_linear_workspace_bytes(int64_t m, int64_t n, int k, int x_type);
 int hb_mxfp4_linear(const void* x, const void* x_scales, int x_type, int64_t m, const void* tiled, int64_t n, int k, void* y, int y_type,
                     void* workspace, size_t workspace_bytes, void* stream);
 
 /* Routed experts, weights and activations both in the format: fc1 and fc2 are stacks of `experts` tile layouts, fc1 [2 inter or inter,
  * hidden] (gated: rows [up; gate], laid out with `gated`; else ReLU^2), fc2 [hidden_out, inter]; hidden and inter multiples of 32,
- * hidden_out of eight. x [m, hidden] BF16 is rounded to the format, h between the two products as well (from its FP32 value). An id
+ * hidden_out of eight, up to 960 experts and a topk of 4096. x [m, hidden] BF16 is rounded to the format, h between the two products as well (from its FP32 value). An id
  * outside base .. base + experts - 1 adds nothing. mode HB_MOE_SUM: out BF16 [m, hidden_out]; HB_MOE_PAIRS_F32 / _BF16: the
- * pairs' outputs [m * topk, hidden_out] (those of skipped pairs unspecified). `workspace`: plain scratch, nothing in it need be zero. */
+ * pairs' outputs [m * topk, hidden_out] (those of skipped pairs unspecified). `workspace`: plain scratch, nothing in it need be zero; that of
+ * about two million pairs at most (more go in passes, one behind the other). */
 typedef struct {
   const void* fc1;
   const void* fc2;

@@ -102,3 +102,36 @@ def test_routed_experts_refusals():
             mxfp4_moe.mxfp4_moe(held, *bad)
     with pytest.raises(RuntimeError):
         mxfp4_moe.mxfp4_moe(held, x, ids, w)  # no CPU path
+
+
+def test_layouts_that_do_not_fit_their_shapes():
+    """Weights handed over in the kernels' layout alone: of the size that the shape has, or refused."""
+    from hibana_amd.kernels import mxfp4_moe
+    lib = _lib.lib()
+    size = lib.hb_mxfp4_tiled_bytes(64, 96)
+    u8 = lambda *s: torch.zeros(s, dtype=torch.uint8)  # noqa: E731
+    assert Mxfp4Linear(None, None, tiled=u8(size), out_features=64, in_features=96).bytes == 64 * 96 * 17 // 32
+    for tiled, n, k in [(None, 64, 96), (u8(size - 1), 64, 96), (u8(size), 96, 96), (u8(size), 0, 0), (u8(size).int(), 64, 96), (u8(2 * size)[::2], 64, 96)]:
+        with pytest.raises(ValueError):
+            Mxfp4Linear(None, None, tiled=tiled, out_features=n, in_features=k)
+    with pytest.raises(ValueError):
+        Mxfp4Linear(u8(64, 48), u8(64, 3), tiled=u8(size + 256))
+    other = lib.hb_mxfp4_tiled_bytes(96, 32)
+    make = lambda a, b, e=4: mxfp4_moe.Mxfp4Experts(None, None, None, None, tiled1=a, tiled2=b, shape1=(e, 64, 96), shape2=(e, 96, 32))  # noqa: E731
+    assert make(u8(4, size), u8(4, other)).gated
+    for a, b, e in [(None, u8(4, other), 4), (u8(3, size), u8(4, other), 4), (u8(4, size), u8(4, size), 4), (u8(961, size), u8(961, other), 961)]:
+        with pytest.raises(ValueError):
+            make(a, b, e)
+
+
+def test_sizes_past_what_a_launch_holds():
+    lib = _lib.lib()
+    assert lib.hb_mxfp4_tiled_bytes(1 << 28, 256) == 0 and lib.hb_mxfp4_tiled_bytes((1 << 28) - 32, 256) > 0  # 2^32 threads
+    assert lib.hb_mxfp4_linear_workspace_bytes(1 << 24, 32, 1 << 13, 0) == 0
+    ex = lambda **c: _lib.HbMxfp4Experts(*{**dict(fc1=256, fc2=256, experts=960, base=0, hidden=256, inter=128, hidden_out=256, gated=1), **c}.values())  # noqa: E731
+    size = lambda e, m, k: lib.hb_mxfp4_moe_workspace_bytes(C.byref(e), m, k)  # noqa: E731
+    assert size(ex(), 4, 2) > 0 and size(ex(experts=961), 4, 2) == 0 and size(ex(), 4, 4097) == 0
+    assert size(ex(), 1 << 18, 8) == size(ex(), 1 << 22, 8)  # passes of 2^21 pairs
+    assert size(ex(inter=1 << 14), 1 << 20, 8) == size(ex(inter=1 << 14), 1 << 22, 8)  # of what a buffer descriptor reaches
+    y = lib.hb_mxfp4_linear(256, None, 0, 4, 256, 64, 128, 264, 0, 256, 1 << 20, None)
+    assert y == _lib.HB_EINVAL  # results on 16 bytes
