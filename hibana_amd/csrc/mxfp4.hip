@@ -54,15 +54,18 @@ __global__ __launch_bounds__(256) void mx_dequantize_kernel(const uint8_t* __res
   mx_values(reinterpret_cast<const uint32_t*>(codes)[i], mx_scale_value(scales[i >> 2]), out + 8 * i);
 }
 
-// silu(g) u in FP32, g not below -80: exp2 of -g log2(e) as a product's two halves, one reciprocal. Off by less than
-// MX_SILU_OFF of its value: an ulp each for exp2 and the reciprocal, half of one for the correction, the sum and the two products.
-constexpr float MX_SILU_OFF = 0x1p-20f;  // (twice the sum of those)
+// The lower end of silu(g) u in FP32, for g between -80 and 2^100: exp(-g) as exp2 of hi = -g log2(e) rounded, times 1 + r with r = -g - hi ln2
+// (the product exact, in one multiply-add), one reciprocal, whose argument is scaled by 1 + MX_SILU_OFF. Without that scaling it is off by
+// less than MX_SILU_OFF of its value: 2^-23 each for exp2 and the reciprocal, 2^-24 each for the correction, the sum and the two products,
+// 80 x 2^-28.4 = 2^-22.1 for ln2 in FP32, together 0.73 x 2^-20 (and 2^-24 for the scaling's rounding); so the exact value lies between
+// this and this (1 + 2 MX_SILU_OFF) (1 + 2^-23), which MX_SILU_SPAN is above.
+constexpr float MX_SILU_OFF = 0x1p-20f, MX_SILU_SPAN = 0x1.2p-19f;
 __device__ __forceinline__ float mx_silu_mul(float g, float u) {
-  constexpr float L = 1.44269504088896340736f, L_LO = (float)(1.44269504088896340736 - (double)1.44269504088896340736f);
-  const float z = __builtin_fminf(__builtin_fmaxf(g, -80.0f), 200.0f);  // (past 200 exp2 is 0 all the same)
-  const float hi = -z * L, lo = __builtin_fmaf(-z, L, -hi) - z * L_LO;
+  const float hi = g * -1.44269504088896340736f;
+  const float r = __builtin_fmaf(hi, -0.693147180559945309f, -g);
   const float e = __builtin_amdgcn_exp2f(hi);
-  return g * __builtin_amdgcn_rcpf(1.0f + __builtin_fmaf(e, 0.693147180559945309f * lo, e)) * u;
+  const float t = __builtin_fmaf(e, r, e);
+  return g * __builtin_amdgcn_rcpf(__builtin_fmaf(t, 1.0f + MX_SILU_OFF, 1.0f + MX_SILU_OFF)) * u;
 }
 
 // silu(gate) * up of [rows, 2 half] rounded to the format in one pass; gate | up, or both in alternating blocks of `pairs` columns.
@@ -72,34 +75,44 @@ __device__ __forceinline__ float mx_silu_mul(float g, float u) {
 template <typename T>
 __global__ __launch_bounds__(256) void mx_silu_quantize_kernel(const T* __restrict__ x, int64_t rows, int half, int pairs, uint8_t* __restrict__ codes,
                                                                uint8_t* __restrict__ scales) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int per_row = half >> 3;
-  if (i >= rows * per_row) return;  // whole groups leave together: half is a multiple of 32
-  const int64_t r = i / per_row;
-  const int c = 8 * (int)(i - r * per_row);
-  const int gate_at = pairs ? (c / pairs) * 2 * pairs + c % pairs : c, up_at = pairs ? gate_at + pairs : half + c;
+  // A launch has 2^31 lanes at most. The row of the workgroup's first lane is one scalar division; the others are in that row or, where a row has 256 lanes
+  // and more, in the next.
+  const uint32_t per_row = (uint32_t)half >> 3, first = blockIdx.x * 256u, i = first + threadIdx.x;
+  if (i >= (uint32_t)rows * per_row) return;  // whole groups leave together: half is a multiple of 32
+  uint32_t r = first / per_row, c8 = first - r * per_row + threadIdx.x;
+  if (per_row >= 256u) {
+    const uint32_t over = c8 >= per_row;
+    r += over;
+    c8 -= over * per_row;
+  } else {
+    const uint32_t more = c8 / per_row;
+    r += more;
+    c8 -= more * per_row;
+  }
+  const uint32_t c = 8 * c8, gate_at = pairs ? (c / (uint32_t)pairs) * 2 * (uint32_t)pairs + c % (uint32_t)pairs : c, up_at = gate_at + (uint32_t)(pairs ? pairs : half);
   Mx8<T> g, u;
-  g.load(x + r * 2 * half + gate_at);
-  u.load(x + r * 2 * half + up_at);
+  x += (int64_t)r * 2 * half;
+  g.load(x + gate_at);
+  u.load(x + up_at);
   Mx8<float> p, q;
-  bool far = false;
+  float least = 0.f, most_g = 0.f;  // (a NaN passes by: its product is one)
 #pragma unroll
   for (int j = 0; j < 8; j++) {
-    p.v[j >> 2][j & 3] = mx_silu_mul(g.at(j), u.at(j));
-    far |= g.at(j) < -80.0f;
+    const float gj = g.at(j);
+    p.v[j >> 2][j & 3] = mx_silu_mul(gj, u.at(j));
+    least = __builtin_fminf(least, gj);
+    if (!std::is_same_v<T, _Float16>) most_g = __builtin_fmaxf(most_g, gj);
   }
+  bool far = least < -80.0f || most_g > 0x1p100f;
   const uint32_t top = quad_max(p.amax());
   uint32_t byte = mx_scale_byte(top);
   const float s = mx_scale_value(byte);
 #pragma unroll
-  for (int j = 0; j < 8; j++) {
-    q.v[j >> 2][j & 3] = p.v[j >> 2][j & 3] * (1.0f + MX_SILU_OFF);
-    p.v[j >> 2][j & 3] *= 1.0f - MX_SILU_OFF;
-  }
+  for (int j = 0; j < 8; j++) q.v[j >> 2][j & 3] = p.v[j >> 2][j & 3] * (1.0f + MX_SILU_SPAN);
   uint32_t code = p.codes(s);
-  constexpr uint32_t OFF = 16;  // ulps of MX_SILU_OFF
+  constexpr uint32_t SPAN = 36;  // ulps: MX_SILU_SPAN of a value is 18 to 36
   far |= code != q.codes(s);
-  far |= byte != 255u && (((top - OFF) ^ (top + OFF)) >> 23) != 0 && top != 0;
+  far |= byte != 255u && ((top ^ (top + SPAN)) >> 23) != 0;
   far |= top != 0 && top < 0x0d800000u;  // below 2^-100
   if (byte == 255u) code = 0;
   if (quad_max(far)) {
@@ -151,8 +164,8 @@ __global__ __launch_bounds__(256) void mx_repack_kernel(uint8_t* __restrict__ co
   scales += (int64_t)blockIdx.y * n * (k / 32);
   tiled += (int64_t)blockIdx.y * at.bytes();
   const int lane = (int)(i & 63);
-  const int64_t tc = i >> 6;
-  const int t = (int)(tc / (at.quads * 4)), c = (int)(tc - (int64_t)t * at.quads * 4);  // chunks past the last only have scales
+  const uint32_t tc = (uint32_t)(i >> 6);  // below 2^26
+  const int t = (int)(tc / (uint32_t)(at.quads * 4)), c = (int)tc - t * at.quads * 4;  // chunks past the last only have scales
   const int64_t row = mx_source_row(t, lane & 31, gated_inter);
   const int group = 2 * c + (lane >> 5);
   const bool in = row < n && group < k / 32;
@@ -451,8 +464,9 @@ template <typename T>
 __global__ __launch_bounds__(256) void mx_quantize_tiles_kernel(const T* __restrict__ x, int64_t rows, int k, uint8_t* __restrict__ tiled) {
   const MxLayout at(rows, k);
   const int lane = threadIdx.x & 63, all = at.quads * 4;  // K's chunks in whole quads: those past the last only have scales
-  const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), t = i / all;
-  const int c = (int)(i - t * all), group = 2 * c + (lane >> 5);
+  const uint32_t i = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // below 2^26
+  const int64_t t = i / (uint32_t)all;
+  const int c = (int)(i - (uint32_t)t * all), group = 2 * c + (lane >> 5);
   const int64_t row = t * MX_ROWS + (lane & 31);
   if (row >= rows) return;
   uint32_t byte = 0;

@@ -230,9 +230,9 @@ __device__ __forceinline__ void mx_round_lane(const MxRound& job, int64_t i) {
   const uint32_t byte = mx_scale_byte(quad_max(v.amax()));
   reinterpret_cast<uint32_t*>(job.codes)[i] = byte == 255u ? 0u : v.codes(mx_scale_value(byte));
   if ((i & 3) == 0) {
-    const int groups = job.k / MX_GROUP;
-    const int64_t row = (i >> 2) / groups;
-    const int group = (int)((i >> 2) - row * groups);
+    const uint32_t groups = (uint32_t)job.k / MX_GROUP, at_group = (uint32_t)(i >> 2);  // below 2^28: the codes are within a descriptor's reach
+    const int64_t row = at_group / groups;
+    const uint32_t group = at_group - (uint32_t)row * groups;
     uint8_t* at = job.scales + row * mx_scale_row(job.k);
     at[mx_scale_at(group)] = (uint8_t)byte;
     if (group == groups - 1 && (groups & 1)) at[mx_scale_at(groups)] = 0;
