@@ -274,8 +274,8 @@ __global__ __launch_bounds__(512) void mx_few_rows_kernel(MxLinear p) {
 
 // More rows: both operands in the tile layout. A workgroup's WM x WN wavefronts hold MT x NT output tiles of 32 x 32 each; 128 k of the
 // workgroup's rows of both operands are a step. LDS holds RING = 4 steps: a step's tiles come by LDS-direct loads (a tile as it lies: a
-// wavefront reads and writes 1024 consecutive bytes, no bank twice), asked for three steps ahead and waited for one step before they are
-// read, so that a step can fetch the next one's first fragments ahead of the barrier between them. A separate array a step: the
+// wavefront reads and writes 1024 consecutive bytes, no bank twice), asked for three steps ahead and waited for before the step ahead of
+// theirs (a second chunk: before theirs), so that a step can fetch the next one's first fragments ahead of the barrier between them. A separate array a step: the
 // compiler then knows that reading one does not wait for the loads into another. k past the matrix has scale 0 on both sides: 2^-254 of
 // anything is nothing in FP32, so what is read in the place of its codes does not matter.
 //
@@ -346,7 +346,9 @@ __device__ __forceinline__ void mx_store_rows(const MxTiles& p, i32x4_t* place, 
 template <typename Y, int WM, int WN, int MT, int NT>
 __global__ __launch_bounds__(64 * WM * WN, 1) void mx_ring_kernel(MxTiles p) {
   constexpr int WAVES = WM * WN, TA = WM * MT, TB = WN * NT, T = TA + TB;
+  static_assert(TB % WAVES == 0);
   constexpr int ASKS_A = (2 * TA + WAVES - 1) / WAVES, ASKS_B = (2 * TB + WAVES - 1) / WAVES, ASKS = ASKS_A + ASKS_B;  // tiles a wavefront asks for a step
+  constexpr int LATE = ASKS_B / 2 + (TA % WAVES == 0 ? ASKS_A / 2 : 0);  // of those, what is of a step's second chunk for certain
   __shared__ i32x4_t buf0[2 * T * 64], buf1[2 * T * 64], buf2[2 * T * 64], buf3[2 * T * 64];  // [2 chunks][A tiles, B tiles][64]
   const MxLayout la(p.m, p.k), lw(p.n, p.k);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
@@ -367,11 +369,17 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void mx_ring_kernel(MxTiles p) {
     __builtin_amdgcn_raw_ptr_buffer_load_lds(ROWS, (mx_lds_t)(BUF + (chunk * T + FIRST + tile) * 64), 16, lane * 16,                       \
                                              min(tile, LEFT - 1) * row_bytes + min(2 * (S) + chunk, chunks - 1) * 1024, 0, 0);            \
   }
-#define MX_ASK(BUF, S, J)                                         \
-  if constexpr ((J) < ASKS_B) {                                   \
-    MX_ASK_OF(rows_b, TB, left_b, TA, BUF, S, J)                  \
-  } else {                                                        \
-    MX_ASK_OF(rows_a, TA, left_a, 0, BUF, S, (J) - ASKS_B)        \
+  // The pieces of chunk 0 first, B's and A's; then the LATE ones, which are of chunk 1 alone. (Where A's are not whole pieces a wavefront and chunk,
+  // all of them go with the first.)
+#define MX_ASK(BUF, S, J)                                                                  \
+  if constexpr ((J) < ASKS_B / 2) {                                                        \
+    MX_ASK_OF(rows_b, TB, left_b, TA, BUF, S, J)                                           \
+  } else if constexpr ((J) < ASKS - LATE) {                                                \
+    MX_ASK_OF(rows_a, TA, left_a, 0, BUF, S, (J) - ASKS_B / 2)                             \
+  } else if constexpr ((J) < ASKS - LATE + ASKS_B / 2) {                                   \
+    MX_ASK_OF(rows_b, TB, left_b, TA, BUF, S, (J) - (ASKS - LATE) + ASKS_B / 2)            \
+  } else {                                                                                 \
+    MX_ASK_OF(rows_a, TA, left_a, 0, BUF, S, (J) - (ASKS - LATE) - ASKS_B / 2 + ASKS_A / 2) \
   }
 
   // the scales of this wavefront's tiles, a quad at a time
@@ -398,7 +406,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void mx_ring_kernel(MxTiles p) {
   mx_unrolled<ASKS>([&](auto j) { MX_ASK(buf0, 2 * q0, j.value) });
   mx_unrolled<ASKS>([&](auto j) { MX_ASK(buf1, 2 * q0 + 1, j.value) });
   mx_unrolled<ASKS>([&](auto j) { MX_ASK(buf2, 2 * q0 + 2, j.value) });
-  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(ASKS) : "memory");
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(ASKS + LATE) : "memory");
   __builtin_amdgcn_s_barrier();
   // a step: for each of its two chunks and each tile of B, the products with all tiles of A. Fragments come ahead of their use: B's two
   // groups of products, A's a chunk.
@@ -410,8 +418,10 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void mx_ring_kernel(MxTiles p) {
   for (int i = 0; i < MT; i++) fa[0][i] = a_at(buf0, 0, i);
 #pragma unroll
   for (int j = 0; j < AHEAD; j++) fb[j] = b_at(buf0, j);
-  // What the step asks of memory (its tiles three steps on, and at a quad's first step the next quad's scales) goes out between the groups of products:
-  // in front of them all, it and the barrier would leave the matrix cores idle for a fifth of the step.
+  // What the step asks of memory (at a quad's first step the next quad's scales, then its tiles three steps on) goes out between the products: in
+  // front of them all, it and the barrier would leave the matrix cores idle for a fifth of the step. At its end what may still be on its way is
+  // the step's own and the step's before LATE ones: the next step reads its own tiles, asked for two steps ago, and chunk 0 of the one behind it. (All of
+  // that one waited for: 2048 rows of 25600 x 5120 148 us, so 144.5.)
 #define MX_STEP(CUR, NEXT, ASKED, S, ODD)                                                                                                  \
   mx_unrolled<GROUPS>([&](auto group) {                                                                                                   \
     constexpr int v = group.value, u = v / NT, j = v % NT, ring = (ODD) * GROUPS + v;                                                      \
@@ -420,16 +430,17 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void mx_ring_kernel(MxTiles p) {
     mx_unrolled<MT>([&](auto tile) {                                                                                                      \
       constexpr int i = tile.value, at = v * MT + i;  /* the step's product */                                                            \
       mx_mfma_in_place<2 * (ODD) + u>(acc[i][j], fb[ring & 3], fa[u][i], now[MT + j], now[i]);                                             \
-      constexpr int before = at * ASKS / (GROUPS * MT), after = (at + 1) * ASKS / (GROUPS * MT);                                           \
-      mx_unrolled<after - before>([&](auto k) { MX_ASK(ASKED, (S) + 3, before + k.value) });                                              \
+      constexpr int ALL = GROUPS * MT, FIRST = (ALL + 3) / 4, H = (ODD) ? 0 : FIRST, W = ALL - FIRST;  /* asked for behind products H .. H + W - 1 */ \
+      constexpr int before = at < H ? 0 : at - H >= W ? ASKS : (at - H) * ASKS / W, after = at < H ? 0 : at + 1 - H >= W ? ASKS : (at + 1 - H) * ASKS / W; \
       if constexpr (!(ODD)) {                                                                                                             \
-        constexpr int from = at * SCALES / (GROUPS * MT), to = (at + 1) * SCALES / (GROUPS * MT);                                          \
+        constexpr int from = at >= H ? SCALES : at * SCALES / H, to = at >= H ? SCALES : (at + 1) * SCALES / H;                             \
         mx_unrolled<to - from>([&](auto k) { scale(from + k.value, min((S) / 2 + 1, la.quads - 1)); });                                    \
       }                                                                                                                                   \
+      mx_unrolled<after - before>([&](auto k) { MX_ASK(ASKED, (S) + 3, before + k.value) });                                              \
       __builtin_amdgcn_sched_barrier(0);                                                                                                  \
     });                                                                                                                                   \
   });                                                                                                                                     \
-  asm volatile("s_waitcnt vmcnt(%0)" ::"n"((ODD) ? ASKS : ASKS + SCALES) : "memory"); /* all but this step's have landed */                \
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"((ODD) ? ASKS + LATE : ASKS + LATE + SCALES) : "memory");                                       \
   __builtin_amdgcn_s_barrier();                                                                                                           \
   __builtin_amdgcn_sched_barrier(0);
 #define MX_QUAD                                                               \
@@ -528,9 +539,11 @@ static MxPlan plan_of(int64_t m, int64_t n, int k, int x_type) {
     const int64_t high = p.square ? 2 * mt : mt, wide = p.square ? 2 * mt : 4;
     return (rows.tiles + high - 1) / high * ((w.tiles + wide - 1) / wide);
   };
-  p.mt = p.square ? (groups(4) >= 160 ? 4 : 2) : rows.tiles;
+  // 256 x 256 a workgroup where such tiles fill the device well enough, and past a round of it where padding the rows to 256 costs no more than an
+  // eighth. us, large and small tiles, 5120 k: 2048 rows of 5120 42 and 45, of 25600 145 and 181; 777 rows of 25600 78 and 74; 1100 rows 88 and 96.
+  p.mt = !p.square ? rows.tiles : groups(4) >= 160 && (groups(4) <= MX_DEVICE || 32 * groups(4) <= 9 * groups(2)) ? 4 : 2;
   // K is shared where the tiles leave half the device idle, by up to eight workgroups of at least eight steps
-  p.shares = (int)std::max<int64_t>(1, std::min<int64_t>({256 / groups(p.mt), rows.quads / 4, 8}));
+  p.shares = (int)std::max<int64_t>(1, std::min<int64_t>({MX_DEVICE / groups(p.mt), rows.quads / 4, 8}));
   p.tiles = (size_t)(rows.bytes() + 255) / 256 * 256;
   p.bytes = p.tiles + (p.shares > 1 ? (size_t)p.shares * m * n * sizeof(float) : 0);
   return p;
