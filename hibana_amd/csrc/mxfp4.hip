@@ -3,7 +3,7 @@
 #include <algorithm>
 #include <atomic>
 
-#include "mxfp4.hpp"
+#include "mxfp4_ring.hpp"
 #include "stream_common.hpp"
 
 namespace hb {
@@ -191,19 +191,6 @@ struct MxLinear {
   int k, waves;
 };
 
-// Four neighbouring results of a row, `left` of them inside the matrix.
-template <typename Y>
-__device__ __forceinline__ void mx_store4(Y* out, const f32x4_t& v, int64_t left, bool whole) {
-  if (whole) {
-    typedef __attribute__((ext_vector_type(4))) Y y4_t;
-    *reinterpret_cast<y4_t*>(out) = y4_t{mx_out<Y>(v[0]), mx_out<Y>(v[1]), mx_out<Y>(v[2]), mx_out<Y>(v[3])};
-  } else {
-#pragma unroll
-    for (int j = 0; j < 4; j++)
-      if (j < left) out[j] = mx_out<Y>(v[j]);
-  }
-}
-
 // Few rows: a workgroup NT tiles of weight rows, its wavefronts the chunks of K. The first weights are asked for, then the workgroup puts
 // the activations into LDS, rounded on the way: each workgroup all of them, which costs less than a launch.
 template <typename T, typename Y, int NT, int RUN>
@@ -272,15 +259,8 @@ __global__ __launch_bounds__(512) void mx_few_rows_kernel(MxLinear p) {
   }
 }
 
-// More rows: both operands in the tile layout. A workgroup's WM x WN wavefronts hold MT x NT output tiles of 32 x 32 each; 128 k of the
-// workgroup's rows of both operands are a step. LDS holds RING = 4 steps: a step's tiles come by LDS-direct loads (a tile as it lies: a
-// wavefront reads and writes 1024 consecutive bytes, no bank twice), asked for three steps ahead and waited for before the step ahead of
-// theirs (a second chunk: before theirs), so that a step can fetch the next one's first fragments ahead of the barrier between them. A separate array a step: the
-// compiler then knows that reading one does not wait for the loads into another. k past the matrix has scale 0 on both sides: 2^-254 of
-// anything is nothing in FP32, so what is read in the place of its codes does not matter.
-//
-// Many rows take 2 x 2 wavefronts of 4 x 4 tiles: 256 accumulator registers, one wavefront a SIMD, and a matrix instruction's operands
-// come from LDS at half of the 128 bytes a cycle that it gives, what is asked for at a quarter.
+// More rows, on the ring (mxfp4_ring.hpp). Many take 2 x 2 wavefronts of 4 x 4 tiles: 256 accumulator registers, one wavefront a SIMD, and a matrix
+// instruction's operands come from LDS at half of the 128 bytes a cycle that it gives, what is asked for at a quarter.
 struct MxTiles {
   const uint8_t* a;
   const uint8_t* w;
@@ -289,184 +269,28 @@ struct MxTiles {
   int k, rows_of_tiles;  // workgroups along m
   int first, last;       // the tiles of weight rows that this launch covers
 };
-typedef __attribute__((address_space(3))) uint8_t* mx_lds_t;
-
-// mx_mfma with the sum staying in its accumulator registers (left to itself the compiler moves 256 of them about) and the scales in byte
-// OP of their words. The two wait states in front cover an operand that a vector instruction has just written, and hide behind the matrix
-// instruction before (32 cycles); mx_sums_done stands before the sums are read.
-template <int OP>
-__device__ __forceinline__ void mx_mfma_in_place(f32x16_t& acc, i32x4_t a, i32x4_t b, uint32_t sa, uint32_t sb) {
-#define MX_MFMA(SELECT) \
-  asm volatile("s_nop 1\n\tv_mfma_scale_f32_32x32x64_f8f6f4 %0, %1, %2, %0, %3, %4 " SELECT " cbsz:4 blgp:4" : "+a"(acc) : "v"(a), "v"(b), "v"(sa), "v"(sb))
-  if constexpr (OP == 0) MX_MFMA("op_sel_hi:[0,0,0]");
-  if constexpr (OP == 1) MX_MFMA("op_sel:[1,1,0] op_sel_hi:[0,0,0]");
-  if constexpr (OP == 2) MX_MFMA("op_sel_hi:[1,1,0]");
-  if constexpr (OP == 3) MX_MFMA("op_sel:[1,1,0] op_sel_hi:[1,1,0]");
-#undef MX_MFMA
-}
-__device__ __forceinline__ void mx_sums_done() { asm volatile("s_nop 15\n\ts_nop 15" ::: "memory"); }
-
-// 32 rows x NT tiles of a wavefront's sums, stored. A lane holds four columns of one row, 8 or 16 bytes: stored as they are, an instruction
-// would touch 32 rows' lines. They go through the wavefront's own part of LDS and leave as whole rows of NT x 32 columns, 16 bytes a
-// lane; a row's 16-byte pieces are XORed with its number so that neither way meets a bank twice. (Where rows do not start on 16 bytes: as
-// they are.)
-template <typename Y, int NT>
-__device__ __forceinline__ void mx_store_rows(const MxTiles& p, i32x4_t* place, int64_t row0, int64_t n0, const f32x16_t (&sums)[NT]) {
-  constexpr int PIECES = NT * MX_ROWS * (int)sizeof(Y) / 16, ROWS = 64 / PIECES > 0 ? 64 / PIECES : 1;
-  const int lane = threadIdx.x & 63, r = lane & 31, g = lane >> 5;
-  Y* y = static_cast<Y*>(p.y);
-  if (p.n * (int)sizeof(Y) % 16) {
-    const int64_t row = row0 + r;
-#pragma unroll
-    for (int j = 0; j < NT; j++)
-#pragma unroll
-      for (int q = 0; q < 4; q++) {
-        const int64_t n = n0 + MX_ROWS * j + 8 * q + 4 * g;
-        if (row < p.m && n < p.n) mx_store4<Y>(y + row * p.n + n, mx_quarter(sums[j], q), p.n - n, false);
-      }
-    return;
-  }
-  uint8_t* bytes = reinterpret_cast<uint8_t*>(place);
-#pragma unroll
-  for (int j = 0; j < NT; j++)
-#pragma unroll
-    for (int q = 0; q < 4; q++) {
-      const int at = (MX_ROWS * j + 8 * q + 4 * g) * (int)sizeof(Y), piece = (at / 16) ^ (r & (PIECES - 1));
-      mx_store4<Y>(reinterpret_cast<Y*>(bytes + (r * PIECES + piece) * 16 + at % 16), mx_quarter(sums[j], q), 4, true);
-    }
-#pragma unroll
-  for (int first = 0; first < MX_ROWS; first += ROWS) {
-    const int row = first + lane / PIECES, piece = lane % PIECES;
-    const int64_t n = n0 + piece * (16 / (int)sizeof(Y));
-    const i32x4_t v = place[row * PIECES + (piece ^ (row & (PIECES - 1)))];
-    if (row0 + row < p.m && n < p.n) *reinterpret_cast<i32x4_t*>(y + (row0 + row) * p.n + n) = v;
-  }
-}
-
 template <typename Y, int WM, int WN, int MT, int NT>
 __global__ __launch_bounds__(64 * WM * WN, 1) void mx_ring_kernel(MxTiles p) {
-  constexpr int WAVES = WM * WN, TA = WM * MT, TB = WN * NT, T = TA + TB;
-  static_assert(TB % WAVES == 0);
-  constexpr int ASKS_A = (2 * TA + WAVES - 1) / WAVES, ASKS_B = (2 * TB + WAVES - 1) / WAVES, ASKS = ASKS_A + ASKS_B;  // tiles a wavefront asks for a step
-  constexpr int LATE = ASKS_B / 2 + (TA % WAVES == 0 ? ASKS_A / 2 : 0);  // of those, what is of a step's second chunk for certain
-  __shared__ i32x4_t buf0[2 * T * 64], buf1[2 * T * 64], buf2[2 * T * 64], buf3[2 * T * 64];  // [2 chunks][A tiles, B tiles][64]
+  using Ring = MxRing<WM, WN, MT, NT>;
+  __shared__ i32x4_t buf0[Ring::BUFFER], buf1[Ring::BUFFER], buf2[Ring::BUFFER], buf3[Ring::BUFFER];
   const MxLayout la(p.m, p.k), lw(p.n, p.k);
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
   // consecutive workgroups go to the eight dies in turn: each die walks a run of tiles, rows fastest, so that its L2 keeps a run of weights
   const int total = gridDim.x, per = (total + 7) / 8, die = blockIdx.x % 8, whole = total % 8 ? total % 8 : 8;  // the first `whole` dies have `per` workgroups, the others one less
   const int at = die * per - (die > whole ? die - whole : 0) + (int)(blockIdx.x / 8);
-  const int a0 = at % p.rows_of_tiles * TA, b0 = p.first + at / p.rows_of_tiles * TB, chunks = la.chunks, row_bytes = chunks * 1024;
+  const int a0 = at % p.rows_of_tiles * Ring::TA, b0 = p.first + at / p.rows_of_tiles * Ring::TB;
   const int pairs = la.quads / 2, q0 = 2 * (int)((int64_t)pairs * blockIdx.y / gridDim.y), q1 = 2 * (int)((int64_t)pairs * (blockIdx.y + 1) / gridDim.y);
-  p.y = static_cast<Y*>(p.y) + (int64_t)blockIdx.y * p.m * p.n;
-
-  const int first_a = min(a0, la.tiles - 1), first_b = min(b0, lw.tiles - 1), left_a = min(TA, la.tiles - first_a), left_b = min(TB, lw.tiles - first_b);
-  const __amdgpu_buffer_rsrc_t rows_a = mx_rows(p.a + (int64_t)first_a * row_bytes, left_a * row_bytes);
-  const __amdgpu_buffer_rsrc_t rows_b = mx_rows(p.w + (int64_t)first_b * row_bytes, left_b * row_bytes);
-  // piece `wave + j * WAVES` of a step's 2 TA (2 TB): tile (that % TA) of chunk (that / TA); past the last piece, tile or chunk: the last again
-#define MX_ASK_OF(ROWS, TILES, LEFT, FIRST, BUF, S, J)                                                                                    \
-  {                                                                                                                                       \
-    const int piece = min(wave + (J) * WAVES, 2 * TILES - 1), chunk = piece / TILES, tile = piece - chunk * TILES;                          \
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(ROWS, (mx_lds_t)(BUF + (chunk * T + FIRST + tile) * 64), 16, lane * 16,                       \
-                                             min(tile, LEFT - 1) * row_bytes + min(2 * (S) + chunk, chunks - 1) * 1024, 0, 0);            \
-  }
-  // The pieces of chunk 0 first, B's and A's; then the LATE ones, which are of chunk 1 alone. (Where A's are not whole pieces a wavefront and chunk,
-  // all of them go with the first.)
-#define MX_ASK(BUF, S, J)                                                                  \
-  if constexpr ((J) < ASKS_B / 2) {                                                        \
-    MX_ASK_OF(rows_b, TB, left_b, TA, BUF, S, J)                                           \
-  } else if constexpr ((J) < ASKS - LATE) {                                                \
-    MX_ASK_OF(rows_a, TA, left_a, 0, BUF, S, (J) - ASKS_B / 2)                             \
-  } else if constexpr ((J) < ASKS - LATE + ASKS_B / 2) {                                   \
-    MX_ASK_OF(rows_b, TB, left_b, TA, BUF, S, (J) - (ASKS - LATE) + ASKS_B / 2)            \
-  } else {                                                                                 \
-    MX_ASK_OF(rows_a, TA, left_a, 0, BUF, S, (J) - (ASKS - LATE) - ASKS_B / 2 + ASKS_A / 2) \
-  }
-
-  // the scales of this wavefront's tiles, a quad at a time
-  constexpr int SCALES = MT + NT;
-  const int scale_bytes = la.quads * 256, first_sa = min(a0 + wm * MT, la.tiles - 1), first_sb = min(b0 + wn * NT, lw.tiles - 1);
-  const int left_sa = min(MT, la.tiles - first_sa), left_sb = min(NT, lw.tiles - first_sb);
-  const __amdgpu_buffer_rsrc_t scales_a = mx_rows(p.a + la.codes() + (int64_t)first_sa * scale_bytes, left_sa * scale_bytes);
-  const __amdgpu_buffer_rsrc_t scales_b = mx_rows(p.w + lw.codes() + (int64_t)first_sb * scale_bytes, left_sb * scale_bytes);
-  uint32_t now[SCALES], next[SCALES];  // A's, then B's
-  auto scale = [&](int t, int q) {
-    next[t] = t < MT ? __builtin_amdgcn_raw_buffer_load_b32(scales_a, lane * 4, min(t, left_sa - 1) * scale_bytes + q * 256, 0)
-                     : __builtin_amdgcn_raw_buffer_load_b32(scales_b, lane * 4, min(t - MT, left_sb - 1) * scale_bytes + q * 256, 0);
-  };
+  Y* y = static_cast<Y*>(p.y) + (int64_t)blockIdx.y * p.m * p.n;
+  const MxOperand a{p.a + (int64_t)a0 * la.chunks * 1024, p.a + la.codes() + (int64_t)a0 * la.quads * 256, la.tiles - a0};
+  const MxOperand b{p.w + (int64_t)b0 * lw.chunks * 1024, p.w + lw.codes() + (int64_t)b0 * lw.quads * 256, lw.tiles - b0};
   f32x16_t acc[MT][NT];
+  Ring::run(buf0, buf1, buf2, buf3, a, b, la.chunks, la.quads, q0, q1, acc);
+  i32x4_t* place = wave == 0 ? buf0 : wave == 1 ? buf1 : wave == 2 ? buf2 : buf3;  // each wavefront takes one of the ring's buffers
 #pragma unroll
-  for (int i = 0; i < MT; i++)
-#pragma unroll
-    for (int j = 0; j < NT; j++)
-#pragma unroll
-      for (int e = 0; e < 16; e++) acc[i][j][e] = 0.f;
-
-#pragma unroll
-  for (int t = 0; t < SCALES; t++) scale(t, q0);
-  mx_unrolled<ASKS>([&](auto j) { MX_ASK(buf0, 2 * q0, j.value) });
-  mx_unrolled<ASKS>([&](auto j) { MX_ASK(buf1, 2 * q0 + 1, j.value) });
-  mx_unrolled<ASKS>([&](auto j) { MX_ASK(buf2, 2 * q0 + 2, j.value) });
-  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(ASKS + LATE) : "memory");
-  __builtin_amdgcn_s_barrier();
-  // a step: for each of its two chunks and each tile of B, the products with all tiles of A. Fragments come ahead of their use: B's two
-  // groups of products, A's a chunk.
-  constexpr int GROUPS = 2 * NT, AHEAD = GROUPS < 3 ? 1 : 2;
-  i32x4_t fa[2][MT], fb[4];
-  auto a_at = [&](const i32x4_t* buf, int chunk, int i) { return buf[(chunk * T + wm * MT + i) * 64 + lane]; };
-  auto b_at = [&](const i32x4_t* buf, int group) { return buf[(group / NT * T + TA + wn * NT + group % NT) * 64 + lane]; };
-#pragma unroll
-  for (int i = 0; i < MT; i++) fa[0][i] = a_at(buf0, 0, i);
-#pragma unroll
-  for (int j = 0; j < AHEAD; j++) fb[j] = b_at(buf0, j);
-  // What the step asks of memory (at a quad's first step the next quad's scales, then its tiles three steps on) goes out between the products: in
-  // front of them all, it and the barrier would leave the matrix cores idle for a fifth of the step. At its end what may still be on its way is
-  // the step's own and the step's before LATE ones: the next step reads its own tiles, asked for two steps ago, and chunk 0 of the one behind it. (All of
-  // that one waited for: 2048 rows of 25600 x 5120 148 us, so 144.5.)
-#define MX_STEP(CUR, NEXT, ASKED, S, ODD)                                                                                                  \
-  mx_unrolled<GROUPS>([&](auto group) {                                                                                                   \
-    constexpr int v = group.value, u = v / NT, j = v % NT, ring = (ODD) * GROUPS + v;                                                      \
-    fb[(ring + AHEAD) & 3] = v + AHEAD < GROUPS ? b_at(CUR, v + AHEAD) : b_at(NEXT, v + AHEAD - GROUPS);                                   \
-    _Pragma("unroll") for (int i = j * MT / NT; i < (j + 1) * MT / NT; i++) fa[1 - u][i] = u == 0 ? a_at(CUR, 1, i) : a_at(NEXT, 0, i);     \
-    mx_unrolled<MT>([&](auto tile) {                                                                                                      \
-      constexpr int i = tile.value, at = v * MT + i;  /* the step's product */                                                            \
-      mx_mfma_in_place<2 * (ODD) + u>(acc[i][j], fb[ring & 3], fa[u][i], now[MT + j], now[i]);                                             \
-      constexpr int ALL = GROUPS * MT, FIRST = (ALL + 3) / 4, H = (ODD) ? 0 : FIRST, W = ALL - FIRST;  /* asked for behind products H .. H + W - 1 */ \
-      constexpr int before = at < H ? 0 : at - H >= W ? ASKS : (at - H) * ASKS / W, after = at < H ? 0 : at + 1 - H >= W ? ASKS : (at + 1 - H) * ASKS / W; \
-      if constexpr (!(ODD)) {                                                                                                             \
-        constexpr int from = at >= H ? SCALES : at * SCALES / H, to = at >= H ? SCALES : (at + 1) * SCALES / H;                             \
-        mx_unrolled<to - from>([&](auto k) { scale(from + k.value, min((S) / 2 + 1, la.quads - 1)); });                                    \
-      }                                                                                                                                   \
-      mx_unrolled<after - before>([&](auto k) { MX_ASK(ASKED, (S) + 3, before + k.value) });                                              \
-      __builtin_amdgcn_sched_barrier(0);                                                                                                  \
-    });                                                                                                                                   \
-  });                                                                                                                                     \
-  asm volatile("s_waitcnt vmcnt(%0)" ::"n"((ODD) ? ASKS + LATE : ASKS + LATE + SCALES) : "memory");                                       \
-  __builtin_amdgcn_s_barrier();                                                                                                           \
-  __builtin_amdgcn_sched_barrier(0);
-#define MX_QUAD                                                               \
-  _Pragma("unroll") for (int t = 0; t < SCALES; t++) now[t] = next[t];
-  for (int q = q0; q < q1; q += 2) {
-    MX_QUAD
-    MX_STEP(buf0, buf1, buf3, 2 * q, 0)
-    MX_STEP(buf1, buf2, buf0, 2 * q + 1, 1)
-    MX_QUAD
-    MX_STEP(buf2, buf3, buf1, 2 * q + 2, 0)
-    MX_STEP(buf3, buf0, buf2, 2 * q + 3, 1)
+  for (int i = 0; i < MT; i++) {
+    const int64_t row0 = (int64_t)(a0 + wm * MT + i) * MX_ROWS;
+    mx_store_rows<Y, NT>(place, p.n, (int64_t)(b0 + wn * NT) * MX_ROWS, acc[i], [&](int r) { return row0 + r < p.m ? y + (row0 + r) * p.n : nullptr; });
   }
-#undef MX_QUAD
-#undef MX_STEP
-#undef MX_ASK
-#undef MX_ASK_OF
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // what was asked for past the end arrives before the workgroup leaves its LDS
-  mx_sums_done();
-#pragma unroll
-  for (int i = 0; i < MT; i++)
-#pragma unroll
-    for (int j = 0; j < NT; j++) asm volatile("" : "+a"(acc[i][j]));
-  __builtin_amdgcn_s_barrier();  // every wavefront has left the ring: each takes one of its buffers
-  i32x4_t* place = wave == 0 ? buf0 : wave == 1 ? buf1 : wave == 2 ? buf2 : buf3;
-#pragma unroll
-  for (int i = 0; i < MT; i++) mx_store_rows<Y, NT>(p, place, (int64_t)(a0 + wm * MT + i) * MX_ROWS, (int64_t)(b0 + wn * NT) * MX_ROWS, acc[i]);
 }
 
 // x [rows, k] rounded into the tile layout, a wavefront a tile: it reads 32 rows of 128 (FP32: 256) bytes, a lane its group,

@@ -4,7 +4,7 @@
 //   h = silu(gate xq) * (up xq) or relu(up xq)^2 in FP32, rounded to the format;  y = down h;  out = the weighted sum of a row's y.
 #include <algorithm>
 
-#include "mxfp4.hpp"
+#include "mxfp4_ring.hpp"
 #include "plan.hpp"
 #include "stream_common.hpp"
 
@@ -53,13 +53,17 @@ __device__ __forceinline__ int mx_slot_of(const MxMoe& p, int id, int first, int
 // i = 64 q + lane holds row lane % 32, columns 8 q + 4 (lane / 32) .. + 3. In two halves with a barrier between: a thread's largest magnitude goes to
 // its word of `tops` (LDS), then the group's gives the scale.
 template <bool GATED>
+__device__ __forceinline__ float mx_h_of(float up, float gate) {
+  const float u = fmaxf(up, 0.f);
+  return GATED ? gate / (1.0f + expf(-gate)) * up : (up != up ? up : u * u);
+}
+template <bool GATED>
 __device__ __forceinline__ f32x4_t mx_h(const f32x4_t& up, const f32x4_t& gate, uint32_t* tops) {
   f32x4_t h;
   uint32_t top = 0;
 #pragma unroll
   for (int j = 0; j < 4; j++) {
-    const float u = fmaxf(up[j], 0.f);
-    h[j] = GATED ? gate[j] / (1.0f + expf(-gate[j])) * up[j] : (up[j] != up[j] ? up[j] : u * u);
+    h[j] = mx_h_of<GATED>(up[j], gate[j]);
     top = max(top, __float_as_uint(h[j]) & 0x7fffffffu);
   }
   tops[threadIdx.x] = top;
@@ -437,6 +441,138 @@ __global__ __launch_bounds__(64 * MX_MOE_WAVES, MT == 1 ? 3 : 2) void mx_fc2_man
   }
 }
 
+// ------------------------------------------------------------------------------------------------ many pairs an expert
+// The ring (mxfp4_ring.hpp) on the plan's slots of MX_RING_ROWS rows: the slot's rows of x rounded into the tile layout, fc1 with h rounded into it from
+// the accumulators, fc2 with each row's results to its pair.
+using MxMoeRing = MxRing<2, 2, 2, 2>;
+constexpr int MX_RING_ROWS = MxMoeRing::TA * MX_ROWS, MX_ROUND_CHUNKS = 4;
+
+// A wavefront MX_ROUND_CHUNKS chunks of a tile of a slot: a lane its group of 32 values, whose codes are the 16 bytes that it owns, as where a linear's rows are
+// rounded; chunks past K have scale 0. The first workgroups of a slot also clear the scales of h behind its last group, which fc1 does
+// not write: what they would multiply is scaled by 2^-127 on the weights' side, but has to be finite.
+__global__ __launch_bounds__(256) void mx_gather_kernel(MxMoe p, MxLayout xs, MxLayout hs) {
+  const int32_t* entry = p.plan + PLAN_HEADER + 4 * (int)blockIdx.y;
+  const int rows = entry[2], p0 = entry[1], lane = threadIdx.x & 63, tile = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (MX_ROWS * tile >= rows) return;
+  const int r = min(MX_ROWS * tile + (lane & 31), rows - 1), row = p.order[p0 + r] / p.topk;  // (rows past the last: that one again)
+  const __bf16* x = static_cast<const __bf16*>(p.x) + (int64_t)row * p.k;
+  const int64_t at = (int64_t)blockIdx.y * MxMoeRing::TA + tile;
+  uint8_t *codes = const_cast<uint8_t*>(p.aq), *scales = const_cast<uint8_t*>(p.as);
+#pragma unroll
+  for (int u = 0; u < MX_ROUND_CHUNKS; u++) {
+    const int c = MX_ROUND_CHUNKS * blockIdx.x + u, group = 2 * c + (lane >> 5);
+    uint32_t byte = 0;
+    i32x4_t code = {0, 0, 0, 0};
+    if (group < p.k / MX_GROUP) {
+      MxGroup<__bf16> v;
+      v.load(x + MX_GROUP * group);
+      code = v.codes(byte);
+    }
+    if (c < xs.chunks) *reinterpret_cast<i32x4_t*>(codes + ((at * xs.chunks + c) * 64 + lane) * 16) = code;
+    scales[(at * xs.quads + (c >> 2)) * 256 + lane * 4 + (c & 3)] = (uint8_t)byte;
+  }
+  if (blockIdx.x == 0)
+    for (int c = p.inter / MX_K; c < hs.quads * 4; c++)
+      if (2 * c + (lane >> 5) >= p.inter / MX_GROUP) p.hs[(at * hs.quads + (c >> 2)) * 256 + lane * 4 + (c & 3)] = 0;
+}
+
+// The slot and the tile of weight rows of a workgroup. Consecutive workgroups go to the eight dies in turn: a die takes two slots at a time, each with all
+// columns, so that its L2 keeps a slot's activations, and the weights where both are one expert's.
+struct MxPlace {
+  int slot, column;
+};
+__device__ __forceinline__ MxPlace mx_place_of(int columns) {
+  const int die = blockIdx.x % 8, at = blockIdx.x / 8, pair = at / (2 * columns), in = at - pair * 2 * columns, second = in >= columns;
+  return {(pair * 8 + die) * 2 + second, in - second * columns};
+}
+__device__ __forceinline__ MxOperand mx_expert_tiles(const MxMoe& p, const MxLayout& at, int e, int tile) {
+  const uint8_t* w = p.w + e * p.expert_bytes;
+  return {w + (int64_t)tile * at.chunks * 1024, w + at.codes() + (int64_t)tile * at.quads * 256, at.tiles - tile};
+}
+__device__ __forceinline__ MxOperand mx_slot_tiles(const MxMoe& p, const MxLayout& at, int slot, int rows) {
+  const int64_t tile = (int64_t)slot * MxMoeRing::TA;
+  return {p.aq + tile * at.chunks * 1024, p.as + tile * at.quads * 256, (rows + MX_ROWS - 1) / MX_ROWS};
+}
+
+template <bool GATED>
+__global__ __launch_bounds__(64 * MxMoeRing::WAVES, 2) void mx_fc1_ring_kernel(MxMoe p, int slots, int columns) {
+  using Ring = MxMoeRing;
+  constexpr int MT = 2, NT = 2;
+  __shared__ i32x4_t buf0[Ring::BUFFER], buf1[Ring::BUFFER], buf2[Ring::BUFFER], buf3[Ring::BUFFER];
+  const MxPlace place = mx_place_of(columns);
+  if (place.slot >= slots) return;
+  const int32_t* entry = p.plan + PLAN_HEADER + 4 * place.slot;
+  const int rows = entry[2];
+  if (rows == 0) return;
+  const MxLayout at(p.n, p.k), to(0, p.inter);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave >> 1, wn = wave & 1, r = lane & 31, g = lane >> 5;
+  f32x16_t acc[MT][NT];
+  Ring::run(buf0, buf1, buf2, buf3, mx_slot_tiles(p, at, place.slot, rows), mx_expert_tiles(p, at, entry[0], place.column * Ring::TB), at.chunks, at.quads, 0, at.quads, acc);
+  // A lane holds 16 of the 32 values of a row's group, lane ^ 32 the others: columns 8 q + 4 g .. + 3 in registers 4 q .. 4 q + 3. Each lane ends with
+  // eight bytes of the group's codes, columns 16 g .. 16 g + 15.
+#pragma unroll
+  for (int i = 0; i < MT; i++) {
+    if (MX_ROWS * (wm * MT + i) >= rows) break;
+#pragma unroll
+    for (int j = 0; j < NT; j += GATED ? 2 : 1) {
+      const int tile = place.column * Ring::TB + wn * NT + j, column = GATED ? tile >> 1 : tile;
+      if (column >= p.inter / MX_GROUP) break;
+      float h[16];
+      uint32_t top = 0;
+#pragma unroll
+      for (int e = 0; e < 16; e++) {
+        h[e] = mx_h_of<GATED>(acc[i][j][e], acc[i][GATED ? j + 1 : j][e]);
+        top = max(top, __float_as_uint(h[e]) & 0x7fffffffu);
+      }
+      top = max(top, (uint32_t)__shfl_xor((int)top, 32));
+      const uint32_t byte = mx_scale_byte(top);
+      const float s = mx_scale_value(byte);
+      uint32_t c[4];
+#pragma unroll
+      for (int q = 0; q < 4; q++) {
+        c[q] = 0;
+        c[q] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c[q], h[4 * q], h[4 * q + 1], s, 0);
+        c[q] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c[q], h[4 * q + 2], h[4 * q + 3], s, 1);
+      }
+      const uint32_t lower = c[0] | c[1] << 16, upper = c[2] | c[3] << 16, other = (uint32_t)__shfl_xor((int)(g ? lower : upper), 32), own = g ? upper : lower;
+      // g = 0: own is its q = 0, 1 and other the partner's; g = 1: other is the partner's (g = 0) q = 2, 3 and own its own
+      const uint32_t first = g ? other : own, second = g ? own : other;  // of the lanes g = 0 and g = 1
+      typedef __attribute__((ext_vector_type(2))) uint32_t u32x2_t;
+      u32x2_t word = {(first & 0xffffu) | second << 16, first >> 16 | (second & 0xffff0000u)};
+      if (byte == 255u) word = u32x2_t{0, 0};
+      const int64_t row_tile = (int64_t)place.slot * Ring::TA + wm * MT + i;
+      const int chunk = column >> 1, half = column & 1;
+      *reinterpret_cast<u32x2_t*>(p.hq + ((row_tile * to.chunks + chunk) * 64 + 32 * half + r) * 16 + 8 * g) = word;
+      if (g == 0) p.hs[(row_tile * to.quads + (chunk >> 2)) * 256 + (32 * half + r) * 4 + (chunk & 3)] = (uint8_t)byte;
+    }
+  }
+}
+
+template <typename Y>
+__global__ __launch_bounds__(64 * MxMoeRing::WAVES, 2) void mx_fc2_ring_kernel(MxMoe p, int slots, int columns) {
+  using Ring = MxMoeRing;
+  constexpr int MT = 2, NT = 2;
+  __shared__ i32x4_t buf0[Ring::BUFFER], buf1[Ring::BUFFER], buf2[Ring::BUFFER], buf3[Ring::BUFFER];
+  const MxPlace place = mx_place_of(columns);
+  if (place.slot >= slots) return;
+  const int32_t* entry = p.plan + PLAN_HEADER + 4 * place.slot;
+  const int rows = entry[2];
+  if (rows == 0) return;
+  const MxLayout at(p.n, p.k);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave >> 1, wn = wave & 1;
+  f32x16_t acc[MT][NT];
+  Ring::run(buf0, buf1, buf2, buf3, mx_slot_tiles(p, at, place.slot, rows), mx_expert_tiles(p, at, entry[0], place.column * Ring::TB), at.chunks, at.quads, 0, at.quads, acc);
+  const int32_t* order = p.order + entry[1];
+  i32x4_t* own = wave == 0 ? buf0 : wave == 1 ? buf1 : wave == 2 ? buf2 : buf3;
+#pragma unroll
+  for (int i = 0; i < MT; i++) {
+    const int row0 = MX_ROWS * (wm * MT + i);
+    if (row0 >= rows) break;
+    mx_store_rows<Y, NT>(own, p.n, (int64_t)(place.column * Ring::TB + wn * NT) * MX_ROWS, acc[i],
+                         [&](int r) { return row0 + r < rows ? static_cast<Y*>(p.y) + (int64_t)order[row0 + r] * p.n : nullptr; });
+  }
+}
+
 namespace {
 struct MxWorkspace {
   MoeWorkspace plan;
@@ -454,6 +590,16 @@ int most_rows(const hb_mxfp4_experts* ex, int topk) {
 
 bool few_pairs(int64_t pairs, int hidden, int inter) { return pairs <= MX_SCAN_PAIRS && MxActs::bytes(std::min<int64_t>(pairs, MX_ROWS), std::max(hidden, inter)) <= 64 * 1024; }
 
+// From this many pairs an expert on (were they shared out evenly) a call runs on the ring: a slot of 128 rows of one expert fills its tiles then, and the rows
+// are worth being laid out.
+constexpr int MX_RING_PAIRS = 64;
+int fc1_rows(const hb_mxfp4_experts* ex) { return ex->gated ? 2 * ex->inter : ex->inter; }
+int64_t ring_groups(int64_t slots, int columns) { return (slots + 15) / 16 * 16 * ((columns + 32 * MxMoeRing::TB - 1) / (32 * MxMoeRing::TB)); }
+bool on_ring(int64_t pairs, const hb_mxfp4_experts* ex) {
+  return pairs >= (int64_t)MX_RING_PAIRS * ex->experts &&
+         ring_groups(moe_max_slots(pairs, ex->experts, 0, MX_RING_ROWS), std::max(fc1_rows(ex), ex->hidden_out)) < (int64_t)1 << 24;  // (a launch holds 2^32 threads)
+}
+
 MxWorkspace carve(const hb_mxfp4_experts* ex, void* base, int64_t m, int topk, bool sum) {
   m = std::min<int64_t>(m, most_rows(ex, topk));
   const int64_t pairs = m * topk;
@@ -468,17 +614,27 @@ MxWorkspace carve(const hb_mxfp4_experts* ex, void* base, int64_t m, int topk, b
     w.plan.plan = reinterpret_cast<int32_t*>(take((PLAN_HEADER + (4 + DONE_PITCH) * moe_max_slots(pairs, ex->experts, 0, MX_ROWS) + 32) * sizeof(int32_t)));
     w.plan.plan_wide = reinterpret_cast<int32_t*>(take((size_t)64 * ex->experts * sizeof(int32_t)));
     w.plan.order = reinterpret_cast<int32_t*>(take((size_t)pairs * sizeof(int32_t)));
-    w.xq = take((size_t)m * (ex->hidden / 2));
-    w.xs = take((size_t)m * mx_scale_row(ex->hidden));
   }
-  w.hq = take((size_t)pairs * (ex->inter / 2));
-  w.hs = take((size_t)pairs * mx_scale_row(ex->inter));
+  if (!few_pairs(pairs, ex->hidden, ex->inter) && on_ring(pairs, ex)) {
+    const int64_t tiles = moe_max_slots(pairs, ex->experts, 0, MX_RING_ROWS) * MxMoeRing::TA;
+    const MxLayout x(0, ex->hidden), h(0, ex->inter);
+    w.xq = take((size_t)tiles * x.chunks * 1024);
+    w.xs = take((size_t)tiles * x.quads * 256);
+    w.hq = take((size_t)tiles * h.chunks * 1024);
+    w.hs = take((size_t)tiles * h.quads * 256);
+  } else {
+    if (!few_pairs(pairs, ex->hidden, ex->inter)) {
+      w.xq = take((size_t)m * (ex->hidden / 2));
+      w.xs = take((size_t)m * mx_scale_row(ex->hidden));
+    }
+    w.hq = take((size_t)pairs * (ex->inter / 2));
+    w.hs = take((size_t)pairs * mx_scale_row(ex->inter));
+  }
   w.y = sum ? take((size_t)pairs * ex->hidden_out * sizeof(float)) : nullptr;
   w.bytes = off;
   return w;
 }
 
-int fc1_rows(const hb_mxfp4_experts* ex) { return ex->gated ? 2 * ex->inter : ex->inter; }
 
 size_t plan_lds_of(int experts) { return ((size_t)(PLAN_WAVES + 1) * experts + 3 * (PLAN_WAVES + 1)) * sizeof(int); }
 constexpr int MX_MOST_TOPK = 4096;
@@ -534,6 +690,20 @@ static int moe_pass(const hb_mxfp4_experts* experts, const void* x, const int32_
   p2.y = sum ? ws.y : out;
   bool narrow = mode == HB_MOE_PAIRS_BF16;
   const unsigned groups1 = (unsigned)((l1.tiles + MX_MOE_TILES - 1) / MX_MOE_TILES), groups2 = (unsigned)((l2.tiles + MX_MOE_TILES - 1) / MX_MOE_TILES);
+  auto combine = [&](bool bf16) {
+    CombineParams c{};
+    c.pairs = ws.y;
+    c.pairs_bf16 = bf16;
+    c.ids = ids;
+    c.weights = weights;
+    c.e_lo = experts->base;
+    c.e_n = experts->experts;
+    c.m = m;
+    c.topk = topk;
+    c.h = experts->hidden_out;
+    c.out = static_cast<uint16_t*>(out);
+    moe_launch_combine(c, s);
+  };
   if (few_pairs(pairs, experts->hidden, experts->inter)) {
     const int most = (int)std::min<int64_t>(MX_ROWS, pairs);
     const size_t room = (size_t)MX_FEW_WAVES * MX_MOE_TILES * 4096;
@@ -560,6 +730,28 @@ static int moe_pass(const hb_mxfp4_experts* experts, const void* x, const int32_
   } else {
     // a summed prefill-sized call keeps its pair outputs in BF16, half the traffic of its widest tensor, as the framework's other routed calls do
     narrow = narrow || (sum && wide);
+    if (on_ring(pairs, experts)) {
+      const int64_t slots = moe_max_slots(pairs, experts->experts, 0, MX_RING_ROWS);
+      if (int e = moe_launch_plan(ids, pairs, experts->base, experts->experts, 0, ws.plan, s, MX_RING_ROWS)) return e;
+      p1.x = x;
+      p1.aq = ws.xq;
+      p1.as = ws.xs;
+      p1.plan = p2.plan = ws.plan.plan;
+      p1.order = p2.order = ws.plan.order;
+      HB_LAUNCH(mx_gather_kernel, dim3((unsigned)(l1.quads * 4 / MX_ROUND_CHUNKS), (unsigned)slots), dim3(64 * MxMoeRing::TA), 0, s, p1, l1, l2);
+      auto launch = [&](auto kernel, const MxLayout& at, const MxMoe& p) {
+        const int columns = (at.tiles + MxMoeRing::TB - 1) / MxMoeRing::TB;
+        HB_LAUNCH(kernel, dim3((unsigned)ring_groups(slots, p.n)), dim3(64 * MxMoeRing::WAVES), 0, s, p, (int)slots, columns);
+      };
+      launch(experts->gated ? mx_fc1_ring_kernel<true> : mx_fc1_ring_kernel<false>, l1, p1);
+      if (narrow) {
+        launch(mx_fc2_ring_kernel<__bf16>, l2, p2);
+      } else {
+        launch(mx_fc2_ring_kernel<float>, l2, p2);
+      }
+      if (sum) combine(narrow);
+      return launch_status();
+    }
     const bool tall = pairs >= (int64_t)experts->experts * 24;
     const int slot_rows = tall ? 2 * MX_ROWS : MX_ROWS;
     const int64_t slots = moe_max_slots(pairs, experts->experts, 0, slot_rows);
@@ -616,20 +808,7 @@ static int moe_pass(const hb_mxfp4_experts* experts, const void* x, const int32_
       fc2((float*)nullptr);
     }
   }
-  if (sum) {
-    CombineParams c{};
-    c.pairs = ws.y;
-    c.pairs_bf16 = narrow;
-    c.ids = ids;
-    c.weights = weights;
-    c.e_lo = experts->base;
-    c.e_n = experts->experts;
-    c.m = m;
-    c.topk = topk;
-    c.h = experts->hidden_out;
-    c.out = static_cast<uint16_t*>(out);
-    moe_launch_combine(c, s);
-  }
+  if (sum) combine(narrow);
   return launch_status();
 }
 

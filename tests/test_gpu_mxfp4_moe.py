@@ -39,7 +39,8 @@ SIZES = [  # rows, experts, top k, hidden, inter, gated
     (1, 8, 2, 256, 128, True), (1, 512, 10, 2048, 512, True), (1, 3, 3, 32, 32, True), (2, 16, 5, 96, 160, False), (4, 64, 22, 1024, 2688, False), (5, 7, 7, 544, 96, True),
     (13, 33, 4, 288, 224, True), (32, 100, 10, 512, 256, True), (40, 4, 2, 128, 64, False), (65, 24, 6, 256, 480, True), (150, 16, 3, 640, 128, False), (333, 12, 8, 256, 96, True), (1100, 9, 4, 96, 64, True), (512, 100, 1, 64, 96, False),
     (3, 9, 5, 2080, 2080, False), (2, 9, 6, 2144, 2080, True), (70, 6, 3, 1280, 1120, True), (30, 40, 4, 2080, 1056, False), (25, 90, 4, 1184, 96, True), (100, 4, 2, 1056, 1184, False),
-    (60, 3, 2, 640, 64, True), (20, 50, 4, 800, 64, True)]
+    (60, 3, 2, 640, 64, True), (20, 50, 4, 800, 64, True),
+    (700, 4, 3, 544, 352, True), (400, 3, 2, 1120, 1056, False), (129, 1, 1, 32, 32, True), (1500, 5, 4, 96, 2080, True), (260, 2, 2, 64, 96, False)]
 
 
 @pytest.mark.parametrize("m, e, k, hidden, inter, gated", SIZES)
