@@ -279,7 +279,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void mx_ring_kernel(MxTiles p) {
   const int total = gridDim.x, per = (total + 7) / 8, die = blockIdx.x % 8, whole = total % 8 ? total % 8 : 8;  // the first `whole` dies have `per` workgroups, the others one less
   const int at = die * per - (die > whole ? die - whole : 0) + (int)(blockIdx.x / 8);
   const int a0 = at % p.rows_of_tiles * Ring::TA, b0 = p.first + at / p.rows_of_tiles * Ring::TB;
-  const int pairs = la.quads / 2, q0 = 2 * (int)((int64_t)pairs * blockIdx.y / gridDim.y), q1 = 2 * (int)((int64_t)pairs * (blockIdx.y + 1) / gridDim.y);
+  const int quads = (la.chunks + 3) / 4, q0 = (int)((int64_t)quads * blockIdx.y / gridDim.y), q1 = (int)((int64_t)quads * (blockIdx.y + 1) / gridDim.y);
   Y* y = static_cast<Y*>(p.y) + (int64_t)blockIdx.y * p.m * p.n;
   const MxOperand a{p.a + (int64_t)a0 * la.chunks * 1024, p.a + la.codes() + (int64_t)a0 * la.quads * 256, la.tiles - a0};
   const MxOperand b{p.w + (int64_t)b0 * lw.chunks * 1024, p.w + lw.codes() + (int64_t)b0 * lw.quads * 256, lw.tiles - b0};

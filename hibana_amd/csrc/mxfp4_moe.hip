@@ -445,35 +445,32 @@ __global__ __launch_bounds__(64 * MX_MOE_WAVES, MT == 1 ? 3 : 2) void mx_fc2_man
 // The ring (mxfp4_ring.hpp) on the plan's slots of MX_RING_ROWS rows: the slot's rows of x rounded into the tile layout, fc1 with h rounded into it from
 // the accumulators, fc2 with each row's results to its pair.
 using MxMoeRing = MxRing<2, 2, 2, 2>;
-constexpr int MX_RING_ROWS = MxMoeRing::TA * MX_ROWS, MX_ROUND_CHUNKS = 4;
+constexpr int MX_RING_ROWS = MxMoeRing::TA * MX_ROWS;
 
-// A wavefront MX_ROUND_CHUNKS chunks of a tile of a slot: a lane its group of 32 values, whose codes are the 16 bytes that it owns, as where a linear's rows are
-// rounded; chunks past K have scale 0. The first workgroups of a slot also clear the scales of h behind its last group, which fc1 does
-// not write: what they would multiply is scaled by 2^-127 on the weights' side, but has to be finite.
-__global__ __launch_bounds__(256) void mx_gather_kernel(MxMoe p, MxLayout xs, MxLayout hs) {
+// The rounded rows (codes and scales by rows, as for the walk) into the tile layout of the slots, a wavefront a quad of chunks of a tile: a lane its group of 32
+// values in each, whose codes are the 16 bytes that it owns; groups past K have scale 0. (Each pair's row rounded here from x instead: 20 us for 16384
+// pairs of 2560, so 3 and 9.) The first workgroups of a slot also clear the scales of h behind its last group, which fc1 does not write: what they
+// would multiply is scaled by 2^-127 on the weights' side, but has to be finite.
+__global__ __launch_bounds__(256) void mx_gather_kernel(MxMoe p, MxLayout xs, MxLayout hs, const uint8_t* __restrict__ from_codes, const uint8_t* __restrict__ from_scales) {
   const int32_t* entry = p.plan + PLAN_HEADER + 4 * (int)blockIdx.y;
-  const int rows = entry[2], p0 = entry[1], lane = threadIdx.x & 63, tile = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int rows = entry[2], p0 = entry[1], lane = threadIdx.x & 63, half = lane >> 5, tile = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (MX_ROWS * tile >= rows) return;
-  const int r = min(MX_ROWS * tile + (lane & 31), rows - 1), row = p.order[p0 + r] / p.topk;  // (rows past the last: that one again)
-  const __bf16* x = static_cast<const __bf16*>(p.x) + (int64_t)row * p.k;
-  const int64_t at = (int64_t)blockIdx.y * MxMoeRing::TA + tile;
+  const int r = min(MX_ROWS * tile + (lane & 31), rows - 1);  // (rows past the last: that one again)
+  const int64_t row = p.order[p0 + r] / p.topk, at = (int64_t)blockIdx.y * MxMoeRing::TA + tile;
+  const int quad = blockIdx.x, groups = p.k / MX_GROUP;
   uint8_t *codes = const_cast<uint8_t*>(p.aq), *scales = const_cast<uint8_t*>(p.as);
+  uint32_t word = 8 * quad + half < groups ? *reinterpret_cast<const uint32_t*>(from_scales + row * mx_scale_row(p.k) + 8 * quad + 4 * half) : 0u;
 #pragma unroll
-  for (int u = 0; u < MX_ROUND_CHUNKS; u++) {
-    const int c = MX_ROUND_CHUNKS * blockIdx.x + u, group = 2 * c + (lane >> 5);
-    uint32_t byte = 0;
-    i32x4_t code = {0, 0, 0, 0};
-    if (group < p.k / MX_GROUP) {
-      MxGroup<__bf16> v;
-      v.load(x + MX_GROUP * group);
-      code = v.codes(byte);
-    }
-    if (c < xs.chunks) *reinterpret_cast<i32x4_t*>(codes + ((at * xs.chunks + c) * 64 + lane) * 16) = code;
-    scales[(at * xs.quads + (c >> 2)) * 256 + lane * 4 + (c & 3)] = (uint8_t)byte;
+  for (int u = 0; u < 4; u++) {
+    const int c = 4 * quad + u, group = 2 * c + half;
+    if (group >= groups) word &= ~(0xffu << (8 * u));
+    if (c < xs.chunks)
+      *reinterpret_cast<i32x4_t*>(codes + ((at * xs.chunks + c) * 64 + lane) * 16) = *reinterpret_cast<const i32x4_t*>(from_codes + row * (p.k / 2) + 16 * min(group, groups - 1));
   }
-  if (blockIdx.x == 0)
+  *reinterpret_cast<uint32_t*>(scales + (at * xs.quads + quad) * 256 + lane * 4) = word;
+  if (quad == 0)
     for (int c = p.inter / MX_K; c < hs.quads * 4; c++)
-      if (2 * c + (lane >> 5) >= p.inter / MX_GROUP) p.hs[(at * hs.quads + (c >> 2)) * 256 + lane * 4 + (c & 3)] = 0;
+      if (2 * c + half >= p.inter / MX_GROUP) p.hs[(at * hs.quads + (c >> 2)) * 256 + lane * 4 + (c & 3)] = 0;
 }
 
 // The slot and the tile of weight rows of a workgroup. Consecutive workgroups go to the eight dies in turn: a die takes two slots at a time, each with all
@@ -507,7 +504,7 @@ __global__ __launch_bounds__(64 * MxMoeRing::WAVES, 2) void mx_fc1_ring_kernel(M
   const MxLayout at(p.n, p.k), to(0, p.inter);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave >> 1, wn = wave & 1, r = lane & 31, g = lane >> 5;
   f32x16_t acc[MT][NT];
-  Ring::run(buf0, buf1, buf2, buf3, mx_slot_tiles(p, at, place.slot, rows), mx_expert_tiles(p, at, entry[0], place.column * Ring::TB), at.chunks, at.quads, 0, at.quads, acc);
+  Ring::run(buf0, buf1, buf2, buf3, mx_slot_tiles(p, at, place.slot, rows), mx_expert_tiles(p, at, entry[0], place.column * Ring::TB), at.chunks, at.quads, 0, (at.chunks + 3) / 4, acc);
   // A lane holds 16 of the 32 values of a row's group, lane ^ 32 the others: columns 8 q + 4 g .. + 3 in registers 4 q .. 4 q + 3. Each lane ends with
   // eight bytes of the group's codes, columns 16 g .. 16 g + 15.
 #pragma unroll
@@ -560,16 +557,21 @@ __global__ __launch_bounds__(64 * MxMoeRing::WAVES, 2) void mx_fc2_ring_kernel(M
   if (rows == 0) return;
   const MxLayout at(p.n, p.k);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave >> 1, wn = wave & 1;
+  int pair[MT];  // of the wavefront's rows, on their way beside the product
+#pragma unroll
+  for (int i = 0; i < MT; i++) pair[i] = p.order[entry[1] + min(MX_ROWS * (wm * MT + i) + (int)(threadIdx.x & 31), rows - 1)];
   f32x16_t acc[MT][NT];
-  Ring::run(buf0, buf1, buf2, buf3, mx_slot_tiles(p, at, place.slot, rows), mx_expert_tiles(p, at, entry[0], place.column * Ring::TB), at.chunks, at.quads, 0, at.quads, acc);
-  const int32_t* order = p.order + entry[1];
+  Ring::run(buf0, buf1, buf2, buf3, mx_slot_tiles(p, at, place.slot, rows), mx_expert_tiles(p, at, entry[0], place.column * Ring::TB), at.chunks, at.quads, 0, (at.chunks + 3) / 4, acc);
   i32x4_t* own = wave == 0 ? buf0 : wave == 1 ? buf1 : wave == 2 ? buf2 : buf3;
 #pragma unroll
   for (int i = 0; i < MT; i++) {
     const int row0 = MX_ROWS * (wm * MT + i);
     if (row0 >= rows) break;
     mx_store_rows<Y, NT>(own, p.n, (int64_t)(place.column * Ring::TB + wn * NT) * MX_ROWS, acc[i],
-                         [&](int r) { return row0 + r < rows ? static_cast<Y*>(p.y) + (int64_t)order[row0 + r] * p.n : nullptr; });
+                         [&](int r) {
+                           const int64_t to = __shfl(pair[i], r);
+                           return row0 + r < rows ? static_cast<Y*>(p.y) + to * p.n : nullptr;
+                         });
   }
 }
 
@@ -577,6 +579,7 @@ namespace {
 struct MxWorkspace {
   MoeWorkspace plan;
   uint8_t *xq, *xs, *hq, *hs;
+  uint8_t *aq, *as;  // on the ring: the slots' rows of x in the tile layout (h is in it too)
   void* y;
   size_t bytes;
 };
@@ -614,19 +617,17 @@ MxWorkspace carve(const hb_mxfp4_experts* ex, void* base, int64_t m, int topk, b
     w.plan.plan = reinterpret_cast<int32_t*>(take((PLAN_HEADER + (4 + DONE_PITCH) * moe_max_slots(pairs, ex->experts, 0, MX_ROWS) + 32) * sizeof(int32_t)));
     w.plan.plan_wide = reinterpret_cast<int32_t*>(take((size_t)64 * ex->experts * sizeof(int32_t)));
     w.plan.order = reinterpret_cast<int32_t*>(take((size_t)pairs * sizeof(int32_t)));
+    w.xq = take((size_t)m * (ex->hidden / 2));
+    w.xs = take((size_t)m * mx_scale_row(ex->hidden));
   }
   if (!few_pairs(pairs, ex->hidden, ex->inter) && on_ring(pairs, ex)) {
     const int64_t tiles = moe_max_slots(pairs, ex->experts, 0, MX_RING_ROWS) * MxMoeRing::TA;
     const MxLayout x(0, ex->hidden), h(0, ex->inter);
-    w.xq = take((size_t)tiles * x.chunks * 1024);
-    w.xs = take((size_t)tiles * x.quads * 256);
+    w.aq = take((size_t)tiles * x.chunks * 1024);
+    w.as = take((size_t)tiles * x.quads * 256);
     w.hq = take((size_t)tiles * h.chunks * 1024);
     w.hs = take((size_t)tiles * h.quads * 256);
   } else {
-    if (!few_pairs(pairs, ex->hidden, ex->inter)) {
-      w.xq = take((size_t)m * (ex->hidden / 2));
-      w.xs = take((size_t)m * mx_scale_row(ex->hidden));
-    }
     w.hq = take((size_t)pairs * (ex->inter / 2));
     w.hs = take((size_t)pairs * mx_scale_row(ex->inter));
   }
@@ -733,12 +734,13 @@ static int moe_pass(const hb_mxfp4_experts* experts, const void* x, const int32_
     if (on_ring(pairs, experts)) {
       const int64_t slots = moe_max_slots(pairs, experts->experts, 0, MX_RING_ROWS);
       if (int e = moe_launch_plan(ids, pairs, experts->base, experts->experts, 0, ws.plan, s, MX_RING_ROWS)) return e;
-      p1.x = x;
-      p1.aq = ws.xq;
-      p1.as = ws.xs;
+      const MxRound job{static_cast<const __bf16*>(x), (int64_t)m * (experts->hidden / 8), experts->hidden, ws.xq, ws.xs};
+      HB_LAUNCH(mx_quantize_rows_kernel, dim3((unsigned)((job.lanes + 255) / 256)), dim3(256), 0, s, job);
+      p1.aq = ws.aq;
+      p1.as = ws.as;
       p1.plan = p2.plan = ws.plan.plan;
       p1.order = p2.order = ws.plan.order;
-      HB_LAUNCH(mx_gather_kernel, dim3((unsigned)(l1.quads * 4 / MX_ROUND_CHUNKS), (unsigned)slots), dim3(64 * MxMoeRing::TA), 0, s, p1, l1, l2);
+      HB_LAUNCH(mx_gather_kernel, dim3((unsigned)l1.quads, (unsigned)slots), dim3(64 * MxMoeRing::TA), 0, s, p1, l1, l2, (const uint8_t*)ws.xq, (const uint8_t*)ws.xs);
       auto launch = [&](auto kernel, const MxLayout& at, const MxMoe& p) {
         const int columns = (at.tiles + MxMoeRing::TB - 1) / MxMoeRing::TB;
         HB_LAUNCH(kernel, dim3((unsigned)ring_groups(slots, p.n)), dim3(64 * MxMoeRing::WAVES), 0, s, p, (int)slots, columns);

@@ -8,8 +8,9 @@ namespace hb {
 typedef __attribute__((address_space(3))) uint8_t* mx_lds_t;
 
 // mx_mfma with the sum staying in its accumulator registers (left to itself the compiler moves 256 of them about) and the scales in byte
-// OP of their words. The two wait states in front cover an operand that a vector instruction has just written, and hide behind the matrix
-// instruction before (32 cycles); mx_sums_done stands before the sums are read.
+// OP of their words. The compiler does not know it for a matrix instruction, so what it has to wait for is waited for here: the two wait states in front cover
+// an operand that a vector instruction has just written, and hide behind the matrix instruction before (32 cycles); mx_sums_done ends every
+// block that the products stand in, so that whatever the compiler does to the sums between blocks comes after them.
 template <int OP>
 __device__ __forceinline__ void mx_mfma_in_place(f32x16_t& acc, i32x4_t a, i32x4_t b, uint32_t sa, uint32_t sb) {
 #define MX_MFMA(SELECT) \
@@ -50,10 +51,11 @@ struct MxRing {
   static constexpr int WAVES = WM * WN, TA = WM * MT, TB = WN * NT, T = TA + TB, SCALES = MT + NT;
   static constexpr int BUFFER = 2 * T * 64;  // [2 chunks][A tiles, B tiles][64]
   static_assert(TB % WAVES == 0);
+  static constexpr bool IN_PLACE = MT * NT > 8;  // the products in asm, which the compiler does not see
   static constexpr int ASKS_A = (2 * TA + WAVES - 1) / WAVES, ASKS_B = (2 * TB + WAVES - 1) / WAVES, ASKS = ASKS_A + ASKS_B;  // tiles a wavefront asks for a step
   static constexpr int LATE = ASKS_B / 2 + (TA % WAVES == 0 ? ASKS_A / 2 : 0);  // of those, what is of a step's second chunk for certain
 
-  // acc = the sums over quads q0 .. q1 - 1 (whole pairs of them) of the matrices' chunks and quads. The buffers are separate arrays of LDS, free
+  // acc = the sums over quads q0 .. q1 - 1 of the matrices' chunks and quads. The buffers are separate arrays of LDS, free
   // again when it returns.
   static __device__ __forceinline__ void run(i32x4_t (&buf0)[BUFFER], i32x4_t (&buf1)[BUFFER], i32x4_t (&buf2)[BUFFER], i32x4_t (&buf3)[BUFFER], const MxOperand& a,
                                              const MxOperand& b, int chunks, int quads, int q0, int q1, f32x16_t (&acc)[MT][NT]) {
@@ -118,47 +120,61 @@ struct MxRing {
     // front of them all, it and the barrier would leave the matrix cores idle for a fifth of the step. At its end what may still be on its way is
     // the step's own and the step's before LATE ones: the next step reads its own tiles, asked for two steps ago, and chunk 0 of the one behind it. (All of
     // that one waited for: 2048 rows of 25600 x 5120 148 us, so 144.5.)
-#define MX_STEP(CUR, NEXT, ASKED, S, ODD)                                                                                                  \
-    mx_unrolled<GROUPS>([&](auto group) {                                                                                                   \
-      constexpr int v = group.value, u = v / NT, j = v % NT, ring = (ODD) * GROUPS + v;                                                      \
-      fb[(ring + AHEAD) & 3] = v + AHEAD < GROUPS ? b_at(CUR, v + AHEAD) : b_at(NEXT, v + AHEAD - GROUPS);                                   \
-      _Pragma("unroll") for (int i = j * MT / NT; i < (j + 1) * MT / NT; i++) fa[1 - u][i] = u == 0 ? a_at(CUR, 1, i) : a_at(NEXT, 0, i);     \
-      mx_unrolled<MT>([&](auto tile) {                                                                                                      \
-        constexpr int i = tile.value, at = v * MT + i;  /* the step's product */                                                            \
-        mx_mfma_in_place<2 * (ODD) + u>(acc[i][j], fb[ring & 3], fa[u][i], now[MT + j], now[i]);                                             \
-        constexpr int ALL = GROUPS * MT, FIRST = (ALL + 3) / 4, H = (ODD) ? 0 : FIRST, W = ALL - FIRST;  /* asked for behind products H .. H + W - 1 */ \
-        constexpr int before = at < H ? 0 : at - H >= W ? ASKS : (at - H) * ASKS / W, after = at < H ? 0 : at + 1 - H >= W ? ASKS : (at + 1 - H) * ASKS / W; \
-        if constexpr (!(ODD)) {                                                                                                             \
-          constexpr int from = at >= H ? SCALES : at * SCALES / H, to = at >= H ? SCALES : (at + 1) * SCALES / H;                             \
-          mx_unrolled<to - from>([&](auto k) { scale(from + k.value, min((S) / 2 + 1, quads - 1)); });                                    \
-        }                                                                                                                                   \
-        mx_unrolled<after - before>([&](auto k) { MX_ASK(ASKED, (S) + 3, before + k.value) });                                              \
-        __builtin_amdgcn_sched_barrier(0);                                                                                                  \
-      });                                                                                                                                   \
-    });                                                                                                                                     \
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((ODD) ? ASKS + LATE : ASKS + LATE + SCALES) : "memory");                                       \
-    __builtin_amdgcn_s_barrier();                                                                                                           \
+#define MX_STEP(CUR, NEXT, ASKED, S, ODD)                                                                                                             \
+    mx_unrolled<GROUPS>([&](auto group) {                                                                                                             \
+      constexpr int v = group.value, u = v / NT, j = v % NT, ring = (ODD) * GROUPS + v;                                                               \
+      fb[(ring + AHEAD) & 3] = v + AHEAD < GROUPS ? b_at(CUR, v + AHEAD) : b_at(NEXT, v + AHEAD - GROUPS);                                            \
+      _Pragma("unroll") for (int i = j * MT / NT; i < (j + 1) * MT / NT; i++) fa[1 - u][i] = u == 0 ? a_at(CUR, 1, i) : a_at(NEXT, 0, i);             \
+      mx_unrolled<MT>([&](auto tile) {                                                                                                                \
+        constexpr int i = tile.value, at = v * MT + i;  /* the step's product */                                                                      \
+        if constexpr (IN_PLACE) {                                                                                                                     \
+          mx_mfma_in_place<2 * (ODD) + u>(acc[i][j], fb[ring & 3], fa[u][i], now[MT + j], now[i]);                                                    \
+        } else {                                                                                                                                      \
+          acc[i][j] = mx_mfma<2 * (ODD) + u, 2 * (ODD) + u>(fb[ring & 3], now[MT + j], fa[u][i], now[i], acc[i][j]);                                  \
+        }                                                                                                                                             \
+        constexpr int ALL = GROUPS * MT, FIRST = (ALL + 3) / 4, H = (ODD) ? 0 : FIRST, W = ALL - FIRST;  /* asked for behind products H .. H + W - 1 */\
+        constexpr int before = at < H ? 0 : at - H >= W ? ASKS : (at - H) * ASKS / W;                                                                 \
+        constexpr int after = at < H ? 0 : at + 1 - H >= W ? ASKS : (at + 1 - H) * ASKS / W;                                                          \
+        if constexpr (!(ODD)) {                                                                                                                       \
+          constexpr int from = at >= H ? SCALES : at * SCALES / H, to = at >= H ? SCALES : (at + 1) * SCALES / H;                                     \
+          mx_unrolled<to - from>([&](auto k) { scale(from + k.value, min((S) / 2 + 1, quads - 1)); });                                                \
+        }                                                                                                                                             \
+        mx_unrolled<after - before>([&](auto k) { MX_ASK(ASKED, (S) + 3, before + k.value) });                                                        \
+        __builtin_amdgcn_sched_barrier(0);                                                                                                            \
+      });                                                                                                                                             \
+    });                                                                                                                                               \
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((ODD) ? ASKS + LATE : ASKS + LATE + SCALES) : "memory");                                                 \
+    __builtin_amdgcn_s_barrier();                                                                                                                     \
     __builtin_amdgcn_sched_barrier(0);
 #define MX_QUAD                                                               \
     _Pragma("unroll") for (int t = 0; t < SCALES; t++) now[t] = next[t];
-    for (int q = q0; q < q1; q += 2) {
+    int q = q0;
+    for (; q + 1 < q1; q += 2) {
       MX_QUAD
       MX_STEP(buf0, buf1, buf3, 2 * q, 0)
       MX_STEP(buf1, buf2, buf0, 2 * q + 1, 1)
       MX_QUAD
       MX_STEP(buf2, buf3, buf1, 2 * q + 2, 0)
       MX_STEP(buf3, buf0, buf2, 2 * q + 3, 1)
+      if (IN_PLACE) mx_sums_done();
+    }
+    if (q < q1) {
+      MX_QUAD
+      MX_STEP(buf0, buf1, buf3, 2 * q, 0)
+      MX_STEP(buf1, buf2, buf0, 2 * q + 1, 1)
+      if (IN_PLACE) mx_sums_done();
     }
 #undef MX_QUAD
 #undef MX_STEP
 #undef MX_ASK
 #undef MX_ASK_OF
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // what was asked for past the end arrives before the workgroup leaves its LDS
-    mx_sums_done();
+    if constexpr (IN_PLACE) {
 #pragma unroll
-    for (int i = 0; i < MT; i++)
+      for (int i = 0; i < MT; i++)
 #pragma unroll
-      for (int j = 0; j < NT; j++) asm volatile("" : "+a"(acc[i][j]));
+        for (int j = 0; j < NT; j++) asm volatile("" : "+a"(acc[i][j]));
+    }
     __builtin_amdgcn_s_barrier();  // every wavefront has left the ring
   }
 };
