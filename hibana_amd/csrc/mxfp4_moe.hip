@@ -593,9 +593,10 @@ int most_rows(const hb_mxfp4_experts* ex, int topk) {
 
 bool few_pairs(int64_t pairs, int hidden, int inter) { return pairs <= MX_SCAN_PAIRS && MxActs::bytes(std::min<int64_t>(pairs, MX_ROWS), std::max(hidden, inter)) <= 64 * 1024; }
 
-// From this many pairs an expert on (were they shared out evenly) a call runs on the ring: a slot of 128 rows of one expert fills its tiles then, and the rows
-// are worth being laid out.
-constexpr int MX_RING_PAIRS = 64;
+// From this many pairs an expert on (were they shared out evenly) a call runs on the ring: a slot of 128 rows of one expert half fills its tiles then, and
+// the rows are worth being laid out. us, walk and ring, 64 experts (2048, 768): 48 pairs each 71 and 79, 64 94 and 82; 256 experts (2048, 512): 146 and
+// 160, 181 and 168; 64 of ReLU^2 (1024, 2560), 62 each, 98 and 79.
+constexpr int MX_RING_PAIRS = 56;
 int fc1_rows(const hb_mxfp4_experts* ex) { return ex->gated ? 2 * ex->inter : ex->inter; }
 int64_t ring_groups(int64_t slots, int columns) { return (slots + 15) / 16 * 16 * ((columns + 32 * MxMoeRing::TB - 1) / (32 * MxMoeRing::TB)); }
 bool on_ring(int64_t pairs, const hb_mxfp4_experts* ex) {
