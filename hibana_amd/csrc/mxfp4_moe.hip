@@ -94,7 +94,8 @@ __device__ __forceinline__ void mx_emit_h(const MxMoe& p, const f32x4_t& h, int 
 
 // ------------------------------------------------------------------------------------------------ few pairs
 // fc1: a workgroup two weight tiles of the slot that begins at pair blockIdx.y (none: it leaves). The slot's expert is known from one
-// id, so the weights are on their way while the slot's rows are looked for and their activations rounded into LDS.
+// id, so the weights are on their way while the slot's rows are looked for and their activations rounded into LDS. Latency bound: one row of 10 of 512
+// experts (2048, 512) 5.8 us for 11 MB of weights.
 constexpr int MX_FEW_WAVES = 8;
 // PARTS lanes a group: values(acts, row of the slot, group, part, pair) puts it there.
 template <int RUN, int PARTS, class Values>
@@ -155,13 +156,11 @@ __global__ __launch_bounds__(64 * MX_FEW_WAVES, RUN == 4 ? 2 : 4) void mx_fc2_fe
 }
 
 // fc2 and the weighted sum of one row (blockIdx.y): a workgroup one tile of columns, its wavefronts the row's pairs in turn, their weighted
-// results added in wavefront order. Reads a row's experts whether or not other rows name them too.
+// results added in wavefront order. Reads a row's experts whether or not other rows name them too. 4.9 us behind the fc1 above, latency too.
 constexpr int MX_ROW_WAVES = 8;
 // ... where a wavefront's share is short: up to this many chunks of a row's pairs. One row of 10 of 512 experts (2048, 512), 80 chunks, fc2 so and as slots
 // with a combine: 16.4 and 19.0 us the call, four rows 25.7 and 32.6; of 22 (1024, 2688), 924 chunks, one row 39.5 and 30.4.
 constexpr int MX_ROW_CHUNKS = 128;
-constexpr int MX_MANY_GROUPS = 1536;
-constexpr int MX_PLAN_PAIRS = 1024;  // from here the plan's launches share the pairs
 __global__ __launch_bounds__(64 * MX_ROW_WAVES, 2) void mx_fc2_row_kernel(MxMoe p) {
   __shared__ f32x4_t part[MX_ROW_WAVES * 4 * 8];
   const MxLayout at(p.n, p.k);
@@ -216,10 +215,18 @@ __global__ __launch_bounds__(64 * MX_ROW_WAVES, 2) void mx_fc2_row_kernel(MxMoe 
 }
 
 // ------------------------------------------------------------------------------------------------ many pairs
+constexpr int MX_PLAN_PAIRS = 1024;  // from here the plan's launches share the pairs
+// Workgroups of a product, about six a compute unit where there are so many: each has several units then, whose weights it asks for ahead. us, 1543 rows of 10
+// of 512 experts (2048, 512), repeated on 2.5 GB of weights: 384 278, 768 251, 1536 240, 3072 250.
+constexpr int MX_MANY_GROUPS = 1536;
+// From this many pairs an expert slots have 64 rows, whose products share a weight tile's registers: 240 us against 292 for the call above (30 pairs an
+// expert), 71 and 74 for 300 rows of 8 of 64 (2048, 768); verify-sized calls are the same either way and keep the registers.
+constexpr int MX_TALL_PAIRS = 24;
 // A wavefront's walk over steps of eight chunks of two weight tiles, for a slot of the plan (up to 32 MT rows of an expert). A step's weights, 16 KB
 // a wavefront, are asked for as soon as the step before has taken its own out of the registers, so they are on their way while sums
 // are joined, rounded and stored; a slot's activations (32 bytes of a row's chunk, read where they lie) stay in registers where one
-// step covers the wavefront's K.
+// step covers the wavefront's K. Bound by reading the weights: 1543 rows of 10 of 512 experts (2048, 512) fc1 114 us, 5.0 TB/s, fc2 73 us, 4.7 with its
+// results; 32 rows 24 and 13 us, 5.1 and 4.7; four rows of 22 of 512 ReLU^2 experts (1024, 2688) 23 and 23 us, 5.2.
 // x [rows, k] rounded for the products of many pairs, eight values a lane: codes by rows, scales as above (a last odd group's partner at 0).
 struct MxRound {
   const __bf16* x;
@@ -442,8 +449,9 @@ __global__ __launch_bounds__(64 * MX_MOE_WAVES, MT == 1 ? 3 : 2) void mx_fc2_man
 }
 
 // ------------------------------------------------------------------------------------------------ many pairs an expert
-// The ring (mxfp4_ring.hpp) on the plan's slots of MX_RING_ROWS rows: the slot's rows of x rounded into the tile layout, fc1 with h rounded into it from
-// the accumulators, fc2 with each row's results to its pair.
+// The ring (mxfp4_ring.hpp) on the plan's slots of MX_RING_ROWS rows: the slot's rounded rows of x brought into the tile layout, fc1 with h rounded into it
+// from the accumulators, fc2 with each row's results to its pair. 2048 rows of 8 of 64 experts (2560, 768), 256 rows each: gather 10.6 us, fc1 66
+// (1.9 PFLOP/s, 9 TB/s into LDS), fc2 53 (1.2: six steps a workgroup, beside which its start and end are long, and 84 MB of results).
 using MxMoeRing = MxRing<2, 2, 2, 2>;
 constexpr int MX_RING_ROWS = MxMoeRing::TA * MX_ROWS;
 
@@ -755,7 +763,7 @@ static int moe_pass(const hb_mxfp4_experts* experts, const void* x, const int32_
       if (sum) combine(narrow);
       return launch_status();
     }
-    const bool tall = pairs >= (int64_t)experts->experts * 24;
+    const bool tall = pairs >= (int64_t)MX_TALL_PAIRS * experts->experts;
     const int slot_rows = tall ? 2 * MX_ROWS : MX_ROWS;
     const int64_t slots = moe_max_slots(pairs, experts->experts, 0, slot_rows);
     const MxRound job{static_cast<const __bf16*>(x), (int64_t)m * (experts->hidden / 8), experts->hidden, ws.xq, ws.xs};
@@ -771,7 +779,6 @@ static int moe_pass(const hb_mxfp4_experts* experts, const void* x, const int32_
     p1.order = p2.order = ws.plan.order;
     p1.aq = ws.xq;
     p1.as = ws.xs;
-    // about six workgroups a compute unit where there are so many: each then has several units, whose weights it asks for ahead
     const int64_t busy = std::min<int64_t>(slots, pairs / slot_rows + std::min<int64_t>(pairs, experts->experts) / 2 + 1);
     auto span_of = [&](int64_t units, int64_t by) {
       const int64_t spans = std::max<int64_t>(1, std::min<int64_t>((units + by - 1) / by, (MX_MANY_GROUPS + busy - 1) / busy));
