@@ -203,14 +203,17 @@ __global__ __launch_bounds__(512) void mx_few_rows_kernel(MxLinear p) {
   constexpr int AT_ONCE = std::is_same_v<T, float> ? 4 : 8;
   MxStream<NT, RUN> s;
   const MxLayout at(p.n, p.k);
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), t0 = blockIdx.x * NT, rows = (int)p.m, groups = p.k / MX_GROUP;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), t0 = blockIdx.x * NT, groups = p.k / MX_GROUP;
+  const int64_t row0 = (int64_t)blockIdx.y * MX_ROWS;
+  const int rows = (int)min((int64_t)MX_ROWS, p.m - row0);
   const MxActs acts(part, rows, p.k);
   // Loads return in order: the first activations are asked for ahead of the weights, or they would stand behind all of them while nothing else is on its way.
   if constexpr (std::is_same_v<T, uint8_t>) {
     const int all = rows * groups;
+    const uint8_t *x = static_cast<const uint8_t*>(p.x) + row0 * (p.k / 2), *x_scales = p.x_scales + row0 * groups;
     auto source = [&](int i, i32x4_t& code, uint32_t& scale) {
-      code = *reinterpret_cast<const i32x4_t*>(static_cast<const uint8_t*>(p.x) + 16 * (int64_t)i);
-      scale = p.x_scales[i];
+      code = *reinterpret_cast<const i32x4_t*>(x + 16 * (int64_t)i);
+      scale = x_scales[i];
     };
     auto put = [&](int i, const i32x4_t& code, uint32_t scale) {
       const int r = i / groups, at = (i - r * groups) * rows + r;
@@ -233,7 +236,8 @@ __global__ __launch_bounds__(512) void mx_few_rows_kernel(MxLinear p) {
   } else {
     const int all = rows * groups * 4;  // eight values from 8 i of the contiguous rows a lane
     const uint32_t inverse = 0xffffffffu / (uint32_t)groups + 1u;  // i / groups = the upper half of i inverse: i below 32 groups, groups below 2^13
-    auto source = [&](Mx8<T>& v, int i) { v.load(static_cast<const T*>(p.x) + 8 * (int64_t)min(i, all - 1)); };
+    const T* x = static_cast<const T*>(p.x) + row0 * p.k;
+    auto source = [&](Mx8<T>& v, int i) { v.load(x + 8 * (int64_t)min(i, all - 1)); };
     auto put = [&](int i, const Mx8<T>& v) {
       const int r = groups == 1 ? i >> 2 : (int)__umulhi((uint32_t)i >> 2, inverse);
       if (i < all) acts.put(r, (i >> 2) - r * groups, i & 3, v);
@@ -258,7 +262,7 @@ __global__ __launch_bounds__(512) void mx_few_rows_kernel(MxLinear p) {
   for (int i = threadIdx.x; i < NT * 256; i += blockDim.x) {
     const f32x4_t sum = mx_joined<NT>(part, p.waves, i);
     const int l = i & 63, q = (i >> 6) & 3, t = t0 + (i >> 8);
-    const int64_t row = l & 31, n = (int64_t)t * MX_ROWS + 8 * q + 4 * (l >> 5);
+    const int64_t row = row0 + (l & 31), n = (int64_t)t * MX_ROWS + 8 * q + 4 * (l >> 5);
     if (row < p.m && n < p.n) mx_store4<Y>(static_cast<Y*>(p.y) + row * p.n + n, sum, p.n - n, p.n % 4 == 0);
   }
 }
@@ -348,17 +352,25 @@ struct MxPlan {
   size_t tiles, bytes;  // workspace: of the activations, of all
 };
 // Few rows (their activations fit LDS): a wavefront's chunks of K and few weight rows a workgroup keep a small matrix's call short, and the rounding rides
-// in it while all of a workgroup's rows are not more than MX_ROUND_VALUES values; past that it is a launch of its own. Where the matrix alone
-// fills the device several times over, the ring takes over from there. us, 25600 x 5120: 8 rows 17.8 rounding inside, 17.4 ring; 16 rows 20.7 and
-// 17.3; 5120 x 5120: 8 rows 8.6 inside, 14.4 ring; 16 rows 10.6 inside, 7.4 and 2 for a launch of its own, 14.3 ring.
-constexpr int64_t MX_ROUND_VALUES = 48 * 1024;
+// in it while all of a workgroup's rows are not more than MX_ROUND_VALUES values; past that it is a launch of its own. us in a graph and called one by one,
+// 20 rows of 4000 x 4096 (80 K values): inside 9.4 and 8.7, ahead 8.6 and 11.9; 31 rows of it (124 K) 11.5 and 10.7, 9.0 and 11.7. Where the matrix alone
+// fills the device several times over, the ring takes over from there: 8 rows of 25600 x 5120 17.8 rounding inside, 17.4 ring; 16 rows 20.7 and 17.3.
+constexpr int64_t MX_ROUND_VALUES = 80 * 1024;
 constexpr int MX_RING_TILES = 768;
+// More rows of a small matrix are passes of 32 rows beside one another, which read its weights again: one launch where the ring takes two, or three with K shared.
+// Up to MX_PASS_VALUES values a pass, and MX_PASSES_WORK of tiles x passes x k. us as above: 128 rows of 4000 x 832 (416 K) passes 7.4 and 8.1, ring 9.8 and
+// 11.4; 256 rows (832 K) 10.2 and 9.4, 9.6 and 11.4; 512 rows 15.5 and 14.5, 10.1 and 11.3; 128 rows of 1000 x 4000 (512 K) 11.5 and 10.6, 13.2 and 14.4.
+constexpr int64_t MX_PASS_VALUES = 128 * 1024, MX_PASSES_WORK = 768 * 1024;
 constexpr int MX_DEVICE = 256;  // compute units
 static MxPlan plan_of(int64_t m, int64_t n, int k, int x_type) {
   const MxLayout rows(m, k), w(n, k);
   MxPlan p{};
   const size_t acts = MxActs::bytes(m, k);
   const bool small = m * k <= MX_ROUND_VALUES;
+  if (m > MX_ROWS && (int64_t)MX_ROWS * k <= MX_PASS_VALUES && (int64_t)rows.tiles * w.tiles * k <= MX_PASSES_WORK) {
+    p.way = MxPlan::FEW_ROUNDING;
+    return p;
+  }
   if (m <= MX_ROWS && acts <= (w.tiles <= 256 ? 144 : 64) * 1024 && (small || w.tiles < MX_RING_TILES)) {
     const bool rounds = x_type != HB_MXFP4 && !small;
     p.way = rounds ? MxPlan::FEW : MxPlan::FEW_ROUNDING;
@@ -402,7 +414,7 @@ static int launch_ring(MxTiles p, const MxPlan& plan, float* sums, hipStream_t s
 
 template <typename T, typename Y, int NT, int RUN>
 static int launch_few(const MxLinear& p, const MxLayout& at, hipStream_t stream) {
-  const size_t lds = std::max(MxActs::bytes(p.m, p.k), (size_t)p.waves * NT * 4096);
+  const size_t lds = std::max(MxActs::bytes(std::min<int64_t>(p.m, MX_ROWS), p.k), (size_t)p.waves * NT * 4096);
   if (lds > 64 * 1024) {
     // set for a device once: the attribute is the loaded kernel's, and each device has its own
     static std::atomic<uint64_t> raised{0};
@@ -414,7 +426,7 @@ static int launch_few(const MxLinear& p, const MxLayout& at, hipStream_t stream)
       raised.fetch_or(bit, std::memory_order_release);
     }
   }
-  HB_LAUNCH((mx_few_rows_kernel<T, Y, NT, RUN>), dim3((unsigned)((at.tiles + NT - 1) / NT)), dim3(64 * p.waves), lds, stream, p);
+  HB_LAUNCH((mx_few_rows_kernel<T, Y, NT, RUN>), dim3((unsigned)((at.tiles + NT - 1) / NT), (unsigned)((p.m + MX_ROWS - 1) / MX_ROWS)), dim3(64 * p.waves), lds, stream, p);
   return HB_OK;
 }
 
