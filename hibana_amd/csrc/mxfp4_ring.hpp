@@ -23,16 +23,24 @@ __device__ __forceinline__ void mx_mfma_in_place(f32x16_t& acc, i32x4_t a, i32x4
 }
 __device__ __forceinline__ void mx_sums_done() { asm volatile("s_nop 15\n\ts_nop 15" ::: "memory"); }
 
-// Four neighbouring results of a row, `left` of them inside the matrix.
+// A vector that starts where its elements do.
+template <typename V, typename E>
+struct __attribute__((packed, aligned(sizeof(E)), may_alias)) MxLoose {
+  V v;
+};
+// Four neighbouring results of a row, `left` of them inside the matrix; `whole`: rows start on four.
 template <typename Y>
 __device__ __forceinline__ void mx_store4(Y* out, const f32x4_t& v, int64_t left, bool whole) {
+  typedef __attribute__((ext_vector_type(4))) Y y4_t;
+  const y4_t y = {mx_out<Y>(v[0]), mx_out<Y>(v[1]), mx_out<Y>(v[2]), mx_out<Y>(v[3])};
   if (whole) {
-    typedef __attribute__((ext_vector_type(4))) Y y4_t;
-    *reinterpret_cast<y4_t*>(out) = y4_t{mx_out<Y>(v[0]), mx_out<Y>(v[1]), mx_out<Y>(v[2]), mx_out<Y>(v[3])};
+    *reinterpret_cast<y4_t*>(out) = y;
+  } else if (left >= 4) {
+    reinterpret_cast<MxLoose<y4_t, Y>*>(out)->v = y;
   } else {
 #pragma unroll
-    for (int j = 0; j < 4; j++)
-      if (j < left) out[j] = mx_out<Y>(v[j]);
+    for (int j = 0; j < 3; j++)
+      if (j < left) out[j] = y[j];
   }
 }
 
@@ -181,24 +189,13 @@ struct MxRing {
 
 // 32 rows x NT tiles of a wavefront's sums, stored. A lane holds four columns of one row, 8 or 16 bytes: stored as they are, an instruction
 // would touch 32 rows' lines. They go through the wavefront's own part of LDS and leave as whole rows of NT x 32 columns, 16 bytes a
-// lane; a row's 16-byte pieces are XORed with its number so that neither way meets a bank twice. (Where rows do not start on 16 bytes: as
-// they are.)
-// row_at(r): where column 0 of the tile's row r goes, or null.
+// lane; a row's 16-byte pieces are XORed with its number so that neither way meets a bank twice. Where rows do not start on 16 bytes the stores do not either, and a
+// row's last piece is stored by columns. (Each lane its four columns, one by one, there: 2000 rows of 2049 x 2048 30.4 us, so 17.4.) row_at(r):
+// where column 0 of the tile's row r goes, or null.
 template <typename Y, int NT, class RowAt>
 __device__ __forceinline__ void mx_store_rows(i32x4_t* place, int64_t columns, int64_t n0, const f32x16_t (&sums)[NT], RowAt&& row_at) {
-  constexpr int PIECES = NT * MX_ROWS * (int)sizeof(Y) / 16, ROWS = 64 / PIECES > 0 ? 64 / PIECES : 1;
+  constexpr int PIECES = NT * MX_ROWS * (int)sizeof(Y) / 16, ROWS = 64 / PIECES > 0 ? 64 / PIECES : 1, EACH = 16 / (int)sizeof(Y);
   const int lane = threadIdx.x & 63, r = lane & 31, g = lane >> 5;
-  if (columns * (int)sizeof(Y) % 16) {
-    Y* row = row_at(r);
-#pragma unroll
-    for (int j = 0; j < NT; j++)
-#pragma unroll
-      for (int q = 0; q < 4; q++) {
-        const int64_t n = n0 + MX_ROWS * j + 8 * q + 4 * g;
-        if (row && n < columns) mx_store4<Y>(row + n, mx_quarter(sums[j], q), columns - n, false);
-      }
-    return;
-  }
   uint8_t* bytes = reinterpret_cast<uint8_t*>(place);
 #pragma unroll
   for (int j = 0; j < NT; j++)
@@ -207,13 +204,31 @@ __device__ __forceinline__ void mx_store_rows(i32x4_t* place, int64_t columns, i
       const int at = (MX_ROWS * j + 8 * q + 4 * g) * (int)sizeof(Y), piece = (at / 16) ^ (r & (PIECES - 1));
       mx_store4<Y>(reinterpret_cast<Y*>(bytes + (r * PIECES + piece) * 16 + at % 16), mx_quarter(sums[j], q), 4, true);
     }
+  auto store = [&](auto whole) {
 #pragma unroll
-  for (int first = 0; first < MX_ROWS; first += ROWS) {
-    const int row = first + lane / PIECES, piece = lane % PIECES;
-    const int64_t n = n0 + piece * (16 / (int)sizeof(Y));
-    const i32x4_t v = place[row * PIECES + (piece ^ (row & (PIECES - 1)))];
-    Y* to = row_at(row);
-    if (to && n < columns) *reinterpret_cast<i32x4_t*>(to + n) = v;
+    for (int first = 0; first < MX_ROWS; first += ROWS) {
+      const int row = first + lane / PIECES, piece = lane % PIECES;
+      const int64_t n = n0 + piece * EACH;
+      const i32x4_t v = place[row * PIECES + (piece ^ (row & (PIECES - 1)))];
+      Y* to = row_at(row);
+      if (!to || n >= columns) continue;
+      if constexpr (decltype(whole)::value) {
+        *reinterpret_cast<i32x4_t*>(to + n) = v;
+      } else if (n + EACH <= columns) {
+        reinterpret_cast<MxLoose<i32x4_t, Y>*>(to + n)->v = v;
+      } else {
+        typedef __attribute__((ext_vector_type(EACH))) Y ys_t;
+        const ys_t y = __builtin_bit_cast(ys_t, v);
+#pragma unroll
+        for (int e = 0; e < EACH - 1; e++)
+          if (n + e < columns) to[n + e] = y[e];
+      }
+    }
+  };
+  if (columns % EACH == 0) {
+    store(std::true_type());
+  } else {
+    store(std::false_type());
   }
 }
 
