@@ -449,36 +449,46 @@ __global__ __launch_bounds__(64 * MX_MOE_WAVES, MT == 1 ? 3 : 2) void mx_fc2_man
 }
 
 // ------------------------------------------------------------------------------------------------ many pairs an expert
-// The ring (mxfp4_ring.hpp) on the plan's slots of MX_RING_ROWS rows: the slot's rounded rows of x brought into the tile layout, fc1 with h rounded into it
-// from the accumulators, fc2 with each row's results to its pair. 2048 rows of 8 of 64 experts (2560, 768), 256 rows each: gather 10.6 us, fc1 66
-// (1.9 PFLOP/s, 9 TB/s into LDS), fc2 53 (1.2: six steps a workgroup, beside which its start and end are long, and 84 MB of results).
+// The ring (mxfp4_ring.hpp) on the plan's slots of MX_RING_ROWS rows: the slot's rows of x rounded into the tile layout, fc1 with h rounded into it
+// from the accumulators, fc2 with each row's results to its pair. 2048 rows of 8 of 64 experts (2560, 768), 256 rows each: gather 15 us, fc1 64
+// (2.0 PFLOP/s, 9 TB/s into LDS), fc2 51 (1.3: six steps a workgroup, beside which its start and end are long, and 84 MB of results).
 using MxMoeRing = MxRing<2, 2, 2, 2>;
 constexpr int MX_RING_ROWS = MxMoeRing::TA * MX_ROWS;
 
-// The rounded rows (codes and scales by rows, as for the walk) into the tile layout of the slots, a wavefront a quad of chunks of a tile: a lane its group of 32
-// values in each, whose codes are the 16 bytes that it owns; groups past K have scale 0. (Each pair's row rounded here from x instead: 20 us for 16384
-// pairs of 2560, so 3 and 9.) The first workgroups of a slot also clear the scales of h behind its last group, which fc1 does not write: what they
-// would multiply is scaled by 2^-127 on the weights' side, but has to be finite.
-__global__ __launch_bounds__(256) void mx_gather_kernel(MxMoe p, MxLayout xs, MxLayout hs, const uint8_t* __restrict__ from_codes, const uint8_t* __restrict__ from_scales) {
-  const int32_t* entry = p.plan + PLAN_HEADER + 4 * (int)blockIdx.y;
-  const int rows = entry[2], p0 = entry[1], lane = threadIdx.x & 63, half = lane >> 5, tile = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (MX_ROWS * tile >= rows) return;
-  const int r = min(MX_ROWS * tile + (lane & 31), rows - 1);  // (rows past the last: that one again)
-  const int64_t row = p.order[p0 + r] / p.topk, at = (int64_t)blockIdx.y * MxMoeRing::TA + tile;
-  const int quad = blockIdx.x, groups = p.k / MX_GROUP;
-  uint8_t *codes = const_cast<uint8_t*>(p.aq), *scales = const_cast<uint8_t*>(p.as);
-  uint32_t word = 8 * quad + half < groups ? *reinterpret_cast<const uint32_t*>(from_scales + row * mx_scale_row(p.k) + 8 * quad + 4 * half) : 0u;
+// Rounding into the tile layout: a wavefront eight rows of a tile (`first` of them on) and a quad of chunks, eight lanes a row's 64 values, a quarter of a
+// group each, so that a load instruction's lanes share eight whole lines and a store's two. (A lane a group, as the layout has it and a linear's rows are
+// rounded, 16384 gathered rows of 2560 took 20 us, so 15.) x: the lane's row; groups past K have scale 0.
+__device__ __forceinline__ void mx_round_quad(const __bf16* x, int k, int chunks, int quad, int first, uint8_t* tile_codes, uint8_t* quad_scales) {
+  const int lane = threadIdx.x & 63, part = lane & 3, half = (lane >> 2) & 1, row = first + (lane >> 3), groups = k / MX_GROUP;
+  Mx8<__bf16> v[4];
+#pragma unroll
+  for (int u = 0; u < 4; u++) v[u].load(x + MX_GROUP * (int64_t)min(2 * (4 * quad + u) + half, groups - 1) + 8 * part);
+  uint32_t word = 0;
 #pragma unroll
   for (int u = 0; u < 4; u++) {
-    const int c = 4 * quad + u, group = 2 * c + half;
-    if (group >= groups) word &= ~(0xffu << (8 * u));
-    if (c < xs.chunks)
-      *reinterpret_cast<i32x4_t*>(codes + ((at * xs.chunks + c) * 64 + lane) * 16) = *reinterpret_cast<const i32x4_t*>(from_codes + row * (p.k / 2) + 16 * min(group, groups - 1));
+    const int c = 4 * quad + u;
+    const bool in = 2 * c + half < groups;
+    const uint32_t byte = in ? mx_scale_byte(quad_max(v[u].amax())) : 0u;
+    word |= byte << (8 * u);
+    if (c < chunks) reinterpret_cast<uint32_t*>(tile_codes + (int64_t)c * 1024 + (32 * half + row) * 16)[part] = in ? v[u].codes(mx_scale_value(byte)) : 0u;
   }
-  *reinterpret_cast<uint32_t*>(scales + (at * xs.quads + quad) * 256 + lane * 4) = word;
+  if (part == 0) reinterpret_cast<uint32_t*>(quad_scales)[32 * half + row] = word;
+}
+// The slots' rows of x rounded into the tile layout, a workgroup a quad of a tile. The first workgroups of a tile also clear the scales of h behind its last
+// group, which fc1 does not write: what they would multiply is scaled by 2^-127 on the weights' side, but has to be finite. (Rows rounded once and their
+// codes gathered took a launch more: 5.4 and 10.6 us.)
+__global__ __launch_bounds__(256) void mx_gather_kernel(MxMoe p, MxLayout xs, MxLayout hs) {
+  const int32_t* entry = p.plan + PLAN_HEADER + 4 * (int)blockIdx.y;
+  const int rows = entry[2], p0 = entry[1], lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int tile = blockIdx.x % MxMoeRing::TA, quad = blockIdx.x / MxMoeRing::TA;
+  if (MX_ROWS * tile >= rows) return;
+  const int64_t at = (int64_t)blockIdx.y * MxMoeRing::TA + tile;
+  const int r = min(MX_ROWS * tile + 8 * wave + (lane >> 3), rows - 1);  // (rows past the last: that one again)
+  const __bf16* x = static_cast<const __bf16*>(p.x) + (int64_t)(p.order[p0 + r] / p.topk) * p.k;
+  mx_round_quad(x, p.k, xs.chunks, quad, 8 * wave, const_cast<uint8_t*>(p.aq) + at * xs.chunks * 1024, const_cast<uint8_t*>(p.as) + (at * xs.quads + quad) * 256);
   if (quad == 0)
-    for (int c = p.inter / MX_K; c < hs.quads * 4; c++)
-      if (2 * c + half >= p.inter / MX_GROUP) p.hs[(at * hs.quads + (c >> 2)) * 256 + lane * 4 + (c & 3)] = 0;
+    for (int c = p.inter / MX_K + wave; c < hs.quads * 4; c += 4)
+      if (2 * c + (lane >> 5) >= p.inter / MX_GROUP) p.hs[(at * hs.quads + (c >> 2)) * 256 + lane * 4 + (c & 3)] = 0;
 }
 
 // The slot and the tile of weight rows of a workgroup. Consecutive workgroups go to the eight dies in turn: a die takes two slots at a time, each with all
@@ -587,7 +597,6 @@ namespace {
 struct MxWorkspace {
   MoeWorkspace plan;
   uint8_t *xq, *xs, *hq, *hs;
-  uint8_t *aq, *as;  // on the ring: the slots' rows of x in the tile layout (h is in it too)
   void* y;
   size_t bytes;
 };
@@ -626,17 +635,19 @@ MxWorkspace carve(const hb_mxfp4_experts* ex, void* base, int64_t m, int topk, b
     w.plan.plan = reinterpret_cast<int32_t*>(take((PLAN_HEADER + (4 + DONE_PITCH) * moe_max_slots(pairs, ex->experts, 0, MX_ROWS) + 32) * sizeof(int32_t)));
     w.plan.plan_wide = reinterpret_cast<int32_t*>(take((size_t)64 * ex->experts * sizeof(int32_t)));
     w.plan.order = reinterpret_cast<int32_t*>(take((size_t)pairs * sizeof(int32_t)));
-    w.xq = take((size_t)m * (ex->hidden / 2));
-    w.xs = take((size_t)m * mx_scale_row(ex->hidden));
   }
   if (!few_pairs(pairs, ex->hidden, ex->inter) && on_ring(pairs, ex)) {
     const int64_t tiles = moe_max_slots(pairs, ex->experts, 0, MX_RING_ROWS) * MxMoeRing::TA;
     const MxLayout x(0, ex->hidden), h(0, ex->inter);
-    w.aq = take((size_t)tiles * x.chunks * 1024);
-    w.as = take((size_t)tiles * x.quads * 256);
+    w.xq = take((size_t)tiles * x.chunks * 1024);
+    w.xs = take((size_t)tiles * x.quads * 256);
     w.hq = take((size_t)tiles * h.chunks * 1024);
     w.hs = take((size_t)tiles * h.quads * 256);
   } else {
+    if (!few_pairs(pairs, ex->hidden, ex->inter)) {
+      w.xq = take((size_t)m * (ex->hidden / 2));
+      w.xs = take((size_t)m * mx_scale_row(ex->hidden));
+    }
     w.hq = take((size_t)pairs * (ex->inter / 2));
     w.hs = take((size_t)pairs * mx_scale_row(ex->inter));
   }
@@ -743,13 +754,12 @@ static int moe_pass(const hb_mxfp4_experts* experts, const void* x, const int32_
     if (on_ring(pairs, experts)) {
       const int64_t slots = moe_max_slots(pairs, experts->experts, 0, MX_RING_ROWS);
       if (int e = moe_launch_plan(ids, pairs, experts->base, experts->experts, 0, ws.plan, s, MX_RING_ROWS)) return e;
-      const MxRound job{static_cast<const __bf16*>(x), (int64_t)m * (experts->hidden / 8), experts->hidden, ws.xq, ws.xs};
-      HB_LAUNCH(mx_quantize_rows_kernel, dim3((unsigned)((job.lanes + 255) / 256)), dim3(256), 0, s, job);
-      p1.aq = ws.aq;
-      p1.as = ws.as;
+      p1.x = x;
+      p1.aq = ws.xq;
+      p1.as = ws.xs;
       p1.plan = p2.plan = ws.plan.plan;
       p1.order = p2.order = ws.plan.order;
-      HB_LAUNCH(mx_gather_kernel, dim3((unsigned)l1.quads, (unsigned)slots), dim3(64 * MxMoeRing::TA), 0, s, p1, l1, l2, (const uint8_t*)ws.xq, (const uint8_t*)ws.xs);
+      HB_LAUNCH(mx_gather_kernel, dim3((unsigned)(l1.quads * MxMoeRing::TA), (unsigned)slots), dim3(256), 0, s, p1, l1, l2);
       auto launch = [&](auto kernel, const MxLayout& at, const MxMoe& p) {
         const int columns = (at.tiles + MxMoeRing::TB - 1) / MxMoeRing::TB;
         HB_LAUNCH(kernel, dim3((unsigned)ring_groups(slots, p.n)), dim3(64 * MxMoeRing::WAVES), 0, s, p, (int)slots, columns);
