@@ -601,10 +601,10 @@ struct MxWorkspace {
   size_t bytes;
 };
 
-// Rows a pass of a call takes (more go in several, one behind the other): what keeps the slots of 64 rows and the experts' last ones within a grid,
-// and the activations within a buffer descriptor's reach.
+// Rows a pass of a call takes (more go in several, one behind the other): 2^18 pairs, which fill the device many times over and keep the workspace to a few
+// GB, and what keeps the activations within a buffer descriptor's reach.
 int most_rows(const hb_mxfp4_experts* ex, int topk) {
-  const int64_t pairs = std::min<int64_t>((int64_t)1 << 21, (((int64_t)1 << 32) - 1) / (ex->inter / 2)), rows = (((int64_t)1 << 32) - 1) / (ex->hidden / 2);
+  const int64_t pairs = std::min<int64_t>((int64_t)1 << 18, (((int64_t)1 << 32) - 1) / (ex->inter / 2)), rows = (((int64_t)1 << 32) - 1) / (ex->hidden / 2);
   return (int)std::max<int64_t>(1, std::min(pairs / topk, rows));
 }
 
@@ -651,7 +651,7 @@ MxWorkspace carve(const hb_mxfp4_experts* ex, void* base, int64_t m, int topk, b
     w.hq = take((size_t)pairs * (ex->inter / 2));
     w.hs = take((size_t)pairs * mx_scale_row(ex->inter));
   }
-  w.y = sum ? take((size_t)pairs * ex->hidden_out * sizeof(float)) : nullptr;
+  w.y = sum ? take((size_t)pairs * ex->hidden_out * (m >= MOE_WIDE_ROWS ? sizeof(uint16_t) : sizeof(float))) : nullptr;  // (a last, small pass of a long call uses half of it)
   w.bytes = off;
   return w;
 }

@@ -4,7 +4,7 @@
     out = sum_k w_k down h_k                                                                              (FP32, rounded once)
 
 fc1 [E, 2 I, H] with rows [up; gate] (gated) or [E, I, H] (ReLU^2), fc2 [E, H_out, I]; H and I multiples of 32. Deterministic,
-graph-capturable, any number of rows (past about two million pairs in passes). No counterpart in the reference.
+graph-capturable, any number of rows (past 2^18 pairs in passes). No counterpart in the reference.
 """
 from __future__ import annotations
 

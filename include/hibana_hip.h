@@ -600,7 +600,7 @@ int hb_mxfp4_linear(const void* x, const void* x_scales, int x_type, int64_t m, 
  * hidden_out of eight, up to 960 experts and a topk of 4096. x [m, hidden] BF16 is rounded to the format, h between the two products as well (from its FP32 value). An id
  * outside base .. base + experts - 1 adds nothing. mode HB_MOE_SUM: out BF16 [m, hidden_out]; HB_MOE_PAIRS_F32 / _BF16: the
  * pairs' outputs [m * topk, hidden_out] (those of skipped pairs unspecified). `workspace`: plain scratch, nothing in it need be zero; that of
- * about two million pairs at most (more go in passes, one behind the other). */
+ * 2^18 pairs at most (more go in passes, one behind the other). */
 typedef struct {
   const void* fc1;
   const void* fc2;
