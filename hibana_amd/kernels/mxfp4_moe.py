@@ -109,6 +109,8 @@ def mxfp4_moe(experts: Mxfp4Experts, x: torch.Tensor, ids: torch.Tensor, weights
     """Routed experts for x [M, H] BF16 with the router's ids [M, k] and weights [M, k] -> BF16 [M, H_out], the weighted sum in
     selection order. An id outside this object's range base .. base + E - 1 adds nothing. With `pairs`, the FP32 (`pairs_bf16`:
     BF16) output of each (row, k) pair [M * k, H_out], unsummed and unweighted; rows of skipped pairs are unspecified."""
+    if not isinstance(experts, Mxfp4Experts):
+        raise ValueError("mxfp4_moe: on Mxfp4Experts")
     if x.dtype != torch.bfloat16 or x.ndim != 2 or x.shape[1] != experts.shape1[2]:
         raise ValueError("mxfp4_moe: x must be BF16 [M, hidden]")
     if ids.ndim != 2 or ids.shape[0] != x.shape[0] or weights.shape != ids.shape:

@@ -6,6 +6,7 @@ import torch
 
 from hibana_amd import _lib
 from hibana_amd.kernels import mxfp4, w3
+from hibana_amd.weights.mxfp4 import Mxfp4Linear
 
 
 def w3_decode(lin, m: int, rows: int | None = None) -> bool:
@@ -48,6 +49,8 @@ def mxfp4_linear(x, lin, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     kind = mxfp4.CODES if ready else mxfp4.TYPES.get(x.dtype)
     out_type = dtype if ready else x.dtype
     to = mxfp4.TYPES.get(out_type)
+    if type(lin) is not Mxfp4Linear and not isinstance(lin, Mxfp4Linear):  # (the layout of another format is not told from this one's)
+        raise ValueError("mxfp4_linear: on an Mxfp4Linear")
     if kind is None or to is None or len(x.shape) != 2 or x.shape[1] != lin.in_features:
         raise ValueError("mxfp4_linear: x must be BF16, FP16 or FP32 [M, in_features], or hold such rows")
     if lin.tiled is None:

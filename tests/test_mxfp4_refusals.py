@@ -104,6 +104,18 @@ def test_routed_experts_refusals():
         mxfp4_moe.mxfp4_moe(held, x, ids, w)  # no CPU path
 
 
+def test_weights_of_another_format_are_refused():
+    from types import SimpleNamespace
+
+    from hibana_amd.kernels import mxfp4_moe
+    x = torch.zeros(2, 64, dtype=torch.bfloat16)
+    other = SimpleNamespace(in_features=64, out_features=32, tiled=torch.zeros(1, dtype=torch.uint8), w3=None, pairs=0)
+    with pytest.raises(ValueError):
+        ops.mxfp4_linear(x, other)
+    with pytest.raises(ValueError):
+        mxfp4_moe.mxfp4_moe(SimpleNamespace(shape1=(1, 64, 64), shape2=(1, 64, 64)), x, torch.zeros(2, 1, dtype=torch.int32), torch.zeros(2, 1))
+
+
 def test_layouts_that_do_not_fit_their_shapes():
     """Weights handed over in the kernels' layout alone: of the size that the shape has, or refused."""
     from hibana_amd.kernels import mxfp4_moe
