@@ -139,6 +139,8 @@ def tile(q: Mxfp4, gated: bool = False) -> torch.Tensor:
     if q.codes.ndim not in (2, 3) or not q.codes.numel():
         raise ValueError("mxfp4.tile: a matrix [N, K] or stacked matrices [E, N, K]")
     _lib.need_one_gpu(q.codes, q.scales)
+    if torch.cuda.is_current_stream_capturing():  # it would lie in the graph's memory, and hold nothing before a replay
+        raise RuntimeError("mxfp4.tile: weights are laid out ahead of a capture")
     n, k = q.shape[-2:]
     size = _lib.lib().hb_mxfp4_tiled_bytes(n, k)
     if size == 0:

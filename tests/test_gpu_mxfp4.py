@@ -162,7 +162,8 @@ def _check_product(got, x64, w64, dtype):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("m, n, k", [(1, 1, 32), (1, 5120, 5120), (2, 17, 96), (5, 33, 128), (8, 640, 2688), (15, 1000, 544), (16, 64, 4096), (17, 80, 160),
                                      (31, 257, 1056), (64, 512, 512), (77, 1024, 2080), (128, 129, 640), (200, 96, 1024), (300, 777, 288), (20, 24600, 2560),
-                                     (2048, 5120, 96), (16, 64, 8192), (130, 130, 4128), (40, 33, 5152), (3, 16416, 96), (7, 16411, 2080), (2048, 8500, 96), (1025, 16500, 64)])
+                                     (2048, 5120, 96), (16, 64, 8192), (130, 130, 4128), (40, 33, 5152), (3, 16416, 96), (7, 16411, 2080), (2048, 8500, 96), (1025, 16500, 64),
+                                     (32, 77, 16384), (30, 24610, 3008), (64, 3000, 4160), (90, 2001, 4128), (128, 2050, 4160), (1100, 9001, 544)])
 def test_linear(m, n, k, dtype):
     from hibana_amd.kernels import mxfp4, ops
     from hibana_amd.weights.mxfp4 import Mxfp4Linear

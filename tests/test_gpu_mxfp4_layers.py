@@ -159,6 +159,21 @@ def test_gated_layer_refusals():
             MoeLayer(**{**dict(router=router, shared_gate=gate, experts=make(), topk=2), **bad})
 
 
+def test_weights_are_laid_out_ahead_of_a_capture():
+    from hibana_amd.kernels import mxfp4_moe, ops
+    from hibana_amd.weights.mxfp4 import Mxfp4Linear
+    lin = Mxfp4Linear(*(t.cuda() for t in _weights(64, 96, 1)))
+    experts = mxfp4_moe.Mxfp4Experts(*(t.cuda() for t in (*_weights(64, 96, 1, (3,)), *_weights(96, 32, 2, (3,)))))
+    x, ids, w = torch.zeros(2, 96, dtype=torch.bfloat16).cuda(), torch.zeros(2, 1, dtype=torch.int32).cuda(), torch.ones(2, 1).cuda()
+    for call in (lambda: ops.mxfp4_linear(x, lin), lambda: mxfp4_moe.mxfp4_moe(experts, x, ids, w)):
+        graph = torch.cuda.CUDAGraph()
+        with pytest.raises(RuntimeError, match="capture"):
+            with torch.cuda.graph(graph):
+                call()
+    assert lin.tiled is None and experts.tiled1 is None
+    assert not ops.mxfp4_linear(x, lin).any() and not mxfp4_moe.mxfp4_moe(experts, x, ids, w).any()  # and the calls go on
+
+
 def test_latent_block_on_relu2_experts():
     """`NemotronMoe` with ReLU^2 experts of the format: its routed part is the operator's on the block's own routing."""
     from hibana_amd.kernels import mxfp4_moe
