@@ -719,8 +719,12 @@ static unsigned plan_groups(const QuantJob* job) {
   return 1u + (job->split_rows ? (unsigned)job->split_rows : (unsigned)((job->lanes + PLAN_THREADS - 1) / PLAN_THREADS));
 }
 
+int moe_plan_counts(int64_t pairs) {
+  return pairs >= PLAN_WIDE_PAIRS && pairs <= PLACE_TABLE_SHARE * PLAN_WIDE_GROUPS ? (int)((pairs + PLACE_TABLE_SHARE - 1) / PLACE_TABLE_SHARE) : 0;
+}
+
 int moe_launch_plan(const int32_t* ids, int64_t pairs, int e_lo, int e_n, int shared_rows, const MoeWorkspace& ws, hipStream_t stream, int slot_rows,
-                    const QuantJob* job, int distinct) {
+                    const QuantJob* job, int distinct, bool counted) {
   const size_t plan_lds = ((size_t)(PLAN_WAVES + 1) * e_n + 3 * (PLAN_WAVES + 1)) * sizeof(int);
   if (plan_lds > 64 * 1024 || e_n > PLAN_THREADS || pairs > 0x3fffffff) return HB_EINVAL;
   const int slot_cap = (int)moe_max_slots(pairs, distinct ? distinct : e_n, shared_rows, slot_rows);
@@ -733,9 +737,10 @@ int moe_launch_plan(const int32_t* ids, int64_t pairs, int e_lo, int e_n, int sh
     if (pairs < PLAN_WIDE_PAIRS) {
       place(moe_place_kernel<false>, PLACE_SHARE, PLACE_SHARE / 64 + 2);
     } else {
-      const int groups = (int)((pairs + PLACE_TABLE_SHARE - 1) / PLACE_TABLE_SHARE);  // the counting workgroups' shares are the placing ones'
-      HB_LAUNCH(moe_plan_kernel<true>, dim3(groups), dim3(PLAN_THREADS), plan_lds, stream, ids, (int)pairs, e_lo, e_n, shared_rows, ws.plan, ws.order,
-                RouteParams{}, 0, 0, slot_rows, slot_cap, ws.plan_wide, groups, 1, QuantJob{});
+      const int groups = moe_plan_counts(pairs);  // the counting workgroups' shares are the placing ones'
+      if (!counted)
+        HB_LAUNCH(moe_plan_kernel<true>, dim3(groups), dim3(PLAN_THREADS), plan_lds, stream, ids, (int)pairs, e_lo, e_n, shared_rows, ws.plan, ws.order,
+                  RouteParams{}, 0, 0, slot_rows, slot_cap, ws.plan_wide, groups, 1, QuantJob{});
       place(moe_place_kernel<true>, PLACE_TABLE_SHARE, PLACE_TABLE_SHARE / 64);
     }
     return HB_OK;

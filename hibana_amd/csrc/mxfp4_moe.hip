@@ -260,6 +260,16 @@ __global__ __launch_bounds__(PLAN_THREADS) void mx_plan_round_kernel(const int32
     mx_round_lane(job, (int64_t)(blockIdx.x - 1) * PLAN_THREADS + threadIdx.x);
   }
 }
+// Of a call whose plan counts the experts' pairs in a launch ahead of placing them: the first `groups` workgroups those counts, the others the rounding.
+__global__ __launch_bounds__(PLAN_THREADS) void mx_count_round_kernel(const int32_t* ids, int pairs, int e_lo, int e_n, int32_t* __restrict__ plan, int32_t* __restrict__ order,
+                                                                      int slot_rows, int slot_cap, int32_t* __restrict__ wide, int groups, MxRound job) {
+  extern __shared__ int plan_lds[];
+  if ((int)blockIdx.x < groups) {
+    plan_work<true>(ids, pairs, e_lo, e_n, 0, plan, order, slot_rows, slot_cap, wide, groups, 1, blockIdx.x, plan_lds);
+  } else {
+    mx_round_lane(job, (int64_t)(blockIdx.x - groups) * PLAN_THREADS + threadIdx.x);
+  }
+}
 
 template <int MT>
 struct MxWalk {
@@ -782,8 +792,13 @@ static int moe_pass(const hb_mxfp4_experts* experts, const void* x, const int32_
       HB_LAUNCH(mx_plan_round_kernel, dim3(1 + (unsigned)((job.lanes + PLAN_THREADS - 1) / PLAN_THREADS)), dim3(PLAN_THREADS), plan_lds, s, ids, (int)pairs, experts->base,
                 experts->experts, ws.plan.plan, ws.plan.order, slot_rows, (int)slots, job);
     } else {
-      if (int e = moe_launch_plan(ids, pairs, experts->base, experts->experts, 0, ws.plan, s, slot_rows)) return e;
-      HB_LAUNCH(mx_quantize_rows_kernel, dim3((unsigned)((job.lanes + 255) / 256)), dim3(256), 0, s, job);
+      const int counts = moe_plan_counts(pairs);
+      const unsigned rounds = (unsigned)((job.lanes + PLAN_THREADS - 1) / PLAN_THREADS);
+      if (counts)
+        HB_LAUNCH(mx_count_round_kernel, dim3(counts + rounds), dim3(PLAN_THREADS), plan_lds, s, ids, (int)pairs, experts->base, experts->experts, ws.plan.plan, ws.plan.order,
+                  slot_rows, (int)slots, ws.plan.plan_wide, counts, job);
+      if (int e = moe_launch_plan(ids, pairs, experts->base, experts->experts, 0, ws.plan, s, slot_rows, nullptr, 0, counts > 0)) return e;
+      if (!counts) HB_LAUNCH(mx_quantize_rows_kernel, dim3((unsigned)((job.lanes + 255) / 256)), dim3(256), 0, s, job);
     }
     p1.plan = p2.plan = ws.plan.plan;
     p1.order = p2.order = ws.plan.order;

@@ -632,8 +632,11 @@ MoeWorkspace moe_carve(void* base, int m, int topk, int experts, int inter, int 
 // Enqueue the plan kernel; HB_EINVAL if the expert count does not fit its LDS.
 // A rounding job rides in the plan's launch (further workgroups beside the one that plans). `distinct`: the most experts of
 // the range that the ids can name (0: all).
+// Workgroups of the count of the experts' pairs that a plan of so many begins with (0: it has no such launch of its own). A caller that has made them in a launch
+// of its own (plan_work<true>, phase 1 of as many groups) says `counted` to moe_launch_plan.
+int moe_plan_counts(int64_t pairs);
 int moe_launch_plan(const int32_t* ids, int64_t pairs, int e_lo, int e_n, int shared_rows, const MoeWorkspace& ws, hipStream_t stream,
-                    int slot_rows = ROWS_PER_SLOT, const QuantJob* job = nullptr, int distinct = 0);
+                    int slot_rows = ROWS_PER_SLOT, const QuantJob* job = nullptr, int distinct = 0, bool counted = false);
 void moe_launch_quant_groups(const QuantJob& job, hipStream_t stream);  // the rounding alone
 void moe_launch_quant_rows(const uint16_t* x, int64_t m, int k, uint8_t* q, float* scales, hipStream_t stream);  // one scale a row
 
