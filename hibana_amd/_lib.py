@@ -192,6 +192,17 @@ def need_one_gpu(*tensors: torch.Tensor) -> None:
             raise ValueError(f"hibana_amd kernels run on the current device, cuda:{here}: got a tensor on {t.device}")
 
 
+def stream_of(x: torch.Tensor, *more: torch.Tensor) -> int:
+    """The current stream, for a launch that takes these tensors: `need_one_gpu` of them all (0.25 us against 0.5 for the two)."""
+    at = x.get_device()
+    if at < 0 or at != torch._C._cuda_getDevice():
+        need_one_gpu(x, *more)
+    for t in more:
+        if t.get_device() != at:
+            need_one_gpu(x, *more)
+    return torch._C._cuda_getCurrentRawStream(at)
+
+
 def need_gpu(*tensors: torch.Tensor) -> None:
     for t in tensors:
         if t is not None and not t.is_cuda:

@@ -80,16 +80,17 @@ def flat(q: Mxfp4, what: str) -> tuple[torch.Tensor, torch.Tensor]:
 
 
 def places(q: Mxfp4, what: str):
-    """(address of the codes, address of the scales, what to hold until the launch that reads them is enqueued), on the current device."""
+    """(address of the codes, address of the scales, what to hold until the launch that reads them is enqueued, the current stream), on the
+    current device."""
     block = q._block
     if block is not None:
-        _lib.need_one_gpu(block)
+        stream = _lib.stream_of(block)
         at = block.data_ptr()
-        return at, at + block.numel() * 16 // 17, block
+        return at, at + block.numel() * 16 // 17, block, stream
     check(q, what)
-    _lib.need_one_gpu(q.codes, q.scales)
+    stream = _lib.stream_of(q.codes, q.scales)
     held = flat(q, what)
-    return held[0].data_ptr(), held[1].data_ptr(), held
+    return held[0].data_ptr(), held[1].data_ptr(), held, stream
 
 
 def rows16(x: torch.Tensor) -> torch.Tensor:
@@ -104,13 +105,13 @@ def quantize(x: torch.Tensor) -> Mxfp4:
     shape = tuple(x.shape)
     if kind is None or not shape or shape[-1] % GROUP:
         raise ValueError(f"mxfp4.quantize: BF16, FP16 or FP32 [..., K], K a multiple of {GROUP}")
-    _lib.need_one_gpu(x)
+    stream = _lib.stream_of(x)
     n = x.numel()
     block = x.new_empty(n // GROUP * 17, dtype=torch.uint8)
     if n:
         xc = rows16(x)  # held until the launch is enqueued
         at = block.data_ptr()
-        code = _lib.lib().hb_mxfp4_quantize(xc.data_ptr(), kind, n // shape[-1], shape[-1], at, at + n // 2, _lib.stream())
+        code = _lib.lib().hb_mxfp4_quantize(xc.data_ptr(), kind, n // shape[-1], shape[-1], at, at + n // 2, stream)
         if code:
             _lib.check(code, "mxfp4.quantize")
     return Mxfp4.of_block(block, shape)
@@ -121,12 +122,12 @@ def dequantize(q: Mxfp4, dtype: torch.dtype = torch.float32) -> torch.Tensor:
     kind = TYPES.get(dtype)
     if kind is None:
         raise ValueError("mxfp4.dequantize: to BF16, FP16 or FP32")
-    codes, scales, held = places(q, "mxfp4.dequantize")
-    out = torch.empty(q.shape, dtype=dtype, device=q.device)
+    codes, scales, held, stream = places(q, "mxfp4.dequantize")
+    out = (q._codes if q._block is None else q._block).new_empty(q.shape, dtype=dtype)
     n = out.numel()
     if n:
         k = q.shape[-1]
-        code = _lib.lib().hb_mxfp4_dequantize(codes, scales, n // k, k, kind, out.data_ptr(), _lib.stream())
+        code = _lib.lib().hb_mxfp4_dequantize(codes, scales, n // k, k, kind, out.data_ptr(), stream)
         if code:
             _lib.check(code, "mxfp4.dequantize")
     return out

@@ -116,7 +116,7 @@ def mxfp4_moe(experts: Mxfp4Experts, x: torch.Tensor, ids: torch.Tensor, weights
     if ids.ndim != 2 or ids.shape[0] != x.shape[0] or weights.shape != ids.shape:
         raise ValueError("mxfp4_moe: ids and weights must be [M, k]")
     st = _struct(experts)
-    _lib.need_one_gpu(x, ids, weights, experts.tiled1, experts.tiled2)
+    stream = _lib.stream_of(x, ids, weights, experts.tiled1, experts.tiled2)
     m, k = ids.shape
     mode = (2 if pairs_bf16 else 1) if pairs else 0
     out = x.new_empty((m * k if pairs else m, experts.shape2[1]), dtype=torch.float32 if mode == 1 else torch.bfloat16)
@@ -133,7 +133,7 @@ def mxfp4_moe(experts: Mxfp4Experts, x: torch.Tensor, ids: torch.Tensor, weights
     ids32 = ids if ids.dtype == torch.int32 and ids.is_contiguous() else ids.to(torch.int32).contiguous()
     wt = weights if weights.dtype == torch.float32 and weights.is_contiguous() else weights.float().contiguous()
     xc = mxfp4.rows16(x)
-    code = lib.hb_mxfp4_moe(st.at, xc.data_ptr(), ids32.data_ptr(), wt.data_ptr(), m, k, mode, out.data_ptr(), ws.data_ptr(), need, _lib.stream())
+    code = lib.hb_mxfp4_moe(st.at, xc.data_ptr(), ids32.data_ptr(), wt.data_ptr(), m, k, mode, out.data_ptr(), ws.data_ptr(), need, stream)
     if code:
         _lib.check(code, "mxfp4_moe")
     return out

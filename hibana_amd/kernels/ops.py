@@ -56,19 +56,23 @@ def mxfp4_linear(x, lin, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     if lin.tiled is None:
         lin.tile()
     if ready:
-        at, scales, held = mxfp4.places(x, "mxfp4_linear")
+        at, scales, held, stream = mxfp4.places(x, "mxfp4_linear")
         _lib.need_one_gpu(lin.tiled)
     else:
-        _lib.need_one_gpu(x, lin.tiled)
+        stream = _lib.stream_of(x, lin.tiled)
         held = mxfp4.rows16(x)  # held until the launch is enqueued
         at, scales = held.data_ptr(), None
     m, n, k = x.shape[0], lin.out_features, lin.in_features
     y = lin.tiled.new_empty((m, n), dtype=out_type)
     if m:
         lib = _lib.lib()
-        need = lib.hb_mxfp4_linear_workspace_bytes(m, n, k, kind)
+        need = lin.rooms.get((m, kind))
+        if need is None:
+            if len(lin.rooms) >= 4096:
+                lin.rooms.clear()
+            need = lin.rooms[m, kind] = lib.hb_mxfp4_linear_workspace_bytes(m, n, k, kind)
         ws = lin.tiled.new_empty(need) if need else None  # (of the capture's own pool in a captured call)
-        code = lib.hb_mxfp4_linear(at, scales, kind, m, lin.tiled.data_ptr(), n, k, y.data_ptr(), to, _lib.ptr(ws), need, _lib.stream())
+        code = lib.hb_mxfp4_linear(at, scales, kind, m, lin.tiled.data_ptr(), n, k, y.data_ptr(), to, _lib.ptr(ws), need, stream)
         if code:
             _lib.check(code, "mxfp4_linear")
     return y
@@ -138,13 +142,13 @@ def silu_mul_quant_mxfp4(gate_up: torch.Tensor, pairs: int = 0) -> mxfp4.Mxfp4:
     half = gate_up.shape[-1] // 2
     if pairs and (pairs < 0 or pairs % 8 or half % pairs):
         raise ValueError("silu_mul_quant_mxfp4: pairs must be a multiple of eight dividing I")
-    _lib.need_one_gpu(gate_up)
+    stream = _lib.stream_of(gate_up)
     n = gate_up.numel() // 2
     block = gate_up.new_empty(n // mxfp4.GROUP * 17, dtype=torch.uint8)
     if n:
         gu = mxfp4.rows16(gate_up)  # held until the launch is enqueued
         at = block.data_ptr()
-        code = _lib.lib().hb_silu_mul_quant_mxfp4(gu.data_ptr(), kind, n // half, half, pairs, at, at + n // 2, _lib.stream())
+        code = _lib.lib().hb_silu_mul_quant_mxfp4(gu.data_ptr(), kind, n // half, half, pairs, at, at + n // 2, stream)
         if code:
             _lib.check(code, "silu_mul_quant_mxfp4")
     return mxfp4.Mxfp4.of_block(block, (*gate_up.shape[:-1], half))

@@ -5,7 +5,7 @@ has no three-bit copy.
 """
 from __future__ import annotations
 
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 
 import torch
 
@@ -21,6 +21,7 @@ class Mxfp4Linear:
     out_features: int = 0
     in_features: int = 0
     w3: object = None
+    rooms: dict = field(default_factory=dict, init=False, repr=False, compare=False)  # the workspace a call of (rows, type) takes
 
     def __post_init__(self):
         if self.codes is not None:
