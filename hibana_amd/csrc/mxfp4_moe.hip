@@ -217,17 +217,13 @@ __global__ __launch_bounds__(64 * MX_ROW_WAVES, 2) void mx_fc2_row_kernel(MxMoe 
 // ------------------------------------------------------------------------------------------------ many pairs
 constexpr int MX_PLAN_PAIRS = 1024;  // from here the plan's launches share the pairs
 // Workgroups of a product, about six a compute unit where there are so many: each has several units then, whose weights it asks for ahead. us, 1543 rows of 10
-// of 512 experts (2048, 512), repeated on 2.5 GB of weights: 384 278, 768 251, 1536 240, 3072 250.
+// of 512 experts (2048, 512), repeated on 2.5 GB of weights: 384 278, 768 251, 1536 240, twice that 250.
 constexpr int MX_MANY_GROUPS = 1536;
 // From this many pairs an expert slots have 64 rows, whose products share a weight tile's registers: 240 us against 292 for the call above (30 pairs an
 // expert), 71 and 74 for 300 rows of 8 of 64 (2048, 768); verify-sized calls are the same either way and keep the registers.
 constexpr int MX_TALL_PAIRS = 24;
-// A wavefront's walk over steps of eight chunks of two weight tiles, for a slot of the plan (up to 32 MT rows of an expert). A step's weights, 16 KB
-// a wavefront, are asked for as soon as the step before has taken its own out of the registers, so they are on their way while sums
-// are joined, rounded and stored; a slot's activations (32 bytes of a row's chunk, read where they lie) stay in registers where one
-// step covers the wavefront's K. Bound by reading the weights: 1543 rows of 10 of 512 experts (2048, 512) fc1 114 us, 5.0 TB/s, fc2 73 us, 4.7 with its
-// results; 32 rows 24 and 13 us, 5.1 and 4.7; four rows of 22 of 512 ReLU^2 experts (1024, 2688) 23 and 23 us, 5.2.
-// x [rows, k] rounded for the products of many pairs, eight values a lane: codes by rows, scales as above (a last odd group's partner at 0).
+// x [rows, k] rounded for the products of many pairs, eight values a lane: codes by rows, scales as above (a last odd group's partner at 0). 1543 x 2048 4.8 us in a
+// launch of its own.
 struct MxRound {
   const __bf16* x;
   int64_t lanes;
@@ -271,6 +267,11 @@ __global__ __launch_bounds__(PLAN_THREADS) void mx_count_round_kernel(const int3
   }
 }
 
+// A wavefront's walk over steps of eight chunks of two weight tiles, for a slot of the plan (up to 32 MT rows of an expert). A step's weights, 16 KB
+// a wavefront, are asked for as soon as the step before has taken its own out of the registers, so they are on their way while sums
+// are joined, rounded and stored; a slot's activations (32 bytes of a row's chunk, read where they lie) stay in registers where one
+// step covers the wavefront's K. Bound by reading the weights: 1543 rows of 10 of 512 experts (2048, 512) fc1 114 us, 5.0 TB/s, fc2 73 us, 4.7 with its
+// results; 32 rows 24 and 13 us, 5.1 and 4.7; four rows of 22 of 512 ReLU^2 experts (1024, 2688) 23 and 23 us, 5.2.
 template <int MT>
 struct MxWalk {
   static constexpr int NT = MX_MOE_TILES;

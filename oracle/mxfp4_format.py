@@ -1,5 +1,5 @@
 """The microscaled four-bit format in FP64 (CPU, torch): the rounding by the borders between neighbouring values, the values back,
-the products and the routed experts on them, straight from their definitions. The checker of the MXFP4 kernels, never the product."""
+the products and the routed experts on them, straight from their definitions. What the tests compare the kernels with, never the product."""
 from __future__ import annotations
 
 import torch
