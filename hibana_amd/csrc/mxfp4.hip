@@ -11,7 +11,7 @@ namespace hb {
 // ------------------------------------------------------------------------------------------------ rounding, and back
 // x [rows, k] -> codes [rows, k / 2], scales [rows, k / 32]. A lane takes eight consecutive values, four lanes a group: loads and
 // stores of a wavefront are consecutive, and the group's largest magnitude is two lane exchanges. Memory bound: 1543 x 5120 of FP32 6.9 us, 5.2 TB/s
-// read and written; one row is 1.5 us, and the call its host work (6.5).
+// read and written; one row is 1.5 us, and the call its host work (6.2).
 template <typename T>
 __global__ __launch_bounds__(256) void mx_quantize_kernel(const T* __restrict__ x, int64_t lanes, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
