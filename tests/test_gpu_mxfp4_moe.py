@@ -81,6 +81,28 @@ def test_ids_outside_the_range_rows_of_none_and_repeats(m):
     assert nothing.shape == (m, 256) and not nothing.any()
 
 
+@pytest.mark.parametrize("m", [1, 9, 40, 300, 1200])
+def test_nothing_of_a_pair_outside_the_range_is_read(m):
+    """Its weight and its place among the pairs' outputs may hold anything, a NaN too; memory the call is given as scratch as well."""
+    from hibana_amd.kernels import mxfp4_moe
+    ex, fc1, fc2 = _experts(5, 128, 96, m != 40, 21, base=2)
+    x, ids, w = _call(m, 10, 4, 128, m)
+    inside = (ids >= 2) & (ids < 7)
+    clean = torch.where(inside, w, torch.zeros_like(w))
+    args = x.cuda(), ids.cuda(), torch.where(inside, w, torch.full_like(w, float("nan"))).cuda()
+    mxfp4_moe.tile(ex)
+    poison = torch.full((1 << 24,), float("nan"), device="cuda")
+    del poison  # what is allocated next lies in it
+    got = mxfp4_moe.mxfp4_moe(ex, *args)
+    assert bool(torch.isfinite(got).all())
+    assert torch.equal(got, mxfp4_moe.mxfp4_moe(ex, args[0], args[1], clean.cuda()))
+    want, off = om.moe(x, ids, clean, fc1, fc2, base=2)
+    if m >= PAIR_ROUNDING_ROWS:
+        y, far = om.moe_pairs(x, ids, fc1, fc2, base=2)
+        off = off + 2.0 ** -8 * ((y.abs() + far) * clean.double()[..., None]).sum(1)
+    _check(got, want, off)
+
+
 def test_every_row_on_one_expert_and_a_row_that_is_not_finite():
     from hibana_amd.kernels import mxfp4_moe
     ex, fc1, fc2 = _experts(5, 128, 64, True, 8)
