@@ -195,7 +195,7 @@ struct MxLinear {
 
 // Few rows: a workgroup NT tiles of weight rows, its wavefronts the chunks of K. The first weights are asked for, then the workgroup puts
 // the activations into LDS, rounded on the way: each workgroup all of them, which costs less than a launch. (32 x 32 x 64 products of which up to 31 columns are
-// idle: the matrix cores have nothing else to do.) One row of 5120 x 5120 5.4 us: latency of the launch, the activations, five chunks of weights
+// idle: the matrix cores have nothing else to do.) One row of 5120 x 5120 5.4 us: latency of the launch, the activations, ten chunks of weights a wavefront
 // and the join. Eight rows of 25600 x 5120 14.2 us: the weights at 4.9 TB/s.
 template <typename T, typename Y, int NT, int RUN>
 __global__ __launch_bounds__(512) void mx_few_rows_kernel(MxLinear p) {
