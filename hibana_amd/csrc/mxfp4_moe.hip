@@ -217,9 +217,9 @@ __global__ __launch_bounds__(64 * MX_ROW_WAVES, 2) void mx_fc2_row_kernel(MxMoe 
 // ------------------------------------------------------------------------------------------------ many pairs
 constexpr int MX_PLAN_PAIRS = 1024;  // from here the plan's launches share the pairs
 // Workgroups of a product, about six a compute unit where there are so many: each has several units then, whose weights it asks for ahead. us, 1543 rows of 10
-// of 512 experts (2048, 512), repeated on 2.5 GB of weights: 384 278, 768 251, 1536 240, twice that 250.
+// of 512 experts (2048, 512), repeated on 2.5 GB of weights, pairs in BF16: 384 278, 768 251, 1536 240, twice that 250.
 constexpr int MX_MANY_GROUPS = 1536;
-// From this many pairs an expert slots have 64 rows, whose products share a weight tile's registers: 240 us against 292 for the call above (30 pairs an
+// From this many pairs an expert slots have 64 rows, whose products share a weight tile's registers: 240 us against 292 for the call above, pairs in BF16 too (30 an
 // expert), 71 and 74 for 300 rows of 8 of 64 (2048, 768); verify-sized calls are the same either way and keep the registers.
 constexpr int MX_TALL_PAIRS = 24;
 // x [rows, k] rounded for the products of many pairs, eight values a lane: codes by rows, scales as above (a last odd group's partner at 0). 1543 x 2048 4.8 us in a
@@ -270,7 +270,7 @@ __global__ __launch_bounds__(PLAN_THREADS) void mx_count_round_kernel(const int3
 // A wavefront's walk over steps of eight chunks of two weight tiles, for a slot of the plan (up to 32 MT rows of an expert). A step's weights, 16 KB
 // a wavefront, are asked for as soon as the step before has taken its own out of the registers, so they are on their way while sums
 // are joined, rounded and stored; a slot's activations (32 bytes of a row's chunk, read where they lie) stay in registers where one
-// step covers the wavefront's K. Bound by reading the weights: 1543 rows of 10 of 512 experts (2048, 512) fc1 114 us, 5.0 TB/s, fc2 73 us, 4.7 with its
+// step covers the wavefront's K. Bound by reading the weights: 1543 rows of 10 of 512 experts (2048, 512) fc1 116 us, 4.9 TB/s, fc2 86 us, 4.8 with its
 // results; 32 rows 24 and 13 us, 5.1 and 4.7; four rows of 22 of 512 ReLU^2 experts (1024, 2688) 23 and 23 us, 5.2.
 template <int MT>
 struct MxWalk {
@@ -662,7 +662,7 @@ MxWorkspace carve(const hb_mxfp4_experts* ex, void* base, int64_t m, int topk, b
     w.hq = take((size_t)pairs * (ex->inter / 2));
     w.hs = take((size_t)pairs * mx_scale_row(ex->inter));
   }
-  w.y = sum ? take((size_t)pairs * ex->hidden_out * (m >= MOE_WIDE_ROWS ? sizeof(uint16_t) : sizeof(float))) : nullptr;  // (a last, small pass of a long call uses half of it)
+  w.y = sum ? take((size_t)pairs * ex->hidden_out * sizeof(float)) : nullptr;
   w.bytes = off;
   return w;
 }
@@ -691,9 +691,11 @@ extern "C" size_t hb_mxfp4_moe_workspace_bytes(const hb_mxfp4_experts* experts, 
   return carve(experts, nullptr, m, topk, true).bytes;
 }
 
-// One pass: m <= most_rows. `wide`: the pairs of a sum in BF16.
-static int moe_pass(const hb_mxfp4_experts* experts, const void* x, const int32_t* ids, const float* weights, int m, int topk, int mode, bool wide, void* out,
-                    void* workspace, hipStream_t s) {
+// One pass: m <= most_rows. A sum's pairs lie in FP32 between fc2 and the combine, at any number of rows: in BF16 the largest tensor of a prefill would be half as
+// large, but each pair would be rounded once more than the result is (1543 rows of 10 of 512 experts (2048, 512): relative
+// error 2.4e-3 where FP32 pairs have 1.7e-3, the error of the result's own rounding; 212 us where they take 234, 126 MB more to write and read).
+static int moe_pass(const hb_mxfp4_experts* experts, const void* x, const int32_t* ids, const float* weights, int m, int topk, int mode, void* out, void* workspace,
+                    hipStream_t s) {
   const bool sum = mode == HB_MOE_SUM;
   const MxWorkspace ws = carve(experts, workspace, m, topk, sum);
   const int64_t pairs = (int64_t)m * topk;
@@ -720,12 +722,11 @@ static int moe_pass(const hb_mxfp4_experts* experts, const void* x, const int32_
   p2.aq = ws.hq;
   p2.as = ws.hs;
   p2.y = sum ? ws.y : out;
-  bool narrow = mode == HB_MOE_PAIRS_BF16;
+  const bool narrow = mode == HB_MOE_PAIRS_BF16;
   const unsigned groups1 = (unsigned)((l1.tiles + MX_MOE_TILES - 1) / MX_MOE_TILES), groups2 = (unsigned)((l2.tiles + MX_MOE_TILES - 1) / MX_MOE_TILES);
-  auto combine = [&](bool bf16) {
+  auto combine = [&] {
     CombineParams c{};
     c.pairs = ws.y;
-    c.pairs_bf16 = bf16;
     c.ids = ids;
     c.weights = weights;
     c.e_lo = experts->base;
@@ -760,8 +761,6 @@ static int moe_pass(const hb_mxfp4_experts* experts, const void* x, const int32_
       launch(long2 ? mx_fc2_few_kernel<float, 4> : mx_fc2_few_kernel<float, 2>, grid2, lds2, p2);
     }
   } else {
-    // a summed prefill-sized call keeps its pair outputs in BF16, half the traffic of its widest tensor, as the framework's other routed calls do
-    narrow = narrow || (sum && wide);
     if (on_ring(pairs, experts)) {
       const int64_t slots = moe_max_slots(pairs, experts->experts, 0, MX_RING_ROWS);
       if (int e = moe_launch_plan(ids, pairs, experts->base, experts->experts, 0, ws.plan, s, MX_RING_ROWS)) return e;
@@ -781,7 +780,7 @@ static int moe_pass(const hb_mxfp4_experts* experts, const void* x, const int32_
       } else {
         launch(mx_fc2_ring_kernel<float>, l2, p2);
       }
-      if (sum) combine(narrow);
+      if (sum) combine();
       return launch_status();
     }
     const bool tall = pairs >= (int64_t)MX_TALL_PAIRS * experts->experts;
@@ -844,7 +843,7 @@ static int moe_pass(const hb_mxfp4_experts* experts, const void* x, const int32_
       fc2((float*)nullptr);
     }
   }
-  if (sum) combine(narrow);
+  if (sum) combine();
   return launch_status();
 }
 
@@ -859,7 +858,7 @@ extern "C" int hb_mxfp4_moe(const hb_mxfp4_experts* experts, const void* x, cons
   const int64_t row = (int64_t)experts->hidden_out * (mode == HB_MOE_SUM ? 2 : mode == HB_MOE_PAIRS_F32 ? 4 * topk : 2 * topk);  // bytes
   for (int lo = 0; lo < m; lo += std::min(most, m - lo)) {
     if (int e = moe_pass(experts, static_cast<const uint16_t*>(x) + (int64_t)lo * experts->hidden, ids + (int64_t)lo * topk, weights + (int64_t)lo * topk, std::min(most, m - lo),
-                         topk, mode, m >= MOE_WIDE_ROWS, static_cast<uint8_t*>(out) + lo * row, workspace, as_stream(stream)))
+                         topk, mode, static_cast<uint8_t*>(out) + lo * row, workspace, as_stream(stream)))
       return e;
   }
   return HB_OK;

@@ -106,8 +106,8 @@ def _struct(experts: Mxfp4Experts) -> _lib.HbMxfp4Experts:
 
 
 def mxfp4_moe(experts: Mxfp4Experts, x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, pairs: bool = False, pairs_bf16: bool = False) -> torch.Tensor:
-    """Routed experts for x [M, H] BF16 with the router's ids [M, k] and weights [M, k] -> BF16 [M, H_out], the weighted sum in
-    selection order. An id outside this object's range base .. base + E - 1 adds nothing. With `pairs`, the FP32 (`pairs_bf16`:
+    """Routed experts for x [M, H] BF16 with the router's ids [M, k] and weights [M, k] -> BF16 [M, H_out], the weighted sum of a row's pairs in
+    FP32, added in an order that the sizes alone decide, and rounded once. An id outside this object's range base .. base + E - 1 adds nothing. With `pairs`, the FP32 (`pairs_bf16`:
     BF16) output of each (row, k) pair [M * k, H_out], unsummed and unweighted; rows of skipped pairs are unspecified."""
     if not isinstance(experts, Mxfp4Experts):
         raise ValueError("mxfp4_moe: on Mxfp4Experts")

@@ -164,7 +164,7 @@ class MoeLayer:
             ids, weights = self.route(x, ctx)
             if self.shared_mlp is None:
                 return self.routed(x, ids, weights)
-            pairs = mxfp4_moe.mxfp4_moe(self.mxfp4, x, ids, weights, pairs=True, pairs_bf16=x.shape[0] >= w3_moe.WIDE_ROWS)
+            pairs = mxfp4_moe.mxfp4_moe(self.mxfp4, x, ids, weights, pairs=True)  # FP32 at any number of rows, as the sum without a shared expert has them
             return ops.moe_combine_pairs(pairs, ids, weights, self.shared_mlp(x), x, self.shared_gate_vec, self.mxfp4.base, self.mxfp4.experts)
         if self.shared_on_linears(x.shape[0]):
             # the reference's own chain: the experts' unsummed pair outputs (BF16 from WIDE_ROWS rows), the shared expert

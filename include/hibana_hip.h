@@ -245,7 +245,7 @@ int hb_debug_workspace_layout(int m, int topk, const hb_w3_experts* routed, int 
 
 /* Routed sum: out[r] = bf16( fma-chain over the row's slots, in selection order, of weights[r, s] * y[r, s] ),
  * y = fc2_e( act( bf16(fc1_e x_r) ) ) in FP32, h rounded to BF16. ids int32 [m, topk]; an id outside
- * [base, base + experts) adds nothing. mode HB_MOE_SUM: out BF16 [m, hidden_out]; HB_MOE_PAIRS_F32 / _BF16: out is
+ * [base, base + experts) adds nothing. mode HB_MOE_SUM: out BF16 [m, hidden_out], FP32 sums of FP32 pairs rounded once; HB_MOE_PAIRS_F32 / _BF16: out is
  * the unsummed pair outputs [m * topk, hidden_out] (rows of dropped pairs are left untouched).
  * With HB_MOE_E4M3 or-ed into mode, x and h go through the reference's activation rounding (hb_w3_quant_groups) before
  * their products, as in the reference kernel (y = fc2_e(Q(act(bf16(fc1_e Q(x_r)))))); without it the weight-only form.
@@ -598,7 +598,7 @@ int hb_mxfp4_linear(const void* x, const void* x_scales, int x_type, int64_t m, 
 /* Routed experts, weights and activations both in the format: fc1 and fc2 are stacks of `experts` tile layouts, fc1 [2 inter or inter,
  * hidden] (gated: rows [up; gate], laid out with `gated`; else ReLU^2), fc2 [hidden_out, inter]; hidden and inter multiples of 32,
  * hidden_out of eight, up to 960 experts and a topk of 4096. x [m, hidden] BF16 is rounded to the format, h between the two products as well (from its FP32 value). An id
- * outside base .. base + experts - 1 adds nothing. mode HB_MOE_SUM: out BF16 [m, hidden_out]; HB_MOE_PAIRS_F32 / _BF16: the
+ * outside base .. base + experts - 1 adds nothing. mode HB_MOE_SUM: out BF16 [m, hidden_out], FP32 sums of FP32 pairs rounded once; HB_MOE_PAIRS_F32 / _BF16: the
  * pairs' outputs [m * topk, hidden_out] (those of skipped pairs unspecified). `workspace`: plain scratch, nothing in it need be zero; that of
  * 2^18 pairs at most (more go in passes, one behind the other). */
 typedef struct {
