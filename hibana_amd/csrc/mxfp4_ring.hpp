@@ -127,49 +127,51 @@ struct MxRing {
     // What the step asks of memory (at a quad's first step the next quad's scales, then its tiles three steps on) goes out between the products: in
     // front of them all, it and the barrier would leave the matrix cores idle for a fifth of the step. At its end what may still be on its way is
     // the step's own and the step's before LATE ones: the next step reads its own tiles, asked for two steps ago, and chunk 0 of the one behind it. (All of
-    // that one waited for: 2048 rows of 25600 x 5120 148 us, so 144.5.)
-#define MX_STEP(CUR, NEXT, ASKED, S, ODD)                                                                                                             \
-    mx_unrolled<GROUPS>([&](auto group) {                                                                                                             \
-      constexpr int v = group.value, u = v / NT, j = v % NT, ring = (ODD) * GROUPS + v;                                                               \
-      fb[(ring + AHEAD) & 3] = v + AHEAD < GROUPS ? b_at(CUR, v + AHEAD) : b_at(NEXT, v + AHEAD - GROUPS);                                            \
-      _Pragma("unroll") for (int i = j * MT / NT; i < (j + 1) * MT / NT; i++) fa[1 - u][i] = u == 0 ? a_at(CUR, 1, i) : a_at(NEXT, 0, i);             \
-      mx_unrolled<MT>([&](auto tile) {                                                                                                                \
-        constexpr int i = tile.value, at = v * MT + i;  /* the step's product */                                                                      \
-        if constexpr (IN_PLACE) {                                                                                                                     \
-          mx_mfma_in_place<2 * (ODD) + u>(acc[i][j], fb[ring & 3], fa[u][i], now[MT + j], now[i]);                                                    \
-        } else {                                                                                                                                      \
-          acc[i][j] = mx_mfma<2 * (ODD) + u, 2 * (ODD) + u>(fb[ring & 3], now[MT + j], fa[u][i], now[i], acc[i][j]);                                  \
-        }                                                                                                                                             \
-        constexpr int ALL = GROUPS * MT, FIRST = (ALL + 3) / 4, H = (ODD) ? 0 : FIRST, W = ALL - FIRST;  /* asked for behind products H .. H + W - 1 */\
-        constexpr int before = at < H ? 0 : at - H >= W ? ASKS : (at - H) * ASKS / W;                                                                 \
-        constexpr int after = at < H ? 0 : at + 1 - H >= W ? ASKS : (at + 1 - H) * ASKS / W;                                                          \
-        if constexpr (!(ODD)) {                                                                                                                       \
-          constexpr int from = at >= H ? SCALES : at * SCALES / H, to = at >= H ? SCALES : (at + 1) * SCALES / H;                                     \
-          mx_unrolled<to - from>([&](auto k) { scale(from + k.value, min((S) / 2 + 1, quads - 1)); });                                                \
-        }                                                                                                                                             \
-        mx_unrolled<after - before>([&](auto k) { MX_ASK(ASKED, (S) + 3, before + k.value) });                                                        \
-        __builtin_amdgcn_sched_barrier(0);                                                                                                            \
-      });                                                                                                                                             \
-    });                                                                                                                                               \
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((ODD) ? ASKS + LATE : ASKS + LATE + SCALES) : "memory");                                                 \
-    __builtin_amdgcn_s_barrier();                                                                                                                     \
+    // that one waited for: 2048 rows of 25600 x 5120 148 us, so 144.5.) The wait counts loads, so every load of the step has to be made: the scales of a quad that no
+    // step takes (MORE = 0) are not asked for, where the compiler would drop them and the wait leave LATE tiles of the next step on their way
+    // (tests/test_mxfp4_ring_waits.py counts them in the machine code).
+#define MX_STEP(CUR, NEXT, ASKED, S, ODD, MORE)                                                                                                         \
+    mx_unrolled<GROUPS>([&](auto group) {                                                                                                               \
+      constexpr int v = group.value, u = v / NT, j = v % NT, ring = (ODD) * GROUPS + v;                                                                 \
+      fb[(ring + AHEAD) & 3] = v + AHEAD < GROUPS ? b_at(CUR, v + AHEAD) : b_at(NEXT, v + AHEAD - GROUPS);                                              \
+      _Pragma("unroll") for (int i = j * MT / NT; i < (j + 1) * MT / NT; i++) fa[1 - u][i] = u == 0 ? a_at(CUR, 1, i) : a_at(NEXT, 0, i);               \
+      mx_unrolled<MT>([&](auto tile) {                                                                                                                  \
+        constexpr int i = tile.value, at = v * MT + i;  /* the step's product */                                                                        \
+        if constexpr (IN_PLACE) {                                                                                                                       \
+          mx_mfma_in_place<2 * (ODD) + u>(acc[i][j], fb[ring & 3], fa[u][i], now[MT + j], now[i]);                                                      \
+        } else {                                                                                                                                        \
+          acc[i][j] = mx_mfma<2 * (ODD) + u, 2 * (ODD) + u>(fb[ring & 3], now[MT + j], fa[u][i], now[i], acc[i][j]);                                    \
+        }                                                                                                                                               \
+        constexpr int ALL = GROUPS * MT, FIRST = (ALL + 3) / 4, H = (ODD) ? 0 : FIRST, W = ALL - FIRST;  /* asked for behind products H .. H + W - 1 */ \
+        constexpr int before = at < H ? 0 : at - H >= W ? ASKS : (at - H) * ASKS / W;                                                                   \
+        constexpr int after = at < H ? 0 : at + 1 - H >= W ? ASKS : (at + 1 - H) * ASKS / W;                                                            \
+        if constexpr (!(ODD) && (MORE)) {                                                                                                               \
+          constexpr int from = at >= H ? SCALES : at * SCALES / H, to = at >= H ? SCALES : (at + 1) * SCALES / H;                                       \
+          mx_unrolled<to - from>([&](auto k) { scale(from + k.value, min((S) / 2 + 1, quads - 1)); });                                                  \
+        }                                                                                                                                               \
+        mx_unrolled<after - before>([&](auto k) { MX_ASK(ASKED, (S) + 3, before + k.value) });                                                          \
+        __builtin_amdgcn_sched_barrier(0);                                                                                                              \
+      });                                                                                                                                               \
+    });                                                                                                                                                 \
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((ODD) || !(MORE) ? ASKS + LATE : ASKS + LATE + SCALES) : "memory");                                        \
+    __builtin_amdgcn_s_barrier();                                                                                                                       \
     __builtin_amdgcn_sched_barrier(0);
 #define MX_QUAD                                                               \
     _Pragma("unroll") for (int t = 0; t < SCALES; t++) now[t] = next[t];
     int q = q0;
     for (; q + 1 < q1; q += 2) {
       MX_QUAD
-      MX_STEP(buf0, buf1, buf3, 2 * q, 0)
-      MX_STEP(buf1, buf2, buf0, 2 * q + 1, 1)
+      MX_STEP(buf0, buf1, buf3, 2 * q, 0, 1)
+      MX_STEP(buf1, buf2, buf0, 2 * q + 1, 1, 1)
       MX_QUAD
-      MX_STEP(buf2, buf3, buf1, 2 * q + 2, 0)
-      MX_STEP(buf3, buf0, buf2, 2 * q + 3, 1)
+      MX_STEP(buf2, buf3, buf1, 2 * q + 2, 0, 1)
+      MX_STEP(buf3, buf0, buf2, 2 * q + 3, 1, 1)
       if (IN_PLACE) mx_sums_done();
     }
     if (q < q1) {
       MX_QUAD
-      MX_STEP(buf0, buf1, buf3, 2 * q, 0)
-      MX_STEP(buf1, buf2, buf0, 2 * q + 1, 1)
+      MX_STEP(buf0, buf1, buf3, 2 * q, 0, 0)
+      MX_STEP(buf1, buf2, buf0, 2 * q + 1, 1, 0)
       if (IN_PLACE) mx_sums_done();
     }
 #undef MX_QUAD
