@@ -55,11 +55,12 @@ __global__ __launch_bounds__(256) void mx_dequantize_kernel(const uint8_t* __res
   mx_values(reinterpret_cast<const uint32_t*>(codes)[i], mx_scale_value(scales[i >> 2]), out + 8 * i);
 }
 
-// The lower end of silu(g) u in FP32, for g between -80 and 2^100: exp(-g) as exp2 of hi = -g log2(e) rounded, times 1 + r with r = -g - hi ln2
+// The lower end of silu(g) u in FP32, for g between -80 and 2^100 whose magnitude, where it is not zero, is 2^-100 and more or that of a 16-bit type: exp(-g) as exp2 of hi = -g log2(e) rounded, times 1 + r with r = -g - hi ln2
 // (the product exact, in one multiply-add), one reciprocal, whose argument is scaled by 1 + MX_SILU_OFF. Without that scaling it is off by
 // less than MX_SILU_OFF of its value: 2^-23 each for exp2 and the reciprocal, 2^-24 each for the correction, the sum and the two products,
 // 80 x 2^-28.4 = 2^-22.1 for ln2 in FP32, together 0.73 x 2^-20 (and 2^-24 for the scaling's rounding); so the exact value lies between
-// this and this (1 + 2 MX_SILU_OFF) (1 + 2^-23), which MX_SILU_SPAN is above.
+// this and this (1 + 2 MX_SILU_OFF) (1 + 2^-23), which MX_SILU_SPAN is above. (A smaller FP32 gate's half is subnormal and loses bits that a large u brings
+// back. BF16's smallest gates have eight bits at most, whose half FP32 holds exactly; FP16's are normal here.)
 constexpr float MX_SILU_OFF = 0x1p-20f, MX_SILU_SPAN = 0x1.2p-19f;
 __device__ __forceinline__ float mx_silu_mul(float g, float u) {
   const float hi = g * -1.44269504088896340736f;
@@ -72,7 +73,7 @@ __device__ __forceinline__ float mx_silu_mul(float g, float u) {
 // silu(gate) * up of [rows, 2 half] rounded to the format in one pass; gate | up, or both in alternating blocks of `pairs` columns.
 // A product within FP32's error of a border between two codes, or a group whose largest is that near a power of two, would
 // round by that error: such a group (a few in a million values) is computed again in 64 bits, and so is one
-// whose products leave FP32's comfortable range. Bound by what it reads: 2048 x 51200 of FP16 49 us, 4.8 TB/s (5.0 is what a plain read of data that is not
+// whose gates or products leave FP32's comfortable range. Bound by what it reads: 2048 x 51200 of FP16 49 us, 4.8 TB/s (5.0 is what a plain read of data that is not
 // in the Infinity Cache reaches); with a 64-bit division a lane and a longer exponential 52.
 template <typename T>
 __global__ __launch_bounds__(256) void mx_silu_quantize_kernel(const T* __restrict__ x, int64_t rows, int half, int pairs, uint8_t* __restrict__ codes,
@@ -98,14 +99,16 @@ __global__ __launch_bounds__(256) void mx_silu_quantize_kernel(const T* __restri
   u.load(x + up_at);
   Mx8<float> p, q;
   float least = 0.f, most_g = 0.f;  // (a NaN passes by: its product is one)
+  uint32_t small_g = 0xffffffffu;   // the bits of the smallest gate that is not zero, less one
 #pragma unroll
   for (int j = 0; j < 8; j++) {
     const float gj = g.at(j);
     p.v[j >> 2][j & 3] = mx_silu_mul(gj, u.at(j));
     least = __builtin_fminf(least, gj);
     if (!std::is_same_v<T, _Float16>) most_g = __builtin_fmaxf(most_g, gj);
+    if (std::is_same_v<T, float>) small_g = min(small_g, (__float_as_uint(gj) & 0x7fffffffu) - 1u);
   }
-  bool far = least < -80.0f || most_g > 0x1p100f;
+  bool far = least < -80.0f || most_g > 0x1p100f || small_g < 0x0d800000u - 1u;  // 2^-100
   const uint32_t top = quad_max(p.amax());
   uint32_t byte = mx_scale_byte(top);
   const float s = mx_scale_value(byte);

@@ -134,7 +134,7 @@ def silu_mul_quant_groups(gate_up: torch.Tensor, pairs: int = 0, torch_chain: bo
 
 def silu_mul_quant_mxfp4(gate_up: torch.Tensor, pairs: int = 0) -> mxfp4.Mxfp4:
     """silu(gate) * up of [..., 2 I] (BF16, FP16 or FP32) rounded to the microscaled four-bit format in the same launch: the codes
-    that the exact product has; columns gate | up, or (`pairs`, a multiple of eight) both alternating in blocks of that many. I a
+    that the product in 64 bits has; columns gate | up, or (`pairs`, a multiple of eight) both alternating in blocks of that many. I a
     multiple of 32. A group with an infinite or undefined product stands for NaN."""
     kind = mxfp4.TYPES.get(gate_up.dtype)
     if kind is None or gate_up.ndim == 0 or gate_up.shape[-1] % 64:

@@ -579,8 +579,8 @@ int hb_mxfp4_quantize(const void* x, int type, int64_t rows, int k, void* codes,
 /* The values back, [rows, k] of `type`: exact in FP32 and BF16, rounded (or infinite) where FP16 does not hold one. */
 int hb_mxfp4_dequantize(const void* codes, const void* scales, int64_t rows, int k, int type, void* out, void* stream);
 /* silu(gate) * up of gate_up [rows, 2 half] rounded to the format in one pass; the columns are gate | up or, `pairs` > 0 (a multiple
- * of eight dividing half), blocks of `pairs` gate columns and their `pairs` up columns. The codes are the exact product's (one beyond
- * FP32's range counts as an infinity). */
+ * of eight dividing half), blocks of `pairs` gate columns and their `pairs` up columns. The codes are those of the product
+ * in 64 bits (one beyond FP32's range counts as an infinity). */
 int hb_silu_mul_quant_mxfp4(const void* gate_up, int type, int64_t rows, int half, int pairs, void* codes, void* scales, void* stream);
 
 /* The weights' tile layout: its bytes for a matrix [n, k] (any n; 0: a size the kernels do not take), row-major codes and scales of
