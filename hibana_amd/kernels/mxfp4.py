@@ -135,7 +135,8 @@ def dequantize(q: Mxfp4, dtype: torch.dtype = torch.float32) -> torch.Tensor:
 
 def tile(q: Mxfp4, gated: bool = False) -> torch.Tensor:
     """Weights [N, K] or stacked ones [E, N, K] in the layout the products read (csrc/mxfp4.hpp): uint8 [bytes] or [E, bytes].
-    `gated`: fc1 of gated experts, rows [up; gate]."""
+    `gated`: fc1 of gated experts, rows [up; gate]. It is there when this returns: a call that finds the weights not laid out does it on its own stream
+    without its caller knowing, and the next call may be another stream's; nor does anything read the codes then, which may be released."""
     check(q, "mxfp4.tile")
     if q.codes.ndim not in (2, 3) or not q.codes.numel():
         raise ValueError("mxfp4.tile: a matrix [N, K] or stacked matrices [E, N, K]")
@@ -155,6 +156,7 @@ def tile(q: Mxfp4, gated: bool = False) -> torch.Tensor:
         _lib.check(_lib.lib().hb_mxfp4_repack(codes[lo * n:].data_ptr(), scales[lo * n:].data_ptr(), count, n, k, int(gated), stacked[lo:].data_ptr(),
                                               _lib.stream()), "mxfp4.tile")
         lo += count
+    torch.cuda.current_stream().synchronize()  # once a matrix
     return tiled
 
 
