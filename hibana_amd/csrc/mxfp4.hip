@@ -199,7 +199,7 @@ struct MxLinear {
 // Few rows: a workgroup NT tiles of weight rows, its wavefronts the chunks of K. The first weights are asked for, then the workgroup puts
 // the activations into LDS, rounded on the way: each workgroup all of them, which costs less than a launch. (32 x 32 x 64 products of which up to 31 columns are
 // idle: the matrix cores have nothing else to do.) One row of 5120 x 5120 5.4 us: latency of the launch, the activations, ten chunks of weights a wavefront
-// and the join. Eight rows of 25600 x 5120 14.2 us: the weights at 4.9 TB/s.
+// and the join. Eight rows of 25600 x 5120 14.2 us where part of the weights are in the Infinity Cache, 17.6 on cold ones: 4.0 TB/s.
 template <typename T, typename Y, int NT, int RUN>
 __global__ __launch_bounds__(512) void mx_few_rows_kernel(MxLinear p) {
   extern __shared__ f32x4_t part[];  // the activations, then [waves][NT * 4][64]
@@ -354,27 +354,38 @@ struct MxPlan {
   bool square;       // RING: the 2 x 2 forms
   size_t tiles, bytes;  // workspace: of the activations, of all
 };
-// Few rows (their activations fit LDS): a wavefront's chunks of K and few weight rows a workgroup keep a small matrix's call short, and the rounding rides
-// in it while all of a workgroup's rows are not more than MX_ROUND_VALUES values; past that it is a launch of its own. us in a graph and called one by one,
-// 20 rows of 4000 x 4096 (80 K values): inside 9.4 and 8.7, ahead 8.6 and 11.9; 31 rows of it (124 K) 11.5 and 10.7, 9.0 and 11.7. Where the matrix alone
-// fills the device several times over, the ring takes over from there: 8 rows of 25600 x 5120 17.8 rounding inside, 17.4 ring; 16 rows 20.7 and 17.3.
-constexpr int64_t MX_ROUND_VALUES = 80 * 1024;
-constexpr int MX_RING_TILES = 768;
-// More rows of a small matrix are passes of 32 rows beside one another, which read its weights again: one launch where the ring takes two, or three with K shared.
-// Up to MX_PASS_VALUES values a pass, and MX_PASSES_WORK of tiles x passes x k. us as above: 128 rows of 4000 x 832 (416 K) passes 7.4 and 8.1, ring 9.8 and
-// 11.4; 256 rows (832 K) 10.2 and 9.4, 9.6 and 11.4; 512 rows 15.5 and 14.5, 10.1 and 11.3; 128 rows of 1000 x 4000 (512 K) 11.5 and 10.6, 13.2 and 14.4.
-constexpr int64_t MX_PASS_VALUES = 128 * 1024, MX_PASSES_WORK = 768 * 1024;
+// Few rows (their activations fit LDS): one tile of weight rows a workgroup, or two, which share a workgroup's activations, where that does not give the busiest
+// compute unit more tiles. us in a graph on cold weights, eight rows of 5120 k, one and two: 256 tiles 8.8 and 9.8, 257 10.7 and 9.8, 384 11.4 and 11.2, 512 12.5
+// and 12.6, 513 14.1 and 15.0, 640 15.7 and 17.5, 768 16.5 and 17.9, 769 18.1 and 17.9, 800 19.9 and 18.0, 1024 21.3 and 19.4, 1280 25.6 and 26.0, 1600 31.9 and
+// 32.5; 32 rows of 1024 k, 320 tiles, 7.1 and 5.9; 128 rows of 4000 x 832 in passes 6.3 and 5.5, 160 rows 7.6 and 7.7.
 constexpr int MX_DEVICE = 256;  // compute units
+static bool two_tiles(int64_t tiles, int64_t passes) {
+  auto busiest = [&](int64_t workgroups) { return (workgroups * passes + MX_DEVICE - 1) / MX_DEVICE; };
+  return 2 * busiest((tiles + 1) / 2) <= busiest(tiles);
+}
+// The rounding rides in that launch, each workgroup all rows, while they are not more than so many values; past it the rounding is a launch of its own. us in a graph and
+// called one by one, inside and ahead: 20 rows of 4000 x 4096 (80 K values) 9.4 and 8.7, 8.6 and 11.9; 31 rows of it (124 K) 11.5 and 10.7, 9.0 and 11.7. More tiles
+// than compute units, cold weights, 5120 k: two tiles a workgroup, 320 tiles, 12 rows (60 K) 11.2 and 11.0, 11.2 and 10.7, 16 rows (80 K) 12.5 and 12.3, 11.4 and 10.8; 800
+// tiles 18.7 and 18.4, 18.9 and 18.3, then 21.1 and 20.7, 19.2 and 18.7; one tile, 640, 8 rows (40 K) 15.7 and 15.3, 16.2 and 15.6, 12 rows 17.3 and 17.0, 16.7 and 16.1.
+static int64_t round_values(int64_t tiles) { return (tiles <= MX_DEVICE ? 80 : two_tiles(tiles, 1) ? 64 : 48) * 1024; }
+// Past that size a matrix of four and more tiles a compute unit goes to the ring. us as above, ahead and ring, 5120 k: 16 rows of 800 tiles 19.2 and 18.7, 20.6 and 20.0, 24 rows
+// 19.8 and 19.1, 20.9 and 20.4; 16 rows of 1280 26.5 and 25.5, 26.7 and 25.7, 24 rows 29.1 and 28.2, 26.9 and 26.0; of 1600 33.0 and 31.8, 31.2 and 30.1.
+constexpr int MX_RING_TILES = 4 * MX_DEVICE;
+// More rows of a small matrix are passes of 32 rows beside one another, which read its weights again: one launch where the ring takes two, or three with K shared.
+// Up to MX_PASS_VALUES values a pass, and MX_PASSES_WORK of tiles x passes x k. us as above, passes and ring: 128 rows of 4000 x 832 (416 K) 5.6 and 6.9, 8.1 and 10.7; 64
+// rows of 4000 x 1664 (416 K) 7.2 and 7.2, 10.5 and 14.2; 128 rows of 1000 x 4000 (512 K) 10.4 and 10.3, 11.5 and 14.2; 256 rows of 12000 x 256 (768 K) 9.2 and 9.1, 7.2
+// and 10.8.
+constexpr int64_t MX_PASS_VALUES = 128 * 1024, MX_PASSES_WORK = 768 * 1024;
 static MxPlan plan_of(int64_t m, int64_t n, int k, int x_type) {
   const MxLayout rows(m, k), w(n, k);
   MxPlan p{};
   const size_t acts = MxActs::bytes(m, k);
-  const bool small = m * k <= MX_ROUND_VALUES;
+  const bool small = m * k <= round_values(w.tiles);
   if (m > MX_ROWS && (int64_t)MX_ROWS * k <= MX_PASS_VALUES && (int64_t)rows.tiles * w.tiles * k <= MX_PASSES_WORK) {
     p.way = MxPlan::FEW_ROUNDING;
     return p;
   }
-  if (m <= MX_ROWS && acts <= (w.tiles <= 256 ? 144 : 64) * 1024 && (small || w.tiles < MX_RING_TILES)) {
+  if (m <= MX_ROWS && acts <= (w.tiles <= 256 ? 144 : 64) * 1024 && (small || w.tiles <= MX_RING_TILES)) {
     const bool rounds = x_type != HB_MXFP4 && !small;
     p.way = rounds ? MxPlan::FEW : MxPlan::FEW_ROUNDING;
     p.tiles = p.bytes = rounds ? (size_t)m * (k / 2 + k / MX_GROUP) : 0;
@@ -451,7 +462,7 @@ static int launch_linear(MxLinear p, uint8_t* workspace, hipStream_t stream) {
     p.waves = std::min(at.chunks, 8);
     auto few = [&](auto* type) {
       using X = std::remove_pointer_t<decltype(type)>;
-      if (at.tiles >= 512) return launch_few<X, Y, 2, 4>(p, at, stream);
+      if (two_tiles(at.tiles, (p.m + MX_ROWS - 1) / MX_ROWS)) return launch_few<X, Y, 2, 4>(p, at, stream);
       return at.chunks >= 32 ? launch_few<X, Y, 1, 4>(p, at, stream) : launch_few<X, Y, 1, 1>(p, at, stream);
     };
     return plan.way == MxPlan::FEW ? few((uint8_t*)nullptr) : few((T*)nullptr);
