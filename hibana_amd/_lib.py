@@ -111,6 +111,7 @@ SIGNATURES = {
     "hb_mxfp4_unpack": (_I, [_P, _I, _L, _I, _I, _P, _P, _P]),
     "hb_mxfp4_linear_workspace_bytes": (_Z, [_L, _L, _I, _I]),
     "hb_mxfp4_moe_workspace_bytes": (_Z, [C.POINTER(HbMxfp4Experts), _I, _I]),
+    "hb_mxfp4_moe_pairs_workspace_bytes": (_Z, [C.POINTER(HbMxfp4Experts), _I, _I]),
     "hb_mxfp4_moe": (_I, [C.POINTER(HbMxfp4Experts), _P, _P, _P, _I, _I, _I, _P, _P, _Z, _P]),
     "hb_mxfp4_linear": (_I, [_P, _P, _I, _L, _P, _L, _I, _P, _I, _P, _Z, _P]),
 }

@@ -686,10 +686,12 @@ int check(const hb_mxfp4_experts* ex) {
 
 using namespace hb;
 
-extern "C" size_t hb_mxfp4_moe_workspace_bytes(const hb_mxfp4_experts* experts, int m, int topk) {
+static size_t workspace_of(const hb_mxfp4_experts* experts, int m, int topk, bool sum) {
   if (check(experts) != HB_OK || m <= 0 || topk <= 0 || topk > MX_MOST_TOPK || (int64_t)m * topk > 0x3fffffff) return 0;
-  return carve(experts, nullptr, m, topk, true).bytes;
+  return carve(experts, nullptr, m, topk, sum).bytes;
 }
+extern "C" size_t hb_mxfp4_moe_workspace_bytes(const hb_mxfp4_experts* experts, int m, int topk) { return workspace_of(experts, m, topk, true); }
+extern "C" size_t hb_mxfp4_moe_pairs_workspace_bytes(const hb_mxfp4_experts* experts, int m, int topk) { return workspace_of(experts, m, topk, false); }
 
 // One pass: m <= most_rows. A sum's pairs lie in FP32 between fc2 and the combine, at any number of rows: in BF16 the largest tensor of a prefill would be half as
 // large, but each pair would be rounded once more than the result is (1543 rows of 10 of 512 experts (2048, 512): relative

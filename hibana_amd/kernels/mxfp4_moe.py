@@ -100,7 +100,7 @@ def _struct(experts: Mxfp4Experts) -> _lib.HbMxfp4Experts:
         have = _lib.HbMxfp4Experts(experts.tiled1.data_ptr(), experts.tiled2.data_ptr(), e, experts.base, h, i, h2, int(experts.gated))
         have.of = (experts.tiled1, experts.tiled2, experts.base, experts.shape1, experts.shape2)
         have.at = C.byref(have)
-        have.bytes_of = {}  # the workspace a call of (rows, k) takes
+        have.bytes_of = {}  # the workspace a call of (rows, k, pairs or a sum) takes
         experts._packed = have
     return have
 
@@ -123,11 +123,11 @@ def mxfp4_moe(experts: Mxfp4Experts, x: torch.Tensor, ids: torch.Tensor, weights
     if m == 0 or k == 0:
         return out if pairs else out.zero_()
     lib = _lib.lib()
-    need = st.bytes_of.get((m, k))
+    need = st.bytes_of.get((m, k, mode > 0))
     if need is None:
         if len(st.bytes_of) >= 4096:
             st.bytes_of.clear()
-        need = st.bytes_of[m, k] = lib.hb_mxfp4_moe_workspace_bytes(st.at, m, k)
+        need = st.bytes_of[m, k, mode > 0] = (lib.hb_mxfp4_moe_pairs_workspace_bytes if mode else lib.hb_mxfp4_moe_workspace_bytes)(st.at, m, k)
     ws = experts.tiled1.new_empty(max(need, 16))  # (of the capture's own pool in a captured call)
     # converted operands keep a name until the launches are enqueued
     ids32 = ids if ids.dtype == torch.int32 and ids.is_contiguous() else ids.to(torch.int32).contiguous()

@@ -600,13 +600,15 @@ int hb_mxfp4_linear(const void* x, const void* x_scales, int x_type, int64_t m, 
  * hidden_out of eight, up to 960 experts and a topk of 4096. x [m, hidden] BF16 is rounded to the format, h between the two products as well (from its FP32 value). An id
  * outside base .. base + experts - 1 adds nothing. mode HB_MOE_SUM: out BF16 [m, hidden_out], FP32 sums of FP32 pairs rounded once; HB_MOE_PAIRS_F32 / _BF16: the
  * pairs' outputs [m * topk, hidden_out] (those of skipped pairs unspecified). `workspace`: plain scratch, nothing in it need be zero; that of
- * 2^18 pairs at most (more go in passes, one behind the other). */
+ * 2^18 pairs at most (more go in passes, one behind the other). hb_mxfp4_moe_workspace_bytes serves every mode; where `out` takes the pairs' outputs,
+ * hb_mxfp4_moe_pairs_workspace_bytes is enough, less a sum's FP32 pairs. */
 typedef struct {
   const void* fc1;
   const void* fc2;
   int experts, base, hidden, inter, hidden_out, gated;
 } hb_mxfp4_experts;
 size_t hb_mxfp4_moe_workspace_bytes(const hb_mxfp4_experts* experts, int m, int topk);
+size_t hb_mxfp4_moe_pairs_workspace_bytes(const hb_mxfp4_experts* experts, int m, int topk);
 int hb_mxfp4_moe(const hb_mxfp4_experts* experts, const void* x, const int32_t* ids, const float* weights, int m, int topk, int mode, void* out,
                  void* workspace, size_t workspace_bytes, void* stream);
 
