@@ -16,6 +16,7 @@ import torch
 from hibana_amd import _lib
 from hibana_amd.kernels import mxfp4
 
+ID_TYPES = (torch.int32, torch.int64, torch.int16, torch.int8, torch.uint8)
 MAX_EXPERTS = 960  # of one object: a plan's counts of them lie in LDS
 
 
@@ -105,6 +106,13 @@ def _struct(experts: Mxfp4Experts) -> _lib.HbMxfp4Experts:
     return have
 
 
+def _ids32(ids: torch.Tensor) -> torch.Tensor:
+    """Contiguous int32 ids. A wider one that int32 does not hold is outside of every range and stays so: cut off, it could name an expert."""
+    if ids.dtype == torch.int64:
+        ids = ids.clamp(-1, 2**31 - 1)
+    return ids.to(torch.int32).contiguous()
+
+
 def mxfp4_moe(experts: Mxfp4Experts, x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, pairs: bool = False, pairs_bf16: bool = False) -> torch.Tensor:
     """Routed experts for x [M, H] BF16 with the router's ids [M, k] and weights [M, k] -> BF16 [M, H_out], the weighted sum of a row's pairs in
     FP32, added in an order that the sizes alone decide, and rounded once. An id outside this object's range base .. base + E - 1 adds nothing. With `pairs`, the FP32 (`pairs_bf16`:
@@ -115,6 +123,8 @@ def mxfp4_moe(experts: Mxfp4Experts, x: torch.Tensor, ids: torch.Tensor, weights
         raise ValueError("mxfp4_moe: x must be BF16 [M, hidden]")
     if ids.ndim != 2 or ids.shape[0] != x.shape[0] or weights.shape != ids.shape:
         raise ValueError("mxfp4_moe: ids and weights must be [M, k]")
+    if ids.dtype not in ID_TYPES:
+        raise ValueError("mxfp4_moe: ids must be whole numbers, int64 at most")
     st = _struct(experts)
     stream = _lib.stream_of(x, ids, weights, experts.tiled1, experts.tiled2)
     m, k = ids.shape
@@ -130,7 +140,7 @@ def mxfp4_moe(experts: Mxfp4Experts, x: torch.Tensor, ids: torch.Tensor, weights
         need = st.bytes_of[m, k, mode > 0] = (lib.hb_mxfp4_moe_pairs_workspace_bytes if mode else lib.hb_mxfp4_moe_workspace_bytes)(st.at, m, k)
     ws = experts.tiled1.new_empty(max(need, 16))  # (of the capture's own pool in a captured call)
     # converted operands keep a name until the launches are enqueued
-    ids32 = ids if ids.dtype == torch.int32 and ids.is_contiguous() else ids.to(torch.int32).contiguous()
+    ids32 = ids if ids.dtype == torch.int32 and ids.is_contiguous() else _ids32(ids)
     wt = weights if weights.dtype == torch.float32 and weights.is_contiguous() else weights.float().contiguous()
     xc = mxfp4.rows16(x)
     code = lib.hb_mxfp4_moe(st.at, xc.data_ptr(), ids32.data_ptr(), wt.data_ptr(), m, k, mode, out.data_ptr(), ws.data_ptr(), need, stream)
