@@ -73,8 +73,8 @@ __device__ __forceinline__ float mx_silu_mul(float g, float u) {
 // silu(gate) * up of [rows, 2 half] rounded to the format in one pass; gate | up, or both in alternating blocks of `pairs` columns.
 // A product within FP32's error of a border between two codes, or a group whose largest is that near a power of two, would
 // round by that error: such a group (a few in a million values) is computed again in 64 bits, and so is one
-// whose gates or products leave FP32's comfortable range. Bound by what it reads: 2048 x 51200 of FP16 49 us, 4.8 TB/s (5.0 is what a plain read of data that is not
-// in the Infinity Cache reaches); with a 64-bit division a lane and a longer exponential 52.
+// whose gates or products leave FP32's comfortable range. Mostly reading: 2048 x 51200 of FP16 49 us, 4.8 TB/s (a plain read of data that is not
+// in the Infinity Cache reaches 6.9); with a 64-bit division a lane and a longer exponential 52.
 template <typename T>
 __global__ __launch_bounds__(256) void mx_silu_quantize_kernel(const T* __restrict__ x, int64_t rows, int half, int pairs, uint8_t* __restrict__ codes,
                                                                uint8_t* __restrict__ scales) {
@@ -198,7 +198,7 @@ struct MxLinear {
 
 // Few rows: a workgroup NT tiles of weight rows, its wavefronts the chunks of K. The first weights are asked for, then the workgroup puts
 // the activations into LDS, rounded on the way: each workgroup all of them, which costs less than a launch. (32 x 32 x 64 products of which up to 31 columns are
-// idle: the matrix cores have nothing else to do.) One row of 5120 x 5120 5.4 us: latency of the launch, the activations, ten chunks of weights a wavefront
+// idle: the matrix cores have nothing else to do.) One row of 5120 x 5120 5.4 us (on cold weights 6.5): latency of the launch, the activations, ten chunks of weights a wavefront
 // and the join. Eight rows of 25600 x 5120 14.2 us where part of the weights are in the Infinity Cache, 17.6 on cold ones: 4.0 TB/s.
 template <typename T, typename Y, int NT, int RUN>
 __global__ __launch_bounds__(512) void mx_few_rows_kernel(MxLinear p) {
@@ -274,7 +274,7 @@ __global__ __launch_bounds__(512) void mx_few_rows_kernel(MxLinear p) {
 // instruction's operands come from LDS at half of the 128 bytes a cycle that it gives, what is asked for at a quarter. 2048 rows of 25600 x 5120:
 // three rounds of the device in 122 us, 4.2 PFLOP/s (the products alone 6.6 on random data, at the clock that the card's power leaves them;
 // without any loads into LDS 15 % less time, with loads from the L2 alone 6 %), the last columns 17. Up to 128 rows a wavefront has all of
-// the workgroup's rows and its own weights: 77 rows 15.3 us, the weights at 4.6 TB/s.
+// the workgroup's rows and its own weights: 77 rows 15.3 us, the weights at 4.6 TB/s, half of them from the Infinity Cache; on cold ones 20.9.
 struct MxTiles {
   const uint8_t* a;
   const uint8_t* w;

@@ -225,7 +225,8 @@ struct MxStream {
     }
     ask(min(c0, at.chunks - 1));
   }
-  // (chunks past the end are asked for again and not multiplied)
+  // (chunks past the end are asked for again and not multiplied) The weights take their place in the Infinity Cache: eight rows of 25600 x 5120 14.0 us where three such
+  // matrices are read in turn, 19.3 where ten are; with MX_NO_REUSE 15.8 and 17.8.
   __device__ __forceinline__ void ask(int c) {
     const uint32_t lane = threadIdx.x & 63;
 #pragma unroll

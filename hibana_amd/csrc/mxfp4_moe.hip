@@ -270,7 +270,7 @@ __global__ __launch_bounds__(PLAN_THREADS) void mx_count_round_kernel(const int3
 // A wavefront's walk over steps of eight chunks of two weight tiles, for a slot of the plan (up to 32 MT rows of an expert). A step's weights, 16 KB
 // a wavefront, are asked for as soon as the step before has taken its own out of the registers, so they are on their way while sums
 // are joined, rounded and stored; a slot's activations (32 bytes of a row's chunk, read where they lie) stay in registers where one
-// step covers the wavefront's K. Bound by reading the weights: 1543 rows of 10 of 512 experts (2048, 512) fc1 116 us, 4.9 TB/s, fc2 86 us, 4.8 with its
+// step covers the wavefront's K. Mostly reading the weights: 1543 rows of 10 of 512 experts (2048, 512) fc1 116 us, 4.9 TB/s where a plain read reaches 6.9, fc2 86 us, 4.8 with its
 // results; 32 rows 24 and 13 us, 5.1 and 4.7; four rows of 22 of 512 ReLU^2 experts (1024, 2688) 23 and 23 us, 5.2.
 template <int MT>
 struct MxWalk {
@@ -461,8 +461,8 @@ __global__ __launch_bounds__(64 * MX_MOE_WAVES, MT == 1 ? 3 : 2) void mx_fc2_man
 
 // ------------------------------------------------------------------------------------------------ many pairs an expert
 // The ring (mxfp4_ring.hpp) on the plan's slots of MX_RING_ROWS rows: the slot's rows of x rounded into the tile layout, fc1 with h rounded into it
-// from the accumulators, fc2 with each row's results to its pair. 2048 rows of 8 of 64 experts (2560, 768), 256 rows each: gather 15 us, fc1 64
-// (2.0 PFLOP/s, 9 TB/s into LDS), fc2 51 (1.3: six steps a workgroup, beside which its start and end are long, and 84 MB of results).
+// from the accumulators, fc2 with each row's results to its pair. 2048 rows of 8 of 64 experts (2560, 768), 256 rows each: gather 15 us, fc1 65
+// (2.0 PFLOP/s, 9 TB/s into LDS), fc2 65 (1.0: six steps a workgroup, beside which its start and end are long, and 168 MB of results; 51 where they are BF16).
 using MxMoeRing = MxRing<2, 2, 2, 2>;
 constexpr int MX_RING_ROWS = MxMoeRing::TA * MX_ROWS;
 
