@@ -368,7 +368,7 @@ static bool two_tiles(int64_t tiles, int64_t passes) {
 // than compute units, cold weights, 5120 k: two tiles a workgroup, 320 tiles, 12 rows (60 K) 11.2 and 11.0, 11.2 and 10.7, 16 rows (80 K) 12.5 and 12.3, 11.4 and 10.8; 800
 // tiles 18.7 and 18.4, 18.9 and 18.3, then 21.1 and 20.7, 19.2 and 18.7; one tile, 640, 8 rows (40 K) 15.7 and 15.3, 16.2 and 15.6, 12 rows 17.3 and 17.0, 16.7 and 16.1.
 static int64_t round_values(int64_t tiles) { return (tiles <= MX_DEVICE ? 80 : two_tiles(tiles, 1) ? 64 : 48) * 1024; }
-// Past that size a matrix of four and more tiles a compute unit goes to the ring. us as above, ahead and ring, 5120 k: 16 rows of 800 tiles 19.2 and 18.7, 20.6 and 20.0, 24 rows
+// Past that size a matrix of more than four tiles a compute unit goes to the ring. us as above, ahead and ring, 5120 k: 16 rows of 800 tiles 19.2 and 18.7, 20.6 and 20.0, 24 rows
 // 19.8 and 19.1, 20.9 and 20.4; 16 rows of 1280 26.5 and 25.5, 26.7 and 25.7, 24 rows 29.1 and 28.2, 26.9 and 26.0; of 1600 33.0 and 31.8, 31.2 and 30.1.
 constexpr int MX_RING_TILES = 4 * MX_DEVICE;
 // More rows of a small matrix are passes of 32 rows beside one another, which read its weights again: one launch where the ring takes two, or three with K shared.
