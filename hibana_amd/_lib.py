@@ -35,10 +35,16 @@ class HbMxfp4Experts(C.Structure):
                 ("hidden_out", C.c_int), ("gated", C.c_int)]
 
 
+class HbAdapters(C.Structure):
+    _fields_ = [("a", C.c_void_p), ("b", C.c_void_p), ("scale", C.c_void_p), ("ranks", C.c_void_p), ("adapters", C.c_int), ("rank", C.c_int),
+                ("k", C.c_int), ("n", C.c_int), ("type", C.c_int)]
+
+
 _P, _I, _L, _Z, _F = C.c_void_p, C.c_int, C.c_int64, C.c_size_t, C.c_float
 _LW = C.POINTER(HbLatentWeights)
 _EX = C.POINTER(HbW3Experts)
 _EX4 = C.POINTER(HbNvfp4Experts)
+_AD = C.POINTER(HbAdapters)
 # name -> (restype, argtypes): every symbol include/hibana_hip.h declares
 SIGNATURES = {
     "hb_version": (_I, []),
@@ -113,6 +119,9 @@ SIGNATURES = {
     "hb_mxfp4_moe_workspace_bytes": (_Z, [C.POINTER(HbMxfp4Experts), _I, _I]),
     "hb_mxfp4_moe_pairs_workspace_bytes": (_Z, [C.POINTER(HbMxfp4Experts), _I, _I]),
     "hb_mxfp4_moe": (_I, [C.POINTER(HbMxfp4Experts), _P, _P, _P, _I, _I, _I, _P, _P, _Z, _P]),
+    "hb_adapters_workspace_bytes": (_Z, [_AD, _L, _I]),
+    "hb_adapters_add": (_I, [_AD, _P, _L, _P, _L, _P, _I, _L, _P, _L, _P, _Z, _P]),
+    "hb_adapters_grads": (_I, [_AD, _P, _L, _P, _L, _P, _I, _L, _P, _P, _P, _P, _Z, _P]),
     "hb_mxfp4_linear": (_I, [_P, _P, _I, _L, _P, _L, _I, _P, _I, _P, _Z, _P]),
 }
 

@@ -1,0 +1,206 @@
+"""Low-rank adapters of many requests at once beside a shared projection, and their gradients: what a fine-tune learns around
+frozen quantized weights, and what a server then holds beside them.
+
+    out[r] = y[r] + scale_i (x[r] a_i^T) b_i,   i = index[r]
+
+A pool holds the adapters of one projection [N, K], both matrices rank by rank: a [adapters, rank, K] and b [adapters, rank, N] (a
+checkpoint's lora_B [N, rank], transposed once). So every product of the forward and the backward pass reads along a matrix's rows. Products
+have FP32 sums; the sums between the two of an adapter stay what FP32 holds of them to 2^-16 (BF16) or better, and the result is rounded
+once. No counterpart in the reference.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from hibana_amd import _lib
+from hibana_amd.kernels.mxfp4 import TYPES
+
+MOST, MOST_RANK = 4096, 256  # what the kernels take: adapters of a pool, their rank
+
+
+class Adapters:
+    """a [adapters, rank, K] and b [adapters, rank, N] of one type (BF16, FP16 or FP32), contiguous. `scale`: FP32 [adapters] or a number (None: 1).
+    `ranks` int32 [adapters]: how many of the `rank` rows are adapter i's (None: all; the rows behind them are not read). Tensors that require gradients get them through `add`."""
+
+    def __init__(self, a: torch.Tensor, b: torch.Tensor, scale: torch.Tensor | float | None = None, ranks: torch.Tensor | None = None):
+        if a.ndim != 3 or b.ndim != 3 or a.shape[:2] != b.shape[:2] or a.dtype != b.dtype or a.dtype not in TYPES or not a.numel() or not b.numel():
+            raise ValueError("Adapters: a [adapters, rank, K] and b [adapters, rank, N], both BF16, FP16 or FP32")
+        if a.shape[0] > MOST or a.shape[1] > MOST_RANK:
+            raise ValueError(f"Adapters: up to {MOST} adapters of a rank up to {MOST_RANK}")
+        if not a.is_contiguous() or not b.is_contiguous():
+            raise ValueError("Adapters: a and b must be contiguous")
+        if isinstance(scale, (int, float)):
+            scale = torch.full((a.shape[0],), float(scale), dtype=torch.float32, device=a.device)
+        if scale is not None and (scale.dtype != torch.float32 or scale.shape != a.shape[:1] or not scale.is_contiguous()):
+            raise ValueError("Adapters: scale FP32 [adapters]")
+        if ranks is not None and (ranks.dtype != torch.int32 or ranks.shape != a.shape[:1] or not ranks.is_contiguous()):
+            raise ValueError("Adapters: ranks int32 [adapters]")
+        if any(t is not None and t.device != a.device for t in (b, scale, ranks)):
+            raise ValueError("Adapters: one device")
+        self.a, self.b, self.scale, self.ranks = a, b, scale, ranks
+        self._struct = self._at = None
+        self._rooms: dict[tuple[int, int], int] = {}
+
+    @classmethod
+    def from_pairs(cls, pairs, dtype: torch.dtype = torch.bfloat16, device: torch.device | str = "cuda") -> "Adapters":
+        """A pool of the adapters (A [r, K], B [N, r], scale) as checkpoints hold them, of any ranks."""
+        pairs = list(pairs)
+        if not pairs or any(x.ndim != 2 or y.ndim != 2 or x.shape[0] != y.shape[1] or x.shape[1] != pairs[0][0].shape[1] or y.shape[0] != pairs[0][1].shape[0] for x, y, _ in pairs):
+            raise ValueError("Adapters.from_pairs: (A [r, K], B [N, r], scale) of one projection")
+        sizes = [x.shape[0] for x, _, _ in pairs]
+        rank = max(max(sizes), 1)
+        pool = cls(torch.zeros((len(pairs), rank, pairs[0][0].shape[1]), dtype=dtype, device=device), torch.zeros((len(pairs), rank, pairs[0][1].shape[0]), dtype=dtype, device=device),
+                   torch.ones(len(pairs), dtype=torch.float32, device=device), torch.tensor(sizes, dtype=torch.int32, device=device))
+        for i, pair in enumerate(pairs):
+            pool.set(i, *pair)
+        return pool
+
+    def set(self, i: int, a: torch.Tensor, b: torch.Tensor, scale: float = 1.0) -> None:
+        """Adapter i replaced by A [r, K], B [N, r], on the current stream. r below the pool's rank needs a pool with `ranks`, a scale one with `scale`."""
+        n, rank, k = self.a.shape
+        r = a.shape[0]
+        if not 0 <= i < n or tuple(a.shape) != (r, k) or tuple(b.shape) != (self.out_features, r) or r > rank or (r < rank and self.ranks is None) or (scale != 1.0 and self.scale is None):
+            raise ValueError(f"Adapters.set: an adapter A [r, {k}], B [{self.out_features}, r] of this pool (rank {rank}{'' if self.ranks is not None else ', all of them of it'})")
+        with torch.no_grad():
+            self.a[i, :r].copy_(a)
+            self.b[i, :r].copy_(b.T)
+            if self.scale is not None:
+                self.scale[i].fill_(float(scale))
+            if self.ranks is not None:
+                self.ranks[i].fill_(r)
+
+    @property
+    def adapters(self) -> int:
+        return self.a.shape[0]
+
+    @property
+    def rank(self) -> int:
+        return self.a.shape[1]
+
+    @property
+    def in_features(self) -> int:
+        return self.a.shape[2]
+
+    @property
+    def out_features(self) -> int:
+        return self.b.shape[2]
+
+    @property
+    def bytes(self) -> int:
+        return (self.a.numel() + self.b.numel()) * self.a.element_size()
+
+    def __getstate__(self):
+        return {**self.__dict__, "_struct": None, "_at": None, "_rooms": {}}
+
+    def struct(self):
+        """What the library takes, made again where a tensor's place has changed (an optimizer may have put another one in)."""
+        at = (self.a.data_ptr(), self.b.data_ptr(), _lib.ptr(self.scale), _lib.ptr(self.ranks))
+        if at != self._at:
+            n, rank, k = self.a.shape
+            self._struct, self._at = C.byref(_lib.HbAdapters(*at, n, rank, k, self.b.shape[2], TYPES[self.a.dtype])), at
+        return self._struct
+
+    def room(self, m: int, grads: int) -> int:
+        need = self._rooms.get((m, grads))
+        if need is None:
+            if len(self._rooms) >= 4096:
+                self._rooms.clear()
+            need = self._rooms[m, grads] = _lib.lib().hb_adapters_workspace_bytes(self.struct(), m, grads)
+        return need
+
+
+def _rows(t: torch.Tensor, width: int, pool: Adapters, what: str) -> torch.Tensor:
+    if t.dtype != pool.a.dtype or t.ndim != 2 or t.shape[1] != width:
+        raise ValueError(f"{what}: {pool.a.dtype} [M, {width}]")
+    return t if t.stride(1) == 1 and t.stride(0) >= width or t.shape[0] == 1 and t.stride(1) == 1 else t.contiguous()
+
+
+def _index(index: torch.Tensor, m: int, what: str) -> torch.Tensor:
+    if index.dtype not in (torch.int32, torch.int64) or index.ndim != 1 or index.shape[0] != m:
+        raise ValueError(f"{what}: an int32 or int64 index [{m}]")
+    return index if index.is_contiguous() else index.contiguous()
+
+
+def _stride(t: torch.Tensor) -> int:
+    return max(t.stride(0), t.shape[1])  # (that of a single row is nobody's)
+
+
+def _add(y: torch.Tensor, x: torch.Tensor, pool: Adapters, index: torch.Tensor, out: torch.Tensor | None) -> torch.Tensor:
+    what = "adapters.add"
+    yr, xr = _rows(y, pool.out_features, pool, what), _rows(x, pool.in_features, pool, what)
+    m = yr.shape[0]
+    if xr.shape[0] != m:
+        raise ValueError(f"{what}: as many rows of x as of y")
+    ix = _index(index, m, what)
+    stream = _lib.stream_of(yr, xr, ix, pool.a)
+    if out is None:
+        out = yr.new_empty((m, yr.shape[1]))
+    elif out.dtype != yr.dtype or out.shape != yr.shape or out.stride(1) != 1 or (m > 1 and out.stride(0) < out.shape[1]) or out.device != yr.device:
+        raise ValueError(f"{what}: out like y, its rows contiguous")
+    if m:
+        need = pool.room(m, 0)
+        ws = yr.new_empty(need, dtype=torch.uint8)  # (of the capture's own pool in a captured call)
+        code = _lib.lib().hb_adapters_add(pool.struct(), xr.data_ptr(), _stride(xr), yr.data_ptr(), _stride(yr), ix.data_ptr(), ix.element_size(), m, out.data_ptr(), _stride(out),
+                                          ws.data_ptr(), need, stream)
+        if code:
+            _lib.check(code, what)
+    return out
+
+
+class _Add(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, y, x, a, b, pool, index):
+        ctx.save_for_backward(x, a, b, index)
+        ctx.pool = pool
+        return _add(y, x, pool, index, None)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, a, b, index = ctx.saved_tensors
+        _, need_x, need_a, need_b, _, _ = ctx.needs_input_grad
+        if not (need_x or need_a or need_b):
+            return dy, None, None, None, None, None
+        dx, da, db = grads(dy, x, Adapters(a.detach(), b.detach(), ctx.pool.scale, ctx.pool.ranks), index)
+        return dy, dx if need_x else None, da.to(a.dtype) if need_a else None, db.to(b.dtype) if need_b else None, None, None
+
+
+def add(y: torch.Tensor, x: torch.Tensor, pool: Adapters, index: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
+    """y [M, N] plus each row's adapter of x [M, K], of the pool's type -> [M, N] (or `out`, which may be y itself). index int32 or int64 [M]: a row whose
+    index is not of the pool (-1) is y's, bit for bit. Any order of rows: those of an adapter share one read of its matrices.
+
+    Differentiable in y, x, pool.a and pool.b. A training step that is to be captured calls `grads` itself: autograd's own streams and a
+    capture do not go together, and the process would end; so a call that records a gradient is refused there."""
+    if torch.is_grad_enabled() and (y.requires_grad or x.requires_grad or pool.a.requires_grad or pool.b.requires_grad):
+        if out is not None:
+            raise ValueError("adapters.add: no `out` where a gradient is recorded")
+        if y.is_cuda and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("adapters.add: a captured step takes adapters.grads (no gradient is recorded in a capture)")
+        return _Add.apply(y, x, pool.a, pool.b, pool, index)
+    return _add(y, x, pool, index, out)
+
+
+def grads(dy: torch.Tensor, x: torch.Tensor, pool: Adapters, index: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """The gradients of `add` given that of its result, dy [M, N]: (dx [M, K] of the pool's type, da FP32 [adapters, rank, K], db FP32 [adapters, rank,
+    N]). An adapter that no row has gets zeros, as do the rows behind an adapter's rank; y's gradient is dy itself. Sums over rows are in a
+    fixed order: the same call gives the same bits."""
+    what = "adapters.grads"
+    dyr, xr = _rows(dy, pool.out_features, pool, what), _rows(x, pool.in_features, pool, what)
+    m = dyr.shape[0]
+    if xr.shape[0] != m:
+        raise ValueError(f"{what}: as many rows of x as of dy")
+    ix = _index(index, m, what)
+    stream = _lib.stream_of(dyr, xr, ix, pool.a)
+    dx = xr.new_empty((m, xr.shape[1]))
+    if not m:
+        return dx, torch.zeros(pool.a.shape, dtype=torch.float32, device=xr.device), torch.zeros(pool.b.shape, dtype=torch.float32, device=xr.device)
+    da, db = xr.new_empty(pool.a.shape, dtype=torch.float32), xr.new_empty(pool.b.shape, dtype=torch.float32)
+    need = pool.room(m, 1)
+    ws = xr.new_empty(need, dtype=torch.uint8)
+    code = _lib.lib().hb_adapters_grads(pool.struct(), xr.data_ptr(), _stride(xr), dyr.data_ptr(), _stride(dyr), ix.data_ptr(), ix.element_size(), m, dx.data_ptr(), da.data_ptr(),
+                                        db.data_ptr(), ws.data_ptr(), need, stream)
+    if code:
+        _lib.check(code, what)
+    return dx, da, db

@@ -612,6 +612,30 @@ size_t hb_mxfp4_moe_pairs_workspace_bytes(const hb_mxfp4_experts* experts, int m
 int hb_mxfp4_moe(const hb_mxfp4_experts* experts, const void* x, const int32_t* ids, const float* weights, int m, int topk, int mode, void* out,
                  void* workspace, size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------ low-rank adapters of many requests beside a shared projection
+ *
+ * A pool of adapters of one projection [n, k]: adapter i adds scale_i b_i^T a_i to it. Both matrices lie rank by rank: a [adapters, rank, k] and
+ * b [adapters, rank, n], of `type` (HB_BF16 / HB_F16 / HB_F32). ranks (or NULL): adapter i has ranks[i] of the `rank` rows, what lies behind them is
+ * not read. scale: FP32 (NULL: 1). Up to 4096 adapters of a rank up to 256; k and n up to 2^22, m up to 2^24. Rows of x, y, dy and out are of `type`, a
+ * stride (in elements) apart; every array on its elements' boundary. index: int32 or int64 [m] (index_bytes 4 or 8), a row's adapter; a row whose
+ * index is outside 0 .. adapters - 1, or whose adapter has rank 0, has none. `workspace`: plain scratch on 16 bytes. No counterpart in the reference. */
+typedef struct {
+  const void* a;
+  const void* b;
+  const float* scale;
+  const int32_t* ranks;
+  int adapters, rank, k, n, type;
+} hb_adapters;
+size_t hb_adapters_workspace_bytes(const hb_adapters* adapters, int64_t m, int grads);
+
+/* out [m, n] = y + scale_i (x a_i^T) b_i, rounded once; rows without an adapter are y's. out may be y (of the same stride). */
+int hb_adapters_add(const hb_adapters* adapters, const void* x, int64_t x_stride, const void* y, int64_t y_stride, const void* index, int index_bytes, int64_t m,
+                    void* out, int64_t out_stride, void* workspace, size_t workspace_bytes, void* stream);
+/* Its gradients, given dy [m, n]: dx [m, k] of `type` (whole rows; zeros for rows without an adapter), da FP32 [adapters, rank, k] and db FP32
+ * [adapters, rank, n] (zeros for adapters that no row has, and behind an adapter's rank). y's gradient is dy. */
+int hb_adapters_grads(const hb_adapters* adapters, const void* x, int64_t x_stride, const void* dy, int64_t dy_stride, const void* index, int index_bytes, int64_t m,
+                      void* dx, float* da, float* db, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
