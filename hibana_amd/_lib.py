@@ -122,6 +122,8 @@ SIGNATURES = {
     "hb_adapters_workspace_bytes": (_Z, [_AD, _L, _I]),
     "hb_adapters_add": (_I, [_AD, _P, _L, _P, _L, _P, _I, _L, _P, _L, _P, _Z, _P]),
     "hb_adapters_grads": (_I, [_AD, _P, _L, _P, _L, _P, _I, _L, _P, _P, _P, _P, _Z, _P]),
+    "hb_route_experts": (_I, [_P, _I, _L, _I, _I, _I, _I, _P, _I, _I, _I, _F, _P, _I, _P, _P, _P]),
+    "hb_route_experts_grad": (_I, [_P, _P, _I, _L, _P, _I, _I, _I, _I, _I, _F, _P, _P]),
     "hb_mxfp4_linear": (_I, [_P, _P, _I, _L, _P, _L, _I, _P, _I, _P, _Z, _P]),
 }
 

@@ -2,10 +2,12 @@
 routing and combine ops of hibana/kernels/flashnext_fused.py that sit either side of the experts)."""
 from __future__ import annotations
 
+from dataclasses import dataclass
+
 import torch
 
 from hibana_amd import _lib
-from hibana_amd.kernels import mxfp4, w3
+from hibana_amd.kernels import adapters, mxfp4, w3
 from hibana_amd.weights.mxfp4 import Mxfp4Linear
 
 
@@ -168,6 +170,116 @@ def route_topk(logits: torch.Tensor, k: int, slots: torch.Tensor | None = None, 
         _lib.check(_lib.lib().hb_route_softmax_topk(_lib.ptr(lg), m, e, k, _lib.ptr(sl), steps, int(repeat), _lib.ptr(ids), _lib.ptr(w),
                                                     _lib.stream()), "route_topk")
     return ids, w
+
+
+SCORING = {"softmax": 0, "sigmoid": 1}  # HB_SOFTMAX, HB_SIGMOID
+
+
+@dataclass(frozen=True, eq=False)
+class Routing:
+    """How `route_experts` routes, for a layer that holds it (`MoeLayer(routing=...)`)."""
+    scoring: str = "softmax"
+    bias: torch.Tensor | None = None  # FP32 [E]
+    groups: int = 1
+    kept: int = 1
+    renormalize: bool = True
+    scale: float = 1.0
+
+    def __call__(self, logits: torch.Tensor, k: int, slots: torch.Tensor | None = None, steps: int = 1):
+        return route_experts(logits, k, self.scoring, bias=self.bias, groups=self.groups, kept=self.kept, renormalize=self.renormalize, scale=self.scale, slots=slots, steps=steps)
+
+
+def _route_logits(logits: torch.Tensor, scoring: str, what: str) -> torch.Tensor:
+    if logits.dtype not in mxfp4.TYPES or logits.ndim != 2 or scoring not in SCORING:
+        raise ValueError(f"{what}: BF16, FP16 or FP32 logits [M, E], scoring softmax or sigmoid")
+    return logits if logits.stride(1) == 1 and logits.stride(0) >= logits.shape[1] else logits.contiguous()
+
+
+def _route_experts(logits: torch.Tensor, k: int, scoring: str, bias, groups: int, kept: int, renormalize: bool, scale: float, slots, steps: int):
+    what = "route_experts"
+    lg = _route_logits(logits, scoring, what)
+    m, e = lg.shape
+    if not (1 <= e <= 1024 and 1 <= kept <= groups <= 64 and e % groups == 0 and 1 <= k <= min(63, kept * (e // groups))):
+        raise ValueError(f"{what}: up to 1024 experts in up to 64 groups of a size, k up to 63 and the experts of the kept groups")
+    if bias is not None and (bias.numel() != e or bias.ndim != 1 or not bias.is_floating_point()):
+        raise ValueError(f"{what}: a bias [E]")
+    if steps < 1 or m % steps or (slots is not None and slots.numel() < m // steps):
+        raise ValueError(f"{what}: whole requests of `steps` rows, a slot for every request")
+    bias32 = None if bias is None else bias.float().contiguous()
+    sl = None if slots is None else slots.to(torch.int32).contiguous()
+    stream = _lib.stream_of(lg, *(t for t in (bias32, sl) if t is not None))
+    ids, weights = lg.new_empty((m, k), dtype=torch.int32), lg.new_empty((m, k), dtype=torch.float32)
+    if m:
+        code = _lib.lib().hb_route_experts(lg.data_ptr(), mxfp4.TYPES[lg.dtype], max(lg.stride(0), e), m, e, k, SCORING[scoring], _lib.ptr(bias32), groups, kept, int(renormalize),
+                                           scale, _lib.ptr(sl), steps, ids.data_ptr(), weights.data_ptr(), stream)
+        if code:
+            _lib.check(code, what)
+    return ids, weights
+
+
+class _RouteExperts(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, k, scoring, renormalize, scale, *rest):
+        bias, groups, kept, slots, steps = rest
+        ids, weights = _route_experts(logits, k, scoring, bias, groups, kept, renormalize, scale, slots, steps)
+        ctx.save_for_backward(logits, ids)
+        ctx.rule = scoring, renormalize, scale
+        ctx.mark_non_differentiable(ids)
+        return ids, weights
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, _, dweights):
+        logits, ids = ctx.saved_tensors
+        scoring, renormalize, scale = ctx.rule
+        return (route_experts_grad(dweights, logits, ids, scoring, renormalize=renormalize, scale=scale), *[None] * 9)
+
+
+def route_experts(logits: torch.Tensor, k: int, scoring: str = "softmax", *, bias: torch.Tensor | None = None, groups: int = 1, kept: int = 1, renormalize: bool = True,
+                  scale: float = 1.0, slots: torch.Tensor | None = None, steps: int = 1):
+    """logits [M, E] (BF16, FP16 or FP32; E up to 1024) -> (int32 ids [M, k], FP32 weights [M, k]), largest choice first. Scores are the logits' softmax or
+    sigmoid; the choice goes by score + bias (FP32 [E], None: 0) among the experts of the `kept` groups (of `groups`, of consecutive experts) whose best
+    two sum highest; equal ones by the lower number. Without a bias the order is the logits' own, else (and between groups) that of the values in FP64. Weights are the plain scores, with
+    `renormalize` divided by their sum, times `scale`. An expert whose logit is -inf (a mask) or NaN is never chosen: slots left over, and all of a padded row's
+    (slots[r // steps] == 0), have id E, which the experts' kernels skip, and weight 0. A row that has a NaN logit has NaN weights.
+
+    Differentiable in the logits, through the weights (the bias only moves the choice). A captured training step calls `route_experts_grad`
+    itself: a call that records a gradient is refused in a capture, as in `adapters.add`. No counterpart in the reference."""
+    if logits.requires_grad and torch.is_grad_enabled():
+        if logits.is_cuda and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("route_experts: a captured step takes route_experts_grad (no gradient is recorded in a capture)")
+        return _RouteExperts.apply(logits, k, scoring, renormalize, scale, bias, groups, kept, slots, steps)
+    return _route_experts(logits, k, scoring, bias, groups, kept, renormalize, scale, slots, steps)
+
+
+def route_experts_grad(dweights: torch.Tensor, logits: torch.Tensor, ids: torch.Tensor, scoring: str = "softmax", *, renormalize: bool = True,
+                       scale: float = 1.0) -> torch.Tensor:
+    """The gradient of `route_experts`' logits [M, E], of their type, given that of its weights (FP32 [M, k]) and the ids it chose (int32 [M, k]; one
+    outside 0 .. E - 1 adds nothing)."""
+    what = "route_experts_grad"
+    lg = _route_logits(logits, scoring, what)
+    m, e = lg.shape
+    if ids.dtype != torch.int32 or ids.ndim != 2 or ids.shape[0] != m or dweights.dtype != torch.float32 or dweights.shape != ids.shape:
+        raise ValueError(f"{what}: dweights FP32 and ids int32, both [M, k]")
+    dw, chosen = dweights.contiguous(), ids.contiguous()
+    stream = _lib.stream_of(lg, dw, chosen)
+    out = lg.new_empty((m, e))
+    if m:
+        code = _lib.lib().hb_route_experts_grad(dw.data_ptr(), lg.data_ptr(), mxfp4.TYPES[lg.dtype], max(lg.stride(0), e), chosen.data_ptr(), m, e, chosen.shape[1],
+                                                SCORING[scoring], int(renormalize), scale, out.data_ptr(), stream)
+        if code:
+            _lib.check(code, what)
+    return out
+
+
+def adapted_linear(x: torch.Tensor, lin, pool: adapters.Adapters, index: torch.Tensor) -> torch.Tensor:
+    """A linear's rows (any of the `Linear` protocol: three-bit, NVFP4 or MXFP4 weights) with each row's own adapter of `pool` beside it
+    (`adapters.add` into the linear's fresh result): the serving form, without gradients."""
+    if pool.in_features != lin.in_features or pool.out_features != lin.out_features:
+        raise ValueError(f"adapted_linear: adapters of a projection [{pool.out_features}, {pool.in_features}] beside one [{lin.out_features}, {lin.in_features}]")
+    y = lin(x)
+    with torch.no_grad():
+        return adapters.add(y, x, pool, index, out=y)
 
 
 ROUTE_CANDIDATES = 20  # a row takes its experts from its 20 largest logits

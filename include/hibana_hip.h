@@ -636,6 +636,23 @@ int hb_adapters_add(const hb_adapters* adapters, const void* x, int64_t x_stride
 int hb_adapters_grads(const hb_adapters* adapters, const void* x, int64_t x_stride, const void* dy, int64_t dy_stride, const void* index, int index_bytes, int64_t m,
                       void* dx, float* da, float* db, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------ routing of rows to experts
+ *
+ * Scores s = softmax or sigmoid of the logits [m, e] (HB_BF16 / HB_F16 / HB_F32, rows `stride` elements apart), e up to 1024. The choice goes by c = s + bias
+ * (FP32 [e] or NULL): a group's score is the sum of its best two c (groups of e / groups consecutive experts, up to 64), and of the experts in the best `kept`
+ * groups the k largest c are chosen, largest first; equal ones by the lower number. Without a bias the order is the logits' own, else (and between groups) that
+ * of the values in FP64.
+ * weights = s, with `renorm` divided by the sum of the chosen experts' s, times scale. An expert whose logit is -inf or NaN (or whose bias is) is never chosen:
+ * slots left over, and those of padded rows (slots[r / steps] == 0; NULL: none), have id e and weight 0. A row that has a NaN logit has NaN weights. k up to 63 and the
+ * experts of `kept` groups; at most sixteen experts a lane where a group has the largest power of two of lanes that 64 / groups holds (any e without groups,
+ * or with a power of two of them). No counterpart in the reference (its routing rules are hb_route_softmax_topk's and hb_route_sigmoid_topk's). */
+enum { HB_SOFTMAX = 0, HB_SIGMOID = 1 };
+int hb_route_experts(const void* logits, int type, int64_t stride, int m, int e, int k, int scoring, const float* bias, int groups, int kept, int renorm,
+                     float scale, const int32_t* slots, int steps, int32_t* ids, float* weights, void* stream);
+/* The logits' gradient [m, e] of their type (on 16 bytes), given the weights' (FP32 [m, k]) and the ids that were chosen (an id outside 0 .. e - 1 adds nothing). */
+int hb_route_experts_grad(const float* dweights, const void* logits, int type, int64_t stride, const int32_t* ids, int m, int e, int k, int scoring, int renorm,
+                          float scale, void* dlogits, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
