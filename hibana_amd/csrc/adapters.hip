@@ -12,15 +12,16 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "common.hpp"
+#include "stream_common.hpp"
 
 namespace hb {
 
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8_t;
 typedef uint32_t u32x4_loose __attribute__((ext_vector_type(4), aligned(2)));  // sixteen bytes at any element: rows of odd length
 
+constexpr int AD_SPLITS = 8;       // of the long axis, at most, in a call of few rows
 constexpr int AD_SELF_ROWS = 256;  // rows up to which a workgroup finds its tile from the index itself
-constexpr int AD_CHUNK = 128;      // rows of an outer product's step: 32 a wavefront
+constexpr int AD_TILE = 32;        // rows of a planned call's tile: the places of a matrix instruction's contraction in an outer product
 constexpr int AD_MOST = 4096;      // adapters
 constexpr int AD_RANK = 256;
 constexpr int AD_MAX_ROWS = 1 << 24;
@@ -80,6 +81,30 @@ __device__ __forceinline__ void ad_store(char* at, const u32x4_t& v, int64_t lef
   }
 }
 
+// A lane's sixteen bytes of a row of n elements, of which `first` is the lane's first: behind the row's end its last sixteen bytes, so that no load is behind a
+// branch (the compiler waits for all that is under way where it does not know how many loads are). TINY: rows shorter than that, element by element.
+template <int KIND, bool TINY>
+__device__ __forceinline__ u32x4_t ad_take(const char* row, int first, int n) {
+  if constexpr (TINY) return ad_load<KIND>(row + first * AdType<KIND>::SIZE, n - first);
+  return *reinterpret_cast<const u32x4_loose*>(row + (int64_t)min(first, n - AD_VEC<KIND>) * AdType<KIND>::SIZE);
+}
+// The elements of the row that `ad_take` was asked for, and no others.
+template <int KIND, bool TINY>
+__device__ __forceinline__ void ad_put(char* row, const u32x4_t& v, int first, int n) {
+  if (first + AD_VEC<KIND> <= n) {
+    *reinterpret_cast<u32x4_loose*>(row + (int64_t)first * AdType<KIND>::SIZE) = v;
+    return;
+  }
+  const int from = TINY ? first : n - AD_VEC<KIND>;
+#pragma unroll
+  for (int j = 0; j < AD_VEC<KIND>; j++) {
+    if (from + j >= first && from + j < n) {
+      if constexpr (AdType<KIND>::SIZE == 4) reinterpret_cast<uint32_t*>(row)[from + j] = v[j];
+      else reinterpret_cast<uint16_t*>(row)[from + j] = (uint16_t)ad_elem<KIND>(v, j);
+    }
+  }
+}
+
 // acc += the 16 x 16 product of two operands whose lanes hold sixteen bytes along the contraction: 32 places of 16-bit types in one
 // instruction, 16 of FP32 in four (instruction i contracts element i of every lane: any order serves that both operands have).
 template <int KIND>
@@ -95,7 +120,7 @@ __device__ __forceinline__ f32x4_t ad_mma(const u32x4_t& a, const u32x4_t& b, f3
 
 // ------------------------------------------------------------------------------------------------ rows by adapter
 
-// Classes 0 .. adapters - 1 are the adapters, `adapters` the rows without one (an index outside the pool, an adapter of rank 0).
+// Classes 0 .. adapters - 1 are the adapters, `adapters` the rows without one (an index outside the pool).
 struct AdIndex {
   const void* index;
   const int32_t* ranks;
@@ -107,63 +132,88 @@ __device__ __forceinline__ int ad_rank(const AdIndex& p, int c) {
 }
 __device__ __forceinline__ int ad_class(const AdIndex& p, int row) {
   const int64_t i = p.wide ? reinterpret_cast<const int64_t*>(p.index)[row] : reinterpret_cast<const int32_t*>(p.index)[row];
-  if (i < 0 || i >= p.adapters) return p.adapters;
-  return p.ranks && p.ranks[i] <= 0 ? p.adapters : (int)i;
+  return i < 0 || i >= p.adapters ? p.adapters : (int)i;
 }
 
-// The plan: int32 arrays [classes + 1] of where a class's rows, its tiles of two heights, its units (runs of `unit` rows, an outer
-// product's share of the work) and its slots (partial sums: the units of classes that have more than one) begin, then the rows in order.
+// The plan: int32 arrays [classes + 1] of where a class's rows, its tiles, its units (runs of `unit` rows, an outer product's share of the work) and
+// its slots (partial sums: the units of classes that have more than one) begin, then the rows in order.
 struct AdPlan {
   int32_t* at;
   int classes;
   __host__ __device__ int32_t* rows() const { return at; }
-  __host__ __device__ int32_t* tiles(int which) const { return at + (1 + which) * (classes + 1); }
-  __host__ __device__ int32_t* units() const { return at + 3 * (classes + 1); }
-  __host__ __device__ int32_t* slots() const { return at + 4 * (classes + 1); }
-  __host__ __device__ int32_t* order() const { return at + 5 * (classes + 1); }
-  static size_t ints(int classes, int64_t m) { return 5 * ((size_t)classes + 1) + m; }
+  __host__ __device__ int32_t* tiles() const { return at + (classes + 1); }
+  __host__ __device__ int32_t* units() const { return at + 2 * (classes + 1); }
+  __host__ __device__ int32_t* slots() const { return at + 3 * (classes + 1); }
+  __host__ __device__ int32_t* order() const { return at + 4 * (classes + 1); }
+  static size_t ints(int classes, int64_t m) { return 4 * ((size_t)classes + 1) + m; }
 };
 
 struct AdPlanParams {
   AdIndex in;
   AdPlan plan;
-  int height[2];  // rows of the two kinds of tile
   int unit;
   int segments;   // wavefronts that count and place rows, each those of one stretch; segments * classes counters in LDS
+  int32_t* tickets;  // the shrink's arrival counters, to be cleared
+  int64_t clear;
 };
 
-// One workgroup: a stable counting sort (rows of a class stay in ascending order, so sums over them are the same every time).
+// One workgroup: a stable counting sort (rows of a class stay in ascending order, so sums over them are the same every time). HELD: up to AD_HELD rows, whose
+// classes and places among their stretch's rows of the class stay in LDS between the two passes; more are read and counted again. Both loops are short on purpose: what
+// this kernel takes is latency, and unrolled over registers its instructions' own first loads were half of it (8192 rows 12.6 us).
+constexpr int AD_HELD = 8192;
+constexpr int AD_COUNTERS = 8000;  // (with the rows held within 64 KB)
+template <bool HELD>
 __global__ __launch_bounds__(1024) void ad_plan_kernel(AdPlanParams p) {
-  extern __shared__ int32_t counters[];  // [segment][class]
-  __shared__ int32_t carry[16][5];
+  extern __shared__ int32_t counters[];  // [segment][class], then (HELD) class | place << 16 of every row, the place among its stretch's rows
+  __shared__ int32_t carry[16][4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, classes = p.plan.classes, m = p.in.m;
+  const int stretch = ((m + p.segments - 1) / p.segments + 63) / 64 * 64;
+  const int from = wave < p.segments ? (int)min((int64_t)wave * stretch, (int64_t)m) : m, upto = min(from + stretch, m);
+  int32_t* held = counters + p.segments * classes;
+  for (int64_t i = threadIdx.x; i < p.clear; i += 1024) p.tickets[i] = 0;
   for (int i = threadIdx.x; i < p.segments * classes; i += 1024) counters[i] = 0;
   __syncthreads();
-  const int stretch = ((m + p.segments - 1) / p.segments + 63) / 64 * 64;
-  const int from = (int)min((int64_t)wave * stretch, (int64_t)m), upto = min(from + stretch, m);
-  volatile int32_t* mine = counters + wave * classes;
-  if (wave < p.segments)
-    for (int r = from + lane; r < upto; r += 64) atomicAdd(const_cast<int32_t*>(mine) + ad_class(p.in, r), 1);
+  volatile int32_t* mine = counters + wave * classes;  // (of a wavefront that has rows)
+  // the lanes that have a class among them, one class after another; each lane's place among its class
+  auto places = [&](int c) {
+    int place = 0;
+    uint64_t left = __ballot(c >= 0);
+    while (left) {
+      const int v = __builtin_amdgcn_readlane(c, __builtin_ctzll(left));
+      const uint64_t same = __ballot(c == v);
+      const int have = mine[v];
+      if (c == v) place = have + __popcll(same & ((1ull << lane) - 1ull));
+      if (lane == 0) mine[v] = have + __popcll(same);
+      left &= ~same;
+    }
+    return place;
+  };
+  int ahead = from + lane < upto ? ad_class(p.in, from + lane) : -1;
+  for (int r0 = from; r0 < upto; r0 += 64) {
+    const int c = ahead, r = r0 + lane;
+    if (r0 + 64 < upto) ahead = r + 64 < upto ? ad_class(p.in, r + 64) : -1;
+    const int place = places(c);
+    if (HELD && r < upto) held[r] = c | place << 16;
+  }
   __syncthreads();
   // each thread a run of classes: counts over the segments, then prefix sums over the threads
   const int per = (classes + 1023) / 1024, c0 = min((int)threadIdx.x * per, classes), c1 = min(c0 + per, classes);
-  int sum[5] = {0, 0, 0, 0, 0};
-  auto add = [&](int (&to)[5], int c, int rows) {
-    const int units = c < p.in.adapters ? (rows + p.unit - 1) / p.unit : 0;
-    to[0] += rows;
-    to[1] += (rows + p.height[0] - 1) / p.height[0];
-    to[2] += (rows + p.height[1] - 1) / p.height[1];
-    to[3] += units;
-    to[4] += units > 1 ? units : 0;
+  int sum[4] = {0, 0, 0, 0};
+  auto add = [&](int (&to)[4], int c, int n) {
+    const int units = c < p.in.adapters ? (n + p.unit - 1) / p.unit : 0;
+    to[0] += n;
+    to[1] += (n + AD_TILE - 1) / AD_TILE;
+    to[2] += units;
+    to[3] += units > 1 ? units : 0;
   };
   for (int c = c0; c < c1; c++) {
-    int rows = 0;
-    for (int s = 0; s < p.segments; s++) rows += counters[s * classes + c];
-    add(sum, c, rows);
+    int n = 0;
+    for (int s = 0; s < p.segments; s++) n += counters[s * classes + c];
+    add(sum, c, n);
   }
-  int before[5];
+  int before[4];
 #pragma unroll
-  for (int j = 0; j < 5; j++) {
+  for (int j = 0; j < 4; j++) {
     int x = sum[j];
     for (int d = 1; d < 64; d <<= 1) {
       const int up = __shfl_up(x, d);
@@ -173,178 +223,102 @@ __global__ __launch_bounds__(1024) void ad_plan_kernel(AdPlanParams p) {
     if (lane == 63) carry[wave][j] = x;
   }
   __syncthreads();
-  for (int w = 0; w < wave; w++)
+  if (c0 < c1)
+    for (int w = 0; w < wave; w++)
 #pragma unroll
-    for (int j = 0; j < 5; j++) before[j] += carry[w][j];
-  int32_t* out[5] = {p.plan.rows(), p.plan.tiles(0), p.plan.tiles(1), p.plan.units(), p.plan.slots()};
+      for (int j = 0; j < 4; j++) before[j] += carry[w][j];
+  int32_t* out[4] = {p.plan.rows(), p.plan.tiles(), p.plan.units(), p.plan.slots()};
   for (int c = c0; c < c1; c++) {
-    int at = before[0], rows = 0;
+    int n = 0;
     for (int s = 0; s < p.segments; s++) {
-      const int n = counters[s * classes + c];
-      counters[s * classes + c] = at + rows;
-      rows += n;
+      const int here = counters[s * classes + c];
+      counters[s * classes + c] = before[0] + n;
+      n += here;
     }
 #pragma unroll
-    for (int j = 0; j < 5; j++) out[j][c] = before[j];
-    add(before, c, rows);
+    for (int j = 0; j < 4; j++) out[j][c] = before[j];
+    add(before, c, n);
     if (c == classes - 1)
 #pragma unroll
-      for (int j = 0; j < 5; j++) out[j][classes] = before[j];
+      for (int j = 0; j < 4; j++) out[j][classes] = before[j];
   }
   __syncthreads();
-  if (wave < p.segments) {
-    int32_t* order = p.plan.order();
-    for (int r0 = from; r0 < upto; r0 += 64) {
-      const int r = r0 + lane, c = r < upto ? ad_class(p.in, r) : -1;
-      uint64_t left = __ballot(c >= 0);
-      while (left) {
-        const int v = __builtin_amdgcn_readlane(c, __builtin_ctzll(left));
-        const uint64_t same = __ballot(c == v);
-        const int base = mine[v];
-        if (c == v) order[base + __popcll(same & ((1ull << lane) - 1ull))] = r;
-        if (lane == 0) mine[v] = base + __popcll(same);
-        left &= ~same;
-      }
+  int32_t* order = p.plan.order();
+  for (int r0 = from; r0 < upto; r0 += 64) {
+    const int r = r0 + lane;
+    if (HELD) {
+      if (r < upto) order[mine[held[r] & 0xffff] + (held[r] >> 16)] = r;
+    } else {
+      const int c = r < upto ? ad_class(p.in, r) : -1, place = places(c);
+      if (c >= 0) order[place] = r;
     }
   }
 }
 
-// The class that place t of an ascending array [classes + 1] of first places is in (by every wavefront for itself).
-__device__ __forceinline__ int ad_find(const int32_t* first, int classes, int t) {
-  const int lane = threadIdx.x & 63;
-  int c = -1;
+// The class whose tiles (or units), which begin at first[class], number t is of, or `classes` if there is none; its first one and its first row and the next class's
+// (one load each for up to 63 classes, side by side). By every wavefront for itself.
+struct AdPlace {
+  int c, first, row, next_row;
+};
+__device__ __forceinline__ AdPlace ad_find(const AdPlan& plan, const int32_t* first, int t) {
+  const int lane = threadIdx.x & 63, classes = plan.classes;
+  AdPlace at{-1, 0, 0, 0};
   for (int i = 0; i <= classes; i += 64) {
-    const int n = __popcll(__ballot(i + lane <= classes && first[min(i + lane, classes)] <= t));
-    c += n;
-    if (n < 64) break;
+    const int mine = first[min(i + lane, classes)], row = plan.rows()[min(i + lane, classes)];
+    const int n = __popcll(__ballot(i + lane <= classes && mine <= t));
+    if (n) {
+      at.first = __builtin_amdgcn_readlane(mine, n - 1);
+      at.row = __builtin_amdgcn_readlane(row, n - 1);
+    }
+    at.c += n;
+    if (n < 64) {
+      if (n) at.next_row = __builtin_amdgcn_readlane(row, n);
+      break;
+    }
+    at.next_row = plan.rows()[min(i + 64, classes)];
   }
-  return c;
+  return at;
 }
 
-// Tile t: its class, its rows' numbers in LDS and how many they are (0: no such tile). Without a plan, t is a row: a tile begins at every
-// T-th row of a class.
-template <int T>
-__device__ __forceinline__ int ad_tile(const AdIndex& p, const AdPlan& plan, int which, int t, int32_t* rows, int& c) {
+// A plan's tile t: its class, its rows' first place in the order and how many they are (0: no such tile).
+__device__ __forceinline__ int ad_tile(const AdPlan& plan, int t, int& c, int& start) {
+  const AdPlace at = ad_find(plan, plan.tiles(), t);
+  c = at.c;
+  if (c >= plan.classes) return 0;
+  start = at.row + (t - at.first) * AD_TILE;
+  return min(AD_TILE, at.next_row - start);
+}
+
+// Few rows, no plan: a tile of up to sixteen begins at every sixteenth row of a class, and every wavefront finds its own from the index itself. Lane l gets
+// the number of the tile's row l % 16 (behind the last one the first again); 0 rows: none begins at row t.
+__device__ __forceinline__ int ad_tile_at(const AdIndex& p, int t, int& c, int& row) {
   const int lane = threadIdx.x & 63;
-  int count;
-  if (plan.at) {
-    if (t >= plan.tiles(which)[plan.classes]) return 0;
-    c = ad_find(plan.tiles(which), plan.classes, t);
-    const int start = plan.rows()[c] + (t - plan.tiles(which)[c]) * T;
-    count = min(T, plan.rows()[c + 1] - start);
-    if (threadIdx.x < T) rows[threadIdx.x] = plan.order()[start + min((int)threadIdx.x, count - 1)];
-  } else {
-    c = ad_class(p, t);
-    uint64_t same[AD_SELF_ROWS / 64];
-    int ahead = 0, all = 0;
+  int mine[AD_SELF_ROWS / 64];
 #pragma unroll
-    for (int j = 0; j < AD_SELF_ROWS / 64; j++) {
-      same[j] = 0;
-      if (64 * j < p.m) same[j] = __ballot(64 * j + lane < p.m && ad_class(p, min(64 * j + lane, p.m - 1)) == c);
-      if (64 * j + 63 < t) ahead += __popcll(same[j]);
-      else if (64 * j <= t) ahead += __popcll(same[j] & ((1ull << (t - 64 * j)) - 1ull));
-      all += __popcll(same[j]);
-    }
-    if (ahead % T) return 0;
-    count = min(T, all - ahead);
-    int at = 0;
+  for (int j = 0; j < AD_SELF_ROWS / 64; j++) mine[j] = 64 * j < p.m ? ad_class(p, min(64 * j + lane, p.m - 1)) : -1;
+  c = __builtin_amdgcn_readfirstlane(ad_class(p, t));
+  uint64_t same[AD_SELF_ROWS / 64];
+  int ahead = 0, all = 0;
 #pragma unroll
-    for (int j = 0; j < AD_SELF_ROWS / 64; j++) {
-      const int place = at + __popcll(same[j] & ((1ull << lane) - 1ull)) - ahead;
-      if ((same[j] >> lane & 1) && place >= 0 && place < T) rows[place] = 64 * j + lane;  // (every wavefront the same)
-      at += __popcll(same[j]);
-    }
-    if ((int)threadIdx.x >= count && threadIdx.x < T) rows[threadIdx.x] = t;  // places behind the last row repeat the first: t itself
+  for (int j = 0; j < AD_SELF_ROWS / 64; j++) {
+    same[j] = __ballot(64 * j + lane < p.m && mine[j] == c);
+    if (64 * j + 63 < t) ahead += __popcll(same[j]);
+    else if (64 * j <= t) ahead += __popcll(same[j] & ((1ull << (t - 64 * j)) - 1ull));
+    all += __popcll(same[j]);
   }
-  __syncthreads();
-  return count;
-}
-
-// ------------------------------------------------------------------------------------------------ shrink
-
-struct AdShrinkJob {
-  const char* v;      // rows, `stride` bytes apart
-  int64_t stride;
-  const char* w;      // [adapters, rank, length]
-  int length, share;  // units of 128 bytes a split
-  float* sums;        // [splits, m, rank]
-};
-struct AdShrink {
-  AdIndex in;
-  AdPlan plan;
-  AdShrinkJob job[2];
-  int chunks;  // of RT x 16 ranks
-};
-
-// A workgroup: a tile's rows times RT x 16 ranks over one split of the long axis, the four wavefronts taking units of 128 bytes in turn (a
-// whole cache line of every row) and joining their sums in LDS.
-template <int KIND, int TM, int RT>
-__global__ __launch_bounds__(256) void ad_shrink_kernel(AdShrink p) {
-  constexpr int VEC = AD_VEC<KIND>, SIZE = AdType<KIND>::SIZE, UNIT = 128 / SIZE;
-  __shared__ int32_t rows[16 * TM];
-  __shared__ f32x4_t part[4][TM * RT][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, group = lane >> 4, col = lane & 15;
-  int c;
-  const int count = ad_tile<16 * TM>(p.in, p.plan, 0, blockIdx.x, rows, c);
-  if (count == 0 || c >= p.in.adapters) return;
-  const AdShrinkJob& job = p.job[blockIdx.z / p.chunks];
-  const int rank = ad_rank(p.in, c), r0 = (blockIdx.z % p.chunks) * 16 * RT;
-  if (r0 >= rank) return;
-  const int units = (job.length + UNIT - 1) / UNIT, whole = job.length / UNIT, u0 = blockIdx.y * job.share, u1 = min(u0 + job.share, units);
-  const char* x[TM];
-  const char* w[RT];
+  if (ahead % 16) return 0;
+  row = t;
+  int at = 0;
 #pragma unroll
-  for (int i = 0; i < TM; i++) x[i] = job.v + rows[16 * i + col] * job.stride + group * 16;
-#pragma unroll
-  for (int i = 0; i < RT; i++) w[i] = job.w + ((int64_t)c * p.in.rank + min(r0 + 16 * i + col, rank - 1)) * job.length * SIZE + group * 16;  // (ranks behind the last: nobody reads the sums)
-  f32x4_t acc[TM][RT] = {};
-  for (int u = u0 + wave; u < min(u1, whole); u += 4) {
-    u32x4_t xv[TM][2], wv[RT][2];
-#pragma unroll
-    for (int h = 0; h < 2; h++) {
-#pragma unroll
-      for (int i = 0; i < RT; i++) wv[i][h] = *reinterpret_cast<const u32x4_loose*>(w[i] + (int64_t)u * 128 + 64 * h);
-#pragma unroll
-      for (int i = 0; i < TM; i++) xv[i][h] = *reinterpret_cast<const u32x4_loose*>(x[i] + (int64_t)u * 128 + 64 * h);
-    }
-#pragma unroll
-    for (int h = 0; h < 2; h++)
-#pragma unroll
-      for (int i = 0; i < TM; i++)
-#pragma unroll
-        for (int j = 0; j < RT; j++) acc[i][j] = ad_mma<KIND>(xv[i][h], wv[j][h], acc[i][j]);
+  for (int j = 0; j < AD_SELF_ROWS / 64; j++) {  // the rows hand their numbers to the lanes of their places, all others theirs to lanes that nobody reads
+    const int place = at + __popcll(same[j] & ((1ull << lane) - 1ull)) - ahead;
+    const bool take = (same[j] >> lane & 1) && place >= 0 && place < 16;
+    const int got = __builtin_amdgcn_ds_permute(4 * (take ? place : 16 + (lane & 31)), 64 * j + lane + 1);  // (0: nothing came)
+    if (lane < 16 && got) row = got - 1;
+    at += __popcll(same[j]);
   }
-  if (u0 <= whole && u1 > whole && (whole - u0) % 4 == wave) {  // the row's last, cut unit, by the wavefront whose turn it is
-#pragma unroll
-    for (int h = 0; h < 2; h++) {
-      const int64_t left = job.length - ((int64_t)whole * UNIT + h * (UNIT / 2) + group * VEC);
-      u32x4_t wv[RT];
-#pragma unroll
-      for (int i = 0; i < RT; i++) wv[i] = ad_load<KIND>(w[i] + (int64_t)whole * 128 + 64 * h, left);
-#pragma unroll
-      for (int i = 0; i < TM; i++) {
-        const u32x4_t xv = ad_load<KIND>(x[i] + (int64_t)whole * 128 + 64 * h, left);
-#pragma unroll
-        for (int j = 0; j < RT; j++) acc[i][j] = ad_mma<KIND>(xv, wv[j], acc[i][j]);
-      }
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < TM; i++)
-#pragma unroll
-    for (int j = 0; j < RT; j++) part[wave][i * RT + j][lane] = acc[i][j];
-  __syncthreads();
-  float* sums = job.sums + (int64_t)blockIdx.y * p.in.m * p.in.rank;
-  for (int t = wave; t < TM * RT; t += 4) {
-    const f32x4_t s = part[0][t][lane] + part[1][t][lane] + part[2][t][lane] + part[3][t][lane];
-    const int r = r0 + 16 * (t % RT) + col;
-    if (r >= rank) continue;
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const int place = 16 * (t / RT) + 4 * group + i;
-      if (place < count) sums[(int64_t)rows[place] * p.in.rank + r] = s[i];
-    }
-  }
+  row = __shfl(row, lane & 15);
+  return min(16, all - ahead);
 }
 
 // ------------------------------------------------------------------------------------------------ FP32 sums as matrix operands
@@ -374,303 +348,648 @@ __device__ __forceinline__ void ad_cut(float v, uint16_t (&part)[PARTS]) {
   }
 }
 
-// The power of two that brings a largest magnitude to 2^14 .. 2^15, and its inverse.
-__device__ __forceinline__ int ad_exponent(float most) { return most > 0.f ? max((int)(__float_as_uint(most) >> 23) - 127, -100) - 14 : -100; }
+// The power of two that brings a largest magnitude to 2^14 .. 2^15 (its exponent, -100 or more).
+__device__ __forceinline__ int ad_exponent(float most) { return most > 0.f ? max((int)(__float_as_uint(most) >> 23) - 127, -86) - 14 : -100; }
 __device__ __forceinline__ float ad_pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
-// Lane's operands along the contraction from eight rows of sixteen bytes: element j of the eight, for each j.
+// FP16 parts times 2^e, e <= 0 (below -40 they are too small to count).
+__device__ __forceinline__ u32x4_t ad_lower(const u32x4_t& v, int e) {
+  const _Float16 by = (_Float16)ad_pow2(max(e, -24)), more = (_Float16)ad_pow2(max(min(e + 24, 0), -24));
+  f16x8_t f = __builtin_bit_cast(f16x8_t, v);
+  f = f * by * more;
+  return __builtin_bit_cast(u32x4_t, f);
+}
+
+// Lane's operand j along the contraction from eight rows of sixteen bytes: their elements j.
+__device__ __forceinline__ u32x4_t ad_turn(const u32x4_t (&v)[8], int j) {
+  u32x4_t out;
+#pragma unroll
+  for (int q = 0; q < 4; q++) out[q] = __builtin_amdgcn_perm(v[2 * q + 1][j >> 1], v[2 * q][j >> 1], j & 1 ? 0x07060302u : 0x05040100u);
+  return out;
+}
+
+// ------------------------------------------------------------------------------------------------ shrink
+
+// acc[i][j] += units u0, u0 + step, .. below u1 of TM x 16 rows times RT x 16 rows of a matrix; the last, cut unit of a row is taken if it is among them.
+// Units of 128 bytes (a whole cache line of every row), DEPTH of them under way.
+template <int KIND, int TM, int RT, int LIMIT = RT>
+__device__ __forceinline__ void ad_shrink_units(const char* const (&x)[TM], const char* const (&w)[LIMIT], int length, int u0, int u1, int step, f32x4_t (&acc)[TM][LIMIT]) {
+  constexpr int VEC = AD_VEC<KIND>, SIZE = AdType<KIND>::SIZE, UNIT = 128 / SIZE, DEPTH = TM + RT <= 3 ? 4 : TM + RT <= 4 ? 3 : 2;
+  const int whole = length / UNIT, end = min(u1, whole), group = (threadIdx.x & 63) >> 4;
+  u32x4_t xv[DEPTH][TM][2], wv[DEPTH][RT][2];
+  auto load = [&](int d, int u) {
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+#pragma unroll
+      for (int i = 0; i < TM; i++) xv[d][i][h] = *reinterpret_cast<const u32x4_loose*>(x[i] + (int64_t)u * 128 + 64 * h);
+#pragma unroll
+      for (int i = 0; i < RT; i++) wv[d][i][h] = *reinterpret_cast<const u32x4_loose*>(w[i] + (int64_t)u * 128 + 64 * h);
+    }
+  };
+  auto products = [&](int d) {
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+#pragma unroll
+      for (int i = 0; i < TM; i++)
+#pragma unroll
+        for (int j = 0; j < RT; j++) acc[i][j] = ad_mma<KIND>(xv[d][i][h], wv[d][j][h], acc[i][j]);
+  };
+  // (no load behind a branch while others are to stay under way: see ad_take)
+  int u = u0, left = u0 < end ? (end - u0 + step - 1) / step : 0;
+  if (left >= DEPTH) {
+#pragma unroll
+    for (int d = 0; d < DEPTH; d++) load(d, u + d * step);
+    for (; left >= 2 * DEPTH; left -= DEPTH) {
+#pragma unroll
+      for (int d = 0; d < DEPTH; d++) {
+        products(d);
+        load(d, u + (d + DEPTH) * step);
+      }
+      u += DEPTH * step;
+    }
+#pragma unroll
+    for (int d = 0; d < DEPTH; d++) products(d);
+    u += DEPTH * step;
+    left -= DEPTH;
+  }
+#pragma unroll
+  for (int d = 0; d < DEPTH - 1; d++)
+    if (d < left) load(d, u + d * step);
+#pragma unroll
+  for (int d = 0; d < DEPTH - 1; d++)
+    if (d < left) products(d);
+  u += left * step;
+  if (u == whole && u < u1) {
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      const int64_t left = length - ((int64_t)whole * UNIT + h * (UNIT / 2) + group * VEC);
+#pragma unroll
+      for (int i = 0; i < RT; i++) wv[0][i][h] = ad_load<KIND>(w[i] + (int64_t)whole * 128 + 64 * h, left);
+#pragma unroll
+      for (int i = 0; i < TM; i++) xv[0][i][h] = ad_load<KIND>(x[i] + (int64_t)whole * 128 + 64 * h, left);
+    }
+    products(0);
+  }
+}
+
+// Few rows: a workgroup's four wavefronts share one split of the long axis of a tile's rows and sixteen ranks, and join their sums in LDS; the splits' sums
+// are joined by their readers.
+struct AdFew {
+  AdIndex in;
+  const char* x;
+  int64_t x_stride;    // bytes
+  const char* a;       // [adapters, rank, k]
+  int k, n, splits, share;  // share: units of 128 bytes a split
+  float* sums;         // [splits, m, rank]
+  const float* scale;
+  const char* b;       // [adapters, rank, n]
+  const char* y;
+  int64_t y_stride;
+  char* out;
+  int64_t out_stride;
+  int padded;          // the rank in LDS, a multiple of 32
+};
+
 template <int KIND>
-__device__ __forceinline__ void ad_turn(const u32x4_t (&v)[8], u32x4_t (&out)[AD_VEC<KIND>]) {
-  if constexpr (AdType<KIND>::SIZE == 2) {
+__global__ __launch_bounds__(256) void ad_shrink_few_kernel(AdFew p) {
+  constexpr int SIZE = AdType<KIND>::SIZE, UNIT = 128 / SIZE;
+  __shared__ f32x4_t part[4][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, group = lane >> 4, col = lane & 15;
+  int c, row;
+  const int count = ad_tile_at(p.in, blockIdx.x, c, row);
+  if (count == 0 || c >= p.in.adapters) return;
+  const int rank = ad_rank(p.in, c), r0 = blockIdx.z * 16;
+  if (r0 >= rank) return;
+  const char* const x[1] = {p.x + row * p.x_stride + group * 16};
+  const char* const w[1] = {p.a + ((int64_t)c * p.in.rank + min(r0 + col, rank - 1)) * p.k * SIZE + group * 16};  // (ranks behind the last: nobody reads the sums)
+  const int u0 = blockIdx.y * p.share;
+  f32x4_t acc[1][1] = {};
+  ad_shrink_units<KIND, 1, 1>(x, w, p.k, u0 + wave, min(u0 + p.share, (p.k + UNIT - 1) / UNIT), 4, acc);
+  part[wave][lane] = acc[0][0];
+  __syncthreads();
+  const int place = 4 * group + wave;  // thread: row 4 group + wave, rank r0 + col
+  const int to = __shfl(row, place);
+  if (place < count && r0 + col < rank) {
+    float s = 0.f;
 #pragma unroll
-    for (int j = 0; j < 8; j++)
+    for (int w4 = 0; w4 < 4; w4++) s += reinterpret_cast<const float*>(&part[w4][lane])[wave];
+    p.sums[((int64_t)blockIdx.y * p.in.m + to) * p.in.rank + r0 + col] = s;
+  }
+}
+
+// A plan's tiles: a workgroup has one split of the long axis for a tile's 32 rows and RT x 16 ranks, its wavefronts taking units in turn. Of a tile's workgroups the last one to
+// arrive adds the splits' sums up, in their order, and leaves them, scaled, as the operands that the second products take: by rows (for the expansion), and with
+// rows and ranks changed over (for the outer product). The splits are there to keep every compute unit at it: one alone reads some 17 GB/s, and the 64 tiles of
+// 2048 rows, a workgroup each, took 24 us for what 256 do in ..
+struct AdShrinkJob {
+  const char* v;      // rows, `stride` bytes apart
+  int64_t stride;
+  const char* w;      // [adapters, rank, length]
+  int length, splits, share;  // units of 128 bytes a split
+  float* parts;       // [tile][chunk][split][row][rank] of sums (several splits), and an arrival counter [tile][chunk]
+  int32_t* tickets;
+  char* by_row;       // [tile][32 ranks][part][row][rank], or null
+  char* by_rank;      // [tile][16 ranks][part][rank][row], or null
+  int8_t* row_power;  // FP16: the exponents that the values are in, [tile][16 ranks][row] ...
+  int8_t* rank_power; // ... and [tile][16 ranks]
+};
+struct AdShrink {
+  AdIndex in;
+  AdPlan plan;
+  AdShrinkJob job[2];
+  const float* scale;
+  int chunks;  // of RT x 16 ranks
+};
+constexpr int AD_WAVES = 4;
+__host__ __device__ constexpr int ad_sixteens(int rank) { return (rank + 15) / 16; }
+__host__ __device__ constexpr int ad_thirties(int rank) { return (rank + 31) / 32; }
+
+template <int KIND, int RT>
+__global__ __launch_bounds__(64 * AD_WAVES) void ad_shrink_kernel(AdShrink p) {
+  constexpr int SIZE = AdType<KIND>::SIZE, UNIT = 128 / SIZE, PARTS = AdType<KIND>::PARTS, OUTER = AdType<KIND>::OUTER, WIDE = 16 * RT, PITCH = WIDE + 1;
+  constexpr int JOINED = AD_WAVES / 2 * 2 * RT * 64 * 16, SUMS = 32 * PITCH * 4;
+  __shared__ __align__(16) char shared[JOINED > SUMS ? JOINED : SUMS];
+  __shared__ int32_t row_power[AD_TILE * RT], rank_power[RT], last;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, group = lane >> 4, col = lane & 15, tile = blockIdx.x;
+  int c, start;
+  const int count = ad_tile(p.plan, tile, c, start);
+  if (count == 0 || c >= p.in.adapters) return;
+  const int chunk = blockIdx.y % p.chunks, of_both = blockIdx.y / p.chunks, second = of_both >= p.job[0].splits, split = second ? of_both - p.job[0].splits : of_both;
+  const AdShrinkJob& job = p.job[second];
+  const int rank = ad_rank(p.in, c), r0 = chunk * WIDE;
+  if (r0 >= rank) return;
+  const float scale = p.scale ? p.scale[c] : 1.0f;
+  const char* x[2];
+  const char* w[RT];
 #pragma unroll
-      for (int q = 0; q < 4; q++) out[j][q] = __builtin_amdgcn_perm(v[2 * q + 1][j >> 1], v[2 * q][j >> 1], j & 1 ? 0x07060302u : 0x05040100u);
+  for (int i = 0; i < 2; i++) x[i] = job.v + p.plan.order()[start + min(16 * i + col, count - 1)] * job.stride + group * 16;  // (rows behind the last: not used)
+#pragma unroll
+  for (int i = 0; i < RT; i++) w[i] = job.w + ((int64_t)c * p.in.rank + min(r0 + 16 * i + col, rank - 1)) * job.length * SIZE + group * 16;
+  f32x4_t acc[2][RT] = {};
+  const int first = split * job.share + wave, units = min((split + 1) * job.share, (job.length + UNIT - 1) / UNIT);
+  // an adapter of a lower rank than the pool's: only the sixteens that it has
+  if (RT == 4 && rank - r0 > 32) ad_shrink_units<KIND, 2, 4, RT>(x, w, job.length, first, units, AD_WAVES, acc);
+  else if (RT >= 2 && rank - r0 > 16) ad_shrink_units<KIND, 2, 2, RT>(x, w, job.length, first, units, AD_WAVES, acc);
+  else ad_shrink_units<KIND, 2, 1, RT>(x, w, job.length, first, units, AD_WAVES, acc);
+  // the wavefronts' sums: the upper half of them to the lower half, again and again
+  f32x4_t* join = reinterpret_cast<f32x4_t*>(shared);
+#pragma unroll
+  for (int half = AD_WAVES / 2; half > 0; half /= 2) {
+    if (wave >= half && wave < 2 * half)
+#pragma unroll
+      for (int i = 0; i < 2 * RT; i++) join[((wave - half) * 2 * RT + i) * 64 + lane] = acc[i / RT][i % RT];
+    __syncthreads();
+    if (wave < half)
+#pragma unroll
+      for (int i = 0; i < 2 * RT; i++) acc[i / RT][i % RT] += join[(wave * 2 * RT + i) * 64 + lane];
+    __syncthreads();
+  }
+  float* sums = reinterpret_cast<float*>(shared);
+  if (wave == 0) {
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+#pragma unroll
+      for (int j = 0; j < RT; j++)
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+          const int place = 16 * i + 4 * group + q, r = 16 * j + col;
+          sums[place * PITCH + r] = place < count && r0 + r < rank ? acc[i][j][q] * scale : 0.f;
+        }
+  }
+  __syncthreads();
+  const int t = threadIdx.x, sixteens = ad_sixteens(p.in.rank);
+  if (job.splits > 1) {  // the sums to memory past this die's cache, and the ticket behind them
+    const int64_t mine = (int64_t)tile * p.chunks + chunk;
+    float* parts = job.parts + mine * job.splits * (AD_TILE * WIDE);
+    for (int i = t; i < AD_TILE * WIDE; i += 64 * AD_WAVES) store_through(&parts[split * (AD_TILE * WIDE) + i], sums[i / WIDE * PITCH + i % WIDE]);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (t == 0) last = __hip_atomic_fetch_add(&job.tickets[mine], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == job.splits - 1;
+    __syncthreads();
+    if (!last) return;
+    for (int i = t; i < AD_TILE * WIDE; i += 64 * AD_WAVES) {
+      float v = 0.f;
+#pragma unroll 8
+      for (int s = 0; s < job.splits; s++) v += load_through(&parts[s * (AD_TILE * WIDE) + i]);
+      sums[i / WIDE * PITCH + i % WIDE] = v;
+    }
+    __syncthreads();
+  }
+  if constexpr (KIND == HB_F16) {
+    if (t < AD_TILE * RT) {  // thread: sixteen ranks of a row
+      const int place = t % AD_TILE, j = t / AD_TILE;
+      float most = 0.f;
+#pragma unroll
+      for (int r = 0; r < 16; r++) {
+        const float size = fabsf(sums[place * PITCH + 16 * j + r]);
+        most = size < INFINITY ? fmaxf(most, size) : most;
+      }
+      const int e = ad_exponent(most);
+      row_power[j * AD_TILE + place] = e;
+      int high = e;
+#pragma unroll
+      for (int d = 1; d < AD_TILE; d <<= 1) high = max(high, __shfl_xor(high, d));
+      if (place == 0) rank_power[j] = high;
+      if (r0 / 16 + j < sixteens) {
+        const int64_t at = (int64_t)tile * sixteens + r0 / 16 + j;
+        if (job.by_row) job.row_power[at * AD_TILE + place] = (int8_t)e;
+        if (job.by_rank && place == 0) job.rank_power[at] = (int8_t)high;
+      }
+    }
+    __syncthreads();
+  }
+  if (job.by_row) {
+    constexpr int ROW = RT == 1 ? 32 : WIDE;  // (up to sixteen ranks: zeros behind them to 32)
+    for (int i = t; i < AD_TILE * ROW; i += 64 * AD_WAVES) {
+      const int r = i % 32, place = i / 32 % AD_TILE, step = i / (32 * AD_TILE);
+      if (r0 + 32 * step >= p.in.rank) break;
+      const float v = 32 * step + r < WIDE ? sums[place * PITCH + 32 * step + r] : 0.f;
+      const int64_t at = ((int64_t)tile * ad_thirties(p.in.rank) + r0 / 32 + step) * PARTS * 1024 + place * 32 + r;
+      if constexpr (SIZE == 4) {
+        reinterpret_cast<float*>(job.by_row)[at] = v;
+      } else {
+        uint16_t part[PARTS];
+        const float unit = KIND == HB_F16 && 32 * step + r < WIDE ? ad_pow2(-row_power[(32 * step + r) / 16 * AD_TILE + place]) : 1.0f;
+        ad_cut<KIND, PARTS>(v * unit, part);
+#pragma unroll
+        for (int q = 0; q < PARTS; q++) reinterpret_cast<uint16_t*>(job.by_row)[at + q * 1024] = part[q];
+      }
+    }
+  }
+  if (job.by_rank) {
+    for (int i = t; i < AD_TILE * WIDE; i += 64 * AD_WAVES) {
+      const int place = i % AD_TILE, r = i / AD_TILE % 16, j = i / (AD_TILE * 16);
+      if (r0 / 16 + j >= sixteens) break;
+      const float v = sums[place * PITCH + 16 * j + r];
+      const int64_t at = ((int64_t)tile * sixteens + r0 / 16 + j) * OUTER * 512 + r * 32 + place;
+      if constexpr (SIZE == 4) {
+        reinterpret_cast<float*>(job.by_rank)[at] = v;
+      } else {
+        uint16_t part[OUTER];
+        ad_cut<KIND, OUTER>(KIND == HB_F16 ? v * ad_pow2(-rank_power[j]) : v, part);
+#pragma unroll
+        for (int q = 0; q < OUTER; q++) reinterpret_cast<uint16_t*>(job.by_rank)[at + q * 512] = part[q];
+      }
+    }
   }
 }
 
 // ------------------------------------------------------------------------------------------------ expand
 
+// acc[j] of TM x 16 rows += 32 ranks: `s` their parts (or FP32 values), v eight ranks of the matrix a lane, sixteen bytes each. Lane l's operand for instruction j
+// is column l * VEC + j: the eight rows, turned in registers, give it all of them, and the results are whole 16-byte pieces of out's rows.
+template <int KIND, int TM, int LIMIT, int WORDS>
+__device__ __forceinline__ void ad_products(const u32x4_t (&s)[LIMIT][WORDS], const u32x4_t (&v)[8], f32x4_t (&acc)[LIMIT][AD_VEC<KIND>]) {  // (of LIMIT, the first TM)
+  if constexpr (KIND == HB_F32) {
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+#pragma unroll
+        for (int t = 0; t < TM; t++) acc[t][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(s[t][i >> 2][i & 3]), __uint_as_float(v[i][j]), acc[t][j], 0, 0, 0);
+  } else {
+#pragma unroll
+    for (int j = 0; j < AD_VEC<KIND>; j++) {
+      const u32x4_t w = ad_turn(v, j);
+#pragma unroll
+      for (int i = 0; i < WORDS; i++)
+#pragma unroll
+        for (int t = 0; t < TM; t++) acc[t][j] = ad_mma<KIND>(s[t][i], w, acc[t][j]);
+    }
+  }
+}
+
+// y + the lane's VEC sums of row i of its four (times 2^e), rounded.
+template <int KIND>
+__device__ __forceinline__ u32x4_t ad_result(const u32x4_t& y, const f32x4_t (&acc)[AD_VEC<KIND>], int i, float unit) {
+  u32x4_t v{0u, 0u, 0u, 0u};
+#pragma unroll
+  for (int j = 0; j < AD_VEC<KIND>; j++) {
+    const float to = ad_value<KIND>(ad_elem<KIND>(y, j)) + (KIND == HB_F16 ? acc[j][i] * unit : acc[j][i]);
+    if constexpr (AdType<KIND>::SIZE == 4) v[j] = __float_as_uint(to);
+    else v[j >> 1] |= ad_bits<KIND>(to) << (16 * (j & 1));
+  }
+  return v;
+}
+
+// Few rows: a workgroup joins the splits' sums of its tile in LDS, then a tile's rows times four wavefronts' columns, sixteen lanes of sixteen bytes each.
+template <int KIND, bool TINY>
+__global__ __launch_bounds__(256) void ad_expand_few_kernel(AdFew p) {
+  constexpr int VEC = AD_VEC<KIND>, SIZE = AdType<KIND>::SIZE, PARTS = AdType<KIND>::PARTS;
+  extern __shared__ __align__(16) char staged[];  // [part][row][padded + 16 bytes]
+  __shared__ int32_t power[16];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, group = lane >> 4, col = lane & 15;
+  int c, row;
+  const int count = ad_tile_at(p.in, blockIdx.x, c, row);
+  if (count == 0) return;
+  const int rank = ad_rank(p.in, c), pitch = p.padded + (SIZE == 2 ? 8 : 4);  // elements
+  if (rank == 0 && p.y == p.out) return;
+  const int stride = gridDim.y * 4;
+  int block = blockIdx.y * 4 + wave;
+  u32x4_t y[4], v[8], next[8];
+  int64_t rows[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) rows[i] = __shfl(row, 4 * group + i);
+  auto base = [&](int first) {  // (rows behind the last: the first again)
+#pragma unroll
+    for (int i = 0; i < 4; i++) y[i] = ad_take<KIND, TINY>(p.y + rows[i] * p.y_stride, first, p.n);
+  };
+  auto load = [&](u32x4_t (&to)[8], int first, int r0) {
+#pragma unroll
+    for (int s = 0; s < 8; s++) to[s] = ad_take<KIND, TINY>(p.b + ((int64_t)c * p.in.rank + min(r0 + 8 * group + s, rank - 1)) * p.n * SIZE, first, p.n);
+  };
+  base(block * 16 * VEC + col * VEC);
+  if (rank == 0) {  // no adapter: the rows as they are
+    for (; block * (16 * VEC) < p.n; block += stride) {
+      const int first = block * 16 * VEC + col * VEC;
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        if (4 * group + i < count) ad_put<KIND, TINY>(p.out + rows[i] * p.out_stride, y[i], first, p.n);
+      base(first + stride * 16 * VEC);
+    }
+    return;
+  }
+  load(v, block * 16 * VEC + col * VEC, 0);
+  {  // the rows' sums, joined over the splits and scaled: sixteen threads a row
+    const int place = threadIdx.x / 16, lane_of = threadIdx.x % 16;
+    const float* sums = p.sums + (int64_t)__shfl(row, place) * p.in.rank;
+    const float scale = p.scale ? p.scale[c] : 1.0f;
+    auto sum = [&](int r) {  // every split's load under way before the first is used
+      float part[AD_SPLITS], to = 0.f;
+#pragma unroll
+      for (int s = 0; s < AD_SPLITS; s++) part[s] = s < p.splits ? sums[(int64_t)s * p.in.m * p.in.rank + r] : 0.f;
+#pragma unroll
+      for (int s = 0; s < AD_SPLITS; s++) to += part[s];
+      return to * scale;
+    };
+    float unit = 1.0f;
+    if constexpr (KIND == HB_F16) {
+      float most = 0.f;
+      for (int r = lane_of; r < rank; r += 16) {
+        const float size = fabsf(sum(r));
+        most = size < INFINITY ? fmaxf(most, size) : most;
+      }
+#pragma unroll
+      for (int d = 1; d < 16; d <<= 1) most = fmaxf(most, __shfl_xor(most, d));
+      const int e = ad_exponent(most);
+      if (lane_of == 0) power[place] = e;
+      unit = ad_pow2(-e);
+    }
+    const int used = (rank + 31) & ~31;
+#pragma unroll 2
+    for (int r = lane_of; r < used; r += 16) {
+      const float to = r < rank ? sum(r) * unit : 0.f;
+      if constexpr (SIZE == 4) {
+        reinterpret_cast<float*>(staged)[place * pitch + r] = to;
+      } else {
+        uint16_t part[PARTS];
+        ad_cut<KIND, PARTS>(to, part);
+#pragma unroll
+        for (int i = 0; i < PARTS; i++) reinterpret_cast<uint16_t*>(staged)[(i * 16 + place) * pitch + r] = part[i];
+      }
+    }
+  }
+  __syncthreads();
+  // (block, 32 ranks) one after another, the next one's matrix under way; idle lanes behind the last column take part in the products
+  for (; block * (16 * VEC) < p.n; block += stride) {
+    const int first = block * 16 * VEC + col * VEC;
+    f32x4_t acc[1][VEC] = {};
+    for (int r0 = 0; r0 < rank; r0 += 32) {
+      const bool on = r0 + 32 < rank;
+      load(next, on ? first : first + stride * 16 * VEC, on ? r0 + 32 : 0);
+      constexpr int WORDS = SIZE == 4 ? 2 : PARTS;
+      u32x4_t s[1][WORDS];
+#pragma unroll
+      for (int i = 0; i < WORDS; i++)
+        s[0][i] = *reinterpret_cast<const u32x4_t*>(SIZE == 4 ? staged + (col * pitch + r0 + 8 * group + 4 * i) * 4 : staged + ((i * 16 + col) * pitch + r0 + 8 * group) * 2);
+      ad_products<KIND, 1, 1, WORDS>(s, v, acc);
+#pragma unroll
+      for (int i = 0; i < 8; i++) v[i] = next[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      if (4 * group + i < count)
+        ad_put<KIND, TINY>(p.out + rows[i] * p.out_stride, ad_result<KIND>(y[i], acc[0], i, KIND == HB_F16 ? ad_pow2(power[4 * group + i]) : 1.0f), first, p.n);
+    base(first + stride * 16 * VEC);
+  }
+}
+
+// A plan's tiles, sixteen rows a workgroup: every wavefront for itself, over every (4 x gridDim.y)-th block of sixteen lanes' columns.
 struct AdExpand {
   AdIndex in;
   AdPlan plan;
-  const float* sums;   // [splits, m, rank]
-  const float* scale;  // [adapters] or null
-  int splits, n, padded;  // padded: the rank in LDS, a multiple of 32
+  const char* by_row;  // the shrink's
+  const int8_t* row_power;
+  int n;
   const char* w;       // [adapters, rank, n]
   const char* y;       // null: zeros
   int64_t y_stride;    // bytes
   char* out;
   int64_t out_stride;
 };
-
-// A workgroup: a tile's rows times four wavefronts' columns, sixteen lanes of sixteen bytes each. Lane l's operand for instruction j is column
-// l * VEC + j: eight rows of the matrix, turned in registers, give it all of them, and the results are whole 16-byte pieces of out's rows.
-template <int KIND, int TM>
+template <int KIND, bool TINY>
 __global__ __launch_bounds__(256) void ad_expand_kernel(AdExpand p) {
   constexpr int VEC = AD_VEC<KIND>, SIZE = AdType<KIND>::SIZE, PARTS = AdType<KIND>::PARTS;
-  extern __shared__ __align__(16) char staged[];  // [part][row][padded + 16 bytes]
-  __shared__ int32_t rows[16 * TM];
-  __shared__ int32_t power[16 * TM];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, group = lane >> 4, col = lane & 15;
-  int c;
-  const int count = ad_tile<16 * TM>(p.in, p.plan, 1, blockIdx.x, rows, c);
-  if (count == 0) return;
-  const int64_t first = ((int64_t)blockIdx.y * 4 + wave) * 16 * VEC + col * VEC, left = p.n - first;
-  if (c >= p.in.adapters) {  // no adapter: the rows as they are
-    if (p.y == p.out) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, group = lane >> 4, col = lane & 15, tile = blockIdx.x >> 1, half = blockIdx.x & 1;
+  int c, start;
+  int count = ad_tile(p.plan, tile, c, start) - 16 * half;
+  if (count <= 0) return;
+  start += 16 * half;
+  count = min(count, 16);
+  const int rank = ad_rank(p.in, c);
+  if (rank == 0 && p.y == p.out) return;
+  int64_t rows[4];
 #pragma unroll
-    for (int i = 0; i < 4 * TM; i++) {
-      const int place = 4 * i + group;
-      if (place < count && left > 0) {
-        const u32x4_t v = p.y ? ad_load<KIND>(p.y + rows[place] * p.y_stride + first * SIZE, left) : u32x4_t{0u, 0u, 0u, 0u};
-        ad_store<KIND>(p.out + rows[place] * p.out_stride + first * SIZE, v, left);
-      }
-    }
-    return;
+  for (int i = 0; i < 4; i++) rows[i] = p.plan.order()[start + min(4 * group + i, count - 1)];
+  const int sixteens = ad_sixteens(p.in.rank), steps = ad_thirties(rank);
+  int power = 0;  // FP16: of row col, the largest over the ranks
+  const int8_t* powers = p.row_power + (int64_t)tile * sixteens * AD_TILE + 16 * half + col;
+  if constexpr (KIND == HB_F16) {
+    power = -128;
+    for (int j = 0; j < ad_sixteens(rank); j++) power = max(power, (int)powers[j * AD_TILE]);
   }
-  const int rank = ad_rank(p.in, c), pitch = p.padded + (SIZE == 2 ? 8 : 4);  // elements
-  u32x4_t yv[TM][4];
+  const char* sums = p.by_row + (int64_t)tile * ad_thirties(p.in.rank) * PARTS * 1024 * SIZE + ((16 * half + col) * 32 + 8 * group) * SIZE;
+  constexpr int WORDS = SIZE == 4 ? 2 : PARTS;
+  u32x4_t s[1][WORDS], y[4], v[8];
+  auto parts = [&](int step) {
 #pragma unroll
-  for (int t = 0; t < TM; t++)
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const int place = 16 * t + 4 * group + i;
-      yv[t][i] = p.y && place < count && left > 0 ? ad_load<KIND>(p.y + rows[place] * p.y_stride + first * SIZE, left) : u32x4_t{0u, 0u, 0u, 0u};
-    }
-  {  // the rows' sums, joined over the splits and scaled
-    constexpr int EACH = 256 / (16 * TM);  // threads a row
-    const int place = threadIdx.x / EACH, lane_of = threadIdx.x % EACH;
-    const float* sums = p.sums + (int64_t)rows[place] * p.in.rank;
-    const float scale = p.scale ? p.scale[c] : 1.0f;
-    auto sum = [&](int r) {
-      float v = 0.f;
-      for (int s = 0; s < p.splits; s++) v += sums[(int64_t)s * p.in.m * p.in.rank + r];
-      return v * scale;
-    };
-    float unit = 1.0f;
-    if constexpr (KIND == HB_F16) {
-      float most = 0.f;
-      for (int r = lane_of; r < rank; r += EACH) {
-        const float v = fabsf(sum(r));
-        most = v < INFINITY ? fmaxf(most, v) : most;
-      }
-#pragma unroll
-      for (int d = 1; d < EACH; d <<= 1) most = fmaxf(most, __shfl_xor(most, d));
-      const int e = ad_exponent(most);
-      if (lane_of == 0) power[place] = e;
-      unit = ad_pow2(-e);
-    }
-    const int used = (rank + 31) & ~31;
-    for (int r = lane_of; r < used; r += EACH) {
-      const float v = r < rank ? sum(r) * unit : 0.f;
-      if constexpr (SIZE == 4) {
-        reinterpret_cast<float*>(staged)[place * pitch + r] = v;
-      } else {
-        uint16_t part[PARTS];
-        ad_cut<KIND, PARTS>(v, part);
-#pragma unroll
-        for (int i = 0; i < PARTS; i++) reinterpret_cast<uint16_t*>(staged)[(i * 16 * TM + place) * pitch + r] = part[i];
+    for (int i = 0; i < WORDS; i++) {
+      s[0][i] = *reinterpret_cast<const u32x4_t*>(sums + (int64_t)step * PARTS * 1024 * SIZE + (SIZE == 4 ? 16 * i : i * 2048));
+      if constexpr (KIND == HB_F16) {
+        const int j = 2 * step + (group >> 1);  // (ranks behind the last sixteen are zero)
+        s[0][i] = ad_lower(s[0][i], j < ad_sixteens(rank) ? powers[j * AD_TILE] - power : 0);
       }
     }
+  };
+  auto matrix = [&](int first, int step) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = ad_take<KIND, TINY>(p.w + ((int64_t)c * p.in.rank + min(32 * step + 8 * group + i, rank - 1)) * p.n * SIZE, first, p.n);
+  };
+  auto base = [&](int first) {  // (rows behind the last: it again)
+#pragma unroll
+    for (int i = 0; i < 4; i++) y[i] = p.y ? ad_take<KIND, TINY>(p.y + rows[i] * p.y_stride, first, p.n) : u32x4_t{0u, 0u, 0u, 0u};
+  };
+  // the wavefront's blocks, the next one's matrix under way while one is added; a rank of up to 32 keeps its sums in registers
+  const int stride = gridDim.y * 4;
+  int block = blockIdx.y * 4 + wave;
+  if (block * 16 * VEC >= p.n) return;
+  base(block * 16 * VEC + col * VEC);
+  if (steps) {
+    matrix(block * 16 * VEC + col * VEC, 0);
+    parts(0);
   }
-  __syncthreads();
-  if (first - col * VEC >= p.n) return;  // a wavefront behind the last column (idle lanes of the others take part in the products)
-  f32x4_t acc[TM][VEC] = {};
-  for (int r0 = 0; r0 < rank; r0 += 32) {
-    u32x4_t v[8];
+  float unit[4];
 #pragma unroll
-    for (int s = 0; s < 8; s++) {
-      const char* at = p.w + (((int64_t)c * p.in.rank + min(r0 + 8 * group + s, rank - 1)) * p.n + first) * SIZE;
-      v[s] = left > 0 ? ad_load<KIND>(at, left) : u32x4_t{0u, 0u, 0u, 0u};
-    }
-    if constexpr (SIZE == 2) {
-      u32x4_t w[VEC];
-      ad_turn<KIND>(v, w);
-#pragma unroll
-      for (int t = 0; t < TM; t++)
-#pragma unroll
-        for (int i = 0; i < PARTS; i++) {
-          const u32x4_t s = *reinterpret_cast<const u32x4_t*>(staged + ((i * 16 * TM + 16 * t + col) * pitch + r0 + 8 * group) * 2);
-#pragma unroll
-          for (int j = 0; j < VEC; j++) acc[t][j] = ad_mma<KIND>(s, w[j], acc[t][j]);
-        }
-    } else {
-#pragma unroll
-      for (int t = 0; t < TM; t++) {
-        const float* s = reinterpret_cast<const float*>(staged) + (16 * t + col) * pitch + r0 + 8 * group;
-#pragma unroll
-        for (int i = 0; i < 8; i++)
-#pragma unroll
-          for (int j = 0; j < VEC; j++) acc[t][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(s[i], __uint_as_float(v[i][j]), acc[t][j], 0, 0, 0);
+  for (int i = 0; i < 4; i++) unit[i] = KIND == HB_F16 ? ad_pow2(max(__shfl(power, 4 * group + i), -126)) : 1.0f;
+  for (; block * 16 * VEC < p.n; block += stride) {
+    const int first = block * 16 * VEC + col * VEC;
+    const bool more = (block + stride) * 16 * VEC < p.n;
+    f32x4_t acc[1][VEC] = {};
+    for (int step = 0; step < steps; step++) {
+      ad_products<KIND, 1, 1, WORDS>(s, v, acc);
+      if (step + 1 < steps) {
+        matrix(first, step + 1);
+        parts(step + 1);
       }
     }
+    if (more) {
+      if (steps) matrix(first + stride * 16 * VEC, 0);
+      if (steps > 1) parts(0);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      if (4 * group + i < count)  // (without an adapter the rows as they are: -0 too)
+        ad_put<KIND, TINY>(p.out + rows[i] * p.out_stride, rank == 0 ? y[i] : ad_result<KIND>(y[i], acc[0], i, unit[i]), first, p.n);
+    if (more) base(first + stride * 16 * VEC);
   }
-  if (left <= 0) return;
-#pragma unroll
-  for (int t = 0; t < TM; t++)
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const int place = 16 * t + 4 * group + i;
-      if (place >= count) continue;
-      float unit = 1.0f;
-      if constexpr (KIND == HB_F16) unit = ad_pow2(power[place]);
-      u32x4_t v{0u, 0u, 0u, 0u};
-#pragma unroll
-      for (int j = 0; j < VEC; j++) {
-        const float to = ad_value<KIND>(ad_elem<KIND>(yv[t][i], j)) + (KIND == HB_F16 ? acc[t][j][i] * unit : acc[t][j][i]);
-        if constexpr (SIZE == 4) v[j] = __float_as_uint(to);
-        else v[j >> 1] |= ad_bits<KIND>(to) << (16 * (j & 1));
-      }
-      ad_store<KIND>(p.out + rows[place] * p.out_stride + first * SIZE, v, left);
-    }
 }
 
 // ------------------------------------------------------------------------------------------------ outer
 
 struct AdOuterJob {
-  const float* sums;   // [splits, m, rank]: of the other side's shrink
-  const char* v;       // rows
-  int64_t stride;      // bytes
+  const char* by_rank;  // of the other side's shrink
+  const int8_t* rank_power;
+  const char* v;        // rows
+  int64_t stride;       // bytes
   int length;
-  float* to;           // [adapters, rank, length]
-  float* parts;        // [slots, rank, length]
+  float* to;            // [adapters, rank, length]
+  float* parts;         // [slots, rank, length]
 };
 struct AdOuter {
   AdIndex in;
   AdPlan plan;
   AdOuterJob job[2];
-  const float* scale;
-  int splits, unit, chunks;
+  int unit, chunks;
 };
 
-// A workgroup: RT x 16 ranks times sixteen lanes' columns over a unit of an adapter's rows, the four wavefronts taking 32 rows of every 128 and joining
-// their sums in LDS. An adapter's only unit writes the gradient, several write partial sums.
-template <int KIND, int RT>
+// A workgroup: RT x 16 ranks times sixteen lanes' columns over a unit of an adapter's rows, the four wavefronts taking its tiles in turn and joining
+// their sums in LDS. A lane's eight rows of sixteen bytes are turned as in the expansion; the next tile's are under way while one is
+// multiplied. An adapter's only unit writes the gradient, several write partial sums.
+template <int KIND, int RT, bool TINY>
 __global__ __launch_bounds__(256) void ad_outer_kernel(AdOuter p) {
-  constexpr int VEC = AD_VEC<KIND>, SIZE = AdType<KIND>::SIZE, PARTS = AdType<KIND>::OUTER, PITCH = AD_CHUNK + (SIZE == 2 ? 8 : 4);
-  constexpr int STAGED = PARTS * 16 * RT * PITCH * SIZE, JOINED = 4 * VEC * 64 * 16;
-  __shared__ __align__(16) char staged[STAGED > JOINED ? STAGED : JOINED];  // [part][rank][row of the chunk]; at the end [wavefront][column of a lane][lane]
-  __shared__ int32_t rows[AD_CHUNK];
-  __shared__ float most_of[4];
+  constexpr int VEC = AD_VEC<KIND>, SIZE = AdType<KIND>::SIZE, PARTS = AdType<KIND>::OUTER, WORDS = SIZE == 4 ? 2 : PARTS;
+  __shared__ f32x4_t join[4 * VEC * 64];  // [wavefront][column of a lane][lane]
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, group = lane >> 4, col = lane & 15;
   const AdOuterJob& job = p.job[blockIdx.z / p.chunks];
-  const int r0 = (blockIdx.z % p.chunks) * 16 * RT, u = blockIdx.y;
-  if (u >= p.plan.units()[p.plan.classes]) return;
-  const int64_t first = (int64_t)blockIdx.x * 16 * VEC + col * VEC, left = job.length - first;
-  if ((int64_t)blockIdx.x * 16 * VEC >= job.length) return;
-  const int c = ad_find(p.plan.units(), p.plan.classes, u);
-  const int which = u - p.plan.units()[c], units = p.plan.units()[c + 1] - p.plan.units()[c];
-  const int start = p.plan.rows()[c] + which * p.unit, end = min(start + p.unit, p.plan.rows()[c + 1]);
-  const int rank = ad_rank(p.in, c);
-  float* to = (units > 1 ? job.parts + (int64_t)(p.plan.slots()[c] + which) * p.in.rank * job.length : job.to + (int64_t)c * p.in.rank * job.length);
-  const float scale = p.scale ? p.scale[c] : 1.0f;
+  const int r0 = (blockIdx.z % p.chunks) * 16 * RT, u = blockIdx.y, sixteens = ad_sixteens(p.in.rank);
+  if (u >= p.plan.units()[p.plan.classes] || (int64_t)blockIdx.x * 16 * VEC >= job.length) return;
+  const int first = blockIdx.x * 16 * VEC + col * VEC, left = job.length - first;
+  const AdPlace at = ad_find(p.plan, p.plan.units(), u);
+  const int c = at.c, which = u - at.first, units = p.plan.units()[c + 1] - at.first;
+  const int start = at.row + which * p.unit, end = min(start + p.unit, at.next_row);
+  const int rank = ad_rank(p.in, c), tile0 = p.plan.tiles()[c] + which * (p.unit / AD_TILE), tiles = r0 < rank ? (end - start + AD_TILE - 1) / AD_TILE : 0;
+  const int have = min(RT, ad_sixteens(rank - r0));  // sixteens of ranks (those behind the adapter's rank are not written)
+  float* to = units > 1 ? job.parts + (int64_t)(p.plan.slots()[c] + which) * p.in.rank * job.length : job.to + (int64_t)c * p.in.rank * job.length;
   f32x4_t acc[RT][VEC] = {};
-  int power = -200;  // FP16: the sums are in units of 2^power
-  for (int at = start; r0 < rank && at < end; at += AD_CHUNK) {
-    const int count = min(AD_CHUNK, end - at);
-    __syncthreads();  // the last chunk's operands are read
-    if (threadIdx.x < AD_CHUNK) rows[threadIdx.x] = p.plan.order()[at + min((int)threadIdx.x, count - 1)];
-    __syncthreads();
-    u32x4_t v[8];
-#pragma unroll
-    for (int s = 0; s < 8; s++) {
-      const int place = 32 * wave + 8 * group + s;
-      v[s] = left > 0 && place < count ? ad_load<KIND>(job.v + rows[place] * job.stride + first * SIZE, left) : u32x4_t{0u, 0u, 0u, 0u};
-    }
-    {  // thread: row t % 128 of the chunk, half of the ranks
-      const int place = threadIdx.x & (AD_CHUNK - 1), from = (threadIdx.x >> 7) * 8 * RT;
-      const float* sums = job.sums + (int64_t)rows[place] * p.in.rank + r0 + from;
-      float g[8 * RT];
-#pragma unroll
-      for (int i = 0; i < 8 * RT; i++) g[i] = 0.f;
-      if (place < count)
-        for (int s = 0; s < p.splits; s++)
-#pragma unroll
-          for (int i = 0; i < 8 * RT; i++) g[i] += r0 + from + i < rank ? sums[(int64_t)s * p.in.m * p.in.rank + i] : 0.f;
-      float unit = 1.0f;
-      if constexpr (KIND == HB_F16) {
-        float most = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8 * RT; i++) {
-          const float size = fabsf(g[i] * scale);
-          most = size < INFINITY ? fmaxf(most, size) : most;
-        }
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) most = fmaxf(most, __shfl_xor(most, d));
-        if (lane == 0) most_of[wave] = most;
-        __syncthreads();
-        const int e = max(power, ad_exponent(fmaxf(fmaxf(most_of[0], most_of[1]), fmaxf(most_of[2], most_of[3]))));
-        if (e != power) {  // the sums so far in the new units
-          const float by = power <= -200 ? 0.f : ad_pow2(max(power - e, -126));
-#pragma unroll
-          for (int i = 0; i < RT; i++)
-#pragma unroll
-            for (int j = 0; j < VEC; j++) acc[i][j] *= by;
-          power = e;
-        }
-        unit = ad_pow2(-power);
-      }
-#pragma unroll
-      for (int i = 0; i < 8 * RT; i++) {
-        const float value = g[i] * scale * unit;
-        if constexpr (SIZE == 4) {
-          reinterpret_cast<float*>(staged)[(from + i) * PITCH + place] = value;
-        } else {
-          uint16_t part[PARTS];
-          ad_cut<KIND, PARTS>(value, part);
-#pragma unroll
-          for (int q = 0; q < PARTS; q++) reinterpret_cast<uint16_t*>(staged)[(q * 16 * RT + from + i) * PITCH + place] = part[q];
-        }
-      }
-    }
-    __syncthreads();
-    if constexpr (SIZE == 2) {
-      u32x4_t w[VEC];
-      ad_turn<KIND>(v, w);
-#pragma unroll
-      for (int t = 0; t < RT; t++)
-#pragma unroll
-        for (int i = 0; i < PARTS; i++) {
-          const u32x4_t s = *reinterpret_cast<const u32x4_t*>(staged + ((i * 16 * RT + 16 * t + col) * PITCH + 32 * wave + 8 * group) * 2);
-#pragma unroll
-          for (int j = 0; j < VEC; j++) acc[t][j] = ad_mma<KIND>(s, w[j], acc[t][j]);
-        }
-    } else {
-#pragma unroll
-      for (int t = 0; t < RT; t++) {
-        const float* s = reinterpret_cast<const float*>(staged) + (16 * t + col) * PITCH + 32 * wave + 8 * group;
-#pragma unroll
-        for (int i = 0; i < 8; i++)
-#pragma unroll
-          for (int j = 0; j < VEC; j++) acc[t][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(s[i], __uint_as_float(v[i][j]), acc[t][j], 0, 0, 0);
-      }
-    }
-  }
-  // D: this lane's columns first .. first + VEC - 1 of ranks 4 group .. + 3 of every sixteen
-  f32x4_t* join = reinterpret_cast<f32x4_t*>(staged);
+  int power[RT];  // FP16: the sums are in units of 2^power, the largest of the unit's tiles
+  const int8_t* powers = job.rank_power + (int64_t)tile0 * sixteens + r0 / 16;
 #pragma unroll
   for (int t = 0; t < RT; t++) {
+    power[t] = 0;
+    if constexpr (KIND == HB_F16) {
+      power[t] = -128;
+      for (int i = lane; i < tiles && t < have; i += 64) power[t] = max(power[t], (int)powers[(int64_t)i * sixteens + t]);
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) power[t] = max(power[t], __shfl_xor(power[t], d));
+    }
+  }
+  // under way: the rows' numbers two tiles ahead, the rows and their sums one
+  int rows[8];
+  u32x4_t next[8], ahead[RT][WORDS];
+  int shift[RT];
+  auto number = [&](int tile) {
+    const int from = start + tile * AD_TILE + 8 * group;
+#pragma unroll
+    for (int s = 0; s < 8; s++) rows[s] = p.plan.order()[min(from + s, end - 1)];
+  };
+  auto load = [&](int tile) {
+#pragma unroll
+    for (int s = 0; s < 8; s++) next[s] = ad_take<KIND, TINY>(job.v + rows[s] * job.stride, first, job.length);
+#pragma unroll
+    for (int t = 0; t < RT; t++) {  // (behind the adapter's sixteens its last one again)
+      const int j = min(t, have - 1);
+      const char* from = job.by_rank + ((int64_t)(tile0 + tile) * sixteens + r0 / 16 + j) * PARTS * 512 * SIZE + (col * 32 + 8 * group) * SIZE;
+#pragma unroll
+      for (int i = 0; i < WORDS; i++) ahead[t][i] = *reinterpret_cast<const u32x4_t*>(from + (SIZE == 4 ? 16 * i : i * 1024));
+      if constexpr (KIND == HB_F16) shift[t] = powers[(int64_t)tile * sixteens + j];
+    }
+  };
+  if (wave < tiles) {
+    number(wave);
+    load(wave);
+    number(min(wave + 4, tiles - 1));
+  }
+  for (int tile = wave; tile < tiles; tile += 4) {
+    u32x4_t v[8], s[RT][WORDS];
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = start + tile * AD_TILE + 8 * group + i < end ? next[i] : u32x4_t{0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int t = 0; t < RT; t++)
+#pragma unroll
+      for (int i = 0; i < WORDS; i++) {
+        s[t][i] = ahead[t][i];
+        if constexpr (KIND == HB_F16) s[t][i] = ad_lower(s[t][i], shift[t] - power[t]);
+      }
+    load(min(tile + 4, tiles - 1));  // (behind the last tile it again: no load behind a branch)
+    number(min(tile + 8, tiles - 1));
+    if (RT == 4 && have > 2) ad_products<KIND, RT, RT, WORDS>(s, v, acc);
+    else if (RT >= 2 && have == 2) ad_products<KIND, 2, RT, WORDS>(s, v, acc);
+    else ad_products<KIND, 1, RT, WORDS>(s, v, acc);
+  }
+  // D: this lane's columns first .. first + VEC - 1 of ranks 4 group .. + 3 of every sixteen
+#pragma unroll
+  for (int t = 0; t < RT; t++) {
+    const float unit = KIND == HB_F16 ? ad_pow2(max(power[t], -126)) : 1.0f;
     __syncthreads();
 #pragma unroll
-    for (int j = 0; j < VEC; j++) join[(wave * VEC + j) * 64 + lane] = acc[t][j];
+    for (int j = 0; j < VEC; j++) join[(wave * VEC + j) * 64 + lane] = KIND == HB_F16 ? acc[t][j] * unit : acc[t][j];
     __syncthreads();
     // thread: rank t * 16 + 4 group + wave of the columns of its lane
     const int r = r0 + 16 * t + 4 * group + wave;
     if (r < p.in.rank && left > 0) {
-      float* row = to + (int64_t)r * job.length + first;
-      const float unit = KIND == HB_F16 && power > -200 ? ad_pow2(power) : 1.0f;
+      float* row = to + (int64_t)r * job.length;
       float sum[VEC];
 #pragma unroll
       for (int j = 0; j < VEC; j++) {
         float v = 0.f;
 #pragma unroll
         for (int w = 0; w < 4; w++) v += reinterpret_cast<const float*>(&join[(w * VEC + j) * 64 + lane])[wave];
-        sum[j] = r < rank ? v * unit : 0.f;
+        sum[j] = r < rank ? v : 0.f;
       }
+      const bool whole = first + VEC <= job.length;
 #pragma unroll
-      for (int j = 0; j < VEC; j++)
-        if (j < left) row[j] = sum[j];
+      for (int q = 0; q < VEC; q += 4) {
+        u32x4_t v;
+#pragma unroll
+        for (int j = 0; j < 4; j++) v[j] = __float_as_uint(sum[q + j]);
+        if (whole) *reinterpret_cast<u32x4_loose*>(row + first + q) = v;
+      }
+      if (!whole) {
+        const int from = TINY ? first : job.length - VEC;  // the lane's columns, of which the ones before `first` are another's
+#pragma unroll
+        for (int j = 0; j < VEC; j++)
+          if (from + j >= first && from + j < job.length) row[from + j] = sum[j];
+      }
     }
   }
 }
@@ -682,26 +1001,40 @@ __global__ __launch_bounds__(256) void ad_join_kernel(AdOuter p) {
   if (units == 1) return;
   const int64_t size = (int64_t)p.in.rank * job.length;
   const float* from = job.parts + (int64_t)p.plan.slots()[c] * size;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < size; i += (int64_t)gridDim.x * 256) {
-    float v = 0.f;
-    for (int u = 0; u < units; u++) v += from[u * size + i];
-    job.to[(int64_t)c * size + i] = v;
+  for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < size; i += (int64_t)gridDim.x * 1024) {
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int u = 0; u < units; u++) {
+      const u32x4_t part = ad_load<HB_F32>(reinterpret_cast<const char*>(from + u * size + i), size - i);
+#pragma unroll
+      for (int j = 0; j < 4; j++) v[j] += __uint_as_float(part[j]);
+    }
+    u32x4_t out;
+#pragma unroll
+    for (int j = 0; j < 4; j++) out[j] = __float_as_uint(v[j]);
+    ad_store<HB_F32>(reinterpret_cast<char*>(job.to + (int64_t)c * size + i), out, size - i);
   }
 }
 
 // ------------------------------------------------------------------------------------------------ host
 
+static size_t up256(size_t v) { return (v + 255) & ~(size_t)255; }
+static int64_t cut(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
 struct AdShape {
   int64_t m;
   int adapters, rank, k, n, kind, size;
-  bool grads, self;
-  int tm0, tm1, rt, splits, unit;  // tile heights / 16 of shrink and expand, rank tiles a shrink's workgroup, splits of the long axis, rows a unit
-  int64_t tiles0, tiles1, units, slots;
-  size_t plan_bytes, sums_bytes, parts_bytes;  // plan | sums (x) | sums (dy) | parts (da) | parts (db)
-  size_t bytes() const { return plan_bytes + sums_bytes * (grads ? 2 : 1) + parts_bytes; }
+  bool grads, few;
+  int splits, rt, unit;  // few: splits of the long axis. Else rank tiles a shrink's workgroup, rows a unit
+  int share, splits_x, splits_dy, chunks;  // units of 128 bytes a split of the shrinks (x alone without gradients), chunks of ranks
+  int64_t tiles, units, slots, tickets;
+  // few: sums. Else plan | tickets | splits' sums | the x side by row or by rank | its powers | the dy side by row | by rank | its powers of both | parts of da | of db
+  size_t sums_bytes, plan_bytes, ticket_bytes, split_bytes, row_bytes, rank_bytes, row_power_bytes, rank_power_bytes, part_a_bytes, part_b_bytes;
+  size_t bytes() const {
+    if (few) return sums_bytes;
+    if (!grads) return plan_bytes + ticket_bytes + split_bytes + row_bytes + row_power_bytes;
+    return plan_bytes + ticket_bytes + split_bytes + row_bytes + row_power_bytes + 2 * (rank_bytes + rank_power_bytes) + part_a_bytes + part_b_bytes;
+  }
 };
-static size_t up256(size_t v) { return (v + 255) & ~(size_t)255; }
-static int64_t cut(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 static bool ad_shape(const hb_adapters* a, int64_t m, bool grads, AdShape& s) {
   if (a->type < HB_BF16 || a->type > HB_F32 || a->adapters <= 0 || a->adapters > AD_MOST || a->rank <= 0 || a->rank > AD_RANK || a->k <= 0 || a->n <= 0 ||
@@ -710,71 +1043,91 @@ static bool ad_shape(const hb_adapters* a, int64_t m, bool grads, AdShape& s) {
   s = AdShape{};
   s.m = m, s.adapters = a->adapters, s.rank = a->rank, s.k = a->k, s.n = a->n, s.kind = a->type, s.size = a->type == HB_F32 ? 4 : 2;
   s.grads = grads;
-  s.self = !grads && m <= AD_SELF_ROWS;
+  s.few = !grads && m <= AD_SELF_ROWS;
   const int64_t classes = std::min<int64_t>(a->adapters + 1, m);
-  s.tm0 = s.self || m < 2048 ? 1 : 2;
-  s.tm1 = s.self || m < 2048 ? 1 : 2;
-  s.tiles0 = s.self ? m : cut(m, 16 * s.tm0) + classes;
-  s.tiles1 = s.self ? m : cut(m, 16 * s.tm1) + classes;
-  s.rt = s.self || a->rank <= 16 ? 1 : a->rank <= 32 ? 2 : 4;
-  const int64_t longest = grads ? std::max(a->k, a->n) : a->k, units = cut(longest, 128 / s.size), chunks = cut(a->rank, 16 * s.rt);
-  const int64_t groups = (s.self ? std::min<int64_t>(m, a->adapters + cut(m, 16)) : cut(m, 16 * s.tm0)) * chunks * (grads ? 2 : 1);
-  s.splits = (int)std::max<int64_t>(1, std::min<int64_t>(cut(1024, groups), cut(units, 16)));
-  s.sums_bytes = up256((size_t)s.splits * m * a->rank * 4);
-  s.plan_bytes = s.self ? 0 : up256(AdPlan::ints(a->adapters + 1, m) * 4);
+  if (s.few) {
+    s.tiles = std::min<int64_t>(m, a->adapters + cut(m, 16));  // at most, of those that begin somewhere
+    const int64_t groups = s.tiles * cut(a->rank, 16);
+    s.splits = (int)std::max<int64_t>(1, std::min<int64_t>({cut(1024, groups), cut(cut(a->k, 128 / s.size), 16), AD_SPLITS}));
+    s.sums_bytes = up256((size_t)s.splits * m * a->rank * 4);
+    return true;
+  }
+  s.tiles = cut(m, AD_TILE) + classes;
+  s.rt = a->rank <= 16 ? 1 : a->rank <= 32 ? 2 : 4;
+  s.plan_bytes = up256(AdPlan::ints(a->adapters + 1, m) * 4);
+  s.chunks = (int)cut(a->rank, 16 * s.rt);
+  const int64_t units_x = cut(a->k, 128 / s.size), units_dy = grads ? cut(a->n, 128 / s.size) : 0;
+  s.share = (int)std::max<int64_t>(2 * AD_WAVES, cut((units_x + units_dy) * cut(m, AD_TILE) * s.chunks, 1024));
+  s.splits_x = (int)cut(units_x, s.share), s.splits_dy = (int)cut(units_dy, s.share);
+  s.tickets = s.tiles * s.chunks * (grads ? 2 : 1);
+  s.ticket_bytes = up256((size_t)s.tickets * 4);
+  s.split_bytes = up256((size_t)s.tiles * s.chunks * ((s.splits_x > 1 ? s.splits_x : 0) + (s.splits_dy > 1 ? s.splits_dy : 0)) * AD_TILE * 16 * s.rt * 4);
+  const int parts = a->type == HB_F32 ? 1 : 2, outer = a->type == HB_BF16 ? 3 : parts;
+  s.row_bytes = up256((size_t)s.tiles * ad_thirties(a->rank) * parts * 1024 * s.size);
+  s.rank_bytes = up256((size_t)s.tiles * ad_sixteens(a->rank) * outer * 512 * s.size);
+  s.row_power_bytes = a->type == HB_F16 ? up256((size_t)s.tiles * ad_sixteens(a->rank) * AD_TILE) : 0;
+  s.rank_power_bytes = a->type == HB_F16 ? up256((size_t)s.tiles * ad_sixteens(a->rank)) : 0;
+  s.unit = 4 * AD_TILE;
   if (grads) {
-    const int64_t blocks = (cut(a->k, 16 * 16 / s.size) + cut(a->n, 16 * 16 / s.size)) * cut(a->rank, 64);
-    s.unit = (int)std::min<int64_t>(std::max<int64_t>(AD_CHUNK, cut(cut(m * blocks, 2048), AD_CHUNK) * AD_CHUNK), 1 << 20);
+    const int64_t blocks = (cut(a->k, 256 / s.size) + cut(a->n, 256 / s.size)) * cut(a->rank, 64);
+    s.unit = (int)std::min<int64_t>(std::max<int64_t>(4 * AD_TILE, cut(cut(m * blocks, 1024), 4 * AD_TILE) * 4 * AD_TILE), 1 << 20);
     s.units = cut(m, s.unit) + classes;
-    s.slots = 2 * (m / s.unit);  // an adapter of more than one unit has fewer than two for every `unit` of its rows
-    s.parts_bytes = up256((size_t)s.slots * a->rank * a->k * 4) + up256((size_t)s.slots * a->rank * a->n * 4);
-  } else {
-    s.unit = AD_CHUNK;
+    s.slots = 2 * (m / s.unit);  // an adapter of more than one unit has at most two for every whole `unit` of its rows
+    s.part_a_bytes = up256((size_t)s.slots * a->rank * a->k * 4);
+    s.part_b_bytes = up256((size_t)s.slots * a->rank * a->n * 4);
   }
   return true;
 }
 
-static int ad_run_plan(const AdShape& s, const AdIndex& in, const AdPlan& plan, hipStream_t stream) {
-  AdPlanParams p{in, plan, {16 * s.tm0, 16 * s.tm1}, s.unit, 1};
-  while (p.segments < 16 && (int64_t)(2 * p.segments) * plan.classes <= 12288) p.segments *= 2;
-  ad_plan_kernel<<<1, 1024, (size_t)p.segments * plan.classes * 4, stream>>>(p);
+static int ad_run_plan(const AdShape& s, const AdIndex& in, const AdPlan& plan, char* ws, hipStream_t stream) {
+  AdPlanParams p{in, plan, s.unit, 1, reinterpret_cast<int32_t*>(ws + s.plan_bytes), s.tickets};
+  while (p.segments < 16 && (int64_t)(2 * p.segments) * plan.classes <= AD_COUNTERS) p.segments *= 2;
+  const size_t lds = (size_t)p.segments * plan.classes * 4;
+  if (s.m <= AD_HELD) ad_plan_kernel<true><<<1, 1024, lds + s.m * 4, stream>>>(p);
+  else ad_plan_kernel<false><<<1, 1024, lds, stream>>>(p);
   return launch_status();
 }
 
 template <int KIND>
-static int ad_run_shrink(const AdShape& s, AdShrink& p, int jobs, hipStream_t stream) {
-  p.chunks = (int)cut(s.rank, 16 * s.rt);
-  for (int j = 0; j < jobs; j++) p.job[j].share = (int)cut(cut(p.job[j].length, 128 / s.size), s.splits);
-  const dim3 grid((unsigned)s.tiles0, (unsigned)s.splits, (unsigned)(p.chunks * jobs));
-#define HB_AD(TM, RT) if (s.tm0 == TM && s.rt == RT) ad_shrink_kernel<KIND, TM, RT><<<grid, 256, 0, stream>>>(p)
-  HB_AD(1, 1); HB_AD(1, 2); HB_AD(1, 4); HB_AD(2, 1); HB_AD(2, 2); HB_AD(2, 4);
-#undef HB_AD
+static int ad_run_shrink(const AdShape& s, AdShrink& p, char* ws, hipStream_t stream) {
+  p.chunks = s.chunks;
+  int32_t* tickets = reinterpret_cast<int32_t*>(ws + s.plan_bytes);
+  float* parts = reinterpret_cast<float*>(ws + s.plan_bytes + s.ticket_bytes);
+  for (int j = 0; j < (s.grads ? 2 : 1); j++) {
+    p.job[j].splits = j ? s.splits_dy : s.splits_x;
+    p.job[j].share = s.share;
+    p.job[j].tickets = tickets + j * s.tiles * s.chunks;
+    p.job[j].parts = parts + (j && s.splits_x > 1 ? s.tiles * s.chunks * s.splits_x * AD_TILE * 16 * s.rt : 0);
+  }
+  const dim3 grid((unsigned)s.tiles, (unsigned)(p.chunks * (s.splits_x + s.splits_dy)));
+  if (s.rt == 1) ad_shrink_kernel<KIND, 1><<<grid, 64 * AD_WAVES, 0, stream>>>(p);
+  if (s.rt == 2) ad_shrink_kernel<KIND, 2><<<grid, 64 * AD_WAVES, 0, stream>>>(p);
+  if (s.rt == 4) ad_shrink_kernel<KIND, 4><<<grid, 64 * AD_WAVES, 0, stream>>>(p);
   return launch_status();
 }
 
 template <int KIND>
 static int ad_run_expand(const AdShape& s, AdExpand& p, hipStream_t stream) {
-  p.splits = s.splits;
-  p.padded = (int)cut(s.rank, 32) * 32;
-  const dim3 grid((unsigned)s.tiles1, (unsigned)cut(p.n, 4 * 16 * AD_VEC<KIND>));
-  const size_t lds = (size_t)AdType<KIND>::PARTS * 16 * s.tm1 * (p.padded * AdType<KIND>::SIZE + 16);
-  if (s.tm1 == 1) ad_expand_kernel<KIND, 1><<<grid, 256, lds, stream>>>(p);
-  else ad_expand_kernel<KIND, 2><<<grid, 256, lds, stream>>>(p);
+  const int64_t groups = cut(p.n, 4 * 16 * AD_VEC<KIND>);
+  const int64_t share = std::max<int64_t>(1, std::min<int64_t>(groups, 2 * s.tiles * groups / 1024));
+  const dim3 grid((unsigned)(2 * s.tiles), (unsigned)cut(groups, share));
+  if (p.n < AD_VEC<KIND>) ad_expand_kernel<KIND, true><<<grid, 256, 0, stream>>>(p);
+  else ad_expand_kernel<KIND, false><<<grid, 256, 0, stream>>>(p);
   return launch_status();
 }
 
 template <int KIND>
 static int ad_run_outer(const AdShape& s, AdOuter& p, hipStream_t stream) {
-  const int rt = s.rank <= 16 ? 1 : s.rank <= 32 ? 2 : 4;
-  p.chunks = (int)cut(s.rank, 16 * rt);
+  p.chunks = s.chunks;
   const int longest = std::max(p.job[0].length, p.job[1].length);
   const dim3 grid((unsigned)cut(longest, 16 * AD_VEC<KIND>), (unsigned)s.units, (unsigned)(2 * p.chunks));
-  if (rt == 1) ad_outer_kernel<KIND, 1><<<grid, 256, 0, stream>>>(p);
-  if (rt == 2) ad_outer_kernel<KIND, 2><<<grid, 256, 0, stream>>>(p);
-  if (rt == 4) ad_outer_kernel<KIND, 4><<<grid, 256, 0, stream>>>(p);
+  const bool tiny = std::min(p.job[0].length, p.job[1].length) < AD_VEC<KIND>;
+#define HB_AD(RT) if (s.rt == RT) { if (tiny) ad_outer_kernel<KIND, RT, true><<<grid, 256, 0, stream>>>(p); else ad_outer_kernel<KIND, RT, false><<<grid, 256, 0, stream>>>(p); }
+  HB_AD(1) HB_AD(2) HB_AD(4)
+#undef HB_AD
   int code = launch_status();
   if (code) return code;
-  const unsigned blocks = (unsigned)std::min<int64_t>(cut((int64_t)s.rank * longest, 256), 1024);
+  const unsigned blocks = (unsigned)std::min<int64_t>(cut((int64_t)s.rank * longest, 1024), 1024);
   ad_join_kernel<<<dim3(blocks, (unsigned)s.adapters, 2), 256, 0, stream>>>(p);
   return launch_status();
 }
@@ -782,13 +1135,28 @@ static int ad_run_outer(const AdShape& s, AdOuter& p, hipStream_t stream) {
 template <int KIND>
 static int ad_add(const hb_adapters* a, const AdShape& s, const AdIndex& in, const void* x, int64_t x_stride, const void* y, int64_t y_stride, void* out, int64_t out_stride,
                   char* ws, hipStream_t stream) {
-  const AdPlan plan{s.self ? nullptr : reinterpret_cast<int32_t*>(ws), s.adapters + 1};
-  float* sums = reinterpret_cast<float*>(ws + s.plan_bytes);
-  int code = s.self ? HB_OK : ad_run_plan(s, in, plan, stream);
+  const char *xr = static_cast<const char*>(x), *yr = static_cast<const char*>(y);
+  char* to = static_cast<char*>(out);
+  if (s.few) {
+    AdFew p{in, xr, x_stride * s.size, static_cast<const char*>(a->a), s.k, s.n, s.splits, (int)cut(cut(s.k, 128 / s.size), s.splits), reinterpret_cast<float*>(ws),
+            a->scale, static_cast<const char*>(a->b), yr, y_stride * s.size, to, out_stride * s.size, ad_thirties(s.rank) * 32};
+    ad_shrink_few_kernel<KIND><<<dim3((unsigned)s.m, (unsigned)s.splits, (unsigned)ad_sixteens(s.rank)), 256, 0, stream>>>(p);
+    if (int code = launch_status()) return code;
+    const size_t lds = (size_t)AdType<KIND>::PARTS * 16 * (p.padded * AdType<KIND>::SIZE + 16);
+    const int64_t groups = cut(s.n, 4 * 16 * AD_VEC<KIND>), share = std::max<int64_t>(1, std::min<int64_t>(groups, s.tiles * groups / 512));
+    const dim3 grid((unsigned)s.m, (unsigned)cut(groups, share));
+    if (s.n < AD_VEC<KIND>) ad_expand_few_kernel<KIND, true><<<grid, 256, lds, stream>>>(p);
+    else ad_expand_few_kernel<KIND, false><<<grid, 256, lds, stream>>>(p);
+    return launch_status();
+  }
+  const AdPlan plan{reinterpret_cast<int32_t*>(ws), s.adapters + 1};
+  char* by_row = ws + s.plan_bytes + s.ticket_bytes + s.split_bytes;
+  int8_t* power = reinterpret_cast<int8_t*>(by_row + s.row_bytes);
+  int code = ad_run_plan(s, in, plan, ws, stream);
   if (code) return code;
-  AdShrink down{in, plan, {{static_cast<const char*>(x), x_stride * s.size, static_cast<const char*>(a->a), s.k, 0, sums}, {}}, 0};
-  if ((code = ad_run_shrink<KIND>(s, down, 1, stream))) return code;
-  AdExpand up{in, plan, sums, a->scale, 0, s.n, 0, static_cast<const char*>(a->b), static_cast<const char*>(y), y_stride * s.size, static_cast<char*>(out), out_stride * s.size};
+  AdShrink down{in, plan, {{xr, x_stride * s.size, static_cast<const char*>(a->a), s.k, 0, 0, nullptr, nullptr, by_row, nullptr, power, nullptr}, {}}, a->scale, 0};
+  if ((code = ad_run_shrink<KIND>(s, down, ws, stream))) return code;
+  AdExpand up{in, plan, by_row, power, s.n, static_cast<const char*>(a->b), yr, y_stride * s.size, to, out_stride * s.size};
   return ad_run_expand<KIND>(s, up, stream);
 }
 
@@ -796,18 +1164,24 @@ template <int KIND>
 static int ad_grads(const hb_adapters* a, const AdShape& s, const AdIndex& in, const void* x, int64_t x_stride, const void* dy, int64_t dy_stride, void* dx, float* da, float* db,
                     char* ws, hipStream_t stream) {
   const AdPlan plan{reinterpret_cast<int32_t*>(ws), s.adapters + 1};
-  float* of_x = reinterpret_cast<float*>(ws + s.plan_bytes);
-  float* of_dy = reinterpret_cast<float*>(ws + s.plan_bytes + s.sums_bytes);
-  float* parts_a = reinterpret_cast<float*>(ws + s.plan_bytes + 2 * s.sums_bytes);
-  float* parts_b = reinterpret_cast<float*>(ws + s.plan_bytes + 2 * s.sums_bytes + up256((size_t)s.slots * s.rank * s.k * 4));
-  int code = ad_run_plan(s, in, plan, stream);
+  char* at = ws + s.plan_bytes + s.ticket_bytes + s.split_bytes;
+  auto take = [&](size_t bytes) { char* here = at; at += bytes; return here; };
+  char* dy_rows = take(s.row_bytes);
+  int8_t* dy_row_power = reinterpret_cast<int8_t*>(take(s.row_power_bytes));
+  char *x_ranks = take(s.rank_bytes), *dy_ranks = take(s.rank_bytes);
+  int8_t *x_power = reinterpret_cast<int8_t*>(take(s.rank_power_bytes)), *dy_power = reinterpret_cast<int8_t*>(take(s.rank_power_bytes));
+  float *part_a = reinterpret_cast<float*>(take(s.part_a_bytes)), *part_b = reinterpret_cast<float*>(take(s.part_b_bytes));
+  int code = ad_run_plan(s, in, plan, ws, stream);
   if (code) return code;
   const char *xr = static_cast<const char*>(x), *dyr = static_cast<const char*>(dy);
-  AdShrink down{in, plan, {{xr, x_stride * s.size, static_cast<const char*>(a->a), s.k, 0, of_x}, {dyr, dy_stride * s.size, static_cast<const char*>(a->b), s.n, 0, of_dy}}, 0};
-  if ((code = ad_run_shrink<KIND>(s, down, 2, stream))) return code;
-  AdExpand up{in, plan, of_dy, a->scale, 0, s.k, 0, static_cast<const char*>(a->a), nullptr, 0, static_cast<char*>(dx), (int64_t)s.k * s.size};
+  AdShrink down{in, plan,
+                {{xr, x_stride * s.size, static_cast<const char*>(a->a), s.k, 0, 0, nullptr, nullptr, nullptr, x_ranks, nullptr, x_power},
+                 {dyr, dy_stride * s.size, static_cast<const char*>(a->b), s.n, 0, 0, nullptr, nullptr, dy_rows, dy_ranks, dy_row_power, dy_power}},
+                a->scale, 0};
+  if ((code = ad_run_shrink<KIND>(s, down, ws, stream))) return code;
+  AdExpand up{in, plan, dy_rows, dy_row_power, s.k, static_cast<const char*>(a->a), nullptr, 0, static_cast<char*>(dx), (int64_t)s.k * s.size};
   if ((code = ad_run_expand<KIND>(s, up, stream))) return code;
-  AdOuter outer{in, plan, {{of_dy, xr, x_stride * s.size, s.k, da, parts_a}, {of_x, dyr, dy_stride * s.size, s.n, db, parts_b}}, a->scale, s.splits, s.unit, 0};
+  AdOuter outer{in, plan, {{dy_ranks, dy_power, xr, x_stride * s.size, s.k, da, part_a}, {x_ranks, x_power, dyr, dy_stride * s.size, s.n, db, part_b}}, s.unit, 0};
   return ad_run_outer<KIND>(s, outer, stream);
 }
 
