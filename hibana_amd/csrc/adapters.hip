@@ -158,8 +158,9 @@ struct AdPlanParams {
 };
 
 // One workgroup: a stable counting sort (rows of a class stay in ascending order, so sums over them are the same every time). HELD: up to AD_HELD rows, whose
-// classes and places among their stretch's rows of the class stay in LDS between the two passes; more are read and counted again. Both loops are short on purpose: what
-// this kernel takes is latency, and unrolled over registers its instructions' own first loads were half of it (8192 rows 12.6 us).
+// classes and places among their stretch's rows of the class stay in LDS between the two passes; more are read and counted again. What this kernel takes is latency:
+// the index comes eight loads a lane side by side (one ahead, 8192 rows took 11.8 us) and waits in LDS for the counting, whose loop is short
+// (unrolled over registers, its own instructions' first loads made it 12.6 us).
 constexpr int AD_HELD = 8192;
 constexpr int AD_COUNTERS = 8000;  // (with the rows held within 64 KB)
 template <bool HELD>
@@ -188,13 +189,25 @@ __global__ __launch_bounds__(1024) void ad_plan_kernel(AdPlanParams p) {
     }
     return place;
   };
-  int ahead = from + lane < upto ? ad_class(p.in, from + lane) : -1;
-  for (int r0 = from; r0 < upto; r0 += 64) {
-    const int c = ahead, r = r0 + lane;
-    if (r0 + 64 < upto) ahead = r + 64 < upto ? ad_class(p.in, r + 64) : -1;
+  // f(rows r0 .. r0 + 63, the lane's class) for the wavefront's rows, in order. Held, the classes lie by row, else in the wavefront's 512 places
+  auto each = [&](auto&& f) {
+    int32_t* batch = HELD ? held + from : held + wave * 512;
+    for (int r0 = from; r0 < upto; r0 += 512) {
+      int c[8];
+#pragma unroll
+      for (int i = 0; i < 8; i++) c[i] = r0 + 64 * i + lane < upto ? ad_class(p.in, r0 + 64 * i + lane) : -1;
+#pragma unroll
+      for (int i = 0; i < 8; i++)
+        if (r0 + 64 * i + lane < upto) batch[64 * i + lane] = c[i];
+#pragma unroll 1
+      for (int i = 0; i < min(512, upto - r0); i += 64) f(r0 + i, r0 + i + lane < upto ? ((volatile int32_t*)batch)[i + lane] : -1);
+      if (HELD) batch += 512;
+    }
+  };
+  each([&](int r0, int c) {
     const int place = places(c);
-    if (HELD && r < upto) held[r] = c | place << 16;
-  }
+    if (HELD && c >= 0) held[r0 + lane] = c | place << 16;
+  });
   __syncthreads();
   // each thread a run of classes: counts over the segments, then prefix sums over the threads
   const int per = (classes + 1023) / 1024, c0 = min((int)threadIdx.x * per, classes), c1 = min(c0 + per, classes);
@@ -244,14 +257,13 @@ __global__ __launch_bounds__(1024) void ad_plan_kernel(AdPlanParams p) {
   }
   __syncthreads();
   int32_t* order = p.plan.order();
-  for (int r0 = from; r0 < upto; r0 += 64) {
-    const int r = r0 + lane;
-    if (HELD) {
-      if (r < upto) order[mine[held[r] & 0xffff] + (held[r] >> 16)] = r;
-    } else {
-      const int c = r < upto ? ad_class(p.in, r) : -1, place = places(c);
-      if (c >= 0) order[place] = r;
-    }
+  if (HELD) {
+    for (int r = from + lane; r < upto; r += 64) order[mine[held[r] & 0xffff] + (held[r] >> 16)] = r;
+  } else {
+    each([&](int r0, int c) {
+      const int place = places(c);
+      if (c >= 0) order[place] = r0 + lane;
+    });
   }
 }
 
@@ -501,6 +513,7 @@ struct AdShrink {
   int chunks;  // of RT x 16 ranks
 };
 constexpr int AD_WAVES = 4;
+constexpr int AD_EXPANDS = 768;   // workgroups of an expansion, about
 __host__ __device__ constexpr int ad_sixteens(int rank) { return (rank + 15) / 16; }
 __host__ __device__ constexpr int ad_thirties(int rank) { return (rank + 31) / 32; }
 
@@ -788,7 +801,7 @@ struct AdExpand {
   int64_t out_stride;
 };
 template <int KIND, bool TINY>
-__global__ __launch_bounds__(256) void ad_expand_kernel(AdExpand p) {
+__global__ __launch_bounds__(256, 3) void ad_expand_kernel(AdExpand p) {
   constexpr int VEC = AD_VEC<KIND>, SIZE = AdType<KIND>::SIZE, PARTS = AdType<KIND>::PARTS;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, group = lane >> 4, col = lane & 15, tile = blockIdx.x >> 1, half = blockIdx.x & 1;
   int c, start;
@@ -913,18 +926,21 @@ __global__ __launch_bounds__(256) void ad_outer_kernel(AdOuter p) {
       for (int d = 1; d < 64; d <<= 1) power[t] = max(power[t], __shfl_xor(power[t], d));
     }
   }
-  // under way: the rows' numbers two tiles ahead, the rows and their sums one
+  // under way: the rows DEPTH tiles ahead, their numbers one more, their sums one
+  constexpr int DEPTH = 1;
   int rows[8];
-  u32x4_t next[8], ahead[RT][WORDS];
+  u32x4_t next[DEPTH][8], ahead[RT][WORDS];
   int shift[RT];
   auto number = [&](int tile) {
     const int from = start + tile * AD_TILE + 8 * group;
 #pragma unroll
     for (int s = 0; s < 8; s++) rows[s] = p.plan.order()[min(from + s, end - 1)];
   };
-  auto load = [&](int tile) {
+  auto load = [&](u32x4_t (&to)[8]) {
 #pragma unroll
-    for (int s = 0; s < 8; s++) next[s] = ad_take<KIND, TINY>(job.v + rows[s] * job.stride, first, job.length);
+    for (int s = 0; s < 8; s++) to[s] = ad_take<KIND, TINY>(job.v + rows[s] * job.stride, first, job.length);
+  };
+  auto sums = [&](int tile) {
 #pragma unroll
     for (int t = 0; t < RT; t++) {  // (behind the adapter's sixteens its last one again)
       const int j = min(t, have - 1);
@@ -934,27 +950,39 @@ __global__ __launch_bounds__(256) void ad_outer_kernel(AdOuter p) {
       if constexpr (KIND == HB_F16) shift[t] = powers[(int64_t)tile * sixteens + j];
     }
   };
+  // (behind the last tile it again: no load behind a branch)
+  const int last = tiles - 1;
   if (wave < tiles) {
     number(wave);
-    load(wave);
-    number(min(wave + 4, tiles - 1));
+#pragma unroll
+    for (int d = 0; d < DEPTH; d++) {
+      load(next[d]);
+      number(min(wave + 4 * (d + 1), last));
+    }
+    sums(wave);
   }
-  for (int tile = wave; tile < tiles; tile += 4) {
-    u32x4_t v[8], s[RT][WORDS];
+  for (int turn = wave; turn < tiles; turn += 4 * DEPTH) {
 #pragma unroll
-    for (int i = 0; i < 8; i++) v[i] = start + tile * AD_TILE + 8 * group + i < end ? next[i] : u32x4_t{0u, 0u, 0u, 0u};
+    for (int d = 0; d < DEPTH; d++) {
+      const int tile = turn + 4 * d;
+      if (d && tile >= tiles) break;
+      u32x4_t v[8], s[RT][WORDS];
 #pragma unroll
-    for (int t = 0; t < RT; t++)
+      for (int i = 0; i < 8; i++) v[i] = start + tile * AD_TILE + 8 * group + i < end ? next[d][i] : u32x4_t{0u, 0u, 0u, 0u};
 #pragma unroll
-      for (int i = 0; i < WORDS; i++) {
-        s[t][i] = ahead[t][i];
-        if constexpr (KIND == HB_F16) s[t][i] = ad_lower(s[t][i], shift[t] - power[t]);
-      }
-    load(min(tile + 4, tiles - 1));  // (behind the last tile it again: no load behind a branch)
-    number(min(tile + 8, tiles - 1));
-    if (RT == 4 && have > 2) ad_products<KIND, RT, RT, WORDS>(s, v, acc);
-    else if (RT >= 2 && have == 2) ad_products<KIND, 2, RT, WORDS>(s, v, acc);
-    else ad_products<KIND, 1, RT, WORDS>(s, v, acc);
+      for (int t = 0; t < RT; t++)
+#pragma unroll
+        for (int i = 0; i < WORDS; i++) {
+          s[t][i] = ahead[t][i];
+          if constexpr (KIND == HB_F16) s[t][i] = ad_lower(s[t][i], shift[t] - power[t]);
+        }
+      load(next[d]);
+      number(min(tile + 4 * (DEPTH + 1), last));
+      sums(min(tile + 4, last));
+      if (RT == 4 && have > 2) ad_products<KIND, RT, RT, WORDS>(s, v, acc);
+      else if (RT >= 2 && have == 2) ad_products<KIND, 2, RT, WORDS>(s, v, acc);
+      else ad_products<KIND, 1, RT, WORDS>(s, v, acc);
+    }
   }
   // D: this lane's columns first .. first + VEC - 1 of ranks 4 group .. + 3 of every sixteen
 #pragma unroll
@@ -1070,7 +1098,7 @@ static bool ad_shape(const hb_adapters* a, int64_t m, bool grads, AdShape& s) {
   s.unit = 4 * AD_TILE;
   if (grads) {
     const int64_t blocks = (cut(a->k, 256 / s.size) + cut(a->n, 256 / s.size)) * cut(a->rank, 64);
-    s.unit = (int)std::min<int64_t>(std::max<int64_t>(4 * AD_TILE, cut(cut(m * blocks, 1024), 4 * AD_TILE) * 4 * AD_TILE), 1 << 20);
+    s.unit = (int)std::min<int64_t>(std::max<int64_t>(4 * AD_TILE, cut(cut(m * blocks, 512), 4 * AD_TILE) * 4 * AD_TILE), 1 << 20);
     s.units = cut(m, s.unit) + classes;
     s.slots = 2 * (m / s.unit);  // an adapter of more than one unit has at most two for every whole `unit` of its rows
     s.part_a_bytes = up256((size_t)s.slots * a->rank * a->k * 4);
@@ -1084,7 +1112,7 @@ static int ad_run_plan(const AdShape& s, const AdIndex& in, const AdPlan& plan, 
   while (p.segments < 16 && (int64_t)(2 * p.segments) * plan.classes <= AD_COUNTERS) p.segments *= 2;
   const size_t lds = (size_t)p.segments * plan.classes * 4;
   if (s.m <= AD_HELD) ad_plan_kernel<true><<<1, 1024, lds + s.m * 4, stream>>>(p);
-  else ad_plan_kernel<false><<<1, 1024, lds, stream>>>(p);
+  else ad_plan_kernel<false><<<1, 1024, lds + 16 * 512 * 4, stream>>>(p);
   return launch_status();
 }
 
@@ -1109,7 +1137,7 @@ static int ad_run_shrink(const AdShape& s, AdShrink& p, char* ws, hipStream_t st
 template <int KIND>
 static int ad_run_expand(const AdShape& s, AdExpand& p, hipStream_t stream) {
   const int64_t groups = cut(p.n, 4 * 16 * AD_VEC<KIND>);
-  const int64_t share = std::max<int64_t>(1, std::min<int64_t>(groups, 2 * s.tiles * groups / 1024));
+  const int64_t share = std::max<int64_t>(1, std::min<int64_t>(groups, cut(s.m, 16) * groups / AD_EXPANDS));
   const dim3 grid((unsigned)(2 * s.tiles), (unsigned)cut(groups, share));
   if (p.n < AD_VEC<KIND>) ad_expand_kernel<KIND, true><<<grid, 256, 0, stream>>>(p);
   else ad_expand_kernel<KIND, false><<<grid, 256, 0, stream>>>(p);
