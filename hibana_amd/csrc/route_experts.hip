@@ -9,6 +9,8 @@
 //
 // The choice is not one of FP32's roundings: without a bias c grows with l, and the logits' own order decides. Else, and between groups, it is that of the
 // formula in FP64; FP32 decides where it can: if two c next to each other in rank are nearer than its error can tell apart, the row is chosen again.
+#include <type_traits>
+
 #include "route.hpp"
 
 namespace hb {
@@ -22,7 +24,8 @@ struct RouteExperts {
   const int32_t* slots;  // row r is real iff slots[r / steps] != 0 (null: every row)
   int m, e, k, steps;
   int groups, kept, size;  // size: experts a group
-  int lanes, per;          // lanes a group (a power of two), experts a lane
+  int lanes, per, shift;   // lanes a group (a power of two, 2^shift), experts a lane
+  int by_per;              // 2^16 / per, up: a tag (below 1024) times it is the tag's lane in units of 2^16
   int renorm;
   float scale;
   int32_t* ids;
@@ -47,23 +50,47 @@ __device__ __forceinline__ T route_max(T a, T b) { return a > b ? a : b; }
 template <typename T>
 __device__ __forceinline__ T route_min(T a, T b) { return a < b ? a : b; }
 
+// e^x and 1 / x. In FP32 by the device's own instructions: this is for the choice, whose error bound counts them (x log2(e) rounded: x 2^-24 of e^x, at most 2^-24 in all
+// where e^x is below 1; the exponential and the reciprocal an ulp each).
+__device__ __forceinline__ float route_exp(float x) { return __expf(x); }
+__device__ __forceinline__ double route_exp(double x) { return exp(x); }
+__device__ __forceinline__ float route_inverse(float x) { return __builtin_amdgcn_rcpf(x); }
+__device__ __forceinline__ double route_inverse(double x) { return 1.0 / x; }
+__device__ __forceinline__ float route_sum(float x) { return wave_sum(x); }
+__device__ __forceinline__ double route_sum(double x) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) x += __shfl_xor(x, d);
+  return x;
+}
+
 // Scores of the lane's experts (a softmax with an infinite logit: those that have one).
 template <bool SIGMOID, typename T, int PER>
 __device__ __forceinline__ void route_scores(const float (&l)[PER], uint32_t open, float most, T (&s)[PER]) {
   if (SIGMOID) {
 #pragma unroll
-    for (int j = 0; j < PER; j++) s[j] = T(1) / (T(1) + exp(-T(l[j])));
+    for (int j = 0; j < PER; j++) s[j] = route_inverse(T(1) + route_exp(-T(l[j])));
   } else {
     T sum = 0;
 #pragma unroll
     for (int j = 0; j < PER; j++) {
-      s[j] = !(open >> j & 1) ? T(0) : most == INFINITY ? T(l[j] == INFINITY ? 1 : 0) : exp(T(l[j]) - T(most));
+      s[j] = !(open >> j & 1) ? T(0) : most == INFINITY ? T(l[j] == INFINITY ? 1 : 0) : route_exp(T(l[j]) - T(most));
       sum += s[j];
     }
+    sum = route_sum(sum);
+    const T by = sum > T(0) ? route_inverse(sum) : T(0);
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d);
-#pragma unroll
-    for (int j = 0; j < PER; j++) s[j] = sum > T(0) ? s[j] / sum : T(0);
+    for (int j = 0; j < PER; j++) s[j] *= by;
+  }
+}
+
+// A value of lane ^ D's (or, D = 4 and 8, its mirror's in eight and sixteen lanes, which holds the same where the smaller ones have been merged).
+template <int D, typename T>
+__device__ __forceinline__ T route_other(T x) {
+  if constexpr (sizeof(T) == 4 && D <= 8) {
+    constexpr int HOW = D == 1 ? 0xB1 : D == 2 ? 0x4E : D == 4 ? 0x141 : 0x140;
+    return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), HOW, 0xF, 0xF, false));
+  } else {
+    return __shfl_xor(x, D);
   }
 }
 
@@ -78,27 +105,26 @@ __device__ __forceinline__ bool route_groups(const RouteExperts& p, const T (&c)
     b2 = route_max(b2, route_min(b1, v));
     b1 = route_max(b1, v);
   }
-  for (int d = 1; d < p.lanes; d <<= 1) {
-    const T o1 = __shfl_xor(b1, d), o2 = __shfl_xor(b2, d);
+  auto merge = [&](auto d) {
+    if (decltype(d)::value >= p.lanes) return;  // uniform
+    const T o1 = route_other<decltype(d)::value>(b1), o2 = route_other<decltype(d)::value>(b2);
     b2 = route_max(route_min(b1, o1), route_max(b2, o2));
     b1 = route_max(b1, o1);
-  }
+  };
+  merge(std::integral_constant<int, 1>{}), merge(std::integral_constant<int, 2>{}), merge(std::integral_constant<int, 4>{});
+  merge(std::integral_constant<int, 8>{}), merge(std::integral_constant<int, 16>{}), merge(std::integral_constant<int, 32>{});
   const T mine = b2 == none ? b1 : b1 + b2;
-  const int group = lane / p.lanes;
+  const int group = lane >> p.shift;
   int ahead = 0;
   for (int g = 0; g < p.groups; g++) {
-    const T other = route_lane(mine, g * p.lanes);
+    const T other = route_lane(mine, g << p.shift);
     ahead += other > mine || (other == mine && g < group) ? 1 : 0;
   }
-  const bool real = group < p.groups, kept = real && ahead < p.kept;
-  T worst = kept ? mine : T(INFINITY), best = real && !kept ? mine : none;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    worst = route_min(worst, __shfl_xor(worst, d));
-    best = route_max(best, __shfl_xor(best, d));
-  }
+  // the ranks are a permutation: the last kept group and the first other one are there
+  const uint64_t last = __ballot(group < p.groups && ahead == p.kept - 1), next = __ballot(group < p.groups && ahead == p.kept);
+  const T worst = route_lane(mine, __builtin_ctzll(last)), best = route_lane(mine, __builtin_ctzll(next));
   gap = best == none || worst == T(INFINITY) ? T(INFINITY) : worst - best;
-  return kept;
+  return group < p.groups && ahead < p.kept;
 }
 
 // The row's choice in FP64: lane s < k gets selection s's tag (lane * per + register), or -1.
@@ -147,8 +173,8 @@ __global__ __launch_bounds__(256) void route_experts_kernel(RouteExperts p) {
     return;
   }
   const char* row = static_cast<const char*>(p.logits) + (int64_t)r * p.stride * (KIND == HB_F32 ? 4 : 2);
-  const int within = lane % p.lanes * p.per, first = lane / p.lanes * p.size + within;
-  const int have = lane / p.lanes < p.groups ? max(min(p.per, p.size - within), 0) : 0;
+  const int within = (lane & (p.lanes - 1)) * p.per, first = (lane >> p.shift) * p.size + within;
+  const int have = (lane >> p.shift) < p.groups ? max(min(p.per, p.size - within), 0) : 0;
   float l[PER], bias[PER];
 #pragma unroll
   for (int j = 0; j < PER; j++) l[j] = route_logit<KIND>(row, min(first + j, p.e - 1)) + 0.f;  // (-0 counts as 0)
@@ -190,8 +216,8 @@ __global__ __launch_bounds__(256) void route_experts_kernel(RouteExperts p) {
       c[j] += bias[j];
       if (open >> j & 1) largest = fmaxf(largest, fabsf(c[j]));
     }
-    // What two sums may seem apart, or in the wrong order, by FP32's roundings: a score is off by 2^-19 of the largest at most (the exponential, the sum over
-    // PER registers and 64 lanes, the division), a sum with the bias by 2^-24 of itself; twice for two, and twice that
+    // What two sums may seem apart, or in the wrong order, by FP32's roundings: a score is off by 2^-19 of the largest at most (its argument, the exponential, the sum over
+    // PER registers and 64 lanes, the reciprocal and the product: 28 halves of an ulp), a sum with the bias by 2^-24 of itself; twice for two, and twice that
     const float off = 0x1p-17f * (SIGMOID ? 1.f : wave_max(size)) + 0x1p-22f * wave_max(largest);
     uint32_t left = open;
     if (p.kept < p.groups) {
@@ -216,13 +242,13 @@ __global__ __launch_bounds__(256) void route_experts_kernel(RouteExperts p) {
     if (__builtin_expect(near, 0)) tag = route_in_64_bits<SIGMOID, PER>(p, l, bias, counted, open, most, lane);
   }
   if (lane >= p.k) tag = -1;
-  const int holder = tag / p.per, id = tag < 0 ? p.e : holder / p.lanes * p.size + holder % p.lanes * p.per + tag % p.per;
+  const int holder = tag * p.by_per >> 16, id = tag < 0 ? p.e : (holder >> p.shift) * p.size + (holder & (p.lanes - 1)) * p.per + tag - holder * p.per;
   const float mine = tag < 0 ? -INFINITY : route_logit<KIND>(row, id);
   float w;
   if (p.renorm) {
     const float top = wave_max(mine);
     if (SIGMOID) {
-      w = top < 0.f ? expf(mine - top) / (1.f + expf(mine)) : 1.f / (1.f + expf(-mine));
+      w = __builtin_amdgcn_readfirstlane(top < 0.f) ? expf(mine - top) / (1.f + expf(mine)) : 1.f / (1.f + expf(-mine));
     } else {
       w = expf(mine - top);
     }
@@ -270,7 +296,7 @@ __global__ __launch_bounds__(256) void route_grad_kernel(RouteGrad p) {
   float g, most = 0.f, sum = 0.f, all = 0.f;
   if (p.renorm) {
     const float top = wave_max(mine);
-    float w = SIGMOID ? top < 0.f ? expf(mine - top) / (1.f + expf(mine)) : 1.f / (1.f + expf(-mine)) : expf(mine - top);
+    float w = SIGMOID ? __builtin_amdgcn_readfirstlane(top < 0.f) ? expf(mine - top) / (1.f + expf(mine)) : 1.f / (1.f + expf(-mine)) : expf(mine - top);
     if (id < 0 || top == -INFINITY) w = 0.f;
     const float total = wave_sum(w);
     if (total > 0.f) w /= total;  // (a NaN stays one)
@@ -357,10 +383,11 @@ extern "C" int hb_route_experts(const void* logits, int type, int64_t stride, in
   if (type < HB_BF16 || type > HB_F32 || (scoring != HB_SOFTMAX && scoring != HB_SIGMOID) || m <= 0 || e <= 0 || e > 64 * ROUTE_PER_LANE || k <= 0 || k > ROUTE_MOST_K ||
       groups <= 0 || groups > 64 || e % groups || kept <= 0 || kept > groups || k > kept * (e / groups) || steps <= 0 || (m > 1 && stride < e))
     return HB_EINVAL;
-  RouteExperts p{logits, stride, bias, slots, m, e, k, steps, groups, kept, e / groups, 1, 0, renorm != 0, scale, ids, weights};
-  while (2 * p.lanes * groups <= 64) p.lanes *= 2;
+  RouteExperts p{logits, stride, bias, slots, m, e, k, steps, groups, kept, e / groups, 1, 0, 0, 0, renorm != 0, scale, ids, weights};
+  while (2 * p.lanes * groups <= 64) p.lanes *= 2, p.shift++;
   p.per = (p.size + p.lanes - 1) / p.lanes;
   if (p.per > ROUTE_PER_LANE) return HB_EINVAL;
+  p.by_per = 65536 / p.per + 1;
   if (!aligned(logits, type == HB_F32 ? 4 : 2) || !aligned(bias, 4) || !aligned(slots, 4) || !aligned(ids, 4) || !aligned(weights, 4)) return HB_EINVAL;
   const hipStream_t s = as_stream(stream);
   if (scoring == HB_SIGMOID)

@@ -18,6 +18,7 @@ from hibana_amd import _lib
 from hibana_amd.kernels.mxfp4 import TYPES
 
 MOST, MOST_RANK = 4096, 256  # what the kernels take: adapters of a pool, their rank
+INDEX = {torch.int32: 4, torch.int64: 8}
 
 
 class Adapters:
@@ -114,38 +115,45 @@ class Adapters:
 def _rows(t: torch.Tensor, width: int, pool: Adapters, what: str) -> torch.Tensor:
     if t.dtype != pool.a.dtype or t.ndim != 2 or t.shape[1] != width:
         raise ValueError(f"{what}: {pool.a.dtype} [M, {width}]")
-    return t if t.stride(1) == 1 and t.stride(0) >= width or t.shape[0] == 1 and t.stride(1) == 1 else t.contiguous()
+    if t.is_contiguous():
+        return t
+    return t if t.stride(1) == 1 and (t.stride(0) >= width or t.shape[0] == 1) else t.contiguous()
 
 
-def _index(index: torch.Tensor, m: int, what: str) -> torch.Tensor:
-    if index.dtype not in (torch.int32, torch.int64) or index.ndim != 1 or index.shape[0] != m:
+def _stride(t: torch.Tensor, width: int) -> int:
+    return width if t.is_contiguous() else max(t.stride(0), width)  # (that of a single row is nobody's)
+
+
+def _operands(v: torch.Tensor, x: torch.Tensor, pool: Adapters, index: torch.Tensor, what: str):
+    """The rows of v [M, N] and x [M, K] and the index as the library takes them, the number of rows and the current stream."""
+    v, x = _rows(v, pool.b.shape[2], pool, what), _rows(x, pool.a.shape[2], pool, what)
+    m = v.shape[0]
+    if x.shape[0] != m:
+        raise ValueError(f"{what}: as many rows of x as there are results")
+    if index.dtype not in INDEX or index.ndim != 1 or index.shape[0] != m:
         raise ValueError(f"{what}: an int32 or int64 index [{m}]")
-    return index if index.is_contiguous() else index.contiguous()
-
-
-def _stride(t: torch.Tensor) -> int:
-    return max(t.stride(0), t.shape[1])  # (that of a single row is nobody's)
+    if not index.is_contiguous():
+        index = index.contiguous()
+    return v, x, index, m, _lib.stream_of(v, x, index, pool.a)
 
 
 def _add(y: torch.Tensor, x: torch.Tensor, pool: Adapters, index: torch.Tensor, out: torch.Tensor | None) -> torch.Tensor:
-    what = "adapters.add"
-    yr, xr = _rows(y, pool.out_features, pool, what), _rows(x, pool.in_features, pool, what)
-    m = yr.shape[0]
-    if xr.shape[0] != m:
-        raise ValueError(f"{what}: as many rows of x as of y")
-    ix = _index(index, m, what)
-    stream = _lib.stream_of(yr, xr, ix, pool.a)
+    yr, xr, ix, m, stream = _operands(y, x, pool, index, "adapters.add")
+    k, n = pool.a.shape[2], pool.b.shape[2]
     if out is None:
-        out = yr.new_empty((m, yr.shape[1]))
-    elif out.dtype != yr.dtype or out.shape != yr.shape or out.stride(1) != 1 or (m > 1 and out.stride(0) < out.shape[1]) or out.device != yr.device:
-        raise ValueError(f"{what}: out like y, its rows contiguous")
+        out = yr.new_empty((m, n))
+        to = n
+    elif out.dtype != yr.dtype or out.shape != yr.shape or out.stride(1) != 1 or (m > 1 and out.stride(0) < n) or out.device != yr.device:
+        raise ValueError("adapters.add: out like y, its rows contiguous")
+    else:
+        to = _stride(out, n)
     if m:
         need = pool.room(m, 0)
         ws = yr.new_empty(need, dtype=torch.uint8)  # (of the capture's own pool in a captured call)
-        code = _lib.lib().hb_adapters_add(pool.struct(), xr.data_ptr(), _stride(xr), yr.data_ptr(), _stride(yr), ix.data_ptr(), ix.element_size(), m, out.data_ptr(), _stride(out),
+        code = _lib.lib().hb_adapters_add(pool.struct(), xr.data_ptr(), _stride(xr, k), yr.data_ptr(), _stride(yr, n), ix.data_ptr(), INDEX[ix.dtype], m, out.data_ptr(), to,
                                           ws.data_ptr(), need, stream)
         if code:
-            _lib.check(code, what)
+            _lib.check(code, "adapters.add")
     return out
 
 
@@ -186,21 +194,16 @@ def grads(dy: torch.Tensor, x: torch.Tensor, pool: Adapters, index: torch.Tensor
     """The gradients of `add` given that of its result, dy [M, N]: (dx [M, K] of the pool's type, da FP32 [adapters, rank, K], db FP32 [adapters, rank,
     N]). An adapter that no row has gets zeros, as do the rows behind an adapter's rank; y's gradient is dy itself. Sums over rows are in a
     fixed order: the same call gives the same bits."""
-    what = "adapters.grads"
-    dyr, xr = _rows(dy, pool.out_features, pool, what), _rows(x, pool.in_features, pool, what)
-    m = dyr.shape[0]
-    if xr.shape[0] != m:
-        raise ValueError(f"{what}: as many rows of x as of dy")
-    ix = _index(index, m, what)
-    stream = _lib.stream_of(dyr, xr, ix, pool.a)
-    dx = xr.new_empty((m, xr.shape[1]))
+    dyr, xr, ix, m, stream = _operands(dy, x, pool, index, "adapters.grads")
+    k, n = pool.a.shape[2], pool.b.shape[2]
+    dx = xr.new_empty((m, k))
     if not m:
         return dx, torch.zeros(pool.a.shape, dtype=torch.float32, device=xr.device), torch.zeros(pool.b.shape, dtype=torch.float32, device=xr.device)
     da, db = xr.new_empty(pool.a.shape, dtype=torch.float32), xr.new_empty(pool.b.shape, dtype=torch.float32)
     need = pool.room(m, 1)
     ws = xr.new_empty(need, dtype=torch.uint8)
-    code = _lib.lib().hb_adapters_grads(pool.struct(), xr.data_ptr(), _stride(xr), dyr.data_ptr(), _stride(dyr), ix.data_ptr(), ix.element_size(), m, dx.data_ptr(), da.data_ptr(),
+    code = _lib.lib().hb_adapters_grads(pool.struct(), xr.data_ptr(), _stride(xr, k), dyr.data_ptr(), _stride(dyr, n), ix.data_ptr(), INDEX[ix.dtype], m, dx.data_ptr(), da.data_ptr(),
                                         db.data_ptr(), ws.data_ptr(), need, stream)
     if code:
-        _lib.check(code, what)
+        _lib.check(code, "adapters.grads")
     return dx, da, db

@@ -192,7 +192,7 @@ class Routing:
 def _route_logits(logits: torch.Tensor, scoring: str, what: str) -> torch.Tensor:
     if logits.dtype not in mxfp4.TYPES or logits.ndim != 2 or scoring not in SCORING:
         raise ValueError(f"{what}: BF16, FP16 or FP32 logits [M, E], scoring softmax or sigmoid")
-    return logits if logits.stride(1) == 1 and logits.stride(0) >= logits.shape[1] else logits.contiguous()
+    return logits if logits.is_contiguous() or (logits.stride(1) == 1 and logits.stride(0) >= logits.shape[1]) else logits.contiguous()
 
 
 def _route_experts(logits: torch.Tensor, k: int, scoring: str, bias, groups: int, kept: int, renormalize: bool, scale: float, slots, steps: int):
@@ -201,12 +201,15 @@ def _route_experts(logits: torch.Tensor, k: int, scoring: str, bias, groups: int
     m, e = lg.shape
     if not (1 <= e <= 1024 and 1 <= kept <= groups <= 64 and e % groups == 0 and 1 <= k <= min(63, kept * (e // groups))):
         raise ValueError(f"{what}: up to 1024 experts in up to 64 groups of a size, k up to 63 and the experts of the kept groups")
-    if bias is not None and (bias.numel() != e or bias.ndim != 1 or not bias.is_floating_point()):
-        raise ValueError(f"{what}: a bias [E]")
+    bias32 = sl = None
+    if bias is not None:
+        if bias.ndim != 1 or bias.shape[0] != e or not bias.is_floating_point():
+            raise ValueError(f"{what}: a bias [E]")
+        bias32 = bias if bias.dtype == torch.float32 and bias.is_contiguous() else bias.float().contiguous()
     if steps < 1 or m % steps or (slots is not None and slots.numel() < m // steps):
         raise ValueError(f"{what}: whole requests of `steps` rows, a slot for every request")
-    bias32 = None if bias is None else bias.float().contiguous()
-    sl = None if slots is None else slots.to(torch.int32).contiguous()
+    if slots is not None:
+        sl = slots if slots.dtype == torch.int32 and slots.is_contiguous() else slots.to(torch.int32).contiguous()
     stream = _lib.stream_of(lg, *(t for t in (bias32, sl) if t is not None))
     ids, weights = lg.new_empty((m, k), dtype=torch.int32), lg.new_empty((m, k), dtype=torch.float32)
     if m:
