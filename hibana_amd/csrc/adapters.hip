@@ -699,17 +699,21 @@ __global__ __launch_bounds__(256) void ad_expand_few_kernel(AdFew p) {
   if (rank == 0 && p.y == p.out) return;
   const int stride = gridDim.y * 4;
   int block = blockIdx.y * 4 + wave;
-  u32x4_t y[4], v[8], next[8];
-  int64_t rows[4];
+  u32x4_t y[4], v[2][8];
+  int rows[4];
 #pragma unroll
   for (int i = 0; i < 4; i++) rows[i] = __shfl(row, 4 * group + i);
   auto base = [&](int first) {  // (rows behind the last: the first again)
 #pragma unroll
     for (int i = 0; i < 4; i++) y[i] = ad_take<KIND, TINY>(p.y + rows[i] * p.y_stride, first, p.n);
   };
-  auto load = [&](u32x4_t (&to)[8], int first, int r0) {
+  // what is under way: (block, 32 ranks) one after another, two ahead of the products (behind the last block the row's end: no load behind a branch)
+  int ahead = block * 16 * VEC + col * VEC, ahead_rank = 0;
+  auto load = [&](u32x4_t (&to)[8]) {
 #pragma unroll
-    for (int s = 0; s < 8; s++) to[s] = ad_take<KIND, TINY>(p.b + ((int64_t)c * p.in.rank + min(r0 + 8 * group + s, rank - 1)) * p.n * SIZE, first, p.n);
+    for (int s = 0; s < 8; s++) to[s] = ad_take<KIND, TINY>(p.b + ((int64_t)c * p.in.rank + min(ahead_rank + 8 * group + s, rank - 1)) * p.n * SIZE, min(ahead, p.n), p.n);
+    ahead_rank += 32;
+    if (ahead_rank >= rank) ahead_rank = 0, ahead += stride * 16 * VEC;
   };
   base(block * 16 * VEC + col * VEC);
   if (rank == 0) {  // no adapter: the rows as they are
@@ -718,11 +722,12 @@ __global__ __launch_bounds__(256) void ad_expand_few_kernel(AdFew p) {
 #pragma unroll
       for (int i = 0; i < 4; i++)
         if (4 * group + i < count) ad_put<KIND, TINY>(p.out + rows[i] * p.out_stride, y[i], first, p.n);
-      base(first + stride * 16 * VEC);
+      base(min(first + stride * 16 * VEC, p.n));
     }
     return;
   }
-  load(v, block * 16 * VEC + col * VEC, 0);
+  load(v[0]);
+  load(v[1]);
   {  // the rows' sums, joined over the splits and scaled: sixteen threads a row
     const int place = threadIdx.x / 16, lane_of = threadIdx.x % 16;
     const float* sums = p.sums + (int64_t)__shfl(row, place) * p.in.rank;
@@ -751,7 +756,7 @@ __global__ __launch_bounds__(256) void ad_expand_few_kernel(AdFew p) {
     const int used = (rank + 31) & ~31;
 #pragma unroll 2
     for (int r = lane_of; r < used; r += 16) {
-      const float to = r < rank ? sum(r) * unit : 0.f;
+      const float to = r < rank && place < count ? sum(r) * unit : 0.f;
       if constexpr (SIZE == 4) {
         reinterpret_cast<float*>(staged)[place * pitch + r] = to;
       } else {
@@ -763,27 +768,33 @@ __global__ __launch_bounds__(256) void ad_expand_few_kernel(AdFew p) {
     }
   }
   __syncthreads();
-  // (block, 32 ranks) one after another, the next one's matrix under way; idle lanes behind the last column take part in the products
-  for (; block * (16 * VEC) < p.n; block += stride) {
-    const int first = block * 16 * VEC + col * VEC;
-    f32x4_t acc[1][VEC] = {};
-    for (int r0 = 0; r0 < rank; r0 += 32) {
-      const bool on = r0 + 32 < rank;
-      load(next, on ? first : first + stride * 16 * VEC, on ? r0 + 32 : 0);
+  f32x4_t acc[1][VEC] = {};
+  int r0 = 0;
+  for (bool more = block * (16 * VEC) < p.n; more;) {  // (idle lanes behind the last column take part in the products)
+#pragma unroll
+    for (int d = 0; d < 2; d++) {
+      if (!more) break;
       constexpr int WORDS = SIZE == 4 ? 2 : PARTS;
       u32x4_t s[1][WORDS];
 #pragma unroll
       for (int i = 0; i < WORDS; i++)
         s[0][i] = *reinterpret_cast<const u32x4_t*>(SIZE == 4 ? staged + (col * pitch + r0 + 8 * group + 4 * i) * 4 : staged + ((i * 16 + col) * pitch + r0 + 8 * group) * 2);
-      ad_products<KIND, 1, 1, WORDS>(s, v, acc);
+      ad_products<KIND, 1, 1, WORDS>(s, v[d], acc);
+      load(v[d]);
+      r0 += 32;
+      if (r0 < rank) continue;
+      const int first = block * 16 * VEC + col * VEC;
 #pragma unroll
-      for (int i = 0; i < 8; i++) v[i] = next[i];
+      for (int i = 0; i < 4; i++)
+        if (4 * group + i < count)
+          ad_put<KIND, TINY>(p.out + rows[i] * p.out_stride, ad_result<KIND>(y[i], acc[0], i, KIND == HB_F16 ? ad_pow2(power[4 * group + i]) : 1.0f), first, p.n);
+#pragma unroll
+      for (int j = 0; j < VEC; j++) acc[0][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+      r0 = 0;
+      block += stride;
+      more = block * (16 * VEC) < p.n;
+      base(min(first + stride * 16 * VEC, p.n));
     }
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-      if (4 * group + i < count)
-        ad_put<KIND, TINY>(p.out + rows[i] * p.out_stride, ad_result<KIND>(y[i], acc[0], i, KIND == HB_F16 ? ad_pow2(power[4 * group + i]) : 1.0f), first, p.n);
-    base(first + stride * 16 * VEC);
   }
 }
 
@@ -1088,7 +1099,6 @@ static bool ad_shape(const hb_adapters* a, int64_t m, bool grads, AdShape& s) {
   s.share = (int)std::max<int64_t>(2 * AD_WAVES, cut((units_x + units_dy) * cut(m, AD_TILE) * s.chunks, 1024));
   s.splits_x = (int)cut(units_x, s.share), s.splits_dy = (int)cut(units_dy, s.share);
   s.tickets = s.tiles * s.chunks * (grads ? 2 : 1);
-  s.ticket_bytes = up256((size_t)s.tickets * 4);
   s.split_bytes = up256((size_t)s.tiles * s.chunks * ((s.splits_x > 1 ? s.splits_x : 0) + (s.splits_dy > 1 ? s.splits_dy : 0)) * AD_TILE * 16 * s.rt * 4);
   const int parts = a->type == HB_F32 ? 1 : 2, outer = a->type == HB_BF16 ? 3 : parts;
   s.row_bytes = up256((size_t)s.tiles * ad_thirties(a->rank) * parts * 1024 * s.size);
@@ -1104,6 +1114,7 @@ static bool ad_shape(const hb_adapters* a, int64_t m, bool grads, AdShape& s) {
     s.part_a_bytes = up256((size_t)s.slots * a->rank * a->k * 4);
     s.part_b_bytes = up256((size_t)s.slots * a->rank * a->n * 4);
   }
+  s.ticket_bytes = up256((size_t)s.tickets * 4);
   return true;
 }
 
@@ -1171,7 +1182,7 @@ static int ad_add(const hb_adapters* a, const AdShape& s, const AdIndex& in, con
     ad_shrink_few_kernel<KIND><<<dim3((unsigned)s.m, (unsigned)s.splits, (unsigned)ad_sixteens(s.rank)), 256, 0, stream>>>(p);
     if (int code = launch_status()) return code;
     const size_t lds = (size_t)AdType<KIND>::PARTS * 16 * (p.padded * AdType<KIND>::SIZE + 16);
-    const int64_t groups = cut(s.n, 4 * 16 * AD_VEC<KIND>), share = std::max<int64_t>(1, std::min<int64_t>(groups, s.tiles * groups / 512));
+    const int64_t groups = cut(s.n, 4 * 16 * AD_VEC<KIND>), share = std::max<int64_t>(1, std::min<int64_t>(groups, s.tiles * groups / 256));
     const dim3 grid((unsigned)s.m, (unsigned)cut(groups, share));
     if (s.n < AD_VEC<KIND>) ad_expand_few_kernel<KIND, true><<<grid, 256, lds, stream>>>(p);
     else ad_expand_few_kernel<KIND, false><<<grid, 256, lds, stream>>>(p);

@@ -18,7 +18,8 @@ The block is assembled from tensors already on the device (a loader's job ends t
 experts' row order (`shared_from_linears`). Budgeted expert selection (HIBANA_MOE_KEEP / HIBANA_MOE_BUDGET /
 HIBANA_MOE_BUDGET_PER_REQUEST of the reference's configuration) is the constructor's `keep` / `budget` / `per_request`:
 decode and verify forwards then read at most a budget of distinct experts (`ops.route_budget`); slots left over name no
-expert, which the 3-bit kernels skip.
+expert, which the 3-bit kernels skip. A layer with another routing rule (`ops.Routing`: sigmoid scores, a bias for balance, groups,
+plain or scaled weights) holds it as `routing`: the logits are then routed by `ops.route_experts`, and the experts take its ids and weights.
 """
 from __future__ import annotations
 
@@ -50,15 +51,18 @@ def shared_from_linears(gate_up: w3.W3Weight, down: w3.W3Weight) -> w3_moe.W3Exp
 class MoeLayer:
     MIN_GUARANTEE = 2  # hibana/model/flashnext/moe.py:146-149
     MIN_CAP = 16
+    routing: ops.Routing | None = None
 
     def __init__(self, router: torch.Tensor, shared_gate: torch.Tensor, experts: w3_moe.W3Experts | mxfp4_moe.Mxfp4Experts, topk: int, shared: w3_moe.W3Experts | None = None,
-                 shared_gate_up=None, shared_down=None, keep: int = 0, budget: int = 0, per_request: int = 0):
+                 shared_gate_up=None, shared_down=None, keep: int = 0, budget: int = 0, per_request: int = 0, routing: ops.Routing | None = None):
         """router BF16 [E, H]; shared_gate [1, H] or [H] (the shared expert's sigmoid gate); `experts` this rank's 3-bit (or
         microscaled four-bit) experts (a range base .. base + experts - 1 of the E); the shared expert as `shared`, or as the two linears
         `shared_gate_up` / `shared_down` with 3-bit copies attached (`.w3`). `keep` (below topk; topk or more, or 0, is
         the served route): each token's own top experts in decode and verify forwards; with `budget`, the cap on the
         distinct experts such a forward reads, `per_request` its share a request
-        (hibana/model/flashnext/moe.py:86-93)."""
+        (hibana/model/flashnext/moe.py:86-93). `routing`: the rule in place of the softmax's, without a `keep`."""
+        if routing is not None and (keep or budget or per_request):
+            raise ValueError("MoeLayer: budgeted selection goes by the softmax rule")
         if keep < 0 or budget < 0 or per_request < 0:
             raise ValueError(f"keep {keep}, budget {budget}, per_request {per_request}: not negative")
         self.router = router.contiguous()
@@ -67,6 +71,7 @@ class MoeLayer:
         self.keep = keep if keep < topk else 0
         self.budget = budget if self.keep else 0
         self.per_request = per_request
+        self.routing = routing
         self.shared_gate = shared_gate.float().reshape(1, -1).contiguous()
         self.shared_gate_vec = self.shared_gate.reshape(-1)
         self.w3 = self.mxfp4 = self.shared = self.shared_mlp = None
@@ -135,6 +140,8 @@ class MoeLayer:
         `ops.route_budget`."""
         logits = torch.mm(x, self.router.T)
         slots, steps = self._padding(ctx)
+        if self.routing is not None:
+            return self.routing(logits, self.topk, slots, steps)
         if self.selects(ctx):
             if not self.budget:
                 return ops.route_topk(logits, self.keep)
@@ -173,6 +180,9 @@ class MoeLayer:
             pairs = w3_moe.w3_moe(self.w3, x, ids, weights, pairs=True, pairs_bf16=x.shape[0] >= w3_moe.WIDE_ROWS, experts_total=self.experts)
             shared = ops.nvfp4_linear(ops.silu_and_mul(ops.nvfp4_linear(x, self.shared_gate_up)), self.shared_down)
             return ops.moe_combine_pairs(pairs, ids, weights, shared, x, self.shared_gate_vec, self.w3.base, self.w3.experts)
+        if self.routing is not None:
+            ids, weights = self.route(x, ctx)
+            return w3_moe.moe_layer(self.w3, x, ids, weights, shared=self.shared, gate_vec=self.shared_gate_vec, experts_total=self.experts)
         # router product, routing (or the budgeted selection), plan, both streams and the combine as one chain
         slots, steps = self._padding(ctx)
         if not self.selects(ctx):
