@@ -12,7 +12,7 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "stream_common.hpp"
+#include "route.hpp"
 
 namespace hb {
 
@@ -26,6 +26,7 @@ constexpr int AD_MOST = 4096;      // adapters
 constexpr int AD_RANK = 256;
 constexpr int AD_MAX_ROWS = 1 << 24;
 constexpr int AD_LONGEST = 1 << 22;  // of either axis
+constexpr int64_t AD_STRIDE = 0xffffffffll;  // bytes from row to row
 
 template <int KIND> struct AdType;
 template <> struct AdType<HB_BF16> { static constexpr int SIZE = 2, PARTS = 2, OUTER = 3; };  // parts that FP32 values are cut into
@@ -80,6 +81,10 @@ __device__ __forceinline__ void ad_store(char* at, const u32x4_t& v, int64_t lef
     }
   }
 }
+
+// Row r of rows `pitch` bytes apart: one multiply-add of 64 bits (three of a 64-bit pitch's, sixteen cycles each).
+__device__ __forceinline__ const char* ad_row(const char* rows, int r, uint32_t pitch) { return rows + (uint64_t)(uint32_t)r * pitch; }
+__device__ __forceinline__ char* ad_row(char* rows, int r, uint32_t pitch) { return rows + (uint64_t)(uint32_t)r * pitch; }
 
 // A lane's sixteen bytes of a row of n elements, of which `first` is the lane's first: behind the row's end its last sixteen bytes, so that no load is behind a
 // branch (the compiler waits for all that is under way where it does not know how many loads are). TINY: rows shorter than that, element by element.
@@ -157,61 +162,12 @@ struct AdPlanParams {
   int64_t clear;
 };
 
-// One workgroup: a stable counting sort (rows of a class stay in ascending order, so sums over them are the same every time). HELD: up to AD_HELD rows, whose
-// classes and places among their stretch's rows of the class stay in LDS between the two passes; more are read and counted again. What this kernel takes is latency:
-// the index comes eight loads a lane side by side (one ahead, 8192 rows took 11.8 us) and waits in LDS for the counting, whose loop is short
-// (unrolled over registers, its own instructions' first loads made it 12.6 us).
-constexpr int AD_HELD = 8192;
-constexpr int AD_COUNTERS = 8000;  // (with the rows held within 64 KB)
-template <bool HELD>
-__global__ __launch_bounds__(1024) void ad_plan_kernel(AdPlanParams p) {
-  extern __shared__ int32_t counters[];  // [segment][class], then (HELD) class | place << 16 of every row, the place among its stretch's rows
-  __shared__ int32_t carry[16][4];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, classes = p.plan.classes, m = p.in.m;
-  const int stretch = ((m + p.segments - 1) / p.segments + 63) / 64 * 64;
-  const int from = wave < p.segments ? (int)min((int64_t)wave * stretch, (int64_t)m) : m, upto = min(from + stretch, m);
-  int32_t* held = counters + p.segments * classes;
-  for (int64_t i = threadIdx.x; i < p.clear; i += 1024) p.tickets[i] = 0;
-  for (int i = threadIdx.x; i < p.segments * classes; i += 1024) counters[i] = 0;
-  __syncthreads();
-  volatile int32_t* mine = counters + wave * classes;  // (of a wavefront that has rows)
-  // the lanes that have a class among them, one class after another; each lane's place among its class
-  auto places = [&](int c) {
-    int place = 0;
-    uint64_t left = __ballot(c >= 0);
-    while (left) {
-      const int v = __builtin_amdgcn_readlane(c, __builtin_ctzll(left));
-      const uint64_t same = __ballot(c == v);
-      const int have = mine[v];
-      if (c == v) place = have + __popcll(same & ((1ull << lane) - 1ull));
-      if (lane == 0) mine[v] = have + __popcll(same);
-      left &= ~same;
-    }
-    return place;
-  };
-  // f(rows r0 .. r0 + 63, the lane's class) for the wavefront's rows, in order. Held, the classes lie by row, else in the wavefront's 512 places
-  auto each = [&](auto&& f) {
-    int32_t* batch = HELD ? held + from : held + wave * 512;
-    for (int r0 = from; r0 < upto; r0 += 512) {
-      int c[8];
-#pragma unroll
-      for (int i = 0; i < 8; i++) c[i] = r0 + 64 * i + lane < upto ? ad_class(p.in, r0 + 64 * i + lane) : -1;
-#pragma unroll
-      for (int i = 0; i < 8; i++)
-        if (r0 + 64 * i + lane < upto) batch[64 * i + lane] = c[i];
-#pragma unroll 1
-      for (int i = 0; i < min(512, upto - r0); i += 64) f(r0 + i, r0 + i + lane < upto ? ((volatile int32_t*)batch)[i + lane] : -1);
-      if (HELD) batch += 512;
-    }
-  };
-  each([&](int r0, int c) {
-    const int place = places(c);
-    if (HELD && c >= 0) held[r0 + lane] = c | place << 16;
-  });
-  __syncthreads();
-  // each thread a run of classes: counts over the segments, then prefix sums over the threads
+// The classes' first places from their numbers of rows: each thread a run of classes, prefix sums over the threads. `rows_of`(class, first row): its rows.
+template <typename Rows>
+__device__ __forceinline__ void ad_plan_classes(const AdPlanParams& p, int32_t (*carry)[4], Rows&& rows_of) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, classes = p.plan.classes;
   const int per = (classes + 1023) / 1024, c0 = min((int)threadIdx.x * per, classes), c1 = min(c0 + per, classes);
-  int sum[4] = {0, 0, 0, 0};
+  int sum[4] = {0, 0, 0, 0}, before[4];
   auto add = [&](int (&to)[4], int c, int n) {
     const int units = c < p.in.adapters ? (n + p.unit - 1) / p.unit : 0;
     to[0] += n;
@@ -219,19 +175,10 @@ __global__ __launch_bounds__(1024) void ad_plan_kernel(AdPlanParams p) {
     to[2] += units;
     to[3] += units > 1 ? units : 0;
   };
-  for (int c = c0; c < c1; c++) {
-    int n = 0;
-    for (int s = 0; s < p.segments; s++) n += counters[s * classes + c];
-    add(sum, c, n);
-  }
-  int before[4];
+  for (int c = c0; c < c1; c++) add(sum, c, rows_of(c, -1));
 #pragma unroll
   for (int j = 0; j < 4; j++) {
-    int x = sum[j];
-    for (int d = 1; d < 64; d <<= 1) {
-      const int up = __shfl_up(x, d);
-      if (lane >= d) x += up;
-    }
+    const int x = wave_inclusive_sum(sum[j]);
     before[j] = x - sum[j];
     if (lane == 63) carry[wave][j] = x;
   }
@@ -242,12 +189,7 @@ __global__ __launch_bounds__(1024) void ad_plan_kernel(AdPlanParams p) {
       for (int j = 0; j < 4; j++) before[j] += carry[w][j];
   int32_t* out[4] = {p.plan.rows(), p.plan.tiles(), p.plan.units(), p.plan.slots()};
   for (int c = c0; c < c1; c++) {
-    int n = 0;
-    for (int s = 0; s < p.segments; s++) {
-      const int here = counters[s * classes + c];
-      counters[s * classes + c] = before[0] + n;
-      n += here;
-    }
+    const int n = rows_of(c, before[0]);
 #pragma unroll
     for (int j = 0; j < 4; j++) out[j][c] = before[j];
     add(before, c, n);
@@ -256,15 +198,109 @@ __global__ __launch_bounds__(1024) void ad_plan_kernel(AdPlanParams p) {
       for (int j = 0; j < 4; j++) out[j][classes] = before[j];
   }
   __syncthreads();
-  int32_t* order = p.plan.order();
-  if (HELD) {
-    for (int r = from + lane; r < upto; r += 64) order[mine[held[r] & 0xffff] + (held[r] >> 16)] = r;
-  } else {
-    each([&](int r0, int c) {
-      const int place = places(c);
-      if (c >= 0) order[place] = r0 + lane;
-    });
+}
+
+// One workgroup: a stable counting sort (rows of a class stay in ascending order, so sums over them are the same every time). What it takes is latency, so the
+// steps are few and side by side. Up to AD_HELD rows whose 64-row pieces have a counter each for every class: a wavefront has up to eight pieces, each lane their
+// classes and its places among them in registers; a wavefront a class adds the pieces' counts up. 8192 rows of 4 adapters .. us (pieces one after another, 12.6).
+constexpr int AD_HELD = 8192;
+constexpr int AD_COUNTERS = 8192;
+__global__ __launch_bounds__(1024) void ad_plan_pieces_kernel(AdPlanParams p) {
+  extern __shared__ int32_t counters[];  // [piece][class], then [class]
+  __shared__ int32_t carry[16][4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, classes = p.plan.classes, m = p.in.m, pieces = (m + 63) / 64;
+  int32_t* all = counters + pieces * classes;
+  int c[8], place[8];
+#pragma unroll
+  for (int i = 0; i < 8; i++) {
+    const int r = (wave + 16 * i) * 64 + lane;
+    c[i] = r < m ? ad_class(p.in, r) : -1;
   }
+  for (int64_t i = threadIdx.x; i < p.clear; i += 1024) p.tickets[i] = 0;
+  for (int i = threadIdx.x; i < pieces * classes; i += 1024) counters[i] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 8; i++) {
+    place[i] = 0;
+    uint64_t left = __ballot(c[i] >= 0);
+    while (left) {
+      const int v = __builtin_amdgcn_readlane(c[i], __builtin_ctzll(left));
+      const uint64_t same = __ballot(c[i] == v);
+      if (c[i] == v) place[i] = __popcll(same & ((1ull << lane) - 1ull));
+      if (lane == 0) counters[(wave + 16 * i) * classes + v] = __popcll(same);
+      left &= ~same;
+    }
+  }
+  __syncthreads();
+  for (int v = wave; v < classes; v += 16) {
+    const int n0 = 2 * lane < pieces ? counters[2 * lane * classes + v] : 0, n1 = 2 * lane + 1 < pieces ? counters[(2 * lane + 1) * classes + v] : 0;
+    const int upto = wave_inclusive_sum(n0 + n1);
+    if (2 * lane < pieces) counters[2 * lane * classes + v] = upto - n1 - n0;
+    if (2 * lane + 1 < pieces) counters[(2 * lane + 1) * classes + v] = upto - n1;
+    if (lane == 63) all[v] = upto;
+  }
+  __syncthreads();
+  ad_plan_classes(p, carry, [&](int v, int first) {
+    const int n = all[v];
+    if (first >= 0) all[v] = first;
+    return n;
+  });
+  int32_t* order = p.plan.order();
+#pragma unroll
+  for (int i = 0; i < 8; i++)
+    if (c[i] >= 0) order[all[c[i]] + counters[(wave + 16 * i) * classes + c[i]] + place[i]] = (wave + 16 * i) * 64 + lane;
+}
+
+// Any number of rows: `segments` wavefronts with a stretch of the rows each, 64 after 64, twice over.
+__global__ __launch_bounds__(1024) void ad_plan_kernel(AdPlanParams p) {
+  extern __shared__ int32_t counters[];  // [segment][class], then [wavefront][512] classes of rows
+  __shared__ int32_t carry[16][4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, classes = p.plan.classes, m = p.in.m;
+  const int stretch = ((m + p.segments - 1) / p.segments + 63) / 64 * 64;
+  const int from = wave < p.segments ? (int)min((int64_t)wave * stretch, (int64_t)m) : m, upto = min(from + stretch, m);
+  for (int64_t i = threadIdx.x; i < p.clear; i += 1024) p.tickets[i] = 0;
+  for (int i = threadIdx.x; i < p.segments * classes; i += 1024) counters[i] = 0;
+  __syncthreads();
+  volatile int32_t* mine = counters + wave * classes;  // (of a wavefront that has rows)
+  volatile int32_t* batch = counters + p.segments * classes + wave * 512;
+  // f(row, its place among the rows of its class) for the wavefront's rows; the classes' counters move up by them
+  auto each = [&](auto&& f) {
+    for (int r0 = from; r0 < upto; r0 += 512) {
+      int c[8];
+#pragma unroll
+      for (int i = 0; i < 8; i++) c[i] = r0 + 64 * i + lane < upto ? ad_class(p.in, r0 + 64 * i + lane) : -1;
+#pragma unroll
+      for (int i = 0; i < 8; i++) batch[64 * i + lane] = c[i];
+#pragma unroll 1
+      for (int i = 0; i < min(512, upto - r0); i += 64) {
+        const int mine_c = batch[i + lane];
+        int place = 0;
+        uint64_t left = __ballot(mine_c >= 0);
+        while (left) {
+          const int v = __builtin_amdgcn_readlane(mine_c, __builtin_ctzll(left));
+          const uint64_t same = __ballot(mine_c == v);
+          const int have = mine[v];
+          if (mine_c == v) place = have + __popcll(same & ((1ull << lane) - 1ull));
+          if (lane == 0) mine[v] = have + __popcll(same);
+          left &= ~same;
+        }
+        if (mine_c >= 0) f(r0 + i + lane, place);
+      }
+    }
+  };
+  each([](int, int) {});
+  __syncthreads();
+  ad_plan_classes(p, carry, [&](int c, int first) {
+    int n = 0;
+    for (int s = 0; s < p.segments; s++) {
+      const int here = counters[s * classes + c];
+      if (first >= 0) counters[s * classes + c] = first + n;
+      n += here;
+    }
+    return n;
+  });
+  int32_t* order = p.plan.order();
+  each([&](int r, int place) { order[place] = r; });
 }
 
 // The class whose tiles (or units), which begin at first[class], number t is of, or `classes` if there is none; its first one and its first row and the next class's
@@ -366,9 +402,9 @@ __device__ __forceinline__ float ad_pow2(int e) { return __uint_as_float((uint32
 
 // FP16 parts times 2^e, e <= 0 (below -40 they are too small to count).
 __device__ __forceinline__ u32x4_t ad_lower(const u32x4_t& v, int e) {
-  const _Float16 by = (_Float16)ad_pow2(max(e, -24)), more = (_Float16)ad_pow2(max(min(e + 24, 0), -24));
   f16x8_t f = __builtin_bit_cast(f16x8_t, v);
-  f = f * by * more;
+  f = f * (_Float16)ad_pow2(max(e, -24));
+  if (__builtin_expect(__ballot(e < -24) != 0, 0)) f = f * (_Float16)ad_pow2(max(min(e + 24, 0), -24));
   return __builtin_bit_cast(u32x4_t, f);
 }
 
@@ -449,16 +485,16 @@ __device__ __forceinline__ void ad_shrink_units(const char* const (&x)[TM], cons
 struct AdFew {
   AdIndex in;
   const char* x;
-  int64_t x_stride;    // bytes
+  uint32_t x_stride;   // bytes
   const char* a;       // [adapters, rank, k]
   int k, n, splits, share;  // share: units of 128 bytes a split
   float* sums;         // [splits, m, rank]
   const float* scale;
   const char* b;       // [adapters, rank, n]
   const char* y;
-  int64_t y_stride;
+  uint32_t y_stride;
   char* out;
-  int64_t out_stride;
+  uint32_t out_stride;
   int padded;          // the rank in LDS, a multiple of 32
 };
 
@@ -472,7 +508,7 @@ __global__ __launch_bounds__(256) void ad_shrink_few_kernel(AdFew p) {
   if (count == 0 || c >= p.in.adapters) return;
   const int rank = ad_rank(p.in, c), r0 = blockIdx.z * 16;
   if (r0 >= rank) return;
-  const char* const x[1] = {p.x + row * p.x_stride + group * 16};
+  const char* const x[1] = {ad_row(p.x, row, p.x_stride) + group * 16};
   const char* const w[1] = {p.a + ((int64_t)c * p.in.rank + min(r0 + col, rank - 1)) * p.k * SIZE + group * 16};  // (ranks behind the last: nobody reads the sums)
   const int u0 = blockIdx.y * p.share;
   f32x4_t acc[1][1] = {};
@@ -495,7 +531,7 @@ __global__ __launch_bounds__(256) void ad_shrink_few_kernel(AdFew p) {
 // 2048 rows, a workgroup each, took 24 us for what 256 do in ..
 struct AdShrinkJob {
   const char* v;      // rows, `stride` bytes apart
-  int64_t stride;
+  uint32_t stride;
   const char* w;      // [adapters, rank, length]
   int length, splits, share;  // units of 128 bytes a split
   float* parts;       // [tile][chunk][split][row][rank] of sums (several splits), and an arrival counter [tile][chunk]
@@ -535,7 +571,7 @@ __global__ __launch_bounds__(64 * AD_WAVES) void ad_shrink_kernel(AdShrink p) {
   const char* x[2];
   const char* w[RT];
 #pragma unroll
-  for (int i = 0; i < 2; i++) x[i] = job.v + p.plan.order()[start + min(16 * i + col, count - 1)] * job.stride + group * 16;  // (rows behind the last: not used)
+  for (int i = 0; i < 2; i++) x[i] = ad_row(job.v, p.plan.order()[start + min(16 * i + col, count - 1)], job.stride) + group * 16;  // (rows behind the last: not used)
 #pragma unroll
   for (int i = 0; i < RT; i++) w[i] = job.w + ((int64_t)c * p.in.rank + min(r0 + 16 * i + col, rank - 1)) * job.length * SIZE + group * 16;
   f32x4_t acc[2][RT] = {};
@@ -705,13 +741,14 @@ __global__ __launch_bounds__(256) void ad_expand_few_kernel(AdFew p) {
   for (int i = 0; i < 4; i++) rows[i] = __shfl(row, 4 * group + i);
   auto base = [&](int first) {  // (rows behind the last: the first again)
 #pragma unroll
-    for (int i = 0; i < 4; i++) y[i] = ad_take<KIND, TINY>(p.y + rows[i] * p.y_stride, first, p.n);
+    for (int i = 0; i < 4; i++) y[i] = ad_take<KIND, TINY>(ad_row(p.y, rows[i], p.y_stride), first, p.n);
   };
   // what is under way: (block, 32 ranks) one after another, two ahead of the products (behind the last block the row's end: no load behind a branch)
+  const char* matrix = p.b + (int64_t)c * p.in.rank * p.n * SIZE;  // (a class without an adapter reads none)
   int ahead = block * 16 * VEC + col * VEC, ahead_rank = 0;
   auto load = [&](u32x4_t (&to)[8]) {
 #pragma unroll
-    for (int s = 0; s < 8; s++) to[s] = ad_take<KIND, TINY>(p.b + ((int64_t)c * p.in.rank + min(ahead_rank + 8 * group + s, rank - 1)) * p.n * SIZE, min(ahead, p.n), p.n);
+    for (int s = 0; s < 8; s++) to[s] = ad_take<KIND, TINY>(ad_row(matrix, min(ahead_rank + 8 * group + s, rank - 1), (uint32_t)p.n * SIZE), min(ahead, p.n), p.n);
     ahead_rank += 32;
     if (ahead_rank >= rank) ahead_rank = 0, ahead += stride * 16 * VEC;
   };
@@ -721,7 +758,7 @@ __global__ __launch_bounds__(256) void ad_expand_few_kernel(AdFew p) {
       const int first = block * 16 * VEC + col * VEC;
 #pragma unroll
       for (int i = 0; i < 4; i++)
-        if (4 * group + i < count) ad_put<KIND, TINY>(p.out + rows[i] * p.out_stride, y[i], first, p.n);
+        if (4 * group + i < count) ad_put<KIND, TINY>(ad_row(p.out, rows[i], p.out_stride), y[i], first, p.n);
       base(min(first + stride * 16 * VEC, p.n));
     }
     return;
@@ -787,7 +824,7 @@ __global__ __launch_bounds__(256) void ad_expand_few_kernel(AdFew p) {
 #pragma unroll
       for (int i = 0; i < 4; i++)
         if (4 * group + i < count)
-          ad_put<KIND, TINY>(p.out + rows[i] * p.out_stride, ad_result<KIND>(y[i], acc[0], i, KIND == HB_F16 ? ad_pow2(power[4 * group + i]) : 1.0f), first, p.n);
+          ad_put<KIND, TINY>(ad_row(p.out, rows[i], p.out_stride), ad_result<KIND>(y[i], acc[0], i, KIND == HB_F16 ? ad_pow2(power[4 * group + i]) : 1.0f), first, p.n);
 #pragma unroll
       for (int j = 0; j < VEC; j++) acc[0][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
       r0 = 0;
@@ -807,9 +844,9 @@ struct AdExpand {
   int n;
   const char* w;       // [adapters, rank, n]
   const char* y;       // null: zeros
-  int64_t y_stride;    // bytes
+  uint32_t y_stride;   // bytes
   char* out;
-  int64_t out_stride;
+  uint32_t out_stride;
 };
 template <int KIND, bool TINY>
 __global__ __launch_bounds__(256, 3) void ad_expand_kernel(AdExpand p) {
@@ -822,7 +859,7 @@ __global__ __launch_bounds__(256, 3) void ad_expand_kernel(AdExpand p) {
   count = min(count, 16);
   const int rank = ad_rank(p.in, c);
   if (rank == 0 && p.y == p.out) return;
-  int64_t rows[4];
+  int rows[4];
 #pragma unroll
   for (int i = 0; i < 4; i++) rows[i] = p.plan.order()[start + min(4 * group + i, count - 1)];
   const int sixteens = ad_sixteens(p.in.rank), steps = ad_thirties(rank);
@@ -845,13 +882,14 @@ __global__ __launch_bounds__(256, 3) void ad_expand_kernel(AdExpand p) {
       }
     }
   };
+  const char* mine = p.w + (int64_t)c * p.in.rank * p.n * SIZE;
   auto matrix = [&](int first, int step) {
 #pragma unroll
-    for (int i = 0; i < 8; i++) v[i] = ad_take<KIND, TINY>(p.w + ((int64_t)c * p.in.rank + min(32 * step + 8 * group + i, rank - 1)) * p.n * SIZE, first, p.n);
+    for (int i = 0; i < 8; i++) v[i] = ad_take<KIND, TINY>(ad_row(mine, min(32 * step + 8 * group + i, rank - 1), (uint32_t)p.n * SIZE), first, p.n);
   };
   auto base = [&](int first) {  // (rows behind the last: it again)
 #pragma unroll
-    for (int i = 0; i < 4; i++) y[i] = p.y ? ad_take<KIND, TINY>(p.y + rows[i] * p.y_stride, first, p.n) : u32x4_t{0u, 0u, 0u, 0u};
+    for (int i = 0; i < 4; i++) y[i] = p.y ? ad_take<KIND, TINY>(ad_row(p.y, rows[i], p.y_stride), first, p.n) : u32x4_t{0u, 0u, 0u, 0u};
   };
   // the wavefront's blocks, the next one's matrix under way while one is added; a rank of up to 32 keeps its sums in registers
   const int stride = gridDim.y * 4;
@@ -883,7 +921,7 @@ __global__ __launch_bounds__(256, 3) void ad_expand_kernel(AdExpand p) {
 #pragma unroll
     for (int i = 0; i < 4; i++)
       if (4 * group + i < count)  // (without an adapter the rows as they are: -0 too)
-        ad_put<KIND, TINY>(p.out + rows[i] * p.out_stride, rank == 0 ? y[i] : ad_result<KIND>(y[i], acc[0], i, unit[i]), first, p.n);
+        ad_put<KIND, TINY>(ad_row(p.out, rows[i], p.out_stride), rank == 0 ? y[i] : ad_result<KIND>(y[i], acc[0], i, unit[i]), first, p.n);
     if (more) base(first + stride * 16 * VEC);
   }
 }
@@ -894,7 +932,7 @@ struct AdOuterJob {
   const char* by_rank;  // of the other side's shrink
   const int8_t* rank_power;
   const char* v;        // rows
-  int64_t stride;       // bytes
+  uint32_t stride;      // bytes
   int length;
   float* to;            // [adapters, rank, length]
   float* parts;         // [slots, rank, length]
@@ -949,7 +987,7 @@ __global__ __launch_bounds__(256) void ad_outer_kernel(AdOuter p) {
   };
   auto load = [&](u32x4_t (&to)[8]) {
 #pragma unroll
-    for (int s = 0; s < 8; s++) to[s] = ad_take<KIND, TINY>(job.v + rows[s] * job.stride, first, job.length);
+    for (int s = 0; s < 8; s++) to[s] = ad_take<KIND, TINY>(ad_row(job.v, rows[s], job.stride), first, job.length);
   };
   auto sums = [&](int tile) {
 #pragma unroll
@@ -979,7 +1017,10 @@ __global__ __launch_bounds__(256) void ad_outer_kernel(AdOuter p) {
       if (d && tile >= tiles) break;
       u32x4_t v[8], s[RT][WORDS];
 #pragma unroll
-      for (int i = 0; i < 8; i++) v[i] = start + tile * AD_TILE + 8 * group + i < end ? next[d][i] : u32x4_t{0u, 0u, 0u, 0u};
+      for (int i = 0; i < 8; i++) v[i] = next[d][i];
+      if (start + (tile + 1) * AD_TILE > end)  // the last tile's rows behind the end: what they repeat may be infinite
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = start + tile * AD_TILE + 8 * group + i < end ? v[i] : u32x4_t{0u, 0u, 0u, 0u};
 #pragma unroll
       for (int t = 0; t < RT; t++)
 #pragma unroll
@@ -1120,10 +1161,13 @@ static bool ad_shape(const hb_adapters* a, int64_t m, bool grads, AdShape& s) {
 
 static int ad_run_plan(const AdShape& s, const AdIndex& in, const AdPlan& plan, char* ws, hipStream_t stream) {
   AdPlanParams p{in, plan, s.unit, 1, reinterpret_cast<int32_t*>(ws + s.plan_bytes), s.tickets};
-  while (p.segments < 16 && (int64_t)(2 * p.segments) * plan.classes <= AD_COUNTERS) p.segments *= 2;
-  const size_t lds = (size_t)p.segments * plan.classes * 4;
-  if (s.m <= AD_HELD) ad_plan_kernel<true><<<1, 1024, lds + s.m * 4, stream>>>(p);
-  else ad_plan_kernel<false><<<1, 1024, lds + 16 * 512 * 4, stream>>>(p);
+  const int64_t pieces = cut(s.m, 64);
+  if (s.m <= AD_HELD && pieces * plan.classes <= AD_COUNTERS) {
+    ad_plan_pieces_kernel<<<1, 1024, (size_t)(pieces + 1) * plan.classes * 4, stream>>>(p);
+  } else {
+    while (p.segments < 16 && (int64_t)(2 * p.segments) * plan.classes <= AD_COUNTERS / 2) p.segments *= 2;
+    ad_plan_kernel<<<1, 1024, (size_t)p.segments * plan.classes * 4 + 16 * 512 * 4, stream>>>(p);
+  }
   return launch_status();
 }
 
@@ -1177,8 +1221,8 @@ static int ad_add(const hb_adapters* a, const AdShape& s, const AdIndex& in, con
   const char *xr = static_cast<const char*>(x), *yr = static_cast<const char*>(y);
   char* to = static_cast<char*>(out);
   if (s.few) {
-    AdFew p{in, xr, x_stride * s.size, static_cast<const char*>(a->a), s.k, s.n, s.splits, (int)cut(cut(s.k, 128 / s.size), s.splits), reinterpret_cast<float*>(ws),
-            a->scale, static_cast<const char*>(a->b), yr, y_stride * s.size, to, out_stride * s.size, ad_thirties(s.rank) * 32};
+    AdFew p{in, xr, (uint32_t)(x_stride * s.size), static_cast<const char*>(a->a), s.k, s.n, s.splits, (int)cut(cut(s.k, 128 / s.size), s.splits), reinterpret_cast<float*>(ws),
+            a->scale, static_cast<const char*>(a->b), yr, (uint32_t)(y_stride * s.size), to, (uint32_t)(out_stride * s.size), ad_thirties(s.rank) * 32};
     ad_shrink_few_kernel<KIND><<<dim3((unsigned)s.m, (unsigned)s.splits, (unsigned)ad_sixteens(s.rank)), 256, 0, stream>>>(p);
     if (int code = launch_status()) return code;
     const size_t lds = (size_t)AdType<KIND>::PARTS * 16 * (p.padded * AdType<KIND>::SIZE + 16);
@@ -1193,9 +1237,9 @@ static int ad_add(const hb_adapters* a, const AdShape& s, const AdIndex& in, con
   int8_t* power = reinterpret_cast<int8_t*>(by_row + s.row_bytes);
   int code = ad_run_plan(s, in, plan, ws, stream);
   if (code) return code;
-  AdShrink down{in, plan, {{xr, x_stride * s.size, static_cast<const char*>(a->a), s.k, 0, 0, nullptr, nullptr, by_row, nullptr, power, nullptr}, {}}, a->scale, 0};
+  AdShrink down{in, plan, {{xr, (uint32_t)(x_stride * s.size), static_cast<const char*>(a->a), s.k, 0, 0, nullptr, nullptr, by_row, nullptr, power, nullptr}, {}}, a->scale, 0};
   if ((code = ad_run_shrink<KIND>(s, down, ws, stream))) return code;
-  AdExpand up{in, plan, by_row, power, s.n, static_cast<const char*>(a->b), yr, y_stride * s.size, to, out_stride * s.size};
+  AdExpand up{in, plan, by_row, power, s.n, static_cast<const char*>(a->b), yr, (uint32_t)(y_stride * s.size), to, (uint32_t)(out_stride * s.size)};
   return ad_run_expand<KIND>(s, up, stream);
 }
 
@@ -1214,13 +1258,13 @@ static int ad_grads(const hb_adapters* a, const AdShape& s, const AdIndex& in, c
   if (code) return code;
   const char *xr = static_cast<const char*>(x), *dyr = static_cast<const char*>(dy);
   AdShrink down{in, plan,
-                {{xr, x_stride * s.size, static_cast<const char*>(a->a), s.k, 0, 0, nullptr, nullptr, nullptr, x_ranks, nullptr, x_power},
-                 {dyr, dy_stride * s.size, static_cast<const char*>(a->b), s.n, 0, 0, nullptr, nullptr, dy_rows, dy_ranks, dy_row_power, dy_power}},
+                {{xr, (uint32_t)(x_stride * s.size), static_cast<const char*>(a->a), s.k, 0, 0, nullptr, nullptr, nullptr, x_ranks, nullptr, x_power},
+                 {dyr, (uint32_t)(dy_stride * s.size), static_cast<const char*>(a->b), s.n, 0, 0, nullptr, nullptr, dy_rows, dy_ranks, dy_row_power, dy_power}},
                 a->scale, 0};
   if ((code = ad_run_shrink<KIND>(s, down, ws, stream))) return code;
-  AdExpand up{in, plan, dy_rows, dy_row_power, s.k, static_cast<const char*>(a->a), nullptr, 0, static_cast<char*>(dx), (int64_t)s.k * s.size};
+  AdExpand up{in, plan, dy_rows, dy_row_power, s.k, static_cast<const char*>(a->a), nullptr, 0, static_cast<char*>(dx), (uint32_t)(s.k * s.size)};
   if ((code = ad_run_expand<KIND>(s, up, stream))) return code;
-  AdOuter outer{in, plan, {{dy_ranks, dy_power, xr, x_stride * s.size, s.k, da, part_a}, {x_ranks, x_power, dyr, dy_stride * s.size, s.n, db, part_b}}, s.unit, 0};
+  AdOuter outer{in, plan, {{dy_ranks, dy_power, xr, (uint32_t)(x_stride * s.size), s.k, da, part_a}, {x_ranks, x_power, dyr, (uint32_t)(dy_stride * s.size), s.n, db, part_b}}, s.unit, 0};
   return ad_run_outer<KIND>(s, outer, stream);
 }
 
@@ -1245,7 +1289,7 @@ extern "C" int hb_adapters_add(const hb_adapters* adapters, const void* x, int64
   AdShape s;
   if (!x || !y || !out || !workspace) return HB_ENULL;
   if (int code = ad_check(adapters, index, index_bytes, m, false, s)) return code;
-  if (x_stride < s.k || y_stride < s.n || out_stride < s.n || !aligned(x, s.size) || !aligned(y, s.size) || !aligned(out, s.size) || !aligned(workspace, 16)) return HB_EINVAL;
+  if (x_stride < s.k || y_stride < s.n || out_stride < s.n || std::max({x_stride, y_stride, out_stride}) > AD_STRIDE / s.size || !aligned(x, s.size) || !aligned(y, s.size) || !aligned(out, s.size) || !aligned(workspace, 16)) return HB_EINVAL;
   if (y == out && y_stride != out_stride) return HB_EINVAL;
   if (workspace_bytes < s.bytes()) return HB_EWORKSPACE;
   const AdIndex in{index, adapters->ranks, index_bytes == 8, (int)m, s.adapters, s.rank};
@@ -1262,7 +1306,7 @@ extern "C" int hb_adapters_grads(const hb_adapters* adapters, const void* x, int
   AdShape s;
   if (!x || !dy || !dx || !da || !db || !workspace) return HB_ENULL;
   if (int code = ad_check(adapters, index, index_bytes, m, true, s)) return code;
-  if (x_stride < s.k || dy_stride < s.n || !aligned(x, s.size) || !aligned(dy, s.size) || !aligned(dx, s.size) || !aligned(da, 4) || !aligned(db, 4) || !aligned(workspace, 16))
+  if (x_stride < s.k || dy_stride < s.n || std::max(x_stride, dy_stride) > AD_STRIDE / s.size || !aligned(x, s.size) || !aligned(dy, s.size) || !aligned(dx, s.size) || !aligned(da, 4) || !aligned(db, 4) || !aligned(workspace, 16))
     return HB_EINVAL;
   if (workspace_bytes < s.bytes()) return HB_EWORKSPACE;
   const AdIndex in{index, adapters->ranks, index_bytes == 8, (int)m, s.adapters, s.rank};

@@ -617,7 +617,7 @@ int hb_mxfp4_moe(const hb_mxfp4_experts* experts, const void* x, const int32_t* 
  * A pool of adapters of one projection [n, k]: adapter i adds scale_i b_i^T a_i to it. Both matrices lie rank by rank: a [adapters, rank, k] and
  * b [adapters, rank, n], of `type` (HB_BF16 / HB_F16 / HB_F32). ranks (or NULL): adapter i has ranks[i] of the `rank` rows, what lies behind them is
  * not read. scale: FP32 (NULL: 1). Up to 4096 adapters of a rank up to 256; k and n up to 2^22, m up to 2^24. Rows of x, y, dy and out are of `type`, a
- * stride (in elements) apart; every array on its elements' boundary. index: int32 or int64 [m] (index_bytes 4 or 8), a row's adapter; a row whose
+ * stride (in elements; below 2^32 bytes) apart; every array on its elements' boundary. index: int32 or int64 [m] (index_bytes 4 or 8), a row's adapter; a row whose
  * index is outside 0 .. adapters - 1, or whose adapter has rank 0, has none. `workspace`: plain scratch on 16 bytes. No counterpart in the reference. */
 typedef struct {
   const void* a;

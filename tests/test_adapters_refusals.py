@@ -30,7 +30,7 @@ def test_pools(change):
         assert lib.hb_adapters_workspace_bytes(_struct(**change), 10, 0) == lib.hb_adapters_workspace_bytes(_struct(**change), 10, 1) == 0
 
 
-@pytest.mark.parametrize("change", [dict(m=0), dict(m=-1), dict(m=(1 << 24) + 1), dict(x_stride=63), dict(index_bytes=2), dict(index=258), dict(x=257), dict(ws=1032)])
+@pytest.mark.parametrize("change", [dict(m=0), dict(m=-1), dict(m=(1 << 24) + 1), dict(x_stride=63), dict(x_stride=1 << 31), dict(index_bytes=2), dict(index=258), dict(x=257), dict(ws=1032)])
 def test_rows(change):
     lib = _lib.lib()
     assert lib.hb_adapters_add(_struct(), *{**CALL, **change}.values()) == _lib.HB_EINVAL
