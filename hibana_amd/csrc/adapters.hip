@@ -169,7 +169,7 @@ __device__ __forceinline__ void ad_plan_classes(const AdPlanParams& p, int32_t (
   const int per = (classes + 1023) / 1024, c0 = min((int)threadIdx.x * per, classes), c1 = min(c0 + per, classes);
   int sum[4] = {0, 0, 0, 0}, before[4];
   auto add = [&](int (&to)[4], int c, int n) {
-    const int units = c < p.in.adapters ? (n + p.unit - 1) / p.unit : 0;
+    const int units = c < p.in.adapters ? max((n + p.unit - 1) / p.unit, 1) : 0;  // (an adapter without rows has one, of none: it writes the zeros)
     to[0] += n;
     to[1] += (n + AD_TILE - 1) / AD_TILE;
     to[2] += units;
@@ -946,7 +946,8 @@ struct AdOuter {
 
 // A workgroup: RT x 16 ranks times sixteen lanes' columns over a unit of an adapter's rows, the four wavefronts taking its tiles in turn and joining
 // their sums in LDS. A lane's eight rows of sixteen bytes are turned as in the expansion; the next tile's are under way while one is
-// multiplied. An adapter's only unit writes the gradient, several write partial sums.
+// multiplied. An adapter's only unit writes the gradient (zeros, if it has no rows), several write partial sums for ad_join_kernel. (Joined by the last of them to
+// arrive instead, whose sums must pass the dies' caches in words: 28 us for the 16 of both kernels at 2048 rows of 5120 x 5120, rank 16.)
 template <int KIND, int RT, bool TINY>
 __global__ __launch_bounds__(256) void ad_outer_kernel(AdOuter p) {
   constexpr int VEC = AD_VEC<KIND>, SIZE = AdType<KIND>::SIZE, PARTS = AdType<KIND>::OUTER, WORDS = SIZE == 4 ? 2 : PARTS;
@@ -960,7 +961,7 @@ __global__ __launch_bounds__(256) void ad_outer_kernel(AdOuter p) {
   const int c = at.c, which = u - at.first, units = p.plan.units()[c + 1] - at.first;
   const int start = at.row + which * p.unit, end = min(start + p.unit, at.next_row);
   const int rank = ad_rank(p.in, c), tile0 = p.plan.tiles()[c] + which * (p.unit / AD_TILE), tiles = r0 < rank ? (end - start + AD_TILE - 1) / AD_TILE : 0;
-  const int have = min(RT, ad_sixteens(rank - r0));  // sixteens of ranks (those behind the adapter's rank are not written)
+  const int have = max(min(RT, ad_sixteens(rank - r0)), 1);  // sixteens of ranks (those behind the adapter's rank are not written)
   float* to = units > 1 ? job.parts + (int64_t)(p.plan.slots()[c] + which) * p.in.rank * job.length : job.to + (int64_t)c * p.in.rank * job.length;
   f32x4_t acc[RT][VEC] = {};
   int power[RT];  // FP16: the sums are in units of 2^power, the largest of the unit's tiles
@@ -1074,11 +1075,13 @@ __global__ __launch_bounds__(256) void ad_outer_kernel(AdOuter p) {
   }
 }
 
-// The partial sums of adapters with several units, in the units' order; zeros for adapters that have no row.
+// The partial sums of adapters with several units, in the units' order.
 __global__ __launch_bounds__(256) void ad_join_kernel(AdOuter p) {
   const AdOuterJob& job = p.job[blockIdx.z];
-  const int c = blockIdx.y, units = p.plan.units()[c + 1] - p.plan.units()[c];
-  if (units == 1) return;
+  if ((int)blockIdx.y >= p.plan.slots()[p.plan.classes]) return;
+  const AdPlace at = ad_find(p.plan, p.plan.slots(), blockIdx.y);
+  const int c = at.c, units = p.plan.slots()[c + 1] - at.first;
+  if (at.first != (int)blockIdx.y) return;  // (an adapter's workgroups are those of its first slot)
   const int64_t size = (int64_t)p.in.rank * job.length;
   const float* from = job.parts + (int64_t)p.plan.slots()[c] * size;
   for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < size; i += (int64_t)gridDim.x * 1024) {
@@ -1149,8 +1152,8 @@ static bool ad_shape(const hb_adapters* a, int64_t m, bool grads, AdShape& s) {
   s.unit = 4 * AD_TILE;
   if (grads) {
     const int64_t blocks = (cut(a->k, 256 / s.size) + cut(a->n, 256 / s.size)) * cut(a->rank, 64);
-    s.unit = (int)std::min<int64_t>(std::max<int64_t>(4 * AD_TILE, cut(cut(m * blocks, 512), 4 * AD_TILE) * 4 * AD_TILE), 1 << 20);
-    s.units = cut(m, s.unit) + classes;
+    s.unit = (int)std::min<int64_t>(std::max<int64_t>(16 * AD_TILE, cut(cut(m * blocks, 512), 4 * AD_TILE) * 4 * AD_TILE), 1 << 20);
+    s.units = cut(m, s.unit) + a->adapters;
     s.slots = 2 * (m / s.unit);  // an adapter of more than one unit has at most two for every whole `unit` of its rows
     s.part_a_bytes = up256((size_t)s.slots * a->rank * a->k * 4);
     s.part_b_bytes = up256((size_t)s.slots * a->rank * a->n * 4);
@@ -1209,9 +1212,9 @@ static int ad_run_outer(const AdShape& s, AdOuter& p, hipStream_t stream) {
   HB_AD(1) HB_AD(2) HB_AD(4)
 #undef HB_AD
   int code = launch_status();
-  if (code) return code;
+  if (code || !s.slots) return code;  // (no adapter has a second unit)
   const unsigned blocks = (unsigned)std::min<int64_t>(cut((int64_t)s.rank * longest, 1024), 1024);
-  ad_join_kernel<<<dim3(blocks, (unsigned)s.adapters, 2), 256, 0, stream>>>(p);
+  ad_join_kernel<<<dim3(blocks, (unsigned)s.slots, 2), 256, 0, stream>>>(p);
   return launch_status();
 }
 

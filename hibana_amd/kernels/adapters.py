@@ -126,7 +126,14 @@ def _stride(t: torch.Tensor, width: int) -> int:
 
 def _operands(v: torch.Tensor, x: torch.Tensor, pool: Adapters, index: torch.Tensor, what: str):
     """The rows of v [M, N] and x [M, K] and the index as the library takes them, the number of rows and the current stream."""
-    v, x = _rows(v, pool.b.shape[2], pool, what), _rows(x, pool.a.shape[2], pool, what)
+    a = pool.a
+    at = a.get_device()
+    if v.ndim == 2 and v.is_contiguous() and x.is_contiguous() and index.is_contiguous() and v.dtype is a.dtype and x.dtype is a.dtype and index.dtype in INDEX \
+            and v.get_device() == at and x.get_device() == at and index.get_device() == at and at >= 0 and at == torch._C._cuda_getDevice():
+        m, n = v.shape
+        if n == pool.b.shape[2] and x.shape == (m, a.shape[2]) and index.shape == (m,):  # as most calls are
+            return v, x, index, m, torch._C._cuda_getCurrentRawStream(at)
+    v, x = _rows(v, pool.b.shape[2], pool, what), _rows(x, a.shape[2], pool, what)
     m = v.shape[0]
     if x.shape[0] != m:
         raise ValueError(f"{what}: as many rows of x as there are results")
@@ -134,14 +141,14 @@ def _operands(v: torch.Tensor, x: torch.Tensor, pool: Adapters, index: torch.Ten
         raise ValueError(f"{what}: an int32 or int64 index [{m}]")
     if not index.is_contiguous():
         index = index.contiguous()
-    return v, x, index, m, _lib.stream_of(v, x, index, pool.a)
+    return v, x, index, m, _lib.stream_of(v, x, index, a)
 
 
 def _add(y: torch.Tensor, x: torch.Tensor, pool: Adapters, index: torch.Tensor, out: torch.Tensor | None) -> torch.Tensor:
     yr, xr, ix, m, stream = _operands(y, x, pool, index, "adapters.add")
     k, n = pool.a.shape[2], pool.b.shape[2]
     if out is None:
-        out = yr.new_empty((m, n))
+        out = torch.empty_like(yr) if yr.is_contiguous() else yr.new_empty((m, n))
         to = n
     elif out.dtype != yr.dtype or out.shape != yr.shape or out.stride(1) != 1 or (m > 1 and out.stride(0) < n) or out.device != yr.device:
         raise ValueError("adapters.add: out like y, its rows contiguous")
@@ -149,7 +156,7 @@ def _add(y: torch.Tensor, x: torch.Tensor, pool: Adapters, index: torch.Tensor, 
         to = _stride(out, n)
     if m:
         need = pool.room(m, 0)
-        ws = yr.new_empty(need, dtype=torch.uint8)  # (of the capture's own pool in a captured call)
+        ws = yr.new_empty(need, dtype=torch.uint8)  # (of the capture's own pool in a captured call; a call's own, so that two at once share nothing)
         code = _lib.lib().hb_adapters_add(pool.struct(), xr.data_ptr(), _stride(xr, k), yr.data_ptr(), _stride(yr, n), ix.data_ptr(), INDEX[ix.dtype], m, out.data_ptr(), to,
                                           ws.data_ptr(), need, stream)
         if code:

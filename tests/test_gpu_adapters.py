@@ -298,3 +298,19 @@ def test_a_pool_of_pairs():
     pool.a = pool.a.clone().mul_(2.0)
     pairs = [(p[0] * 2, *p[1:]) for p in pairs]
     close()
+
+
+@pytest.mark.parametrize("count", [3, 1000])
+def test_gradients_of_several_units_of_rows(count):
+    """Adapters of many rows, of one and of none in a call, in a small pool and among many: partial sums are those of the adapters that have them."""
+    from hibana_amd.kernels import adapters
+    m, k, n, rank = 3000, 70, 40, 5
+    y, x, a, b, scale, ranks, _ = make(m, k, n, rank, count, torch.bfloat16, seed=30)
+    index = torch.full((m,), count - 1, dtype=torch.int32)
+    index[::3], index[5], index[6] = 0, 1, -1
+    case = (y, x, a, b, scale, ranks, index)
+    got = adapters.grads(y.cuda(), x.cuda(), pool_of(a, b, scale, ranks), index.cuda())
+    for name, g, w, bound in zip(("dx", "da", "db"), got, oracle.grads(*case), oracle.grads_bound(*case)):
+        within(g, w, bound, name)
+    for g, w in zip(adapters.grads(y.cuda(), x.cuda(), pool_of(a, b, scale, ranks), index.cuda()), got):
+        assert torch.equal(g, w)  # the same call, the same bits
