@@ -42,7 +42,7 @@ __device__ __forceinline__ float ad_value(uint32_t bits) {
 }
 template <int KIND>
 __device__ __forceinline__ uint32_t ad_bits(float v) {
-  if constexpr (KIND == HB_BF16) return f32_to_bf16_bits(v);
+  if constexpr (KIND == HB_BF16) return bf16_of(v);
   if constexpr (KIND == HB_F16) return __builtin_bit_cast(uint16_t, (_Float16)v);
   return __float_as_uint(v);
 }
@@ -202,7 +202,8 @@ __device__ __forceinline__ void ad_plan_classes(const AdPlanParams& p, int32_t (
 
 // One workgroup: a stable counting sort (rows of a class stay in ascending order, so sums over them are the same every time). What it takes is latency, so the
 // steps are few and side by side. Up to AD_HELD rows whose 64-row pieces have a counter each for every class: a wavefront has up to eight pieces, each lane their
-// classes and its places among them in registers; a wavefront a class adds the pieces' counts up. 8192 rows of 4 adapters .. us (pieces one after another, 12.6).
+// classes and its places among them in registers; a wavefront a class adds the pieces' counts up. 8192 rows of 4 adapters 9.1 us, 4096 of 6 5.8 (a wavefront's pieces
+// one after another through one counter a class: 13.0 and 7.8).
 constexpr int AD_HELD = 8192;
 constexpr int AD_COUNTERS = 8192;
 __global__ __launch_bounds__(1024) void ad_plan_pieces_kernel(AdPlanParams p) {
@@ -422,7 +423,7 @@ __device__ __forceinline__ u32x4_t ad_turn(const u32x4_t (&v)[8], int j) {
 // Units of 128 bytes (a whole cache line of every row), DEPTH of them under way.
 template <int KIND, int TM, int RT, int LIMIT = RT>
 __device__ __forceinline__ void ad_shrink_units(const char* const (&x)[TM], const char* const (&w)[LIMIT], int length, int u0, int u1, int step, f32x4_t (&acc)[TM][LIMIT]) {
-  constexpr int VEC = AD_VEC<KIND>, SIZE = AdType<KIND>::SIZE, UNIT = 128 / SIZE, DEPTH = TM + RT <= 3 ? 4 : TM + RT <= 4 ? 3 : 2;
+  constexpr int VEC = AD_VEC<KIND>, SIZE = AdType<KIND>::SIZE, UNIT = 128 / SIZE, DEPTH = TM == 1 ? 4 : 2;
   const int whole = length / UNIT, end = min(u1, whole), group = (threadIdx.x & 63) >> 4;
   u32x4_t xv[DEPTH][TM][2], wv[DEPTH][RT][2];
   auto load = [&](int d, int u) {
@@ -527,8 +528,11 @@ __global__ __launch_bounds__(256) void ad_shrink_few_kernel(AdFew p) {
 
 // A plan's tiles: a workgroup has one split of the long axis for a tile's 32 rows and RT x 16 ranks, its wavefronts taking units in turn. Of a tile's workgroups the last one to
 // arrive adds the splits' sums up, in their order, and leaves them, scaled, as the operands that the second products take: by rows (for the expansion), and with
-// rows and ranks changed over (for the outer product). The splits are there to keep every compute unit at it: one alone reads some 17 GB/s, and the 64 tiles of
-// 2048 rows, a workgroup each, took 24 us for what 256 do in ..
+// rows and ranks changed over (for the outer product).
+//
+// The splits are there to keep every compute unit at it: one alone reads some 20 GB/s. Both shrinks of 2048 rows of 5120 at rank 16 (42 MB) take 17.7 us in 1024 workgroups, of
+// which the data 9, the way to it and the joining of the splits the rest (in 128 workgroups of the whole axis each: 24 us). Where the rank is high the matrices' own reads count:
+// every tile reads its adapter's again, from the die's cache (8192 rows of 12800 and 2560, ranks 8 .. 64, 252 MB: 96 us, 63 of them with the matrices' loads left out).
 struct AdShrinkJob {
   const char* v;      // rows, `stride` bytes apart
   uint32_t stride;
@@ -711,12 +715,13 @@ __device__ __forceinline__ void ad_products(const u32x4_t (&s)[LIMIT][WORDS], co
 // y + the lane's VEC sums of row i of its four (times 2^e), rounded.
 template <int KIND>
 __device__ __forceinline__ u32x4_t ad_result(const u32x4_t& y, const f32x4_t (&acc)[AD_VEC<KIND>], int i, float unit) {
-  u32x4_t v{0u, 0u, 0u, 0u};
+  u32x4_t v;
+  auto value = [&](int j) { return ad_value<KIND>(ad_elem<KIND>(y, j)) + (KIND == HB_F16 ? acc[j][i] * unit : acc[j][i]); };
 #pragma unroll
-  for (int j = 0; j < AD_VEC<KIND>; j++) {
-    const float to = ad_value<KIND>(ad_elem<KIND>(y, j)) + (KIND == HB_F16 ? acc[j][i] * unit : acc[j][i]);
-    if constexpr (AdType<KIND>::SIZE == 4) v[j] = __float_as_uint(to);
-    else v[j >> 1] |= ad_bits<KIND>(to) << (16 * (j & 1));
+  for (int q = 0; q < 4; q++) {
+    if constexpr (KIND == HB_F32) v[q] = __float_as_uint(value(q));
+    else if constexpr (KIND == HB_BF16) v[q] = bf16_pair(value(2 * q), value(2 * q + 1));
+    else v[q] = ad_bits<KIND>(value(2 * q)) | ad_bits<KIND>(value(2 * q + 1)) << 16;
   }
   return v;
 }
@@ -1166,10 +1171,10 @@ static int ad_run_plan(const AdShape& s, const AdIndex& in, const AdPlan& plan, 
   AdPlanParams p{in, plan, s.unit, 1, reinterpret_cast<int32_t*>(ws + s.plan_bytes), s.tickets};
   const int64_t pieces = cut(s.m, 64);
   if (s.m <= AD_HELD && pieces * plan.classes <= AD_COUNTERS) {
-    ad_plan_pieces_kernel<<<1, 1024, (size_t)(pieces + 1) * plan.classes * 4, stream>>>(p);
+    HB_LAUNCH((ad_plan_pieces_kernel), dim3(1), dim3(1024), (size_t)(pieces + 1) * plan.classes * 4, stream, p);
   } else {
     while (p.segments < 16 && (int64_t)(2 * p.segments) * plan.classes <= AD_COUNTERS / 2) p.segments *= 2;
-    ad_plan_kernel<<<1, 1024, (size_t)p.segments * plan.classes * 4 + 16 * 512 * 4, stream>>>(p);
+    HB_LAUNCH((ad_plan_kernel), dim3(1), dim3(1024), (size_t)p.segments * plan.classes * 4 + 16 * 512 * 4, stream, p);
   }
   return launch_status();
 }
@@ -1186,9 +1191,9 @@ static int ad_run_shrink(const AdShape& s, AdShrink& p, char* ws, hipStream_t st
     p.job[j].parts = parts + (j && s.splits_x > 1 ? s.tiles * s.chunks * s.splits_x * AD_TILE * 16 * s.rt : 0);
   }
   const dim3 grid((unsigned)s.tiles, (unsigned)(p.chunks * (s.splits_x + s.splits_dy)));
-  if (s.rt == 1) ad_shrink_kernel<KIND, 1><<<grid, 64 * AD_WAVES, 0, stream>>>(p);
-  if (s.rt == 2) ad_shrink_kernel<KIND, 2><<<grid, 64 * AD_WAVES, 0, stream>>>(p);
-  if (s.rt == 4) ad_shrink_kernel<KIND, 4><<<grid, 64 * AD_WAVES, 0, stream>>>(p);
+  if (s.rt == 1) HB_LAUNCH((ad_shrink_kernel<KIND, 1>), grid, dim3(64 * AD_WAVES), 0, stream, p);
+  if (s.rt == 2) HB_LAUNCH((ad_shrink_kernel<KIND, 2>), grid, dim3(64 * AD_WAVES), 0, stream, p);
+  if (s.rt == 4) HB_LAUNCH((ad_shrink_kernel<KIND, 4>), grid, dim3(64 * AD_WAVES), 0, stream, p);
   return launch_status();
 }
 
@@ -1197,8 +1202,8 @@ static int ad_run_expand(const AdShape& s, AdExpand& p, hipStream_t stream) {
   const int64_t groups = cut(p.n, 4 * 16 * AD_VEC<KIND>);
   const int64_t share = std::max<int64_t>(1, std::min<int64_t>(groups, cut(s.m, 16) * groups / AD_EXPANDS));
   const dim3 grid((unsigned)(2 * s.tiles), (unsigned)cut(groups, share));
-  if (p.n < AD_VEC<KIND>) ad_expand_kernel<KIND, true><<<grid, 256, 0, stream>>>(p);
-  else ad_expand_kernel<KIND, false><<<grid, 256, 0, stream>>>(p);
+  if (p.n < AD_VEC<KIND>) HB_LAUNCH((ad_expand_kernel<KIND, true>), grid, dim3(256), 0, stream, p);
+  else HB_LAUNCH((ad_expand_kernel<KIND, false>), grid, dim3(256), 0, stream, p);
   return launch_status();
 }
 
@@ -1208,13 +1213,13 @@ static int ad_run_outer(const AdShape& s, AdOuter& p, hipStream_t stream) {
   const int longest = std::max(p.job[0].length, p.job[1].length);
   const dim3 grid((unsigned)cut(longest, 16 * AD_VEC<KIND>), (unsigned)s.units, (unsigned)(2 * p.chunks));
   const bool tiny = std::min(p.job[0].length, p.job[1].length) < AD_VEC<KIND>;
-#define HB_AD(RT) if (s.rt == RT) { if (tiny) ad_outer_kernel<KIND, RT, true><<<grid, 256, 0, stream>>>(p); else ad_outer_kernel<KIND, RT, false><<<grid, 256, 0, stream>>>(p); }
+#define HB_AD(RT) if (s.rt == RT) { if (tiny) HB_LAUNCH((ad_outer_kernel<KIND, RT, true>), grid, dim3(256), 0, stream, p); else HB_LAUNCH((ad_outer_kernel<KIND, RT, false>), grid, dim3(256), 0, stream, p); }
   HB_AD(1) HB_AD(2) HB_AD(4)
 #undef HB_AD
   int code = launch_status();
   if (code || !s.slots) return code;  // (no adapter has a second unit)
   const unsigned blocks = (unsigned)std::min<int64_t>(cut((int64_t)s.rank * longest, 1024), 1024);
-  ad_join_kernel<<<dim3(blocks, (unsigned)s.slots, 2), 256, 0, stream>>>(p);
+  HB_LAUNCH((ad_join_kernel), dim3(blocks, (unsigned)s.slots, 2), dim3(256), 0, stream, p);
   return launch_status();
 }
 
@@ -1226,13 +1231,13 @@ static int ad_add(const hb_adapters* a, const AdShape& s, const AdIndex& in, con
   if (s.few) {
     AdFew p{in, xr, (uint32_t)(x_stride * s.size), static_cast<const char*>(a->a), s.k, s.n, s.splits, (int)cut(cut(s.k, 128 / s.size), s.splits), reinterpret_cast<float*>(ws),
             a->scale, static_cast<const char*>(a->b), yr, (uint32_t)(y_stride * s.size), to, (uint32_t)(out_stride * s.size), ad_thirties(s.rank) * 32};
-    ad_shrink_few_kernel<KIND><<<dim3((unsigned)s.m, (unsigned)s.splits, (unsigned)ad_sixteens(s.rank)), 256, 0, stream>>>(p);
+    HB_LAUNCH((ad_shrink_few_kernel<KIND>), dim3((unsigned)s.m, (unsigned)s.splits, (unsigned)ad_sixteens(s.rank)), dim3(256), 0, stream, p);
     if (int code = launch_status()) return code;
     const size_t lds = (size_t)AdType<KIND>::PARTS * 16 * (p.padded * AdType<KIND>::SIZE + 16);
     const int64_t groups = cut(s.n, 4 * 16 * AD_VEC<KIND>), share = std::max<int64_t>(1, std::min<int64_t>(groups, s.tiles * groups / 256));
     const dim3 grid((unsigned)s.m, (unsigned)cut(groups, share));
-    if (s.n < AD_VEC<KIND>) ad_expand_few_kernel<KIND, true><<<grid, 256, lds, stream>>>(p);
-    else ad_expand_few_kernel<KIND, false><<<grid, 256, lds, stream>>>(p);
+    if (s.n < AD_VEC<KIND>) HB_LAUNCH((ad_expand_few_kernel<KIND, true>), grid, dim3(256), lds, stream, p);
+    else HB_LAUNCH((ad_expand_few_kernel<KIND, false>), grid, dim3(256), lds, stream, p);
     return launch_status();
   }
   const AdPlan plan{reinterpret_cast<int32_t*>(ws), s.adapters + 1};

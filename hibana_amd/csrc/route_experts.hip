@@ -367,9 +367,9 @@ __global__ __launch_bounds__(256) void route_grad_kernel(RouteGrad p) {
 template <int KIND, bool SIGMOID>
 static int route_experts_run(const RouteExperts& p, hipStream_t stream) {
   const unsigned blocks = (unsigned)((p.m + 3) / 4);
-  if (p.per <= 4) route_experts_kernel<KIND, SIGMOID, 4><<<blocks, 256, 0, stream>>>(p);
-  else if (p.per <= 8) route_experts_kernel<KIND, SIGMOID, 8><<<blocks, 256, 0, stream>>>(p);
-  else route_experts_kernel<KIND, SIGMOID, 16><<<blocks, 256, 0, stream>>>(p);
+  if (p.per <= 4) HB_LAUNCH((route_experts_kernel<KIND, SIGMOID, 4>), dim3(blocks), dim3(256), 0, stream, p);
+  else if (p.per <= 8) HB_LAUNCH((route_experts_kernel<KIND, SIGMOID, 8>), dim3(blocks), dim3(256), 0, stream, p);
+  else HB_LAUNCH((route_experts_kernel<KIND, SIGMOID, 16>), dim3(blocks), dim3(256), 0, stream, p);
   return launch_status();
 }
 
@@ -405,7 +405,7 @@ extern "C" int hb_route_experts_grad(const float* dweights, const void* logits, 
   const RouteGrad p{dweights, logits, stride, ids, m, e, k, renorm != 0, scale, dlogits};
   const unsigned blocks = (unsigned)((m + 3) / 4);
   const hipStream_t s = as_stream(stream);
-#define HB_RG(KIND) if (type == KIND) { if (scoring == HB_SIGMOID) route_grad_kernel<KIND, true><<<blocks, 256, 0, s>>>(p); else route_grad_kernel<KIND, false><<<blocks, 256, 0, s>>>(p); }
+#define HB_RG(KIND) if (type == KIND) { if (scoring == HB_SIGMOID) HB_LAUNCH((route_grad_kernel<KIND, true>), dim3(blocks), dim3(256), 0, s, p); else HB_LAUNCH((route_grad_kernel<KIND, false>), dim3(blocks), dim3(256), 0, s, p); }
   HB_RG(HB_BF16) HB_RG(HB_F16) HB_RG(HB_F32)
 #undef HB_RG
   return launch_status();

@@ -26,23 +26,27 @@ class Adapters:
     `ranks` int32 [adapters]: how many of the `rank` rows are adapter i's (None: all; the rows behind them are not read). Tensors that require gradients get them through `add`."""
 
     def __init__(self, a: torch.Tensor, b: torch.Tensor, scale: torch.Tensor | float | None = None, ranks: torch.Tensor | None = None):
+        if isinstance(scale, (int, float)):
+            scale = torch.full(a.shape[:1], float(scale), dtype=torch.float32, device=a.device)
+        self.a, self.b, self.scale, self.ranks = a, b, scale, ranks
+        self._check()
+        self._struct = self._at = None
+        self._rooms: dict[tuple[int, int], int] = {}
+
+    def _check(self) -> None:
+        a, b, scale, ranks = self.a, self.b, self.scale, self.ranks
         if a.ndim != 3 or b.ndim != 3 or a.shape[:2] != b.shape[:2] or a.dtype != b.dtype or a.dtype not in TYPES or not a.numel() or not b.numel():
             raise ValueError("Adapters: a [adapters, rank, K] and b [adapters, rank, N], both BF16, FP16 or FP32")
         if a.shape[0] > MOST or a.shape[1] > MOST_RANK:
             raise ValueError(f"Adapters: up to {MOST} adapters of a rank up to {MOST_RANK}")
         if not a.is_contiguous() or not b.is_contiguous():
             raise ValueError("Adapters: a and b must be contiguous")
-        if isinstance(scale, (int, float)):
-            scale = torch.full((a.shape[0],), float(scale), dtype=torch.float32, device=a.device)
         if scale is not None and (scale.dtype != torch.float32 or scale.shape != a.shape[:1] or not scale.is_contiguous()):
             raise ValueError("Adapters: scale FP32 [adapters]")
         if ranks is not None and (ranks.dtype != torch.int32 or ranks.shape != a.shape[:1] or not ranks.is_contiguous()):
             raise ValueError("Adapters: ranks int32 [adapters]")
         if any(t is not None and t.device != a.device for t in (b, scale, ranks)):
             raise ValueError("Adapters: one device")
-        self.a, self.b, self.scale, self.ranks = a, b, scale, ranks
-        self._struct = self._at = None
-        self._rooms: dict[tuple[int, int], int] = {}
 
     @classmethod
     def from_pairs(cls, pairs, dtype: torch.dtype = torch.bfloat16, device: torch.device | str = "cuda") -> "Adapters":
@@ -99,6 +103,8 @@ class Adapters:
         """What the library takes, made again where a tensor's place has changed (an optimizer may have put another one in)."""
         at = (self.a.data_ptr(), self.b.data_ptr(), _lib.ptr(self.scale), _lib.ptr(self.ranks))
         if at != self._at:
+            self._check()
+            self._rooms.clear()
             n, rank, k = self.a.shape
             self._struct, self._at = C.byref(_lib.HbAdapters(*at, n, rank, k, self.b.shape[2], TYPES[self.a.dtype])), at
         return self._struct
@@ -155,9 +161,10 @@ def _add(y: torch.Tensor, x: torch.Tensor, pool: Adapters, index: torch.Tensor, 
     else:
         to = _stride(out, n)
     if m:
+        struct = pool.struct()
         need = pool.room(m, 0)
         ws = yr.new_empty(need, dtype=torch.uint8)  # (of the capture's own pool in a captured call; a call's own, so that two at once share nothing)
-        code = _lib.lib().hb_adapters_add(pool.struct(), xr.data_ptr(), _stride(xr, k), yr.data_ptr(), _stride(yr, n), ix.data_ptr(), INDEX[ix.dtype], m, out.data_ptr(), to,
+        code = _lib.lib().hb_adapters_add(struct, xr.data_ptr(), _stride(xr, k), yr.data_ptr(), _stride(yr, n), ix.data_ptr(), INDEX[ix.dtype], m, out.data_ptr(), to,
                                           ws.data_ptr(), need, stream)
         if code:
             _lib.check(code, "adapters.add")
@@ -183,7 +190,7 @@ class _Add(torch.autograd.Function):
 
 
 def add(y: torch.Tensor, x: torch.Tensor, pool: Adapters, index: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
-    """y [M, N] plus each row's adapter of x [M, K], of the pool's type -> [M, N] (or `out`, which may be y itself). index int32 or int64 [M]: a row whose
+    """y [M, N] plus each row's adapter of x [M, K], of the pool's type -> [M, N] (or `out`: y itself, or memory that y's rows are not in). index int32 or int64 [M]: a row whose
     index is not of the pool (-1) is y's, bit for bit. Any order of rows: those of an adapter share one read of its matrices.
 
     Differentiable in y, x, pool.a and pool.b. A training step that is to be captured calls `grads` itself: autograd's own streams and a
@@ -207,9 +214,10 @@ def grads(dy: torch.Tensor, x: torch.Tensor, pool: Adapters, index: torch.Tensor
     if not m:
         return dx, torch.zeros(pool.a.shape, dtype=torch.float32, device=xr.device), torch.zeros(pool.b.shape, dtype=torch.float32, device=xr.device)
     da, db = xr.new_empty(pool.a.shape, dtype=torch.float32), xr.new_empty(pool.b.shape, dtype=torch.float32)
+    struct = pool.struct()
     need = pool.room(m, 1)
     ws = xr.new_empty(need, dtype=torch.uint8)
-    code = _lib.lib().hb_adapters_grads(pool.struct(), xr.data_ptr(), _stride(xr, k), dyr.data_ptr(), _stride(dyr, n), ix.data_ptr(), INDEX[ix.dtype], m, dx.data_ptr(), da.data_ptr(),
+    code = _lib.lib().hb_adapters_grads(struct, xr.data_ptr(), _stride(xr, k), dyr.data_ptr(), _stride(dyr, n), ix.data_ptr(), INDEX[ix.dtype], m, dx.data_ptr(), da.data_ptr(),
                                         db.data_ptr(), ws.data_ptr(), need, stream)
     if code:
         _lib.check(code, "adapters.grads")

@@ -114,3 +114,16 @@ def test_a_pool_can_be_copied_and_pickled():
     pool.struct()
     for twin in (copy.copy(pool), copy.deepcopy(pool), pickle.loads(pickle.dumps(pool))):
         assert torch.equal(twin.a, pool.a) and twin.struct()._obj.a == twin.a.data_ptr()
+
+
+def test_a_tensor_put_in_another_s_place_is_looked_at():
+    pool = adapters.Adapters(torch.zeros(2, 3, 8), torch.zeros(2, 3, 6), 1.0)
+    pool.struct()
+    for name, bad in [("a", torch.zeros(2, 4, 8)), ("b", torch.zeros(2, 3, 12)[..., ::2]), ("scale", torch.zeros(3)), ("ranks", torch.zeros(2))]:
+        kept = getattr(pool, name)
+        setattr(pool, name, bad)
+        with pytest.raises(ValueError):
+            pool.struct()
+        setattr(pool, name, kept)
+    pool.a = torch.zeros(2, 3, 10)
+    assert pool.struct()._obj.k == 10
