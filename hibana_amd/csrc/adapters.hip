@@ -87,20 +87,25 @@ __device__ __forceinline__ const char* ad_row(const char* rows, int r, uint32_t 
 __device__ __forceinline__ char* ad_row(char* rows, int r, uint32_t pitch) { return rows + (uint64_t)(uint32_t)r * pitch; }
 
 // A lane's sixteen bytes of a row of n elements, of which `first` is the lane's first: behind the row's end its last sixteen bytes, so that no load is behind a
-// branch (the compiler waits for all that is under way where it does not know how many loads are). TINY: rows shorter than that, element by element.
-template <int KIND, bool TINY>
+// branch (the compiler waits for all that is under way where it does not know how many loads are). AD_TINY: rows shorter than that, element by element.
+enum { AD_NEAR = 0, AD_TINY = 1, AD_PAST = 2 };  // AD_PAST: past the caches
+template <int KIND, int HOW>
 __device__ __forceinline__ u32x4_t ad_take(const char* row, int first, int n) {
-  if constexpr (TINY) return ad_load<KIND>(row + first * AdType<KIND>::SIZE, n - first);
-  return *reinterpret_cast<const u32x4_loose*>(row + (int64_t)min(first, n - AD_VEC<KIND>) * AdType<KIND>::SIZE);
+  if constexpr (HOW == AD_TINY) return ad_load<KIND>(row + first * AdType<KIND>::SIZE, n - first);
+  const u32x4_loose* at = reinterpret_cast<const u32x4_loose*>(row + (int64_t)min(first, n - AD_VEC<KIND>) * AdType<KIND>::SIZE);
+  if constexpr (HOW == AD_PAST) return __builtin_nontemporal_load(at);
+  return *at;
 }
 // The elements of the row that `ad_take` was asked for, and no others.
-template <int KIND, bool TINY>
+template <int KIND, int HOW>
 __device__ __forceinline__ void ad_put(char* row, const u32x4_t& v, int first, int n) {
   if (first + AD_VEC<KIND> <= n) {
-    *reinterpret_cast<u32x4_loose*>(row + (int64_t)first * AdType<KIND>::SIZE) = v;
+    u32x4_loose* at = reinterpret_cast<u32x4_loose*>(row + (int64_t)first * AdType<KIND>::SIZE);
+    if constexpr (HOW == AD_PAST) __builtin_nontemporal_store(v, at);
+    else *at = v;
     return;
   }
-  const int from = TINY ? first : n - AD_VEC<KIND>;
+  const int from = HOW == AD_TINY ? first : n - AD_VEC<KIND>;
 #pragma unroll
   for (int j = 0; j < AD_VEC<KIND>; j++) {
     if (from + j >= first && from + j < n) {
@@ -554,6 +559,13 @@ struct AdShrink {
 };
 constexpr int AD_WAVES = 4;
 constexpr int AD_EXPANDS = 768;   // workgroups of an expansion, about
+// Results of this many bytes are stored past the caches: half of what the dies' hold. Through them they push out what is still to be read, and whoever reads them next finds
+// little there. Add of 4096 rows of 5120 at rank 32 (42 MB of results) 52 -> 45 us a call, two of 5120 at rank 16 with gradients (21 MB of dx) 43.9 -> 42.5 (y's rows
+// read so too: 48 us).
+constexpr int64_t AD_PAST_BYTES = 16 << 20;
+// Rows of this many bytes, both sides' together, are read past the caches by the outer products, after which nobody reads them: half of the last-level cache's. 8192 rows of
+// 12800 and 2560 (252 MB, and 210 MB of dx past the caches) 274 -> 227 us the call; 42 MB are the slower for it, 43.9 -> 45.1.
+constexpr int64_t AD_PAST_ROWS = 128ll << 20;
 __host__ __device__ constexpr int ad_sixteens(int rank) { return (rank + 15) / 16; }
 __host__ __device__ constexpr int ad_thirties(int rank) { return (rank + 31) / 32; }
 
@@ -727,7 +739,7 @@ __device__ __forceinline__ u32x4_t ad_result(const u32x4_t& y, const f32x4_t (&a
 }
 
 // Few rows: a workgroup joins the splits' sums of its tile in LDS, then a tile's rows times four wavefronts' columns, sixteen lanes of sixteen bytes each.
-template <int KIND, bool TINY>
+template <int KIND, int HOW>
 __global__ __launch_bounds__(256) void ad_expand_few_kernel(AdFew p) {
   constexpr int VEC = AD_VEC<KIND>, SIZE = AdType<KIND>::SIZE, PARTS = AdType<KIND>::PARTS;
   extern __shared__ __align__(16) char staged[];  // [part][row][padded + 16 bytes]
@@ -746,14 +758,14 @@ __global__ __launch_bounds__(256) void ad_expand_few_kernel(AdFew p) {
   for (int i = 0; i < 4; i++) rows[i] = __shfl(row, 4 * group + i);
   auto base = [&](int first) {  // (rows behind the last: the first again)
 #pragma unroll
-    for (int i = 0; i < 4; i++) y[i] = ad_take<KIND, TINY>(ad_row(p.y, rows[i], p.y_stride), first, p.n);
+    for (int i = 0; i < 4; i++) y[i] = ad_take<KIND, HOW>(ad_row(p.y, rows[i], p.y_stride), first, p.n);
   };
   // what is under way: (block, 32 ranks) one after another, two ahead of the products (behind the last block the row's end: no load behind a branch)
   const char* matrix = p.b + (int64_t)c * p.in.rank * p.n * SIZE;  // (a class without an adapter reads none)
   int ahead = block * 16 * VEC + col * VEC, ahead_rank = 0;
   auto load = [&](u32x4_t (&to)[8]) {
 #pragma unroll
-    for (int s = 0; s < 8; s++) to[s] = ad_take<KIND, TINY>(ad_row(matrix, min(ahead_rank + 8 * group + s, rank - 1), (uint32_t)p.n * SIZE), min(ahead, p.n), p.n);
+    for (int s = 0; s < 8; s++) to[s] = ad_take<KIND, HOW == AD_TINY ? AD_TINY : AD_NEAR>(ad_row(matrix, min(ahead_rank + 8 * group + s, rank - 1), (uint32_t)p.n * SIZE), min(ahead, p.n), p.n);
     ahead_rank += 32;
     if (ahead_rank >= rank) ahead_rank = 0, ahead += stride * 16 * VEC;
   };
@@ -763,7 +775,7 @@ __global__ __launch_bounds__(256) void ad_expand_few_kernel(AdFew p) {
       const int first = block * 16 * VEC + col * VEC;
 #pragma unroll
       for (int i = 0; i < 4; i++)
-        if (4 * group + i < count) ad_put<KIND, TINY>(ad_row(p.out, rows[i], p.out_stride), y[i], first, p.n);
+        if (4 * group + i < count) ad_put<KIND, HOW>(ad_row(p.out, rows[i], p.out_stride), y[i], first, p.n);
       base(min(first + stride * 16 * VEC, p.n));
     }
     return;
@@ -829,7 +841,7 @@ __global__ __launch_bounds__(256) void ad_expand_few_kernel(AdFew p) {
 #pragma unroll
       for (int i = 0; i < 4; i++)
         if (4 * group + i < count)
-          ad_put<KIND, TINY>(ad_row(p.out, rows[i], p.out_stride), ad_result<KIND>(y[i], acc[0], i, KIND == HB_F16 ? ad_pow2(power[4 * group + i]) : 1.0f), first, p.n);
+          ad_put<KIND, HOW>(ad_row(p.out, rows[i], p.out_stride), ad_result<KIND>(y[i], acc[0], i, KIND == HB_F16 ? ad_pow2(power[4 * group + i]) : 1.0f), first, p.n);
 #pragma unroll
       for (int j = 0; j < VEC; j++) acc[0][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
       r0 = 0;
@@ -853,7 +865,7 @@ struct AdExpand {
   char* out;
   uint32_t out_stride;
 };
-template <int KIND, bool TINY>
+template <int KIND, int HOW>
 __global__ __launch_bounds__(256, 3) void ad_expand_kernel(AdExpand p) {
   constexpr int VEC = AD_VEC<KIND>, SIZE = AdType<KIND>::SIZE, PARTS = AdType<KIND>::PARTS;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, group = lane >> 4, col = lane & 15, tile = blockIdx.x >> 1, half = blockIdx.x & 1;
@@ -890,11 +902,11 @@ __global__ __launch_bounds__(256, 3) void ad_expand_kernel(AdExpand p) {
   const char* mine = p.w + (int64_t)c * p.in.rank * p.n * SIZE;
   auto matrix = [&](int first, int step) {
 #pragma unroll
-    for (int i = 0; i < 8; i++) v[i] = ad_take<KIND, TINY>(ad_row(mine, min(32 * step + 8 * group + i, rank - 1), (uint32_t)p.n * SIZE), first, p.n);
+    for (int i = 0; i < 8; i++) v[i] = ad_take<KIND, HOW == AD_TINY ? AD_TINY : AD_NEAR>(ad_row(mine, min(32 * step + 8 * group + i, rank - 1), (uint32_t)p.n * SIZE), first, p.n);
   };
   auto base = [&](int first) {  // (rows behind the last: it again)
 #pragma unroll
-    for (int i = 0; i < 4; i++) y[i] = p.y ? ad_take<KIND, TINY>(ad_row(p.y, rows[i], p.y_stride), first, p.n) : u32x4_t{0u, 0u, 0u, 0u};
+    for (int i = 0; i < 4; i++) y[i] = p.y ? ad_take<KIND, HOW == AD_TINY ? AD_TINY : AD_NEAR>(ad_row(p.y, rows[i], p.y_stride), first, p.n) : u32x4_t{0u, 0u, 0u, 0u};
   };
   // the wavefront's blocks, the next one's matrix under way while one is added; a rank of up to 32 keeps its sums in registers
   const int stride = gridDim.y * 4;
@@ -926,7 +938,7 @@ __global__ __launch_bounds__(256, 3) void ad_expand_kernel(AdExpand p) {
 #pragma unroll
     for (int i = 0; i < 4; i++)
       if (4 * group + i < count)  // (without an adapter the rows as they are: -0 too)
-        ad_put<KIND, TINY>(ad_row(p.out, rows[i], p.out_stride), rank == 0 ? y[i] : ad_result<KIND>(y[i], acc[0], i, unit[i]), first, p.n);
+        ad_put<KIND, HOW>(ad_row(p.out, rows[i], p.out_stride), rank == 0 ? y[i] : ad_result<KIND>(y[i], acc[0], i, unit[i]), first, p.n);
     if (more) base(first + stride * 16 * VEC);
   }
 }
@@ -953,8 +965,8 @@ struct AdOuter {
 // their sums in LDS. A lane's eight rows of sixteen bytes are turned as in the expansion; the next tile's are under way while one is
 // multiplied. An adapter's only unit writes the gradient (zeros, if it has no rows), several write partial sums for ad_join_kernel. (Joined by the last of them to
 // arrive instead, whose sums must pass the dies' caches in words: 28 us for the 16 of both kernels at 2048 rows of 5120 x 5120, rank 16.)
-template <int KIND, int RT, bool TINY>
-__global__ __launch_bounds__(256) void ad_outer_kernel(AdOuter p) {
+template <int KIND, int RT, int HOW>
+__global__ __launch_bounds__(256, RT == 1 ? 3 : 2) void ad_outer_kernel(AdOuter p) {
   constexpr int VEC = AD_VEC<KIND>, SIZE = AdType<KIND>::SIZE, PARTS = AdType<KIND>::OUTER, WORDS = SIZE == 4 ? 2 : PARTS;
   __shared__ f32x4_t join[4 * VEC * 64];  // [wavefront][column of a lane][lane]
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, group = lane >> 4, col = lane & 15;
@@ -981,66 +993,61 @@ __global__ __launch_bounds__(256) void ad_outer_kernel(AdOuter p) {
       for (int d = 1; d < 64; d <<= 1) power[t] = max(power[t], __shfl_xor(power[t], d));
     }
   }
-  // under way: the rows DEPTH tiles ahead, their numbers one more, their sums one
-  constexpr int DEPTH = 1;
-  int rows[8];
-  u32x4_t next[DEPTH][8], ahead[RT][WORDS];
-  int shift[RT];
-  auto number = [&](int tile) {
-    const int from = start + tile * AD_TILE + 8 * group;
+  // The tiles, for USED of the RT sixteens: a loop of its own for each (one that chose inside moved its sums between the register files every time, 450 registers for 240). Under
+  // way: the rows and their sums one tile ahead, the rows' numbers two.
+  auto run = [&](auto used) {
+    constexpr int USED = decltype(used)::value;
+    int rows[8], shift[USED];
+    u32x4_t next[8], ahead[USED][WORDS];
+    f32x4_t sum[USED][VEC] = {};
+    auto number = [&](int tile) {
+      const int from = start + tile * AD_TILE + 8 * group;
 #pragma unroll
-    for (int s = 0; s < 8; s++) rows[s] = p.plan.order()[min(from + s, end - 1)];
-  };
-  auto load = [&](u32x4_t (&to)[8]) {
+      for (int s = 0; s < 8; s++) rows[s] = p.plan.order()[min(from + s, end - 1)];
+    };
+    auto load = [&](int tile) {
 #pragma unroll
-    for (int s = 0; s < 8; s++) to[s] = ad_take<KIND, TINY>(ad_row(job.v, rows[s], job.stride), first, job.length);
-  };
-  auto sums = [&](int tile) {
+      for (int s = 0; s < 8; s++) next[s] = ad_take<KIND, HOW>(ad_row(job.v, rows[s], job.stride), first, job.length);
 #pragma unroll
-    for (int t = 0; t < RT; t++) {  // (behind the adapter's sixteens its last one again)
-      const int j = min(t, have - 1);
-      const char* from = job.by_rank + ((int64_t)(tile0 + tile) * sixteens + r0 / 16 + j) * PARTS * 512 * SIZE + (col * 32 + 8 * group) * SIZE;
+      for (int t = 0; t < USED; t++) {  // (behind the adapter's sixteens its last one again)
+        const int j = min(t, have - 1);
+        const char* from = job.by_rank + ((int64_t)(tile0 + tile) * sixteens + r0 / 16 + j) * PARTS * 512 * SIZE + (col * 32 + 8 * group) * SIZE;
 #pragma unroll
-      for (int i = 0; i < WORDS; i++) ahead[t][i] = *reinterpret_cast<const u32x4_t*>(from + (SIZE == 4 ? 16 * i : i * 1024));
-      if constexpr (KIND == HB_F16) shift[t] = powers[(int64_t)tile * sixteens + j];
-    }
-  };
-  // (behind the last tile it again: no load behind a branch)
-  const int last = tiles - 1;
-  if (wave < tiles) {
+        for (int i = 0; i < WORDS; i++) ahead[t][i] = *reinterpret_cast<const u32x4_t*>(from + (SIZE == 4 ? 16 * i : i * 1024));
+        if constexpr (KIND == HB_F16) shift[t] = powers[(int64_t)tile * sixteens + j];
+      }
+    };
+    const int last = tiles - 1;  // (behind the last tile it again: no load behind a branch)
     number(wave);
+    load(wave);
+    number(min(wave + 4, last));
+    for (int tile = wave; tile < tiles; tile += 4) {
+      u32x4_t v[8], s[USED][WORDS];
 #pragma unroll
-    for (int d = 0; d < DEPTH; d++) {
-      load(next[d]);
-      number(min(wave + 4 * (d + 1), last));
-    }
-    sums(wave);
-  }
-  for (int turn = wave; turn < tiles; turn += 4 * DEPTH) {
-#pragma unroll
-    for (int d = 0; d < DEPTH; d++) {
-      const int tile = turn + 4 * d;
-      if (d && tile >= tiles) break;
-      u32x4_t v[8], s[RT][WORDS];
-#pragma unroll
-      for (int i = 0; i < 8; i++) v[i] = next[d][i];
+      for (int i = 0; i < 8; i++) v[i] = next[i];
       if (start + (tile + 1) * AD_TILE > end)  // the last tile's rows behind the end: what they repeat may be infinite
 #pragma unroll
         for (int i = 0; i < 8; i++) v[i] = start + tile * AD_TILE + 8 * group + i < end ? v[i] : u32x4_t{0u, 0u, 0u, 0u};
 #pragma unroll
-      for (int t = 0; t < RT; t++)
+      for (int t = 0; t < USED; t++)
 #pragma unroll
         for (int i = 0; i < WORDS; i++) {
           s[t][i] = ahead[t][i];
           if constexpr (KIND == HB_F16) s[t][i] = ad_lower(s[t][i], shift[t] - power[t]);
         }
-      load(next[d]);
-      number(min(tile + 4 * (DEPTH + 1), last));
-      sums(min(tile + 4, last));
-      if (RT == 4 && have > 2) ad_products<KIND, RT, RT, WORDS>(s, v, acc);
-      else if (RT >= 2 && have == 2) ad_products<KIND, 2, RT, WORDS>(s, v, acc);
-      else ad_products<KIND, 1, RT, WORDS>(s, v, acc);
+      load(min(tile + 4, last));
+      number(min(tile + 8, last));
+      ad_products<KIND, USED, USED, WORDS>(s, v, sum);
     }
+#pragma unroll
+    for (int t = 0; t < USED; t++)
+#pragma unroll
+      for (int j = 0; j < VEC; j++) acc[t][j] = sum[t][j];
+  };
+  if (wave < tiles) {
+    if (RT == 4 && have > 2) run(std::integral_constant<int, RT>{});
+    else if (RT >= 2 && have == 2) run(std::integral_constant<int, RT < 2 ? 1 : 2>{});
+    else run(std::integral_constant<int, 1>{});
   }
   // D: this lane's columns first .. first + VEC - 1 of ranks 4 group .. + 3 of every sixteen
 #pragma unroll
@@ -1071,7 +1078,7 @@ __global__ __launch_bounds__(256) void ad_outer_kernel(AdOuter p) {
         if (whole) *reinterpret_cast<u32x4_loose*>(row + first + q) = v;
       }
       if (!whole) {
-        const int from = TINY ? first : job.length - VEC;  // the lane's columns, of which the ones before `first` are another's
+        const int from = HOW == AD_TINY ? first : job.length - VEC;  // the lane's columns, of which the ones before `first` are another's
 #pragma unroll
         for (int j = 0; j < VEC; j++)
           if (from + j >= first && from + j < job.length) row[from + j] = sum[j];
@@ -1202,8 +1209,9 @@ static int ad_run_expand(const AdShape& s, AdExpand& p, hipStream_t stream) {
   const int64_t groups = cut(p.n, 4 * 16 * AD_VEC<KIND>);
   const int64_t share = std::max<int64_t>(1, std::min<int64_t>(groups, cut(s.m, 16) * groups / AD_EXPANDS));
   const dim3 grid((unsigned)(2 * s.tiles), (unsigned)cut(groups, share));
-  if (p.n < AD_VEC<KIND>) HB_LAUNCH((ad_expand_kernel<KIND, true>), grid, dim3(256), 0, stream, p);
-  else HB_LAUNCH((ad_expand_kernel<KIND, false>), grid, dim3(256), 0, stream, p);
+  if (p.n < AD_VEC<KIND>) HB_LAUNCH((ad_expand_kernel<KIND, AD_TINY>), grid, dim3(256), 0, stream, p);
+  else if (s.m * p.n * s.size >= AD_PAST_BYTES) HB_LAUNCH((ad_expand_kernel<KIND, AD_PAST>), grid, dim3(256), 0, stream, p);
+  else HB_LAUNCH((ad_expand_kernel<KIND, AD_NEAR>), grid, dim3(256), 0, stream, p);
   return launch_status();
 }
 
@@ -1213,7 +1221,12 @@ static int ad_run_outer(const AdShape& s, AdOuter& p, hipStream_t stream) {
   const int longest = std::max(p.job[0].length, p.job[1].length);
   const dim3 grid((unsigned)cut(longest, 16 * AD_VEC<KIND>), (unsigned)s.units, (unsigned)(2 * p.chunks));
   const bool tiny = std::min(p.job[0].length, p.job[1].length) < AD_VEC<KIND>;
-#define HB_AD(RT) if (s.rt == RT) { if (tiny) HB_LAUNCH((ad_outer_kernel<KIND, RT, true>), grid, dim3(256), 0, stream, p); else HB_LAUNCH((ad_outer_kernel<KIND, RT, false>), grid, dim3(256), 0, stream, p); }
+#define HB_AD(RT) \
+  if (s.rt == RT) { \
+    if (tiny) HB_LAUNCH((ad_outer_kernel<KIND, RT, AD_TINY>), grid, dim3(256), 0, stream, p); \
+    else if (s.m * (s.k + s.n) * s.size >= AD_PAST_ROWS) HB_LAUNCH((ad_outer_kernel<KIND, RT, AD_PAST>), grid, dim3(256), 0, stream, p); \
+    else HB_LAUNCH((ad_outer_kernel<KIND, RT, AD_NEAR>), grid, dim3(256), 0, stream, p); \
+  }
   HB_AD(1) HB_AD(2) HB_AD(4)
 #undef HB_AD
   int code = launch_status();
@@ -1236,8 +1249,8 @@ static int ad_add(const hb_adapters* a, const AdShape& s, const AdIndex& in, con
     const size_t lds = (size_t)AdType<KIND>::PARTS * 16 * (p.padded * AdType<KIND>::SIZE + 16);
     const int64_t groups = cut(s.n, 4 * 16 * AD_VEC<KIND>), share = std::max<int64_t>(1, std::min<int64_t>(groups, s.tiles * groups / 256));
     const dim3 grid((unsigned)s.m, (unsigned)cut(groups, share));
-    if (s.n < AD_VEC<KIND>) HB_LAUNCH((ad_expand_few_kernel<KIND, true>), grid, dim3(256), lds, stream, p);
-    else HB_LAUNCH((ad_expand_few_kernel<KIND, false>), grid, dim3(256), lds, stream, p);
+    if (s.n < AD_VEC<KIND>) HB_LAUNCH((ad_expand_few_kernel<KIND, AD_TINY>), grid, dim3(256), lds, stream, p);
+    else HB_LAUNCH((ad_expand_few_kernel<KIND, AD_NEAR>), grid, dim3(256), lds, stream, p);
     return launch_status();
   }
   const AdPlan plan{reinterpret_cast<int32_t*>(ws), s.adapters + 1};
@@ -1270,10 +1283,11 @@ static int ad_grads(const hb_adapters* a, const AdShape& s, const AdIndex& in, c
                  {dyr, (uint32_t)(dy_stride * s.size), static_cast<const char*>(a->b), s.n, 0, 0, nullptr, nullptr, dy_rows, dy_ranks, dy_row_power, dy_power}},
                 a->scale, 0};
   if ((code = ad_run_shrink<KIND>(s, down, ws, stream))) return code;
-  AdExpand up{in, plan, dy_rows, dy_row_power, s.k, static_cast<const char*>(a->a), nullptr, 0, static_cast<char*>(dx), (uint32_t)(s.k * s.size)};
-  if ((code = ad_run_expand<KIND>(s, up, stream))) return code;
+  // the outer products ahead of dx: they read x and dy again while the last-level cache holds what it can of them
   AdOuter outer{in, plan, {{dy_ranks, dy_power, xr, (uint32_t)(x_stride * s.size), s.k, da, part_a}, {x_ranks, x_power, dyr, (uint32_t)(dy_stride * s.size), s.n, db, part_b}}, s.unit, 0};
-  return ad_run_outer<KIND>(s, outer, stream);
+  if ((code = ad_run_outer<KIND>(s, outer, stream))) return code;
+  AdExpand up{in, plan, dy_rows, dy_row_power, s.k, static_cast<const char*>(a->a), nullptr, 0, static_cast<char*>(dx), (uint32_t)(s.k * s.size)};
+  return ad_run_expand<KIND>(s, up, stream);
 }
 
 static int ad_check(const hb_adapters* a, const void* index, int index_bytes, int64_t m, bool grads, AdShape& s) {

@@ -24,8 +24,8 @@ def add(y, x, a, b, scale, ranks, index):
 
 
 def grads(dy, x, a, b, scale, ranks, index):
-    dx = torch.zeros(x.shape, dtype=torch.float64)
-    da, db = torch.zeros(a.shape, dtype=torch.float64), torch.zeros(b.shape, dtype=torch.float64)
+    dx = torch.zeros(x.shape, dtype=torch.float64, device=x.device)
+    da, db = torch.zeros(a.shape, dtype=torch.float64, device=x.device), torch.zeros(b.shape, dtype=torch.float64, device=x.device)
     for rows, i, ai, bi, s in _each(a, b, scale, ranks, index):
         xr, dyr = x[rows].double(), dy[rows].double()
         g = s * dyr @ bi.T
@@ -50,7 +50,7 @@ LARGEST = {torch.bfloat16: 0.0, torch.float16: 2.0 ** -39, torch.float32: 0.0}
 def add_bound(y, x, a, b, scale, ranks, index):
     """Element by element: one rounding of the result and the FP32 sums' errors."""
     dtype = y.dtype
-    bound = torch.zeros(y.shape, dtype=torch.float64)
+    bound = torch.zeros(y.shape, dtype=torch.float64, device=x.device)
     for rows, _, ai, bi, s in _each(a, b, scale, ranks, index):
         inner = x[rows].double().abs() @ ai.abs().T
         rel = _two(x.shape[1], 2 * len(ai), TWO_PARTS[dtype])
@@ -61,8 +61,8 @@ def add_bound(y, x, a, b, scale, ranks, index):
 
 def grads_bound(dy, x, a, b, scale, ranks, index):
     dtype = x.dtype
-    dx = torch.zeros(x.shape, dtype=torch.float64)
-    da, db = torch.zeros(a.shape, dtype=torch.float64), torch.zeros(b.shape, dtype=torch.float64)
+    dx = torch.zeros(x.shape, dtype=torch.float64, device=x.device)
+    da, db = torch.zeros(a.shape, dtype=torch.float64, device=x.device), torch.zeros(b.shape, dtype=torch.float64, device=x.device)
     for rows, i, ai, bi, s in _each(a, b, scale, ranks, index):
         xr, dyr, m = x[rows].double().abs(), dy[rows].double().abs(), len(rows)
         g, h = abs(s) * dyr @ bi.abs().T, abs(s) * xr @ ai.abs().T

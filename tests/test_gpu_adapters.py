@@ -314,3 +314,22 @@ def test_gradients_of_several_units_of_rows(count):
         within(g, w, bound, name)
     for g, w in zip(adapters.grads(y.cuda(), x.cuda(), pool_of(a, b, scale, ranks), index.cuda()), got):
         assert torch.equal(g, w)  # the same call, the same bits
+
+
+@pytest.mark.parametrize("kind", TYPES)
+def test_results_and_rows_past_the_caches(kind):
+    """Results of more than 16 MB, rows of more than 128: the same sums by other loads and stores (the oracle in 64 bits on the GPU). Odd widths."""
+    from hibana_amd.kernels import adapters
+    m, k, n, rank, count = 2100, 9, 32001 if kind != "f32" else 16003, 3, 2
+    g = torch.Generator(device="cuda").manual_seed(31)
+    normal = lambda *s: torch.randn(*s, device="cuda", generator=g)  # noqa: E731
+    for wide, narrow in ((n, k), (k, n)):
+        y, x = normal(m, wide).to(TYPES[kind]), normal(m, narrow).to(TYPES[kind])
+        a, b = (normal(count, rank, narrow) / narrow ** 0.5).to(TYPES[kind]), (0.3 * normal(count, rank, wide)).to(TYPES[kind])
+        case = (y, x, a, b, torch.tensor([0.5, 2.0], device="cuda"), None, (torch.arange(m, device="cuda") * 3 // m - 1).int())
+        pool, index = adapters.Adapters(a, b, case[4]), case[-1]
+        off = (adapters.add(y, x, pool, index).double() - oracle.add(*case)).abs()
+        assert bool((off <= oracle.add_bound(*case)).all())
+        del off
+        for got, want, bound in zip(adapters.grads(y, x, pool, index), oracle.grads(*case), oracle.grads_bound(*case)):
+            assert bool(((got.double() - want).abs() <= bound).all())
