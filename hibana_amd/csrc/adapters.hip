@@ -852,7 +852,39 @@ __global__ __launch_bounds__(256) void ad_expand_few_kernel(AdFew p) {
   }
 }
 
-// A plan's tiles, sixteen rows a workgroup: every wavefront for itself, over every (4 x gridDim.y)-th block of sixteen lanes' columns.
+// The partial sums of adapters with several units, in the units' order: block `block` of `blocks` for the adapter whose first slot is `slot`. (dx's expansion has them as
+// further workgroups: a launch of their own for so little is 5 us.)
+struct AdJoinJob {
+  int length;
+  float* to;           // [adapters, rank, length]
+  const float* parts;  // [slots, rank, length]
+};
+struct AdJoin {
+  AdJoinJob job[2];
+  int slots, blocks;
+};
+__device__ __forceinline__ void ad_join(const AdIndex& in, const AdPlan& plan, const AdJoinJob& job, int slot, int block, int blocks) {
+  if (slot >= plan.slots()[plan.classes]) return;
+  const AdPlace at = ad_find(plan, plan.slots(), slot);
+  if (at.first != slot) return;
+  const int units = plan.slots()[at.c + 1] - slot;
+  const int64_t size = (int64_t)in.rank * job.length;
+  const float* from = job.parts + slot * size;
+  for (int64_t i = ((int64_t)block * 256 + threadIdx.x) * 4; i < size; i += (int64_t)blocks * 1024) {
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int u = 0; u < units; u++) {
+      const u32x4_t part = ad_load<HB_F32>(reinterpret_cast<const char*>(from + u * size + i), size - i);
+#pragma unroll
+      for (int j = 0; j < 4; j++) v[j] += __uint_as_float(part[j]);
+    }
+    u32x4_t out;
+#pragma unroll
+    for (int j = 0; j < 4; j++) out[j] = __float_as_uint(v[j]);
+    ad_store<HB_F32>(reinterpret_cast<char*>(job.to + (int64_t)at.c * size + i), out, size - i);
+  }
+}
+
+// A plan's tiles, sixteen rows a workgroup: every wavefront for itself, over every (4 x share)-th block of sixteen lanes' columns.
 struct AdExpand {
   AdIndex in;
   AdPlan plan;
@@ -864,9 +896,16 @@ struct AdExpand {
   uint32_t y_stride;   // bytes
   char* out;
   uint32_t out_stride;
+  int share;           // workgroups a tile (gridDim.y, less those that join)
+  AdJoin join;
 };
 template <int KIND, int HOW>
 __global__ __launch_bounds__(256, 3) void ad_expand_kernel(AdExpand p) {
+  if ((int)blockIdx.y >= p.share) {
+    const int i = (blockIdx.y - p.share) * gridDim.x + blockIdx.x, of = p.join.slots * p.join.blocks;
+    if (i < 2 * of) ad_join(p.in, p.plan, p.join.job[i >= of], i % of / p.join.blocks, i % p.join.blocks, p.join.blocks);
+    return;
+  }
   constexpr int VEC = AD_VEC<KIND>, SIZE = AdType<KIND>::SIZE, PARTS = AdType<KIND>::PARTS;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, group = lane >> 4, col = lane & 15, tile = blockIdx.x >> 1, half = blockIdx.x & 1;
   int c, start;
@@ -909,7 +948,7 @@ __global__ __launch_bounds__(256, 3) void ad_expand_kernel(AdExpand p) {
     for (int i = 0; i < 4; i++) y[i] = p.y ? ad_take<KIND, HOW == AD_TINY ? AD_TINY : AD_NEAR>(ad_row(p.y, rows[i], p.y_stride), first, p.n) : u32x4_t{0u, 0u, 0u, 0u};
   };
   // the wavefront's blocks, the next one's matrix under way while one is added; a rank of up to 32 keeps its sums in registers
-  const int stride = gridDim.y * 4;
+  const int stride = p.share * 4;
   int block = blockIdx.y * 4 + wave;
   if (block * 16 * VEC >= p.n) return;
   base(block * 16 * VEC + col * VEC);
@@ -963,7 +1002,7 @@ struct AdOuter {
 
 // A workgroup: RT x 16 ranks times sixteen lanes' columns over a unit of an adapter's rows, the four wavefronts taking its tiles in turn and joining
 // their sums in LDS. A lane's eight rows of sixteen bytes are turned as in the expansion; the next tile's are under way while one is
-// multiplied. An adapter's only unit writes the gradient (zeros, if it has no rows), several write partial sums for ad_join_kernel. (Joined by the last of them to
+// multiplied. An adapter's only unit writes the gradient (zeros, if it has no rows), several write partial sums for ad_join. (Joined by the last of them to
 // arrive instead, whose sums must pass the dies' caches in words: 28 us for the 16 of both kernels at 2048 rows of 5120 x 5120, rank 16.)
 template <int KIND, int RT, int HOW>
 __global__ __launch_bounds__(256, RT == 1 ? 3 : 2) void ad_outer_kernel(AdOuter p) {
@@ -1087,29 +1126,6 @@ __global__ __launch_bounds__(256, RT == 1 ? 3 : 2) void ad_outer_kernel(AdOuter 
   }
 }
 
-// The partial sums of adapters with several units, in the units' order.
-__global__ __launch_bounds__(256) void ad_join_kernel(AdOuter p) {
-  const AdOuterJob& job = p.job[blockIdx.z];
-  if ((int)blockIdx.y >= p.plan.slots()[p.plan.classes]) return;
-  const AdPlace at = ad_find(p.plan, p.plan.slots(), blockIdx.y);
-  const int c = at.c, units = p.plan.slots()[c + 1] - at.first;
-  if (at.first != (int)blockIdx.y) return;  // (an adapter's workgroups are those of its first slot)
-  const int64_t size = (int64_t)p.in.rank * job.length;
-  const float* from = job.parts + (int64_t)p.plan.slots()[c] * size;
-  for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < size; i += (int64_t)gridDim.x * 1024) {
-    float v[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int u = 0; u < units; u++) {
-      const u32x4_t part = ad_load<HB_F32>(reinterpret_cast<const char*>(from + u * size + i), size - i);
-#pragma unroll
-      for (int j = 0; j < 4; j++) v[j] += __uint_as_float(part[j]);
-    }
-    u32x4_t out;
-#pragma unroll
-    for (int j = 0; j < 4; j++) out[j] = __float_as_uint(v[j]);
-    ad_store<HB_F32>(reinterpret_cast<char*>(job.to + (int64_t)c * size + i), out, size - i);
-  }
-}
-
 // ------------------------------------------------------------------------------------------------ host
 
 static size_t up256(size_t v) { return (v + 255) & ~(size_t)255; }
@@ -1208,7 +1224,8 @@ template <int KIND>
 static int ad_run_expand(const AdShape& s, AdExpand& p, hipStream_t stream) {
   const int64_t groups = cut(p.n, 4 * 16 * AD_VEC<KIND>);
   const int64_t share = std::max<int64_t>(1, std::min<int64_t>(groups, cut(s.m, 16) * groups / AD_EXPANDS));
-  const dim3 grid((unsigned)(2 * s.tiles), (unsigned)cut(groups, share));
+  p.share = (int)cut(groups, share);
+  const dim3 grid((unsigned)(2 * s.tiles), (unsigned)(p.share + cut(2ll * p.join.slots * p.join.blocks, 2 * s.tiles)));
   if (p.n < AD_VEC<KIND>) HB_LAUNCH((ad_expand_kernel<KIND, AD_TINY>), grid, dim3(256), 0, stream, p);
   else if (s.m * p.n * s.size >= AD_PAST_BYTES) HB_LAUNCH((ad_expand_kernel<KIND, AD_PAST>), grid, dim3(256), 0, stream, p);
   else HB_LAUNCH((ad_expand_kernel<KIND, AD_NEAR>), grid, dim3(256), 0, stream, p);
@@ -1229,10 +1246,6 @@ static int ad_run_outer(const AdShape& s, AdOuter& p, hipStream_t stream) {
   }
   HB_AD(1) HB_AD(2) HB_AD(4)
 #undef HB_AD
-  int code = launch_status();
-  if (code || !s.slots) return code;  // (no adapter has a second unit)
-  const unsigned blocks = (unsigned)std::min<int64_t>(cut((int64_t)s.rank * longest, 1024), 1024);
-  HB_LAUNCH((ad_join_kernel), dim3(blocks, (unsigned)s.slots, 2), dim3(256), 0, stream, p);
   return launch_status();
 }
 
@@ -1260,7 +1273,7 @@ static int ad_add(const hb_adapters* a, const AdShape& s, const AdIndex& in, con
   if (code) return code;
   AdShrink down{in, plan, {{xr, (uint32_t)(x_stride * s.size), static_cast<const char*>(a->a), s.k, 0, 0, nullptr, nullptr, by_row, nullptr, power, nullptr}, {}}, a->scale, 0};
   if ((code = ad_run_shrink<KIND>(s, down, ws, stream))) return code;
-  AdExpand up{in, plan, by_row, power, s.n, static_cast<const char*>(a->b), yr, (uint32_t)(y_stride * s.size), to, (uint32_t)(out_stride * s.size)};
+  AdExpand up{in, plan, by_row, power, s.n, static_cast<const char*>(a->b), yr, (uint32_t)(y_stride * s.size), to, (uint32_t)(out_stride * s.size), 0, {}};
   return ad_run_expand<KIND>(s, up, stream);
 }
 
@@ -1286,7 +1299,8 @@ static int ad_grads(const hb_adapters* a, const AdShape& s, const AdIndex& in, c
   // the outer products ahead of dx: they read x and dy again while the last-level cache holds what it can of them
   AdOuter outer{in, plan, {{dy_ranks, dy_power, xr, (uint32_t)(x_stride * s.size), s.k, da, part_a}, {x_ranks, x_power, dyr, (uint32_t)(dy_stride * s.size), s.n, db, part_b}}, s.unit, 0};
   if ((code = ad_run_outer<KIND>(s, outer, stream))) return code;
-  AdExpand up{in, plan, dy_rows, dy_row_power, s.k, static_cast<const char*>(a->a), nullptr, 0, static_cast<char*>(dx), (uint32_t)(s.k * s.size)};
+  AdExpand up{in, plan, dy_rows, dy_row_power, s.k, static_cast<const char*>(a->a), nullptr, 0, static_cast<char*>(dx), (uint32_t)(s.k * s.size), 0,
+              {{{s.k, da, part_a}, {s.n, db, part_b}}, (int)s.slots, (int)std::min<int64_t>(cut((int64_t)s.rank * std::max(s.k, s.n), 1024), 1024)}};
   return ad_run_expand<KIND>(s, up, stream);
 }
 
