@@ -205,16 +205,29 @@ __device__ __forceinline__ void ad_plan_classes(const AdPlanParams& p, int32_t (
   __syncthreads();
 }
 
+// The lanes of the same class, of eight times 64 rows side by side, by the ballots of its bits: as many steps for rows of one class as of 64. (A lane without a row,
+// c < 0, gets nothing to use.)
+__device__ __forceinline__ void ad_same(const int (&c)[8], int bits, uint64_t (&same)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; i++) same[i] = __ballot(c[i] >= 0);
+  for (int b = 0; b < bits; b++)
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const uint64_t on = __ballot(c[i] >> b & 1);
+      same[i] &= c[i] >> b & 1 ? on : ~on;
+    }
+}
+
 // One workgroup: a stable counting sort (rows of a class stay in ascending order, so sums over them are the same every time). What it takes is latency, so the
 // steps are few and side by side. Up to AD_HELD rows whose 64-row pieces have a counter each for every class: a wavefront has up to eight pieces, each lane their
-// classes and its places among them in registers; a wavefront a class adds the pieces' counts up. 8192 rows of 4 adapters 9.1 us, 4096 of 6 5.8 (a wavefront's pieces
-// one after another through one counter a class: 13.0 and 7.8).
+// classes and its places among them in registers; a wavefront a class adds the pieces' counts up. 8192 rows of 4 adapters 7.2 us, of 64 11, 4096 of 4 5.8 (through the
+// other kernel's one counter a class and wavefront: 8192 rows of 64 adapters 15.7).
 constexpr int AD_HELD = 8192;
-constexpr int AD_COUNTERS = 8192;
+constexpr int AD_COUNTERS = 15360;  // of 64 KB of LDS, less the prefix sums'
 __global__ __launch_bounds__(1024) void ad_plan_pieces_kernel(AdPlanParams p) {
   extern __shared__ int32_t counters[];  // [piece][class], then [class]
   __shared__ int32_t carry[16][4];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, classes = p.plan.classes, m = p.in.m, pieces = (m + 63) / 64;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, classes = p.plan.classes, m = p.in.m, pieces = (m + 63) / 64, bits = 32 - __builtin_clz(classes - 1);
   int32_t* all = counters + pieces * classes;
   int c[8], place[8];
 #pragma unroll
@@ -225,17 +238,12 @@ __global__ __launch_bounds__(1024) void ad_plan_pieces_kernel(AdPlanParams p) {
   for (int64_t i = threadIdx.x; i < p.clear; i += 1024) p.tickets[i] = 0;
   for (int i = threadIdx.x; i < pieces * classes; i += 1024) counters[i] = 0;
   __syncthreads();
+  uint64_t same[8];
+  ad_same(c, bits, same);
 #pragma unroll
   for (int i = 0; i < 8; i++) {
-    place[i] = 0;
-    uint64_t left = __ballot(c[i] >= 0);
-    while (left) {
-      const int v = __builtin_amdgcn_readlane(c[i], __builtin_ctzll(left));
-      const uint64_t same = __ballot(c[i] == v);
-      if (c[i] == v) place[i] = __popcll(same & ((1ull << lane) - 1ull));
-      if (lane == 0) counters[(wave + 16 * i) * classes + v] = __popcll(same);
-      left &= ~same;
-    }
+    place[i] = __popcll(same[i] & ((1ull << lane) - 1ull));
+    if (c[i] >= 0 && place[i] == 0) counters[(wave + 16 * i) * classes + c[i]] = __popcll(same[i]);
   }
   __syncthreads();
   for (int v = wave; v < classes; v += 16) {
@@ -257,40 +265,39 @@ __global__ __launch_bounds__(1024) void ad_plan_pieces_kernel(AdPlanParams p) {
     if (c[i] >= 0) order[all[c[i]] + counters[(wave + 16 * i) * classes + c[i]] + place[i]] = (wave + 16 * i) * 64 + lane;
 }
 
-// Any number of rows: `segments` wavefronts with a stretch of the rows each, 64 after 64, twice over.
+// Any number of rows: `segments` wavefronts with a stretch of the rows each, 512 after 512, twice over, the next ones' classes under way. What one compute unit can read: 65536
+// rows of 4 adapters 59 us, of 512 107, and of 4096 (three wavefronts' counters are all that fit) 307.
 __global__ __launch_bounds__(1024) void ad_plan_kernel(AdPlanParams p) {
-  extern __shared__ int32_t counters[];  // [segment][class], then [wavefront][512] classes of rows
+  extern __shared__ int32_t counters[];  // [segment][class]
   __shared__ int32_t carry[16][4];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, classes = p.plan.classes, m = p.in.m;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, classes = p.plan.classes, m = p.in.m, bits = 32 - __builtin_clz(classes - 1);
   const int stretch = ((m + p.segments - 1) / p.segments + 63) / 64 * 64;
   const int from = wave < p.segments ? (int)min((int64_t)wave * stretch, (int64_t)m) : m, upto = min(from + stretch, m);
   for (int64_t i = threadIdx.x; i < p.clear; i += 1024) p.tickets[i] = 0;
   for (int i = threadIdx.x; i < p.segments * classes; i += 1024) counters[i] = 0;
   __syncthreads();
   volatile int32_t* mine = counters + wave * classes;  // (of a wavefront that has rows)
-  volatile int32_t* batch = counters + p.segments * classes + wave * 512;
   // f(row, its place among the rows of its class) for the wavefront's rows; the classes' counters move up by them
   auto each = [&](auto&& f) {
+    int next[8];
+    auto load = [&](int r0) {  // (behind the last row it again: no load behind a branch)
+#pragma unroll
+      for (int i = 0; i < 8; i++) next[i] = ad_class(p.in, min(r0 + 64 * i + lane, m - 1));
+    };
+    load(from);
     for (int r0 = from; r0 < upto; r0 += 512) {
       int c[8];
+      uint64_t same[8];
 #pragma unroll
-      for (int i = 0; i < 8; i++) c[i] = r0 + 64 * i + lane < upto ? ad_class(p.in, r0 + 64 * i + lane) : -1;
+      for (int i = 0; i < 8; i++) c[i] = r0 + 64 * i + lane < upto ? next[i] : -1;
+      load(min(r0 + 512, m - 1));
+      ad_same(c, bits, same);
 #pragma unroll
-      for (int i = 0; i < 8; i++) batch[64 * i + lane] = c[i];
-#pragma unroll 1
-      for (int i = 0; i < min(512, upto - r0); i += 64) {
-        const int mine_c = batch[i + lane];
-        int place = 0;
-        uint64_t left = __ballot(mine_c >= 0);
-        while (left) {
-          const int v = __builtin_amdgcn_readlane(mine_c, __builtin_ctzll(left));
-          const uint64_t same = __ballot(mine_c == v);
-          const int have = mine[v];
-          if (mine_c == v) place = have + __popcll(same & ((1ull << lane) - 1ull));
-          if (lane == 0) mine[v] = have + __popcll(same);
-          left &= ~same;
-        }
-        if (mine_c >= 0) f(r0 + i + lane, place);
+      for (int i = 0; i < 8; i++) {
+        if (c[i] < 0) continue;
+        const int have = mine[c[i]], before = __popcll(same[i] & ((1ull << lane) - 1ull));
+        if (before == 0) mine[c[i]] = have + __popcll(same[i]);  // (behind every lane's read: a wavefront's come in order)
+        f(r0 + 64 * i + lane, have + before);
       }
     }
   };
@@ -1193,11 +1200,11 @@ static bool ad_shape(const hb_adapters* a, int64_t m, bool grads, AdShape& s) {
 static int ad_run_plan(const AdShape& s, const AdIndex& in, const AdPlan& plan, char* ws, hipStream_t stream) {
   AdPlanParams p{in, plan, s.unit, 1, reinterpret_cast<int32_t*>(ws + s.plan_bytes), s.tickets};
   const int64_t pieces = cut(s.m, 64);
-  if (s.m <= AD_HELD && pieces * plan.classes <= AD_COUNTERS) {
+  if (s.m <= AD_HELD && (pieces + 1) * plan.classes <= AD_COUNTERS) {
     HB_LAUNCH((ad_plan_pieces_kernel), dim3(1), dim3(1024), (size_t)(pieces + 1) * plan.classes * 4, stream, p);
   } else {
-    while (p.segments < 16 && (int64_t)(2 * p.segments) * plan.classes <= AD_COUNTERS / 2) p.segments *= 2;
-    HB_LAUNCH((ad_plan_kernel), dim3(1), dim3(1024), (size_t)p.segments * plan.classes * 4 + 16 * 512 * 4, stream, p);
+    p.segments = std::max(1, std::min(16, AD_COUNTERS / plan.classes));
+    HB_LAUNCH((ad_plan_kernel), dim3(1), dim3(1024), (size_t)p.segments * plan.classes * 4, stream, p);
   }
   return launch_status();
 }
