@@ -16,6 +16,7 @@
 namespace hb {
 
 constexpr int ROUTE_MOST_K = 63;  // a selection a lane, and one more to compare the last with
+constexpr int ROUTE_MOST_ROWS = 1 << 25;  // (a launch's lanes are counted in 32 bits)
 
 struct RouteExperts {
   const void* logits;
@@ -380,7 +381,7 @@ using namespace hb;
 extern "C" int hb_route_experts(const void* logits, int type, int64_t stride, int m, int e, int k, int scoring, const float* bias, int groups, int kept, int renorm, float scale,
                                 const int32_t* slots, int steps, int32_t* ids, float* weights, void* stream) {
   if (!logits || !ids || !weights) return HB_ENULL;
-  if (type < HB_BF16 || type > HB_F32 || (scoring != HB_SOFTMAX && scoring != HB_SIGMOID) || m <= 0 || e <= 0 || e > 64 * ROUTE_PER_LANE || k <= 0 || k > ROUTE_MOST_K ||
+  if (type < HB_BF16 || type > HB_F32 || (scoring != HB_SOFTMAX && scoring != HB_SIGMOID) || m <= 0 || m > ROUTE_MOST_ROWS || e <= 0 || e > 64 * ROUTE_PER_LANE || k <= 0 || k > ROUTE_MOST_K ||
       groups <= 0 || groups > 64 || e % groups || kept <= 0 || kept > groups || k > kept * (e / groups) || steps <= 0 || (m > 1 && stride < e))
     return HB_EINVAL;
   RouteExperts p{logits, stride, bias, slots, m, e, k, steps, groups, kept, e / groups, 1, 0, 0, 0, renorm != 0, scale, ids, weights};
@@ -398,7 +399,7 @@ extern "C" int hb_route_experts(const void* logits, int type, int64_t stride, in
 extern "C" int hb_route_experts_grad(const float* dweights, const void* logits, int type, int64_t stride, const int32_t* ids, int m, int e, int k, int scoring, int renorm,
                                      float scale, void* dlogits, void* stream) {
   if (!dweights || !logits || !ids || !dlogits) return HB_ENULL;
-  if (type < HB_BF16 || type > HB_F32 || (scoring != HB_SOFTMAX && scoring != HB_SIGMOID) || m <= 0 || e <= 0 || e > 64 * ROUTE_PER_LANE || k <= 0 || k > ROUTE_MOST_K ||
+  if (type < HB_BF16 || type > HB_F32 || (scoring != HB_SOFTMAX && scoring != HB_SIGMOID) || m <= 0 || m > ROUTE_MOST_ROWS || e <= 0 || e > 64 * ROUTE_PER_LANE || k <= 0 || k > ROUTE_MOST_K ||
       (m > 1 && stride < e))
     return HB_EINVAL;
   if (!aligned(logits, type == HB_F32 ? 4 : 2) || !aligned(dweights, 4) || !aligned(ids, 4) || !aligned(dlogits, 16)) return HB_EINVAL;

@@ -28,10 +28,14 @@ class Adapters:
     def __init__(self, a: torch.Tensor, b: torch.Tensor, scale: torch.Tensor | float | None = None, ranks: torch.Tensor | None = None):
         if isinstance(scale, (int, float)):
             scale = torch.full(a.shape[:1], float(scale), dtype=torch.float32, device=a.device)
+        self._rooms: dict[tuple[int, int], int] = {}
         self.a, self.b, self.scale, self.ranks = a, b, scale, ranks
         self._check()
-        self._struct = self._at = None
-        self._rooms: dict[tuple[int, int], int] = {}
+
+    def __setattr__(self, name, value):
+        object.__setattr__(self, name, value)
+        if name in ("a", "b", "scale", "ranks"):  # what the library was given last is not of these
+            object.__setattr__(self, "_at", None)
 
     def _check(self) -> None:
         a, b, scale, ranks = self.a, self.b, self.scale, self.ranks
@@ -41,8 +45,8 @@ class Adapters:
             raise ValueError(f"Adapters: up to {MOST} adapters of a rank up to {MOST_RANK}")
         if not a.is_contiguous() or not b.is_contiguous():
             raise ValueError("Adapters: a and b must be contiguous")
-        if scale is not None and (scale.dtype != torch.float32 or scale.shape != a.shape[:1] or not scale.is_contiguous()):
-            raise ValueError("Adapters: scale FP32 [adapters]")
+        if scale is not None and (scale.dtype != torch.float32 or scale.shape != a.shape[:1] or not scale.is_contiguous() or scale.requires_grad):
+            raise ValueError("Adapters: scale FP32 [adapters], which takes no gradient")
         if ranks is not None and (ranks.dtype != torch.int32 or ranks.shape != a.shape[:1] or not ranks.is_contiguous()):
             raise ValueError("Adapters: ranks int32 [adapters]")
         if any(t is not None and t.device != a.device for t in (b, scale, ranks)):
@@ -97,16 +101,23 @@ class Adapters:
         return (self.a.numel() + self.b.numel()) * self.a.element_size()
 
     def __getstate__(self):
-        return {**self.__dict__, "_struct": None, "_at": None, "_rooms": {}}
+        """A copy or a pickle takes the tensors, not the structure of their addresses."""
+        return {name: v for name, v in self.__dict__.items() if name not in ("_struct", "_at", "_rooms")}
+
+    def __setstate__(self, state):
+        self._rooms = {}
+        for name, v in state.items():
+            setattr(self, name, v)
 
     def struct(self):
-        """What the library takes, made again where a tensor's place has changed (an optimizer may have put another one in)."""
-        at = (self.a.data_ptr(), self.b.data_ptr(), _lib.ptr(self.scale), _lib.ptr(self.ranks))
+        """What the library takes, made again where a tensor is another one, or its place or shape has changed (an optimizer may have put other memory in)."""
+        a, b, scale, ranks = self.a, self.b, self.scale, self.ranks
+        at = (a.data_ptr(), b.data_ptr(), _lib.ptr(scale), _lib.ptr(ranks), a.shape, b.shape, a.stride(), b.stride())
         if at != self._at:
             self._check()
             self._rooms.clear()
-            n, rank, k = self.a.shape
-            self._struct, self._at = C.byref(_lib.HbAdapters(*at, n, rank, k, self.b.shape[2], TYPES[self.a.dtype])), at
+            n, rank, k = a.shape
+            self._struct, self._at = C.byref(_lib.HbAdapters(*at[:4], n, rank, k, b.shape[2], TYPES[a.dtype])), at
         return self._struct
 
     def room(self, m: int, grads: int) -> int:
@@ -191,11 +202,12 @@ class _Add(torch.autograd.Function):
 
 def add(y: torch.Tensor, x: torch.Tensor, pool: Adapters, index: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
     """y [M, N] plus each row's adapter of x [M, K], of the pool's type -> [M, N] (or `out`: y itself, or memory that y's rows are not in). index int32 or int64 [M]: a row whose
-    index is not of the pool (-1) is y's, bit for bit. Any order of rows: those of an adapter share one read of its matrices.
+    index is not of the pool (-1) is y's, bit for bit. Any order of rows: those of an adapter share one read of its matrices. An infinity in b (of the gradients: in a, x or
+    dy) may come out as NaN: it is multiplied with values that are held in parts, some of them zero.
 
     Differentiable in y, x, pool.a and pool.b. A training step that is to be captured calls `grads` itself: autograd's own streams and a
     capture do not go together, and the process would end; so a call that records a gradient is refused there."""
-    if torch.is_grad_enabled() and (y.requires_grad or x.requires_grad or pool.a.requires_grad or pool.b.requires_grad):
+    if torch.is_grad_enabled() and (y.requires_grad or x.requires_grad or pool.a.requires_grad or pool.b.requires_grad or (out is not None and out.requires_grad)):
         if out is not None:
             raise ValueError("adapters.add: no `out` where a gradient is recorded")
         if y.is_cuda and torch.cuda.is_current_stream_capturing():

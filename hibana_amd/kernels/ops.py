@@ -190,8 +190,8 @@ class Routing:
 
 
 def _route_logits(logits: torch.Tensor, scoring: str, what: str) -> torch.Tensor:
-    if logits.dtype not in mxfp4.TYPES or logits.ndim != 2 or scoring not in SCORING:
-        raise ValueError(f"{what}: BF16, FP16 or FP32 logits [M, E], scoring softmax or sigmoid")
+    if logits.dtype not in mxfp4.TYPES or logits.ndim != 2 or scoring not in SCORING or logits.shape[0] > 1 << 25:
+        raise ValueError(f"{what}: BF16, FP16 or FP32 logits [M, E] of up to 2^25 rows, scoring softmax or sigmoid")
     return logits if logits.is_contiguous() or (logits.stride(1) == 1 and logits.stride(0) >= logits.shape[1]) else logits.contiguous()
 
 

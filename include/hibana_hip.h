@@ -628,7 +628,8 @@ typedef struct {
 } hb_adapters;
 size_t hb_adapters_workspace_bytes(const hb_adapters* adapters, int64_t m, int grads);
 
-/* out [m, n] = y + scale_i (x a_i^T) b_i, rounded once; rows without an adapter are y's. out may be y (of the same stride). */
+/* out [m, n] = y + scale_i (x a_i^T) b_i, rounded once; rows without an adapter are y's. out may be y (of the same stride). An infinity in
+ * b (below: in a, x or dy) may come out as NaN, since the inner sums it is multiplied with are held in parts, some of them zero. */
 int hb_adapters_add(const hb_adapters* adapters, const void* x, int64_t x_stride, const void* y, int64_t y_stride, const void* index, int index_bytes, int64_t m,
                     void* out, int64_t out_stride, void* workspace, size_t workspace_bytes, void* stream);
 /* Its gradients, given dy [m, n]: dx [m, k] of `type` (whole rows; zeros for rows without an adapter), da FP32 [adapters, rank, k] and db FP32
@@ -638,7 +639,7 @@ int hb_adapters_grads(const hb_adapters* adapters, const void* x, int64_t x_stri
 
 /* ------------------------------------------------------------------ routing of rows to experts
  *
- * Scores s = softmax or sigmoid of the logits [m, e] (HB_BF16 / HB_F16 / HB_F32, rows `stride` elements apart), e up to 1024. The choice goes by c = s + bias
+ * Scores s = softmax or sigmoid of the logits [m, e] (HB_BF16 / HB_F16 / HB_F32, rows `stride` elements apart), e up to 1024, m up to 2^25. The choice goes by c = s + bias
  * (FP32 [e] or NULL): a group's score is the sum of its best two c (groups of e / groups consecutive experts, up to 64), and of the experts in the best `kept`
  * groups the k largest c are chosen, largest first; equal ones by the lower number. Without a bias the order is the logits' own, else (and between groups) that
  * of the values in FP64.

@@ -127,3 +127,11 @@ def test_a_tensor_put_in_another_s_place_is_looked_at():
         setattr(pool, name, kept)
     pool.a = torch.zeros(2, 3, 10)
     assert pool.struct()._obj.k == 10
+
+
+def test_a_scale_takes_no_gradient():
+    with pytest.raises(ValueError, match="scale"):
+        adapters.Adapters(torch.zeros(2, 4, 8), torch.zeros(2, 4, 8), torch.ones(2, requires_grad=True))
+    pool = adapters.Adapters(torch.zeros(2, 4, 8), torch.zeros(2, 4, 8))
+    with pytest.raises(ValueError, match="out"):
+        adapters.add(torch.zeros(1, 8), torch.zeros(1, 8), pool, torch.zeros(1, dtype=torch.int64), out=torch.zeros(1, 8, requires_grad=True))

@@ -333,3 +333,44 @@ def test_results_and_rows_past_the_caches(kind):
         del off
         for got, want, bound in zip(adapters.grads(y, x, pool, index), oracle.grads(*case), oracle.grads_bound(*case)):
             assert bool(((got.double() - want).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("m,count", [(257, 3), (320, 2559), (320, 2560), (4096, 200), (8192, 118), (8192, 119), (8193, 4), (12000, 300), (20000, 4096)])
+def test_rows_among_many_adapters(m, count):
+    """The grouping of rows by adapter at the sizes where its kernels, their wavefronts and their counters change. Small whole numbers: every sum is exact."""
+    from hibana_amd.kernels import adapters
+    g = torch.Generator().manual_seed(m + count)
+    whole = lambda *s: torch.randint(-1, 2, s, generator=g)  # noqa: E731
+    y, x, a, b = whole(m, 16), whole(m, 8), whole(count, 2, 8), whole(count, 2, 16)
+    index = torch.randint(-1, count, (m,), generator=g)
+    index[m // 2:m // 2 + 200] = count - 1  # a run of one adapter's among them
+    of = index.clamp(min=0)
+    there = (index >= 0).long()[:, None]
+    inner = (x[:, None, :] * a[of]).sum(2) * there
+    back = (y[:, None, :] * b[of]).sum(2) * there
+    pool = adapters.Adapters(a.bfloat16().cuda(), b.bfloat16().cuda())
+    y16, x16, where = y.bfloat16().cuda(), x.bfloat16().cuda(), index.cuda()
+    assert torch.equal(adapters.add(y16, x16, pool, where).cpu().long(), y + (inner[:, :, None] * b[of]).sum(1))
+    dx, da, db = (t.cpu().long() for t in adapters.grads(y16, x16, pool, where))
+    assert torch.equal(dx, (back[:, :, None] * a[of]).sum(1))
+    assert torch.equal(da, torch.zeros_like(a).index_add_(0, of, back[:, :, None] * x[:, None, :]))
+    assert torch.equal(db, torch.zeros_like(b).index_add_(0, of, inner[:, :, None] * y[:, None, :]))
+
+
+def test_a_pool_cut_and_put_elsewhere():
+    """Fewer adapters at the same addresses, memory of another shape put in a parameter's place, a copy of a pool in use."""
+    import copy
+    from hibana_amd.kernels import adapters
+    y, x, a, b, scale, _, _ = (None if t is None else t.cuda() for t in make(6, 40, 24, 8, 3, torch.float32, seed=40))
+    index = torch.arange(6, device="cuda") % 3
+    pool = adapters.Adapters(a, b)
+    three = adapters.add(y, x, pool, index)
+    other = copy.deepcopy(pool)
+    other.b.zero_()
+    assert torch.equal(adapters.add(y, x, other, index), y) and torch.equal(adapters.add(y, x, pool, index), three)
+    pool.a, pool.b = pool.a[:1], pool.b[:1]
+    one = adapters.add(y, x, pool, index)
+    assert torch.equal(one[index > 0], y[index > 0]) and torch.equal(one[index == 0], three[index == 0])
+    pool.a, pool.b = a, b
+    pool.a.data, pool.b.data = a.data[:, :4].contiguous(), b.data[:, :4].contiguous()
+    assert torch.equal(adapters.add(y, x, pool, index), adapters.add(y, x, adapters.Adapters(a.clone(), b.clone()), index))

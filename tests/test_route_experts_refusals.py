@@ -45,3 +45,10 @@ def test_tensors():
         ops.route_experts(logits, 4)
     with pytest.raises(RuntimeError):
         ops.route_experts_grad(dw, logits, ids)
+
+
+def test_rows_past_what_a_launch_counts():
+    assert _lib.lib().hb_route_experts(*{**CALL, "m": (1 << 25) + 1}.values()) == _lib.HB_EINVAL
+    assert _lib.lib().hb_route_experts_grad(*{**GRAD, "m": (1 << 25) + 1}.values()) == _lib.HB_EINVAL
+    with pytest.raises(ValueError, match="rows"):
+        ops.route_experts(torch.empty((1 << 32) + 1, 1, dtype=torch.bfloat16, device="meta"), 1)
