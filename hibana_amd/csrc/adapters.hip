@@ -19,8 +19,12 @@ namespace hb {
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8_t;
 typedef uint32_t u32x4_loose __attribute__((ext_vector_type(4), aligned(2)));  // sixteen bytes at any element: rows of odd length
 
-constexpr int AD_SPLITS = 8;       // of the long axis, at most, in a call of few rows
-constexpr int AD_SELF_ROWS = 256;  // rows up to which a workgroup finds its tile from the index itself
+// Splits of the long axis, at most, in a call of few rows; its readers join them. One row of 5120 at rank 16, both kernels with nothing in the caches: one split 16.2 us, five
+// 11.9, ten 10.4; 64 rows of 32 adapters of up to 64 ranks do not care.
+constexpr int AD_SPLITS = 12;
+// Rows up to which a workgroup finds its tile from the index itself, in two launches for three. 256 rows of 5120 x 5120, eight adapters, rank 16: 13.3 us a call in a graph, with a
+// plan 17.8; of 32 adapters 15.0 and 19.7; 512 rows of 32 adapters 26 and 21.
+constexpr int AD_SELF_ROWS = 256;
 constexpr int AD_TILE = 32;        // rows of a planned call's tile: the places of a matrix instruction's contraction in an outer product
 constexpr int AD_MOST = 4096;      // adapters
 constexpr int AD_RANK = 256;
@@ -205,22 +209,24 @@ __device__ __forceinline__ void ad_plan_classes(const AdPlanParams& p, int32_t (
   __syncthreads();
 }
 
-// The lanes of the same class, of eight times 64 rows side by side, by the ballots of its bits: as many steps for rows of one class as of 64. (A lane without a row,
+// The lanes of the same class, of up to eight times 64 rows side by side, by the ballots of its bits: as many steps for rows of one class as of 64. (A lane without a row,
 // c < 0, gets nothing to use.)
-__device__ __forceinline__ void ad_same(const int (&c)[8], int bits, uint64_t (&same)[8]) {
+__device__ __forceinline__ void ad_same(const int (&c)[8], int bits, int pieces, uint64_t (&same)[8]) {
 #pragma unroll
   for (int i = 0; i < 8; i++) same[i] = __ballot(c[i] >= 0);
   for (int b = 0; b < bits; b++)
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-      const uint64_t on = __ballot(c[i] >> b & 1);
-      same[i] &= c[i] >> b & 1 ? on : ~on;
+      if (i >= pieces) break;  // uniform
+      const int mine = __builtin_amdgcn_sbfe(c[i], b, 1);  // 0 or -1
+      const uint64_t on = __ballot(mine != 0);
+      same[i] &= (uint64_t)(~((uint32_t)(on >> 32) ^ mine)) << 32 | (~((uint32_t)on ^ mine));
     }
 }
 
 // One workgroup: a stable counting sort (rows of a class stay in ascending order, so sums over them are the same every time). What it takes is latency, so the
 // steps are few and side by side. Up to AD_HELD rows whose 64-row pieces have a counter each for every class: a wavefront has up to eight pieces, each lane their
-// classes and its places among them in registers; a wavefront a class adds the pieces' counts up. 8192 rows of 4 adapters 7.2 us, of 64 11, 4096 of 4 5.8 (through the
+// classes and its places among them in registers; a wavefront a class adds the pieces' counts up. 8192 rows of 4 adapters 7.6 us, of 64 11, 4096 of 4 5.4 (through the
 // other kernel's one counter a class and wavefront: 8192 rows of 64 adapters 15.7).
 constexpr int AD_HELD = 8192;
 constexpr int AD_COUNTERS = 15360;  // of 64 KB of LDS, less the prefix sums'
@@ -239,7 +245,7 @@ __global__ __launch_bounds__(1024) void ad_plan_pieces_kernel(AdPlanParams p) {
   for (int i = threadIdx.x; i < pieces * classes; i += 1024) counters[i] = 0;
   __syncthreads();
   uint64_t same[8];
-  ad_same(c, bits, same);
+  ad_same(c, bits, (pieces - wave + 15) / 16, same);
 #pragma unroll
   for (int i = 0; i < 8; i++) {
     place[i] = __popcll(same[i] & ((1ull << lane) - 1ull));
@@ -266,7 +272,7 @@ __global__ __launch_bounds__(1024) void ad_plan_pieces_kernel(AdPlanParams p) {
 }
 
 // Any number of rows: `segments` wavefronts with a stretch of the rows each, 512 after 512, twice over, the next ones' classes under way. What one compute unit can read: 65536
-// rows of 4 adapters 59 us, of 512 107, and of 4096 (three wavefronts' counters are all that fit) 307.
+// rows of 4 adapters 57 us, of 512 100, and of 4096 (three wavefronts' counters are all that fit) 280.
 __global__ __launch_bounds__(1024) void ad_plan_kernel(AdPlanParams p) {
   extern __shared__ int32_t counters[];  // [segment][class]
   __shared__ int32_t carry[16][4];
@@ -291,7 +297,7 @@ __global__ __launch_bounds__(1024) void ad_plan_kernel(AdPlanParams p) {
 #pragma unroll
       for (int i = 0; i < 8; i++) c[i] = r0 + 64 * i + lane < upto ? next[i] : -1;
       load(min(r0 + 512, m - 1));
-      ad_same(c, bits, same);
+      ad_same(c, bits, 8, same);
 #pragma unroll
       for (int i = 0; i < 8; i++) {
         if (c[i] < 0) continue;
@@ -350,36 +356,64 @@ __device__ __forceinline__ int ad_tile(const AdPlan& plan, int t, int& c, int& s
   return min(AD_TILE, at.next_row - start);
 }
 
-// Few rows, no plan: a tile of up to sixteen begins at every sixteenth row of a class, and every wavefront finds its own from the index itself. Lane l gets
-// the number of the tile's row l % 16 (behind the last one the first again); 0 rows: none begins at row t.
-__device__ __forceinline__ int ad_tile_at(const AdIndex& p, int t, int& c, int& row) {
-  const int lane = threadIdx.x & 63;
-  int mine[AD_SELF_ROWS / 64];
+// Few rows, no plan: a tile of up to sixteen begins at every sixteenth row of a class, and every wavefront finds tile t from the index itself, by the ballots of the
+// classes' bits. Lane l gets the number of the tile's row l % 16 (behind the last one the first again); 0 rows: no such tile.
+template <int GROUPS>
+__device__ __forceinline__ int ad_tile_of(const AdIndex& p, int t, int& c, int& row) {  // of up to GROUPS times 64 rows
+  const int lane = threadIdx.x & 63, groups = (p.m + 63) / 64;
+  int mine[GROUPS], ahead[GROUPS];  // a row's class, how many rows of it are ahead of it
+  uint64_t there[GROUPS], same[GROUPS][GROUPS];
 #pragma unroll
-  for (int j = 0; j < AD_SELF_ROWS / 64; j++) mine[j] = 64 * j < p.m ? ad_class(p, min(64 * j + lane, p.m - 1)) : -1;
-  c = __builtin_amdgcn_readfirstlane(ad_class(p, t));
-  uint64_t same[AD_SELF_ROWS / 64];
-  int ahead = 0, all = 0;
+  for (int j = 0; j < GROUPS; j++) {
+    mine[j] = j < groups ? ad_class(p, min(64 * j + lane, p.m - 1)) : 0;
+    there[j] = __ballot(64 * j + lane < p.m);
 #pragma unroll
-  for (int j = 0; j < AD_SELF_ROWS / 64; j++) {
-    same[j] = __ballot(64 * j + lane < p.m && mine[j] == c);
-    if (64 * j + 63 < t) ahead += __popcll(same[j]);
-    else if (64 * j <= t) ahead += __popcll(same[j] & ((1ull << (t - 64 * j)) - 1ull));
-    all += __popcll(same[j]);
+    for (int i = 0; i <= j; i++) same[j][i] = there[i];
   }
-  if (ahead % 16) return 0;
-  row = t;
-  int at = 0;
+  for (int b = 0; b < 32 - __builtin_clz(p.adapters); b++) {
+    uint64_t on[GROUPS];
 #pragma unroll
-  for (int j = 0; j < AD_SELF_ROWS / 64; j++) {  // the rows hand their numbers to the lanes of their places, all others theirs to lanes that nobody reads
-    const int place = at + __popcll(same[j] & ((1ull << lane) - 1ull)) - ahead;
-    const bool take = (same[j] >> lane & 1) && place >= 0 && place < 16;
-    const int got = __builtin_amdgcn_ds_permute(4 * (take ? place : 16 + (lane & 31)), 64 * j + lane + 1);  // (0: nothing came)
+    for (int j = 0; j < GROUPS; j++) {
+      if (j >= groups) break;  // uniform
+      const int bit = __builtin_amdgcn_sbfe(mine[j], b, 1);  // 0 or -1
+      on[j] = __ballot(bit != 0);
+#pragma unroll
+      for (int i = 0; i <= j; i++) same[j][i] &= (uint64_t)(~((uint32_t)(on[i] >> 32) ^ bit)) << 32 | (~((uint32_t)on[i] ^ bit));
+    }
+  }
+  int before = 0, first = -1;
+#pragma unroll
+  for (int j = 0; j < GROUPS; j++) {
+    ahead[j] = __popcll(same[j][j] & ((1ull << lane) - 1ull));
+#pragma unroll
+    for (int i = 0; i < j; i++) ahead[j] += __popcll(same[j][i]);
+    const uint64_t begin = __ballot(64 * j + lane < p.m && ahead[j] % 16 == 0);
+    const uint64_t hit = __ballot((begin >> lane & 1) && before + __popcll(begin & ((1ull << lane) - 1ull)) == t);
+    if (hit) {
+      c = __builtin_amdgcn_readlane(mine[j], __builtin_ctzll(hit));
+      first = __builtin_amdgcn_readlane(ahead[j], __builtin_ctzll(hit));
+    }
+    before += __popcll(begin);
+  }
+  if (first < 0) return 0;
+  int all = 0;
+  row = 0;
+#pragma unroll
+  for (int j = 0; j < GROUPS; j++) {  // the rows hand their numbers to the lanes of their places, all others theirs to lanes that nobody reads
+    const bool of = 64 * j + lane < p.m && mine[j] == c;
+    const int place = ahead[j] - first;
+    const int got = __builtin_amdgcn_ds_permute(4 * (of && place >= 0 && place < 16 ? place : 16 + (lane & 31)), 64 * j + lane + 1);  // (0: nothing came)
     if (lane < 16 && got) row = got - 1;
-    at += __popcll(same[j]);
+    all += __popcll(__ballot(of));
   }
-  row = __shfl(row, lane & 15);
-  return min(16, all - ahead);
+  const int count = min(16, all - first);
+  row = __shfl(row, (lane & 15) < count ? lane & 15 : 0);
+  return count;
+}
+__device__ __forceinline__ int ad_tile_at(const AdIndex& p, int t, int& c, int& row) {
+  if (p.m > 128) return ad_tile_of<AD_SELF_ROWS / 64>(p, t, c, row);
+  if (p.m > 64) return ad_tile_of<2>(p, t, c, row);
+  return ad_tile_of<1>(p, t, c, row);
 }
 
 // ------------------------------------------------------------------------------------------------ FP32 sums as matrix operands
@@ -494,7 +528,8 @@ __device__ __forceinline__ void ad_shrink_units(const char* const (&x)[TM], cons
 }
 
 // Few rows: a workgroup's four wavefronts share one split of the long axis of a tile's rows and sixteen ranks, and join their sums in LDS; the splits' sums
-// are joined by their readers.
+// are joined by their readers (no arrival counters, which a launch would have to clear). Latency bounds it: 64 rows of 5120, 32 adapters of up to 64 ranks (10 MB of matrices), 8.0 us
+// with nothing in the caches, one row of rank 16 5.0.
 struct AdFew {
   AdIndex in;
   const char* x;
@@ -565,7 +600,7 @@ struct AdShrink {
   int chunks;  // of RT x 16 ranks
 };
 constexpr int AD_WAVES = 4;
-constexpr int AD_EXPANDS = 768;   // workgroups of an expansion, about
+constexpr int AD_EXPANDS = 768;   // workgroups of an expansion, about: 4096 rows of 5120 26.6 us (in 256: 36.2, in 2048: 26.5)
 // Results of this many bytes are stored past the caches: half of what the dies' hold. Through them they push out what is still to be read, and whoever reads them next finds
 // little there. Add of 4096 rows of 5120 at rank 32 (42 MB of results) 52 -> 45 us a call, two of 5120 at rank 16 with gradients (21 MB of dx) 43.9 -> 42.5 (y's rows
 // read so too: 48 us).
@@ -745,7 +780,9 @@ __device__ __forceinline__ u32x4_t ad_result(const u32x4_t& y, const f32x4_t (&a
   return v;
 }
 
-// Few rows: a workgroup joins the splits' sums of its tile in LDS, then a tile's rows times four wavefronts' columns, sixteen lanes of sixteen bytes each.
+// Few rows: a workgroup joins the splits' sums of its tile in LDS, then a tile's rows times four wavefronts' columns, sixteen lanes of sixteen bytes each. 64 rows of 25600, 32
+// adapters of up to 64 ranks (55 MB of matrices and rows): 21 us with nothing in the caches, 2.6 TB/s: a wavefront has few steps behind its start, and 250 registers of
+// matrix rows under way leave room for two a SIMD. One row of 5120 at rank 16 5.4 us.
 template <int KIND, int HOW>
 __global__ __launch_bounds__(256) void ad_expand_few_kernel(AdFew p) {
   constexpr int VEC = AD_VEC<KIND>, SIZE = AdType<KIND>::SIZE, PARTS = AdType<KIND>::PARTS;
@@ -891,7 +928,9 @@ __device__ __forceinline__ void ad_join(const AdIndex& in, const AdPlan& plan, c
   }
 }
 
-// A plan's tiles, sixteen rows a workgroup: every wavefront for itself, over every (4 x share)-th block of sixteen lanes' columns.
+// A plan's tiles, sixteen rows a workgroup: every wavefront for itself, over every (4 x share)-th block of sixteen lanes' columns. It is bound by what it stores and y's
+// rows: 4096 rows of 5120 at rank 32 (84 MB) 26.4 us with nothing in the caches, 3.2 TB/s, in three wavefronts a SIMD (two: 38; two tiles of rows a wavefront share the
+// matrix's turning in registers and were slower); dx of 2048 rows of 5120 (21 MB and the join) 9.5.
 struct AdExpand {
   AdIndex in;
   AdPlan plan;
@@ -1010,7 +1049,9 @@ struct AdOuter {
 // A workgroup: RT x 16 ranks times sixteen lanes' columns over a unit of an adapter's rows, the four wavefronts taking its tiles in turn and joining
 // their sums in LDS. A lane's eight rows of sixteen bytes are turned as in the expansion; the next tile's are under way while one is
 // multiplied. An adapter's only unit writes the gradient (zeros, if it has no rows), several write partial sums for ad_join. (Joined by the last of them to
-// arrive instead, whose sums must pass the dies' caches in words: 28 us for the 16 of both kernels at 2048 rows of 5120 x 5120, rank 16.)
+// arrive instead, whose sums must pass the dies' caches in words: 28 us for the 16 of both kernels at 2048 rows of 5120 x 5120, rank 16.) The rows' reads bound it: there 11.1 us
+// for 42 MB that the shrink has just read, 3.8 TB/s; 8192 rows of 12800 and 2560, FP16, ranks up to 64, 67 us for 252 MB, past the last-level cache, 3.8 TB/s.
+// A unit has 512 rows or more: of 128 the parts cost their join more (10.4 us for 9.4 of the launch that has it), of 2048 the products are in too few workgroups (15.3 for 11.1).
 template <int KIND, int RT, int HOW>
 __global__ __launch_bounds__(256, RT == 1 ? 3 : 2) void ad_outer_kernel(AdOuter p) {
   constexpr int VEC = AD_VEC<KIND>, SIZE = AdType<KIND>::SIZE, PARTS = AdType<KIND>::OUTER, WORDS = SIZE == 4 ? 2 : PARTS;
@@ -1164,9 +1205,9 @@ static bool ad_shape(const hb_adapters* a, int64_t m, bool grads, AdShape& s) {
   s.few = !grads && m <= AD_SELF_ROWS;
   const int64_t classes = std::min<int64_t>(a->adapters + 1, m);
   if (s.few) {
-    s.tiles = std::min<int64_t>(m, a->adapters + cut(m, 16));  // at most, of those that begin somewhere
+    s.tiles = std::min<int64_t>(m, a->adapters + cut(m, 16));  // at most: p classes of m rows have (m - p) / 16 + p of them or fewer
     const int64_t groups = s.tiles * cut(a->rank, 16);
-    s.splits = (int)std::max<int64_t>(1, std::min<int64_t>({cut(1024, groups), cut(cut(a->k, 128 / s.size), 16), AD_SPLITS}));
+    s.splits = (int)std::max<int64_t>(1, std::min<int64_t>({cut(1024, groups), cut(cut(a->k, 128 / s.size), 8), AD_SPLITS}));
     s.sums_bytes = up256((size_t)s.splits * m * a->rank * 4);
     return true;
   }
@@ -1264,11 +1305,13 @@ static int ad_add(const hb_adapters* a, const AdShape& s, const AdIndex& in, con
   if (s.few) {
     AdFew p{in, xr, (uint32_t)(x_stride * s.size), static_cast<const char*>(a->a), s.k, s.n, s.splits, (int)cut(cut(s.k, 128 / s.size), s.splits), reinterpret_cast<float*>(ws),
             a->scale, static_cast<const char*>(a->b), yr, (uint32_t)(y_stride * s.size), to, (uint32_t)(out_stride * s.size), ad_thirties(s.rank) * 32};
-    HB_LAUNCH((ad_shrink_few_kernel<KIND>), dim3((unsigned)s.m, (unsigned)s.splits, (unsigned)ad_sixteens(s.rank)), dim3(256), 0, stream, p);
+    HB_LAUNCH((ad_shrink_few_kernel<KIND>), dim3((unsigned)s.tiles, (unsigned)s.splits, (unsigned)ad_sixteens(s.rank)), dim3(256), 0, stream, p);
     if (int code = launch_status()) return code;
     const size_t lds = (size_t)AdType<KIND>::PARTS * 16 * (p.padded * AdType<KIND>::SIZE + 16);
-    const int64_t groups = cut(s.n, 4 * 16 * AD_VEC<KIND>), share = std::max<int64_t>(1, std::min<int64_t>(groups, s.tiles * groups / 256));
-    const dim3 grid((unsigned)s.m, (unsigned)cut(groups, share));
+    // workgroups enough for every compute unit twice: what finds its rows and joins their sums has then several blocks of columns to do it for. 64 rows of 25600, 36 tiles:
+    // 21 us in 17 workgroups a tile, 25 in 8 or 50
+    const int64_t groups = cut(s.n, 4 * 16 * AD_VEC<KIND>), share = std::max<int64_t>(1, std::min<int64_t>(groups, s.tiles * groups / 512));
+    const dim3 grid((unsigned)s.tiles, (unsigned)cut(groups, share));
     if (s.n < AD_VEC<KIND>) HB_LAUNCH((ad_expand_few_kernel<KIND, AD_TINY>), grid, dim3(256), lds, stream, p);
     else HB_LAUNCH((ad_expand_few_kernel<KIND, AD_NEAR>), grid, dim3(256), lds, stream, p);
     return launch_status();
