@@ -4,7 +4,8 @@
 //   g[r] = s_i dy[r] b_i^T;  dx[r] = g[r] a_i;  da_i = sum over i's rows of g[r]^T x[r];  db_i = sum of s_i (x[r] a_i^T)^T dy[r]
 //
 // Both matrices of an adapter lie rank by rank along their long axis, so the six products are of three kinds:
-//   shrink   rows [m, long] times a matrix's rows: contraction over the long axis, [m, rank] FP32 sums, the long axis cut into `splits`
+//   shrink   rows [m, long] times a matrix's rows: contraction over the long axis, [m, rank] FP32 sums, the long axis cut into splits
+//            that other workgroups have
 //   expand   [m, rank] times the matrix: contraction over the rank, added to y's rows (or alone: dx)
 //   outer    [m, rank]^T times rows [m, long]: contraction over an adapter's rows, FP32
 // Rows are grouped by adapter: a tile's rows are one adapter's, gathered by number. All of it is bound by memory (few operations a byte at
@@ -781,8 +782,8 @@ __device__ __forceinline__ u32x4_t ad_result(const u32x4_t& y, const f32x4_t (&a
 }
 
 // Few rows: a workgroup joins the splits' sums of its tile in LDS, then a tile's rows times four wavefronts' columns, sixteen lanes of sixteen bytes each. 64 rows of 25600, 32
-// adapters of up to 64 ranks (55 MB of matrices and rows): 21 us with nothing in the caches, 2.6 TB/s: a wavefront has few steps behind its start, and 250 registers of
-// matrix rows under way leave room for two a SIMD. One row of 5120 at rank 16 5.4 us.
+// adapters of up to 64 ranks (55 MB of matrices and rows): 21 us with nothing in the caches, 2.6 TB/s: a wavefront has few steps behind its start, and its 228 registers,
+// most of them matrix rows under way, leave room for two a SIMD. One row of 5120 at rank 16 5.4 us.
 template <int KIND, int HOW>
 __global__ __launch_bounds__(256) void ad_expand_few_kernel(AdFew p) {
   constexpr int VEC = AD_VEC<KIND>, SIZE = AdType<KIND>::SIZE, PARTS = AdType<KIND>::PARTS;
@@ -929,8 +930,8 @@ __device__ __forceinline__ void ad_join(const AdIndex& in, const AdPlan& plan, c
 }
 
 // A plan's tiles, sixteen rows a workgroup: every wavefront for itself, over every (4 x share)-th block of sixteen lanes' columns. It is bound by what it stores and y's
-// rows: 4096 rows of 5120 at rank 32 (84 MB) 26.4 us with nothing in the caches, 3.2 TB/s, in three wavefronts a SIMD (two: 38; two tiles of rows a wavefront share the
-// matrix's turning in registers and were slower); dx of 2048 rows of 5120 (21 MB and the join) 9.5.
+// rows: 4096 rows of 5120 at rank 32 (84 MB) 26.4 us with nothing in the caches, 3.2 TB/s, in three wavefronts a SIMD (with two tiles of
+// rows a wavefront the matrix is turned in registers half as often, and there is room for two: slower); dx of 2048 rows of 5120 (21 MB and the join) 9.5.
 struct AdExpand {
   AdIndex in;
   AdPlan plan;

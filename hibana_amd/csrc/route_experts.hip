@@ -162,6 +162,10 @@ __device__ __forceinline__ int route_in_64_bits(const RouteExperts& p, const flo
 }
 
 // Lane l holds the experts l % lanes * per .. + per - 1 of group l / lanes: whole groups in neighbouring lanes, and experts in ascending order of lane, then register.
+//
+// Up to some thousand rows the launch's latency (one row of 512 BF16 logits, top 10: 5.1 us with nothing in the caches, 777 rows of 60 FP16 ones 5.5), then the instructions: 8192
+// rows of 256 FP32 logits (8.4 MB, 1.7 us of reads), sigmoid, a bias, 4 of 8 groups, top 8: 17 us, 609 vector and 390 scalar instructions a row, of which the groups,
+// the threshold and the ranks of the chosen (ballots and counts of them) are most. The library's exponential and division, and groups merged through LDS, were more of them.
 template <int KIND, bool SIGMOID, int PER>
 __global__ __launch_bounds__(256) void route_experts_kernel(RouteExperts p) {
   const int lane = threadIdx.x & 63, r = blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -281,6 +285,10 @@ struct RouteGrad {
   void* out;              // [m, e]
 };
 
+// A wavefront a row: the chosen experts' values in its lanes, then the row's columns in 16-byte pieces, each piece the sum over the chosen of those that are its own. 8192 rows of 256
+// FP32 with a sigmoid, which writes 8.4 MB and reads the chosen logits alone, 7.9 us with nothing in the caches; a softmax without `renorm`, which goes
+// over the row three times, 2049 rows of 512 BF16 10.8: latency of the passes one behind the other.
+//
 // With `renorm` dl = w (dw - sum of dw w) at the chosen experts (the sigmoid's: times 1 - s), zero elsewhere. Without: the sigmoid's dw s (1 - s) there; the softmax's
 // s (dw - sum of dw s) at every expert, dw zero at those that were not chosen.
 template <int KIND, bool SIGMOID>
