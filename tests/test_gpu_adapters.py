@@ -374,3 +374,29 @@ def test_a_pool_cut_and_put_elsewhere():
     pool.a, pool.b = a, b
     pool.a.data, pool.b.data = a.data[:, :4].contiguous(), b.data[:, :4].contiguous()
     assert torch.equal(adapters.add(y, x, pool, index), adapters.add(y, x, adapters.Adapters(a.clone(), b.clone()), index))
+
+
+def test_rows_past_four_gibibytes():
+    """Rows whose bytes begin past 2^32 from the first's. Whole numbers: every sum is exact, dx is its exact value rounded once."""
+    from hibana_amd.kernels import adapters
+    m, k, n, rank, count = 900_000, 24, 2504, 2, 3
+    g = torch.Generator(device="cuda").manual_seed(50)
+    whole = lambda *s: torch.randint(-1, 2, s, device="cuda", dtype=torch.int8, generator=g).bfloat16()  # noqa: E731
+    y, x, a, b = whole(m, n), whole(m, k), whole(count, rank, k), whole(count, rank, n)
+    index = torch.randint(-1, count, (m,), device="cuda", generator=g)
+    pool = adapters.Adapters(a, b)
+    out = adapters.add(y, x, pool, index)
+    dx, da, db = adapters.grads(y, x, pool, index)
+    want_a, want_b = torch.zeros(a.shape, device="cuda", dtype=torch.float64), torch.zeros(b.shape, device="cuda", dtype=torch.float64)
+    for at in range(0, m, 50_000):
+        rows = slice(at, min(at + 50_000, m))
+        ys, xs, to, back = y[rows].float(), x[rows].float(), y[rows].float(), torch.zeros(x[rows].shape, device="cuda")
+        for i in range(count):
+            of = (index[rows] == i).float()[:, None]
+            inner, outer = (xs @ a[i].float().t().contiguous()) * of, (ys @ b[i].float().t().contiguous()) * of
+            to += inner @ b[i].float()
+            back += outer @ a[i].float()
+            want_a[i] += (outer.t().contiguous() @ xs).double()
+            want_b[i] += (inner.t().contiguous() @ ys).double()
+        assert torch.equal(out[rows], to.bfloat16()) and torch.equal(dx[rows], back.bfloat16()), at
+    assert torch.equal(da.double(), want_a) and torch.equal(db.double(), want_b)
