@@ -34,9 +34,9 @@ constexpr int AD_LONGEST = 1 << 22;  // of either axis
 constexpr int64_t AD_STRIDE = 0xffffffffll;  // bytes from row to row
 
 template <int KIND> struct AdType;
-template <> struct AdType<HB_BF16> { static constexpr int SIZE = 2, PARTS = 2, OUTER = 3; };  // parts that FP32 values are cut into
-template <> struct AdType<HB_F16> { static constexpr int SIZE = 2, PARTS = 2, OUTER = 2; };
-template <> struct AdType<HB_F32> { static constexpr int SIZE = 4, PARTS = 1, OUTER = 1; };
+template <> struct AdType<HB_BF16> { static constexpr int SIZE = 2, PARTS = 3; };  // parts that FP32 values are cut into
+template <> struct AdType<HB_F16> { static constexpr int SIZE = 2, PARTS = 3; };
+template <> struct AdType<HB_F32> { static constexpr int SIZE = 4, PARTS = 1; };
 template <int KIND> constexpr int AD_VEC = 16 / AdType<KIND>::SIZE;  // elements of a 16-byte load: the columns a lane holds
 
 template <int KIND>
@@ -419,14 +419,15 @@ __device__ __forceinline__ int ad_tile_at(const AdIndex& p, int t, int& c, int& 
 
 // ------------------------------------------------------------------------------------------------ FP32 sums as matrix operands
 
-// The sums are operands of the second product. To keep what FP32 holds of them, a value goes in as the sum of two or three of the type's:
-// BF16 by cutting (8 bits a part, never past the value's size: no overflow; two parts 2^-16 of it, three all of it), FP16 by rounding what a power of two
-// has brought below 2^15 (two parts: 2^-22, or 2^-40 of the largest).
-template <int KIND, int PARTS>
-__device__ __forceinline__ void ad_cut(float v, uint16_t (&part)[PARTS]) {
+// The sums are operands of the second product. To keep what FP32 holds of them, a value goes in as the sum of three of the type's: BF16 by cutting (8 bits a
+// part, never past the value's size: no overflow; three parts are all of it), FP16 by rounding what a power of two has brought below 2^15 (all of it down to 2^-39 of the
+// largest, FP16's smallest step). Two parts hold 2^-16 of a BF16 sum, 2^-22 of an FP16 one.
+template <int KIND>
+__device__ __forceinline__ void ad_cut(float v, uint16_t (&part)[AdType<KIND>::PARTS]) {
+  constexpr int PARTS = AdType<KIND>::PARTS;
   const bool finite = fabsf(v) < INFINITY;
+  float rest = v;
   if constexpr (KIND == HB_BF16) {
-    float rest = v;
 #pragma unroll
     for (int i = 0; i < PARTS; i++) {
       if (i == PARTS - 1) {
@@ -438,9 +439,12 @@ __device__ __forceinline__ void ad_cut(float v, uint16_t (&part)[PARTS]) {
       }
     }
   } else {
-    const _Float16 high = (_Float16)v;
-    part[0] = __builtin_bit_cast(uint16_t, high);
-    part[1] = finite ? __builtin_bit_cast(uint16_t, (_Float16)(v - (float)high)) : 0;
+#pragma unroll
+    for (int i = 0; i < PARTS; i++) {
+      const _Float16 top = (_Float16)rest;
+      part[i] = finite || i == 0 ? __builtin_bit_cast(uint16_t, top) : 0;
+      rest -= (float)top;
+    }
   }
 }
 
@@ -614,7 +618,7 @@ __host__ __device__ constexpr int ad_thirties(int rank) { return (rank + 31) / 3
 
 template <int KIND, int RT>
 __global__ __launch_bounds__(64 * AD_WAVES) void ad_shrink_kernel(AdShrink p) {
-  constexpr int SIZE = AdType<KIND>::SIZE, UNIT = 128 / SIZE, PARTS = AdType<KIND>::PARTS, OUTER = AdType<KIND>::OUTER, WIDE = 16 * RT, PITCH = WIDE + 1;
+  constexpr int SIZE = AdType<KIND>::SIZE, UNIT = 128 / SIZE, PARTS = AdType<KIND>::PARTS, WIDE = 16 * RT, PITCH = WIDE + 1;
   constexpr int JOINED = AD_WAVES / 2 * 2 * RT * 64 * 16, SUMS = 32 * PITCH * 4;
   __shared__ __align__(16) char shared[JOINED > SUMS ? JOINED : SUMS];
   __shared__ int32_t row_power[AD_TILE * RT], rank_power[RT], last;
@@ -718,7 +722,7 @@ __global__ __launch_bounds__(64 * AD_WAVES) void ad_shrink_kernel(AdShrink p) {
       } else {
         uint16_t part[PARTS];
         const float unit = KIND == HB_F16 && 32 * step + r < WIDE ? ad_pow2(-row_power[(32 * step + r) / 16 * AD_TILE + place]) : 1.0f;
-        ad_cut<KIND, PARTS>(v * unit, part);
+        ad_cut<KIND>(v * unit, part);
 #pragma unroll
         for (int q = 0; q < PARTS; q++) reinterpret_cast<uint16_t*>(job.by_row)[at + q * 1024] = part[q];
       }
@@ -729,14 +733,14 @@ __global__ __launch_bounds__(64 * AD_WAVES) void ad_shrink_kernel(AdShrink p) {
       const int place = i % AD_TILE, r = i / AD_TILE % 16, j = i / (AD_TILE * 16);
       if (r0 / 16 + j >= sixteens) break;
       const float v = sums[place * PITCH + 16 * j + r];
-      const int64_t at = ((int64_t)tile * sixteens + r0 / 16 + j) * OUTER * 512 + r * 32 + place;
+      const int64_t at = ((int64_t)tile * sixteens + r0 / 16 + j) * PARTS * 512 + r * 32 + place;
       if constexpr (SIZE == 4) {
         reinterpret_cast<float*>(job.by_rank)[at] = v;
       } else {
-        uint16_t part[OUTER];
-        ad_cut<KIND, OUTER>(KIND == HB_F16 ? v * ad_pow2(-rank_power[j]) : v, part);
+        uint16_t part[PARTS];
+        ad_cut<KIND>(KIND == HB_F16 ? v * ad_pow2(-rank_power[j]) : v, part);
 #pragma unroll
-        for (int q = 0; q < OUTER; q++) reinterpret_cast<uint16_t*>(job.by_rank)[at + q * 512] = part[q];
+        for (int q = 0; q < PARTS; q++) reinterpret_cast<uint16_t*>(job.by_rank)[at + q * 512] = part[q];
       }
     }
   }
@@ -782,7 +786,7 @@ __device__ __forceinline__ u32x4_t ad_result(const u32x4_t& y, const f32x4_t (&a
 }
 
 // Few rows: a workgroup joins the splits' sums of its tile in LDS, then a tile's rows times four wavefronts' columns, sixteen lanes of sixteen bytes each. 64 rows of 25600, 32
-// adapters of up to 64 ranks (55 MB of matrices and rows): 21 us with nothing in the caches, 2.6 TB/s: a wavefront has few steps behind its start, and its 228 registers,
+// adapters of up to 64 ranks (55 MB of matrices and rows): 21 us with nothing in the caches, 2.6 TB/s: a wavefront has few steps behind its start, and its 230 registers,
 // most of them matrix rows under way, leave room for two a SIMD. One row of 5120 at rank 16 5.4 us.
 template <int KIND, int HOW>
 __global__ __launch_bounds__(256) void ad_expand_few_kernel(AdFew p) {
@@ -860,7 +864,7 @@ __global__ __launch_bounds__(256) void ad_expand_few_kernel(AdFew p) {
         reinterpret_cast<float*>(staged)[place * pitch + r] = to;
       } else {
         uint16_t part[PARTS];
-        ad_cut<KIND, PARTS>(to, part);
+        ad_cut<KIND>(to, part);
 #pragma unroll
         for (int i = 0; i < PARTS; i++) reinterpret_cast<uint16_t*>(staged)[(i * 16 + place) * pitch + r] = part[i];
       }
@@ -1055,7 +1059,7 @@ struct AdOuter {
 // A unit has 512 rows or more: of 128 the parts cost their join more (10.4 us for 9.4 of the launch that has it), of 2048 the products are in too few workgroups (15.3 for 11.1).
 template <int KIND, int RT, int HOW>
 __global__ __launch_bounds__(256, RT == 1 ? 3 : 2) void ad_outer_kernel(AdOuter p) {
-  constexpr int VEC = AD_VEC<KIND>, SIZE = AdType<KIND>::SIZE, PARTS = AdType<KIND>::OUTER, WORDS = SIZE == 4 ? 2 : PARTS;
+  constexpr int VEC = AD_VEC<KIND>, SIZE = AdType<KIND>::SIZE, PARTS = AdType<KIND>::PARTS, WORDS = SIZE == 4 ? 2 : PARTS;
   __shared__ f32x4_t join[4 * VEC * 64];  // [wavefront][column of a lane][lane]
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, group = lane >> 4, col = lane & 15;
   const AdOuterJob& job = p.job[blockIdx.z / p.chunks];
@@ -1221,9 +1225,9 @@ static bool ad_shape(const hb_adapters* a, int64_t m, bool grads, AdShape& s) {
   s.splits_x = (int)cut(units_x, s.share), s.splits_dy = (int)cut(units_dy, s.share);
   s.tickets = s.tiles * s.chunks * (grads ? 2 : 1);
   s.split_bytes = up256((size_t)s.tiles * s.chunks * ((s.splits_x > 1 ? s.splits_x : 0) + (s.splits_dy > 1 ? s.splits_dy : 0)) * AD_TILE * 16 * s.rt * 4);
-  const int parts = a->type == HB_F32 ? 1 : 2, outer = a->type == HB_BF16 ? 3 : parts;
+  const int parts = a->type == HB_F32 ? AdType<HB_F32>::PARTS : AdType<HB_BF16>::PARTS;
   s.row_bytes = up256((size_t)s.tiles * ad_thirties(a->rank) * parts * 1024 * s.size);
-  s.rank_bytes = up256((size_t)s.tiles * ad_sixteens(a->rank) * outer * 512 * s.size);
+  s.rank_bytes = up256((size_t)s.tiles * ad_sixteens(a->rank) * parts * 512 * s.size);
   s.row_power_bytes = a->type == HB_F16 ? up256((size_t)s.tiles * ad_sixteens(a->rank) * AD_TILE) : 0;
   s.rank_power_bytes = a->type == HB_F16 ? up256((size_t)s.tiles * ad_sixteens(a->rank)) : 0;
   s.unit = 4 * AD_TILE;

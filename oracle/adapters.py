@@ -41,9 +41,9 @@ def _two(length, terms, parts):
     return (length + 40) * 2.0 ** -23 + parts + (terms + 8) * 2.0 ** -23
 
 
-# FP32 inner sums as operands: BF16 in two parts, the first cut (what is left is below 2^-7 of the value), the second rounded (2^-9 of that); in three, exact
-# to 2^-24; FP16 in two rounded parts, 2^-11 each, of values brought below 2^15, whose own smallest step is 2^-24: 2^-25 / 2^14 of the largest
-TWO_PARTS = {torch.bfloat16: 2.0 ** -16, torch.float16: 2.0 ** -22, torch.float32: 0.0}
+# FP32 inner sums as operands, in three parts of the type: BF16 cut to 8 bits each, all of the 24; FP16 rounded to 11 bits each (2^-33), of values brought
+# below 2^15, whose own smallest step is 2^-24: 2^-25 / 2^14 of the largest
+PARTS = {torch.bfloat16: 2.0 ** -24, torch.float16: 2.0 ** -33, torch.float32: 0.0}
 LARGEST = {torch.bfloat16: 0.0, torch.float16: 2.0 ** -39, torch.float32: 0.0}
 
 
@@ -53,7 +53,7 @@ def add_bound(y, x, a, b, scale, ranks, index):
     bound = torch.zeros(y.shape, dtype=torch.float64, device=x.device)
     for rows, _, ai, bi, s in _each(a, b, scale, ranks, index):
         inner = x[rows].double().abs() @ ai.abs().T
-        rel = _two(x.shape[1], 2 * len(ai), TWO_PARTS[dtype])
+        rel = _two(x.shape[1], 3 * len(ai), PARTS[dtype])
         bound[rows] = abs(s) * (rel * (inner @ bi.abs()) + LARGEST[dtype] * inner.amax(1, keepdim=True) * bi.abs().sum(0))
     out = add(y, x, a, b, scale, ranks, index)
     return bound + (torch.finfo(dtype).eps / 2 + 2.0 ** -23) * (out.abs() + bound) + SMALLEST[dtype]
@@ -66,11 +66,10 @@ def grads_bound(dy, x, a, b, scale, ranks, index):
     for rows, i, ai, bi, s in _each(a, b, scale, ranks, index):
         xr, dyr, m = x[rows].double().abs(), dy[rows].double().abs(), len(rows)
         g, h = abs(s) * dyr @ bi.abs().T, abs(s) * xr @ ai.abs().T
-        dx[rows] = _two(dy.shape[1], 2 * len(ai), TWO_PARTS[dtype]) * (g @ ai.abs()) + LARGEST[dtype] * g.amax(1, keepdim=True) * ai.abs().sum(0)
+        dx[rows] = _two(dy.shape[1], 3 * len(ai), PARTS[dtype]) * (g @ ai.abs()) + LARGEST[dtype] * g.amax(1, keepdim=True) * ai.abs().sum(0)
         # (sums over rows: an adapter's largest value is the unit of all of its rows in FP16)
-        outer = 2.0 ** -24 if dtype == torch.bfloat16 else TWO_PARTS[dtype]
-        da[i, :len(ai)] = _two(dy.shape[1], 3 * m, outer) * (g.T @ xr) + LARGEST[dtype] * g.max() * xr.sum(0)
-        db[i, :len(bi)] = _two(x.shape[1], 3 * m, outer) * (h.T @ dyr) + LARGEST[dtype] * h.max() * dyr.sum(0)
+        da[i, :len(ai)] = _two(dy.shape[1], 3 * m, PARTS[dtype]) * (g.T @ xr) + LARGEST[dtype] * g.max() * xr.sum(0)
+        db[i, :len(bi)] = _two(x.shape[1], 3 * m, PARTS[dtype]) * (h.T @ dyr) + LARGEST[dtype] * h.max() * dyr.sum(0)
     want = grads(dy, x, a, b, scale, ranks, index)
     return (dx + (torch.finfo(dtype).eps / 2 + 2.0 ** -23) * (want[0].abs() + dx) + SMALLEST[dtype],
             da + 2.0 ** -22 * want[1].abs() + 2.0 ** -149, db + 2.0 ** -22 * want[2].abs() + 2.0 ** -149)
