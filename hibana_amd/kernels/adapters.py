@@ -110,9 +110,12 @@ class Adapters:
             setattr(self, name, v)
 
     def struct(self):
-        """What the library takes, made again where a tensor is another one, or its place or shape has changed (an optimizer may have put other memory in)."""
+        """What the library takes, looked at and made again where a tensor is another one, or its place, type or shape has changed (an optimizer may have put other memory
+        in, at the old address too)."""
         a, b, scale, ranks = self.a, self.b, self.scale, self.ranks
-        at = (a.data_ptr(), b.data_ptr(), _lib.ptr(scale), _lib.ptr(ranks), a.shape, b.shape, a.stride(), b.stride())
+        at = (a.data_ptr(), b.data_ptr(), None if scale is None else scale.data_ptr(), None if ranks is None else ranks.data_ptr(), a.shape, b.shape,
+              a.dtype, b.dtype, a.is_contiguous(), b.is_contiguous(), scale is None or (scale.dtype, scale.numel(), scale.is_contiguous()),
+              ranks is None or (ranks.dtype, ranks.numel(), ranks.is_contiguous()))
         if at != self._at:
             self._check()
             self._rooms.clear()
