@@ -187,20 +187,19 @@ def _add(y: torch.Tensor, x: torch.Tensor, pool: Adapters, index: torch.Tensor, 
 
 class _Add(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, y, x, a, b, pool, index):
-        ctx.save_for_backward(x, a, b, index)
-        ctx.pool = pool
+    def forward(ctx, y, x, a, b, scale, ranks, index, pool):
+        ctx.save_for_backward(x, a, b, scale, ranks, index)  # (the pool may hold others when the gradient is asked for)
         return _add(y, x, pool, index, None)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, a, b, index = ctx.saved_tensors
-        _, need_x, need_a, need_b, _, _ = ctx.needs_input_grad
+        x, a, b, scale, ranks, index = ctx.saved_tensors
+        _, need_x, need_a, need_b = ctx.needs_input_grad[:4]
         if not (need_x or need_a or need_b):
-            return dy, None, None, None, None, None
-        dx, da, db = grads(dy, x, Adapters(a.detach(), b.detach(), ctx.pool.scale, ctx.pool.ranks), index)
-        return dy, dx if need_x else None, da.to(a.dtype) if need_a else None, db.to(b.dtype) if need_b else None, None, None
+            return dy, *[None] * 7
+        dx, da, db = grads(dy, x, Adapters(a.detach(), b.detach(), scale, ranks), index)
+        return dy, dx if need_x else None, da.to(a.dtype) if need_a else None, db.to(b.dtype) if need_b else None, *[None] * 4
 
 
 def add(y: torch.Tensor, x: torch.Tensor, pool: Adapters, index: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
@@ -215,7 +214,7 @@ def add(y: torch.Tensor, x: torch.Tensor, pool: Adapters, index: torch.Tensor, o
             raise ValueError("adapters.add: no `out` where a gradient is recorded")
         if y.is_cuda and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("adapters.add: a captured step takes adapters.grads (no gradient is recorded in a capture)")
-        return _Add.apply(y, x, pool.a, pool.b, pool, index)
+        return _Add.apply(y, x, pool.a, pool.b, pool.scale, pool.ranks, index, pool)
     return _add(y, x, pool, index, out)
 
 
