@@ -209,9 +209,12 @@ def add(y: torch.Tensor, x: torch.Tensor, pool: Adapters, index: torch.Tensor, o
 
     Differentiable in y, x, pool.a and pool.b. A training step that is to be captured calls `grads` itself: autograd's own streams and a
     capture do not go together, and the process would end; so a call that records a gradient is refused there."""
-    if torch.is_grad_enabled() and (y.requires_grad or x.requires_grad or pool.a.requires_grad or pool.b.requires_grad or (out is not None and out.requires_grad)):
+    if torch.is_grad_enabled() and (y.requires_grad or x.requires_grad or pool.a.requires_grad or pool.b.requires_grad or (out is not None and out.requires_grad)
+                                    or (pool.scale is not None and pool.scale.requires_grad)):
         if out is not None:
             raise ValueError("adapters.add: no `out` where a gradient is recorded")
+        if pool.scale is not None and pool.scale.requires_grad:
+            raise ValueError("adapters.add: a pool's scale takes no gradient")
         if y.is_cuda and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("adapters.add: a captured step takes adapters.grads (no gradient is recorded in a capture)")
         return _Add.apply(y, x, pool.a, pool.b, pool.scale, pool.ranks, index, pool)

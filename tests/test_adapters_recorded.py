@@ -77,3 +77,10 @@ def test_several_passes_at_scales_of_their_own():
     once = _gradients(pool, y, x)
     torch.testing.assert_close(got[2], 4 * once[2])
     torch.testing.assert_close(got[3], 4 * once[3])
+
+
+def test_a_scale_that_begins_to_take_a_gradient_is_refused():
+    pool, y, x, _, index = _case()
+    pool.scale.requires_grad_()
+    with pytest.raises(ValueError, match="scale"):
+        adapters.add(y, x, pool, index)
