@@ -6,6 +6,7 @@ from functools import lru_cache
 from pathlib import Path
 
 import torch
+from torch.autograd import forward_ad
 
 LIBRARY = Path(__file__).resolve().parent / "libhibana_hip.so"
 
@@ -213,6 +214,13 @@ def stream_of(x: torch.Tensor, *more: torch.Tensor) -> int:
         if t.get_device() != at:
             need_one_gpu(x, *more)
     return torch._C._cuda_getCurrentRawStream(at)
+
+
+def no_tangents(what: str, *tensors: torch.Tensor | None) -> None:
+    """Refuses forward-mode tangents: a call whose kernels have no product with them would lose them without a word. (Asked for where a level of
+    `torch.autograd.forward_ad` is open; outside of one no tensor has any.)"""
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{what}: no forward-mode gradient (an input carries a tangent)")
 
 
 def need_gpu(*tensors: torch.Tensor) -> None:

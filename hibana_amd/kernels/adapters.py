@@ -13,6 +13,7 @@ from __future__ import annotations
 import ctypes as C
 
 import torch
+from torch.autograd import forward_ad
 
 from hibana_amd import _lib
 from hibana_amd.kernels.mxfp4 import TYPES
@@ -207,8 +208,10 @@ def add(y: torch.Tensor, x: torch.Tensor, pool: Adapters, index: torch.Tensor, o
     index is not of the pool (-1) is y's, bit for bit. Any order of rows: those of an adapter share one read of its matrices. An infinity in b (of the gradients: in a, x or
     dy) may come out as NaN: it is multiplied with values that are held in parts, some of them zero.
 
-    Differentiable in y, x, pool.a and pool.b. A training step that is to be captured calls `grads` itself: autograd's own streams and a
+    Differentiable in y, x, pool.a and pool.b, in reverse (an input with a forward-mode tangent is refused). A training step that is to be captured calls `grads` itself: autograd's own streams and a
     capture do not go together, and the process would end; so a call that records a gradient is refused there."""
+    if forward_ad._current_level >= 0:
+        _lib.no_tangents("adapters.add", y, x, pool.a, pool.b, pool.scale)
     if torch.is_grad_enabled() and (y.requires_grad or x.requires_grad or pool.a.requires_grad or pool.b.requires_grad or (out is not None and out.requires_grad)
                                     or (pool.scale is not None and pool.scale.requires_grad)):
         if out is not None:
@@ -225,6 +228,8 @@ def grads(dy: torch.Tensor, x: torch.Tensor, pool: Adapters, index: torch.Tensor
     """The gradients of `add` given that of its result, dy [M, N]: (dx [M, K] of the pool's type, da FP32 [adapters, rank, K], db FP32 [adapters, rank,
     N]). An adapter that no row has gets zeros, as do the rows behind an adapter's rank; y's gradient is dy itself. Sums over rows are in a
     fixed order: the same call gives the same bits."""
+    if forward_ad._current_level >= 0:
+        _lib.no_tangents("adapters.grads", dy, x, pool.a, pool.b, pool.scale)
     dyr, xr, ix, m, stream = _operands(dy, x, pool, index, "adapters.grads")
     k, n = pool.a.shape[2], pool.b.shape[2]
     dx = xr.new_empty((m, k))

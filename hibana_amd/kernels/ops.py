@@ -5,6 +5,7 @@ from __future__ import annotations
 from dataclasses import dataclass
 
 import torch
+from torch.autograd import forward_ad
 
 from hibana_amd import _lib
 from hibana_amd.kernels import adapters, mxfp4, w3
@@ -246,8 +247,10 @@ def route_experts(logits: torch.Tensor, k: int, scoring: str = "softmax", *, bia
     `renormalize` divided by their sum, times `scale`. An expert whose logit is -inf (a mask) or NaN is never chosen: slots left over, and all of a padded row's
     (slots[r // steps] == 0), have id E, which the experts' kernels skip, and weight 0. A row that has a NaN logit has NaN weights.
 
-    Differentiable in the logits, through the weights (the bias only moves the choice). A captured training step calls `route_experts_grad`
+    Differentiable in the logits, in reverse (a forward-mode tangent is refused), through the weights (the bias only moves the choice). A captured training step calls `route_experts_grad`
     itself: a call that records a gradient is refused in a capture, as in `adapters.add`. No counterpart in the reference."""
+    if forward_ad._current_level >= 0:
+        _lib.no_tangents("route_experts", logits)
     if logits.requires_grad and torch.is_grad_enabled():
         if logits.is_cuda and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("route_experts: a captured step takes route_experts_grad (no gradient is recorded in a capture)")
@@ -260,6 +263,8 @@ def route_experts_grad(dweights: torch.Tensor, logits: torch.Tensor, ids: torch.
     """The gradient of `route_experts`' logits [M, E], of their type, given that of its weights (FP32 [M, k]) and the ids it chose (int32 [M, k]; one
     outside 0 .. E - 1 adds nothing)."""
     what = "route_experts_grad"
+    if forward_ad._current_level >= 0:
+        _lib.no_tangents(what, dweights, logits)
     lg = _route_logits(logits, scoring, what)
     m, e = lg.shape
     if ids.dtype != torch.int32 or ids.ndim != 2 or ids.shape[0] != m or dweights.dtype != torch.float32 or dweights.shape != ids.shape:
