@@ -209,7 +209,9 @@ def add(y: torch.Tensor, x: torch.Tensor, pool: Adapters, index: torch.Tensor, o
     dy) may come out as NaN: it is multiplied with values that are held in parts, some of them zero.
 
     Differentiable in y, x, pool.a and pool.b, in reverse (an input with a forward-mode tangent is refused). A training step that is to be captured calls `grads` itself: autograd's own streams and a
-    capture do not go together, and the process would end; so a call that records a gradient is refused there."""
+    capture do not go together, and the process would end; so a call that records a gradient is refused there. The framework's frozen linears
+    record none of their rows: where x takes a gradient (adapters below this one), y has to as well, from a projection that gives dy W (a function
+    of the program's own over `lin.dequantize()`; or y.requires_grad_(), whose gradient the program takes on itself); a y without one is refused."""
     if forward_ad._current_level >= 0:
         _lib.no_tangents("adapters.add", y, x, pool.a, pool.b, pool.scale)
     if torch.is_grad_enabled() and (y.requires_grad or x.requires_grad or pool.a.requires_grad or pool.b.requires_grad or (out is not None and out.requires_grad)
@@ -218,6 +220,8 @@ def add(y: torch.Tensor, x: torch.Tensor, pool: Adapters, index: torch.Tensor, o
             raise ValueError("adapters.add: no `out` where a gradient is recorded")
         if pool.scale is not None and pool.scale.requires_grad:
             raise ValueError("adapters.add: a pool's scale takes no gradient")
+        if x.requires_grad and not y.requires_grad:
+            raise ValueError("adapters.add: x takes a gradient and y none, so that the projection's own part of it, dy W, would be missing")
         if y.is_cuda and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("adapters.add: a captured step takes adapters.grads (no gradient is recorded in a capture)")
         return _Add.apply(y, x, pool.a, pool.b, pool.scale, pool.ranks, index, pool)

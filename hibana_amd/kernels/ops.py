@@ -248,7 +248,8 @@ def route_experts(logits: torch.Tensor, k: int, scoring: str = "softmax", *, bia
     (slots[r // steps] == 0), have id E, which the experts' kernels skip, and weight 0. A row that has a NaN logit has NaN weights.
 
     Differentiable in the logits, in reverse (a forward-mode tangent is refused), through the weights (the bias only moves the choice). A captured training step calls `route_experts_grad`
-    itself: a call that records a gradient is refused in a capture, as in `adapters.add`. No counterpart in the reference."""
+    itself: a call that records a gradient is refused in a capture, as in `adapters.add`. The experts' calls read the weights' values alone and record
+    nothing: a router that learns sums their pairs (`pairs=True`) with the weights itself. No counterpart in the reference."""
     if forward_ad._current_level >= 0:
         _lib.no_tangents("route_experts", logits)
     if logits.requires_grad and torch.is_grad_enabled():

@@ -19,7 +19,8 @@ experts' row order (`shared_from_linears`). Budgeted expert selection (HIBANA_MO
 HIBANA_MOE_BUDGET_PER_REQUEST of the reference's configuration) is the constructor's `keep` / `budget` / `per_request`:
 decode and verify forwards then read at most a budget of distinct experts (`ops.route_budget`); slots left over name no
 expert, which the 3-bit kernels skip. A layer with another routing rule (`ops.Routing`: sigmoid scores, a bias for balance, groups,
-plain or scaled weights) holds it as `routing`: the logits are then routed by `ops.route_experts`, and the experts take its ids and weights.
+plain or scaled weights) holds it as `routing`: the logits are then routed by `ops.route_experts`, and the experts take its ids and weights (values alone: the layer is a serving
+form and records no gradient).
 """
 from __future__ import annotations
 

@@ -11,7 +11,8 @@ product: mxfp4_linear(silu_mul_quant_mxfp4(mxfp4_linear(x, gate_up), pairs), dow
 
 With `adapters`, a pool beside each linear (or None), and a call's `index`, each row's own adapter is added to both products
 (`adapters.add`): the forms above that make the two products in one call, or round the product in between in the same launch, are
-not taken then but for the microscaled format's, whose down adapters read the rows that its linear reads, rounded to four bits.
+not taken then but for the microscaled format's, whose down adapters read the rows that its linear reads, rounded to four bits. A serving
+form: no gradient is recorded, of the rows or of pools that take one.
 
 Assembled from linears already loaded. The reference's NVFP4 activation paths (`prequantized`, the fused prefill
 gate/up GEMM that rounds SiLU(gate) * up to NVFP4 in its epilogue) have no counterpart: the NVFP4 kernels here are

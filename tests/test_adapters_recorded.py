@@ -84,3 +84,45 @@ def test_a_scale_that_begins_to_take_a_gradient_is_refused():
     pool.scale.requires_grad_()
     with pytest.raises(ValueError, match="scale"):
         adapters.add(y, x, pool, index)
+
+
+def test_a_projection_without_a_gradient_beside_rows_with_one_is_refused():
+    """y of a frozen linear's kernels records nothing: x's gradient would lack the projection's own part, dy W, and a layer below would learn from the rest."""
+    pool, y, x, dy, index = _case()
+    with pytest.raises(ValueError, match="dy W"):
+        adapters.add(y.detach(), x, pool, index)
+    adapters.add(y.detach(), x.detach(), pool, index).backward(dy)  # the lowest adapted layer
+    da = pool.a.grad.clone()
+    with torch.no_grad():
+        assert not adapters.add(y.detach(), x, pool, index).requires_grad
+    adapters.add(y.detach().requires_grad_(), x, pool, index).backward(dy)  # the caller's own dy W beside it
+    assert x.grad is not None and torch.equal(pool.a.grad, 2 * da)
+
+
+def test_two_adapted_layers_learn_through_a_projection_that_records_its_gradient():
+    """The layers' frozen projections as a function of the program's own (dx = dy W), against differences of the loss in the lower layer's adapters."""
+    class Frozen(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x, w):
+            ctx.save_for_backward(w)
+            return x @ w.T
+
+        @staticmethod
+        def backward(ctx, dy):
+            return dy @ ctx.saved_tensors[0], None
+    g = torch.Generator().manual_seed(2)
+    normal = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    low, high = (adapters.Adapters(torch.nn.Parameter(normal(2, 3, 8)), torch.nn.Parameter(normal(2, 3, 8))) for _ in range(2))
+    w0, w1, x, dy, index = normal(8, 8), normal(8, 8), normal(5, 8), normal(5, 8), torch.tensor([0, 1, -1, 1, 0])
+
+    def loss(low, high, x, w0, w1, dy):
+        h = adapters.add(x @ w0.T, x, low, index)
+        return (adapters.add(Frozen.apply(h, w1), h, high, index) * dy).sum()
+    args = (x, w0, w1, dy)
+    loss(low, high, *args).backward()
+    grad, step = low.a.grad.clone(), torch.sign(normal(2, 3, 8))
+    with torch.no_grad():
+        ends = [loss(adapters.Adapters(low.a + s * step, low.b), high, *args).double() for s in (0.5, -0.5)]
+        # linear in low.a, so the difference is the gradient but for FP32's roundings: at most 8 + 1 + 8 + 1 of them behind one another, 40 more in the sum
+        size = loss(adapters.Adapters(low.a.abs() + 0.5, low.b.abs()), adapters.Adapters(high.a.abs(), high.b.abs()), *(t.abs() for t in args)).item()
+    assert abs((ends[0] - ends[1]).item() - (grad.double() * step).sum().item()) <= 4 * 58 * 2.0 ** -24 * size
