@@ -11,6 +11,7 @@
 // Rows are grouped by adapter: a tile's rows are one adapter's, gathered by number. All of it is bound by memory (few operations a byte at
 // any rank here); the matrix instructions are there so that one read of an adapter's matrix serves a tile's rows.
 #include <algorithm>
+#include <cstdlib>
 #include <type_traits>
 
 #include "route.hpp"
@@ -1359,6 +1360,22 @@ static int ad_grads(const hb_adapters* a, const AdShape& s, const AdIndex& in, c
   return ad_run_expand<KIND>(s, up, stream);
 }
 
+// Whether two sets of m rows of `width` bytes share any: y's rows are read while others of out's are written, so these are y's own or none of them.
+static bool ad_rows_meet(int64_t y, int64_t y_stride, int64_t out, int64_t out_stride, int64_t m, int64_t width) {
+  if (out >= y + (m - 1) * y_stride + width || y >= out + (m - 1) * out_stride + width) return false;
+  if (y_stride == out_stride) {  // out's row r begins `in` bytes behind y's row r + ahead begins
+    int64_t ahead = (out - y) / y_stride, in = (out - y) % y_stride;
+    if (in < 0) in += y_stride, ahead--;
+    return (in < width && std::abs(ahead) < m) || (y_stride - in < width && std::abs(ahead + 1) < m);
+  }
+  for (int64_t r = 0; r < m; r++) {  // y's row r and the first of out's that ends behind its begin
+    const int64_t at = y + r * y_stride, behind = at - out - width;
+    const int64_t row = behind < 0 ? 0 : behind / out_stride + 1;
+    if (row < m && out + row * out_stride < at + width) return true;
+  }
+  return false;
+}
+
 static int ad_check(const hb_adapters* a, const void* index, int index_bytes, int64_t m, bool grads, AdShape& s) {
   if (!a || !a->a || !a->b || !index) return HB_ENULL;
   if ((index_bytes != 4 && index_bytes != 8) || !ad_shape(a, m, grads, s)) return HB_EINVAL;
@@ -1383,6 +1400,7 @@ extern "C" int hb_adapters_add(const hb_adapters* adapters, const void* x, int64
   if (x_stride < s.k || y_stride < s.n || out_stride < s.n || std::max({x_stride, y_stride, out_stride}) > AD_STRIDE / s.size || !aligned(x, s.size) || !aligned(y, s.size) || !aligned(out, s.size) || !aligned(workspace, 16)) return HB_EINVAL;
   if (y == out && y_stride != out_stride) return HB_EINVAL;
   if (workspace_bytes < s.bytes()) return HB_EWORKSPACE;
+  if (y != out && ad_rows_meet(reinterpret_cast<int64_t>(y), y_stride * s.size, reinterpret_cast<int64_t>(out), out_stride * s.size, m, (int64_t)s.n * s.size)) return HB_EINVAL;
   const AdIndex in{index, adapters->ranks, index_bytes == 8, (int)m, s.adapters, s.rank};
   auto run = [&](auto kind) {
     return ad_add<decltype(kind)::value>(adapters, s, in, x, x_stride, y, y_stride, out, out_stride, static_cast<char*>(workspace), as_stream(stream));

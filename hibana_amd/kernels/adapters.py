@@ -204,7 +204,7 @@ class _Add(torch.autograd.Function):
 
 
 def add(y: torch.Tensor, x: torch.Tensor, pool: Adapters, index: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
-    """y [M, N] plus each row's adapter of x [M, K], of the pool's type -> [M, N] (or `out`: y itself, or memory that y's rows are not in). index int32 or int64 [M]: a row whose
+    """y [M, N] plus each row's adapter of x [M, K], of the pool's type -> [M, N] (or `out`: y itself, or memory that no row of y has a part of: else refused). index int32 or int64 [M]: a row whose
     index is not of the pool (-1) is y's, bit for bit. Any order of rows: those of an adapter share one read of its matrices. An infinity in b (of the gradients: in a, x or
     dy) may come out as NaN: it is multiplied with values that are held in parts, some of them zero.
 

@@ -628,7 +628,8 @@ typedef struct {
 } hb_adapters;
 size_t hb_adapters_workspace_bytes(const hb_adapters* adapters, int64_t m, int grads);
 
-/* out [m, n] = y + scale_i (x a_i^T) b_i, rounded once; rows without an adapter are y's. out may be y (of the same stride). An infinity in
+/* out [m, n] = y + scale_i (x a_i^T) b_i, rounded once; rows without an adapter are y's. out is y (of the same stride) or memory that no row of y has a part of
+ * (else HB_EINVAL); x, which is read before any of out is written, may lie in it. An infinity in
  * b (below: in a, x or dy) may come out as NaN, since the inner sums it is multiplied with are held in parts, some of them zero. */
 int hb_adapters_add(const hb_adapters* adapters, const void* x, int64_t x_stride, const void* y, int64_t y_stride, const void* index, int index_bytes, int64_t m,
                     void* out, int64_t out_stride, void* workspace, size_t workspace_bytes, void* stream);
