@@ -225,7 +225,10 @@ def add(y: torch.Tensor, x: torch.Tensor, pool: Adapters, index: torch.Tensor, o
         if y.is_cuda and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("adapters.add: a captured step takes adapters.grads (no gradient is recorded in a capture)")
         return _Add.apply(y, x, pool.a, pool.b, pool.scale, pool.ranks, index, pool)
-    return _add(y, x, pool, index, out)
+    got = _add(y, x, pool, index, out)
+    if out is not None:
+        torch._C._increment_version((out,))  # (`torch.autograd.graph.increment_version` at half its time)
+    return got
 
 
 def grads(dy: torch.Tensor, x: torch.Tensor, pool: Adapters, index: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:

@@ -9,7 +9,8 @@ from oracle import adapters as oracle
 @pytest.fixture(autouse=True)
 def formulas(monkeypatch):
     def add(y, x, pool, index, out):
-        return oracle.add(y, x, pool.a, pool.b, pool.scale, pool.ranks, index).to(y.dtype)
+        to = oracle.add(y, x, pool.a, pool.b, pool.scale, pool.ranks, index).to(y.dtype)
+        return to if out is None else (out.data.copy_(to), out)[1]  # (as a kernel writes it: past autograd)
 
     def grads(dy, x, pool, index):
         dx, da, db = oracle.grads(dy, x, pool.a, pool.b, pool.scale, pool.ranks, index)
@@ -126,3 +127,19 @@ def test_two_adapted_layers_learn_through_a_projection_that_records_its_gradient
         # linear in low.a, so the difference is the gradient but for FP32's roundings: at most 8 + 1 + 8 + 1 of them behind one another, 40 more in the sum
         size = loss(adapters.Adapters(low.a.abs() + 0.5, low.b.abs()), adapters.Adapters(high.a.abs(), high.b.abs()), *(t.abs() for t in args)).item()
     assert abs((ends[0] - ends[1]).item() - (grad.double() * step).sum().item()) <= 4 * 58 * 2.0 ** -24 * size
+
+
+def test_a_result_put_into_a_tensor_is_a_change_of_it():
+    """Who keeps the old values for a gradient is told, as by any operation in place; on tensors of inference mode there is nobody to tell."""
+    pool, y, x, _, index = _case()
+    y, weight = y.detach(), torch.ones(6, requires_grad=True)
+    kept = (weight * y).sum()
+    at = y._version
+    with torch.no_grad():
+        assert adapters.add(y, x, pool, index, out=y) is y
+    assert y._version > at
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        kept.backward()
+    with torch.inference_mode():
+        z = y.clone()
+        assert adapters.add(z, x, pool, index, out=z) is z and not torch.equal(z, y)
