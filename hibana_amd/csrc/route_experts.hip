@@ -223,12 +223,13 @@ __global__ __launch_bounds__(256) void route_experts_kernel(RouteExperts p) {
     }
     // What two sums may seem apart, or in the wrong order, by FP32's roundings: a score is off by 2^-19 of the largest at most (its argument, the exponential, the sum over
     // PER registers and 64 lanes, the reciprocal and the product: 28 halves of an ulp), a sum with the bias by 2^-24 of itself; twice for two, and twice that
-    const float off = 0x1p-17f * (SIGMOID ? 1.f : wave_max(size)) + 0x1p-22f * wave_max(largest);
+    largest = wave_max(largest);
+    const float off = 0x1p-17f * (SIGMOID ? 1.f : wave_max(size)) + 0x1p-22f * largest;
     uint32_t left = open;
     if (p.kept < p.groups) {
       float gap;
       if (!route_groups<float, PER>(p, c, open, lane, gap)) left = 0;
-      near = gap <= 3.f * off;
+      near = gap <= 3.f * off || largest >= 0x1p126f;  // (the sum of two may be past FP32's range)
     }
     uint32_t top;
 #pragma unroll
