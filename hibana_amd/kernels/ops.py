@@ -202,6 +202,9 @@ def _route_experts(logits: torch.Tensor, k: int, scoring: str, bias, groups: int
     m, e = lg.shape
     if not (1 <= e <= 1024 and 1 <= kept <= groups <= 64 and e % groups == 0 and 1 <= k <= min(63, kept * (e // groups))):
         raise ValueError(f"{what}: up to 1024 experts in up to 64 groups of a size, k up to 63 and the experts of the kept groups")
+    lanes = 1 << (64 // groups).bit_length() - 1  # of a wavefront that a group has, up to sixteen experts in each
+    if e // groups > 16 * lanes:
+        raise ValueError(f"{what}: {groups} groups have up to {16 * lanes} experts each")
     bias32 = sl = None
     if bias is not None:
         if bias.ndim != 1 or bias.shape[0] != e or not bias.is_floating_point():
@@ -242,8 +245,8 @@ class _RouteExperts(torch.autograd.Function):
 def route_experts(logits: torch.Tensor, k: int, scoring: str = "softmax", *, bias: torch.Tensor | None = None, groups: int = 1, kept: int = 1, renormalize: bool = True,
                   scale: float = 1.0, slots: torch.Tensor | None = None, steps: int = 1):
     """logits [M, E] (BF16, FP16 or FP32; E up to 1024) -> (int32 ids [M, k], FP32 weights [M, k]), largest choice first. Scores are the logits' softmax or
-    sigmoid; the choice goes by score + bias (FP32 [E], None: 0) among the experts of the `kept` groups (of `groups`, of consecutive experts) whose best
-    two sum highest; equal ones by the lower number. Without a bias the order is the logits' own, else (and between groups) that of the values in FP64. Weights are the plain scores, with
+    sigmoid; the choice goes by score + bias (FP32 [E], None: 0) among the experts of the `kept` groups (of `groups`, of consecutive experts, up to 16 times the power of
+    two that 64 / groups holds: all that there are where the groups are a power of two) whose best two sum highest; equal ones by the lower number. Without a bias the order is the logits' own, else (and between groups) that of the values in FP64. Weights are the plain scores, with
     `renormalize` divided by their sum, times `scale`. An expert whose logit is -inf (a mask) or NaN is never chosen: slots left over, and all of a padded row's
     (slots[r // steps] == 0), have id E, which the experts' kernels skip, and weight 0. A row that has a NaN logit has NaN weights.
 
