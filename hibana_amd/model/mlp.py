@@ -10,8 +10,9 @@ With both linears in the microscaled four-bit format (`Mxfp4Linear`) the activat
 product: mxfp4_linear(silu_mul_quant_mxfp4(mxfp4_linear(x, gate_up), pairs), down).
 
 With `adapters`, a pool beside each linear (or None), and a call's `index`, each row's own adapter is added to both products
-(`adapters.add`): the forms above that make the two products in one call, or round the product in between in the same launch, are
-not taken then but for the microscaled format's, whose down adapters read the rows that its linear reads, rounded to four bits. A serving
+(`adapters.add`), which are then calls of their own; rows without an adapter have the bits that they have without an `index`. A pool of the down
+projection reads the SiLU product in BF16 where its linear reads that or (3-bit decode) the groups rounded from it, and the microscaled
+format's own rows, rounded to four bits, where its linear reads those. A serving
 form: no gradient is recorded, of the rows or of pools that take one.
 
 Assembled from linears already loaded. The reference's NVFP4 activation paths (`prequantized`, the fused prefill
@@ -45,7 +46,7 @@ class Mlp:
         (`mxfp4.Mxfp4`), the result BF16. `index` int32 or int64 [rows]: each row's adapter (-1: none); without it no adapter is added."""
         if prequantized is not None:
             raise ValueError("Mlp: NVFP4 activations are not taken by the weight-only kernels")
-        if index is not None:
+        if index is not None and any(pool is not None for pool in self.adapters):
             return self._adapted(x, index)
         pairs = self.gate_up.pairs
         if isinstance(self.gate_up, Mxfp4Linear):
@@ -56,10 +57,13 @@ class Mlp:
             return w3.w3_mlp(x, self.gate_up.w3, self.down.w3, pairs)
         gate_up = ops.nvfp4_linear(x, self.gate_up)
         if ops.w3_decode(self.down, gate_up.shape[0]):
-            # 3-bit decode: the SiLU product in BF16 rounded per 32-group for the 3-bit GEMM, in one launch
-            x_q, x_scale = ops.silu_mul_quant_groups(gate_up, pairs, torch_chain=True)
-            return w3.w3_linear(x_q, self.down.w3, x_scale)
+            return self._down_in_three_bits(gate_up)
         return ops.nvfp4_linear(ops.silu_and_mul(gate_up, pairs), self.down)
+
+    def _down_in_three_bits(self, gate_up: torch.Tensor) -> torch.Tensor:
+        """3-bit decode: the SiLU product in BF16 rounded per 32-group for the 3-bit GEMM, in one launch."""
+        x_q, x_scale = ops.silu_mul_quant_groups(gate_up, self.gate_up.pairs, torch_chain=True)
+        return w3.w3_linear(x_q, self.down.w3, x_scale)
 
     def _adapted(self, x: torch.Tensor, index: torch.Tensor) -> torch.Tensor:
         if not isinstance(x, torch.Tensor):
@@ -74,5 +78,9 @@ class Mlp:
             rounded = ops.silu_mul_quant_mxfp4(gate_up, pairs)
             y = ops.mxfp4_linear(rounded, self.down, gate_up.dtype)
             return y if self.adapters[1] is None else add(y, mxfp4.dequantize(rounded, gate_up.dtype), self.adapters[1])
-        h = ops.silu_and_mul(add(ops.nvfp4_linear(x, self.gate_up), x, self.adapters[0]), pairs)
+        gate_up = add(ops.nvfp4_linear(x, self.gate_up), x, self.adapters[0])
+        if ops.w3_decode(self.down, gate_up.shape[0]):  # the groups that it reads without adapters too
+            y = self._down_in_three_bits(gate_up)
+            return y if self.adapters[1] is None else add(y, ops.silu_and_mul(gate_up, pairs), self.adapters[1])
+        h = ops.silu_and_mul(gate_up, pairs)
         return add(ops.nvfp4_linear(h, self.down), h, self.adapters[1])
