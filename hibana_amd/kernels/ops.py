@@ -213,7 +213,7 @@ def _route_experts(logits: torch.Tensor, k: int, scoring: str, bias, groups: int
     if steps < 1 or m % steps or (slots is not None and slots.numel() < m // steps):
         raise ValueError(f"{what}: whole requests of `steps` rows, a slot for every request")
     if slots is not None:
-        sl = slots if slots.dtype == torch.int32 and slots.is_contiguous() else slots.ne(0).to(torch.int32)  # (what 32 bits do not hold stays apart from 0)
+        sl = slots if slots.dtype == torch.int32 and slots.is_contiguous() else slots.ne(0).to(torch.int32).contiguous()  # (what 32 bits do not hold stays apart from 0)
     stream = _lib.stream_of(lg, *(t for t in (bias32, sl) if t is not None))
     ids, weights = lg.new_empty((m, k), dtype=torch.int32), lg.new_empty((m, k), dtype=torch.float32)
     if m:

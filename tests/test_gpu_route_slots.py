@@ -10,6 +10,7 @@ pytestmark = pytest.mark.gpu
 def test_padded_rows(slots):
     from hibana_amd.kernels import ops
     logits = torch.randn(12, 20, generator=torch.Generator().manual_seed(0)).cuda()
+    assert torch.equal(ops.route_experts(logits, 3, slots=slots.view(2, 3).t().cuda(), steps=2)[0], ops.route_experts(logits, 3, slots=slots.view(2, 3).t().contiguous().cuda(), steps=2)[0])
     whole, padded = ops.route_experts(logits, 3), slots.ne(0).logical_not().repeat_interleave(2).cuda()
     ids, weights = ops.route_experts(logits, 3, slots=slots.cuda(), steps=2)
     assert torch.equal(ids, whole[0].masked_fill(padded[:, None], 20)) and torch.equal(weights, whole[1].masked_fill(padded[:, None], 0.0))
