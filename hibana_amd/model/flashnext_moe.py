@@ -150,6 +150,11 @@ class MoeLayer:
                                     per_request=self.per_request, min_cap=self.MIN_CAP)
         return ops.route_topk(logits, self.topk, slots, steps, repeat=False)
 
+    def _choice(self, x: torch.Tensor, ctx):
+        """`route` as the layer's own calls take it: values alone (a router that is a parameter records nothing, in a capture either)."""
+        with torch.no_grad():
+            return self.route(x, ctx)
+
     def routed(self, x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor) -> torch.Tensor:
         """The routed experts' weighted sum (this rank's part) for x [M, H] -> BF16 [M, H]."""
         if self.mxfp4 is not None:
@@ -169,7 +174,7 @@ class MoeLayer:
     def __call__(self, x: torch.Tensor, ctx=None) -> torch.Tensor:
         x = x.contiguous()
         if self.mxfp4 is not None:
-            ids, weights = self.route(x, ctx)
+            ids, weights = self._choice(x, ctx)
             if self.shared_mlp is None:
                 return self.routed(x, ids, weights)
             pairs = mxfp4_moe.mxfp4_moe(self.mxfp4, x, ids, weights, pairs=True)  # FP32 at any number of rows, as the sum without a shared expert has them
@@ -177,12 +182,12 @@ class MoeLayer:
         if self.shared_on_linears(x.shape[0]):
             # the reference's own chain: the experts' unsummed pair outputs (BF16 from WIDE_ROWS rows), the shared expert
             # on its linears (silu(gate) * up in between), the combine over both
-            ids, weights = self.route(x, ctx)
+            ids, weights = self._choice(x, ctx)
             pairs = w3_moe.w3_moe(self.w3, x, ids, weights, pairs=True, pairs_bf16=x.shape[0] >= w3_moe.WIDE_ROWS, experts_total=self.experts)
             shared = ops.nvfp4_linear(ops.silu_and_mul(ops.nvfp4_linear(x, self.shared_gate_up)), self.shared_down)
             return ops.moe_combine_pairs(pairs, ids, weights, shared, x, self.shared_gate_vec, self.w3.base, self.w3.experts)
         if self.routing is not None:
-            ids, weights = self.route(x, ctx)
+            ids, weights = self._choice(x, ctx)
             return w3_moe.moe_layer(self.w3, x, ids, weights, shared=self.shared, gate_vec=self.shared_gate_vec, experts_total=self.experts)
         # router product, routing (or the budgeted selection), plan, both streams and the combine as one chain
         slots, steps = self._padding(ctx)
