@@ -972,10 +972,10 @@ __global__ __launch_bounds__(256, 3) void ad_expand_kernel(AdExpand p) {
   for (int i = 0; i < 4; i++) rows[i] = p.plan.order()[start + min(4 * group + i, count - 1)];
   const int sixteens = ad_sixteens(p.in.rank), steps = ad_thirties(rank);
   int power = 0;  // FP16: of row col, the largest over the ranks
-  const int8_t* powers = p.row_power + (int64_t)tile * sixteens * AD_TILE + 16 * half + col;
+  const int8_t* powers = p.row_power + (int64_t)tile * sixteens * AD_TILE + 16 * half;  // (the wavefront's)
   if constexpr (KIND == HB_F16) {
     power = -128;
-    for (int j = 0; j < ad_sixteens(rank); j++) power = max(power, (int)powers[j * AD_TILE]);
+    for (int j = 0; j < ad_sixteens(rank); j++) power = max(power, (int)powers[j * AD_TILE + col]);
   }
   const char* sums = p.by_row + (int64_t)tile * ad_thirties(p.in.rank) * PARTS * 1024 * SIZE + ((16 * half + col) * 32 + 8 * group) * SIZE;
   constexpr int WORDS = SIZE == 4 ? 2 : PARTS;
@@ -986,7 +986,7 @@ __global__ __launch_bounds__(256, 3) void ad_expand_kernel(AdExpand p) {
       s[0][i] = *reinterpret_cast<const u32x4_t*>(sums + (int64_t)step * PARTS * 1024 * SIZE + (SIZE == 4 ? 16 * i : i * 2048));
       if constexpr (KIND == HB_F16) {
         const int j = 2 * step + (group >> 1);  // (ranks behind the last sixteen are zero)
-        s[0][i] = ad_lower(s[0][i], j < ad_sixteens(rank) ? powers[j * AD_TILE] - power : 0);
+        s[0][i] = ad_lower(s[0][i], j < ad_sixteens(rank) ? powers[j * AD_TILE + col] - power : 0);
       }
     }
   };
