@@ -422,7 +422,7 @@ __device__ __forceinline__ int ad_tile_at(const AdIndex& p, int t, int& c, int& 
 
 // The sums are operands of the second product. To keep what FP32 holds of them, a value goes in as the sum of three of the type's: BF16 by cutting (8 bits a
 // part, never past the value's size: no overflow; three parts are all of it), FP16 by rounding what a power of two has brought below 2^15 (all of it down to 2^-39 of the
-// largest, FP16's smallest step). Two parts hold 2^-16 of a BF16 sum, 2^-22 of an FP16 one.
+// largest, half of FP16's smallest step; 2^-37 where `ad_lower` brings the parts to a larger unit). Two parts hold 2^-16 of a BF16 sum, 2^-22 of an FP16 one.
 template <int KIND>
 __device__ __forceinline__ void ad_cut(float v, uint16_t (&part)[AdType<KIND>::PARTS]) {
   constexpr int PARTS = AdType<KIND>::PARTS;
@@ -453,7 +453,7 @@ __device__ __forceinline__ void ad_cut(float v, uint16_t (&part)[AdType<KIND>::P
 __device__ __forceinline__ int ad_exponent(float most) { return most > 0.f ? max((int)(__float_as_uint(most) >> 23) - 127, -86) - 14 : -100; }
 __device__ __forceinline__ float ad_pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
-// FP16 parts times 2^e, e <= 0 (below -40 they are too small to count).
+// FP16 parts times 2^e, e <= 0 (what falls below FP16's smallest step, 2^-38 of the unit's largest, is gone)
 __device__ __forceinline__ u32x4_t ad_lower(const u32x4_t& v, int e) {
   f16x8_t f = __builtin_bit_cast(f16x8_t, v);
   f = f * (_Float16)ad_pow2(max(e, -24));

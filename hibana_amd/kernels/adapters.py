@@ -5,7 +5,7 @@ frozen quantized weights, and what a server then holds beside them.
 
 A pool holds the adapters of one projection [N, K], both matrices rank by rank: a [adapters, rank, K] and b [adapters, rank, N] (a
 checkpoint's lora_B [N, rank], transposed once). So every product of the forward and the backward pass reads along a matrix's rows. Products
-have FP32 sums; the sums between the two of an adapter keep all that FP32 holds of them (FP16: to 2^-39 of the largest), and the result is rounded
+have FP32 sums; the sums between the two of an adapter keep all that FP32 holds of them (FP16: to 2^-37 of the largest), and the result is rounded
 once. No counterpart in the reference.
 """
 from __future__ import annotations

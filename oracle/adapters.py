@@ -42,9 +42,10 @@ def _two(length, terms, parts):
 
 
 # FP32 inner sums as operands, in three parts of the type: BF16 cut to 8 bits each, all of the 24; FP16 rounded to 11 bits each (2^-33), of values brought
-# below 2^15, whose own smallest step is 2^-24: 2^-25 / 2^14 of the largest
+# below 2^15, whose own smallest step is 2^-24: each of the three parts may be off by 2^-25 where it is brought down to a larger unit, the last one by its
+# rounding too, 4 * 2^-25 / 2^14 of the largest
 PARTS = {torch.bfloat16: 2.0 ** -24, torch.float16: 2.0 ** -33, torch.float32: 0.0}
-LARGEST = {torch.bfloat16: 0.0, torch.float16: 2.0 ** -39, torch.float32: 0.0}
+LARGEST = {torch.bfloat16: 0.0, torch.float16: 2.0 ** -37, torch.float32: 0.0}
 
 
 def add_bound(y, x, a, b, scale, ranks, index):
