@@ -129,7 +129,10 @@ class Adapters:
         if need is None:
             if len(self._rooms) >= 4096:
                 self._rooms.clear()
-            need = self._rooms[m, grads] = _lib.lib().hb_adapters_workspace_bytes(self.struct(), m, grads)
+            need = _lib.lib().hb_adapters_workspace_bytes(self.struct(), m, grads)
+            if not need:
+                raise ValueError(f"adapters: up to 2^24 rows and axes of up to 2^22, not {m} rows beside a projection [{self.out_features}, {self.in_features}]")
+            self._rooms[m, grads] = need
         return need
 
 

@@ -38,3 +38,11 @@ def test_what_does_not_fit_is_refused(name, change):
     held.data = change(held.data)
     with pytest.raises(ValueError):
         pool.struct()
+
+
+@pytest.mark.parametrize("m,k", [((1 << 24) + 1, 8), (1, (1 << 22) + 1)])
+def test_sizes_past_the_library_s_are_refused_by_name(m, k):
+    pool = adapters.Adapters(torch.zeros(1, 1, k), torch.zeros(1, 1, 6))
+    for grads in (0, 1):
+        with pytest.raises(ValueError, match="rows"):
+            pool.room(m, grads)
