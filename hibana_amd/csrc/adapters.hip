@@ -607,12 +607,15 @@ struct AdShrink {
 };
 constexpr int AD_WAVES = 4;
 constexpr int AD_EXPANDS = 768;   // workgroups of an expansion, about: 4096 rows of 5120 26.6 us (in 256: 36.2, in 2048: 26.5)
-// Results of this many bytes are stored past the caches: half of what the dies' hold. Through them they push out what is still to be read, and whoever reads them next finds
-// little there. Add of 4096 rows of 5120 at rank 32 (42 MB of results) 52 -> 45 us a call, two of 5120 at rank 16 with gradients (21 MB of dx) 43.9 -> 42.5 (y's rows
-// read so too: 48 us).
+// Results of this many bytes are stored past the caches: half of what the dies' hold. Through them they push out what is still to be read. Add of 4096 rows of 5120 at rank 32
+// (42 MB of results) 52 -> 45 us a call (y's rows read so too: 48 us). Rows of 2560 x 5120, rank 16, in a graph, through the caches and past them: 1600 (16 MB) 27.2 and 26.3 us, 2400
+// 31.6 and 30.2, 4096 44.8 and 41.2, 8192 75.9 and 76.7; with a reader of the results behind it (silu_and_mul of them) 35.7 and 35.5, 43.0 and 42.8, 62.9 and 65.0, 107 and
+// 113.6: a reader of a fresh 42 MB loses more than the call gains. Into y itself, as the linears and blocks call it, the two are the same with and without the reader. Gradients of 2048 rows
+// of 5120 (21 MB of dx) 43.5 and 42.4, of 4096 74.0 and 72.6, of 8192 118.4 and 115.0.
 constexpr int64_t AD_PAST_BYTES = 16 << 20;
 // Rows of this many bytes, both sides' together, are read past the caches by the outer products, after which nobody reads them: half of the last-level cache's. 8192 rows of
-// 12800 and 2560 (252 MB, and 210 MB of dx past the caches) 274 -> 227 us the call; 42 MB are the slower for it, 43.9 -> 45.1.
+// 12800 and 2560 (252 MB, and 210 MB of dx past the caches) 274 -> 227 us the call. Rows of 5120 and 5120 in a graph, through the caches and past them: 42 MB 42.2 and 43.9 us, 61 55.7
+// and 57.2, 84 72.6 and 70.3, 123 96.2 and 92.8, 168 126.5 and 115.5: the two meet near 70 MB.
 constexpr int64_t AD_PAST_ROWS = 128ll << 20;
 __host__ __device__ constexpr int ad_sixteens(int rank) { return (rank + 15) / 16; }
 __host__ __device__ constexpr int ad_thirties(int rank) { return (rank + 31) / 32; }
@@ -788,7 +791,7 @@ __device__ __forceinline__ u32x4_t ad_result(const u32x4_t& y, const f32x4_t (&a
 
 // Few rows: a workgroup joins the splits' sums of its tile in LDS, then a tile's rows times four wavefronts' columns, sixteen lanes of sixteen bytes each. 64 rows of 25600, 32
 // adapters of up to 64 ranks (55 MB of matrices and rows): 21 us with nothing in the caches, 2.6 TB/s: a wavefront has few steps behind its start, and its 230 registers,
-// most of them matrix rows under way, leave room for two a SIMD. One row of 5120 at rank 16 5.4 us.
+// most of them matrix rows under way, leave room for two a SIMD. One row of 5120 at rank 16 5.6 us.
 template <int KIND, int HOW>
 __global__ __launch_bounds__(256) void ad_expand_few_kernel(AdFew p) {
   constexpr int VEC = AD_VEC<KIND>, SIZE = AdType<KIND>::SIZE, PARTS = AdType<KIND>::PARTS;
@@ -935,8 +938,8 @@ __device__ __forceinline__ void ad_join(const AdIndex& in, const AdPlan& plan, c
 }
 
 // A plan's tiles, sixteen rows a workgroup: every wavefront for itself, over every (4 x share)-th block of sixteen lanes' columns. It is bound by what it stores and y's
-// rows: 4096 rows of 5120 at rank 32 (84 MB) 26.4 us with nothing in the caches, 3.2 TB/s, in three wavefronts a SIMD (with two tiles of
-// rows a wavefront the matrix is turned in registers half as often, and there is room for two: slower); dx of 2048 rows of 5120 (21 MB and the join) 9.5.
+// rows: 4096 rows of 5120 at rank 32 (84 MB) 26.6 us with nothing in the caches, 3.2 TB/s, in three wavefronts a SIMD (with two tiles of
+// rows a wavefront the matrix is turned in registers half as often, and there is room for two: slower); dx of 2048 rows of 5120 (21 MB and the join) 9.8.
 struct AdExpand {
   AdIndex in;
   AdPlan plan;
@@ -1056,7 +1059,8 @@ struct AdOuter {
 // their sums in LDS. A lane's eight rows of sixteen bytes are turned as in the expansion; the next tile's are under way while one is
 // multiplied. An adapter's only unit writes the gradient (zeros, if it has no rows), several write partial sums for ad_join. (Joined by the last of them to
 // arrive instead, whose sums must pass the dies' caches in words: 28 us for the 16 of both kernels at 2048 rows of 5120 x 5120, rank 16.) The rows' reads bound it: there 11.1 us
-// for 42 MB that the shrink has just read, 3.8 TB/s; 8192 rows of 12800 and 2560, FP16, ranks up to 64, 67 us for 252 MB, past the last-level cache, 3.8 TB/s.
+// for 42 MB that the shrink has just read, 3.8 TB/s; 8192 rows of 12800 and 2560, FP16, ranks up to 64, 77 us for 252 MB, past the last-level cache, 3.3 TB/s
+// (64 at the least; of two parts a sum 66).
 // A unit has 512 rows or more: of 128 the parts cost their join more (10.4 us for 9.4 of the launch that has it), of 2048 the products are in too few workgroups (15.3 for 11.1).
 template <int KIND, int RT, int HOW>
 __global__ __launch_bounds__(256, RT == 1 ? 3 : 2) void ad_outer_kernel(AdOuter p) {
